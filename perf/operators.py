@@ -303,7 +303,7 @@ def run_verify(s):
     whole = (torch.where(pr > 0, pr, 0.0).clamp(max=1.0) * 2.0 ** 38).long()
     left = torch.where(left.sum(1, keepdim=True) > 0, left, whole)
     cum = left.cumsum(1)
-    ui = (u[bi, a] * 2.0 ** 24).long().clamp(0, (1 << 24) - 1)
+    ui = (u[:, G] * 2.0 ** 24).long().clamp(0, (1 << 24) - 1)
     tot = cum[:, -1]
     mark = (tot >> 24) * ui + (((tot & 0xffffff) * ui) >> 24)
     tok = (cum <= mark[:, None]).sum(1).clamp(max=V - 1)
