@@ -349,6 +349,54 @@ int ta_block_tail(const void* att, float* x, const void* w_proj, const float* ln
                   const void* w_mlp, const float* ln_next_w, const void* w_qkv, float eps, int dtype, int B, int C,
                   void* h, void* qkv, void* ws, int64_t ws_bytes, int* sync, void* stream);
 
+/* Serving over an 8-bit paged key / value cache (no counterpart in the reference, whose cache is one fp32 tensor per
+ * sequence).
+ * A page holds `page` tokens (16, 32 or 64) of one sequence. pool (n_pages, Hkv, 2 * page * dh + 16) bytes: per (page, kv
+ * head) the e4m3 codes of its keys, those of its values, the fp32 scales of the two (value = code * scale) and 8 unused
+ * bytes. tail (B, Hkv, 2, 2, page * dh) in `dtype` (bf16 or f16): the open page of each sequence and the page before it,
+ * by page parity, keys then values. table (B, max_pages) int32, row stride table_sb: the pool page of each page of a
+ * sequence, read for full pages only. Inside a page the elements of each 16-token group stand in fragment order:
+ *   keys   [h][r][g][t][e]          token 8 r + g, dim h * 4E + t * E + e (E = min(16, dh / 4); r 2, g 8, t 4)
+ *   values [c][g][t][m][r][kh][lo]  token 8 kh + 2 t + lo, dim (c M + m) 16 + 8 r + g (M = min(2, dh / 16))
+ * New rows: sequence b owns rows [start[b], start[b + 1]) (start: B + 1 int32, device) of the n_rows rows of the call, at
+ * positions pos[b], pos[b] + 1, ...; max_new bounds the rows of one sequence (it sizes the grid). Rows that do not fit
+ * these numbers, and pages outside the pool, are recorded in the device error record and left out.
+ *
+ * ta_paged_append: rotates the first `rot` dims of k (and q, into q_out (n_rows, Hq, dh) contiguous; q_out NULL: none)
+ *   by the position's angles, y1 = x1 cos - x2 sin, y2 = x2 cos + x1 sin on dims i and i + rot / 2 (cosv / sinv
+ *   (n_pos, rot / 2) fp32; rot 0: none), in fp32 rounded once to the dtype, and puts k and v into the cache: into the
+ *   tail (pages from the last but one on) and, for each page whose last token arrives, into the pool: scale = top / 448,
+ *   code = e4m3(x * (448 / top)), top the largest magnitude of the page's page x dh values of that head. Below 2^-100 a
+ *   page has codes 0 and scale 1; with an infinity or NaN in it codes 0 and scale NaN. The codes depend on the tokens
+ *   alone. A sequence may be cut back afterwards (pos reduced) to any length from (last page - 1) * page on, last page =
+ *   (pos + new - 1) / page: those tokens are still in the tail.
+ * ta_paged_attn: out[r] = sum over t of softmax_t(scale q_r . K_t) V_t, for query i of a sequence the positions t <=
+ *   pos + i (and t > pos + i - window when window > 0), after ta_paged_append has put the same rows into the cache. Hq a
+ *   multiple of Hkv: query head hq reads kv head hq / (Hq / Hkv). lse (n_rows, Hq) fp32 or NULL: the natural logarithm of
+ *   the sum of exponentials (-inf, with zero rows in out, where nothing is attended). ws: scratch of at least
+ *   ta_paged_attn_workspace bytes, zeroed before its first use; every call leaves it ready for the next. Calls that share
+ *   it must not overlap on the GPU.
+ * ta_verify_drafts: speculative sampling. p (B, G + 1, V) the target's and q (B, G, V) the draft's probabilities (dtype;
+ *   unit inner stride, strides in elements), drafts (B, G), u (B, G + 1) uniform numbers in [0, 1), one for each
+ *   draft and the last for the draw, n (B) drafts of each sequence or NULL (G). Draft i stands while u_i q_i(d_i) < p_i(d_i); accepted[b] = a, the drafts before the first that
+ *   does not stand. tokens (B, G + 1): the a drafts, then a token drawn at u_G from max(p_a - q_a, 0) (from p_a when a =
+ *   n[b], or when nothing is left), then -1. The weights are summed in steps of 2^-38 as 64-bit integers, u in steps of
+ *   2^-24: the token is the first whose cumulative sum exceeds floor(u_G * total). A row of
+ *   no positive weight gives V - 1. */
+int ta_paged_append(void* pool, void* tail, const int32_t* table, int64_t table_sb, int n_pages, int max_pages, int page,
+                    int dtype, int B, int Hkv, int dh, const void* k, const void* v, int64_t k_sr, int64_t k_sh,
+                    int64_t v_sr, int64_t v_sh, int n_rows, const int32_t* start, const int32_t* pos, int max_new,
+                    const float* cosv, const float* sinv, int n_pos, int rot, const void* q, int Hq, int64_t q_sr,
+                    int64_t q_sh, void* q_out, void* stream);
+int64_t ta_paged_attn_workspace(int B, int Hq, int Hkv, int dh, int max_new);
+int ta_paged_attn(const void* pool, const void* tail, const int32_t* table, int64_t table_sb, int n_pages, int max_pages,
+                  int page, int dtype, int B, int Hq, int Hkv, int dh, const void* q, int64_t q_sr, int64_t q_sh,
+                  int n_rows, const int32_t* start, const int32_t* pos, int max_new, float scale, int window, void* out,
+                  int64_t o_sr, int64_t o_sh, float* lse, void* ws, int64_t ws_bytes, void* stream);
+int ta_verify_drafts(const void* p, int64_t p_sb, int64_t p_sr, const void* q, int64_t q_sb, int64_t q_sr, int dtype, int B,
+                     int G, int V, const int64_t* drafts, const float* u, const int32_t* n, int64_t* tokens,
+                     int32_t* accepted, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,115 @@
+"""CPU checks of the serving operators: rejected arguments, the page allocator, the order of a page's elements."""
+import ctypes
+
+import pytest
+import torch
+
+
+def test_rejected_arguments_without_gpu():
+    """The entry points refuse bad arguments with a message before any CUDA call."""
+    from treeattn_b200 import _lib
+    lib = _lib.load()
+    a = 1 << 20  # an aligned address that is never dereferenced
+    f = ctypes.c_float(0.125)
+
+    def attn(page=64, dtype=1, B=2, Hq=4, Hkv=4, dh=64, q=a, window=0, pool=a, n_pages=9, max_pages=3, sb=3):
+        return lib.ta_paged_attn(pool, a, a, sb, n_pages, max_pages, page, dtype, B, Hq, Hkv, dh, q, 256, 64, 2, a, a, 1, f,
+                                 window, a, 256, 64, None, a, 1 << 30, None)
+
+    for kw, what in ((dict(page=48), 'pages of 48'), (dict(dtype=0), 'dtype'), (dict(dh=48), 'head dim'),
+                     (dict(Hq=6), 'multiple of Hkv'), (dict(window=-2), 'window'), (dict(q=a + 2), 'aligned'),
+                     (dict(pool=None), 'null'), (dict(n_pages=0), 'page counts'), (dict(sb=2), 'page counts'),
+                     (dict(pool=a + 4), 'aligned'), (dict(B=-1), 'bad sizes'), (dict(q=None), 'null')):
+        assert attn(**kw) == _lib.TA_ERR_ARG
+        assert 'ta_paged_attn' in _lib.last_error() and what in _lib.last_error(), (kw, _lib.last_error())
+    assert attn(B=0) == _lib.TA_OK
+
+    def append(k=a, rot=64, cos=a, q=a, qo=a, dtype=2, max_new=1):
+        return lib.ta_paged_append(a, a, a, 3, 9, 3, 16, dtype, 2, 4, 64, k, a, 256, 64, 256, 64, 2, a, a, max_new, cos, a,
+                                   100, rot, q, 8, 512, 64, qo, None)
+
+    for kw, what in ((dict(rot=63), 'rotated dims'), (dict(rot=128), 'rotated dims'), (dict(cos=None), 'null'),
+                     (dict(q=None), 'null'), (dict(k=a + 8), 'aligned'), (dict(dtype=0), 'dtype'), (dict(max_new=-1), 'bad sizes')):
+        assert append(**kw) == _lib.TA_ERR_ARG
+        assert 'ta_paged_append' in _lib.last_error() and what in _lib.last_error(), (kw, _lib.last_error())
+
+    def verify(p=a, dtype=0, G=4, V=100):
+        return lib.ta_verify_drafts(p, 500, 100, a, 400, 100, dtype, 2, G, V, a, a, None, a, a, None)
+
+    for kw, what in ((dict(p=None), 'null'), (dict(dtype=7), 'dtype'), (dict(G=-1), 'bad sizes'), (dict(V=0), 'bad sizes'),
+                     (dict(G=5000), 'bad sizes')):
+        assert verify(**kw) == _lib.TA_ERR_ARG
+        assert 'ta_verify_drafts' in _lib.last_error() and what in _lib.last_error(), (kw, _lib.last_error())
+
+
+def test_cpu_tensors_are_refused():
+    from treeattn_b200 import paged
+    with pytest.raises(ValueError, match='CUDA'):
+        paged.PagedKV.empty(4, 2, 64, torch.zeros(1, 2, dtype=torch.int32), 16)
+    p = torch.rand(2, 3, 8)
+    with pytest.raises(ValueError, match='CUDA'):
+        paged.verify_drafts(p, p[:, :2], torch.zeros(2, 2, dtype=torch.int64), torch.rand(2, 3))
+
+
+def test_page_pool():
+    """Pages are handed out once, come back, and a request that cannot be met changes nothing."""
+    from treeattn_b200.paged import PagePool
+    pool = PagePool(10, 3, 6, 16, device='cpu')
+    pool.reserve([17, 0, 64])
+    assert [len(o) for o in pool.owned] == [2, 0, 4]
+    seen = [pg for o in pool.owned for pg in o]
+    assert len(set(seen)) == 6 and set(seen) | set(pool.free) == set(range(10))
+    for b, o in enumerate(pool.owned):
+        assert pool.table[b, :len(o)].tolist() == o
+    pool.reserve([1, 1, 1])
+    assert [len(o) for o in pool.owned] == [2, 1, 4]
+    before = ([list(o) for o in pool.owned], list(pool.free), pool.table.clone())
+    with pytest.raises(MemoryError):
+        pool.reserve([96, 17, 64])
+    with pytest.raises(ValueError, match='above'):
+        pool.reserve([97, 0, 0])
+    assert before[0] == pool.owned and before[1] == pool.free and torch.equal(before[2], pool.table)
+    pool.release(2)
+    pool.reserve([96, 17, 0])
+    assert [len(o) for o in pool.owned] == [6, 2, 0]
+    assert sorted(pg for o in pool.owned for pg in o) + sorted(pool.free) != [] and len(pool.free) == 2
+
+
+@pytest.mark.parametrize('dh', [16, 32, 64, 128])
+def test_page_order(dh):
+    """The element order of a page, spelled out from the layout's definition."""
+    from treeattn_b200.paged import PagedKV
+    P = 32
+    c = PagedKV.__new__(PagedKV)
+    c.page, c.head_dim = P, dh
+    x = torch.arange(P * dh)
+    K, V = c._keys(x), c._values(x)
+    E, M = min(16, dh // 4), min(2, dh // 16)
+    at = 0
+    for s in range(P // 16):
+        for h in range(dh // (4 * E)):
+            for r in range(2):
+                for g in range(8):
+                    for t in range(4):
+                        for e in range(E):
+                            assert K[16 * s + 8 * r + g, h * 4 * E + t * E + e] == at
+                            at += 1
+    at = 0
+    for s in range(P // 16):
+        for cc in range(dh // (16 * M)):
+            for g in range(8):
+                for t in range(4):
+                    for m in range(M):
+                        for r in range(2):
+                            for kh in range(2):
+                                for lo in range(2):
+                                    assert V[16 * s + 8 * kh + 2 * t + lo, (cc * M + m) * 16 + 8 * r + g] == at
+                                    at += 1
+
+
+def test_rotation_table():
+    from treeattn_b200.paged import rotation_table
+    cos, sin = rotation_table(50, 8, device='cpu')
+    assert cos.shape == sin.shape == (50, 4) and cos.dtype == torch.float32
+    assert torch.allclose(cos.double() ** 2 + sin.double() ** 2, torch.ones(50, 4).double(), atol=1e-6)
+    assert cos[0].eq(1).all() and abs(float(sin[7, 0]) - 0.6569865987187891) < 1e-7

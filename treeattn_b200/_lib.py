@@ -64,9 +64,13 @@ SIGNATURES = {
     'ta_add_splits_ln': [P, P, I, I, I, I, P, F, P, P],
     'ta_argmax_finish': [P, I, I, I, P, P, P],
     'ta_block_tail_plan': [I, I, I, I, P, P],
+    'ta_paged_append': [P, P, P, L, I, I, I, I, I, I, I, P, P, L, L, L, L, I, P, P, I, P, P, I, I, P, I, L, L, P, P],
+    'ta_paged_attn_workspace': [I, I, I, I, I],
+    'ta_paged_attn': [P, P, P, L, I, I, I, I, I, I, I, I, P, L, L, I, P, P, I, F, I, P, L, L, P, P, L, P],
+    'ta_verify_drafts': [P, L, L, P, L, L, I, I, I, I, P, P, P, P, P, P],
     'ta_block_tail': [P, P, P, P, P, P, P, P, F, I, I, I, P, P, P, L, P, P],
 }
-_RESTYPES = {'ta_last_error': ctypes.c_char_p, 'ta_level_nodes': c_int64}
+_RESTYPES = {'ta_last_error': ctypes.c_char_p, 'ta_level_nodes': c_int64, 'ta_paged_attn_workspace': c_int64}
 
 _lib = None
 

@@ -8,7 +8,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 
 def build(verbose=True):
     csrc = os.path.join(HERE, 'csrc')
-    cmd = ['make', '-C', csrc]
+    cmd = ['make', '-j2', '-C', csrc]
     r = subprocess.run(cmd, capture_output=not verbose, text=True)
     if r.returncode != 0:
         raise RuntimeError('building libtreeattn_b200.so failed:\n%s' % ((r.stdout or '') + (r.stderr or '')))

@@ -1,7 +1,7 @@
 // Shared device helpers for the treeattn_b200 kernels (sm_100a only).
 //
-// Everything in this library is one translation unit (treeattn_b200.cu includes the kernel headers), so
-// the device error record below is a single symbol that every kernel writes to and the host reads back.
+// Each translation unit of the library has its own device error record (the symbol below is static); the host reads
+// and clears all of them (ta_device_error).
 #pragma once
 
 #include <cuda_runtime.h>
@@ -26,7 +26,7 @@ enum DevErrCode : int {
 };
 
 // code, kernel id, detail a, detail b. The first error wins (atomicCAS on code).
-__device__ int g_dev_err[4];
+static __device__ int g_dev_err[4];
 
 __device__ __forceinline__ void record_error(int code, int kernel, int a, int b) {
   if (atomicCAS(&g_dev_err[0], 0, code) == 0) {
@@ -51,6 +51,9 @@ enum KernelId : int {
   K_ROWS = 11,
   K_PREFILL = 12,
   K_WAIT_PROBE = 13,
+  K_PAGED_APPEND = 16,
+  K_PAGED_ATTN = 17,
+  K_VERIFY = 18,
 };
 
 // ------------------------------------------------------------------------------------------------ types
@@ -226,7 +229,7 @@ __device__ __forceinline__ bool mbar_poll_bounded(uint64_t* bar, uint32_t parity
 // after limit_ns and records DEV_WAIT_TIMEOUT (kernel K_WAIT_PROBE, where = 7). Once no thread waits any more the
 // abandoned barrier is invalidated (what a give-up path must do before its shared memory is reused), and the
 // kernel ends normally.
-__global__ void wait_probe_kernel(uint64_t limit_ns) {
+static __global__ void wait_probe_kernel(uint64_t limit_ns) {
   __shared__ __align__(8) uint64_t bar;
   if (threadIdx.x == 0) {
     mbar_init(&bar, 1);

@@ -1,0 +1,183 @@
+// C ABI of the serving operators: the 8-bit paged cache (append, attention) and the verification of drafted tokens.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <climits>
+
+#include "../../include/treeattn_b200.h"
+#include "host.cuh"
+#include "paged.cuh"
+#include "verify.cuh"
+
+namespace ta_host {
+// This translation unit's device error record (see ta_device_error).
+cudaError_t paged_device_error(int* out4) {
+  cudaError_t e = cudaMemcpyFromSymbol(out4, ta::g_dev_err, 4 * sizeof(int));
+  const int zero[4] = {0, 0, 0, 0};
+  return e == cudaSuccess ? cudaMemcpyToSymbol(ta::g_dev_err, zero, 4 * sizeof(int)) : e;
+}
+}  // namespace ta_host
+
+namespace {
+
+using namespace ta_host;
+
+// Arguments that describe the cache and the call's rows, shared by the entry points.
+int check_cache(const char* who, const void* pool, const void* tail, const int32_t* table, int64_t table_sb, int n_pages,
+                int max_pages, int page, int dtype, int B, int Hq, int Hkv, int dh, int n_rows, const int32_t* start,
+                const int32_t* pos, int max_new) {
+  if (dtype != TA_BF16 && dtype != TA_F16) return fail(TA_ERR_ARG, "%s: bad dtype %d (bfloat16 or float16)", who, dtype);
+  if (!valid_dh(dh)) return fail(TA_ERR_ARG, "%s: unsupported head dim %d (16, 32, 64, 128)", who, dh);
+  if (page != 16 && page != 32 && page != 64)
+    return fail(TA_ERR_ARG, "%s: pages of %d tokens (16, 32 or 64)", who, page);
+  if (B < 0 || B > 65535 || Hkv < 1 || Hkv > 4096 || Hq < Hkv || Hq > 65535 || Hq % Hkv != 0 || n_rows < 0 || max_new < 0)
+    return fail(TA_ERR_ARG, "%s: bad sizes B=%d Hq=%d Hkv=%d rows=%d max_new=%d (Hq a multiple of Hkv)", who, B, Hq, Hkv,
+                n_rows, max_new);
+  if (n_pages < 1 || max_pages < 0 || table_sb < max_pages || (int64_t)(max_pages + 1) * page > INT_MAX)
+    return fail(TA_ERR_ARG, "%s: bad page counts n_pages=%d max_pages=%d (row stride %lld)", who, n_pages, max_pages,
+                (long long)table_sb);
+  if (!pool || !tail || !table || !start || !pos) return fail(TA_ERR_ARG, "%s: null pointer", who);
+  if (!aligned16(pool) || !aligned16(tail)) return fail(TA_ERR_ARG, "%s: the pool and the tail must be 16-byte aligned", who);
+  return TA_OK;
+}
+
+template <typename T, int DH>
+int run_append(const ta::AppendParams& a, int B, cudaStream_t st) {
+  const int P = a.c.P;
+  const int n_page = (a.max_new - 1) / P + 2;  // pages that one sequence's new tokens can touch
+  if ((int64_t)n_page * a.c.Hkv > INT_MAX / 2) return fail(TA_ERR_ARG, "ta_paged_append: too many pages in one call");
+  ta::AppendParams p = a;
+  p.page_ctas = n_page * a.c.Hkv;
+  int q_ctas = 0;
+  if (a.q_out) {
+    const int64_t work = ((int64_t)a.max_new * a.Hq * (DH - a.rot / 2) + ta::APPEND_THREADS * 4 - 1) / (ta::APPEND_THREADS * 4);
+    q_ctas = (int)std::min<int64_t>(work, std::max(1, 148 * 16 / std::max(B, 1)));
+  }
+  const size_t smem = (size_t)2 * P * (DH + 8) * 2;
+  p.c = a.c;
+  ta::paged_append_kernel<T, DH><<<dim3(p.page_ctas + q_ctas, B), ta::APPEND_THREADS, smem, st>>>(p);
+  return check_launch("ta_paged_append");
+}
+
+template <typename T, int DH, int NT>
+int run_attn_nt(const ta::AttnParams& p, cudaStream_t st) {
+  const int64_t rows = (int64_t)p.max_new * (p.Hq / p.c.Hkv);
+  const int64_t tiles = (rows + 8 * NT - 1) / (8 * NT);
+  if (tiles > INT_MAX) return fail(TA_ERR_ARG, "ta_paged_attn: too many rows");
+  static SmemAttr attr;
+  constexpr int smem = ta::attn_smem_bytes<DH, NT>();
+  if (int r = allow_smem(attr, ta::paged_attn_kernel<T, DH, NT>, smem, "ta_paged_attn")) return r;
+  ta::paged_attn_kernel<T, DH, NT><<<dim3((unsigned)tiles, p.c.Hkv, p.B), ta::ATTN_WARPS * 32, smem, st>>>(p);
+  return check_launch("ta_paged_attn");
+}
+
+template <typename T, int DH>
+int run_attn(const ta::AttnParams& p, cudaStream_t st) {
+  const int64_t rows = (int64_t)p.max_new * (p.Hq / p.c.Hkv);
+  if (rows <= 8) return run_attn_nt<T, DH, 1>(p, st);
+  if (rows <= 16 || DH == 128) return run_attn_nt<T, DH, 2>(p, st);  // 32 rows of head dim 128 do not fit the registers
+  return run_attn_nt<T, DH, DH == 128 ? 2 : 4>(p, st);
+}
+
+}  // namespace
+
+extern "C" {
+
+int ta_paged_append(void* pool, void* tail, const int32_t* table, int64_t table_sb, int n_pages, int max_pages, int page,
+                    int dtype, int B, int Hkv, int dh, const void* k, const void* v, int64_t k_sr, int64_t k_sh,
+                    int64_t v_sr, int64_t v_sh, int n_rows, const int32_t* start, const int32_t* pos, int max_new,
+                    const float* cosv, const float* sinv, int n_pos, int rot, const void* q, int Hq, int64_t q_sr,
+                    int64_t q_sh, void* q_out, void* stream) {
+  g_err.clear();
+  const char* who = "ta_paged_append";
+  if (!q_out) Hq = Hkv;
+  if (int r = check_cache(who, pool, tail, table, table_sb, n_pages, max_pages, page, dtype, B, Hq, Hkv, dh, n_rows, start,
+                          pos, max_new))
+    return r;
+  if (rot < 0 || rot > dh || rot % 2 != 0) return fail(TA_ERR_ARG, "%s: rotated dims %d (even, at most the head dim %d)", who, rot, dh);
+  if (B == 0 || n_rows == 0 || max_new == 0) return TA_OK;
+  if (!k || !v || (rot && (!cosv || !sinv || n_pos < 1)) || (q_out && !q)) return fail(TA_ERR_ARG, "%s: null pointer", who);
+  if (!rows_aligned(k, 2, {k_sr, k_sh}) || !rows_aligned(v, 2, {v_sr, v_sh}))
+    return fail(TA_ERR_ARG, "%s: k and v rows must be 16-byte aligned", who);
+  ta::AppendParams p{};
+  p.c = {reinterpret_cast<unsigned char*>(pool), tail, table, table_sb, n_pages, max_pages, Hkv, page};
+  p.k = k; p.v = v; p.q = q;
+  p.k_sr = k_sr; p.k_sh = k_sh; p.v_sr = v_sr; p.v_sh = v_sh; p.q_sr = q_sr; p.q_sh = q_sh;
+  p.q_out = q_out;
+  p.start = start; p.pos = pos;
+  p.cosv = cosv; p.sinv = sinv; p.n_pos = n_pos; p.rot = rot;
+  p.n_rows = n_rows; p.max_new = max_new; p.Hq = Hq;
+  const cudaStream_t st = S(stream);
+#define TA_APPEND(T)                                                              \
+  switch (dh) {                                                                   \
+    case 16: return run_append<T, 16>(p, B, st);                                  \
+    case 32: return run_append<T, 32>(p, B, st);                                  \
+    case 64: return run_append<T, 64>(p, B, st);                                  \
+    default: return run_append<T, 128>(p, B, st);                                 \
+  }
+  if (dtype == TA_BF16) { TA_APPEND(__nv_bfloat16) } else { TA_APPEND(__half) }
+#undef TA_APPEND
+}
+
+int64_t ta_paged_attn_workspace(int B, int Hq, int Hkv, int dh, int max_new) {
+  (void)B; (void)Hq; (void)Hkv; (void)dh; (void)max_new;
+  return 0;
+}
+
+int ta_paged_attn(const void* pool, const void* tail, const int32_t* table, int64_t table_sb, int n_pages, int max_pages,
+                  int page, int dtype, int B, int Hq, int Hkv, int dh, const void* q, int64_t q_sr, int64_t q_sh,
+                  int n_rows, const int32_t* start, const int32_t* pos, int max_new, float scale, int window, void* out,
+                  int64_t o_sr, int64_t o_sh, float* lse, void* ws, int64_t ws_bytes, void* stream) {
+  g_err.clear();
+  const char* who = "ta_paged_attn";
+  if (int r = check_cache(who, pool, tail, table, table_sb, n_pages, max_pages, page, dtype, B, Hq, Hkv, dh, n_rows, start,
+                          pos, max_new))
+    return r;
+  if (window < 0) return fail(TA_ERR_ARG, "%s: window %d", who, window);
+  if (B == 0 || n_rows == 0 || max_new == 0) return TA_OK;
+  if (!q || !out) return fail(TA_ERR_ARG, "%s: null pointer", who);
+  if (!rows_aligned(q, 2, {q_sr, q_sh}) || !rows_aligned(out, 2, {o_sr, o_sh}))
+    return fail(TA_ERR_ARG, "%s: q and out rows must be 16-byte aligned", who);
+  if ((int64_t)max_new * (Hq / Hkv) > INT_MAX / 2) return fail(TA_ERR_ARG, "%s: too many rows", who);
+  ta::AttnParams p{};
+  p.c = {const_cast<unsigned char*>(reinterpret_cast<const unsigned char*>(pool)), const_cast<void*>(tail), table, table_sb,
+         n_pages, max_pages, Hkv, page};
+  p.q = q; p.q_sr = q_sr; p.q_sh = q_sh;
+  p.start = start; p.pos = pos;
+  p.B = B; p.n_rows = n_rows; p.max_new = max_new; p.Hq = Hq;
+  p.scale = scale; p.window = window;
+  p.out = out; p.o_sr = o_sr; p.o_sh = o_sh; p.lse = lse;
+  (void)ws; (void)ws_bytes;
+  const cudaStream_t st = S(stream);
+#define TA_ATTN(T)                                                              \
+  switch (dh) {                                                                 \
+    case 16: return run_attn<T, 16>(p, st);                                     \
+    case 32: return run_attn<T, 32>(p, st);                                     \
+    case 64: return run_attn<T, 64>(p, st);                                     \
+    default: return run_attn<T, 128>(p, st);                                    \
+  }
+  if (dtype == TA_BF16) { TA_ATTN(__nv_bfloat16) } else { TA_ATTN(__half) }
+#undef TA_ATTN
+}
+
+int ta_verify_drafts(const void* p, int64_t p_sb, int64_t p_sr, const void* q, int64_t q_sb, int64_t q_sr, int dtype, int B,
+                     int G, int V, const int64_t* drafts, const float* u, const int32_t* n, int64_t* tokens,
+                     int32_t* accepted, void* stream) {
+  g_err.clear();
+  const char* who = "ta_verify_drafts";
+  if (!valid_dtype(dtype)) return fail(TA_ERR_ARG, "%s: bad dtype %d", who, dtype);
+  if (B < 0 || G < 0 || G > 1024 || V < 1 || V > (1 << 24))
+    return fail(TA_ERR_ARG, "%s: bad sizes B=%d G=%d V=%d (at most 1024 drafts, 2^24 words)", who, B, G, V);
+  if (B == 0) return TA_OK;
+  if (!p || !u || !tokens || !accepted || (G && (!q || !drafts))) return fail(TA_ERR_ARG, "%s: null pointer", who);
+  ta::VerifyParams a{p, q, p_sb, p_sr, q_sb, q_sr, drafts, u, n, B, G, V, tokens, accepted};
+  const cudaStream_t st = S(stream);
+  switch (dtype) {
+    case TA_F32: ta::verify_kernel<float><<<B, ta::VERIFY_THREADS, 0, st>>>(a); break;
+    case TA_BF16: ta::verify_kernel<__nv_bfloat16><<<B, ta::VERIFY_THREADS, 0, st>>>(a); break;
+    default: ta::verify_kernel<__half><<<B, ta::VERIFY_THREADS, 0, st>>>(a); break;
+  }
+  return check_launch(who);
+}
+
+}  // extern "C"

@@ -1,0 +1,731 @@
+// The 8-bit paged key / value cache: its layout, appending to it with the position rotation, and attention over it.
+//
+// A page holds P tokens (16, 32 or 64) of one sequence. The pool keeps one record of 2 * P * DH + 16 bytes per (page,
+// kv head): the e4m3 codes of the keys, those of the values, then the fp32 scales of the two; value = code * scale. A page
+// is quantised once, when its last token arrives, from 16-bit values: until then its tokens live in the 16-bit tail, a
+// ring of two pages per (sequence, kv head) addressed by the page's parity. So the codes depend on the tokens alone, not on
+// how they arrived, and a sequence can be cut back to any length whose last page is still in the ring.
+//
+// Inside a page (record and tail alike) the elements of each 16-token group stand in the order in which the m16n8k16
+// fragments take them, so that a warp reads a fragment with one vector load per lane from consecutive addresses:
+//   keys    [h][r][g][t][e]            token = 8 r + g, dim = h * 4E + t * E + e       (E = min(16, DH / 4))
+//   values  [c][g][t][m][r][kh][lo]    token = 8 kh + 2 t + lo, dim = (c * M + m) * 16 + 8 r + g    (M = 2, 1 at DH 16)
+// with g = lane / 4 and t = lane % 4.
+#pragma once
+#include <type_traits>
+#include <cuda_fp8.h>
+#include "common.cuh"
+
+namespace ta {
+
+template <int DH>
+struct PageShape {
+  static constexpr int E = DH >= 64 ? 16 : DH / 4;  // key elements of one token that a lane holds together
+  static constexpr int HG = DH / (4 * E);
+  static constexpr int M = DH >= 32 ? 2 : 1;        // 16-dim tiles of the values that a lane holds together
+  static constexpr int C = DH / (16 * M);
+};
+
+// Offset of an element in its 16-token group (DH * 16 elements), i = token of the group.
+template <int DH>
+__device__ __forceinline__ int key_offset(int i, int d) {
+  using S = PageShape<DH>;
+  const int h = d / (4 * S::E), t = (d / S::E) % 4, e = d % S::E;
+  return (((h * 2 + (i >> 3)) * 8 + (i & 7)) * 4 + t) * S::E + e;
+}
+template <int DH>
+__device__ __forceinline__ int value_offset(int i, int d) {
+  using S = PageShape<DH>;
+  const int c = d / (16 * S::M), m = (d / 16) % S::M, r = (d >> 3) & 1, g = d & 7;
+  const int kh = i >> 3, t = (i >> 1) & 3, lo = i & 1;
+  return ((((c * 8 + g) * 4 + t) * S::M + m) * 2 + r) * 4 + kh * 2 + lo;
+}
+
+// The cache of one layer, as every kernel here takes it.
+struct PagedCache {
+  unsigned char* pool;   // (n_pages, Hkv, record)
+  void* tail;            // (B, Hkv, 2 parities, 2 key / value, P * DH) 16-bit
+  const int32_t* table;  // (B, max_pages) page of each P tokens
+  int64_t table_sb;
+  int n_pages, max_pages, Hkv, P;
+};
+
+// Sequence b's new rows: rows [start[b], start[b + 1]) at positions pos[b] ... . Returns false (after recording the fault)
+// when the numbers do not describe rows of this call: nothing of the sequence is then read or written.
+struct NewRows {
+  int row0, n, pos;
+};
+__device__ __forceinline__ bool new_rows(const int32_t* start, const int32_t* pos, int b, int n_rows, int max_new,
+                                         const PagedCache& c, int kernel, NewRows& out) {
+  const int r0 = start[b], r1 = start[b + 1], p = pos[b];
+  out.row0 = r0;
+  out.n = r1 - r0;
+  out.pos = p;
+  if (r0 < 0 || r1 < r0 || r1 > n_rows || r1 - r0 > max_new) {
+    if (threadIdx.x == 0) record_error(DEV_INDEX_RANGE, kernel, b, r1 - r0);
+    return false;
+  }
+  if (p < 0 || (int64_t)p + (r1 - r0) > (int64_t)c.max_pages * c.P + (c.P - 1)) {
+    if (threadIdx.x == 0) record_error(DEV_POS_RANGE, kernel, b, p);
+    return false;
+  }
+  return true;
+}
+
+// ------------------------------------------------------------------------------------------------ append
+// One CTA per (sequence, page that its new tokens reach, kv head), and CTAs for the rotation of the queries.
+//   y1 = x1 cos - x2 sin, y2 = x2 cos + x1 sin   (dims i and i + rot / 2; products and sums rounded one by one in fp32)
+// rounded once to the 16-bit type: what the tail holds and what a full page is quantised from.
+//   scale = top / 448, code = e4m3(x * (448 / top)), top = the largest magnitude of the page's P x DH values.
+// A page whose top is below 2^-100 has codes 0 and scale 1; one that holds an infinity or NaN has codes 0 and scale NaN, so
+// that it reads back as NaN.
+constexpr int APPEND_THREADS = 128;
+
+struct AppendParams {
+  PagedCache c;
+  const void *k, *v, *q;
+  int64_t k_sr, k_sh, v_sr, v_sh, q_sr, q_sh;
+  void* q_out;  // (rows, Hq, DH) contiguous, or null
+  const int32_t *start, *pos;
+  const float *cosv, *sinv;  // (n_pos, rot / 2)
+  int n_pos, rot;
+  int n_rows, max_new, Hq;
+  int page_ctas;  // CTAs of a sequence that take pages; the others rotate queries
+};
+
+// Largest magnitude as the bit pattern of the 16-bit type (ordered like the values, infinities and NaN on top).
+template <typename T>
+__device__ __forceinline__ float bits_value(uint32_t b);
+template <>
+__device__ __forceinline__ float bits_value<__nv_bfloat16>(uint32_t b) { return __uint_as_float(b << 16); }
+template <>
+__device__ __forceinline__ float bits_value<__half>(uint32_t b) {
+  return __half2float(__ushort_as_half((unsigned short)b));
+}
+
+__device__ __forceinline__ uint16_t fp8x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+template <typename T, int DH>
+__global__ void __launch_bounds__(APPEND_THREADS) paged_append_kernel(AppendParams p) {
+  using S = PageShape<DH>;
+  constexpr int PITCH = DH + 8;  // shared rows: a fragment's 8 tokens fall on distinct banks
+  extern __shared__ __align__(16) unsigned char append_smem[];
+  __shared__ uint32_t tops[2][APPEND_THREADS / 32];
+  const int b = blockIdx.y, tid = threadIdx.x;
+  NewRows nr;
+  if (!new_rows(p.start, p.pos, b, p.n_rows, p.max_new, p.c, K_PAGED_APPEND, nr) || nr.n == 0) return;
+  const int half_rot = p.rot / 2;
+  if (p.rot && nr.pos + nr.n > p.n_pos) {
+    if (tid == 0) record_error(DEV_POS_RANGE, K_PAGED_APPEND, b, nr.pos + nr.n);
+    return;
+  }
+  if ((int)blockIdx.x >= p.page_ctas) {
+    // queries: pairs (or single elements beyond rot), consecutive threads on consecutive dims
+    const int cta = blockIdx.x - p.page_ctas, n_cta = gridDim.x - p.page_ctas;
+    const int per_head = DH - half_rot;  // half_rot pairs and DH - rot single elements
+    const int64_t total = (int64_t)nr.n * p.Hq * per_head;
+    for (int64_t id = (int64_t)cta * APPEND_THREADS + tid; id < total; id += (int64_t)n_cta * APPEND_THREADS) {
+      const int i = (int)(id % per_head);
+      const int64_t rh = id / per_head;
+      const int h = (int)(rh % p.Hq), r = (int)(rh / p.Hq);
+      const T* src = reinterpret_cast<const T*>(p.q) + (int64_t)(nr.row0 + r) * p.q_sr + (int64_t)h * p.q_sh;
+      T* dst = reinterpret_cast<T*>(p.q_out) + ((int64_t)(nr.row0 + r) * p.Hq + h) * DH;
+      if (i < half_rot) {
+        const int64_t at = (int64_t)(nr.pos + r) * half_rot + i;
+        const float c = p.cosv[at], s = p.sinv[at], x1 = to_f32(src[i]), x2 = to_f32(src[i + half_rot]);
+        dst[i] = from_f32<T>(__fsub_rn(__fmul_rn(x1, c), __fmul_rn(x2, s)));
+        dst[i + half_rot] = from_f32<T>(__fadd_rn(__fmul_rn(x2, c), __fmul_rn(x1, s)));
+      } else {
+        dst[i + half_rot] = src[i + half_rot];
+      }
+    }
+    return;
+  }
+  const int P = p.c.P, h = blockIdx.x % p.c.Hkv;
+  const int end = nr.pos + nr.n;
+  const int j = nr.pos / P + (int)blockIdx.x / p.c.Hkv;  // page
+  if (j * P >= end) return;
+  const bool full = (j + 1) * P <= end;
+  // The last two pages stay in 16 bits. Where the first page has earlier tokens in the tail, pages from the second after it
+  // on may share its slots: its own CTA, which reads those tokens, writes the later pages there after that.
+  const int f = nr.pos / P, last = (end - 1) / P;
+  const bool shares = nr.pos % P != 0 && j >= f + 2;
+  const bool keep = j >= last - 1 && !shares;
+  if (!full && shares) return;
+  const int i0 = max(nr.pos - j * P, 0), i1 = min(end - j * P, P);  // the page's new tokens
+  T* sk = reinterpret_cast<T*>(append_smem);
+  T* sv = sk + P * PITCH;
+  T* tk = reinterpret_cast<T*>(p.c.tail) + ((((int64_t)b * p.c.Hkv + h) * 2 + (j & 1)) * 2) * ((int64_t)P * DH);
+  T* tv = tk + (int64_t)P * DH;
+  // the page's tokens, token-major: new rows from the projection, earlier ones (of a page that is now full) from the tail
+  constexpr int VPR = DH / 8;
+  for (int id = tid; id < (i1 - i0) * VPR; id += APPEND_THREADS) {
+    const int i = i0 + id / VPR, d = (id % VPR) * 8;
+    const int64_t row = nr.row0 + (j * P + i - nr.pos);
+    *reinterpret_cast<uint4*>(sk + i * PITCH + d) =
+        *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.k) + row * p.k_sr + h * p.k_sh + d);
+    *reinterpret_cast<uint4*>(sv + i * PITCH + d) =
+        *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.v) + row * p.v_sr + h * p.v_sh + d);
+  }
+  if (full) {
+    for (int id = tid; id < i0 * DH; id += APPEND_THREADS) {
+      const int i = id / DH, d = id % DH;
+      sk[i * PITCH + d] = tk[(i >> 4) * 16 * DH + key_offset<DH>(i & 15, d)];
+      sv[i * PITCH + d] = tv[(i >> 4) * 16 * DH + value_offset<DH>(i & 15, d)];
+    }
+  }
+  __syncthreads();
+  if (half_rot) {
+    for (int id = tid; id < (i1 - i0) * half_rot; id += APPEND_THREADS) {
+      const int i = i0 + id / half_rot, d = id % half_rot;
+      const int64_t at = (int64_t)(j * P + i) * half_rot + d;
+      const float c = p.cosv[at], s = p.sinv[at];
+      const float x1 = to_f32(sk[i * PITCH + d]), x2 = to_f32(sk[i * PITCH + d + half_rot]);
+      sk[i * PITCH + d] = from_f32<T>(__fsub_rn(__fmul_rn(x1, c), __fmul_rn(x2, s)));
+      sk[i * PITCH + d + half_rot] = from_f32<T>(__fadd_rn(__fmul_rn(x2, c), __fmul_rn(x1, s)));
+    }
+    __syncthreads();
+  }
+  if (keep) {
+    for (int id = tid; id < (i1 - i0) * DH; id += APPEND_THREADS) {
+      const int i = i0 + id / DH, d = id % DH;
+      tk[(i >> 4) * 16 * DH + key_offset<DH>(i & 15, d)] = sk[i * PITCH + d];
+      tv[(i >> 4) * 16 * DH + value_offset<DH>(i & 15, d)] = sv[i * PITCH + d];
+    }
+  }
+  if (!full) return;
+  if (j == f && nr.pos % P != 0) {
+    // (the earlier tokens are in shared memory since the barrier after their loads)
+    for (int jj = max(f + 2, last - 1); jj <= last; ++jj) {
+      T* ok = reinterpret_cast<T*>(p.c.tail) + ((((int64_t)b * p.c.Hkv + h) * 2 + (jj & 1)) * 2) * ((int64_t)P * DH);
+      T* ov = ok + (int64_t)P * DH;
+      const int n = min(end - jj * P, P);
+      for (int id = tid; id < n * DH; id += APPEND_THREADS) {
+        const int i = id / DH, d = id % DH;
+        const int64_t row = nr.row0 + (jj * P + i - nr.pos);
+        const T* kr = reinterpret_cast<const T*>(p.k) + row * p.k_sr + h * p.k_sh;
+        const T* vr = reinterpret_cast<const T*>(p.v) + row * p.v_sr + h * p.v_sh;
+        T y = kr[d];
+        if (d < p.rot) {
+          const bool lo = d < half_rot;
+          const int64_t at = (int64_t)(jj * P + i) * half_rot + (lo ? d : d - half_rot);
+          const float c = p.cosv[at], s = p.sinv[at], x = to_f32(y), o = to_f32(kr[lo ? d + half_rot : d - half_rot]);
+          y = from_f32<T>(lo ? __fsub_rn(__fmul_rn(x, c), __fmul_rn(o, s)) : __fadd_rn(__fmul_rn(x, c), __fmul_rn(o, s)));
+        }
+        ok[(i >> 4) * 16 * DH + key_offset<DH>(i & 15, d)] = y;
+        ov[(i >> 4) * 16 * DH + value_offset<DH>(i & 15, d)] = vr[d];
+      }
+    }
+  }
+  uint32_t mk = 0, mv = 0;
+  for (int id = tid; id < P * VPR; id += APPEND_THREADS) {
+    const int at = (id / VPR) * PITCH + (id % VPR) * 8;
+    const uint4 a = *reinterpret_cast<const uint4*>(sk + at), w = *reinterpret_cast<const uint4*>(sv + at);
+    const uint32_t ka[4] = {a.x, a.y, a.z, a.w}, va[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      mk = max(mk, max(ka[x] & 0x7fffu, (ka[x] >> 16) & 0x7fffu));
+      mv = max(mv, max(va[x] & 0x7fffu, (va[x] >> 16) & 0x7fffu));
+    }
+  }
+  mk = __reduce_max_sync(0xffffffffu, mk);
+  mv = __reduce_max_sync(0xffffffffu, mv);
+  if ((tid & 31) == 0) {
+    tops[0][tid >> 5] = mk;
+    tops[1][tid >> 5] = mv;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < APPEND_THREADS / 32; ++w) {
+    mk = max(mk, tops[0][w]);
+    mv = max(mv, tops[1][w]);
+  }
+  const int phys = j < p.c.max_pages ? p.c.table[b * p.c.table_sb + j] : -1;
+  if (phys < 0 || phys >= p.c.n_pages) {
+    if (tid == 0) record_error(DEV_INDEX_RANGE, K_PAGED_APPEND, b, phys);
+    return;
+  }
+  float mul[2], scale[2];
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const float top = bits_value<T>(x ? mv : mk);
+    const bool odd = !(top <= 3.402823466e38f), tiny = top < 7.888609052e-31f;  // 2^-100
+    mul[x] = odd || tiny ? 0.f : __fdiv_rn(448.f, top);
+    scale[x] = odd ? __int_as_float(0x7fc00000) : (tiny ? 1.f : __fdiv_rn(top, 448.f));
+  }
+  unsigned char* rec = p.c.pool + ((int64_t)phys * p.c.Hkv + h) * (2 * P * DH + 16);
+  if (tid == 0) {
+    reinterpret_cast<float*>(rec + 2 * P * DH)[0] = scale[0];
+    reinterpret_cast<float*>(rec + 2 * P * DH)[1] = scale[1];
+  }
+  // a page with a non-finite element has codes 0 (0 * NaN would not be)
+  const bool zk = mul[0] == 0.f, zv = mul[1] == 0.f;
+  for (int id = tid; id < P * DH / 4; id += APPEND_THREADS) {
+    // keys: 4 consecutive dims of one token
+    const int grp = id / (4 * DH), o = (id % (4 * DH)) * 4;  // offset in the group's 16 * DH elements
+    const int e = o % S::E, t = (o / S::E) % 4, g = (o / (4 * S::E)) % 8, r = (o / (32 * S::E)) % 2, hg = o / (64 * S::E);
+    const T* a = sk + (grp * 16 + r * 8 + g) * PITCH + hg * 4 * S::E + t * S::E + e;
+    uint32_t w = fp8x2(to_f32(a[0]) * mul[0], to_f32(a[1]) * mul[0]) |
+                 ((uint32_t)fp8x2(to_f32(a[2]) * mul[0], to_f32(a[3]) * mul[0]) << 16);
+    reinterpret_cast<uint32_t*>(rec)[id] = zk ? 0u : w;
+    // values: one dim of 4 tokens
+    const int x = o / 4, vr = x % 2, m = (x / 2) % S::M, vt = (x / (2 * S::M)) % 4, vg = (x / (8 * S::M)) % 8,
+              c = x / (64 * S::M);
+    const T* v0 = sv + (grp * 16 + 2 * vt) * PITCH + (c * S::M + m) * 16 + vr * 8 + vg;
+    w = fp8x2(to_f32(v0[0]) * mul[1], to_f32(v0[PITCH]) * mul[1]) |
+        ((uint32_t)fp8x2(to_f32(v0[8 * PITCH]) * mul[1], to_f32(v0[9 * PITCH]) * mul[1]) << 16);
+    reinterpret_cast<uint32_t*>(rec + P * DH)[id] = zv ? 0u : w;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ attention
+// out[r] = sum_t softmax_t(scale q_r . K_t) V_t over the positions t <= pos + i of query i (and t > pos + i - window).
+// Rows of a (sequence, kv head): query i, head gq of the group -> row i * group + gq. A warp takes 8 NT rows as the N side of
+// mma.m16n8k16 and the keys (S^T = K Q^T) or the head dims (O^T = V^T P^T) as the M side, so that one key or value fragment
+// serves every row and a lone row costs one n-tile.
+//  * codes go to f16 exactly; q is scaled by a power of two per row (exact, undone in the score's factor) so that bf16
+//    rows fit f16 as well; the products are exact and the sums fp32.
+//  * the value scale joins the weight: w_t = exp2(s_t + log2 vs - ref), with the running reference taken over s + log2 vs, so
+//    that every w stays in f16's range (at most 2^12); the denominator adds w / vs in fp32. w is rounded to f16 (2^-12
+//    relative) for the product, the denominator takes it unrounded.
+//  * the open page is read in 16 bits from the tail, in the same element order, with the 16-bit type's own mma.
+constexpr float ATTN_SHIFT = 12.f;
+
+struct AttnParams {
+  PagedCache c;
+  const void* q;
+  int64_t q_sr, q_sh;
+  const int32_t *start, *pos;
+  int B, n_rows, max_new, Hq;
+  float scale;
+  int window;  // 0 = the whole prefix
+  void* out;
+  int64_t o_sr, o_sh;
+  float* lse;  // (rows, Hq) or null
+};
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <typename T>
+__device__ __forceinline__ void mma_16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    mma_f16(d, a, b0, b1);
+  else
+    mma_bf16(d, a, b0, b1);
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+// two e4m3 codes -> f16x2
+__device__ __forceinline__ uint32_t codes_f16x2(uint32_t two) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 c;\n\tcvt.u16.u32 c, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, c;\n\t}" : "=r"(r) : "r"(two));
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <int BYTES>
+__device__ __forceinline__ void load_words(const void* p, uint32_t (&w)[BYTES / 4]) {
+  if constexpr (BYTES >= 16) {
+#pragma unroll
+    for (int i = 0; i < BYTES / 16; ++i) {
+      const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+      w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+    }
+  } else if constexpr (BYTES == 8) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x; w[1] = v.y;
+  } else {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  }
+}
+
+// The rows of one tile: query fragments and what the masks and scores need, per lane for its two columns of each n-tile.
+template <typename T, int DH, int NT>
+struct RowTile {
+  using S = PageShape<DH>;
+  uint32_t qf[DH / 16][NT][2];  // f16, scaled per row
+  float cs[NT][2];              // score factor of the row: scale * log2(e) / (its power of two)
+  int qpos[NT][2];              // position of the row's query; -1: no such row
+
+  // row0: first row of the tile; R rows in all (n queries x group heads)
+  __device__ __forceinline__ void load(const AttnParams& p, const NewRows& nr, int h, int group, int row0, int R) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int rr = row0 + nt * 8 + g;
+      const bool live = rr < R;
+      const T* src = reinterpret_cast<const T*>(p.q);
+      if (live) src += (int64_t)(nr.row0 + rr / group) * p.q_sr + (int64_t)(h * group + rr % group) * p.q_sh;
+      float x[DH / 4];
+      float top = 0.f;
+#pragma unroll
+      for (int hg = 0; hg < S::HG; ++hg)
+#pragma unroll
+        for (int e = 0; e < S::E; e += 4) {
+          uint32_t w[2] = {0u, 0u};
+          if (live) load_words<8>(src + hg * 4 * S::E + t * S::E + e, w);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float f = bits_value<T>((w[i >> 1] >> (16 * (i & 1))) & 0xffffu);
+            x[hg * S::E + e + i] = f;
+            top = fmaxf(top, fabsf(f));
+          }
+        }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // 2^ex * top in [2^14, 2^15): exact, and what falls below f16's range is below 2^-39 of the row's largest element
+      int ex = 0;
+      if (top > 0.f && top <= 3.402823466e38f) ex = 14 - ilogbf(top);
+      ex = min(ex, 120);
+      const float up = exp2f((float)ex);
+#pragma unroll
+      for (int kk = 0; kk < DH / 16; ++kk) {
+        qf[kk][nt][0] = pack2<__half>(x[kk * 4] * up, x[kk * 4 + 1] * up);
+        qf[kk][nt][1] = pack2<__half>(x[kk * 4 + 2] * up, x[kk * 4 + 3] * up);
+      }
+      const float f = p.scale * 1.4426950408889634f * exp2f((float)-ex);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        cs[nt][i] = __shfl_sync(0xffffffffu, f, (2 * t + i) * 4);
+        const int col = row0 + nt * 8 + 2 * t + i;
+        qpos[nt][i] = col < R ? nr.pos + col / group : -1;
+      }
+    }
+  }
+};
+
+// Running softmax of a warp: reference (log2 units, uniform over the 8 lanes of a column), denominator (each lane its
+// own tokens' part), numerator O^T.
+template <int DH, int NT>
+struct SoftState {
+  float m[NT][2], l[NT][2], o[DH / 16][NT][4];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+      for (int x = 0; x < DH / 16; ++x)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[x][nt][i] = 0.f;
+    }
+  }
+};
+
+// Scores -> weights for TG 16-token groups: s holds the raw sums and leaves as the packed P^T fragments pf. ks / lv / iv: per
+// group the key scale, log2 of the value scale and its inverse. tok0: position of the first token; tokens from `limit` on
+// are not the unit's.
+template <typename T, int DH, int NT, int TG>
+__device__ __forceinline__ void soft_step(const RowTile<T, DH, NT>& rt, SoftState<DH, NT>& st, float (&s)[TG][NT][4],
+                                          const float (&ks)[TG], const float (&lv)[TG], const float (&iv)[TG], int tok0,
+                                          int limit, int window, bool mask) {
+  const int g = (threadIdx.x & 31) >> 2;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int x = 0; x < TG; ++x)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float v = fmaf(s[x][nt][i], ks[x] * rt.cs[nt][i & 1], lv[x]);
+        if (mask) {
+          const int tok = tok0 + x * 16 + (i >> 1) * 8 + g, qp = rt.qpos[nt][i & 1];
+          if (tok > qp || tok >= limit || (window > 0 && tok <= qp - window)) v = -INFINITY;
+        }
+        s[x][nt][i] = v;
+        top[i & 1] = fmaxf(top[i & 1], v);
+      }
+    float ref[2];
+    bool moved = false;
+    float fac[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 4));
+      top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 8));
+      top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 16));
+      const float mn = fmaxf(st.m[nt][i], top[i]);
+      fac[i] = mn == st.m[nt][i] ? 1.f : exp2f(st.m[nt][i] - mn);
+      moved |= mn != st.m[nt][i];
+      st.m[nt][i] = mn;
+      ref[i] = mn == -INFINITY ? 0.f : mn - ATTN_SHIFT;
+    }
+    if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) st.l[nt][i] *= fac[i];
+#pragma unroll
+      for (int x = 0; x < DH / 16; ++x)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) st.o[x][nt][i] *= fac[i & 1];
+    }
+#pragma unroll
+    for (int x = 0; x < TG; ++x) {
+      float sum[2];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        // a masked token weighs 0 whatever its page holds
+        const float v = s[x][nt][i];
+        s[x][nt][i] = v == -INFINITY ? 0.f : exp2f(v - ref[i & 1]);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        sum[i] = s[x][nt][i] + s[x][nt][i + 2];
+        st.l[nt][i] += sum[i] == 0.f ? 0.f : sum[i] * iv[x];
+      }
+    }
+  }
+}
+
+// One unit of TG 16-token groups of 8-bit pages: kp / vp per group its key and value codes.
+template <typename T, int DH, int NT, int TG>
+__device__ __forceinline__ void attend_codes(const RowTile<T, DH, NT>& rt, SoftState<DH, NT>& st,
+                                             const unsigned char* const (&kp)[TG], const unsigned char* const (&vp)[TG],
+                                             const float (&ks)[TG], const float (&lv)[TG], const float (&iv)[TG],
+                                             int tok0, int limit, int window, bool mask) {
+  using S = PageShape<DH>;
+  const int lane = threadIdx.x & 31;
+  float s[TG][NT][4];
+#pragma unroll
+  for (int x = 0; x < TG; ++x)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[x][nt][i] = 0.f;
+#pragma unroll
+  for (int hg = 0; hg < S::HG; ++hg)
+#pragma unroll
+    for (int x = 0; x < TG; ++x) {
+      uint32_t w0[S::E / 4], w1[S::E / 4];
+      load_words<S::E>(kp[x] + (hg * 2 * 32 + lane) * S::E, w0);
+      load_words<S::E>(kp[x] + ((hg * 2 + 1) * 32 + lane) * S::E, w1);
+#pragma unroll
+      for (int e = 0; e < S::E / 4; ++e) {
+        const uint32_t a[4] = {codes_f16x2(w0[e]), codes_f16x2(w1[e]), codes_f16x2(w0[e] >> 16), codes_f16x2(w1[e] >> 16)};
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) mma_f16(s[x][nt], a, rt.qf[hg * (S::E / 4) + e][nt][0], rt.qf[hg * (S::E / 4) + e][nt][1]);
+      }
+    }
+  soft_step<T, DH, NT, TG>(rt, st, s, ks, lv, iv, tok0, limit, window, mask);
+  uint32_t pf[TG][NT][2];
+#pragma unroll
+  for (int x = 0; x < TG; ++x)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      pf[x][nt][0] = transpose8x8(pack2<__half>(s[x][nt][0], s[x][nt][1]));
+      pf[x][nt][1] = transpose8x8(pack2<__half>(s[x][nt][2], s[x][nt][3]));
+    }
+#pragma unroll
+  for (int x = 0; x < TG; ++x)
+#pragma unroll
+    for (int c = 0; c < S::C; ++c) {
+      uint32_t w[2 * S::M];
+      load_words<8 * S::M>(vp[x] + (c * 32 + lane) * 8 * S::M, w);
+#pragma unroll
+      for (int m = 0; m < S::M; ++m) {
+        const uint32_t a[4] = {codes_f16x2(w[2 * m]), codes_f16x2(w[2 * m + 1]), codes_f16x2(w[2 * m] >> 16),
+                               codes_f16x2(w[2 * m + 1] >> 16)};
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) mma_f16(st.o[c * S::M + m][nt], a, pf[x][nt][0], pf[x][nt][1]);
+      }
+    }
+}
+
+// One 16-token group of the open page, 16-bit elements in the same order. len: tokens the sequence holds; later slots
+// of the page hold anything and are masked in the scores and zeroed in the values.
+template <typename T, int DH, int NT>
+__device__ __forceinline__ void attend_tail(const AttnParams& p, const NewRows& nr, int h, int group, int row0, int R,
+                                            const RowTile<T, DH, NT>& rt, SoftState<DH, NT>& st, const T* kp, const T* vp,
+                                            int tok0, int len) {
+  using S = PageShape<DH>;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  float s[1][NT][4];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[0][nt][i] = 0.f;
+  const T* qr[NT];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int rr = min(row0 + nt * 8 + g, R - 1);
+    qr[nt] = reinterpret_cast<const T*>(p.q) + (int64_t)(nr.row0 + rr / group) * p.q_sr +
+             (int64_t)(h * group + rr % group) * p.q_sh;
+  }
+#pragma unroll
+  for (int hg = 0; hg < S::HG; ++hg)
+#pragma unroll
+    for (int e = 0; e < S::E / 4; ++e) {
+      uint32_t w0[2], w1[2];
+      load_words<8>(kp + (hg * 2 * 32 + lane) * S::E + e * 4, w0);
+      load_words<8>(kp + ((hg * 2 + 1) * 32 + lane) * S::E + e * 4, w1);
+      const uint32_t a[4] = {w0[0], w1[0], w0[1], w1[1]};
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        uint32_t q[2];
+        load_words<8>(qr[nt] + hg * 4 * S::E + t * S::E + e * 4, q);
+        mma_16<T>(s[0][nt], a, q[0], q[1]);
+      }
+    }
+  // unscaled rows: the score factor without the f16 rows' power of two
+  RowTile<T, DH, NT> plain;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      plain.cs[nt][i] = p.scale * 1.4426950408889634f;
+      plain.qpos[nt][i] = rt.qpos[nt][i];
+    }
+  const float one[1] = {1.f}, zero[1] = {0.f};
+  soft_step<T, DH, NT, 1>(plain, st, s, one, zero, one, tok0, len, p.window, true);
+  uint32_t pf[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    pf[nt][0] = transpose8x8(pack2<T>(s[0][nt][0], s[0][nt][1]));
+    pf[nt][1] = transpose8x8(pack2<T>(s[0][nt][2], s[0][nt][3]));
+  }
+  const int k0 = tok0 + 2 * t;
+  const uint32_t keep0 = (k0 < len ? 0xffffu : 0u) | (k0 + 1 < len ? 0xffff0000u : 0u);
+  const uint32_t keep1 = (k0 + 8 < len ? 0xffffu : 0u) | (k0 + 9 < len ? 0xffff0000u : 0u);
+#pragma unroll
+  for (int c = 0; c < S::C; ++c) {
+    uint32_t w[4 * S::M];
+    load_words<16 * S::M>(vp + (c * 32 + lane) * 8 * S::M, w);
+#pragma unroll
+    for (int m = 0; m < S::M; ++m) {
+      const uint32_t a[4] = {w[4 * m] & keep0, w[4 * m + 2] & keep0, w[4 * m + 1] & keep1, w[4 * m + 3] & keep1};
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) mma_16<T>(st.o[c * S::M + m][nt], a, pf[nt][0], pf[nt][1]);
+    }
+  }
+}
+
+// A (row tile, kv head, sequence) per CTA: its 4 warps take the 64-token units in turn, each with its own running softmax,
+// and the four states are joined in shared memory.
+constexpr int ATTN_WARPS = 4;
+
+template <int DH, int NT>
+__host__ __device__ constexpr int attn_smem_bytes() {
+  return ATTN_WARPS * 8 * NT * (DH + 4) * 4 + ATTN_WARPS * 8 * NT * 2 * 4;
+}
+
+template <typename T, int DH, int NT>
+__global__ void __launch_bounds__(ATTN_WARPS * 32) paged_attn_kernel(AttnParams p) {
+  constexpr int ROWS = 8 * NT, PITCH = DH + 4;
+  extern __shared__ __align__(16) unsigned char attn_smem[];
+  float* so = reinterpret_cast<float*>(attn_smem);       // (warp, row, DH)
+  float* sm = so + ATTN_WARPS * ROWS * PITCH;            // (warp, row)
+  float* sl = sm + ATTN_WARPS * ROWS;
+  const int b = blockIdx.z, h = blockIdx.y, row0 = blockIdx.x * ROWS;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  NewRows nr;
+  if (!new_rows(p.start, p.pos, b, p.n_rows, p.max_new, p.c, K_PAGED_ATTN, nr)) return;
+  const int group = p.Hq / p.c.Hkv, R = nr.n * group, P = p.c.P;
+  if (row0 >= R) return;
+  const int len = nr.pos + nr.n, n_full = len / P;
+  const int qlo = nr.pos + row0 / group, qhi = nr.pos + (min(R, row0 + ROWS) - 1) / group;
+  const int lo = p.window > 0 ? max(0, qlo - p.window + 1) : 0;
+  const int p0 = lo / P, p1 = min(n_full, qhi / P + 1), limit = p1 * P;
+  const int per = 64 / P;
+  RowTile<T, DH, NT> rt;
+  rt.load(p, nr, h, group, row0, R);
+  SoftState<DH, NT> st;
+  st.clear();
+  const int32_t* tab = p.c.table + b * p.c.table_sb;
+  const int64_t rec_bytes = 2 * P * DH + 16;
+  for (int u = p0 + warp * per; u < p1; u += ATTN_WARPS * per) {
+    const unsigned char *kp[4], *vp[4];
+    float ks[4], lv[4], iv[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int pg = min(u + x * 16 / P, p1 - 1);
+      int phys = tab[pg];
+      if (phys < 0 || phys >= p.c.n_pages) {
+        if (lane == 0) record_error(DEV_INDEX_RANGE, K_PAGED_ATTN, b, phys);
+        phys = 0;
+      }
+      const unsigned char* rec = p.c.pool + ((int64_t)phys * p.c.Hkv + h) * rec_bytes;
+      kp[x] = rec + (x * 16 % P) * DH;
+      vp[x] = kp[x] + P * DH;
+      const float2 sc = *reinterpret_cast<const float2*>(rec + 2 * P * DH);
+      ks[x] = sc.x;
+      lv[x] = log2f(sc.y);
+      iv[x] = 1.f / sc.y;
+    }
+    const int tok0 = u * P;
+    const bool mask = tok0 + 63 > min(qlo, limit - 1) || (p.window > 0 && tok0 <= qhi - p.window);
+    attend_codes<T, DH, NT, 4>(rt, st, kp, vp, ks, lv, iv, tok0, limit, p.window, mask);
+  }
+  if (n_full * P <= qhi) {
+    const T* tk = reinterpret_cast<const T*>(p.c.tail) +
+                  ((((int64_t)b * p.c.Hkv + h) * 2 + (n_full & 1)) * 2) * ((int64_t)P * DH);
+    for (int x = warp; n_full * P + x * 16 <= qhi; x += ATTN_WARPS)
+      attend_tail<T, DH, NT>(p, nr, h, group, row0, R, rt, st, tk + x * 16 * DH, tk + (int64_t)P * DH + x * 16 * DH,
+                             n_full * P + x * 16, len);
+  }
+  // join the warps
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float l = st.l[nt][i];
+      l += __shfl_xor_sync(0xffffffffu, l, 4);
+      l += __shfl_xor_sync(0xffffffffu, l, 8);
+      l += __shfl_xor_sync(0xffffffffu, l, 16);
+      const int col = nt * 8 + 2 * t + i;
+      if (g == 0) {
+        sm[warp * ROWS + col] = st.m[nt][i];
+        sl[warp * ROWS + col] = l;
+      }
+#pragma unroll
+      for (int x = 0; x < DH / 16; ++x) {
+        so[(warp * ROWS + col) * PITCH + x * 16 + g] = st.o[x][nt][i];
+        so[(warp * ROWS + col) * PITCH + x * 16 + 8 + g] = st.o[x][nt][i + 2];
+      }
+    }
+  __syncthreads();
+  for (int id = tid; id < ROWS * DH; id += ATTN_WARPS * 32) {
+    const int col = id / DH, d = id % DH, rr = row0 + col;
+    if (rr >= R) break;
+    float m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < ATTN_WARPS; ++w) m = fmaxf(m, sm[w * ROWS + col]);
+    float L = 0.f, o = 0.f;
+#pragma unroll
+    for (int w = 0; w < ATTN_WARPS; ++w) {
+      const float f = sm[w * ROWS + col] == -INFINITY ? 0.f : exp2f(sm[w * ROWS + col] - m);
+      if (f == 0.f && m != -INFINITY && sl[w * ROWS + col] == 0.f) continue;
+      L += sl[w * ROWS + col] * f;
+      o += so[(w * ROWS + col) * PITCH + d] * f;
+    }
+    const int64_t row = nr.row0 + rr / group;
+    const int hq = h * group + rr % group;
+    reinterpret_cast<T*>(p.out)[row * p.o_sr + hq * p.o_sh + d] = from_f32<T>(L == 0.f ? 0.f : o / L);
+    if (p.lse && d == 0)
+      p.lse[row * p.Hq + hq] = L == 0.f ? -INFINITY : (m - ATTN_SHIFT + log2f(L)) * 0.69314718055994531f;
+  }
+}
+
+}  // namespace ta

@@ -1,11 +1,10 @@
 // C ABI of the treeattn_b200 kernels: argument checks, launch shapes, dispatch over dtype x head dim.
-// Single translation unit: every kernel header is included here.
+// The serving operators (paged cache, draft verification) are in paged.cu; every other kernel header is included here.
 #include <cuda_runtime.h>
 
 #include <algorithm>
 #include <atomic>
 #include <climits>
-#include <cstdarg>
 #include <cstdio>
 #include <map>
 #include <mutex>
@@ -21,110 +20,18 @@
 #include "decode.cuh"
 #include "dyn.cuh"
 #include "forest.cuh"
+#include "host.cuh"
 #include "linear.cuh"
 #include "model_ops.cuh"
 #include "prefill.cuh"
 
+namespace ta_host {
+cudaError_t paged_device_error(int* out4);  // the error record of paged.cu, read and cleared
+}
+
 namespace {
 
-thread_local std::string g_err;
-
-int fail(int code, const char* fmt, ...) {
-  char buf[512];
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(buf, sizeof(buf), fmt, ap);
-  va_end(ap);
-  g_err = buf;
-  return code;
-}
-
-int check_launch(const char* what) {
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return fail(TA_ERR_CUDA, "%s: launch failed: %s", what, cudaGetErrorString(e));
-  return TA_OK;
-}
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
-// a row of dh elements of `esize` bytes read in 16-byte chunks: base and every stride must keep 16-byte
-// alignment
-bool rows_aligned(const void* base, int esize, std::initializer_list<int64_t> strides) {
-  if (!aligned16(base)) return false;
-  for (int64_t s : strides)
-    if ((s * esize) % 16 != 0) return false;
-  return true;
-}
-
-int esize_of(int dtype) { return dtype == TA_F32 ? 4 : 2; }
-
-bool valid_dtype(int dtype) { return dtype == TA_F32 || dtype == TA_BF16 || dtype == TA_F16; }
-
-bool valid_dh(int dh) { return dh == 16 || dh == 32 || dh == 64 || dh == 128; }
-
-cudaStream_t S(void* s) { return reinterpret_cast<cudaStream_t>(s); }
-
-// Per-device state of one launcher. cudaFuncSetAttribute and the occupancy and SM-count queries answer for the
-// current device only, so a process that drives several GPUs keeps one entry per device (the first 64 devices
-// are cached; others are asked again on every call).
-constexpr int kDevCache = 64;
-
-int current_device() {
-  int dev = -1;
-  if (cudaGetDevice(&dev) != cudaSuccess) dev = -1;
-  return dev;
-}
-
-// The dynamic shared-memory size a call site has allowed for its kernel, per device (0 = not yet).
-struct SmemAttr {
-  std::atomic<size_t> bytes[kDevCache];
-};
-
-// Allow `bytes` of dynamic shared memory for kern on the current device. The attribute is always set to the most
-// the device gives one block beside the kernel's static shared memory: a kernel launched from several call sites
-// (or launcher instantiations) then never has its limit lowered by one of them under another's launch.
-template <typename K>
-int allow_smem(SmemAttr& a, K* kern, size_t bytes, const char* what) {
-  const int dev = current_device();
-  const bool cached = dev >= 0 && dev < kDevCache;
-  if (cached) {
-    const size_t have = a.bytes[dev].load(std::memory_order_relaxed);
-    if (have >= bytes) return TA_OK;
-    if (have != 0) return fail(TA_ERR_ARG, "%s: %zu B of dynamic shared memory, above the %zu B a block can have",
-                               what, bytes, have);
-  }
-  int optin = 0;
-  cudaFuncAttributes fa;
-  if (cudaDeviceGetAttribute(&optin, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev < 0 ? 0 : dev) != cudaSuccess ||
-      cudaFuncGetAttributes(&fa, kern) != cudaSuccess)
-    return check_launch(what);
-  const size_t most = (size_t)optin > fa.sharedSizeBytes ? (size_t)optin - fa.sharedSizeBytes : 0;
-  if (bytes > most)
-    return fail(TA_ERR_ARG, "%s: %zu B of dynamic shared memory, above the %zu B a block can have", what, bytes, most);
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most) != cudaSuccess) {
-    const cudaError_t e = cudaGetLastError();
-    return fail(TA_ERR_CUDA, "%s: dynamic shared memory limit of %zu B refused: %s", what, most, cudaGetErrorString(e));
-  }
-  if (cached) a.bytes[dev].store(most, std::memory_order_relaxed);
-  return TA_OK;
-}
-
-// Launch with programmatic stream serialization: the kernel may start while the previous kernel of the stream is
-// still running (it calls griddepcontrol.wait before reading anything that kernel writes).
-template <typename... KArgs, typename... Args>
-cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args&&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
-}
+using namespace ta_host;
 
 // Dispatch F<T, DH>::run(args...) over the runtime dtype and head dim.
 template <template <typename, int> class F, typename T, typename... Args>
@@ -1051,6 +958,10 @@ int ta_device_error(int* out4) {
   const int zero[4] = {0, 0, 0, 0};
   e = cudaMemcpyToSymbol(ta::g_dev_err, zero, 4 * sizeof(int));
   if (e != cudaSuccess) return fail(TA_ERR_CUDA, "ta_device_error: %s", cudaGetErrorString(e));
+  int other[4];
+  e = ta_host::paged_device_error(other);
+  if (e != cudaSuccess) return fail(TA_ERR_CUDA, "ta_device_error: %s", cudaGetErrorString(e));
+  if (out4[0] == 0) std::copy(other, other + 4, out4);
   return TA_OK;
 }
 

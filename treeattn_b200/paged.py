@@ -1,0 +1,254 @@
+"""Serving over an 8-bit paged key / value cache: the cache, appending to it with the position rotation, attention over
+it for one or several new tokens of each sequence, and the verification of drafted tokens.
+
+The reference's engine keeps one fp32 tensor per sequence and decodes one token at a time (engine.py:74-81, 149-177); these
+operators are the dense model's side of speculative decoding: the segment-tree Decoder drafts, the dense model verifies
+(speculative.py runs the two together). Like every entry point of this package they take CUDA tensors, check them, and
+enqueue on the current stream without synchronising."""
+import math
+
+import torch
+
+from . import _lib
+from ._ops import _DT, _need_cuda, _p, _stream
+
+PAGE_SIZES = (16, 32, 64)
+
+
+class PagedKV:
+    """The cache of one layer: the tensors that the kernels read and write (include/treeattn_b200.h has the layout).
+
+    pool (n_pages, n_kv_head, 2 * page * head_dim + 16) uint8: a record per (page, kv head): e4m3 codes of the keys, of the
+    values, their two fp32 scales. tail (batch, n_kv_head, 2, 2, page * head_dim) bf16 or f16: the open page of each sequence
+    and the one before it. table (batch, max_pages) int32: the pool page of each page of a sequence (several layers may
+    share one). PagedKV.empty allocates pool and tail."""
+    __slots__ = ('pool', 'tail', 'table', 'page', 'head_dim')
+
+    def __init__(self, pool, tail, table, page, head_dim):
+        self.pool, self.tail, self.table, self.page, self.head_dim = pool, tail, table, int(page), int(head_dim)
+        if self.page not in PAGE_SIZES:
+            raise ValueError('PagedKV: pages of 16, 32 or 64 tokens (got %d)' % self.page)
+        if pool.dtype != torch.uint8 or pool.dim() != 3 or pool.shape[2] != 2 * self.page * self.head_dim + 16:
+            raise ValueError('PagedKV: pool must be (n_pages, n_kv_head, 2 * page * head_dim + 16) uint8')
+        if tail.dim() != 5 or tail.shape[1:] != (pool.shape[1], 2, 2, self.page * self.head_dim):
+            raise ValueError('PagedKV: tail must be (batch, n_kv_head, 2, 2, page * head_dim)')
+        if tail.dtype not in (torch.bfloat16, torch.float16):
+            raise TypeError('PagedKV: the tail holds bfloat16 or float16 (got %s)' % tail.dtype)
+        if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != tail.shape[0] or (
+                table.shape[1] > 1 and table.stride(1) != 1):
+            raise ValueError('PagedKV: table must be (batch, max_pages) int32 with unit inner stride')
+        if not (pool.is_contiguous() and tail.is_contiguous()):
+            raise ValueError('PagedKV: pool and tail must be contiguous')
+        _need_cuda('PagedKV', pool, tail, table)
+
+    @classmethod
+    def empty(cls, n_pages, n_kv_head, head_dim, table, page=64, dtype=torch.bfloat16):
+        dev = table.device
+        return cls(torch.zeros(n_pages, n_kv_head, 2 * page * head_dim + 16, device=dev, dtype=torch.uint8),
+                   torch.zeros(table.shape[0], n_kv_head, 2, 2, page * head_dim, device=dev, dtype=dtype), table, page,
+                   head_dim)
+
+    @property
+    def n_kv_head(self):
+        return self.pool.shape[1]
+
+    def _keys(self, x):
+        P, dh = self.page, self.head_dim
+        E = min(16, dh // 4)
+        d = x.dim() - 1
+        return x.unflatten(-1, (P // 16, dh // (4 * E), 2, 8, 4, E)).permute(
+            *range(d), d, d + 2, d + 3, d + 1, d + 4, d + 5).reshape(*x.shape[:-1], P, dh)
+
+    def _values(self, x):
+        P, dh = self.page, self.head_dim
+        M = min(2, dh // 16)
+        d = x.dim() - 1
+        return x.unflatten(-1, (P // 16, dh // (16 * M), 8, 4, M, 2, 2, 2)).permute(
+            *range(d), d, d + 6, d + 3, d + 7, d + 1, d + 4, d + 5, d + 2).reshape(*x.shape[:-1], P, dh)
+
+    def read(self, b, length):
+        """Keys and values (n_kv_head, length, head_dim) fp32 of sequence b's first `length` positions, as attention sees
+        them: full pages from the codes, the rest from the tail."""
+        P, n = self.page, self.page * self.head_dim
+        full = length // P
+        rec = self.pool[self.table[b, :full].long()]
+        codes = rec[..., :2 * n].view(torch.float8_e4m3fn)
+        scale = rec[..., 2 * n:2 * n + 8].contiguous().view(torch.float32)
+        out = []
+        for i, order in enumerate((self._keys, self._values)):
+            x = order(codes[..., i * n:(i + 1) * n]).float() * scale[..., i, None, None]
+            x = x.transpose(0, 1).reshape(self.n_kv_head, full * P, self.head_dim)
+            rest = order(self.tail[b, :, full % 2, i])[:, :length - full * P].float()
+            out.append(torch.cat([x, rest], 1))
+        return out
+
+
+class PagePool:
+    """Which pages of a pool are free, and the table of those that are not: host bookkeeping for a batch of sequences. The
+    device table is updated by one small copy when a sequence gets new pages."""
+
+    def __init__(self, n_pages, batch, max_pages, page, device='cuda'):
+        self.page, self.n_pages, self.max_pages = int(page), int(n_pages), int(max_pages)
+        self.free = list(range(n_pages - 1, -1, -1))
+        self.owned = [[] for _ in range(batch)]
+        self.host = torch.zeros(batch, max_pages, dtype=torch.int32)
+        self.table = torch.zeros(batch, max_pages, device=device, dtype=torch.int32)
+
+    def reserve(self, lengths):
+        """Makes room for lengths[b] positions of each sequence b (a list; shorter ones keep what they have). Raises
+        MemoryError, with nothing changed, when the pool has too few free pages."""
+        need = [max(0, -(-int(n) // self.page) - len(o)) for n, o in zip(lengths, self.owned)]
+        for n, k in zip(lengths, need):
+            if -(-int(n) // self.page) > self.max_pages:
+                raise ValueError('PagePool: %d positions above the %d of a sequence' % (n, self.max_pages * self.page))
+        if sum(need) > len(self.free):
+            raise MemoryError('PagePool: %d pages wanted, %d free' % (sum(need), len(self.free)))
+        for b, k in enumerate(need):
+            for _ in range(k):
+                self.host[b, len(self.owned[b])] = self.free[-1]
+                self.owned[b].append(self.free.pop())
+        if any(need):
+            self.table.copy_(self.host)
+
+    def release(self, b):
+        """Gives sequence b's pages back."""
+        self.free.extend(reversed(self.owned[b]))
+        self.owned[b] = []
+
+
+def rotation_table(n_pos, rot, base=10000.0, device='cuda'):
+    """(cos, sin) (n_pos, rot / 2) fp32 of the angles pos * base^(-2 i / rot), formed in 64 bits."""
+    if rot < 2 or rot % 2:
+        raise ValueError('rotation_table: rot must be even and positive (got %d)' % rot)
+    f = base ** (-torch.arange(0, rot, 2, device=device, dtype=torch.float64) / rot)
+    a = torch.arange(n_pos, device=device, dtype=torch.float64)[:, None] * f
+    return a.cos().float(), a.sin().float()
+
+
+def _rows(name, cache, start, pos):
+    if start.dtype != torch.int32 or pos.dtype != torch.int32 or not start.is_contiguous() or not pos.is_contiguous():
+        raise TypeError('%s: start and pos must be contiguous int32' % name)
+    B = pos.shape[0]
+    if start.dim() != 1 or pos.dim() != 1 or start.shape[0] != B + 1 or B != cache.table.shape[0]:
+        raise ValueError('%s: start (batch + 1,) and pos (batch,) for the cache\'s %d sequences' % (
+            name, cache.table.shape[0]))
+    return B
+
+
+def _heads(name, cache, x, dtype):
+    if x.dim() != 3 or x.shape[2] != cache.head_dim:
+        raise ValueError('%s: rows must be (n, heads, %d)' % (name, cache.head_dim))
+    if x.dtype != dtype:
+        raise TypeError('%s: %s rows for a cache with a %s tail' % (name, x.dtype, dtype))
+    if x.stride(2) != 1:
+        raise ValueError('%s: the innermost (head) dimension must be contiguous' % name)
+
+
+def paged_append(cache, k, v, start, pos, max_new, q=None, rotation=None, q_out=None):
+    """Puts new rows into the cache: sequence b's rows [start[b], start[b + 1]) of k and v (n, n_kv_head, head_dim) (any row
+    and head strides) go to positions pos[b], pos[b] + 1, .... `max_new` bounds the rows of one sequence. rotation = (cos, sin)
+    (rotation_table) turns the first dims of k, and of q (n, n_head, head_dim) into q_out (allocated here when not given).
+    Without a rotation q is returned as it is. A page is quantised when its last token arrives; afterwards a sequence may be
+    cut back to any length whose page is the last or last but one written."""
+    pool, tail, table = cache.pool, cache.tail, cache.table
+    dt = tail.dtype
+    _need_cuda('paged_append', k, v, start, pos, q)
+    B = _rows('paged_append', cache, start, pos)
+    _heads('paged_append', cache, k, dt)
+    _heads('paged_append', cache, v, dt)
+    n, H, dh = k.shape
+    if H != pool.shape[1] or v.shape != k.shape:
+        raise ValueError('paged_append: k and v must be (n, %d, %d)' % (pool.shape[1], dh))
+    cos = sin = None
+    rot = n_pos = 0
+    if rotation is not None:
+        cos, sin = rotation
+        if (cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.shape != sin.shape or cos.dim() != 2 or
+                not cos.is_contiguous() or not sin.is_contiguous()):
+            raise ValueError('paged_append: rotation must be two contiguous fp32 tables (positions, rot / 2)')
+        _need_cuda('paged_append', cos, sin)
+        n_pos, rot = cos.shape[0], 2 * cos.shape[1]
+    Hq = qr = qh = 0
+    qo = None
+    if q is not None:
+        _heads('paged_append', cache, q, dt)
+        if q.shape[0] != n:
+            raise ValueError('paged_append: q has %d rows, k %d' % (q.shape[0], n))
+        if rot:
+            Hq, qr, qh = q.shape[1], q.stride(0), q.stride(1)
+            if q_out is None:
+                q_out = torch.empty(n, Hq, dh, device=q.device, dtype=dt)
+            elif q_out.shape != q.shape or q_out.dtype != dt or not q_out.is_contiguous():
+                raise ValueError('paged_append: q_out must be contiguous, of q\'s shape and type')
+            qo = q_out
+        else:
+            q_out = q
+    _lib.call('ta_paged_append', pool.data_ptr(), tail.data_ptr(), table.data_ptr(), table.stride(0), pool.shape[0],
+              table.shape[1], cache.page, _DT[dt], B, H, dh, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0),
+              v.stride(1), n, start.data_ptr(), pos.data_ptr(), int(max_new), _p(cos), _p(sin), n_pos, rot,
+              q.data_ptr() if qo is not None else None, Hq, qr, qh, _p(qo), _stream(k))
+    return q_out
+
+
+def paged_attn_workspace(batch, n_head, n_kv_head, head_dim, max_new, device='cuda'):
+    """A zeroed workspace for paged_attn at these sizes: one per stream of calls, kept by the caller."""
+    n = _lib.load().ta_paged_attn_workspace(int(batch), int(n_head), int(n_kv_head), int(head_dim), int(max_new))
+    return torch.zeros(max(int(n), 16), device=device, dtype=torch.uint8)
+
+
+def paged_attn(cache, q, start, pos, max_new, scale=None, window=0, out=None, lse=None, ws=None):
+    """Attention of new rows q (n, n_head, head_dim) over the cache, after paged_append has put the same rows into it: query
+    i of sequence b sees the positions up to pos[b] + i (its last `window` ones when window > 0). n_head is a multiple of the
+    cache's kv heads. Returns out (n, n_head, head_dim) in q's type; rows of no sequence are left as they are. lse (n, n_head)
+    fp32, when given, receives the natural logarithm of each row's sum of exponentials. ws: a workspace of
+    paged_attn_workspace that the caller keeps (allocated for the call when not given)."""
+    pool, tail, table = cache.pool, cache.tail, cache.table
+    dt = tail.dtype
+    _need_cuda('paged_attn', q, start, pos)
+    B = _rows('paged_attn', cache, start, pos)
+    _heads('paged_attn', cache, q, dt)
+    n, Hq, dh = q.shape
+    H = pool.shape[1]
+    if out is None:
+        out = torch.empty(n, Hq, dh, device=q.device, dtype=dt)
+    else:
+        _heads('paged_attn', cache, out, dt)
+        if out.shape != q.shape:
+            raise ValueError('paged_attn: out must have q\'s shape')
+    if lse is not None and (lse.shape != (n, Hq) or lse.dtype != torch.float32 or not lse.is_contiguous()):
+        raise ValueError('paged_attn: lse must be (n, n_head) fp32, contiguous')
+    if ws is None:
+        ws = paged_attn_workspace(B, Hq, H, dh, max_new, q.device)
+    _lib.call('ta_paged_attn', pool.data_ptr(), tail.data_ptr(), table.data_ptr(), table.stride(0), pool.shape[0],
+              table.shape[1], cache.page, _DT[dt], B, Hq, H, dh, q.data_ptr(), q.stride(0), q.stride(1), n, start.data_ptr(),
+              pos.data_ptr(), int(max_new), 1.0 / math.sqrt(dh) if scale is None else float(scale), int(window),
+              out.data_ptr(), out.stride(0), out.stride(1), _p(lse), ws.data_ptr(), ws.numel(), _stream(q))
+    return out
+
+
+def verify_drafts(p, q, drafts, u, n_draft=None):
+    """Which drafted tokens stand, and the token that follows them. p (B, G + 1, V) the target's probabilities after each
+    prefix, q (B, G, V) those the drafts were drawn from (fp32, bf16 or f16; any outer strides), drafts (B, G) int64, u
+    (B, G + 1) fp32 uniform in [0, 1) (one for each draft, the last for the draw), n_draft (B,) int32 the drafts of each sequence (all G when None). Returns tokens
+    (B, G + 1) int64 - the drafts that stand, the token drawn after them, then -1 - and accepted (B,) int32. The output is
+    distributed as sampling from p, whatever q is."""
+    _need_cuda('verify_drafts', p, q, drafts, u, n_draft)
+    if p.dim() != 3 or q.dim() != 3 or q.shape != (p.shape[0], p.shape[1] - 1, p.shape[2]):
+        raise ValueError('verify_drafts: p (B, G + 1, V) and q (B, G, V)')
+    B, G, V = q.shape
+    if p.dtype != q.dtype or p.dtype not in _DT:
+        raise TypeError('verify_drafts: p and q must share float32, bfloat16 or float16')
+    if p.stride(2) != 1 or (G and q.stride(2) != 1):
+        raise ValueError('verify_drafts: the innermost (vocabulary) dimension must be contiguous')
+    if drafts.shape != (B, G) or drafts.dtype != torch.int64 or not drafts.is_contiguous():
+        raise ValueError('verify_drafts: drafts must be (B, G) int64, contiguous')
+    if u.shape != (B, G + 1) or u.dtype != torch.float32 or not u.is_contiguous():
+        raise ValueError('verify_drafts: u must be (B, G + 1) fp32, contiguous')
+    if n_draft is not None and (n_draft.shape != (B,) or n_draft.dtype != torch.int32 or not n_draft.is_contiguous()):
+        raise ValueError('verify_drafts: n_draft must be (B,) int32, contiguous')
+    tokens = torch.empty(B, G + 1, device=p.device, dtype=torch.int64)
+    accepted = torch.empty(B, device=p.device, dtype=torch.int32)
+    _lib.call('ta_verify_drafts', p.data_ptr(), p.stride(0), p.stride(1), q.data_ptr(), q.stride(0), q.stride(1),
+              _DT[p.dtype], B, G, V, drafts.data_ptr(), u.data_ptr(), _p(n_draft), tokens.data_ptr(), accepted.data_ptr(),
+              _stream(p))
+    return tokens, accepted
