@@ -63,6 +63,24 @@ inline int current_device() {
   return dev;
 }
 
+// SMs of the current device (148 where there is none to ask).
+inline int sm_count() {
+  static std::atomic<int> have[kDevCache];
+  const int dev = current_device();
+  const bool cached = dev >= 0 && dev < kDevCache;
+  if (cached) {
+    const int n = have[dev].load(std::memory_order_relaxed);
+    if (n > 0) return n;
+  }
+  int n = 0;
+  if (dev < 0 || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) {
+    cudaGetLastError();
+    return 148;
+  }
+  if (cached) have[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
+
 // The dynamic shared-memory size a call site has allowed for its kernel, per device (0 = not yet).
 struct SmemAttr {
   std::atomic<size_t> bytes[kDevCache];

@@ -71,9 +71,55 @@ int run_attn_nt(const ta::AttnParams& p, cudaStream_t st) {
   return check_launch("ta_paged_attn");
 }
 
+// The split form: counters (one per item, 256-byte aligned end), then two states for every warp of the grid.
+int64_t counter_bytes(int64_t B, int64_t Hkv) { return (B * Hkv * 4 + 255) / 256 * 256; }
+
+template <int DH, int NT>
+int64_t split_bytes(int64_t B, int64_t Hkv) {
+  using SH = ta::SplitShape<DH, NT>;
+  return counter_bytes(B, Hkv) + (int64_t)sm_count() * SH::WARPS * 2 * SH::STATE * 4;
+}
+
+template <int DH>
+int64_t split_bytes_dh(int64_t B, int64_t Hkv, int64_t rows) {
+  if (rows <= 8) return split_bytes<DH, 1>(B, Hkv);
+  if (rows <= 16) return split_bytes<DH, 2>(B, Hkv);
+  if (rows <= 24) return split_bytes<DH, 3>(B, Hkv);
+  return split_bytes<DH, 4>(B, Hkv);
+}
+
+constexpr int kSplitRows = 32;  // rows of one (sequence, kv head) up to which the cache's bytes bound the call
+
+bool split_takes(int64_t B, int64_t Hkv, int64_t rows, int64_t max_pages, int P) {
+  return rows <= kSplitRows && B <= ta::SPLIT_MAX_BATCH && B * Hkv * (max_pages * P / 64 + 4) <= INT_MAX;
+}
+
+template <typename T, int DH, int NT>
+int run_split(const ta::AttnParams& p, void* ws, int64_t ws_bytes, cudaStream_t st) {
+  using SH = ta::SplitShape<DH, NT>;
+  const int64_t need = split_bytes<DH, NT>(p.B, p.c.Hkv);
+  if (!ws || !aligned16(ws) || ws_bytes < need)
+    return fail(TA_ERR_ARG, "ta_paged_attn: a workspace of %lld bytes is needed (16-byte aligned; got %lld)", (long long)need,
+                (long long)ws_bytes);
+  static SmemAttr attr;
+  const int smem = SH::RING + SH::BAR_BYTES + 12 * (p.B + 1);
+  if (int r = allow_smem(attr, ta::paged_split_kernel<T, DH, NT>, smem, "ta_paged_attn")) return r;
+  float* states = reinterpret_cast<float*>(reinterpret_cast<char*>(ws) + counter_bytes(p.B, p.c.Hkv));
+  const cudaError_t e = launch_pdl(ta::paged_split_kernel<T, DH, NT>, dim3(sm_count()), dim3(SH::WARPS * 32), smem, st, p,
+                                   reinterpret_cast<int32_t*>(ws), states);
+  if (e != cudaSuccess) return fail(TA_ERR_CUDA, "ta_paged_attn: launch failed: %s", cudaGetErrorString(e));
+  return TA_OK;
+}
+
 template <typename T, int DH>
-int run_attn(const ta::AttnParams& p, cudaStream_t st) {
+int run_attn(const ta::AttnParams& p, void* ws, int64_t ws_bytes, cudaStream_t st) {
   const int64_t rows = (int64_t)p.max_new * (p.Hq / p.c.Hkv);
+  if (split_takes(p.B, p.c.Hkv, rows, p.c.max_pages, p.c.P)) {
+    if (rows <= 8) return run_split<T, DH, 1>(p, ws, ws_bytes, st);
+    if (rows <= 16) return run_split<T, DH, 2>(p, ws, ws_bytes, st);
+    if (rows <= 24) return run_split<T, DH, 3>(p, ws, ws_bytes, st);
+    return run_split<T, DH, 4>(p, ws, ws_bytes, st);
+  }
   if (rows <= 8) return run_attn_nt<T, DH, 1>(p, st);
   if (rows <= 16 || DH == 128) return run_attn_nt<T, DH, 2>(p, st);  // 32 rows of head dim 128 do not fit the registers
   return run_attn_nt<T, DH, DH == 128 ? 2 : 4>(p, st);
@@ -120,8 +166,15 @@ int ta_paged_append(void* pool, void* tail, const int32_t* table, int64_t table_
 }
 
 int64_t ta_paged_attn_workspace(int B, int Hq, int Hkv, int dh, int max_new) {
-  (void)B; (void)Hq; (void)Hkv; (void)dh; (void)max_new;
-  return 0;
+  if (B < 1 || Hkv < 1 || Hq < Hkv || max_new < 1 || !valid_dh(dh)) return 0;
+  const int64_t rows = (int64_t)max_new * (Hq / Hkv);
+  if (rows > kSplitRows) return 0;
+  switch (dh) {
+    case 16: return split_bytes_dh<16>(B, Hkv, rows);
+    case 32: return split_bytes_dh<32>(B, Hkv, rows);
+    case 64: return split_bytes_dh<64>(B, Hkv, rows);
+    default: return split_bytes_dh<128>(B, Hkv, rows);
+  }
 }
 
 int ta_paged_attn(const void* pool, const void* tail, const int32_t* table, int64_t table_sb, int n_pages, int max_pages,
@@ -147,14 +200,13 @@ int ta_paged_attn(const void* pool, const void* tail, const int32_t* table, int6
   p.B = B; p.n_rows = n_rows; p.max_new = max_new; p.Hq = Hq;
   p.scale = scale; p.window = window;
   p.out = out; p.o_sr = o_sr; p.o_sh = o_sh; p.lse = lse;
-  (void)ws; (void)ws_bytes;
   const cudaStream_t st = S(stream);
 #define TA_ATTN(T)                                                              \
   switch (dh) {                                                                 \
-    case 16: return run_attn<T, 16>(p, st);                                     \
-    case 32: return run_attn<T, 32>(p, st);                                     \
-    case 64: return run_attn<T, 64>(p, st);                                     \
-    default: return run_attn<T, 128>(p, st);                                    \
+    case 16: return run_attn<T, 16>(p, ws, ws_bytes, st);                                   \
+    case 32: return run_attn<T, 32>(p, ws, ws_bytes, st);                                   \
+    case 64: return run_attn<T, 64>(p, ws, ws_bytes, st);                                   \
+    default: return run_attn<T, 128>(p, ws, ws_bytes, st);                                  \
   }
   if (dtype == TA_BF16) { TA_ATTN(__nv_bfloat16) } else { TA_ATTN(__half) }
 #undef TA_ATTN

@@ -336,6 +336,11 @@ __device__ __forceinline__ uint32_t codes_f16x2(uint32_t two) {
   asm("{\n\t.reg .b16 c;\n\tcvt.u16.u32 c, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, c;\n\t}" : "=r"(r) : "r"(two));
   return r;
 }
+__device__ __forceinline__ float exp2_fast(float x) {  // results below 2^-126 are 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b);
 template <>
@@ -469,7 +474,7 @@ __device__ __forceinline__ void soft_step(const RowTile<T, DH, NT>& rt, SoftStat
       top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 8));
       top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 16));
       const float mn = fmaxf(st.m[nt][i], top[i]);
-      fac[i] = mn == st.m[nt][i] ? 1.f : exp2f(st.m[nt][i] - mn);
+      fac[i] = mn == st.m[nt][i] ? 1.f : exp2_fast(st.m[nt][i] - mn);
       moved |= mn != st.m[nt][i];
       st.m[nt][i] = mn;
       ref[i] = mn == -INFINITY ? 0.f : mn - ATTN_SHIFT;
@@ -489,7 +494,7 @@ __device__ __forceinline__ void soft_step(const RowTile<T, DH, NT>& rt, SoftStat
       for (int i = 0; i < 4; ++i) {
         // a masked token weighs 0 whatever its page holds
         const float v = s[x][nt][i];
-        s[x][nt][i] = v == -INFINITY ? 0.f : exp2f(v - ref[i & 1]);
+        s[x][nt][i] = v == -INFINITY ? 0.f : exp2_fast(v - ref[i & 1]);
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -554,26 +559,26 @@ __device__ __forceinline__ void attend_codes(const RowTile<T, DH, NT>& rt, SoftS
     }
 }
 
+// A query fragment in the tail's type: the power of two keeps bf16 rows exact as well.
+template <typename T>
+__device__ __forceinline__ uint32_t as_type(uint32_t f16x2) {
+  if constexpr (std::is_same<T, __half>::value) return f16x2;
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&f16x2));
+  return pack2<T>(f.x, f.y);
+}
+
 // One 16-token group of the open page, 16-bit elements in the same order. len: tokens the sequence holds; later slots
 // of the page hold anything and are masked in the scores and zeroed in the values.
 template <typename T, int DH, int NT>
-__device__ __forceinline__ void attend_tail(const AttnParams& p, const NewRows& nr, int h, int group, int row0, int R,
-                                            const RowTile<T, DH, NT>& rt, SoftState<DH, NT>& st, const T* kp, const T* vp,
-                                            int tok0, int len) {
+__device__ __forceinline__ void attend_tail(const RowTile<T, DH, NT>& rt, SoftState<DH, NT>& st, const T* kp, const T* vp,
+                                            int tok0, int len, int window) {
   using S = PageShape<DH>;
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int lane = threadIdx.x & 31, t = lane & 3;
   float s[1][NT][4];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int i = 0; i < 4; ++i) s[0][nt][i] = 0.f;
-  const T* qr[NT];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int rr = min(row0 + nt * 8 + g, R - 1);
-    qr[nt] = reinterpret_cast<const T*>(p.q) + (int64_t)(nr.row0 + rr / group) * p.q_sr +
-             (int64_t)(h * group + rr % group) * p.q_sh;
-  }
 #pragma unroll
   for (int hg = 0; hg < S::HG; ++hg)
 #pragma unroll
@@ -583,23 +588,11 @@ __device__ __forceinline__ void attend_tail(const AttnParams& p, const NewRows& 
       load_words<8>(kp + ((hg * 2 + 1) * 32 + lane) * S::E + e * 4, w1);
       const uint32_t a[4] = {w0[0], w1[0], w0[1], w1[1]};
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        uint32_t q[2];
-        load_words<8>(qr[nt] + hg * 4 * S::E + t * S::E + e * 4, q);
-        mma_16<T>(s[0][nt], a, q[0], q[1]);
-      }
-    }
-  // unscaled rows: the score factor without the f16 rows' power of two
-  RowTile<T, DH, NT> plain;
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      plain.cs[nt][i] = p.scale * 1.4426950408889634f;
-      plain.qpos[nt][i] = rt.qpos[nt][i];
+      for (int nt = 0; nt < NT; ++nt)
+        mma_16<T>(s[0][nt], a, as_type<T>(rt.qf[hg * (S::E / 4) + e][nt][0]), as_type<T>(rt.qf[hg * (S::E / 4) + e][nt][1]));
     }
   const float one[1] = {1.f}, zero[1] = {0.f};
-  soft_step<T, DH, NT, 1>(plain, st, s, one, zero, one, tok0, len, p.window, true);
+  soft_step<T, DH, NT, 1>(rt, st, s, one, zero, one, tok0, len, window, true);
   uint32_t pf[NT][2];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
@@ -682,8 +675,8 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32) paged_attn_kernel(AttnParams 
     const T* tk = reinterpret_cast<const T*>(p.c.tail) +
                   ((((int64_t)b * p.c.Hkv + h) * 2 + (n_full & 1)) * 2) * ((int64_t)P * DH);
     for (int x = warp; n_full * P + x * 16 <= qhi; x += ATTN_WARPS)
-      attend_tail<T, DH, NT>(p, nr, h, group, row0, R, rt, st, tk + x * 16 * DH, tk + (int64_t)P * DH + x * 16 * DH,
-                             n_full * P + x * 16, len);
+      attend_tail<T, DH, NT>(rt, st, tk + x * 16 * DH, tk + (int64_t)P * DH + x * 16 * DH, n_full * P + x * 16, len,
+                             p.window);
   }
   // join the warps
 #pragma unroll
@@ -726,6 +719,349 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32) paged_attn_kernel(AttnParams 
     if (p.lse && d == 0)
       p.lse[row * p.Hq + hq] = L == 0.f ? -INFINITY : (m - ATTN_SHIFT + log2f(L)) * 0.69314718055994531f;
   }
+}
+
+// ------------------------------------------------------------------------------------------------ attention, few rows
+// At most 32 rows per (sequence, kv head): the cache's bytes bound it. An item is a (sequence, kv head); its units are
+// runs of 64 tokens of full pages, then of 32 tokens of the open page. The units of all items, in order, are shared out
+// evenly over the warps of one resident grid, whatever the lengths are: a warp takes a run of units that may end one item and
+// begin another. Each warp keeps its own ring of units in shared memory, filled by bulk copies (a record of a full page is
+// one copy, scales included), so the only waits are for its own copies.
+// An item that one warp holds whole is written out at once; of the others each warp leaves its state (maximum, sum,
+// numerator) in the workspace, and the warp that comes last (a counter per item) joins them in order. The counters are left
+// at zero.
+template <int DH, int NT>
+struct SplitShape {
+  // A unit's bytes bound the number of rings: two units ahead of the one at work, for as many warps as fit
+  static constexpr int STAGE = 128 * DH + 64;
+  static constexpr int NS = 3;
+  static constexpr int WARPS = DH == 128 ? 4 : 8;
+  static constexpr int STATE = 8 * NT * DH + 16 * NT;  // floats: numerator fragments, then (maximum, sum) per row
+  static constexpr int BAR_BYTES = WARPS * NS * 8;
+  static constexpr int RING = WARPS * NS * STAGE;
+};
+
+constexpr int SPLIT_MIN_UNITS = 4;   // units per warp while warps are plenty: below, joining costs more than it spreads
+constexpr int SPLIT_MAX_BATCH = 2048;  // sequences whose geometry is kept in shared memory (12 bytes each)
+
+// The units of one item.
+struct Item {
+  int pos, n, row0;
+  int len, p0, p1;    // tokens held; full pages [p0, p1)
+  int nu8, units;
+};
+__device__ __forceinline__ Item item_of(int row0, int n, int pos, int P, int window) {
+  Item it;
+  it.row0 = row0;
+  it.n = n;
+  it.pos = pos;
+  it.len = pos + n;
+  it.p1 = it.len / P;
+  it.p0 = window > 0 ? max(0, pos - window + 1) / P : 0;
+  const int per = 64 / P;
+  it.nu8 = (it.p1 - it.p0 + per - 1) / per;
+  it.units = n > 0 ? it.nu8 + (it.len - it.p1 * P + 31) / 32 : 0;
+  return it;
+}
+
+template <typename T, int DH, int NT>
+__global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
+    paged_split_kernel(AttnParams p, int32_t* counters, float* states) {
+  using SH = SplitShape<DH, NT>;
+  constexpr int WARPS = SH::WARPS, NS = SH::NS, ROWS = 8 * NT;
+  constexpr int TG = NT >= 3 ? 2 : 4;  // a whole unit's scores beside 24 or 32 rows' numerators do not fit the registers
+  extern __shared__ __align__(128) unsigned char split_smem[];
+  __shared__ int warp_sums[WARPS];
+  unsigned char* ring = split_smem;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(split_smem + SH::RING);
+  int* s_first = reinterpret_cast<int*>(split_smem + SH::RING + SH::BAR_BYTES);  // first unit of sequence b (B + 1)
+  int* s_row = s_first + p.B + 1;
+  int* s_pos = s_row + p.B + 1;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int P = p.c.P, Hkv = p.c.Hkv, group = p.Hq / Hkv, per = 64 / P;
+  const int rec = 2 * P * DH + 16;
+  uint64_t* bar = bars + warp * NS;
+  if (lane == 0) {
+    for (int i = 0; i < NS; ++i) mbar_init(bar + i, 1);
+    fence_mbar_init();
+  }
+  pdl_wait();
+  pdl_launch_dependents();
+  // where each sequence's units begin
+  {
+    const int chunk = (p.B + WARPS * 32 - 1) / (WARPS * 32);
+    const int b0 = min(p.B, tid * chunk), b1 = min(p.B, b0 + chunk);
+    int sum = 0;
+    for (int b = b0; b < b1; ++b) {
+      const int r0 = p.start[b], n = p.start[b + 1] - r0, ps = p.pos[b];
+      int units = 0;
+      if (r0 < 0 || n < 0 || r0 + n > p.n_rows || n > p.max_new)
+        record_error(DEV_INDEX_RANGE, K_PAGED_ATTN, b, n);
+      else if (ps < 0 || (int64_t)ps + n > (int64_t)p.c.max_pages * P + (P - 1))
+        record_error(DEV_POS_RANGE, K_PAGED_ATTN, b, ps);
+      else
+        units = item_of(r0, n, ps, P, p.window).units * Hkv;
+      s_first[b + 1] = units;
+      s_row[b] = r0;
+      s_pos[b] = ps;
+      if (b == p.B - 1) s_row[b + 1] = r0 + n;
+      sum += units;
+    }
+    int inc = sum;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += y;
+    }
+    if (lane == 31) warp_sums[warp] = inc;
+    __syncthreads();
+    int at = inc - sum;
+    for (int w = 0; w < warp; ++w) at += warp_sums[w];
+    for (int b = b0; b < b1; ++b) {
+      at += s_first[b + 1];
+      s_first[b + 1] = at;
+    }
+    if (tid == 0) s_first[0] = 0;
+    __syncthreads();
+  }
+  const int total = s_first[p.B];
+  if (total == 0) return;
+  const int n_work = min((int)gridDim.x * WARPS, (total + SPLIT_MIN_UNITS - 1) / SPLIT_MIN_UNITS);
+  const int me = warp * gridDim.x + blockIdx.x;
+  if (me >= n_work) return;
+  auto first_of = [&](int w) { return (int)((int64_t)total * w / n_work); };
+  auto owner_of = [&](int u) { return (int)((((int64_t)u + 1) * n_work - 1) / total); };
+  const int u0 = first_of(me), u1 = first_of(me + 1);
+  const int32_t* table = p.c.table;
+
+  // A run of units of one item: [k, end) of it.
+  struct Run {
+    Item it;
+    int b, h, k, end, u_item;
+  };
+  auto open = [&](Run& r, int u) {
+    int lo = 0, hi = p.B - 1;
+    while (lo < hi) {  // the last sequence that begins at or before u and has units
+      const int mid = (lo + hi + 1) / 2;
+      if (s_first[mid] <= u) lo = mid;
+      else hi = mid - 1;
+    }
+    r.b = lo;
+    r.it = item_of(s_row[lo], s_row[lo + 1] - s_row[lo], s_pos[lo], P, p.window);
+    const int in = u - s_first[lo];
+    r.h = in / r.it.units;
+    r.k = in % r.it.units;
+    r.u_item = u - r.k;
+    r.end = min(r.it.units, r.k + (u1 - u));
+  };
+
+  // ---- copies: `ahead` runs NS units before the one at work
+  Run ahead{};
+  int au = u0;          // its unit
+  int batch = 0;        // page of the item that lane 0's table entry stands for
+  int entry = 0, entry_next = 0;
+  auto load_entry = [&](int page) {
+    return page < ahead.it.p1 ? table[ahead.b * p.c.table_sb + page] : 0;
+  };
+  auto begin_ahead = [&]() {
+    open(ahead, au);
+    batch = ahead.it.p0 + ahead.k * per;
+    entry = load_entry(batch + lane);
+    entry_next = load_entry(batch + 32 + lane);
+  };
+  auto issue = [&](int slot) {
+    unsigned char* dst = ring + (warp * NS + slot) * SH::STAGE;
+    if (ahead.k < ahead.it.nu8) {
+      const int page = ahead.it.p0 + ahead.k * per;
+      if (page >= batch + 32) {
+        batch += 32;
+        entry = entry_next;
+        entry_next = load_entry(batch + 32 + lane);
+      }
+      // a unit's pages beyond the last full one are copies of it (masked, but finite)
+      const int at = min(page + (lane < per ? lane : 0), ahead.it.p1 - 1) - batch;
+      int phys = __shfl_sync(0xffffffffu, entry, at);
+      if (phys < 0 || phys >= p.c.n_pages) {
+        record_error(DEV_INDEX_RANGE, K_PAGED_ATTN, ahead.b, phys);
+        phys = 0;
+      }
+      if (lane == 0) mbar_arrive_expect_tx(bar + slot, (uint32_t)(per * rec));
+      __syncwarp();
+      if (lane < per)
+        bulk_g2s(dst + lane * rec, p.c.pool + ((int64_t)phys * Hkv + ahead.h) * rec, (uint32_t)rec, bar + slot);
+    } else if (lane == 0) {
+      const int t0 = (ahead.k - ahead.it.nu8) * 32;  // token of the open page
+      const int left = ahead.it.len - ahead.it.p1 * P - t0;
+      const uint32_t bytes = (uint32_t)(left > 16 ? 2 : 1) * 16 * DH * 2;
+      const T* src = reinterpret_cast<const T*>(p.c.tail) +
+                     ((((int64_t)ahead.b * Hkv + ahead.h) * 2 + (ahead.it.p1 & 1)) * 2) * ((int64_t)P * DH) + t0 * DH;
+      mbar_arrive_expect_tx(bar + slot, 2 * bytes);
+      bulk_g2s(dst, src, bytes, bar + slot);
+      bulk_g2s(dst + 64 * DH, src + (int64_t)P * DH, bytes, bar + slot);
+    }
+    __syncwarp();
+    ++au;
+    if (++ahead.k == ahead.end && au < u1) begin_ahead();
+  };
+
+  begin_ahead();
+  for (int i = 0; i < NS; ++i)
+    if (au < u1) issue(i);
+
+  RowTile<T, DH, NT> rt;
+  SoftState<DH, NT> st;
+  Run run;
+  bool ok = true;
+  int u = u0, step = 0;  // step: units consumed
+  while (u < u1) {
+    open(run, u);
+    const Item& it = run.it;
+    const int R = it.n * group;
+    NewRows nr;
+    nr.row0 = it.row0;
+    nr.n = it.n;
+    nr.pos = it.pos;
+    rt.load(p, nr, run.h, group, 0, R);
+    st.clear();
+    const int qhi = it.pos + it.n - 1;
+    for (int k = run.k; k < run.end; ++k, ++u, ++step) {
+      const int slot = step % NS;
+      const unsigned char* src = ring + (warp * NS + slot) * SH::STAGE;
+      if (!mbar_wait_bounded(bar + slot, (step / NS) & 1, K_PAGED_ATTN, 1)) {
+        ok = false;
+        break;
+      }
+      if (k < it.nu8) {
+        const int tok0 = (it.p0 + k * per) * P, limit = it.p1 * P;
+        const bool mask = tok0 + 63 > min(it.pos, limit - 1) || (p.window > 0 && tok0 <= qhi - p.window);
+#pragma unroll 1
+        for (int y = 0; y < 4; y += TG) {  // 16-token groups at a time
+          const unsigned char *kp[TG], *vp[TG];
+          float ks[TG], lv[TG], iv[TG];
+#pragma unroll
+          for (int x = 0; x < TG; ++x) {
+            const unsigned char* rp = src + ((y + x) * 16 / P) * rec;
+            kp[x] = rp + ((y + x) * 16 % P) * DH;
+            vp[x] = kp[x] + P * DH;
+            const float2 sc = *reinterpret_cast<const float2*>(rp + 2 * P * DH);
+            ks[x] = sc.x;
+            lv[x] = log2f(sc.y);
+            iv[x] = 1.f / sc.y;
+          }
+          attend_codes<T, DH, NT, TG>(rt, st, kp, vp, ks, lv, iv, tok0 + y * 16, limit, p.window, mask);
+        }
+      } else {
+        const T* tk = reinterpret_cast<const T*>(src);
+        const T* tv = reinterpret_cast<const T*>(src + 64 * DH);
+        const int tok0 = it.p1 * P + (k - it.nu8) * 32;
+        for (int x = 0; x < 2 && tok0 + x * 16 < it.len; ++x)
+          attend_tail<T, DH, NT>(rt, st, tk + x * 16 * DH, tv + x * 16 * DH, tok0 + x * 16, it.len, p.window);
+      }
+      __syncwarp();  // every lane has read the unit
+      if (au < u1) issue(slot);
+    }
+    if (!ok) break;
+    // ---- the run's end: out, or into the workspace
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float& l = st.l[nt][i];
+        l += __shfl_xor_sync(0xffffffffu, l, 4);
+        l += __shfl_xor_sync(0xffffffffu, l, 8);
+        l += __shfl_xor_sync(0xffffffffu, l, 16);
+      }
+    bool write = run.k == 0 && run.end == it.units;
+    if (!write) {
+      float* mine = states + ((int64_t)me * 2 + (run.u_item + run.k == u0 ? 0 : 1)) * SH::STATE;
+#pragma unroll
+      for (int x = 0; x < DH / 16; ++x)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          __stcg(reinterpret_cast<float4*>(mine) + (x * NT + nt) * 32 + lane,
+                 make_float4(st.o[x][nt][0], st.o[x][nt][1], st.o[x][nt][2], st.o[x][nt][3]));
+      if (g == 0) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          __stcg(reinterpret_cast<float4*>(mine + ROWS * DH) + nt * 4 + t,
+                 make_float4(st.m[nt][0], st.m[nt][1], st.l[nt][0], st.l[nt][1]));
+      }
+      __threadfence();
+      __syncwarp();
+      const int wa = owner_of(run.u_item), wb = owner_of(run.u_item + it.units - 1);
+      int32_t* cnt = counters + run.b * Hkv + run.h;
+      int before = 0;
+      if (lane == 0) before = atomicAdd(cnt, 1);
+      before = __shfl_sync(0xffffffffu, before, 0);
+      write = before == wb - wa;
+      if (write) {
+        __threadfence();
+        if (lane == 0) *cnt = 0;
+        // the item's states in order: the first one is its warp's second unless that warp begins with the item
+        auto state_of = [&](int w) {
+          return states + ((int64_t)w * 2 + (w == wa && first_of(wa) < run.u_item ? 1 : 0)) * SH::STATE;
+        };
+        float top[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) top[nt][0] = top[nt][1] = -INFINITY;
+        for (int w = wa; w <= wb; ++w) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const float4 ml = __ldcg(reinterpret_cast<const float4*>(state_of(w) + ROWS * DH) + nt * 4 + t);
+            top[nt][0] = fmaxf(top[nt][0], ml.x);
+            top[nt][1] = fmaxf(top[nt][1], ml.y);
+          }
+        }
+        st.clear();
+#pragma unroll 2
+        for (int w = wa; w <= wb; ++w) {
+          const float* s = state_of(w);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const float4 ml = __ldcg(reinterpret_cast<const float4*>(s + ROWS * DH) + nt * 4 + t);
+            const float f0 = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - top[nt][0]);
+            const float f1 = ml.y == -INFINITY ? 0.f : exp2_fast(ml.y - top[nt][1]);
+            st.l[nt][0] += ml.z * f0;
+            st.l[nt][1] += ml.w * f1;
+#pragma unroll
+            for (int x = 0; x < DH / 16; ++x) {
+              const float4 o = __ldcg(reinterpret_cast<const float4*>(s) + (x * NT + nt) * 32 + lane);
+              st.o[x][nt][0] += o.x * f0;
+              st.o[x][nt][1] += o.y * f1;
+              st.o[x][nt][2] += o.z * f0;
+              st.o[x][nt][3] += o.w * f1;
+            }
+          }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          st.m[nt][0] = top[nt][0];
+          st.m[nt][1] = top[nt][1];
+        }
+      }
+    }
+    if (write) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int rr = nt * 8 + 2 * t + i;
+          if (rr >= R) continue;
+          const float l = st.l[nt][i], inv = l == 0.f ? 0.f : 1.f / l;
+          const int64_t row = it.row0 + rr / group;
+          const int hq = run.h * group + rr % group;
+          T* o = reinterpret_cast<T*>(p.out) + row * p.o_sr + (int64_t)hq * p.o_sh;
+#pragma unroll
+          for (int x = 0; x < DH / 16; ++x) {
+            o[x * 16 + g] = from_f32<T>(l == 0.f ? 0.f : st.o[x][nt][i] * inv);
+            o[x * 16 + 8 + g] = from_f32<T>(l == 0.f ? 0.f : st.o[x][nt][i + 2] * inv);
+          }
+          if (p.lse && g == 0)
+            p.lse[row * p.Hq + hq] = l == 0.f ? -INFINITY : (st.m[nt][i] - ATTN_SHIFT + log2f(l)) * 0.69314718055994531f;
+        }
+    }
+  }
+  if (!ok)  // no copy of this warp may still be in flight when its CTA ends
+    for (int i = step + 1; i < step + NS && u0 + i < au; ++i) mbar_wait_bounded(bar + i % NS, (i / NS) & 1, K_PAGED_ATTN, 2);
 }
 
 }  // namespace ta
