@@ -91,7 +91,7 @@ int64_t split_bytes_dh(int64_t B, int64_t Hkv, int64_t rows) {
 constexpr int kSplitRows = 32;  // rows of one (sequence, kv head) up to which the cache's bytes bound the call
 
 bool split_takes(int64_t B, int64_t Hkv, int64_t rows, int64_t max_pages, int P) {
-  return rows <= kSplitRows && B <= ta::SPLIT_MAX_BATCH && B * Hkv * (max_pages * P / 64 + 4) <= INT_MAX;
+  return rows <= kSplitRows && B <= ta::SPLIT_MAX_BATCH && B * Hkv * (max_pages * P / 32 + 5) <= INT_MAX;
 }
 
 template <typename T, int DH, int NT>
@@ -123,6 +123,23 @@ int run_attn(const ta::AttnParams& p, void* ws, int64_t ws_bytes, cudaStream_t s
   if (rows <= 8) return run_attn_nt<T, DH, 1>(p, st);
   if (rows <= 16 || DH == 128) return run_attn_nt<T, DH, 2>(p, st);  // 32 rows of head dim 128 do not fit the registers
   return run_attn_nt<T, DH, DH == 128 ? 2 : 4>(p, st);
+}
+
+// Clusters of cs CTAs, one per sequence, with programmatic dependent launch.
+cudaError_t launch_verify(void (*kern)(ta::VerifyParams), int cs, cudaStream_t st, const ta::VerifyParams& a) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(a.B * cs));
+  cfg.blockDim = dim3(ta::VERIFY_THREADS);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cs;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, kern, a);
 }
 
 }  // namespace
@@ -218,18 +235,25 @@ int ta_verify_drafts(const void* p, int64_t p_sb, int64_t p_sr, const void* q, i
   g_err.clear();
   const char* who = "ta_verify_drafts";
   if (!valid_dtype(dtype)) return fail(TA_ERR_ARG, "%s: bad dtype %d", who, dtype);
-  if (B < 0 || G < 0 || G > 1024 || V < 1 || V > (1 << 24))
+  if (B < 0 || B > INT_MAX / 8 || G < 0 || G > 1024 || V < 1 || V > (1 << 24))
     return fail(TA_ERR_ARG, "%s: bad sizes B=%d G=%d V=%d (at most 1024 drafts, 2^24 words)", who, B, G, V);
   if (B == 0) return TA_OK;
   if (!p || !u || !tokens || !accepted || (G && (!q || !drafts))) return fail(TA_ERR_ARG, "%s: null pointer", who);
-  ta::VerifyParams a{p, q, p_sb, p_sr, q_sb, q_sr, drafts, u, n, B, G, V, tokens, accepted};
+  ta::VerifyParams a{p, q, p_sb, p_sr, q_sb, q_sr, drafts, u, n, B, G, V, 0, tokens, accepted};
+  // CTAs of a sequence: more while the shares stay above 4096 words and all CTAs are resident together (4 an SM)
+  int cs = 1;
+  while (cs < ta::VERIFY_MAX_CLUSTER && V / (2 * cs) >= 4096 && (int64_t)B * 2 * cs <= 4 * (int64_t)sm_count()) cs *= 2;
+  const int step = 32 * 16 / esize_of(dtype), warps = cs * ta::VERIFY_WARPS;
+  a.seg = ((V + warps - 1) / warps + step - 1) / step * step;
   const cudaStream_t st = S(stream);
+  cudaError_t e;
   switch (dtype) {
-    case TA_F32: ta::verify_kernel<float><<<B, ta::VERIFY_THREADS, 0, st>>>(a); break;
-    case TA_BF16: ta::verify_kernel<__nv_bfloat16><<<B, ta::VERIFY_THREADS, 0, st>>>(a); break;
-    default: ta::verify_kernel<__half><<<B, ta::VERIFY_THREADS, 0, st>>>(a); break;
+    case TA_F32: e = launch_verify(ta::verify_kernel<float>, cs, st, a); break;
+    case TA_BF16: e = launch_verify(ta::verify_kernel<__nv_bfloat16>, cs, st, a); break;
+    default: e = launch_verify(ta::verify_kernel<__half>, cs, st, a); break;
   }
-  return check_launch(who);
+  if (e != cudaSuccess) return fail(TA_ERR_CUDA, "%s: launch failed: %s", who, cudaGetErrorString(e));
+  return TA_OK;
 }
 
 }  // extern "C"

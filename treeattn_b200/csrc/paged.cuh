@@ -330,11 +330,21 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-// two e4m3 codes -> f16x2
-__device__ __forceinline__ uint32_t codes_f16x2(uint32_t two) {
-  uint32_t r;
-  asm("{\n\t.reg .b16 c;\n\tcvt.u16.u32 c, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, c;\n\t}" : "=r"(r) : "r"(two));
-  return r;
+// four e4m3 codes -> two f16x2
+__device__ __forceinline__ void codes_f16x4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(w));
+}
+__device__ __forceinline__ float log2_fast(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 __device__ __forceinline__ float exp2_fast(float x) {  // results below 2^-126 are 0
   float y;
@@ -374,7 +384,7 @@ template <typename T, int DH, int NT>
 struct RowTile {
   using S = PageShape<DH>;
   uint32_t qf[DH / 16][NT][2];  // f16, scaled per row
-  float cs[NT][2];              // score factor of the row: scale * log2(e) / (its power of two)
+  float cs[NT][2];              // score factor of the row, positive: |scale| * log2(e) / (its power of two)
   int qpos[NT][2];              // position of the row's query; -1: no such row
 
   // row0: first row of the tile; R rows in all (n queries x group heads)
@@ -404,16 +414,15 @@ struct RowTile {
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       // 2^ex * top in [2^14, 2^15): exact, and what falls below f16's range is below 2^-39 of the row's largest element
-      int ex = 0;
-      if (top > 0.f && top <= 3.402823466e38f) ex = 14 - ilogbf(top);
-      ex = min(ex, 120);
-      const float up = exp2f((float)ex);
+      const int ex = min(14 + 127 - (int)(__float_as_uint(top) >> 23), 120);
+      // the sign of the scale joins the row; at scale 0 the row is 0
+      const float up = p.scale == 0.f ? 0.f : copysignf(__int_as_float((ex + 127) << 23), p.scale);
 #pragma unroll
       for (int kk = 0; kk < DH / 16; ++kk) {
         qf[kk][nt][0] = pack2<__half>(x[kk * 4] * up, x[kk * 4 + 1] * up);
         qf[kk][nt][1] = pack2<__half>(x[kk * 4 + 2] * up, x[kk * 4 + 3] * up);
       }
-      const float f = p.scale * 1.4426950408889634f * exp2f((float)-ex);
+      const float f = p.scale == 0.f ? 1.f : fabsf(p.scale) * 1.4426950408889634f * __int_as_float((127 - ex) << 23);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         cs[nt][i] = __shfl_sync(0xffffffffu, f, (2 * t + i) * 4);
@@ -442,32 +451,45 @@ struct SoftState {
   }
 };
 
-// Scores -> weights for TG 16-token groups: s holds the raw sums and leaves as the packed P^T fragments pf. ks / lv / iv: per
-// group the key scale, log2 of the value scale and its inverse. tok0: position of the first token; tokens from `limit` on
-// are not the unit's.
+// Scores -> weights for TG 16-token groups, in place: s holds the raw sums. ks / lv / iv: per group the key scale, log2 of the
+// value scale and its inverse. tok0: position of the first token; tokens from `limit` on are not the unit's. The factors
+// are positive, so that the maximum is taken over the raw sums.
 template <typename T, int DH, int NT, int TG>
 __device__ __forceinline__ void soft_step(const RowTile<T, DH, NT>& rt, SoftState<DH, NT>& st, float (&s)[TG][NT][4],
                                           const float (&ks)[TG], const float (&lv)[TG], const float (&iv)[TG], int tok0,
                                           int limit, int window, bool mask) {
   const int g = (threadIdx.x & 31) >> 2;
+  uint32_t gone[NT];  // masked elements, bit x * 4 + i
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) gone[nt] = 0u;
+  if (mask) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int last = min(rt.qpos[nt][i], limit - 1), first = window > 0 ? rt.qpos[nt][i] - window + 1 : 0;
+#pragma unroll
+        for (int x = 0; x < TG; ++x)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const int tok = tok0 + x * 16 + r * 8 + g;
+            if (tok > last || tok < first) {
+              s[x][nt][r * 2 + i] = -INFINITY;
+              gone[nt] |= 1u << (x * 4 + r * 2 + i);
+            }
+          }
+      }
+  }
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int x = 0; x < TG; ++x)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float v = fmaf(s[x][nt][i], ks[x] * rt.cs[nt][i & 1], lv[x]);
-        if (mask) {
-          const int tok = tok0 + x * 16 + (i >> 1) * 8 + g, qp = rt.qpos[nt][i & 1];
-          if (tok > qp || tok >= limit || (window > 0 && tok <= qp - window)) v = -INFINITY;
-        }
-        s[x][nt][i] = v;
-        top[i & 1] = fmaxf(top[i & 1], v);
-      }
-    float ref[2];
+      for (int i = 0; i < 2; ++i)
+        top[i] = fmaxf(top[i], fmaf(fmaxf(s[x][nt][i], s[x][nt][i + 2]), ks[x] * rt.cs[nt][i], lv[x]));
+    float ref[2], fac[2];
     bool moved = false;
-    float fac[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 4));
@@ -488,20 +510,24 @@ __device__ __forceinline__ void soft_step(const RowTile<T, DH, NT>& rt, SoftStat
         for (int i = 0; i < 4; ++i) st.o[x][nt][i] *= fac[i & 1];
     }
 #pragma unroll
-    for (int x = 0; x < TG; ++x) {
-      float sum[2];
+    for (int x = 0; x < TG; ++x)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        // a masked token weighs 0 whatever its page holds
-        const float v = s[x][nt][i];
-        s[x][nt][i] = v == -INFINITY ? 0.f : exp2_fast(v - ref[i & 1]);
-      }
+      for (int i = 0; i < 4; ++i)
+        s[x][nt][i] = exp2_fast(fmaf(s[x][nt][i], ks[x] * rt.cs[nt][i & 1], lv[x] - ref[i & 1]));
+    if (mask) {  // a masked token weighs 0 whatever its page's scales are
+#pragma unroll
+      for (int x = 0; x < TG; ++x)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (gone[nt] >> (x * 4 + i) & 1u) s[x][nt][i] = 0.f;
+    }
+#pragma unroll
+    for (int x = 0; x < TG; ++x)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        sum[i] = s[x][nt][i] + s[x][nt][i + 2];
-        st.l[nt][i] += sum[i] == 0.f ? 0.f : sum[i] * iv[x];
+        const float sum = s[x][nt][i] + s[x][nt][i + 2];
+        st.l[nt][i] += sum == 0.f ? 0.f : sum * iv[x];
       }
-    }
   }
 }
 
@@ -529,7 +555,9 @@ __device__ __forceinline__ void attend_codes(const RowTile<T, DH, NT>& rt, SoftS
       load_words<S::E>(kp[x] + ((hg * 2 + 1) * 32 + lane) * S::E, w1);
 #pragma unroll
       for (int e = 0; e < S::E / 4; ++e) {
-        const uint32_t a[4] = {codes_f16x2(w0[e]), codes_f16x2(w1[e]), codes_f16x2(w0[e] >> 16), codes_f16x2(w1[e] >> 16)};
+        uint32_t a[4];
+        codes_f16x4(w0[e], a[0], a[2]);
+        codes_f16x4(w1[e], a[1], a[3]);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) mma_f16(s[x][nt], a, rt.qf[hg * (S::E / 4) + e][nt][0], rt.qf[hg * (S::E / 4) + e][nt][1]);
       }
@@ -551,8 +579,9 @@ __device__ __forceinline__ void attend_codes(const RowTile<T, DH, NT>& rt, SoftS
       load_words<8 * S::M>(vp[x] + (c * 32 + lane) * 8 * S::M, w);
 #pragma unroll
       for (int m = 0; m < S::M; ++m) {
-        const uint32_t a[4] = {codes_f16x2(w[2 * m]), codes_f16x2(w[2 * m + 1]), codes_f16x2(w[2 * m] >> 16),
-                               codes_f16x2(w[2 * m + 1] >> 16)};
+        uint32_t a[4];
+        codes_f16x4(w[2 * m], a[0], a[2]);
+        codes_f16x4(w[2 * m + 1], a[1], a[3]);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) mma_f16(st.o[c * S::M + m][nt], a, pf[x][nt][0], pf[x][nt][1]);
       }
@@ -567,50 +596,68 @@ __device__ __forceinline__ uint32_t as_type(uint32_t f16x2) {
   return pack2<T>(f.x, f.y);
 }
 
-// One 16-token group of the open page, 16-bit elements in the same order. len: tokens the sequence holds; later slots
-// of the page hold anything and are masked in the scores and zeroed in the values.
-template <typename T, int DH, int NT>
+// TG 16-token groups of the open page, 16-bit elements in the same order. len: tokens the sequence holds; later slots of
+// the page hold anything and are masked in the scores and zeroed in the values.
+template <typename T, int DH, int NT, int TG>
 __device__ __forceinline__ void attend_tail(const RowTile<T, DH, NT>& rt, SoftState<DH, NT>& st, const T* kp, const T* vp,
                                             int tok0, int len, int window) {
   using S = PageShape<DH>;
   const int lane = threadIdx.x & 31, t = lane & 3;
-  float s[1][NT][4];
+  float s[TG][NT][4];
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
+  for (int x = 0; x < TG; ++x)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s[0][nt][i] = 0.f;
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[x][nt][i] = 0.f;
 #pragma unroll
   for (int hg = 0; hg < S::HG; ++hg)
 #pragma unroll
     for (int e = 0; e < S::E / 4; ++e) {
-      uint32_t w0[2], w1[2];
-      load_words<8>(kp + (hg * 2 * 32 + lane) * S::E + e * 4, w0);
-      load_words<8>(kp + ((hg * 2 + 1) * 32 + lane) * S::E + e * 4, w1);
-      const uint32_t a[4] = {w0[0], w1[0], w0[1], w1[1]};
+      uint32_t b0[NT], b1[NT];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-        mma_16<T>(s[0][nt], a, as_type<T>(rt.qf[hg * (S::E / 4) + e][nt][0]), as_type<T>(rt.qf[hg * (S::E / 4) + e][nt][1]));
+      for (int nt = 0; nt < NT; ++nt) {
+        b0[nt] = as_type<T>(rt.qf[hg * (S::E / 4) + e][nt][0]);
+        b1[nt] = as_type<T>(rt.qf[hg * (S::E / 4) + e][nt][1]);
+      }
+#pragma unroll
+      for (int x = 0; x < TG; ++x) {
+        uint32_t w0[2], w1[2];
+        load_words<8>(kp + x * 16 * DH + (hg * 2 * 32 + lane) * S::E + e * 4, w0);
+        load_words<8>(kp + x * 16 * DH + ((hg * 2 + 1) * 32 + lane) * S::E + e * 4, w1);
+        const uint32_t a[4] = {w0[0], w1[0], w0[1], w1[1]};
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) mma_16<T>(s[x][nt], a, b0[nt], b1[nt]);
+      }
     }
-  const float one[1] = {1.f}, zero[1] = {0.f};
-  soft_step<T, DH, NT, 1>(rt, st, s, one, zero, one, tok0, len, window, true);
-  uint32_t pf[NT][2];
+  float one[TG], zero[TG];
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    pf[nt][0] = transpose8x8(pack2<T>(s[0][nt][0], s[0][nt][1]));
-    pf[nt][1] = transpose8x8(pack2<T>(s[0][nt][2], s[0][nt][3]));
+  for (int x = 0; x < TG; ++x) {
+    one[x] = 1.f;
+    zero[x] = 0.f;
   }
-  const int k0 = tok0 + 2 * t;
-  const uint32_t keep0 = (k0 < len ? 0xffffu : 0u) | (k0 + 1 < len ? 0xffff0000u : 0u);
-  const uint32_t keep1 = (k0 + 8 < len ? 0xffffu : 0u) | (k0 + 9 < len ? 0xffff0000u : 0u);
+  soft_step<T, DH, NT, TG>(rt, st, s, one, zero, one, tok0, len, window, true);
 #pragma unroll
-  for (int c = 0; c < S::C; ++c) {
-    uint32_t w[4 * S::M];
-    load_words<16 * S::M>(vp + (c * 32 + lane) * 8 * S::M, w);
+  for (int x = 0; x < TG; ++x) {
+    uint32_t pf[NT][2];
 #pragma unroll
-    for (int m = 0; m < S::M; ++m) {
-      const uint32_t a[4] = {w[4 * m] & keep0, w[4 * m + 2] & keep0, w[4 * m + 1] & keep1, w[4 * m + 3] & keep1};
+    for (int nt = 0; nt < NT; ++nt) {
+      pf[nt][0] = transpose8x8(pack2<T>(s[x][nt][0], s[x][nt][1]));
+      pf[nt][1] = transpose8x8(pack2<T>(s[x][nt][2], s[x][nt][3]));
+    }
+    const int k0 = tok0 + x * 16 + 2 * t;
+    const uint32_t keep0 = (k0 < len ? 0xffffu : 0u) | (k0 + 1 < len ? 0xffff0000u : 0u);
+    const uint32_t keep1 = (k0 + 8 < len ? 0xffffu : 0u) | (k0 + 9 < len ? 0xffff0000u : 0u);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) mma_16<T>(st.o[c * S::M + m][nt], a, pf[nt][0], pf[nt][1]);
+    for (int c = 0; c < S::C; ++c) {
+      uint32_t w[4 * S::M];
+      load_words<16 * S::M>(vp + x * 16 * DH + (c * 32 + lane) * 8 * S::M, w);
+#pragma unroll
+      for (int m = 0; m < S::M; ++m) {
+        const uint32_t a[4] = {w[4 * m] & keep0, w[4 * m + 2] & keep0, w[4 * m + 1] & keep1, w[4 * m + 3] & keep1};
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) mma_16<T>(st.o[c * S::M + m][nt], a, pf[nt][0], pf[nt][1]);
+      }
     }
   }
 }
@@ -664,8 +711,8 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32) paged_attn_kernel(AttnParams 
       vp[x] = kp[x] + P * DH;
       const float2 sc = *reinterpret_cast<const float2*>(rec + 2 * P * DH);
       ks[x] = sc.x;
-      lv[x] = log2f(sc.y);
-      iv[x] = 1.f / sc.y;
+      lv[x] = log2_fast(sc.y);
+      iv[x] = rcp_fast(sc.y);
     }
     const int tok0 = u * P;
     const bool mask = tok0 + 63 > min(qlo, limit - 1) || (p.window > 0 && tok0 <= qhi - p.window);
@@ -675,8 +722,8 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32) paged_attn_kernel(AttnParams 
     const T* tk = reinterpret_cast<const T*>(p.c.tail) +
                   ((((int64_t)b * p.c.Hkv + h) * 2 + (n_full & 1)) * 2) * ((int64_t)P * DH);
     for (int x = warp; n_full * P + x * 16 <= qhi; x += ATTN_WARPS)
-      attend_tail<T, DH, NT>(rt, st, tk + x * 16 * DH, tk + (int64_t)P * DH + x * 16 * DH, n_full * P + x * 16, len,
-                             p.window);
+      attend_tail<T, DH, NT, 1>(rt, st, tk + x * 16 * DH, tk + (int64_t)P * DH + x * 16 * DH, n_full * P + x * 16, len,
+                                p.window);
   }
   // join the warps
 #pragma unroll
@@ -732,16 +779,21 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32) paged_attn_kernel(AttnParams 
 // at zero.
 template <int DH, int NT>
 struct SplitShape {
-  // A unit's bytes bound the number of rings: two units ahead of the one at work, for as many warps as fit
-  static constexpr int STAGE = 128 * DH + 64;
+  // Eight warps' rings, two units ahead of the one at work, fill the shared memory at 8 KB a unit.
+  static constexpr int UT = DH == 128 ? 32 : 64;     // tokens of a unit of full pages
+  static constexpr int TT = UT / 2;                  // tokens of a unit of the open page (16 bits)
+  static constexpr int STAGE = 2 * UT * DH + UT;     // codes, and 16 bytes of scales for up to UT / 16 records
   static constexpr int NS = 3;
-  static constexpr int WARPS = DH == 128 ? 4 : 8;
+  static constexpr int WARPS = 8;
   static constexpr int STATE = 8 * NT * DH + 16 * NT;  // floats: numerator fragments, then (maximum, sum) per row
   static constexpr int BAR_BYTES = WARPS * NS * 8;
   static constexpr int RING = WARPS * NS * STAGE;
 };
 
-constexpr int SPLIT_MIN_UNITS = 4;   // units per warp while warps are plenty: below, joining costs more than it spreads
+#ifndef TA_MIN_UNITS
+#define TA_MIN_UNITS 2
+#endif
+constexpr int SPLIT_MIN_UNITS = TA_MIN_UNITS;   // units per warp while warps are plenty: below, joining costs more than it spreads
 constexpr int SPLIT_MAX_BATCH = 2048;  // sequences whose geometry is kept in shared memory (12 bytes each)
 
 // The units of one item.
@@ -750,17 +802,17 @@ struct Item {
   int len, p0, p1;    // tokens held; full pages [p0, p1)
   int nu8, units;
 };
-__device__ __forceinline__ Item item_of(int row0, int n, int pos, int P, int window) {
+template <int UT>
+__device__ __forceinline__ Item item_of(int row0, int n, int pos, int lp, int window) {
   Item it;
   it.row0 = row0;
   it.n = n;
   it.pos = pos;
   it.len = pos + n;
-  it.p1 = it.len / P;
-  it.p0 = window > 0 ? max(0, pos - window + 1) / P : 0;
-  const int per = 64 / P;
-  it.nu8 = (it.p1 - it.p0 + per - 1) / per;
-  it.units = n > 0 ? it.nu8 + (it.len - it.p1 * P + 31) / 32 : 0;
+  it.p1 = it.len >> lp;
+  it.p0 = window > 0 ? max(0, pos - window + 1) >> lp : 0;
+  it.nu8 = (((it.p1 - it.p0) << lp) + UT - 1) / UT;
+  it.units = n > 0 ? it.nu8 + (it.len - (it.p1 << lp) + UT / 2 - 1) / (UT / 2) : 0;
   return it;
 }
 
@@ -768,8 +820,8 @@ template <typename T, int DH, int NT>
 __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
     paged_split_kernel(AttnParams p, int32_t* counters, float* states) {
   using SH = SplitShape<DH, NT>;
-  constexpr int WARPS = SH::WARPS, NS = SH::NS, ROWS = 8 * NT;
-  constexpr int TG = NT >= 3 ? 2 : 4;  // a whole unit's scores beside 24 or 32 rows' numerators do not fit the registers
+  constexpr int WARPS = SH::WARPS, NS = SH::NS, ROWS = 8 * NT, UT = SH::UT, TT = SH::TT;
+  constexpr int TG = NT >= 3 ? 2 : UT / 16;  // 64 tokens' scores beside 24 or 32 rows' numerators do not fit the registers
   extern __shared__ __align__(128) unsigned char split_smem[];
   __shared__ int warp_sums[WARPS];
   unsigned char* ring = split_smem;
@@ -778,8 +830,10 @@ __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
   int* s_row = s_first + p.B + 1;
   int* s_pos = s_row + p.B + 1;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int P = p.c.P, Hkv = p.c.Hkv, group = p.Hq / Hkv, per = 64 / P;
-  const int rec = 2 * P * DH + 16;
+  const int P = p.c.P, lp = 31 - __clz(P), Hkv = p.c.Hkv, group = p.Hq / Hkv;
+  const int64_t rec = 2 * P * DH + 16;
+  // a unit in shared memory: records of Pe tokens (whole ones, or a part of one with its scales)
+  const int Pe = min(P, UT), lpe = 31 - __clz(Pe), per = UT >> lpe, rec_e = 2 * Pe * DH + 16;
   uint64_t* bar = bars + warp * NS;
   if (lane == 0) {
     for (int i = 0; i < NS; ++i) mbar_init(bar + i, 1);
@@ -800,7 +854,7 @@ __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
       else if (ps < 0 || (int64_t)ps + n > (int64_t)p.c.max_pages * P + (P - 1))
         record_error(DEV_POS_RANGE, K_PAGED_ATTN, b, ps);
       else
-        units = item_of(r0, n, ps, P, p.window).units * Hkv;
+        units = item_of<UT>(r0, n, ps, lp, p.window).units * Hkv;
       s_first[b + 1] = units;
       s_row[b] = r0;
       s_pos[b] = ps;
@@ -846,7 +900,7 @@ __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
       else hi = mid - 1;
     }
     r.b = lo;
-    r.it = item_of(s_row[lo], s_row[lo + 1] - s_row[lo], s_pos[lo], P, p.window);
+    r.it = item_of<UT>(s_row[lo], s_row[lo + 1] - s_row[lo], s_pos[lo], lp, p.window);
     const int in = u - s_first[lo];
     r.h = in / r.it.units;
     r.k = in % r.it.units;
@@ -864,14 +918,14 @@ __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
   };
   auto begin_ahead = [&]() {
     open(ahead, au);
-    batch = ahead.it.p0 + ahead.k * per;
+    batch = ahead.it.p0 + ((ahead.k * UT) >> lp);
     entry = load_entry(batch + lane);
     entry_next = load_entry(batch + 32 + lane);
   };
   auto issue = [&](int slot) {
     unsigned char* dst = ring + (warp * NS + slot) * SH::STAGE;
     if (ahead.k < ahead.it.nu8) {
-      const int page = ahead.it.p0 + ahead.k * per;
+      const int page = ahead.it.p0 + ((ahead.k * UT) >> lp);
       if (page >= batch + 32) {
         batch += 32;
         entry = entry_next;
@@ -884,19 +938,24 @@ __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
         record_error(DEV_INDEX_RANGE, K_PAGED_ATTN, ahead.b, phys);
         phys = 0;
       }
-      if (lane == 0) mbar_arrive_expect_tx(bar + slot, (uint32_t)(per * rec));
+      const unsigned char* src = p.c.pool + ((int64_t)phys * Hkv + ahead.h) * rec;
+      if (lane == 0) mbar_arrive_expect_tx(bar + slot, (uint32_t)(per * rec_e));
       __syncwarp();
-      if (lane < per)
-        bulk_g2s(dst + lane * rec, p.c.pool + ((int64_t)phys * Hkv + ahead.h) * rec, (uint32_t)rec, bar + slot);
+      if (P <= UT) {
+        if (lane < per) bulk_g2s(dst + lane * rec_e, src, (uint32_t)rec_e, bar + slot);
+      } else if (lane < 3) {  // keys, values and scales of a part of the page
+        const int in = (ahead.k * UT) & (P - 1);
+        bulk_g2s(dst + lane * UT * DH, src + lane * P * DH + (lane < 2 ? in * DH : 0), lane < 2 ? UT * DH : 16, bar + slot);
+      }
     } else if (lane == 0) {
-      const int t0 = (ahead.k - ahead.it.nu8) * 32;  // token of the open page
-      const int left = ahead.it.len - ahead.it.p1 * P - t0;
-      const uint32_t bytes = (uint32_t)(left > 16 ? 2 : 1) * 16 * DH * 2;
+      const int t0 = (ahead.k - ahead.it.nu8) * TT;  // token of the open page
+      const int left = min(ahead.it.len - (ahead.it.p1 << lp) - t0, TT);
+      const uint32_t bytes = (uint32_t)((left + 15) >> 4) * 16 * DH * 2;
       const T* src = reinterpret_cast<const T*>(p.c.tail) +
                      ((((int64_t)ahead.b * Hkv + ahead.h) * 2 + (ahead.it.p1 & 1)) * 2) * ((int64_t)P * DH) + t0 * DH;
       mbar_arrive_expect_tx(bar + slot, 2 * bytes);
       bulk_g2s(dst, src, bytes, bar + slot);
-      bulk_g2s(dst + 64 * DH, src + (int64_t)P * DH, bytes, bar + slot);
+      bulk_g2s(dst + UT * DH, src + (int64_t)P * DH, bytes, bar + slot);
     }
     __syncwarp();
     ++au;
@@ -931,30 +990,28 @@ __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
         break;
       }
       if (k < it.nu8) {
-        const int tok0 = (it.p0 + k * per) * P, limit = it.p1 * P;
-        const bool mask = tok0 + 63 > min(it.pos, limit - 1) || (p.window > 0 && tok0 <= qhi - p.window);
+        const int tok0 = (it.p0 << lp) + k * UT, limit = it.p1 << lp;
+        const bool mask = tok0 + UT - 1 > min(it.pos, limit - 1) || (p.window > 0 && tok0 <= qhi - p.window);
 #pragma unroll 1
-        for (int y = 0; y < 4; y += TG) {  // 16-token groups at a time
+        for (int y = 0; y < UT / 16; y += TG) {  // 16-token groups at a time
           const unsigned char *kp[TG], *vp[TG];
           float ks[TG], lv[TG], iv[TG];
 #pragma unroll
           for (int x = 0; x < TG; ++x) {
-            const unsigned char* rp = src + ((y + x) * 16 / P) * rec;
-            kp[x] = rp + ((y + x) * 16 % P) * DH;
-            vp[x] = kp[x] + P * DH;
-            const float2 sc = *reinterpret_cast<const float2*>(rp + 2 * P * DH);
+            const unsigned char* rp = src + (((y + x) * 16) >> lpe) * rec_e;
+            kp[x] = rp + (((y + x) * 16) & (Pe - 1)) * DH;
+            vp[x] = kp[x] + Pe * DH;
+            const float2 sc = *reinterpret_cast<const float2*>(rp + 2 * Pe * DH);
             ks[x] = sc.x;
-            lv[x] = log2f(sc.y);
-            iv[x] = 1.f / sc.y;
+            lv[x] = log2_fast(sc.y);
+            iv[x] = rcp_fast(sc.y);
           }
           attend_codes<T, DH, NT, TG>(rt, st, kp, vp, ks, lv, iv, tok0 + y * 16, limit, p.window, mask);
         }
       } else {
-        const T* tk = reinterpret_cast<const T*>(src);
-        const T* tv = reinterpret_cast<const T*>(src + 64 * DH);
-        const int tok0 = it.p1 * P + (k - it.nu8) * 32;
-        for (int x = 0; x < 2 && tok0 + x * 16 < it.len; ++x)
-          attend_tail<T, DH, NT>(rt, st, tk + x * 16 * DH, tv + x * 16 * DH, tok0 + x * 16, it.len, p.window);
+        const int tok0 = (it.p1 << lp) + (k - it.nu8) * TT;
+        attend_tail<T, DH, NT, TT / 16>(rt, st, reinterpret_cast<const T*>(src), reinterpret_cast<const T*>(src + UT * DH),
+                                        tok0, it.len, p.window);
       }
       __syncwarp();  // every lane has read the unit
       if (au < u1) issue(slot);
@@ -974,14 +1031,13 @@ __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
     if (!write) {
       float* mine = states + ((int64_t)me * 2 + (run.u_item + run.k == u0 ? 0 : 1)) * SH::STATE;
 #pragma unroll
-      for (int x = 0; x < DH / 16; ++x)
+      for (int nt = 0; nt < NT; ++nt) {
+        if (nt * 8 + 2 * t >= R) continue;  // columns of no row are neither written nor read
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int x = 0; x < DH / 16; ++x)
           __stcg(reinterpret_cast<float4*>(mine) + (x * NT + nt) * 32 + lane,
                  make_float4(st.o[x][nt][0], st.o[x][nt][1], st.o[x][nt][2], st.o[x][nt][3]));
-      if (g == 0) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        if (g == 0)
           __stcg(reinterpret_cast<float4*>(mine + ROWS * DH) + nt * 4 + t,
                  make_float4(st.m[nt][0], st.m[nt][1], st.l[nt][0], st.l[nt][1]));
       }
@@ -1000,42 +1056,55 @@ __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
         auto state_of = [&](int w) {
           return states + ((int64_t)w * 2 + (w == wa && first_of(wa) < run.u_item ? 1 : 0)) * SH::STATE;
         };
-        float top[NT][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) top[nt][0] = top[nt][1] = -INFINITY;
-        for (int w = wa; w <= wb; ++w) {
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const float4 ml = __ldcg(reinterpret_cast<const float4*>(state_of(w) + ROWS * DH) + nt * 4 + t);
-            top[nt][0] = fmaxf(top[nt][0], ml.x);
-            top[nt][1] = fmaxf(top[nt][1], ml.y);
-          }
-        }
+        // each column's maximum over the states, 8 states at a time on the column's lanes
         st.clear();
-#pragma unroll 2
-        for (int w = wa; w <= wb; ++w) {
-          const float* s = state_of(w);
+        for (int w = wa + g; w <= wb; w += 8) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            const float4 ml = __ldcg(reinterpret_cast<const float4*>(s + ROWS * DH) + nt * 4 + t);
-            const float f0 = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - top[nt][0]);
-            const float f1 = ml.y == -INFINITY ? 0.f : exp2_fast(ml.y - top[nt][1]);
-            st.l[nt][0] += ml.z * f0;
-            st.l[nt][1] += ml.w * f1;
-#pragma unroll
-            for (int x = 0; x < DH / 16; ++x) {
-              const float4 o = __ldcg(reinterpret_cast<const float4*>(s) + (x * NT + nt) * 32 + lane);
-              st.o[x][nt][0] += o.x * f0;
-              st.o[x][nt][1] += o.y * f1;
-              st.o[x][nt][2] += o.z * f0;
-              st.o[x][nt][3] += o.w * f1;
-            }
+            if (nt * 8 + 2 * t >= R) continue;
+            const float4 ml = __ldcg(reinterpret_cast<const float4*>(state_of(w) + ROWS * DH) + nt * 4 + t);
+            st.m[nt][0] = fmaxf(st.m[nt][0], ml.x);
+            st.m[nt][1] = fmaxf(st.m[nt][1], ml.y);
           }
         }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          st.m[nt][0] = top[nt][0];
-          st.m[nt][1] = top[nt][1];
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            for (int o = 4; o < 32; o <<= 1) st.m[nt][i] = fmaxf(st.m[nt][i], __shfl_xor_sync(0xffffffffu, st.m[nt][i], o));
+        constexpr int PER = DH / 16 * NT, UN = PER >= 16 ? 1 : (PER >= 8 ? 2 : 4);  // states in flight
+        for (int w = wa; w <= wb; w += UN) {
+          float4 ml[UN][NT], o[UN][NT][DH / 16];
+#pragma unroll
+          for (int y = 0; y < UN; ++y)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              ml[y][nt] = make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
+              const bool live = w + y <= wb && nt * 8 + 2 * t < R;
+              const float* s = state_of(min(w + y, wb));
+              if (live) ml[y][nt] = __ldcg(reinterpret_cast<const float4*>(s + ROWS * DH) + nt * 4 + t);
+#pragma unroll
+              for (int x = 0; x < DH / 16; ++x) {
+                o[y][nt][x] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (live) o[y][nt][x] = __ldcg(reinterpret_cast<const float4*>(s) + (x * NT + nt) * 32 + lane);
+              }
+            }
+#pragma unroll
+          for (int y = 0; y < UN; ++y)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              const float f0 = ml[y][nt].x == -INFINITY ? 0.f : exp2_fast(ml[y][nt].x - st.m[nt][0]);
+              const float f1 = ml[y][nt].y == -INFINITY ? 0.f : exp2_fast(ml[y][nt].y - st.m[nt][1]);
+              st.l[nt][0] += ml[y][nt].z * f0;
+              st.l[nt][1] += ml[y][nt].w * f1;
+#pragma unroll
+              for (int x = 0; x < DH / 16; ++x) {
+                st.o[x][nt][0] += o[y][nt][x].x * f0;
+                st.o[x][nt][1] += o[y][nt][x].y * f1;
+                st.o[x][nt][2] += o[y][nt][x].z * f0;
+                st.o[x][nt][3] += o[y][nt][x].w * f1;
+              }
+            }
         }
       }
     }
