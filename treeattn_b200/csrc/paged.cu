@@ -91,7 +91,7 @@ int64_t split_bytes_dh(int64_t B, int64_t Hkv, int64_t rows) {
 constexpr int kSplitRows = 32;  // rows of one (sequence, kv head) up to which the cache's bytes bound the call
 
 bool split_takes(int64_t B, int64_t Hkv, int64_t rows, int64_t max_pages, int P) {
-  return rows <= kSplitRows && B <= ta::SPLIT_MAX_BATCH && B * Hkv * (max_pages * P / 32 + 5) <= INT_MAX;
+  return rows <= kSplitRows && B <= ta::SPLIT_MAX_BATCH && B * Hkv * (max_pages * P / 32 + 7) <= INT_MAX;
 }
 
 template <typename T, int DH, int NT>

@@ -387,30 +387,40 @@ struct RowTile {
   float cs[NT][2];              // score factor of the row, positive: |scale| * log2(e) / (its power of two)
   int qpos[NT][2];              // position of the row's query; -1: no such row
 
+  // The rows' elements as stored, in fragment order: fetched early, turned into fragments by finish.
+  struct Raw {
+    uint32_t w[NT][DH / 8];
+  };
+
   // row0: first row of the tile; R rows in all (n queries x group heads)
-  __device__ __forceinline__ void load(const AttnParams& p, const NewRows& nr, int h, int group, int row0, int R) {
+  static __device__ __forceinline__ void fetch(const AttnParams& p, int q_row0, int h, int group, int row0, int R, Raw& raw) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int rr = row0 + nt * 8 + g;
       const bool live = rr < R;
       const T* src = reinterpret_cast<const T*>(p.q);
-      if (live) src += (int64_t)(nr.row0 + rr / group) * p.q_sr + (int64_t)(h * group + rr % group) * p.q_sh;
-      float x[DH / 4];
-      float top = 0.f;
+      if (live) src += (int64_t)(q_row0 + rr / group) * p.q_sr + (int64_t)(h * group + rr % group) * p.q_sh;
 #pragma unroll
       for (int hg = 0; hg < S::HG; ++hg)
 #pragma unroll
         for (int e = 0; e < S::E; e += 4) {
           uint32_t w[2] = {0u, 0u};
           if (live) load_words<8>(src + hg * 4 * S::E + t * S::E + e, w);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float f = bits_value<T>((w[i >> 1] >> (16 * (i & 1))) & 0xffffu);
-            x[hg * S::E + e + i] = f;
-            top = fmaxf(top, fabsf(f));
-          }
+          raw.w[nt][(hg * S::E + e) / 2] = w[0];
+          raw.w[nt][(hg * S::E + e) / 2 + 1] = w[1];
         }
+    }
+  }
+
+  __device__ __forceinline__ void finish(const AttnParams& p, int pos, int group, int row0, int R, const Raw& raw) {
+    const int lane = threadIdx.x & 31, t = lane & 3;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float top = 0.f;
+#pragma unroll
+      for (int i = 0; i < DH / 8; ++i)
+        top = fmaxf(top, fmaxf(fabsf(bits_value<T>(raw.w[nt][i] & 0xffffu)), fabsf(bits_value<T>(raw.w[nt][i] >> 16))));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       // 2^ex * top in [2^14, 2^15): exact, and what falls below f16's range is below 2^-39 of the row's largest element
@@ -418,16 +428,15 @@ struct RowTile {
       // the sign of the scale joins the row; at scale 0 the row is 0
       const float up = p.scale == 0.f ? 0.f : copysignf(__int_as_float((ex + 127) << 23), p.scale);
 #pragma unroll
-      for (int kk = 0; kk < DH / 16; ++kk) {
-        qf[kk][nt][0] = pack2<__half>(x[kk * 4] * up, x[kk * 4 + 1] * up);
-        qf[kk][nt][1] = pack2<__half>(x[kk * 4 + 2] * up, x[kk * 4 + 3] * up);
-      }
+      for (int i = 0; i < DH / 8; ++i)
+        qf[i / 2][nt][i & 1] =
+            pack2<__half>(bits_value<T>(raw.w[nt][i] & 0xffffu) * up, bits_value<T>(raw.w[nt][i] >> 16) * up);
       const float f = p.scale == 0.f ? 1.f : fabsf(p.scale) * 1.4426950408889634f * __int_as_float((127 - ex) << 23);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         cs[nt][i] = __shfl_sync(0xffffffffu, f, (2 * t + i) * 4);
         const int col = row0 + nt * 8 + 2 * t + i;
-        qpos[nt][i] = col < R ? nr.pos + col / group : -1;
+        qpos[nt][i] = col < R ? pos + col / group : -1;
       }
     }
   }
@@ -690,7 +699,11 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32) paged_attn_kernel(AttnParams 
   const int p0 = lo / P, p1 = min(n_full, qhi / P + 1), limit = p1 * P;
   const int per = 64 / P;
   RowTile<T, DH, NT> rt;
-  rt.load(p, nr, h, group, row0, R);
+  {
+    typename RowTile<T, DH, NT>::Raw raw;
+    rt.fetch(p, nr.row0, h, group, row0, R, raw);
+    rt.finish(p, nr.pos, group, row0, R, raw);
+  }
   SoftState<DH, NT> st;
   st.clear();
   const int32_t* tab = p.c.table + b * p.c.table_sb;
@@ -775,8 +788,8 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32) paged_attn_kernel(AttnParams 
 // begin another. Each warp keeps its own ring of units in shared memory, filled by bulk copies (a record of a full page is
 // one copy, scales included), so the only waits are for its own copies.
 // An item that one warp holds whole is written out at once; of the others each warp leaves its state (maximum, sum,
-// numerator) in the workspace, and the warp that comes last (a counter per item) joins them in order. The counters are left
-// at zero.
+// numerator) in the workspace, and the warp that comes last (a counter per item), or its CTA, joins them in order. The
+// counters are left at zero.
 template <int DH, int NT>
 struct SplitShape {
   // Eight warps' rings, two units ahead of the one at work, fill the shared memory at 8 KB a unit.
@@ -794,13 +807,16 @@ struct SplitShape {
 #define TA_MIN_UNITS 2
 #endif
 constexpr int SPLIT_MIN_UNITS = TA_MIN_UNITS;   // units per warp while warps are plenty: below, joining costs more than it spreads
+// An item's own cost, in units (its queries' loads, its output or state): without it a warp whose run is many short sequences
+// comes last (64 uneven sequences, one of them a single token: 67 us without it, 64.5 with)
+constexpr int SPLIT_ITEM_COST = 2;
 constexpr int SPLIT_MAX_BATCH = 2048;  // sequences whose geometry is kept in shared memory (12 bytes each)
 
 // The units of one item.
 struct Item {
   int pos, n, row0;
   int len, p0, p1;    // tokens held; full pages [p0, p1)
-  int nu8, units;
+  int nu8, units;     // units of full pages, of all
 };
 template <int UT>
 __device__ __forceinline__ Item item_of(int row0, int n, int pos, int lp, int window) {
@@ -816,14 +832,180 @@ __device__ __forceinline__ Item item_of(int row0, int n, int pos, int lp, int wi
   return it;
 }
 
+// Joins the states of an item's parts, in order, into st: part 0 at `first`, part w at later + w * stride. Two rows or
+// fewer leave three quarters of a state's lanes without a row (four or fewer: half), which then take other parts.
+template <int DH, int NT>
+__device__ __forceinline__ void join_states(SoftState<DH, NT>& st, const float* first, const float* later, int stride,
+                                            int parts, int R) {
+  constexpr int ROWS = 8 * NT;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int fold = NT > 1 || R > 4 ? 1 : (R > 2 ? 2 : 4);  // parts side by side
+  const int tc = t % (4 / fold), side = t / (4 / fold);    // column pair and side of this lane
+  st.clear();
+  constexpr int UN = DH / 16 * NT >= 8 ? 2 : 4;  // parts in flight (on each side)
+  for (int w0 = 0; w0 < parts; w0 += UN * fold) {
+    float4 ml[UN][NT], o[UN][NT][DH / 16];
+#pragma unroll
+    for (int y = 0; y < UN; ++y) {
+      const int w = w0 + y * fold + side;
+      const float* s = w == 0 ? first : later + (int64_t)w * stride;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        ml[y][nt] = make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
+        const bool live = w < parts && nt * 8 + 2 * tc < R;
+        if (live) ml[y][nt] = __ldcg(reinterpret_cast<const float4*>(s + ROWS * DH) + nt * 4 + tc);
+#pragma unroll
+        for (int x = 0; x < DH / 16; ++x) {
+          o[y][nt][x] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (live) o[y][nt][x] = __ldcg(reinterpret_cast<const float4*>(s) + (x * NT + nt) * 32 + g * 4 + tc);
+        }
+      }
+    }
+    // a part that saw nothing, or nothing but NaN, has no maximum: its sums count as they are
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float f[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float mn = st.m[nt][i];
+#pragma unroll
+        for (int y = 0; y < UN; ++y) mn = fmaxf(mn, i ? ml[y][nt].y : ml[y][nt].x);
+        f[i] = st.m[nt][i] == -INFINITY ? 1.f : exp2_fast(st.m[nt][i] - mn);
+        st.m[nt][i] = mn;
+        st.l[nt][i] *= f[i];
+      }
+#pragma unroll
+      for (int x = 0; x < DH / 16; ++x)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) st.o[x][nt][i] *= f[i & 1];
+#pragma unroll
+      for (int y = 0; y < UN; ++y) {
+        const float f0 = ml[y][nt].x == -INFINITY ? 1.f : exp2_fast(ml[y][nt].x - st.m[nt][0]);
+        const float f1 = ml[y][nt].y == -INFINITY ? 1.f : exp2_fast(ml[y][nt].y - st.m[nt][1]);
+        st.l[nt][0] += ml[y][nt].z * f0;
+        st.l[nt][1] += ml[y][nt].w * f1;
+#pragma unroll
+        for (int x = 0; x < DH / 16; ++x) {
+          st.o[x][nt][0] += o[y][nt][x].x * f0;
+          st.o[x][nt][1] += o[y][nt][x].y * f1;
+          st.o[x][nt][2] += o[y][nt][x].z * f0;
+          st.o[x][nt][3] += o[y][nt][x].w * f1;
+        }
+      }
+    }
+  }
+  if (fold > 1)  // the sides meet
+    for (int d = 4 / fold; d < 4; d <<= 1) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float om = __shfl_xor_sync(0xffffffffu, st.m[0][i], d), mn = fmaxf(st.m[0][i], om);
+        const float f = st.m[0][i] == -INFINITY ? 1.f : exp2_fast(st.m[0][i] - mn);
+        st.m[0][i] = mn;
+        st.l[0][i] *= f;
+        st.l[0][i] += __shfl_xor_sync(0xffffffffu, st.l[0][i], d);
+#pragma unroll
+        for (int x = 0; x < DH / 16; ++x)
+#pragma unroll
+          for (int j = i; j < 4; j += 2) {
+            st.o[x][0][j] *= f;
+            st.o[x][0][j] += __shfl_xor_sync(0xffffffffu, st.o[x][0][j], d);
+          }
+      }
+    }
+}
+
+// An item whose parts are all in the workspace: part 0 is the second state of warp `first`, part w the first state of warp
+// first + w.
+struct Join {
+  int row0, n, h, first, parts;
+};
+
+// Joins 16 dims (tile x) of an item's states, in order, and writes them out: the form for large states, in which all warps
+// of a CTA share. No load is conditional (a branch around each kept them apart): a place without a part reads the last one and
+// counts it 0 times, columns of no row come to nothing.
+template <typename T, int DH, int NT>
+__device__ __noinline__ void join_tile(const AttnParams& p, const Join& j, const float* states, int x) {
+  using SH = SplitShape<DH, NT>;
+  constexpr int ROWS = 8 * NT, UN = 8;  // parts in flight
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int group = p.Hq / p.c.Hkv, R = j.n * group, parts = j.parts;
+  auto state_of = [&](int w) {
+    w = min(w, parts - 1);
+    return states + ((int64_t)(j.first + w) * 2 + (w == 0 ? 1 : 0)) * SH::STATE;
+  };
+  // maxima, sums and numerators together: a new maximum scales what there is
+  float m[NT][2], l[NT][2], acc[NT][4];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    m[nt][0] = m[nt][1] = -INFINITY;
+    l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[nt][i] = 0.f;
+  }
+#pragma unroll 1
+  for (int w0 = 0; w0 < parts; w0 += UN) {
+    float4 ml[UN][NT], o[UN][NT];
+#pragma unroll
+    for (int y = 0; y < UN; ++y) {
+      const float4* s = reinterpret_cast<const float4*>(state_of(w0 + y));
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        ml[y][nt] = __ldcg(s + ROWS * DH / 4 + nt * 4 + t);
+        o[y][nt] = __ldcg(s + (x * NT + nt) * 32 + lane);
+      }
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float mn = m[nt][i];
+#pragma unroll
+        for (int y = 0; y < UN; ++y) mn = fmaxf(mn, i ? ml[y][nt].y : ml[y][nt].x);
+        // (a part that saw nothing, or nothing but NaN, has no maximum: its sums count as they are)
+        const float f = m[nt][i] == -INFINITY ? 1.f : exp2_fast(m[nt][i] - mn);
+        m[nt][i] = mn;
+        l[nt][i] *= f;
+        acc[nt][i] *= f;
+        acc[nt][i + 2] *= f;
+#pragma unroll
+        for (int y = 0; y < UN; ++y) {
+          const float my = i ? ml[y][nt].y : ml[y][nt].x;
+          const float fy = w0 + y >= parts ? 0.f : (my == -INFINITY ? 1.f : exp2_fast(my - mn));
+          l[nt][i] += (i ? ml[y][nt].w : ml[y][nt].z) * fy;
+          acc[nt][i] += (i ? o[y][nt].y : o[y][nt].x) * fy;
+          acc[nt][i + 2] += (i ? o[y][nt].w : o[y][nt].z) * fy;
+        }
+      }
+  }
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int rr = nt * 8 + 2 * t + i;
+      if (rr >= R) continue;
+      const int64_t row = j.row0 + rr / group;
+      const int hq = j.h * group + rr % group;
+      T* out = reinterpret_cast<T*>(p.out) + row * p.o_sr + (int64_t)hq * p.o_sh + x * 16 + g;
+      const float inv = l[nt][i] == 0.f ? 0.f : 1.f / l[nt][i];
+      out[0] = from_f32<T>(acc[nt][i] * inv);
+      out[8] = from_f32<T>(acc[nt][i + 2] * inv);
+      if (p.lse && g == 0 && x == 0)
+        p.lse[row * p.Hq + hq] =
+            l[nt][i] == 0.f ? -INFINITY : (m[nt][i] - ATTN_SHIFT + log2f(l[nt][i])) * 0.69314718055994531f;
+    }
+}
+
 template <typename T, int DH, int NT>
 __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
     paged_split_kernel(AttnParams p, int32_t* counters, float* states) {
   using SH = SplitShape<DH, NT>;
   constexpr int WARPS = SH::WARPS, NS = SH::NS, ROWS = 8 * NT, UT = SH::UT, TT = SH::TT;
+  constexpr bool LATE = DH / 16 * NT > 8;  // joins by the whole CTA at its end
   constexpr int TG = NT >= 3 ? 2 : UT / 16;  // 64 tokens' scores beside 24 or 32 rows' numerators do not fit the registers
   extern __shared__ __align__(128) unsigned char split_smem[];
   __shared__ int warp_sums[WARPS];
+  __shared__ Join joins[2 * WARPS];  // items that a warp of this CTA came last at: a warp has two parts at most
+  __shared__ int n_joins;
   unsigned char* ring = split_smem;
   uint64_t* bars = reinterpret_cast<uint64_t*>(split_smem + SH::RING);
   int* s_first = reinterpret_cast<int*>(split_smem + SH::RING + SH::BAR_BYTES);  // first unit of sequence b (B + 1)
@@ -839,6 +1021,7 @@ __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
     for (int i = 0; i < NS; ++i) mbar_init(bar + i, 1);
     fence_mbar_init();
   }
+  if (tid == 0) n_joins = 0;
   pdl_wait();
   pdl_launch_dependents();
   // where each sequence's units begin
@@ -854,7 +1037,7 @@ __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
       else if (ps < 0 || (int64_t)ps + n > (int64_t)p.c.max_pages * P + (P - 1))
         record_error(DEV_POS_RANGE, K_PAGED_ATTN, b, ps);
       else
-        units = item_of<UT>(r0, n, ps, lp, p.window).units * Hkv;
+        units = n > 0 ? (item_of<UT>(r0, n, ps, lp, p.window).units + SPLIT_ITEM_COST) * Hkv : 0;
       s_first[b + 1] = units;
       s_row[b] = r0;
       s_pos[b] = ps;
@@ -880,44 +1063,55 @@ __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
   const int total = s_first[p.B];
   if (total == 0) return;
   const int n_work = min((int)gridDim.x * WARPS, (total + SPLIT_MIN_UNITS - 1) / SPLIT_MIN_UNITS);
-  const int me = warp * gridDim.x + blockIdx.x;
-  if (me >= n_work) return;
+  // a few warps: one on each SM first; all of them: neighbours share an SM, which spreads the joins
+  const int me = n_work < (int)gridDim.x * WARPS ? warp * gridDim.x + blockIdx.x : blockIdx.x * WARPS + warp;
   auto first_of = [&](int w) { return (int)((int64_t)total * w / n_work); };
   auto owner_of = [&](int u) { return (int)((((int64_t)u + 1) * n_work - 1) / total); };
-  const int u0 = first_of(me), u1 = first_of(me + 1);
+  const int u0 = me < n_work ? first_of(me) : 0, u1 = me < n_work ? first_of(me + 1) : 0;
   const int32_t* table = p.c.table;
 
-  // A run of units of one item: [k, end) of it.
+  // A run of units of one item: [k, end) of it. Places in the order of all items count SPLIT_ITEM_COST empty ones before an
+  // item's units.
   struct Run {
     Item it;
-    int b, h, k, end, u_item;
+    int b, h, k, end;
+    int at;    // place of the item's first unit
+    int next;  // place after the run
   };
+  // the first run from place u on; false when only empty places are left
   auto open = [&](Run& r, int u) {
-    int lo = 0, hi = p.B - 1;
-    while (lo < hi) {  // the last sequence that begins at or before u and has units
-      const int mid = (lo + hi + 1) / 2;
-      if (s_first[mid] <= u) lo = mid;
-      else hi = mid - 1;
+    while (u < u1) {
+      int lo = 0, hi = p.B - 1;
+      while (lo < hi) {  // the last sequence that begins at or before u
+        const int mid = (lo + hi + 1) / 2;
+        if (s_first[mid] <= u) lo = mid;
+        else hi = mid - 1;
+      }
+      r.b = lo;
+      r.it = item_of<UT>(s_row[lo], s_row[lo + 1] - s_row[lo], s_pos[lo], lp, p.window);
+      const int size = r.it.units + SPLIT_ITEM_COST, in = u - s_first[lo];
+      r.h = in / size;
+      r.at = u - in % size + SPLIT_ITEM_COST;
+      r.k = max(0, u - r.at);
+      r.end = min(r.it.units, u1 - r.at);
+      r.next = min(u1, r.at + r.it.units);
+      if (r.k < r.end) return true;
+      u = r.next;
     }
-    r.b = lo;
-    r.it = item_of<UT>(s_row[lo], s_row[lo + 1] - s_row[lo], s_pos[lo], lp, p.window);
-    const int in = u - s_first[lo];
-    r.h = in / r.it.units;
-    r.k = in % r.it.units;
-    r.u_item = u - r.k;
-    r.end = min(r.it.units, r.k + (u1 - u));
+    return false;
   };
 
   // ---- copies: `ahead` runs NS units before the one at work
   Run ahead{};
-  int au = u0;          // its unit
+  bool more = true;     // it has a unit to copy
   int batch = 0;        // page of the item that lane 0's table entry stands for
   int entry = 0, entry_next = 0;
   auto load_entry = [&](int page) {
     return page < ahead.it.p1 ? table[ahead.b * p.c.table_sb + page] : 0;
   };
-  auto begin_ahead = [&]() {
-    open(ahead, au);
+  auto begin_ahead = [&](int u) {
+    more = open(ahead, u);
+    if (!more) return;
     batch = ahead.it.p0 + ((ahead.k * UT) >> lp);
     entry = load_entry(batch + lane);
     entry_next = load_entry(batch + 32 + lane);
@@ -958,31 +1152,30 @@ __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
       bulk_g2s(dst + UT * DH, src + (int64_t)P * DH, bytes, bar + slot);
     }
     __syncwarp();
-    ++au;
-    if (++ahead.k == ahead.end && au < u1) begin_ahead();
+    if (++ahead.k == ahead.end) begin_ahead(ahead.next);
   };
-
-  begin_ahead();
-  for (int i = 0; i < NS; ++i)
-    if (au < u1) issue(i);
 
   RowTile<T, DH, NT> rt;
   SoftState<DH, NT> st;
   Run run;
+  typename RowTile<T, DH, NT>::Raw raw;
+  begin_ahead(u0);
+  const bool idle = !more;
+  run = ahead;
+  // the first run's queries are fetched before the copies fill the memory's queues
+  if (!idle) rt.fetch(p, run.it.row0, run.h, group, 0, run.it.n * group, raw);
+  int issued = 0;
+  for (; issued < NS && more; ++issued) issue(issued);
   bool ok = true;
-  int u = u0, step = 0;  // step: units consumed
-  while (u < u1) {
-    open(run, u);
+  int step = 0;  // units consumed
+  for (bool first = true; !idle && (first || open(run, run.next)); first = false) {
+    if (!first) rt.fetch(p, run.it.row0, run.h, group, 0, run.it.n * group, raw);
+    rt.finish(p, run.it.pos, group, 0, run.it.n * group, raw);
     const Item& it = run.it;
     const int R = it.n * group;
-    NewRows nr;
-    nr.row0 = it.row0;
-    nr.n = it.n;
-    nr.pos = it.pos;
-    rt.load(p, nr, run.h, group, 0, R);
     st.clear();
     const int qhi = it.pos + it.n - 1;
-    for (int k = run.k; k < run.end; ++k, ++u, ++step) {
+    for (int k = run.k; k < run.end; ++k, ++step) {
       const int slot = step % NS;
       const unsigned char* src = ring + (warp * NS + slot) * SH::STAGE;
       if (!mbar_wait_bounded(bar + slot, (step / NS) & 1, K_PAGED_ATTN, 1)) {
@@ -1014,7 +1207,10 @@ __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
                                         tok0, it.len, p.window);
       }
       __syncwarp();  // every lane has read the unit
-      if (au < u1) issue(slot);
+      if (more) {
+        issue(slot);
+        ++issued;
+      }
     }
     if (!ok) break;
     // ---- the run's end: out, or into the workspace
@@ -1029,7 +1225,8 @@ __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
       }
     bool write = run.k == 0 && run.end == it.units;
     if (!write) {
-      float* mine = states + ((int64_t)me * 2 + (run.u_item + run.k == u0 ? 0 : 1)) * SH::STATE;
+      // a warp's first state is of an item that others began, its second of one that it begins
+      float* mine = states + ((int64_t)me * 2 + (run.k > 0 ? 0 : 1)) * SH::STATE;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         if (nt * 8 + 2 * t >= R) continue;  // columns of no row are neither written nor read
@@ -1043,68 +1240,20 @@ __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
       }
       __threadfence();
       __syncwarp();
-      const int wa = owner_of(run.u_item), wb = owner_of(run.u_item + it.units - 1);
+      const int wa = owner_of(run.at), wb = owner_of(run.at + it.units - 1);
       int32_t* cnt = counters + run.b * Hkv + run.h;
       int before = 0;
       if (lane == 0) before = atomicAdd(cnt, 1);
       before = __shfl_sync(0xffffffffu, before, 0);
-      write = before == wb - wa;
-      if (write) {
+      if (before == wb - wa) {
         __threadfence();
         if (lane == 0) *cnt = 0;
-        // the item's states in order: the first one is its warp's second unless that warp begins with the item
-        auto state_of = [&](int w) {
-          return states + ((int64_t)w * 2 + (w == wa && first_of(wa) < run.u_item ? 1 : 0)) * SH::STATE;
-        };
-        // each column's maximum over the states, 8 states at a time on the column's lanes
-        st.clear();
-        for (int w = wa + g; w <= wb; w += 8) {
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            if (nt * 8 + 2 * t >= R) continue;
-            const float4 ml = __ldcg(reinterpret_cast<const float4*>(state_of(w) + ROWS * DH) + nt * 4 + t);
-            st.m[nt][0] = fmaxf(st.m[nt][0], ml.x);
-            st.m[nt][1] = fmaxf(st.m[nt][1], ml.y);
-          }
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            for (int o = 4; o < 32; o <<= 1) st.m[nt][i] = fmaxf(st.m[nt][i], __shfl_xor_sync(0xffffffffu, st.m[nt][i], o));
-        constexpr int PER = DH / 16 * NT, UN = PER >= 16 ? 1 : (PER >= 8 ? 2 : 4);  // states in flight
-        for (int w = wa; w <= wb; w += UN) {
-          float4 ml[UN][NT], o[UN][NT][DH / 16];
-#pragma unroll
-          for (int y = 0; y < UN; ++y)
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              ml[y][nt] = make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
-              const bool live = w + y <= wb && nt * 8 + 2 * t < R;
-              const float* s = state_of(min(w + y, wb));
-              if (live) ml[y][nt] = __ldcg(reinterpret_cast<const float4*>(s + ROWS * DH) + nt * 4 + t);
-#pragma unroll
-              for (int x = 0; x < DH / 16; ++x) {
-                o[y][nt][x] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (live) o[y][nt][x] = __ldcg(reinterpret_cast<const float4*>(s) + (x * NT + nt) * 32 + lane);
-              }
-            }
-#pragma unroll
-          for (int y = 0; y < UN; ++y)
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              const float f0 = ml[y][nt].x == -INFINITY ? 0.f : exp2_fast(ml[y][nt].x - st.m[nt][0]);
-              const float f1 = ml[y][nt].y == -INFINITY ? 0.f : exp2_fast(ml[y][nt].y - st.m[nt][1]);
-              st.l[nt][0] += ml[y][nt].z * f0;
-              st.l[nt][1] += ml[y][nt].w * f1;
-#pragma unroll
-              for (int x = 0; x < DH / 16; ++x) {
-                st.o[x][nt][0] += o[y][nt][x].x * f0;
-                st.o[x][nt][1] += o[y][nt][x].y * f1;
-                st.o[x][nt][2] += o[y][nt][x].z * f0;
-                st.o[x][nt][3] += o[y][nt][x].w * f1;
-              }
-            }
+        if constexpr (LATE) {
+          if (lane == 0) joins[atomicAdd(&n_joins, 1)] = Join{it.row0, it.n, run.h, wa, wb - wa + 1};
+        } else {
+          const float* later = states + (int64_t)wa * 2 * SH::STATE;
+          join_states<DH, NT>(st, later + SH::STATE, later, 2 * SH::STATE, wb - wa + 1, R);
+          write = true;
         }
       }
     }
@@ -1130,7 +1279,14 @@ __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
     }
   }
   if (!ok)  // no copy of this warp may still be in flight when its CTA ends
-    for (int i = step + 1; i < step + NS && u0 + i < au; ++i) mbar_wait_bounded(bar + i % NS, (i / NS) & 1, K_PAGED_ATTN, 2);
+    for (int i = step + 1; i < issued; ++i) mbar_wait_bounded(bar + i % NS, (i / NS) & 1, K_PAGED_ATTN, 2);
+  if constexpr (LATE) {
+    // What this CTA's warps completed, joined by all of them once their units are done: one warp alone took 16 to 20 us for
+    // 12 parts of 20 rows at head dim 128, which kept it from its own next units (60 us in all against 54). Small states are
+    // joined on the spot, while the other warps stream (64 sequences, one row: 65 us against 73).
+    __syncthreads();
+    for (int i = warp; i < n_joins * (DH / 16); i += WARPS) join_tile<T, DH, NT>(p, joins[i / (DH / 16)], states, i % (DH / 16));
+  }
 }
 
 }  // namespace ta

@@ -10,7 +10,7 @@ import math
 import torch
 
 from . import _lib
-from ._ops import _DT, _need_cuda, _p, _stream
+from ._ops import _DT, _need_cuda, _p
 
 PAGE_SIZES = (16, 32, 64)
 
@@ -26,20 +26,24 @@ class PagedKV:
 
     def __init__(self, pool, tail, table, page, head_dim):
         self.pool, self.tail, self.table, self.page, self.head_dim = pool, tail, table, int(page), int(head_dim)
+        n = self.page * self.head_dim
         if self.page not in PAGE_SIZES:
             raise ValueError('PagedKV: pages of 16, 32 or 64 tokens (got %d)' % self.page)
-        if pool.dtype != torch.uint8 or pool.dim() != 3 or pool.shape[2] != 2 * self.page * self.head_dim + 16:
+        shape = pool.shape
+        if pool.dtype is not torch.uint8 or len(shape) != 3 or shape[2] != 2 * n + 16:
             raise ValueError('PagedKV: pool must be (n_pages, n_kv_head, 2 * page * head_dim + 16) uint8')
-        if tail.dim() != 5 or tail.shape[1:] != (pool.shape[1], 2, 2, self.page * self.head_dim):
+        tshape = tail.shape
+        if len(tshape) != 5 or tshape[1:] != (shape[1], 2, 2, n):
             raise ValueError('PagedKV: tail must be (batch, n_kv_head, 2, 2, page * head_dim)')
-        if tail.dtype not in (torch.bfloat16, torch.float16):
+        if tail.dtype is not torch.bfloat16 and tail.dtype is not torch.float16:
             raise TypeError('PagedKV: the tail holds bfloat16 or float16 (got %s)' % tail.dtype)
-        if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != tail.shape[0] or (
+        if table.dtype is not torch.int32 or table.dim() != 2 or table.shape[0] != tshape[0] or (
                 table.shape[1] > 1 and table.stride(1) != 1):
             raise ValueError('PagedKV: table must be (batch, max_pages) int32 with unit inner stride')
         if not (pool.is_contiguous() and tail.is_contiguous()):
             raise ValueError('PagedKV: pool and tail must be contiguous')
-        _need_cuda('PagedKV', pool, tail, table)
+        if not (pool.is_cuda and tail.is_cuda and table.is_cuda):
+            _need_cuda('PagedKV', pool, tail, table)
 
     @classmethod
     def empty(cls, n_pages, n_kv_head, head_dim, table, page=64, dtype=torch.bfloat16):
@@ -125,23 +129,46 @@ def rotation_table(n_pos, rot, base=10000.0, device='cuda'):
     return a.cos().float(), a.sin().float()
 
 
+# A decode step's calls take a few microseconds on the GPU: the checks below ask each tensor once, the entry points are looked
+# up once, and the current stream is read without building a torch Stream object (2.3 -> 0.2 us).
+_entry = {}
+
+
+def _call(name, *args):
+    fn = _entry.get(name)
+    if fn is None:
+        fn = _entry[name] = getattr(_lib.load(), name)
+    if fn(*args) != _lib.TA_OK:
+        raise _lib.TreeAttnError('%s: %s' % (name, _lib.last_error()))
+
+
+def _stream(t):
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
 def _rows(name, cache, start, pos):
-    if start.dtype != torch.int32 or pos.dtype != torch.int32 or not start.is_contiguous() or not pos.is_contiguous():
+    if start.dtype is not torch.int32 or pos.dtype is not torch.int32 or not (start.is_contiguous() and pos.is_contiguous()):
         raise TypeError('%s: start and pos must be contiguous int32' % name)
-    B = pos.shape[0]
-    if start.dim() != 1 or pos.dim() != 1 or start.shape[0] != B + 1 or B != cache.table.shape[0]:
-        raise ValueError('%s: start (batch + 1,) and pos (batch,) for the cache\'s %d sequences' % (
-            name, cache.table.shape[0]))
+    B = cache.table.shape[0]
+    if start.shape != (B + 1,) or pos.shape != (B,):
+        raise ValueError('%s: start (batch + 1,) and pos (batch,) for the cache\'s %d sequences' % (name, B))
+    if not (start.is_cuda and pos.is_cuda):
+        _need_cuda(name, start, pos)
     return B
 
 
 def _heads(name, cache, x, dtype):
-    if x.dim() != 3 or x.shape[2] != cache.head_dim:
+    """Checks rows (n, heads, head_dim) and returns their shape and strides."""
+    shape, stride = x.shape, x.stride()
+    if len(shape) != 3 or shape[2] != cache.head_dim:
         raise ValueError('%s: rows must be (n, heads, %d)' % (name, cache.head_dim))
-    if x.dtype != dtype:
+    if x.dtype is not dtype:
         raise TypeError('%s: %s rows for a cache with a %s tail' % (name, x.dtype, dtype))
-    if x.stride(2) != 1:
+    if stride[2] != 1:
         raise ValueError('%s: the innermost (head) dimension must be contiguous' % name)
+    if not x.is_cuda:
+        _need_cuda(name, x)
+    return shape, stride
 
 
 def paged_append(cache, k, v, start, pos, max_new, q=None, rotation=None, q_out=None):
@@ -152,41 +179,40 @@ def paged_append(cache, k, v, start, pos, max_new, q=None, rotation=None, q_out=
     cut back to any length whose page is the last or last but one written."""
     pool, tail, table = cache.pool, cache.tail, cache.table
     dt = tail.dtype
-    _need_cuda('paged_append', k, v, start, pos, q)
     B = _rows('paged_append', cache, start, pos)
-    _heads('paged_append', cache, k, dt)
-    _heads('paged_append', cache, v, dt)
-    n, H, dh = k.shape
-    if H != pool.shape[1] or v.shape != k.shape:
-        raise ValueError('paged_append: k and v must be (n, %d, %d)' % (pool.shape[1], dh))
-    cos = sin = None
-    rot = n_pos = 0
+    kshape, ks = _heads('paged_append', cache, k, dt)
+    vshape, vs = _heads('paged_append', cache, v, dt)
+    n, H, dh = kshape
+    n_pages, n_kv, _ = pool.shape
+    if H != n_kv or vshape != kshape:
+        raise ValueError('paged_append: k and v must be (n, %d, %d)' % (n_kv, dh))
+    cos = sin = qp = qo = None
+    rot = n_pos = Hq = qr = qh = 0
     if rotation is not None:
         cos, sin = rotation
-        if (cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.shape != sin.shape or cos.dim() != 2 or
-                not cos.is_contiguous() or not sin.is_contiguous()):
+        if (cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or cos.shape != sin.shape or cos.dim() != 2 or
+                not (cos.is_contiguous() and sin.is_contiguous())):
             raise ValueError('paged_append: rotation must be two contiguous fp32 tables (positions, rot / 2)')
         _need_cuda('paged_append', cos, sin)
-        n_pos, rot = cos.shape[0], 2 * cos.shape[1]
-    Hq = qr = qh = 0
-    qo = None
+        n_pos, rot = cos.shape
+        rot *= 2
+        cos, sin = cos.data_ptr(), sin.data_ptr()
     if q is not None:
-        _heads('paged_append', cache, q, dt)
-        if q.shape[0] != n:
-            raise ValueError('paged_append: q has %d rows, k %d' % (q.shape[0], n))
+        qshape, qs = _heads('paged_append', cache, q, dt)
+        if qshape[0] != n:
+            raise ValueError('paged_append: q has %d rows, k %d' % (qshape[0], n))
         if rot:
-            Hq, qr, qh = q.shape[1], q.stride(0), q.stride(1)
+            Hq, qr, qh = qshape[1], qs[0], qs[1]
             if q_out is None:
-                q_out = torch.empty(n, Hq, dh, device=q.device, dtype=dt)
-            elif q_out.shape != q.shape or q_out.dtype != dt or not q_out.is_contiguous():
+                q_out = torch.empty(qshape, device=q.device, dtype=dt)
+            elif q_out.shape != qshape or q_out.dtype is not dt or not q_out.is_contiguous():
                 raise ValueError('paged_append: q_out must be contiguous, of q\'s shape and type')
-            qo = q_out
+            qp, qo = q.data_ptr(), q_out.data_ptr()
         else:
             q_out = q
-    _lib.call('ta_paged_append', pool.data_ptr(), tail.data_ptr(), table.data_ptr(), table.stride(0), pool.shape[0],
-              table.shape[1], cache.page, _DT[dt], B, H, dh, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0),
-              v.stride(1), n, start.data_ptr(), pos.data_ptr(), int(max_new), _p(cos), _p(sin), n_pos, rot,
-              q.data_ptr() if qo is not None else None, Hq, qr, qh, _p(qo), _stream(k))
+    _call('ta_paged_append', pool.data_ptr(), tail.data_ptr(), table.data_ptr(), table.stride(0), n_pages, table.shape[1],
+          cache.page, _DT[dt], B, H, dh, k.data_ptr(), v.data_ptr(), ks[0], ks[1], vs[0], vs[1], n, start.data_ptr(),
+          pos.data_ptr(), max_new, cos, sin, n_pos, rot, qp, Hq, qr, qh, qo, _stream(k))
     return q_out
 
 
@@ -204,25 +230,25 @@ def paged_attn(cache, q, start, pos, max_new, scale=None, window=0, out=None, ls
     paged_attn_workspace that the caller keeps (allocated for the call when not given)."""
     pool, tail, table = cache.pool, cache.tail, cache.table
     dt = tail.dtype
-    _need_cuda('paged_attn', q, start, pos)
     B = _rows('paged_attn', cache, start, pos)
-    _heads('paged_attn', cache, q, dt)
-    n, Hq, dh = q.shape
-    H = pool.shape[1]
+    qshape, qs = _heads('paged_attn', cache, q, dt)
+    n, Hq, dh = qshape
+    n_pages, H, _ = pool.shape
     if out is None:
-        out = torch.empty(n, Hq, dh, device=q.device, dtype=dt)
+        out = torch.empty(qshape, device=q.device, dtype=dt)
+        os = (Hq * dh, dh)
     else:
-        _heads('paged_attn', cache, out, dt)
-        if out.shape != q.shape:
+        oshape, os = _heads('paged_attn', cache, out, dt)
+        if oshape != qshape:
             raise ValueError('paged_attn: out must have q\'s shape')
-    if lse is not None and (lse.shape != (n, Hq) or lse.dtype != torch.float32 or not lse.is_contiguous()):
+    if lse is not None and (lse.shape != (n, Hq) or lse.dtype is not torch.float32 or not lse.is_contiguous()):
         raise ValueError('paged_attn: lse must be (n, n_head) fp32, contiguous')
     if ws is None:
         ws = paged_attn_workspace(B, Hq, H, dh, max_new, q.device)
-    _lib.call('ta_paged_attn', pool.data_ptr(), tail.data_ptr(), table.data_ptr(), table.stride(0), pool.shape[0],
-              table.shape[1], cache.page, _DT[dt], B, Hq, H, dh, q.data_ptr(), q.stride(0), q.stride(1), n, start.data_ptr(),
-              pos.data_ptr(), int(max_new), 1.0 / math.sqrt(dh) if scale is None else float(scale), int(window),
-              out.data_ptr(), out.stride(0), out.stride(1), _p(lse), ws.data_ptr(), ws.numel(), _stream(q))
+    _call('ta_paged_attn', pool.data_ptr(), tail.data_ptr(), table.data_ptr(), table.stride(0), n_pages, table.shape[1],
+          cache.page, _DT[dt], B, Hq, H, dh, q.data_ptr(), qs[0], qs[1], n, start.data_ptr(), pos.data_ptr(), max_new,
+          1.0 / math.sqrt(dh) if scale is None else scale, window, out.data_ptr(), os[0], os[1], _p(lse), ws.data_ptr(),
+          ws.nbytes, _stream(q))
     return out
 
 
@@ -232,23 +258,25 @@ def verify_drafts(p, q, drafts, u, n_draft=None):
     (B, G + 1) fp32 uniform in [0, 1) (one for each draft, the last for the draw), n_draft (B,) int32 the drafts of each sequence (all G when None). Returns tokens
     (B, G + 1) int64 - the drafts that stand, the token drawn after them, then -1 - and accepted (B,) int32. The output is
     distributed as sampling from p, whatever q is."""
-    _need_cuda('verify_drafts', p, q, drafts, u, n_draft)
-    if p.dim() != 3 or q.dim() != 3 or q.shape != (p.shape[0], p.shape[1] - 1, p.shape[2]):
+    pshape, qshape, ps, qs, dt = p.shape, q.shape, p.stride(), q.stride(), p.dtype
+    if len(qshape) != 3 or pshape != (qshape[0], qshape[1] + 1, qshape[2]):
         raise ValueError('verify_drafts: p (B, G + 1, V) and q (B, G, V)')
-    B, G, V = q.shape
-    if p.dtype != q.dtype or p.dtype not in _DT:
+    B, G, V = qshape
+    if dt is not q.dtype or dt not in _DT:
         raise TypeError('verify_drafts: p and q must share float32, bfloat16 or float16')
-    if p.stride(2) != 1 or (G and q.stride(2) != 1):
+    if ps[2] != 1 or (G and qs[2] != 1):
         raise ValueError('verify_drafts: the innermost (vocabulary) dimension must be contiguous')
-    if drafts.shape != (B, G) or drafts.dtype != torch.int64 or not drafts.is_contiguous():
+    if drafts.shape != (B, G) or drafts.dtype is not torch.int64 or not drafts.is_contiguous():
         raise ValueError('verify_drafts: drafts must be (B, G) int64, contiguous')
-    if u.shape != (B, G + 1) or u.dtype != torch.float32 or not u.is_contiguous():
+    if u.shape != (B, G + 1) or u.dtype is not torch.float32 or not u.is_contiguous():
         raise ValueError('verify_drafts: u must be (B, G + 1) fp32, contiguous')
-    if n_draft is not None and (n_draft.shape != (B,) or n_draft.dtype != torch.int32 or not n_draft.is_contiguous()):
+    if n_draft is not None and (n_draft.shape != (B,) or n_draft.dtype is not torch.int32 or not n_draft.is_contiguous()):
         raise ValueError('verify_drafts: n_draft must be (B,) int32, contiguous')
-    tokens = torch.empty(B, G + 1, device=p.device, dtype=torch.int64)
-    accepted = torch.empty(B, device=p.device, dtype=torch.int32)
-    _lib.call('ta_verify_drafts', p.data_ptr(), p.stride(0), p.stride(1), q.data_ptr(), q.stride(0), q.stride(1),
-              _DT[p.dtype], B, G, V, drafts.data_ptr(), u.data_ptr(), _p(n_draft), tokens.data_ptr(), accepted.data_ptr(),
-              _stream(p))
+    if not (p.is_cuda and q.is_cuda and drafts.is_cuda and u.is_cuda):
+        _need_cuda('verify_drafts', p, q, drafts, u)
+    _need_cuda('verify_drafts', n_draft)
+    tokens = torch.empty((B, G + 1), device=p.device, dtype=torch.int64)
+    accepted = torch.empty((B,), device=p.device, dtype=torch.int32)
+    _call('ta_verify_drafts', p.data_ptr(), ps[0], ps[1], q.data_ptr(), qs[0], qs[1], _DT[dt], B, G, V, drafts.data_ptr(),
+          u.data_ptr(), _p(n_draft), tokens.data_ptr(), accepted.data_ptr(), _stream(p))
     return tokens, accepted
