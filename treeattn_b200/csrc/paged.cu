@@ -43,18 +43,17 @@ int check_cache(const char* who, const void* pool, const void* tail, const int32
 
 template <typename T, int DH>
 int run_append(const ta::AppendParams& a, int B, cudaStream_t st) {
-  const int P = a.c.P;
-  const int n_page = (a.max_new - 1) / P + 2;  // pages that one sequence's new tokens can touch
-  if ((int64_t)n_page * a.c.Hkv > INT_MAX / 2) return fail(TA_ERR_ARG, "ta_paged_append: too many pages in one call");
+  const int64_t spans = (a.max_new - 1) / ta::APPEND_SPAN + 2;  // that one sequence's new tokens can touch
+  if (spans * a.c.Hkv > INT_MAX / 2 || (int64_t)a.max_new * a.Hq * DH > INT_MAX)
+    return fail(TA_ERR_ARG, "ta_paged_append: too many rows of one sequence in a call");
   ta::AppendParams p = a;
-  p.page_ctas = n_page * a.c.Hkv;
+  p.page_ctas = (int)spans * a.c.Hkv;
   int q_ctas = 0;
-  if (a.q_out) {
-    const int64_t work = ((int64_t)a.max_new * a.Hq * (DH - a.rot / 2) + ta::APPEND_THREADS * 4 - 1) / (ta::APPEND_THREADS * 4);
-    q_ctas = (int)std::min<int64_t>(work, std::max(1, 148 * 16 / std::max(B, 1)));
+  if (a.q_out) {  // four 16-byte pieces to a thread, as far as that fills the GPU
+    const int64_t work = ((int64_t)a.max_new * a.Hq * (DH / 8) + ta::APPEND_THREADS * 4 - 1) / (ta::APPEND_THREADS * 4);
+    q_ctas = (int)std::min<int64_t>(work, std::max(1, sm_count() * 32 / std::max(B, 1)));
   }
-  const size_t smem = (size_t)2 * P * (DH + 8) * 2;
-  p.c = a.c;
+  const size_t smem = (size_t)2 * ta::APPEND_SPAN * (DH + 8) * 2;
   ta::paged_append_kernel<T, DH><<<dim3(p.page_ctas + q_ctas, B), ta::APPEND_THREADS, smem, st>>>(p);
   return check_launch("ta_paged_append");
 }

@@ -72,8 +72,32 @@ __device__ __forceinline__ bool new_rows(const int32_t* start, const int32_t* po
   return true;
 }
 
+template <int BYTES>
+__device__ __forceinline__ void load_words(const void* p, uint32_t (&w)[BYTES / 4]) {
+  if constexpr (BYTES >= 16) {
+#pragma unroll
+    for (int i = 0; i < BYTES / 16; ++i) {
+      const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+      w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+    }
+  } else if constexpr (BYTES == 8) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x; w[1] = v.y;
+  } else {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  }
+}
+template <int BYTES>
+__device__ __forceinline__ void store_words(void* p, const uint32_t (&w)[BYTES / 4]) {
+  if constexpr (BYTES == 16)
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  else if constexpr (BYTES == 8)
+    *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+  else
+    *reinterpret_cast<uint32_t*>(p) = w[0];
+}
+
 // ------------------------------------------------------------------------------------------------ append
-// One CTA per (sequence, page that its new tokens reach, kv head), and CTAs for the rotation of the queries.
 //   y1 = x1 cos - x2 sin, y2 = x2 cos + x1 sin   (dims i and i + rot / 2; products and sums rounded one by one in fp32)
 // rounded once to the 16-bit type: what the tail holds and what a full page is quantised from.
 //   scale = top / 448, code = e4m3(x * (448 / top)), top = the largest magnitude of the page's P x DH values.
@@ -90,7 +114,7 @@ struct AppendParams {
   const float *cosv, *sinv;  // (n_pos, rot / 2)
   int n_pos, rot;
   int n_rows, max_new, Hq;
-  int page_ctas;  // CTAs of a sequence that take pages; the others rotate queries
+  int page_ctas;  // CTAs of a sequence that take keys and values; the others rotate queries
 };
 
 // Largest magnitude as the bit pattern of the 16-bit type (ordered like the values, infinities and NaN on top).
@@ -109,12 +133,39 @@ __device__ __forceinline__ uint16_t fp8x2(float lo, float hi) {
   return r;
 }
 
+// Eight elements of one row rotated against the eight half_rot further on.
+template <typename T>
+__device__ __forceinline__ void rotate8(uint4& a, uint4& b, const float* cosv, const float* sinv) {
+  float x[8], y[8], c[8], s[8];
+  load_vec_f32<T>(reinterpret_cast<const T*>(&a), x);
+  load_vec_f32<T>(reinterpret_cast<const T*>(&b), y);
+#pragma unroll
+  for (int i = 0; i < 8; i += 4) {
+    ldg_vec_f32<float>(cosv + i, c + i);
+    ldg_vec_f32<float>(sinv + i, s + i);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float u = __fsub_rn(__fmul_rn(x[i], c[i]), __fmul_rn(y[i], s[i]));
+    y[i] = __fadd_rn(__fmul_rn(y[i], c[i]), __fmul_rn(x[i], s[i]));
+    x[i] = u;
+  }
+  store_vec_from_f32<T>(reinterpret_cast<T*>(&a), x);
+  store_vec_from_f32<T>(reinterpret_cast<T*>(&b), y);
+}
+
+// 64 positions (64 / P pages) of one (sequence, kv head) per CTA, and CTAs for the rotation of the queries. The rows come
+// in 16-byte pieces, eight elements and their partners to a thread; they meet in shared memory, a warp finds the largest
+// magnitudes of its 16 tokens, and the codes leave in 16-byte pieces of the page's order. HBM-bound for prompts (4 x 8192
+// tokens, 12 heads of 64: 41 us, 6.1 TB/s), launch-bound for single tokens.
+constexpr int APPEND_SPAN = 64;
+
 template <typename T, int DH>
 __global__ void __launch_bounds__(APPEND_THREADS) paged_append_kernel(AppendParams p) {
   using S = PageShape<DH>;
   constexpr int PITCH = DH + 8;  // shared rows: a fragment's 8 tokens fall on distinct banks
   extern __shared__ __align__(16) unsigned char append_smem[];
-  __shared__ uint32_t tops[2][APPEND_THREADS / 32];
+  __shared__ uint32_t tops[2][APPEND_SPAN / 16];
   const int b = blockIdx.y, tid = threadIdx.x;
   NewRows nr;
   if (!new_rows(p.start, p.pos, b, p.n_rows, p.max_new, p.c, K_PAGED_APPEND, nr) || nr.n == 0) return;
@@ -123,162 +174,219 @@ __global__ void __launch_bounds__(APPEND_THREADS) paged_append_kernel(AppendPara
     if (tid == 0) record_error(DEV_POS_RANGE, K_PAGED_APPEND, b, nr.pos + nr.n);
     return;
   }
+  const bool vec = half_rot % 8 == 0;  // pairs by eight
   if ((int)blockIdx.x >= p.page_ctas) {
-    // queries: pairs (or single elements beyond rot), consecutive threads on consecutive dims
+    // ---- queries
     const int cta = blockIdx.x - p.page_ctas, n_cta = gridDim.x - p.page_ctas;
-    const int per_head = DH - half_rot;  // half_rot pairs and DH - rot single elements
-    const int64_t total = (int64_t)nr.n * p.Hq * per_head;
-    for (int64_t id = (int64_t)cta * APPEND_THREADS + tid; id < total; id += (int64_t)n_cta * APPEND_THREADS) {
-      const int i = (int)(id % per_head);
-      const int64_t rh = id / per_head;
-      const int h = (int)(rh % p.Hq), r = (int)(rh / p.Hq);
-      const T* src = reinterpret_cast<const T*>(p.q) + (int64_t)(nr.row0 + r) * p.q_sr + (int64_t)h * p.q_sh;
-      T* dst = reinterpret_cast<T*>(p.q_out) + ((int64_t)(nr.row0 + r) * p.Hq + h) * DH;
-      if (i < half_rot) {
-        const int64_t at = (int64_t)(nr.pos + r) * half_rot + i;
-        const float c = p.cosv[at], s = p.sinv[at], x1 = to_f32(src[i]), x2 = to_f32(src[i + half_rot]);
+    const T* q = reinterpret_cast<const T*>(p.q);
+    T* o = reinterpret_cast<T*>(p.q_out);
+    const int pairs = vec ? half_rot / 8 : half_rot;           // pieces (or single elements) with a partner
+    const int per = pairs + (vec ? (DH - p.rot) / 8 : DH - p.rot);  // of a row and head
+    const int total = nr.n * p.Hq * per;
+    for (int id = cta * APPEND_THREADS + tid; id < total; id += n_cta * APPEND_THREADS) {
+      const int i = id % per, rh = id / per, h = rh % p.Hq, r = rh / p.Hq;
+      const T* src = q + (int64_t)(nr.row0 + r) * p.q_sr + (int64_t)h * p.q_sh;
+      T* dst = o + ((int64_t)(nr.row0 + r) * p.Hq + h) * DH;
+      const int64_t at = (int64_t)(nr.pos + r) * half_rot;
+      if (vec) {
+        const int d = i < pairs ? i * 8 : p.rot + (i - pairs) * 8;
+        uint4 x = __ldg(reinterpret_cast<const uint4*>(src + d));
+        if (i < pairs) {
+          uint4 y = __ldg(reinterpret_cast<const uint4*>(src + d + half_rot));
+          rotate8<T>(x, y, p.cosv + at + d, p.sinv + at + d);
+          *reinterpret_cast<uint4*>(dst + d + half_rot) = y;
+        }
+        *reinterpret_cast<uint4*>(dst + d) = x;
+      } else if (i < pairs) {
+        const float c = p.cosv[at + i], s = p.sinv[at + i], x1 = to_f32(src[i]), x2 = to_f32(src[i + half_rot]);
         dst[i] = from_f32<T>(__fsub_rn(__fmul_rn(x1, c), __fmul_rn(x2, s)));
         dst[i + half_rot] = from_f32<T>(__fadd_rn(__fmul_rn(x2, c), __fmul_rn(x1, s)));
       } else {
-        dst[i + half_rot] = src[i + half_rot];
+        dst[p.rot + i - pairs] = src[p.rot + i - pairs];
       }
     }
     return;
   }
-  const int P = p.c.P, h = blockIdx.x % p.c.Hkv;
+  // ---- keys and values
+  const int P = p.c.P, lp = 31 - __clz(P), h = blockIdx.x % p.c.Hkv;
   const int end = nr.pos + nr.n;
-  const int j = nr.pos / P + (int)blockIdx.x / p.c.Hkv;  // page
-  if (j * P >= end) return;
-  const bool full = (j + 1) * P <= end;
+  const int base = (nr.pos / APPEND_SPAN + (int)blockIdx.x / p.c.Hkv) * APPEND_SPAN;  // position of shared row 0
+  if (base >= end) return;
+  const int f = nr.pos >> lp, last = (end - 1) >> lp;  // first and last page with new tokens
+  const int j0 = base >> lp;                           // first page of this CTA
+  const int full_end = min(end >> lp << lp, base + APPEND_SPAN) - base;  // rows below this are of full pages
+  const int i0 = max(nr.pos - base, 0), i1 = min(end - base, APPEND_SPAN);  // rows with new tokens
   // The last two pages stay in 16 bits. Where the first page has earlier tokens in the tail, pages from the second after it
-  // on may share its slots: its own CTA, which reads those tokens, writes the later pages there after that.
-  const int f = nr.pos / P, last = (end - 1) / P;
-  const bool shares = nr.pos % P != 0 && j >= f + 2;
-  const bool keep = j >= last - 1 && !shares;
-  if (!full && shares) return;
-  const int i0 = max(nr.pos - j * P, 0), i1 = min(end - j * P, P);  // the page's new tokens
+  // on may share its slots: the CTA that reads those tokens writes the later pages there after that.
+  const bool old = (nr.pos & (P - 1)) != 0, reader = f >= j0 && f < j0 + (APPEND_SPAN >> lp);
+  const int keep = max((last - 1) * P - base, i0);  // rows from here on go to the tail
+  const bool keeps = keep < i1 && (!old || reader || last < f + 2 || j0 + (APPEND_SPAN >> lp) <= f + 2);
   T* sk = reinterpret_cast<T*>(append_smem);
-  T* sv = sk + P * PITCH;
-  T* tk = reinterpret_cast<T*>(p.c.tail) + ((((int64_t)b * p.c.Hkv + h) * 2 + (j & 1)) * 2) * ((int64_t)P * DH);
-  T* tv = tk + (int64_t)P * DH;
-  // the page's tokens, token-major: new rows from the projection, earlier ones (of a page that is now full) from the tail
+  T* sv = sk + APPEND_SPAN * PITCH;
+  T* tail = reinterpret_cast<T*>(p.c.tail) + ((int64_t)b * p.c.Hkv + h) * 4 * ((int64_t)P * DH);
+  auto tail_k = [&](int page) { return tail + (page & 1) * 2 * ((int64_t)P * DH); };
+  const T* kr = reinterpret_cast<const T*>(p.k) + (int64_t)h * p.k_sh;
+  const T* vr = reinterpret_cast<const T*>(p.v) + (int64_t)h * p.v_sh;
   constexpr int VPR = DH / 8;
-  for (int id = tid; id < (i1 - i0) * VPR; id += APPEND_THREADS) {
-    const int i = i0 + id / VPR, d = (id % VPR) * 8;
-    const int64_t row = nr.row0 + (j * P + i - nr.pos);
-    *reinterpret_cast<uint4*>(sk + i * PITCH + d) =
-        *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.k) + row * p.k_sr + h * p.k_sh + d);
-    *reinterpret_cast<uint4*>(sv + i * PITCH + d) =
-        *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.v) + row * p.v_sr + h * p.v_sh + d);
-  }
-  if (full) {
-    for (int id = tid; id < i0 * DH; id += APPEND_THREADS) {
+  // rows [r0, r1) of the span at position `from` into shared memory, keys rotated
+  auto load_rows = [&](int from, int r0, int r1) {
+    const int64_t row = (int64_t)nr.row0 + from - nr.pos;
+    if (!half_rot) {
+#pragma unroll 4
+      for (int id = tid; id < (r1 - r0) * VPR; id += APPEND_THREADS) {
+        const int i = r0 + id / VPR, d = id % VPR * 8;
+        *reinterpret_cast<uint4*>(sk + i * PITCH + d) = __ldg(reinterpret_cast<const uint4*>(kr + (row + i) * p.k_sr + d));
+        *reinterpret_cast<uint4*>(sv + i * PITCH + d) = __ldg(reinterpret_cast<const uint4*>(vr + (row + i) * p.v_sr + d));
+      }
+      return;
+    }
+    if (vec) {
+      const int pairs = half_rot / 8, per = VPR - pairs;
+#pragma unroll 4
+      for (int id = tid; id < (r1 - r0) * per; id += APPEND_THREADS) {
+        const int i = r0 + id / per, c = id % per;
+        const int d = c < pairs ? c * 8 : p.rot + (c - pairs) * 8;
+        const T* src = kr + (row + i) * p.k_sr;
+        uint4 x = __ldg(reinterpret_cast<const uint4*>(src + d));
+        if (c < pairs) {
+          uint4 y = __ldg(reinterpret_cast<const uint4*>(src + d + half_rot));
+          const int64_t at = (int64_t)(from + i) * half_rot + d;
+          rotate8<T>(x, y, p.cosv + at, p.sinv + at);
+          *reinterpret_cast<uint4*>(sk + i * PITCH + d + half_rot) = y;
+        }
+        *reinterpret_cast<uint4*>(sk + i * PITCH + d) = x;
+      }
+    } else {
+      for (int id = tid; id < (r1 - r0) * (DH - half_rot); id += APPEND_THREADS) {
+        const int i = r0 + id / (DH - half_rot), d = id % (DH - half_rot);
+        const T* src = kr + (row + i) * p.k_sr;
+        if (d < half_rot) {
+          const int64_t at = (int64_t)(from + i) * half_rot + d;
+          const float c = p.cosv[at], s = p.sinv[at], x1 = to_f32(src[d]), x2 = to_f32(src[d + half_rot]);
+          sk[i * PITCH + d] = from_f32<T>(__fsub_rn(__fmul_rn(x1, c), __fmul_rn(x2, s)));
+          sk[i * PITCH + d + half_rot] = from_f32<T>(__fadd_rn(__fmul_rn(x2, c), __fmul_rn(x1, s)));
+        } else {
+          sk[i * PITCH + d + half_rot] = src[d + half_rot];
+        }
+      }
+    }
+#pragma unroll 4
+    for (int id = tid; id < (r1 - r0) * VPR; id += APPEND_THREADS) {
+      const int i = r0 + id / VPR, d = id % VPR * 8;
+      *reinterpret_cast<uint4*>(sv + i * PITCH + d) = __ldg(reinterpret_cast<const uint4*>(vr + (row + i) * p.v_sr + d));
+    }
+  };
+  // ... and from there into the tail
+  auto keep_rows = [&](int from, int r0, int r1) {
+    for (int id = tid; id < (r1 - r0) * DH; id += APPEND_THREADS) {
+      const int r = r0 + id / DH, d = id % DH, i = (from + r) & (P - 1);
+      T* ok = tail_k((from + r) >> lp) + (i >> 4) * 16 * DH;
+      ok[key_offset<DH>(i & 15, d)] = sk[r * PITCH + d];
+      ok[(int64_t)P * DH + value_offset<DH>(i & 15, d)] = sv[r * PITCH + d];
+    }
+  };
+  if (full_end > i0 || keeps) load_rows(base, i0, i1);
+  if (reader && old && ((f + 1) << lp) <= end) {  // the first page's earlier tokens
+    const T* ok = tail_k(f);
+    const int r0 = (f << lp) - base;
+    for (int id = tid; id < (nr.pos & (P - 1)) * DH; id += APPEND_THREADS) {
       const int i = id / DH, d = id % DH;
-      sk[i * PITCH + d] = tk[(i >> 4) * 16 * DH + key_offset<DH>(i & 15, d)];
-      sv[i * PITCH + d] = tv[(i >> 4) * 16 * DH + value_offset<DH>(i & 15, d)];
+      sk[(r0 + i) * PITCH + d] = ok[(i >> 4) * 16 * DH + key_offset<DH>(i & 15, d)];
+      sv[(r0 + i) * PITCH + d] = ok[(int64_t)P * DH + (i >> 4) * 16 * DH + value_offset<DH>(i & 15, d)];
     }
   }
   __syncthreads();
-  if (half_rot) {
-    for (int id = tid; id < (i1 - i0) * half_rot; id += APPEND_THREADS) {
-      const int i = i0 + id / half_rot, d = id % half_rot;
-      const int64_t at = (int64_t)(j * P + i) * half_rot + d;
-      const float c = p.cosv[at], s = p.sinv[at];
-      const float x1 = to_f32(sk[i * PITCH + d]), x2 = to_f32(sk[i * PITCH + d + half_rot]);
-      sk[i * PITCH + d] = from_f32<T>(__fsub_rn(__fmul_rn(x1, c), __fmul_rn(x2, s)));
-      sk[i * PITCH + d + half_rot] = from_f32<T>(__fadd_rn(__fmul_rn(x2, c), __fmul_rn(x1, s)));
-    }
-    __syncthreads();
-  }
-  if (keep) {
-    for (int id = tid; id < (i1 - i0) * DH; id += APPEND_THREADS) {
-      const int i = i0 + id / DH, d = id % DH;
-      tk[(i >> 4) * 16 * DH + key_offset<DH>(i & 15, d)] = sk[i * PITCH + d];
-      tv[(i >> 4) * 16 * DH + value_offset<DH>(i & 15, d)] = sv[i * PITCH + d];
-    }
-  }
-  if (!full) return;
-  if (j == f && nr.pos % P != 0) {
-    // (the earlier tokens are in shared memory since the barrier after their loads)
-    for (int jj = max(f + 2, last - 1); jj <= last; ++jj) {
-      T* ok = reinterpret_cast<T*>(p.c.tail) + ((((int64_t)b * p.c.Hkv + h) * 2 + (jj & 1)) * 2) * ((int64_t)P * DH);
-      T* ov = ok + (int64_t)P * DH;
-      const int n = min(end - jj * P, P);
-      for (int id = tid; id < n * DH; id += APPEND_THREADS) {
-        const int i = id / DH, d = id % DH;
-        const int64_t row = nr.row0 + (jj * P + i - nr.pos);
-        const T* kr = reinterpret_cast<const T*>(p.k) + row * p.k_sr + h * p.k_sh;
-        const T* vr = reinterpret_cast<const T*>(p.v) + row * p.v_sr + h * p.v_sh;
-        T y = kr[d];
-        if (d < p.rot) {
-          const bool lo = d < half_rot;
-          const int64_t at = (int64_t)(jj * P + i) * half_rot + (lo ? d : d - half_rot);
-          const float c = p.cosv[at], s = p.sinv[at], x = to_f32(y), o = to_f32(kr[lo ? d + half_rot : d - half_rot]);
-          y = from_f32<T>(lo ? __fsub_rn(__fmul_rn(x, c), __fmul_rn(o, s)) : __fadd_rn(__fmul_rn(x, c), __fmul_rn(o, s)));
+  if (keeps) keep_rows(base, keep, i1);
+  // ---- full pages: rows [g0 * 16, full_end), whole groups of 16 tokens
+  const int g0 = max((f << lp) - base, 0) >> 4, g1 = full_end >> 4;
+  if (g1 <= g0) return;
+  {
+    const int warp = tid >> 5, lane = tid & 31;
+    if (warp >= g0 && warp < g1) {
+      uint32_t mk = 0, mv = 0;
+      for (int id = lane; id < 16 * VPR; id += 32) {
+        const int at = (warp * 16 + id / VPR) * PITCH + (id % VPR) * 8;
+        const uint4 a = *reinterpret_cast<const uint4*>(sk + at), w = *reinterpret_cast<const uint4*>(sv + at);
+        const uint32_t ka[4] = {a.x, a.y, a.z, a.w}, va[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          mk = max(mk, max(ka[x] & 0x7fffu, (ka[x] >> 16) & 0x7fffu));
+          mv = max(mv, max(va[x] & 0x7fffu, (va[x] >> 16) & 0x7fffu));
         }
-        ok[(i >> 4) * 16 * DH + key_offset<DH>(i & 15, d)] = y;
-        ov[(i >> 4) * 16 * DH + value_offset<DH>(i & 15, d)] = vr[d];
+      }
+      mk = __reduce_max_sync(0xffffffffu, mk);
+      mv = __reduce_max_sync(0xffffffffu, mv);
+      if (lane == 0) {
+        tops[0][warp] = mk;
+        tops[1][warp] = mv;
       }
     }
   }
-  uint32_t mk = 0, mv = 0;
-  for (int id = tid; id < P * VPR; id += APPEND_THREADS) {
-    const int at = (id / VPR) * PITCH + (id % VPR) * 8;
-    const uint4 a = *reinterpret_cast<const uint4*>(sk + at), w = *reinterpret_cast<const uint4*>(sv + at);
-    const uint32_t ka[4] = {a.x, a.y, a.z, a.w}, va[4] = {w.x, w.y, w.z, w.w};
+  __syncthreads();
+  const int gpp = P >> 4;  // groups of a page
+#pragma unroll 1
+  for (int pg = g0; pg < g1; pg += gpp) {
+    const int j = (base >> lp) + (pg >> (lp - 4));
+    const int phys = p.c.table[b * p.c.table_sb + j];
+    if (phys < 0 || phys >= p.c.n_pages) {
+      if (tid == 0) record_error(DEV_INDEX_RANGE, K_PAGED_APPEND, b, phys);
+      continue;
+    }
+    float mul[2], scale[2];
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      mk = max(mk, max(ka[x] & 0x7fffu, (ka[x] >> 16) & 0x7fffu));
-      mv = max(mv, max(va[x] & 0x7fffu, (va[x] >> 16) & 0x7fffu));
+    for (int x = 0; x < 2; ++x) {
+      uint32_t bits = 0;
+      for (int g = 0; g < gpp; ++g) bits = max(bits, tops[x][pg + g]);
+      const float top = bits_value<T>(bits);
+      const bool odd = !(top <= 3.402823466e38f), tiny = top < 7.888609052e-31f;  // 2^-100
+      mul[x] = odd || tiny ? 0.f : __fdiv_rn(448.f, top);
+      scale[x] = odd ? __int_as_float(0x7fc00000) : (tiny ? 1.f : __fdiv_rn(top, 448.f));
+    }
+    unsigned char* rec = p.c.pool + ((int64_t)phys * p.c.Hkv + h) * (2 * P * DH + 16);
+    if (tid == 0) *reinterpret_cast<float2*>(rec + 2 * P * DH) = make_float2(scale[0], scale[1]);
+    // a page with a non-finite element has codes 0 (0 * NaN would not be)
+    const bool zk = mul[0] == 0.f, zv = mul[1] == 0.f;
+    for (int id = tid; id < P * DH / S::E; id += APPEND_THREADS) {
+      // keys: E consecutive dims of one token
+      const int t = id % 4, g = id / 4 % 8, r = id / 32 % 2, hg = id / 64 % S::HG, grp = id / (64 * S::HG);
+      const T* a = sk + ((pg + grp) * 16 + r * 8 + g) * PITCH + (hg * 4 + t) * S::E;
+      uint32_t w[S::E / 4];
+#pragma unroll
+      for (int e = 0; e < S::E / 4; ++e) {
+        uint32_t two[2];
+        load_words<8>(a + e * 4, two);
+        w[e] = zk ? 0u
+                  : fp8x2(bits_value<T>(two[0] & 0xffffu) * mul[0], bits_value<T>(two[0] >> 16) * mul[0]) |
+                        ((uint32_t)fp8x2(bits_value<T>(two[1] & 0xffffu) * mul[0], bits_value<T>(two[1] >> 16) * mul[0]) << 16);
+      }
+      store_words<S::E>(rec + (int64_t)id * S::E, w);
+    }
+    for (int id = tid; id < P * DH / (8 * S::M); id += APPEND_THREADS) {
+      // values: 2 M dims (8 apart) of 4 tokens
+      const int t = id % 4, g = id / 4 % 8, c = id / 32 % S::C, grp = id / (32 * S::C);
+      const T* a = sv + ((pg + grp) * 16 + 2 * t) * PITCH + c * S::M * 16 + g;
+      uint32_t w[2 * S::M];
+#pragma unroll
+      for (int x = 0; x < 2 * S::M; ++x) {
+        const T* v0 = a + x * 8;
+        w[x] = zv ? 0u
+                  : fp8x2(to_f32(v0[0]) * mul[1], to_f32(v0[PITCH]) * mul[1]) |
+                        ((uint32_t)fp8x2(to_f32(v0[8 * PITCH]) * mul[1], to_f32(v0[9 * PITCH]) * mul[1]) << 16);
+      }
+      store_words<8 * S::M>(rec + P * DH + (int64_t)id * 8 * S::M, w);
     }
   }
-  mk = __reduce_max_sync(0xffffffffu, mk);
-  mv = __reduce_max_sync(0xffffffffu, mv);
-  if ((tid & 31) == 0) {
-    tops[0][tid >> 5] = mk;
-    tops[1][tid >> 5] = mv;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < APPEND_THREADS / 32; ++w) {
-    mk = max(mk, tops[0][w]);
-    mv = max(mv, tops[1][w]);
-  }
-  const int phys = j < p.c.max_pages ? p.c.table[b * p.c.table_sb + j] : -1;
-  if (phys < 0 || phys >= p.c.n_pages) {
-    if (tid == 0) record_error(DEV_INDEX_RANGE, K_PAGED_APPEND, b, phys);
-    return;
-  }
-  float mul[2], scale[2];
-#pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    const float top = bits_value<T>(x ? mv : mk);
-    const bool odd = !(top <= 3.402823466e38f), tiny = top < 7.888609052e-31f;  // 2^-100
-    mul[x] = odd || tiny ? 0.f : __fdiv_rn(448.f, top);
-    scale[x] = odd ? __int_as_float(0x7fc00000) : (tiny ? 1.f : __fdiv_rn(top, 448.f));
-  }
-  unsigned char* rec = p.c.pool + ((int64_t)phys * p.c.Hkv + h) * (2 * P * DH + 16);
-  if (tid == 0) {
-    reinterpret_cast<float*>(rec + 2 * P * DH)[0] = scale[0];
-    reinterpret_cast<float*>(rec + 2 * P * DH)[1] = scale[1];
-  }
-  // a page with a non-finite element has codes 0 (0 * NaN would not be)
-  const bool zk = mul[0] == 0.f, zv = mul[1] == 0.f;
-  for (int id = tid; id < P * DH / 4; id += APPEND_THREADS) {
-    // keys: 4 consecutive dims of one token
-    const int grp = id / (4 * DH), o = (id % (4 * DH)) * 4;  // offset in the group's 16 * DH elements
-    const int e = o % S::E, t = (o / S::E) % 4, g = (o / (4 * S::E)) % 8, r = (o / (32 * S::E)) % 2, hg = o / (64 * S::E);
-    const T* a = sk + (grp * 16 + r * 8 + g) * PITCH + hg * 4 * S::E + t * S::E + e;
-    uint32_t w = fp8x2(to_f32(a[0]) * mul[0], to_f32(a[1]) * mul[0]) |
-                 ((uint32_t)fp8x2(to_f32(a[2]) * mul[0], to_f32(a[3]) * mul[0]) << 16);
-    reinterpret_cast<uint32_t*>(rec)[id] = zk ? 0u : w;
-    // values: one dim of 4 tokens
-    const int x = o / 4, vr = x % 2, m = (x / 2) % S::M, vt = (x / (2 * S::M)) % 4, vg = (x / (8 * S::M)) % 8,
-              c = x / (64 * S::M);
-    const T* v0 = sv + (grp * 16 + 2 * vt) * PITCH + (c * S::M + m) * 16 + vr * 8 + vg;
-    w = fp8x2(to_f32(v0[0]) * mul[1], to_f32(v0[PITCH]) * mul[1]) |
-        ((uint32_t)fp8x2(to_f32(v0[8 * PITCH]) * mul[1], to_f32(v0[9 * PITCH]) * mul[1]) << 16);
-    reinterpret_cast<uint32_t*>(rec + P * DH)[id] = zv ? 0u : w;
+  if (reader && old && last >= f + 2) {
+    // later pages of other CTAs into the tail (the earlier tokens have been read); the first page is full then, so that no
+    // thread has left above
+    const int from = max(max(last - 1, f + 2) << lp, base + APPEND_SPAN);
+    for (int span = from / APPEND_SPAN * APPEND_SPAN; span < end; span += APPEND_SPAN) {
+      const int r0 = max(from - span, 0), r1 = min(end - span, APPEND_SPAN);
+      __syncthreads();
+      load_rows(span, r0, r1);
+      __syncthreads();
+      keep_rows(span, r0, r1);
+    }
   }
 }
 
@@ -363,22 +471,6 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-template <int BYTES>
-__device__ __forceinline__ void load_words(const void* p, uint32_t (&w)[BYTES / 4]) {
-  if constexpr (BYTES >= 16) {
-#pragma unroll
-    for (int i = 0; i < BYTES / 16; ++i) {
-      const uint4 v = reinterpret_cast<const uint4*>(p)[i];
-      w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
-    }
-  } else if constexpr (BYTES == 8) {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
-    w[0] = v.x; w[1] = v.y;
-  } else {
-    w[0] = *reinterpret_cast<const uint32_t*>(p);
-  }
-}
-
 // The rows of one tile: query fragments and what the masks and scores need, per lane for its two columns of each n-tile.
 template <typename T, int DH, int NT>
 struct RowTile {
