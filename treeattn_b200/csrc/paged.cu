@@ -7,6 +7,7 @@
 #include "../../include/treeattn_b200.h"
 #include "host.cuh"
 #include "paged.cuh"
+#include "paged_tile.cuh"
 #include "verify.cuh"
 
 namespace ta_host {
@@ -110,6 +111,41 @@ int run_split(const ta::AttnParams& p, void* ws, int64_t ws_bytes, cudaStream_t 
   return TA_OK;
 }
 
+// The tile form (head dims 64 and 128): CTAs that share a tile's blocks, as many as make the tiles fill the GPU.
+int64_t tiles_of(int64_t rows) { return (rows + ta::TILE_ROWS - 1) / ta::TILE_ROWS; }
+int tile_splits(int64_t B, int64_t Hkv, int64_t rows, int dh) {
+  const int64_t items = B * Hkv * tiles_of(rows), room = (int64_t)sm_count() * (dh == 64 ? 2 : 1);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(ta::TILE_MAX_SPLITS, room / std::max<int64_t>(1, items)));
+}
+int64_t tile_bytes(int64_t B, int64_t Hkv, int64_t rows, int dh) {
+  const int splits = tile_splits(B, Hkv, rows, dh);
+  if (splits == 1) return 0;
+  const int64_t items = B * Hkv * tiles_of(rows);
+  return counter_bytes(items, 1) + items * splits * ta::TILE_ROWS * (dh + 2) * 4;
+}
+
+template <typename T, int DH>
+int run_tile(const ta::AttnParams& p, int64_t rows, void* ws, int64_t ws_bytes, cudaStream_t st) {
+  using C = ta::TileShape<T, DH>;
+  const int64_t need = tile_bytes(p.B, p.c.Hkv, rows, DH), tiles = tiles_of(rows);
+  if (need > 0 && (!ws || !aligned16(ws) || ws_bytes < need))
+    return fail(TA_ERR_ARG, "ta_paged_attn: a workspace of %lld bytes is needed (16-byte aligned; got %lld)", (long long)need,
+                (long long)ws_bytes);
+  ta::TileParams tp{};
+  tp.a = p;
+  tp.tiles = (int)tiles;
+  tp.splits = tile_splits(p.B, p.c.Hkv, rows, DH);
+  tp.counters = reinterpret_cast<int32_t*>(ws);
+  tp.states = reinterpret_cast<float*>(reinterpret_cast<char*>(ws) + counter_bytes((int64_t)p.B * p.c.Hkv * tiles, 1));
+  static SmemAttr attr;
+  constexpr int smem = 1024 + C::BYTES + (int)sizeof(ta::TileBars);
+  if (int r = allow_smem(attr, ta::paged_tile_kernel<T, DH>, smem, "ta_paged_attn")) return r;
+  const cudaError_t e = launch_pdl(ta::paged_tile_kernel<T, DH>, dim3((unsigned)(tiles * tp.splits), p.c.Hkv, p.B),
+                                   dim3(ta::TILE_THREADS), smem, st, tp);
+  if (e != cudaSuccess) return fail(TA_ERR_CUDA, "ta_paged_attn: launch failed: %s", cudaGetErrorString(e));
+  return TA_OK;
+}
+
 template <typename T, int DH>
 int run_attn(const ta::AttnParams& p, void* ws, int64_t ws_bytes, cudaStream_t st) {
   const int64_t rows = (int64_t)p.max_new * (p.Hq / p.c.Hkv);
@@ -118,6 +154,9 @@ int run_attn(const ta::AttnParams& p, void* ws, int64_t ws_bytes, cudaStream_t s
     if (rows <= 16) return run_split<T, DH, 2>(p, ws, ws_bytes, st);
     if (rows <= 24) return run_split<T, DH, 3>(p, ws, ws_bytes, st);
     return run_split<T, DH, 4>(p, ws, ws_bytes, st);
+  }
+  if constexpr (DH >= 64) {
+    if (rows > kSplitRows) return run_tile<T, DH>(p, rows, ws, ws_bytes, st);
   }
   if (rows <= 8) return run_attn_nt<T, DH, 1>(p, st);
   if (rows <= 16 || DH == 128) return run_attn_nt<T, DH, 2>(p, st);  // 32 rows of head dim 128 do not fit the registers
@@ -184,7 +223,7 @@ int ta_paged_append(void* pool, void* tail, const int32_t* table, int64_t table_
 int64_t ta_paged_attn_workspace(int B, int Hq, int Hkv, int dh, int max_new) {
   if (B < 1 || Hkv < 1 || Hq < Hkv || max_new < 1 || !valid_dh(dh)) return 0;
   const int64_t rows = (int64_t)max_new * (Hq / Hkv);
-  if (rows > kSplitRows) return 0;
+  if (rows > kSplitRows) return dh >= 64 ? tile_bytes(B, Hkv, rows, dh) : 0;
   switch (dh) {
     case 16: return split_bytes_dh<16>(B, Hkv, rows);
     case 32: return split_bytes_dh<32>(B, Hkv, rows);

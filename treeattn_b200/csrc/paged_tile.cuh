@@ -1,0 +1,529 @@
+// Attention over the 8-bit paged cache for many rows of one (sequence, kv head): prompt chunks and long runs of drafts, on
+// the 5th-generation tensor cores. The mathematics and the cache are those of paged.cuh; here the products bound it.
+//
+// A CTA takes 128 rows (query-major: query i, head gq of the group -> row i * group + gq) and runs through 64-token blocks:
+//   warps 4-7  converters: warp w reads the codes of one 16-token group (the next block's are in registers by then), turns
+//              them into f16 and stores them as 128-byte-swizzled tiles: K (64 tokens x DH) and V transposed (DH x 64 tokens),
+//              both K-major operands. A lane's fragment order gives it 32 bytes of a K row and token pairs of V columns, so
+//              neither store meets a bank twice.
+//   warp 8     one thread issues tcgen05.mma: S = Q K^T of block j, then O += P V of block j - 1 (accumulator in tensor
+//              memory), so that the softmax of one block runs beside the products of its neighbours.
+//   warps 0-3  softmax, one thread per row: maximum, weights (f16, into shared memory), denominator; O is rescaled in tensor
+//              memory only when a row's reference has to rise by more than 2^8.
+// The open page is the last block: 16-bit elements as they are, with a copy of the queries in that type.
+// The exponentials bound it at head dim 64 (128 x 64 of them a block at 16 a cycle), the products' issue and the softmax
+// warps' other instructions come next. Where the tiles do not fill the GPU, the blocks of a tile are shared by several
+// CTAs; their states meet in the workspace and the last to come (a counter per tile) joins them.
+#pragma once
+#include <cstddef>
+#include "paged.cuh"
+#include "tc.cuh"
+
+namespace ta {
+
+constexpr int TILE_ROWS = 128;
+constexpr int TILE_KT = 64;
+constexpr int TILE_THREADS = 288;
+constexpr int TILE_MAX_SPLITS = 8;
+constexpr int K_PAGED_TILE = 19;
+
+template <typename T, int DH>
+struct TileShape {
+  static constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
+  static constexpr int NS = 2;                          // K / V stages
+  static constexpr int HALVES = DH / 64;                // 64-dim column blocks of Q and K
+  static constexpr int Q_BYTES = TILE_ROWS * DH * 2;
+  static constexpr int K_BYTES = TILE_KT * DH * 2;      // and of V
+  static constexpr int P_BYTES = TILE_ROWS * TILE_KT * 2;
+  static constexpr int Q2 = BF ? Q_BYTES : 0;           // the queries in bf16, for the open page
+  static constexpr int BYTES = Q_BYTES + Q2 + NS * 2 * K_BYTES + 2 * P_BYTES;
+  static constexpr int CTAS = DH == 64 ? 2 : 1;         // per SM
+  static constexpr int STATE = TILE_ROWS * (DH + 2);    // floats: numerators (4 dims of every row together), maxima, sums
+};
+
+struct TileBars {
+  uint64_t kv_full[2], kv_empty[2], s_full[2], s_free[2], p_full[2], o_full[2], mma_done;
+  alignas(16) float scale[2][4][4];  // per stage and 16-token group: key scale, log2 of the value scale, its inverse
+  uint32_t tmem_base;
+  int abort_flag, last;
+};
+
+static_assert(offsetof(TileBars, scale) % 16 == 0, "the scales are read as float4");
+
+struct TileParams {
+  AttnParams a;
+  int tiles, splits;
+  int32_t* counters;  // (B, Hkv, tiles), zero between launches
+  float* states;      // (B, Hkv, tiles, splits) states
+};
+
+// a 16-byte piece of a swizzled tile's row (128 bytes)
+__device__ __forceinline__ unsigned char* tile_piece(unsigned char* tile, int row, int c) {
+  return tile + row * 128 + ((c ^ (row & 7)) << 4);
+}
+
+template <typename T, int DH>
+__global__ void __launch_bounds__(TILE_THREADS, TileShape<T, DH>::CTAS) paged_tile_kernel(TileParams tp) {
+  using C = TileShape<T, DH>;
+  using S = PageShape<DH>;
+  constexpr int NS = C::NS;
+  constexpr float SHIFT = 6.f, RISE = 8.f;  // weights stay below 2^(SHIFT + RISE) = 2^14
+  constexpr uint32_t TM_S = 0, TM_O = 128, TM_COLS = 256;
+  const AttnParams& p = tp.a;
+  extern __shared__ unsigned char tile_smem_raw[];
+  const uint32_t raw_a = smem_u32(tile_smem_raw);
+  unsigned char* sQ = tile_smem_raw + (((raw_a + 1023u) & ~1023u) - raw_a);
+  unsigned char* sQ2 = C::BF ? sQ + C::Q_BYTES : sQ;
+  unsigned char* sKV = sQ + C::Q_BYTES + C::Q2;
+  unsigned char* sP = sKV + NS * 2 * C::K_BYTES;
+  TileBars& bar = *reinterpret_cast<TileBars*>(sP + 2 * C::P_BYTES);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int split = blockIdx.x % tp.splits, tile = tp.tiles - 1 - (int)(blockIdx.x / tp.splits);  // heavy (late) tiles first
+  const int b = blockIdx.z, h = blockIdx.y, row0 = tile * TILE_ROWS;
+  pdl_wait();
+  pdl_launch_dependents();
+  NewRows nr;
+  if (!new_rows(p.start, p.pos, b, p.n_rows, p.max_new, p.c, K_PAGED_ATTN, nr)) return;
+  const int group = p.Hq / p.c.Hkv, R = nr.n * group, P = p.c.P, lp = 31 - __clz(P);
+  if (row0 >= R) return;
+  const int len = nr.pos + nr.n, n_full = len >> lp;
+  const int qlo = nr.pos + row0 / group, qhi = nr.pos + (min(R, row0 + TILE_ROWS) - 1) / group;
+  const int p0 = (p.window > 0 ? max(0, qlo - p.window + 1) : 0) >> lp, p1 = min(n_full, (qhi >> lp) + 1);
+  const int first_tok = p0 << lp, limit = p1 << lp;
+  const int n_code = (limit - first_tok + TILE_KT - 1) / TILE_KT;              // blocks of full pages
+  const int n_all = n_code + ((n_full << lp) <= qhi ? 1 : 0);                  // and the open page
+  const int j0 = (int)((int64_t)n_all * split / tp.splits), j1 = (int)((int64_t)n_all * (split + 1) / tp.splits);
+  const int nblk = j1 - j0;
+
+  if (tid == 0) {
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&bar.kv_full[s], 4);
+      mbar_init(&bar.kv_empty[s], 1);
+      mbar_init(&bar.s_full[s], 1);
+      mbar_init(&bar.s_free[s], 4);
+      mbar_init(&bar.p_full[s], 4);
+      mbar_init(&bar.o_full[s], 1);
+    }
+    mbar_init(&bar.mma_done, 1);
+    bar.abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 8) {
+    tmem_alloc(&bar.tmem_base, TM_COLS);
+    tmem_relinquish();
+  }
+  // ---- the queries: a thread a row
+  const int rr = row0 + tid;
+  float cs = 1.f;
+  int qpos = -1;
+  if (warp < 4) {
+    uint4 q[DH / 8];
+    const bool live = rr < R;
+    const T* src = reinterpret_cast<const T*>(p.q);
+    if (live) {
+      src += (int64_t)(nr.row0 + rr / group) * p.q_sr + (int64_t)(h * group + rr % group) * p.q_sh;
+      qpos = nr.pos + rr / group;
+    }
+    float top = 0.f;
+#pragma unroll
+    for (int c = 0; c < DH / 8; ++c) q[c] = live ? __ldg(reinterpret_cast<const uint4*>(src) + c) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+    for (int c = 0; c < DH / 8; ++c) {
+      float x[8];
+      load_vec_f32<T>(reinterpret_cast<const T*>(&q[c]), x);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
+    }
+    // as in RowTile: the row's power of two, the sign of the scale, a zero row at scale 0
+    const int ex = min(14 + 127 - (int)(__float_as_uint(top) >> 23), 120);
+    const float up = p.scale == 0.f ? 0.f : copysignf(__int_as_float((ex + 127) << 23), p.scale);
+    cs = p.scale == 0.f ? 1.f : fabsf(p.scale) * 1.4426950408889634f * __int_as_float((127 - ex) << 23);
+#pragma unroll
+    for (int c = 0; c < DH / 8; ++c) {
+      float x[8];
+      load_vec_f32<T>(reinterpret_cast<const T*>(&q[c]), x);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] *= up;
+      const int at = (c >> 3) * TILE_ROWS * 128;
+      store_vec_from_f32<__half>(reinterpret_cast<__half*>(tile_piece(sQ + at, tid, c & 7)), x);
+      if constexpr (C::BF) store_vec_from_f32<T>(reinterpret_cast<T*>(tile_piece(sQ2 + at, tid, c & 7)), x);
+    }
+  }
+  fence_proxy_async_smem();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+
+  if (warp >= 4 && warp < 8) {
+    // ---------------------------------------------------------------- converters
+    const int cw = warp - 4;
+    constexpr int KW = S::HG * 2 * (S::E / 4), VW = S::C * 2 * S::M;  // words of a lane: keys, values
+    const int32_t* table = p.c.table + b * p.c.table_sb;
+    const int64_t rec = 2 * P * DH + 16;
+    const int n_mine = min(j1, n_code) - j0;  // blocks of codes
+    auto entry = [&](int j) {
+      const int page = min(p0 + ((j * TILE_KT + cw * 16) >> lp), p1 - 1);  // beyond the last page: the last again (masked)
+      return table[page];
+    };
+    auto fetch = [&](int j, int phys, uint32_t (&kw)[KW], uint32_t (&vw)[VW], float2& sc) {
+      if (phys < 0 || phys >= p.c.n_pages) {
+        record_error(DEV_INDEX_RANGE, K_PAGED_ATTN, b, phys);
+        phys = 0;
+      }
+      const unsigned char* r = p.c.pool + ((int64_t)phys * p.c.Hkv + h) * rec;
+      const unsigned char* k = r + ((j * TILE_KT + cw * 16) & (P - 1)) * DH;
+      const unsigned char* v = k + P * DH;
+#pragma unroll
+      for (int x = 0; x < KW / 4; ++x) {
+        const uint4 w = __ldg(reinterpret_cast<const uint4*>(k) + x * 32 + lane);
+        kw[4 * x] = w.x; kw[4 * x + 1] = w.y; kw[4 * x + 2] = w.z; kw[4 * x + 3] = w.w;
+      }
+#pragma unroll
+      for (int x = 0; x < VW / 4; ++x) {
+        const uint4 w = __ldg(reinterpret_cast<const uint4*>(v) + x * 32 + lane);
+        vw[4 * x] = w.x; vw[4 * x + 1] = w.y; vw[4 * x + 2] = w.z; vw[4 * x + 3] = w.w;
+      }
+      sc = __ldg(reinterpret_cast<const float2*>(r + 2 * P * DH));
+    };
+    uint32_t kw[KW], vw[VW];
+    float2 sc;
+    int next = 0;
+    if (n_mine > 0) fetch(j0, entry(j0), kw, vw, sc);
+    if (n_mine > 1) next = entry(j0 + 1);
+    bool ok = true;
+    for (int n = 0; n < nblk; ++n) {
+      const int st = n % NS;
+      unsigned char* sK = sKV + st * 2 * C::K_BYTES;
+      unsigned char* sV = sK + C::K_BYTES;
+      uint32_t kn[KW], vn[VW];
+      float2 sn = make_float2(1.f, 1.f);
+      if (n + 1 < n_mine) {
+        fetch(j0 + n + 1, next, kn, vn, sn);
+        if (n + 2 < n_mine) next = entry(j0 + n + 2);
+      }
+      if (n >= NS && !mbar_wait_bounded(&bar.kv_empty[st], ((n / NS) - 1) & 1, K_PAGED_TILE, 1)) {
+        atomicExch(&bar.abort_flag, 1);
+        ok = false;
+      }
+      if (!ok || *reinterpret_cast<volatile int*>(&bar.abort_flag)) break;
+      const int row = cw * 16 + g;  // a K row of this lane, and the one 8 further on
+      if (n < n_mine) {
+#pragma unroll
+        for (int hg = 0; hg < S::HG; ++hg)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            uint32_t f[8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) codes_f16x4(kw[(hg * 2 + r) * 4 + e], f[2 * e], f[2 * e + 1]);
+            unsigned char* tileK = sK + hg * TILE_KT * 128;
+            *reinterpret_cast<uint4*>(tile_piece(tileK, row + 8 * r, 2 * t)) = make_uint4(f[0], f[1], f[2], f[3]);
+            *reinterpret_cast<uint4*>(tile_piece(tileK, row + 8 * r, 2 * t + 1)) = make_uint4(f[4], f[5], f[6], f[7]);
+          }
+#pragma unroll
+        for (int x = 0; x < VW; ++x) {  // (c, m, r): 4 tokens of one dim
+          const int d = (x / 2) * 16 + (x & 1) * 8 + g;
+          uint32_t lo, hi;
+          codes_f16x4(vw[x], lo, hi);
+          *reinterpret_cast<uint32_t*>(tile_piece(sV, d, 2 * cw) + 4 * t) = lo;
+          *reinterpret_cast<uint32_t*>(tile_piece(sV, d, 2 * cw + 1) + 4 * t) = hi;
+        }
+        if (lane == 0) *reinterpret_cast<float4*>(bar.scale[st][cw]) = make_float4(sc.x, log2_fast(sc.y), rcp_fast(sc.y), 0.f);
+      } else {
+        // the open page: 16-bit elements; rows it does not hold are zeroed (their keys are masked as well)
+        const T* tk = reinterpret_cast<const T*>(p.c.tail) +
+                      ((((int64_t)b * p.c.Hkv + h) * 2 + (n_full & 1)) * 2) * ((int64_t)P * DH) + cw * 16 * DH;
+        const T* tv = tk + (int64_t)P * DH;
+        const int held = len - (n_full << lp) - cw * 16;  // tokens of this group
+        if (held > 0) {
+#pragma unroll
+          for (int hg = 0; hg < S::HG; ++hg)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              uint32_t w[8];
+              load_words<32>(tk + ((hg * 2 + r) * 32 + lane) * S::E, w);
+              unsigned char* tileK = sK + hg * TILE_KT * 128;
+              *reinterpret_cast<uint4*>(tile_piece(tileK, row + 8 * r, 2 * t)) = make_uint4(w[0], w[1], w[2], w[3]);
+              *reinterpret_cast<uint4*>(tile_piece(tileK, row + 8 * r, 2 * t + 1)) = make_uint4(w[4], w[5], w[6], w[7]);
+            }
+        }
+        const uint32_t keep0 = (2 * t < held ? 0xffffu : 0u) | (2 * t + 1 < held ? 0xffff0000u : 0u);
+        const uint32_t keep1 = (2 * t + 8 < held ? 0xffffu : 0u) | (2 * t + 9 < held ? 0xffff0000u : 0u);
+#pragma unroll
+        for (int x = 0; x < VW; ++x) {
+          const int d = (x / 2) * 16 + (x & 1) * 8 + g;
+          uint32_t w[2] = {0u, 0u};
+          if (held > 0) load_words<8>(tv + ((x / (2 * S::M)) * 32 + lane) * 8 * S::M + (x % (2 * S::M)) * 4, w);
+          *reinterpret_cast<uint32_t*>(tile_piece(sV, d, 2 * cw) + 4 * t) = w[0] & keep0;
+          *reinterpret_cast<uint32_t*>(tile_piece(sV, d, 2 * cw + 1) + 4 * t) = w[1] & keep1;
+        }
+        if (lane == 0) *reinterpret_cast<float4*>(bar.scale[st][cw]) = make_float4(1.f, 0.f, 1.f, 0.f);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar.kv_full[st]);
+#pragma unroll
+      for (int x = 0; x < KW; ++x) kw[x] = kn[x];
+#pragma unroll
+      for (int x = 0; x < VW; ++x) vw[x] = vn[x];
+      sc = sn;
+    }
+  } else if (warp == 8) {
+    // ---------------------------------------------------------------- MMA issuer
+    if (lane == 0 && nblk > 0) {
+      constexpr uint32_t S_F16 = umma_idesc_f16(TILE_ROWS, TILE_KT, false, false), S_T = umma_idesc_f16(TILE_ROWS, TILE_KT, C::BF, false);
+      constexpr uint32_t O_F16 = umma_idesc_f16(TILE_ROWS, DH, false, false), O_T = umma_idesc_f16(TILE_ROWS, DH, C::BF, false);
+      const uint32_t tS = bar.tmem_base + TM_S, tO = bar.tmem_base + TM_O;
+      const uint32_t aQ = smem_u32(sQ), aQ2 = smem_u32(sQ2), aKV = smem_u32(sKV), aP = smem_u32(sP);
+      bool ok = true;
+      auto issue_pv = [&](int n) -> bool {
+        if (!mbar_wait_bounded(&bar.p_full[n & 1], (n >> 1) & 1, K_PAGED_TILE, 2)) return false;
+        if (*reinterpret_cast<volatile int*>(&bar.abort_flag)) return false;
+        tc_fence_after();
+        const uint32_t pa = aP + (n & 1) * C::P_BYTES, va = aKV + (n % NS) * 2 * C::K_BYTES + C::K_BYTES;
+#pragma unroll
+        for (int k = 0; k < TILE_KT / 16; ++k)
+          umma_f16(tO, sw128_desc(pa + k * 32, 16, 1024), sw128_desc(va + k * 32, 16, 1024), j0 + n < n_code ? O_F16 : O_T,
+                   n > 0 || k > 0);
+        umma_commit(&bar.o_full[n & 1]);
+        umma_commit(&bar.kv_empty[n % NS]);
+        return true;
+      };
+      for (int n = 0; n < nblk; ++n) {
+        if (!(ok = mbar_wait_bounded(&bar.kv_full[n % NS], (n / NS) & 1, K_PAGED_TILE, 3))) break;
+        if (n >= 2 && !(ok = mbar_wait_bounded(&bar.s_free[n & 1], ((n >> 1) - 1) & 1, K_PAGED_TILE, 4))) break;
+        if (*reinterpret_cast<volatile int*>(&bar.abort_flag)) { ok = false; break; }
+        tc_fence_after();
+        const bool code = j0 + n < n_code;
+        const uint32_t qa = code ? aQ : aQ2, ka = aKV + (n % NS) * 2 * C::K_BYTES;
+#pragma unroll
+        for (int k = 0; k < DH / 16; ++k)
+          umma_f16(tS + (n & 1) * TILE_KT, sw128_desc(qa + (k >> 2) * (TILE_ROWS * 128) + (k & 3) * 32, 16, 1024),
+                   sw128_desc(ka + (k >> 2) * (TILE_KT * 128) + (k & 3) * 32, 16, 1024), code ? S_F16 : S_T, k > 0);
+        umma_commit(&bar.s_full[n & 1]);
+        if (n >= 1 && !(ok = issue_pv(n - 1))) break;
+      }
+      if (ok) ok = issue_pv(nblk - 1);
+      if (!ok) atomicExch(&bar.abort_flag, 1);
+      umma_commit(&bar.mma_done);
+      mbar_wait_bounded(&bar.mma_done, 0, K_PAGED_TILE, 5);  // every MMA of this CTA has completed
+    }
+    __syncwarp();
+  } else {
+    // ---------------------------------------------------------------- softmax (thread = row)
+    const uint32_t lane_base = bar.tmem_base + ((uint32_t)(warp * 32) << 16);
+    float ref = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int n = 0; n < nblk; ++n) {
+      if (!mbar_wait_bounded(&bar.kv_full[n % NS], (n / NS) & 1, K_PAGED_TILE, 6) ||  // (the scales)
+          !mbar_poll_bounded(&bar.s_full[n & 1], (n >> 1) & 1, K_PAGED_TILE, 7)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const bool code = j0 + n < n_code;
+      const int tok0 = code ? first_tok + (j0 + n) * TILE_KT : n_full << lp;
+      const int lim = code ? limit : len;
+      const bool mask = tok0 + TILE_KT - 1 > min(qlo, lim - 1) || (p.window > 0 && tok0 <= qhi - p.window);
+      // this row's visible columns are [c0, c1)
+      const int c1 = min(min(qpos + 1, lim) - tok0, TILE_KT), c0 = p.window > 0 ? qpos - p.window + 1 - tok0 : 0;
+      float ks[4], lv[4], iv[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const float4 f = *reinterpret_cast<const float4*>(bar.scale[n % NS][x]);
+        ks[x] = f.x * cs;
+        lv[x] = f.y;
+        iv[x] = f.z;
+      }
+      float top = -INFINITY;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float v[32];
+        tmem_ld32(lane_base + TM_S + (n & 1) * TILE_KT + half * 32, v);
+        if (mask) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (half * 32 + i < c0 || half * 32 + i >= c1) v[i] = -INFINITY;
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          float m0 = v[x * 16], m1 = v[x * 16 + 1], m2 = v[x * 16 + 2], m3 = v[x * 16 + 3];
+#pragma unroll
+          for (int i = 4; i < 16; i += 4) {
+            m0 = fmaxf(m0, v[x * 16 + i]);
+            m1 = fmaxf(m1, v[x * 16 + i + 1]);
+            m2 = fmaxf(m2, v[x * 16 + i + 2]);
+            m3 = fmaxf(m3, v[x * 16 + i + 3]);
+          }
+          top = fmaxf(top, fmaf(fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)), ks[half * 2 + x], lv[half * 2 + x]));
+        }
+      }
+      const bool rise = top > ref + RISE || (ref == -INFINITY && top > -INFINITY);
+      if (__any_sync(0xffffffffu, rise)) {
+        const float f = rise && ref != -INFINITY ? exp2_fast(ref - top) : 1.f;
+        if (rise) ref = top;
+        l *= f;
+        if (n > 0) {
+          // O holds the blocks before this one: their products have to be complete
+          if (!mbar_wait_bounded(&bar.o_full[(n - 1) & 1], ((n - 1) >> 1) & 1, K_PAGED_TILE, 8)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < DH; c += 32) {
+            float o[32];
+            tmem_ld32(lane_base + TM_O + c, o);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] *= f;
+            tmem_st32(lane_base + TM_O + c, o);
+          }
+          tmem_wait_st();
+        }
+      }
+      // the weights' buffer was last read by the products of block n - 2
+      if (n >= 2 && !mbar_wait_bounded(&bar.o_full[n & 1], ((n >> 1) - 1) & 1, K_PAGED_TILE, 9)) {
+        ok = false;
+        break;
+      }
+      const float base = (ref == -INFINITY ? 0.f : ref) - SHIFT;
+      unsigned char* tileP = sP + (n & 1) * C::P_BYTES;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float v[32];
+        tmem_ld32(lane_base + TM_S + (n & 1) * TILE_KT + half * 32, v);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[x * 16 + i] = exp2_fast(fmaf(v[x * 16 + i], ks[half * 2 + x], lv[half * 2 + x] - base));
+          if (mask) {  // a masked token weighs 0 whatever its score and scales are
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (half * 32 + x * 16 + i < c0 || half * 32 + x * 16 + i >= c1) v[x * 16 + i] = 0.f;
+          }
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) {
+            s0 += v[x * 16 + i];
+            s1 += v[x * 16 + i + 1];
+            s2 += v[x * 16 + i + 2];
+            s3 += v[x * 16 + i + 3];
+          }
+          const float sum = (s0 + s1) + (s2 + s3);
+          l += sum == 0.f ? 0.f : sum * iv[half * 2 + x];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (code)
+            store_vec_from_f32<__half>(reinterpret_cast<__half*>(tile_piece(tileP, tid, half * 4 + i)), v + i * 8);
+          else
+            store_vec_from_f32<T>(reinterpret_cast<T*>(tile_piece(tileP, tid, half * 4 + i)), v + i * 8);
+        }
+      }
+      fence_proxy_async_smem();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&bar.s_free[n & 1]);
+        mbar_arrive(&bar.p_full[n & 1]);
+      }
+    }
+    if (ok && nblk > 0) ok = mbar_wait_bounded(&bar.o_full[(nblk - 1) & 1], ((nblk - 1) >> 1) & 1, K_PAGED_TILE, 10);
+    if (!ok) atomicExch(&bar.abort_flag, 1);
+    tc_fence_after();
+    named_bar_sync(1, 128);
+    const bool good = *reinterpret_cast<volatile int*>(&bar.abort_flag) == 0;  // one outcome for the 4 warps
+    named_bar_sync(1, 128);
+    const bool live = rr < R;
+    T* out = nullptr;
+    int64_t out_row = 0;
+    int hq = 0;
+    if (live) {
+      out_row = nr.row0 + rr / group;
+      hq = h * group + rr % group;
+      out = reinterpret_cast<T*>(p.out) + out_row * p.o_sr + (int64_t)hq * p.o_sh;
+    }
+    auto finish = [&]() {
+      if (p.lse && live) p.lse[out_row * p.Hq + hq] = l == 0.f ? -INFINITY : (ref - SHIFT + log2f(l)) * 0.69314718055994531f;
+    };
+    if (good && tp.splits == 1) {
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll 1
+      for (int c = 0; c < DH; c += 32) {
+        float o[32];
+        tmem_ld32(lane_base + TM_O + c, o);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] *= inv;
+        if (live) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) store_vec_from_f32<T>(out + c + i, o + i);
+        }
+      }
+      finish();
+    } else if (good) {
+      // this CTA's share of the blocks; the last of the tile's CTAs joins them in order
+      const int64_t item = ((int64_t)b * p.c.Hkv + h) * tp.tiles + tile;
+      float* states = tp.states + item * tp.splits * C::STATE;
+      float* mine = states + split * C::STATE;
+#pragma unroll 1
+      for (int c = 0; c < DH; c += 32) {
+        float o[32];
+        if (nblk > 0) tmem_ld32(lane_base + TM_O + c, o);
+#pragma unroll
+        for (int i = 0; i < 32; i += 4)
+          __stcg(reinterpret_cast<float4*>(mine) + (c + i) / 4 * TILE_ROWS + tid,
+                 nblk > 0 ? make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]) : make_float4(0.f, 0.f, 0.f, 0.f));
+      }
+      __stcg(mine + TILE_ROWS * DH + tid, ref);
+      __stcg(mine + TILE_ROWS * (DH + 1) + tid, l);
+      __threadfence();
+      named_bar_sync(1, 128);
+      if (tid == 0) bar.last = atomicAdd(tp.counters + item, 1) == tp.splits - 1;
+      named_bar_sync(1, 128);
+      if (bar.last) {
+        __threadfence();
+        if (tid == 0) tp.counters[item] = 0;
+        float f[TILE_MAX_SPLITS];
+        ref = -INFINITY;
+#pragma unroll
+        for (int s = 0; s < TILE_MAX_SPLITS; ++s) {
+          f[s] = -INFINITY;
+          if (s < tp.splits) f[s] = __ldcg(states + s * C::STATE + TILE_ROWS * DH + tid);
+          ref = fmaxf(ref, f[s]);
+        }
+        l = 0.f;
+#pragma unroll
+        for (int s = 0; s < TILE_MAX_SPLITS; ++s) {
+          // (a share that saw nothing, or nothing but NaN, has no maximum: its sums count as they are)
+          f[s] = s >= tp.splits ? 0.f : (f[s] == -INFINITY ? 1.f : exp2_fast(f[s] - ref));
+          if (s < tp.splits) l += __ldcg(states + s * C::STATE + TILE_ROWS * (DH + 1) + tid) * f[s];
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll 1
+        for (int c = 0; c < DH; c += 8) {
+          float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int s = 0; s < TILE_MAX_SPLITS; ++s)
+            if (s < tp.splits) {
+              const float4* src = reinterpret_cast<const float4*>(states + s * C::STATE) + c / 4 * TILE_ROWS + tid;
+              const float4 x = __ldcg(src), y = __ldcg(src + TILE_ROWS);
+              o[0] += x.x * f[s]; o[1] += x.y * f[s]; o[2] += x.z * f[s]; o[3] += x.w * f[s];
+              o[4] += y.x * f[s]; o[5] += y.y * f[s]; o[6] += y.z * f[s]; o[7] += y.w * f[s];
+            }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o[i] *= inv;
+          if (live) store_vec_from_f32<T>(out + c, o);
+        }
+        finish();
+      }
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(bar.tmem_base, TM_COLS);
+  }
+}
+
+}  // namespace ta
