@@ -1157,8 +1157,10 @@ __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
   const int n_work = min((int)gridDim.x * WARPS, (total + SPLIT_MIN_UNITS - 1) / SPLIT_MIN_UNITS);
   // a few warps: one on each SM first; all of them: neighbours share an SM, which spreads the joins
   const int me = n_work < (int)gridDim.x * WARPS ? warp * gridDim.x + blockIdx.x : blockIdx.x * WARPS + warp;
-  auto first_of = [&](int w) { return (int)((int64_t)total * w / n_work); };
-  auto owner_of = [&](int u) { return (int)((((int64_t)u + 1) * n_work - 1) / total); };
+  // even shares, the first `over` warps with one more (32-bit divisions only)
+  const int share = total / n_work, over = total % n_work;
+  auto first_of = [&](int w) { return w * share + min(w, over); };
+  auto owner_of = [&](int u) { return u < (share + 1) * over ? u / (share + 1) : over + (u - (share + 1) * over) / share; };
   const int u0 = me < n_work ? first_of(me) : 0, u1 = me < n_work ? first_of(me + 1) : 0;
   const int32_t* table = p.c.table;
 

@@ -2,7 +2,7 @@
 // the 5th-generation tensor cores. The mathematics and the cache are those of paged.cuh; here the products bound it.
 //
 // A CTA takes 128 rows (query-major: query i, head gq of the group -> row i * group + gq) and runs through 64-token blocks:
-//   warps 4-7  converters: warp w reads the codes of one 16-token group (the next block's are in registers by then), turns
+//   warps 4-7  converters: warp w reads the codes of one 16-token group (the next two blocks' are on their way to registers), turns
 //              them into f16 and stores them as 128-byte-swizzled tiles: K (64 tokens x DH) and V transposed (DH x 64 tokens),
 //              both K-major operands. A lane's fragment order gives it 32 bytes of a K row and token pairs of V columns, so
 //              neither store meets a bank twice.
@@ -30,7 +30,7 @@ constexpr int K_PAGED_TILE = 19;
 template <typename T, int DH>
 struct TileShape {
   static constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
-  static constexpr int NS = 2;                          // K / V stages
+  static constexpr int NS = 2;                          // K and V stages (as many as score and weight buffers)
   static constexpr int HALVES = DH / 64;                // 64-dim column blocks of Q and K
   static constexpr int Q_BYTES = TILE_ROWS * DH * 2;
   static constexpr int K_BYTES = TILE_KT * DH * 2;      // and of V
@@ -42,8 +42,9 @@ struct TileShape {
 };
 
 struct TileBars {
-  uint64_t kv_full[2], kv_empty[2], s_full[2], s_free[2], p_full[2], o_full[2], mma_done;
-  alignas(16) float scale[2][4][4];  // per stage and 16-token group: key scale, log2 of the value scale, its inverse
+  uint64_t k_full[2], v_full[2], s_full[2], s_free[2], p_full[2], o_full[2], mma_done;
+  // per block (of four in turn) and 16-token group: key scale, log2 of the value scale, its inverse
+  alignas(16) float scale[4][4][4];
   uint32_t tmem_base;
   int abort_flag, last;
 };
@@ -56,6 +57,67 @@ struct TileParams {
   int32_t* counters;  // (B, Hkv, tiles), zero between launches
   float* states;      // (B, Hkv, tiles, splits) states
 };
+
+// 64 consecutive fp32 columns of this thread's TMEM lane, waited for before returning.
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, float (&v)[64]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31]), "=f"(v[32]), "=f"(v[33]), "=f"(v[34]), "=f"(v[35]), "=f"(v[36]), "=f"(v[37]), "=f"(v[38]), "=f"(v[39]), "=f"(v[40]), "=f"(v[41]), "=f"(v[42]), "=f"(v[43]), "=f"(v[44]), "=f"(v[45]), "=f"(v[46]), "=f"(v[47]), "=f"(v[48]), "=f"(v[49]), "=f"(v[50]), "=f"(v[51]), "=f"(v[52]), "=f"(v[53]), "=f"(v[54]), "=f"(v[55]), "=f"(v[56]), "=f"(v[57]), "=f"(v[58]), "=f"(v[59]), "=f"(v[60]), "=f"(v[61]), "=f"(v[62]), "=f"(v[63])
+      : "r"(taddr)
+      : "memory");
+}
+
+// A bounded wait for a phase that is usually complete already, or about to be: tests without suspending, and looks at the
+// clock (itself hundreds of cycles) only after some time. With the waits that suspend and read it first a softmax step spent
+// 700 of 3600 cycles on barriers that were already complete.
+__device__ __forceinline__ bool tile_wait(uint64_t* bar, uint32_t parity, int where) {
+  uint64_t t0 = 0;
+  for (uint32_t spins = 0;; ++spins) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if ((spins & 255u) == 255u) {
+      const uint64_t now = global_timer_ns();
+      if (t0 == 0) t0 = now;
+      if (now - t0 > TA_WAIT_LIMIT_NS) {
+        record_error(DEV_WAIT_TIMEOUT, K_PAGED_TILE, where, (int)parity);
+        return false;
+      }
+    }
+  }
+}
+
+// Two fp32 at a time, and the largest of three.
+__device__ __forceinline__ uint64_t f32x2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 f32x2_parts(uint64_t x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma_x2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 
 // a 16-byte piece of a swizzled tile's row (128 bytes)
 __device__ __forceinline__ unsigned char* tile_piece(unsigned char* tile, int row, int c) {
@@ -98,8 +160,8 @@ __global__ void __launch_bounds__(TILE_THREADS, TileShape<T, DH>::CTAS) paged_ti
 
   if (tid == 0) {
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&bar.kv_full[s], 4);
-      mbar_init(&bar.kv_empty[s], 1);
+      mbar_init(&bar.k_full[s], 4);
+      mbar_init(&bar.v_full[s], 4);
       mbar_init(&bar.s_full[s], 1);
       mbar_init(&bar.s_free[s], 4);
       mbar_init(&bar.p_full[s], 4);
@@ -186,27 +248,30 @@ __global__ void __launch_bounds__(TILE_THREADS, TileShape<T, DH>::CTAS) paged_ti
       }
       sc = __ldg(reinterpret_cast<const float2*>(r + 2 * P * DH));
     };
-    uint32_t kw[KW], vw[VW];
-    float2 sc;
-    int next = 0;
-    if (n_mine > 0) fetch(j0, entry(j0), kw, vw, sc);
-    if (n_mine > 1) next = entry(j0 + 1);
+    // block n: its codes are in the registers given, which then take those of block n + 2 (two sets in turn: moving one to
+    // the other would wait for the loads); ent: the table entry of that block
     bool ok = true;
-    for (int n = 0; n < nblk; ++n) {
+    auto block = [&](int n, uint32_t (&kw)[KW], uint32_t (&vw)[VW], float2& sc, int& ent) -> bool {
       const int st = n % NS;
       unsigned char* sK = sKV + st * 2 * C::K_BYTES;
       unsigned char* sV = sK + C::K_BYTES;
-      uint32_t kn[KW], vn[VW];
-      float2 sn = make_float2(1.f, 1.f);
-      if (n + 1 < n_mine) {
-        fetch(j0 + n + 1, next, kn, vn, sn);
-        if (n + 2 < n_mine) next = entry(j0 + n + 2);
-      }
-      if (n >= NS && !mbar_wait_bounded(&bar.kv_empty[st], ((n / NS) - 1) & 1, K_PAGED_TILE, 1)) {
-        atomicExch(&bar.abort_flag, 1);
-        ok = false;
-      }
-      if (!ok || *reinterpret_cast<volatile int*>(&bar.abort_flag)) break;
+      // K's stage is free when the scores of block n - 2 are there, long before V's (the products of block n - 2 with the
+      // weights): so K goes first, and the next scores do not wait for the softmax. (The scales' place was last read by the
+      // softmax of block n - 4, which V's stage of block n - 1 waited for.)
+      auto free_of = [&](uint64_t* done, int where) {
+        if (n >= NS && !mbar_wait_bounded(done + st, ((n / NS) - 1) & 1, K_PAGED_TILE, where)) {
+          atomicExch(&bar.abort_flag, 1);
+          ok = false;
+        }
+        if (*reinterpret_cast<volatile int*>(&bar.abort_flag)) ok = false;
+        return ok;
+      };
+      auto filled = [&](uint64_t* full) {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(full + st);
+      };
+      if (!free_of(bar.s_full, 1)) return false;
       const int row = cw * 16 + g;  // a K row of this lane, and the one 8 further on
       if (n < n_mine) {
 #pragma unroll
@@ -220,6 +285,10 @@ __global__ void __launch_bounds__(TILE_THREADS, TileShape<T, DH>::CTAS) paged_ti
             *reinterpret_cast<uint4*>(tile_piece(tileK, row + 8 * r, 2 * t)) = make_uint4(f[0], f[1], f[2], f[3]);
             *reinterpret_cast<uint4*>(tile_piece(tileK, row + 8 * r, 2 * t + 1)) = make_uint4(f[4], f[5], f[6], f[7]);
           }
+        if (lane == 0)
+          *reinterpret_cast<float4*>(bar.scale[n & 3][cw]) = make_float4(sc.x, log2_fast(sc.y), rcp_fast(sc.y), 0.f);
+        filled(bar.k_full);
+        if (!free_of(bar.o_full, 11)) return false;
 #pragma unroll
         for (int x = 0; x < VW; ++x) {  // (c, m, r): 4 tokens of one dim
           const int d = (x / 2) * 16 + (x & 1) * 8 + g;
@@ -228,7 +297,6 @@ __global__ void __launch_bounds__(TILE_THREADS, TileShape<T, DH>::CTAS) paged_ti
           *reinterpret_cast<uint32_t*>(tile_piece(sV, d, 2 * cw) + 4 * t) = lo;
           *reinterpret_cast<uint32_t*>(tile_piece(sV, d, 2 * cw + 1) + 4 * t) = hi;
         }
-        if (lane == 0) *reinterpret_cast<float4*>(bar.scale[st][cw]) = make_float4(sc.x, log2_fast(sc.y), rcp_fast(sc.y), 0.f);
       } else {
         // the open page: 16-bit elements; rows it does not hold are zeroed (their keys are masked as well)
         const T* tk = reinterpret_cast<const T*>(p.c.tail) +
@@ -247,6 +315,9 @@ __global__ void __launch_bounds__(TILE_THREADS, TileShape<T, DH>::CTAS) paged_ti
               *reinterpret_cast<uint4*>(tile_piece(tileK, row + 8 * r, 2 * t + 1)) = make_uint4(w[4], w[5], w[6], w[7]);
             }
         }
+        if (lane == 0) *reinterpret_cast<float4*>(bar.scale[n & 3][cw]) = make_float4(1.f, 0.f, 1.f, 0.f);
+        filled(bar.k_full);
+        if (!free_of(bar.o_full, 11)) return false;
         const uint32_t keep0 = (2 * t < held ? 0xffffu : 0u) | (2 * t + 1 < held ? 0xffff0000u : 0u);
         const uint32_t keep1 = (2 * t + 8 < held ? 0xffffu : 0u) | (2 * t + 9 < held ? 0xffff0000u : 0u);
 #pragma unroll
@@ -257,16 +328,26 @@ __global__ void __launch_bounds__(TILE_THREADS, TileShape<T, DH>::CTAS) paged_ti
           *reinterpret_cast<uint32_t*>(tile_piece(sV, d, 2 * cw) + 4 * t) = w[0] & keep0;
           *reinterpret_cast<uint32_t*>(tile_piece(sV, d, 2 * cw + 1) + 4 * t) = w[1] & keep1;
         }
-        if (lane == 0) *reinterpret_cast<float4*>(bar.scale[st][cw]) = make_float4(1.f, 0.f, 1.f, 0.f);
       }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bar.kv_full[st]);
-#pragma unroll
-      for (int x = 0; x < KW; ++x) kw[x] = kn[x];
-#pragma unroll
-      for (int x = 0; x < VW; ++x) vw[x] = vn[x];
-      sc = sn;
+      if (n + 2 < n_mine) {
+        fetch(j0 + n + 2, ent, kw, vw, sc);
+        if (n + 4 < n_mine) ent = entry(j0 + n + 4);
+      }
+      filled(bar.v_full);
+      return true;
+    };
+    uint32_t ka[KW], va[VW], kb[KW], vb[VW];
+    float2 sa, sb;
+    int ea = 0, eb = 0;
+    if (n_mine > 0) ea = entry(j0);
+    if (n_mine > 1) eb = entry(j0 + 1);
+    if (n_mine > 0) fetch(j0, ea, ka, va, sa);
+    if (n_mine > 1) fetch(j0 + 1, eb, kb, vb, sb);
+    if (n_mine > 2) ea = entry(j0 + 2);
+    if (n_mine > 3) eb = entry(j0 + 3);
+    for (int n = 0; n < nblk; n += 2) {
+      if (!block(n, ka, va, sa, ea)) break;
+      if (n + 1 < nblk && !block(n + 1, kb, vb, sb, eb)) break;
     }
   } else if (warp == 8) {
     // ---------------------------------------------------------------- MMA issuer
@@ -277,7 +358,9 @@ __global__ void __launch_bounds__(TILE_THREADS, TileShape<T, DH>::CTAS) paged_ti
       const uint32_t aQ = smem_u32(sQ), aQ2 = smem_u32(sQ2), aKV = smem_u32(sKV), aP = smem_u32(sP);
       bool ok = true;
       auto issue_pv = [&](int n) -> bool {
-        if (!mbar_wait_bounded(&bar.p_full[n & 1], (n >> 1) & 1, K_PAGED_TILE, 2)) return false;
+        if (!tile_wait(&bar.v_full[n % NS], (n / NS) & 1, 12) ||
+            !tile_wait(&bar.p_full[n & 1], (n >> 1) & 1, 2))
+          return false;
         if (*reinterpret_cast<volatile int*>(&bar.abort_flag)) return false;
         tc_fence_after();
         const uint32_t pa = aP + (n & 1) * C::P_BYTES, va = aKV + (n % NS) * 2 * C::K_BYTES + C::K_BYTES;
@@ -286,12 +369,11 @@ __global__ void __launch_bounds__(TILE_THREADS, TileShape<T, DH>::CTAS) paged_ti
           umma_f16(tO, sw128_desc(pa + k * 32, 16, 1024), sw128_desc(va + k * 32, 16, 1024), j0 + n < n_code ? O_F16 : O_T,
                    n > 0 || k > 0);
         umma_commit(&bar.o_full[n & 1]);
-        umma_commit(&bar.kv_empty[n % NS]);
         return true;
       };
       for (int n = 0; n < nblk; ++n) {
-        if (!(ok = mbar_wait_bounded(&bar.kv_full[n % NS], (n / NS) & 1, K_PAGED_TILE, 3))) break;
-        if (n >= 2 && !(ok = mbar_wait_bounded(&bar.s_free[n & 1], ((n >> 1) - 1) & 1, K_PAGED_TILE, 4))) break;
+        if (!(ok = tile_wait(&bar.k_full[n % NS], (n / NS) & 1, 3))) break;
+        if (n >= 2 && !(ok = tile_wait(&bar.s_free[n & 1], ((n >> 1) - 1) & 1, 4))) break;
         if (*reinterpret_cast<volatile int*>(&bar.abort_flag)) { ok = false; break; }
         tc_fence_after();
         const bool code = j0 + n < n_code;
@@ -315,8 +397,8 @@ __global__ void __launch_bounds__(TILE_THREADS, TileShape<T, DH>::CTAS) paged_ti
     float ref = -INFINITY, l = 0.f;
     bool ok = true;
     for (int n = 0; n < nblk; ++n) {
-      if (!mbar_wait_bounded(&bar.kv_full[n % NS], (n / NS) & 1, K_PAGED_TILE, 6) ||  // (the scales)
-          !mbar_poll_bounded(&bar.s_full[n & 1], (n >> 1) & 1, K_PAGED_TILE, 7)) {
+      if (!tile_wait(&bar.k_full[n % NS], (n / NS) & 1, 6) ||  // (the scales)
+          !tile_wait(&bar.s_full[n & 1], (n >> 1) & 1, 7)) {
         ok = false;
         break;
       }
@@ -327,36 +409,30 @@ __global__ void __launch_bounds__(TILE_THREADS, TileShape<T, DH>::CTAS) paged_ti
       const bool mask = tok0 + TILE_KT - 1 > min(qlo, lim - 1) || (p.window > 0 && tok0 <= qhi - p.window);
       // this row's visible columns are [c0, c1)
       const int c1 = min(min(qpos + 1, lim) - tok0, TILE_KT), c0 = p.window > 0 ? qpos - p.window + 1 - tok0 : 0;
-      float ks[4], lv[4], iv[4];
+      float ks[4], lv[4];
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        const float4 f = *reinterpret_cast<const float4*>(bar.scale[n % NS][x]);
+        const float2 f = *reinterpret_cast<const float2*>(bar.scale[n & 3][x]);
         ks[x] = f.x * cs;
         lv[x] = f.y;
-        iv[x] = f.z;
+      }
+      float v[64];
+      tmem_ld64(lane_base + TM_S + (n & 1) * TILE_KT, v);
+      if (mask) {
+#pragma unroll
+        for (int i = 0; i < 64; ++i)
+          if (i < c0 || i >= c1) v[i] = -INFINITY;
       }
       float top = -INFINITY;
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        float v[32];
-        tmem_ld32(lane_base + TM_S + (n & 1) * TILE_KT + half * 32, v);
-        if (mask) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (half * 32 + i < c0 || half * 32 + i >= c1) v[i] = -INFINITY;
-        }
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          float m0 = v[x * 16], m1 = v[x * 16 + 1], m2 = v[x * 16 + 2], m3 = v[x * 16 + 3];
-#pragma unroll
-          for (int i = 4; i < 16; i += 4) {
-            m0 = fmaxf(m0, v[x * 16 + i]);
-            m1 = fmaxf(m1, v[x * 16 + i + 1]);
-            m2 = fmaxf(m2, v[x * 16 + i + 2]);
-            m3 = fmaxf(m3, v[x * 16 + i + 3]);
-          }
-          top = fmaxf(top, fmaf(fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)), ks[half * 2 + x], lv[half * 2 + x]));
-        }
+      for (int x = 0; x < 4; ++x) {
+        float m0 = max3(v[x * 16], v[x * 16 + 1], v[x * 16 + 2]), m1 = max3(v[x * 16 + 3], v[x * 16 + 4], v[x * 16 + 5]);
+        m0 = max3(m0, v[x * 16 + 6], v[x * 16 + 7]);
+        m1 = max3(m1, v[x * 16 + 8], v[x * 16 + 9]);
+        m0 = max3(m0, v[x * 16 + 10], v[x * 16 + 11]);
+        m1 = max3(m1, v[x * 16 + 12], v[x * 16 + 13]);
+        m0 = max3(m0, v[x * 16 + 14], v[x * 16 + 15]);
+        top = fmaxf(top, fmaf(fmaxf(m0, m1), ks[x], lv[x]));
       }
       const bool rise = top > ref + RISE || (ref == -INFINITY && top > -INFINITY);
       if (__any_sync(0xffffffffu, rise)) {
@@ -365,7 +441,7 @@ __global__ void __launch_bounds__(TILE_THREADS, TileShape<T, DH>::CTAS) paged_ti
         l *= f;
         if (n > 0) {
           // O holds the blocks before this one: their products have to be complete
-          if (!mbar_wait_bounded(&bar.o_full[(n - 1) & 1], ((n - 1) >> 1) & 1, K_PAGED_TILE, 8)) {
+          if (!tile_wait(&bar.o_full[(n - 1) & 1], ((n - 1) >> 1) & 1, 8)) {
             ok = false;
             break;
           }
@@ -382,43 +458,45 @@ __global__ void __launch_bounds__(TILE_THREADS, TileShape<T, DH>::CTAS) paged_ti
         }
       }
       // the weights' buffer was last read by the products of block n - 2
-      if (n >= 2 && !mbar_wait_bounded(&bar.o_full[n & 1], ((n >> 1) - 1) & 1, K_PAGED_TILE, 9)) {
+      if (n >= 2 && !tile_wait(&bar.o_full[n & 1], ((n >> 1) - 1) & 1, 9)) {
         ok = false;
         break;
       }
       const float base = (ref == -INFINITY ? 0.f : ref) - SHIFT;
       unsigned char* tileP = sP + (n & 1) * C::P_BYTES;
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        float v[32];
-        tmem_ld32(lane_base + TM_S + (n & 1) * TILE_KT + half * 32, v);
+      for (int x = 0; x < 4; ++x) {
+        const uint64_t k2 = f32x2(ks[x], ks[x]), b2 = f32x2(lv[x] - base, lv[x] - base);
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) v[x * 16 + i] = exp2_fast(fmaf(v[x * 16 + i], ks[half * 2 + x], lv[half * 2 + x] - base));
-          if (mask) {  // a masked token weighs 0 whatever its score and scales are
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (half * 32 + x * 16 + i < c0 || half * 32 + x * 16 + i >= c1) v[x * 16 + i] = 0.f;
-          }
-#pragma unroll
-          for (int i = 0; i < 16; i += 4) {
-            s0 += v[x * 16 + i];
-            s1 += v[x * 16 + i + 1];
-            s2 += v[x * 16 + i + 2];
-            s3 += v[x * 16 + i + 3];
-          }
-          const float sum = (s0 + s1) + (s2 + s3);
-          l += sum == 0.f ? 0.f : sum * iv[half * 2 + x];
+        for (int i = x * 16; i < x * 16 + 16; i += 2) {
+          const float2 e = f32x2_parts(fma_x2(f32x2(v[i], v[i + 1]), k2, b2));
+          v[i] = exp2_fast(e.x);
+          v[i + 1] = exp2_fast(e.y);
         }
+      }
+      if (mask) {  // a masked token weighs 0 whatever its score and scales are
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (code)
-            store_vec_from_f32<__half>(reinterpret_cast<__half*>(tile_piece(tileP, tid, half * 4 + i)), v + i * 8);
-          else
-            store_vec_from_f32<T>(reinterpret_cast<T*>(tile_piece(tileP, tid, half * 4 + i)), v + i * 8);
+        for (int i = 0; i < 64; ++i)
+          if (i < c0 || i >= c1) v[i] = 0.f;
+      }
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        uint64_t a0 = f32x2(v[x * 16], v[x * 16 + 1]), a1 = f32x2(v[x * 16 + 2], v[x * 16 + 3]);
+#pragma unroll
+        for (int i = x * 16 + 4; i < x * 16 + 16; i += 4) {
+          a0 = add_x2(a0, f32x2(v[i], v[i + 1]));
+          a1 = add_x2(a1, f32x2(v[i + 2], v[i + 3]));
         }
+        const float2 a = f32x2_parts(add_x2(a0, a1));
+        const float sum = a.x + a.y;
+        l += sum == 0.f ? 0.f : sum * bar.scale[n & 3][x][2];
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (code)
+          store_vec_from_f32<__half>(reinterpret_cast<__half*>(tile_piece(tileP, tid, i)), v + i * 8);
+        else
+          store_vec_from_f32<T>(reinterpret_cast<T*>(tile_piece(tileP, tid, i)), v + i * 8);
       }
       fence_proxy_async_smem();
       tc_fence_before();
@@ -428,7 +506,7 @@ __global__ void __launch_bounds__(TILE_THREADS, TileShape<T, DH>::CTAS) paged_ti
         mbar_arrive(&bar.p_full[n & 1]);
       }
     }
-    if (ok && nblk > 0) ok = mbar_wait_bounded(&bar.o_full[(nblk - 1) & 1], ((nblk - 1) >> 1) & 1, K_PAGED_TILE, 10);
+    if (ok && nblk > 0) ok = tile_wait(&bar.o_full[(nblk - 1) & 1], ((nblk - 1) >> 1) & 1, 10);
     if (!ok) atomicExch(&bar.abort_flag, 1);
     tc_fence_after();
     named_bar_sync(1, 128);
