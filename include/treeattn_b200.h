@@ -368,14 +368,14 @@ int ta_block_tail(const void* att, float* x, const void* w_proj, const float* ln
  *   tail (pages from the last but one on) and, for each page whose last token arrives, into the pool: scale = top / 448,
  *   code = e4m3(x * (448 / top)), top the largest magnitude of the page's page x dh values of that head. Below 2^-100 a
  *   page has codes 0 and scale 1; with an infinity or NaN in it codes 0 and scale NaN. The codes depend on the tokens
- *   alone. A sequence may be cut back afterwards (pos reduced) to any length from (last page - 1) * page on, last page =
- *   (pos + new - 1) / page: those tokens are still in the tail.
+ *   alone. A sequence may be cut back afterwards (pos reduced) to any length from (last page - 1) * page on, last page = the
+ *   furthest page that was ever written, (pos + new - 1) / page: those tokens are still in the tail.
  * ta_paged_attn: out[r] = sum over t of softmax_t(scale q_r . K_t) V_t, for query i of a sequence the positions t <=
  *   pos + i (and t > pos + i - window when window > 0), after ta_paged_append has put the same rows into the cache. Hq a
  *   multiple of Hkv: query head hq reads kv head hq / (Hq / Hkv). lse (n_rows, Hq) fp32 or NULL: the natural logarithm of
  *   the sum of exponentials (-inf, with zero rows in out, where nothing is attended). ws: scratch of at least
- *   ta_paged_attn_workspace bytes, zeroed before its first use; every call leaves it ready for the next. Calls that share
- *   it must not overlap on the GPU.
+ *   ta_paged_attn_workspace bytes, zeroed before its first use; every call leaves it ready for the next. Calls of any shapes
+ *   may share it; they must not overlap on the GPU.
  * ta_verify_drafts: speculative sampling. p (B, G + 1, V) the target's and q (B, G, V) the draft's probabilities (dtype;
  *   unit inner stride, strides in elements), drafts (B, G), u (B, G + 1) uniform numbers in [0, 1), one for each
  *   draft and the last for the draw, n (B) drafts of each sequence or NULL (G). Draft i stands while u_i q_i(d_i) < p_i(d_i); accepted[b] = a, the drafts before the first that

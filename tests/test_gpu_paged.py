@@ -189,6 +189,22 @@ def test_cut_back_and_append_again():
     _no_device_error()
 
 
+@pytest.mark.parametrize('page', [16, 32, 64])
+def test_every_offset_keeps_the_last_two_pages(page):
+    """Calls that begin at every offset of a page and of the 64 positions around it, of lengths around a page, two pages and
+    64: full pages read back, and after cutting back the last page but one comes from the 16-bit copy, token for token."""
+    B = 128
+    for n in (1, page - 1, page, page + 1, 2 * page - 1, 2 * page, 2 * page + 5, 65, 3 * page + 2, 150):
+        r = Rig(B, 1, 16, page, BF, 128 + 200, seed=n)
+        pos = list(range(B))
+        r.append(pos)
+        r.append([n] * B)
+        r.check_reads()
+        r.len = [max(0, (p + n - 1) // page * page - 1) for p in pos]  # all but one token of the page before the last
+        r.check_reads()
+    _no_device_error()
+
+
 def test_odd_pages():
     """Pages of zeros, of values below 2^-100, of the type's largest values, with an infinity, with a NaN."""
     page, dh = 16, 32
@@ -367,6 +383,59 @@ def test_long_table_and_many_sequences():
     got = P.paged_attn(r.cache, q, _starts([1] * B), _i32(before), 1)
     want, tol, _, _ = _attend_ref(r, q, [1] * B, before, 0.25, 0)
     assert ((got.double() - want).abs() <= tol).all()
+    _no_device_error()
+
+
+def test_one_workspace_for_many_shapes():
+    """A workspace large enough for every call serves calls of other shapes in turn: few rows, other batches and heads, tiles."""
+    P = _mod()
+    calls = []
+    for B, H, Hq, dh, n, before, seed in ((1, 2, 2, 64, 1, 3000, 1), (40, 4, 8, 64, 2, 200, 2), (2, 2, 4, 64, 300, 900, 3),
+                                          (3, 8, 8, 128, 1, 2000, 4), (2, 1, 8, 128, 3, 2500, 5), (64, 12, 12, 16, 1, 40, 6)):
+        r = Rig(B, H, dh, 32, BF, before + n, seed=seed)
+        r.append([before] * B)
+        r.append([n] * B)
+        q = r.randn(B * n, Hq, dh)
+        calls.append((r, q, n, [before] * B, Hq))
+    ws = torch.zeros(64 << 20, device=DEV, dtype=torch.uint8)
+    want = [_attend_ref(r, q, [n] * r.B, pos, 1 / math.sqrt(r.dh), 0)[:2] for r, q, n, pos, _ in calls]
+    for _ in range(2):
+        for (r, q, n, pos, _), (w, tol) in zip(calls, want):
+            got = P.paged_attn(r.cache, q, _starts([n] * r.B), _i32(pos), n, ws=ws)
+            assert ((got.double() - w).abs() <= tol).all()
+    with pytest.raises(RuntimeError, match='workspace'):
+        r, q, n, pos, _ = calls[0]
+        P.paged_attn(r.cache, q, _starts([n]), _i32(pos), n, ws=ws[:4096])
+    _no_device_error()
+
+
+def test_more_sequences_than_one_plan_holds():
+    """2100 sequences, some with nothing new."""
+    P = _mod()
+    B = 2100
+    r = Rig(B, 1, 16, 16, HF, 48, seed=9)
+    before, new = [b % 40 for b in range(B)], [(b % 3 != 0) * 1 for b in range(B)]
+    r.append(before)
+    r.append(new)
+    q = r.randn(sum(new), 2, 16)
+    got = P.paged_attn(r.cache, q, _starts(new), _i32(before), 1)
+    want, tol, _, _ = _attend_ref(r, q, new, before, 0.25, 0)
+    assert ((got.double() - want).abs() <= tol).all()
+    _no_device_error()
+
+
+@pytest.mark.parametrize('n', [1, 60])
+def test_scales_and_windows_at_their_ends(n):
+    """A negative scale, scale 0 (the mean of the values), a window of the largest integer (the whole prefix)."""
+    P = _mod()
+    r = Rig(2, 2, 64, 16, BF, 200, seed=8)
+    r.append([100, 30])
+    r.append([n, n])
+    q = r.randn(2 * n, 2, 64)
+    for scale, window in ((-0.3, 0), (0.0, 0), (0.125, 2 ** 31 - 1), (-0.2, 33)):
+        got = P.paged_attn(r.cache, q, _starts([n, n]), _i32([100, 30]), n, scale=scale, window=window)
+        want, tol, _, _ = _attend_ref(r, q, [n, n], [100, 30], scale, 0 if window > 1000 else window)
+        assert ((got.double() - want).abs() <= tol.abs() + 1e-5).all(), (scale, window)
     _no_device_error()
 
 

@@ -62,6 +62,14 @@ def test_chunks_drafts_and_single_tokens_agree(dt):
     assert _ops.device_error()[0] == 0
 
 
+def _restart(dec, idx, n):
+    """The decoder, emptied and fed the first n tokens."""
+    dec.pos, dec._floor = [0] * dec.batch, [0] * dec.batch
+    dec.forward(idx[:, :81])
+    dec.forward(idx[:, 81:n])
+    return dec
+
+
 def test_cut_back():
     """Drafts that are dropped leave no trace in the logits that follow; what is gone from the 16-bit pages is refused."""
     from treeattn_b200.speculative import PagedDecoder
@@ -78,6 +86,12 @@ def test_cut_back():
     assert torch.equal(a.forward(idx[:, 93:98]), b.forward(idx[:, 93:98]))
     with pytest.raises(ValueError, match='cannot go'):
         a.cut_back([98, 60])
+    # positions up to 100 (page 6) were written: page 4's place is gone even after going back to page 5 and on from there
+    a.cut_back([81, 81])
+    a.forward(idx[:, 81:82])
+    with pytest.raises(ValueError, match='cannot go'):
+        a.cut_back([79, 82])
+    assert torch.equal(a.forward(idx[:, 82:98]), PagedDecoder.forward(_restart(b, idx, 82), idx[:, 82:98]))
     with pytest.raises(ValueError, match='cannot go'):
         a.cut_back([99, 98])
     with pytest.raises(ValueError, match='max_len'):

@@ -71,40 +71,43 @@ int run_attn_nt(const ta::AttnParams& p, cudaStream_t st) {
   return check_launch("ta_paged_attn");
 }
 
-// The split form: counters (one per item, 256-byte aligned end), then two states for every warp of the grid.
-int64_t counter_bytes(int64_t B, int64_t Hkv) { return (B * Hkv * 4 + 255) / 256 * 256; }
+// A workspace begins with the arrival counters, one per item, in a place of one size for every call: whatever shapes share a
+// workspace, no call's states lie where another's counters are expected to be zero.
+constexpr int64_t kItems = 1 << 16;
+constexpr int64_t kCounterBytes = kItems * 4;
 
+// The split form: two states for every warp of the grid.
 template <int DH, int NT>
-int64_t split_bytes(int64_t B, int64_t Hkv) {
+int64_t split_bytes() {
   using SH = ta::SplitShape<DH, NT>;
-  return counter_bytes(B, Hkv) + (int64_t)sm_count() * SH::WARPS * 2 * SH::STATE * 4;
+  return kCounterBytes + (int64_t)sm_count() * SH::WARPS * 2 * SH::STATE * 4;
 }
 
 template <int DH>
-int64_t split_bytes_dh(int64_t B, int64_t Hkv, int64_t rows) {
-  if (rows <= 8) return split_bytes<DH, 1>(B, Hkv);
-  if (rows <= 16) return split_bytes<DH, 2>(B, Hkv);
-  if (rows <= 24) return split_bytes<DH, 3>(B, Hkv);
-  return split_bytes<DH, 4>(B, Hkv);
+int64_t split_bytes_dh(int64_t rows) {
+  if (rows <= 8) return split_bytes<DH, 1>();
+  if (rows <= 16) return split_bytes<DH, 2>();
+  if (rows <= 24) return split_bytes<DH, 3>();
+  return split_bytes<DH, 4>();
 }
 
 constexpr int kSplitRows = 32;  // rows of one (sequence, kv head) up to which the cache's bytes bound the call
 
 bool split_takes(int64_t B, int64_t Hkv, int64_t rows, int64_t max_pages, int P) {
-  return rows <= kSplitRows && B <= ta::SPLIT_MAX_BATCH && B * Hkv * (max_pages * P / 32 + 7) <= INT_MAX;
+  return rows <= kSplitRows && B <= ta::SPLIT_MAX_BATCH && B * Hkv <= kItems && B * Hkv * (max_pages * P / 32 + 7) <= INT_MAX;
 }
 
 template <typename T, int DH, int NT>
 int run_split(const ta::AttnParams& p, void* ws, int64_t ws_bytes, cudaStream_t st) {
   using SH = ta::SplitShape<DH, NT>;
-  const int64_t need = split_bytes<DH, NT>(p.B, p.c.Hkv);
+  const int64_t need = split_bytes<DH, NT>();
   if (!ws || !aligned16(ws) || ws_bytes < need)
     return fail(TA_ERR_ARG, "ta_paged_attn: a workspace of %lld bytes is needed (16-byte aligned; got %lld)", (long long)need,
                 (long long)ws_bytes);
   static SmemAttr attr;
   const int smem = SH::RING + SH::BAR_BYTES + 12 * (p.B + 1);
   if (int r = allow_smem(attr, ta::paged_split_kernel<T, DH, NT>, smem, "ta_paged_attn")) return r;
-  float* states = reinterpret_cast<float*>(reinterpret_cast<char*>(ws) + counter_bytes(p.B, p.c.Hkv));
+  float* states = reinterpret_cast<float*>(reinterpret_cast<char*>(ws) + kCounterBytes);
   const cudaError_t e = launch_pdl(ta::paged_split_kernel<T, DH, NT>, dim3(sm_count()), dim3(SH::WARPS * 32), smem, st, p,
                                    reinterpret_cast<int32_t*>(ws), states);
   if (e != cudaSuccess) return fail(TA_ERR_CUDA, "ta_paged_attn: launch failed: %s", cudaGetErrorString(e));
@@ -121,7 +124,7 @@ int64_t tile_bytes(int64_t B, int64_t Hkv, int64_t rows, int dh) {
   const int splits = tile_splits(B, Hkv, rows, dh);
   if (splits == 1) return 0;
   const int64_t items = B * Hkv * tiles_of(rows);
-  return counter_bytes(items, 1) + items * splits * ta::TILE_ROWS * (dh + 2) * 4;
+  return kCounterBytes + items * splits * ta::TILE_ROWS * (dh + 2) * 4;
 }
 
 template <typename T, int DH>
@@ -136,7 +139,7 @@ int run_tile(const ta::AttnParams& p, int64_t rows, void* ws, int64_t ws_bytes, 
   tp.tiles = (int)tiles;
   tp.splits = tile_splits(p.B, p.c.Hkv, rows, DH);
   tp.counters = reinterpret_cast<int32_t*>(ws);
-  tp.states = reinterpret_cast<float*>(reinterpret_cast<char*>(ws) + counter_bytes((int64_t)p.B * p.c.Hkv * tiles, 1));
+  tp.states = reinterpret_cast<float*>(reinterpret_cast<char*>(ws) + kCounterBytes);
   static SmemAttr attr;
   constexpr int smem = 1024 + C::BYTES + (int)sizeof(ta::TileBars);
   if (int r = allow_smem(attr, ta::paged_tile_kernel<T, DH>, smem, "ta_paged_attn")) return r;
@@ -225,10 +228,10 @@ int64_t ta_paged_attn_workspace(int B, int Hq, int Hkv, int dh, int max_new) {
   const int64_t rows = (int64_t)max_new * (Hq / Hkv);
   if (rows > kSplitRows) return dh >= 64 ? tile_bytes(B, Hkv, rows, dh) : 0;
   switch (dh) {
-    case 16: return split_bytes_dh<16>(B, Hkv, rows);
-    case 32: return split_bytes_dh<32>(B, Hkv, rows);
-    case 64: return split_bytes_dh<64>(B, Hkv, rows);
-    default: return split_bytes_dh<128>(B, Hkv, rows);
+    case 16: return split_bytes_dh<16>(rows);
+    case 32: return split_bytes_dh<32>(rows);
+    case 64: return split_bytes_dh<64>(rows);
+    default: return split_bytes_dh<128>(rows);
   }
 }
 
@@ -242,6 +245,7 @@ int ta_paged_attn(const void* pool, const void* tail, const int32_t* table, int6
                           pos, max_new))
     return r;
   if (window < 0) return fail(TA_ERR_ARG, "%s: window %d", who, window);
+  if (window >= (int64_t)(max_pages + 1) * page) window = 0;  // longer than any sequence
   if (B == 0 || n_rows == 0 || max_new == 0) return TA_OK;
   if (!q || !out) return fail(TA_ERR_ARG, "%s: null pointer", who);
   if (!rows_aligned(q, 2, {q_sr, q_sh}) || !rows_aligned(out, 2, {o_sr, o_sh}))

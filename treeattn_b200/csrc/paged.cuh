@@ -216,11 +216,11 @@ __global__ void __launch_bounds__(APPEND_THREADS) paged_append_kernel(AppendPara
   const int j0 = base >> lp;                           // first page of this CTA
   const int full_end = min(end >> lp << lp, base + APPEND_SPAN) - base;  // rows below this are of full pages
   const int i0 = max(nr.pos - base, 0), i1 = min(end - base, APPEND_SPAN);  // rows with new tokens
-  // The last two pages stay in 16 bits. Where the first page has earlier tokens in the tail, pages from the second after it
-  // on may share its slots: the CTA that reads those tokens writes the later pages there after that.
+  // The last two pages stay in 16 bits. Where the first page has earlier tokens in the tail and the last page is the second
+  // after it or later, one of the two may share its slots: then the CTA that reads those tokens writes both, after that.
   const bool old = (nr.pos & (P - 1)) != 0, reader = f >= j0 && f < j0 + (APPEND_SPAN >> lp);
   const int keep = max((last - 1) * P - base, i0);  // rows from here on go to the tail
-  const bool keeps = keep < i1 && (!old || reader || last < f + 2 || j0 + (APPEND_SPAN >> lp) <= f + 2);
+  const bool keeps = keep < i1 && (!old || reader || last < f + 2);
   T* sk = reinterpret_cast<T*>(append_smem);
   T* sv = sk + APPEND_SPAN * PITCH;
   T* tail = reinterpret_cast<T*>(p.c.tail) + ((int64_t)b * p.c.Hkv + h) * 4 * ((int64_t)P * DH);
@@ -379,7 +379,7 @@ __global__ void __launch_bounds__(APPEND_THREADS) paged_append_kernel(AppendPara
   if (reader && old && last >= f + 2) {
     // later pages of other CTAs into the tail (the earlier tokens have been read); the first page is full then, so that no
     // thread has left above
-    const int from = max(max(last - 1, f + 2) << lp, base + APPEND_SPAN);
+    const int from = max((last - 1) << lp, base + APPEND_SPAN);
     for (int span = from / APPEND_SPAN * APPEND_SPAN; span < end; span += APPEND_SPAN) {
       const int r0 = max(from - span, 0), r1 = min(end - span, APPEND_SPAN);
       __syncthreads();

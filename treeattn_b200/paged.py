@@ -176,7 +176,7 @@ def paged_append(cache, k, v, start, pos, max_new, q=None, rotation=None, q_out=
     and head strides) go to positions pos[b], pos[b] + 1, .... `max_new` bounds the rows of one sequence. rotation = (cos, sin)
     (rotation_table) turns the first dims of k, and of q (n, n_head, head_dim) into q_out (allocated here when not given).
     Without a rotation q is returned as it is. A page is quantised when its last token arrives; afterwards a sequence may be
-    cut back to any length whose page is the last or last but one written."""
+    cut back to any length whose page is the last or last but one that was ever written."""
     pool, tail, table = cache.pool, cache.tail, cache.table
     dt = tail.dtype
     B = _rows('paged_append', cache, start, pos)
@@ -217,7 +217,8 @@ def paged_append(cache, k, v, start, pos, max_new, q=None, rotation=None, q_out=
 
 
 def paged_attn_workspace(batch, n_head, n_kv_head, head_dim, max_new, device='cuda'):
-    """A zeroed workspace for paged_attn at these sizes: one per stream of calls, kept by the caller."""
+    """A zeroed workspace for paged_attn at these sizes: one per stream of calls, kept by the caller. Calls of other sizes
+    may share it when it is large enough for each."""
     n = _lib.load().ta_paged_attn_workspace(int(batch), int(n_head), int(n_kv_head), int(head_dim), int(max_new))
     return torch.zeros(max(int(n), 16), device=device, dtype=torch.uint8)
 

@@ -35,7 +35,8 @@ class PagedDecoder:
         per_seq = -(-self.max_len // page)
         self.pool = PagePool(n_pages or batch * per_seq, batch, per_seq, page, self.dev)
         self.caches = [PagedKV.empty(self.pool.n_pages, n_head, self.dh, self.pool.table, page, dtype) for _ in range(n_layer)]
-        self.pos = [0] * batch  # positions that each sequence holds
+        self.pos = [0] * batch     # positions that each sequence holds
+        self._floor = [0] * batch  # and how far back it can be cut: the start of the page before the furthest one written
         self._start = {}
         self._ws = {}
 
@@ -71,13 +72,15 @@ class PagedDecoder:
             f = _ops.gelu_(h @ L['c_fc'].t())
             _ops.add_ln(x, f @ L['c_mlp'].t(), W['layers'][i + 1]['ln1'] if i + 1 < len(W['layers']) else W['ln_f'], h)
         self.pos = [p + n for p in self.pos]
+        page = self.pool.page
+        self._floor = [max(f, ((p - 1) // page - 1) * page) for f, p in zip(self._floor, self.pos)]
         return (h @ W['wte'].t()).view(B, n, -1)
 
     def cut_back(self, pos):
         """Drops positions from pos[b] on (rejected drafts). A sequence can lose what is still in 16 bits: back to the start of
-        the page before the last one written."""
+        the page before the furthest one written."""
         for b, (old, new) in enumerate(zip(self.pos, pos)):
-            if not 0 <= new <= old or (old > 0 and new < ((old - 1) // self.pool.page - 1) * self.pool.page):
+            if not max(0, self._floor[b]) <= new <= old:
                 raise ValueError('PagedDecoder: sequence %d cannot go from %d back to %d positions' % (b, old, new))
         self.pos = list(pos)
 
