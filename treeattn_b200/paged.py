@@ -130,7 +130,8 @@ def rotation_table(n_pos, rot, base=10000.0, device='cuda'):
 
 
 # A decode step's calls take a few microseconds on the GPU: the checks below ask each tensor once, the entry points are looked
-# up once, and the current stream is read without building a torch Stream object (2.3 -> 0.2 us).
+# up once, the current stream is read without building a torch Stream object (2.3 -> 0.2 us), and outputs are allocated like
+# an input (2.4 -> 1.4 us).
 _entry = {}
 
 
@@ -193,7 +194,8 @@ def paged_append(cache, k, v, start, pos, max_new, q=None, rotation=None, q_out=
         if (cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or cos.shape != sin.shape or cos.dim() != 2 or
                 not (cos.is_contiguous() and sin.is_contiguous())):
             raise ValueError('paged_append: rotation must be two contiguous fp32 tables (positions, rot / 2)')
-        _need_cuda('paged_append', cos, sin)
+        if not (cos.is_cuda and sin.is_cuda):
+            _need_cuda('paged_append', cos, sin)
         n_pos, rot = cos.shape
         rot *= 2
         cos, sin = cos.data_ptr(), sin.data_ptr()
@@ -204,7 +206,7 @@ def paged_append(cache, k, v, start, pos, max_new, q=None, rotation=None, q_out=
         if rot:
             Hq, qr, qh = qshape[1], qs[0], qs[1]
             if q_out is None:
-                q_out = torch.empty(qshape, device=q.device, dtype=dt)
+                q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
             elif q_out.shape != qshape or q_out.dtype is not dt or not q_out.is_contiguous():
                 raise ValueError('paged_append: q_out must be contiguous, of q\'s shape and type')
             qp, qo = q.data_ptr(), q_out.data_ptr()
@@ -236,7 +238,7 @@ def paged_attn(cache, q, start, pos, max_new, scale=None, window=0, out=None, ls
     n, Hq, dh = qshape
     n_pages, H, _ = pool.shape
     if out is None:
-        out = torch.empty(qshape, device=q.device, dtype=dt)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         os = (Hq * dh, dh)
     else:
         oshape, os = _heads('paged_attn', cache, out, dt)
@@ -273,11 +275,10 @@ def verify_drafts(p, q, drafts, u, n_draft=None):
         raise ValueError('verify_drafts: u must be (B, G + 1) fp32, contiguous')
     if n_draft is not None and (n_draft.shape != (B,) or n_draft.dtype is not torch.int32 or not n_draft.is_contiguous()):
         raise ValueError('verify_drafts: n_draft must be (B,) int32, contiguous')
-    if not (p.is_cuda and q.is_cuda and drafts.is_cuda and u.is_cuda):
-        _need_cuda('verify_drafts', p, q, drafts, u)
-    _need_cuda('verify_drafts', n_draft)
-    tokens = torch.empty((B, G + 1), device=p.device, dtype=torch.int64)
-    accepted = torch.empty((B,), device=p.device, dtype=torch.int32)
+    if not (p.is_cuda and q.is_cuda and drafts.is_cuda and u.is_cuda and (n_draft is None or n_draft.is_cuda)):
+        _need_cuda('verify_drafts', p, q, drafts, u, n_draft)
+    tokens = torch.empty_like(u, dtype=torch.int64)
+    accepted = u.new_empty((B,), dtype=torch.int32) if n_draft is None else torch.empty_like(n_draft)
     _call('ta_verify_drafts', p.data_ptr(), ps[0], ps[1], q.data_ptr(), qs[0], qs[1], _DT[dt], B, G, V, drafts.data_ptr(),
           u.data_ptr(), _p(n_draft), tokens.data_ptr(), accepted.data_ptr(), _stream(p))
     return tokens, accepted
