@@ -55,8 +55,10 @@ int run_append(const ta::AppendParams& a, int B, cudaStream_t st) {
     q_ctas = (int)std::min<int64_t>(work, std::max(1, sm_count() * 32 / std::max(B, 1)));
   }
   const size_t smem = (size_t)2 * ta::APPEND_SPAN * (DH + 8) * 2;
-  ta::paged_append_kernel<T, DH><<<dim3(p.page_ctas + q_ctas, B), ta::APPEND_THREADS, smem, st>>>(p);
-  return check_launch("ta_paged_append");
+  const cudaError_t e = launch_pdl(ta::paged_append_kernel<T, DH>, dim3(p.page_ctas + q_ctas, B), dim3(ta::APPEND_THREADS), smem,
+                                   st, p);
+  if (e != cudaSuccess) return fail(TA_ERR_CUDA, "ta_paged_append: launch failed: %s", cudaGetErrorString(e));
+  return TA_OK;
 }
 
 template <typename T, int DH, int NT>

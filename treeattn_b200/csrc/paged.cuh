@@ -167,6 +167,8 @@ __global__ void __launch_bounds__(APPEND_THREADS) paged_append_kernel(AppendPara
   extern __shared__ __align__(16) unsigned char append_smem[];
   __shared__ uint32_t tops[2][APPEND_SPAN / 16];
   const int b = blockIdx.y, tid = threadIdx.x;
+  pdl_wait();
+  pdl_launch_dependents();
   NewRows nr;
   if (!new_rows(p.start, p.pos, b, p.n_rows, p.max_new, p.c, K_PAGED_APPEND, nr) || nr.n == 0) return;
   const int half_rot = p.rot / 2;
