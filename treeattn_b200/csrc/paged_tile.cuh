@@ -58,14 +58,16 @@ struct TileParams {
   float* states;      // (B, Hkv, tiles, splits) states
 };
 
-// 64 consecutive fp32 columns of this thread's TMEM lane, waited for before returning.
-__device__ __forceinline__ void tmem_ld64(uint32_t taddr, float (&v)[64]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31]), "=f"(v[32]), "=f"(v[33]), "=f"(v[34]), "=f"(v[35]), "=f"(v[36]), "=f"(v[37]), "=f"(v[38]), "=f"(v[39]), "=f"(v[40]), "=f"(v[41]), "=f"(v[42]), "=f"(v[43]), "=f"(v[44]), "=f"(v[45]), "=f"(v[46]), "=f"(v[47]), "=f"(v[48]), "=f"(v[49]), "=f"(v[50]), "=f"(v[51]), "=f"(v[52]), "=f"(v[53]), "=f"(v[54]), "=f"(v[55]), "=f"(v[56]), "=f"(v[57]), "=f"(v[58]), "=f"(v[59]), "=f"(v[60]), "=f"(v[61]), "=f"(v[62]), "=f"(v[63])
-      : "r"(taddr)
-      : "memory");
+// 16 consecutive fp32 columns of this thread's TMEM lane on their way to v; complete after tmem_got.
+__device__ __forceinline__ void tmem_get16(uint32_t taddr, float (&v)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+               : "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_got(float (&v)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+  asm volatile("" : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]));  // no use of v moves above the wait
 }
 
 // A bounded wait for a phase that is usually complete already, or about to be: tests without suspending, and looks at the
@@ -397,8 +399,9 @@ __global__ void __launch_bounds__(TILE_THREADS, TileShape<T, DH>::CTAS) paged_ti
     float ref = -INFINITY, l = 0.f;
     bool ok = true;
     for (int n = 0; n < nblk; ++n) {
-      if (!tile_wait(&bar.k_full[n % NS], (n / NS) & 1, 6) ||  // (the scales)
-          !tile_wait(&bar.s_full[n & 1], (n >> 1) & 1, 7)) {
+      // The scores of block n: the issuing thread had seen its K (and scales) complete, and the same arrival stands for every
+      // product issued before, those of block n - 2 with the weights among them, whose buffer this step overwrites.
+      if (!tile_wait(&bar.s_full[n & 1], (n >> 1) & 1, 7)) {
         ok = false;
         break;
       }
@@ -416,24 +419,33 @@ __global__ void __launch_bounds__(TILE_THREADS, TileShape<T, DH>::CTAS) paged_ti
         ks[x] = f.x * cs;
         lv[x] = f.y;
       }
-      float v[64];
-      tmem_ld64(lane_base + TM_S + (n & 1) * TILE_KT, v);
-      if (mask) {
-#pragma unroll
-        for (int i = 0; i < 64; ++i)
-          if (i < c0 || i >= c1) v[i] = -INFINITY;
-      }
+      // two passes over the scores, 16 columns at a time with the next ones on their way: all 64 at once do not fit the 96
+      // registers that two CTAs an SM leave a thread
+      const uint32_t tS = lane_base + TM_S + (n & 1) * TILE_KT;
+      float va[16], vb[16];
+      tmem_get16(tS, va);
+      tmem_got(va);
       float top = -INFINITY;
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        float m0 = max3(v[x * 16], v[x * 16 + 1], v[x * 16 + 2]), m1 = max3(v[x * 16 + 3], v[x * 16 + 4], v[x * 16 + 5]);
-        m0 = max3(m0, v[x * 16 + 6], v[x * 16 + 7]);
-        m1 = max3(m1, v[x * 16 + 8], v[x * 16 + 9]);
-        m0 = max3(m0, v[x * 16 + 10], v[x * 16 + 11]);
-        m1 = max3(m1, v[x * 16 + 12], v[x * 16 + 13]);
-        m0 = max3(m0, v[x * 16 + 14], v[x * 16 + 15]);
+        float(&v)[16] = x & 1 ? vb : va;
+        float(&next)[16] = x & 1 ? va : vb;
+        if (x < 3) tmem_get16(tS + (x + 1) * 16, next);
+        if (mask) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (x * 16 + i < c0 || x * 16 + i >= c1) v[i] = -INFINITY;
+        }
+        float m0 = max3(v[0], v[1], v[2]), m1 = max3(v[3], v[4], v[5]);
+        m0 = max3(m0, v[6], v[7]);
+        m1 = max3(m1, v[8], v[9]);
+        m0 = max3(m0, v[10], v[11]);
+        m1 = max3(m1, v[12], v[13]);
+        m0 = max3(m0, v[14], v[15]);
         top = fmaxf(top, fmaf(fmaxf(m0, m1), ks[x], lv[x]));
+        if (x < 3) tmem_got(next);
       }
+      tmem_get16(tS, va);
       const bool rise = top > ref + RISE || (ref == -INFINITY && top > -INFINITY);
       if (__any_sync(0xffffffffu, rise)) {
         const float f = rise && ref != -INFINITY ? exp2_fast(ref - top) : 1.f;
@@ -457,47 +469,48 @@ __global__ void __launch_bounds__(TILE_THREADS, TileShape<T, DH>::CTAS) paged_ti
           tmem_wait_st();
         }
       }
-      // the weights' buffer was last read by the products of block n - 2
-      if (n >= 2 && !tile_wait(&bar.o_full[n & 1], ((n >> 1) - 1) & 1, 9)) {
-        ok = false;
-        break;
-      }
       const float base = (ref == -INFINITY ? 0.f : ref) - SHIFT;
       unsigned char* tileP = sP + (n & 1) * C::P_BYTES;
+      tmem_got(va);
+      auto weights = [&](auto masked, auto type) {
+        using W = decltype(type);
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const uint64_t k2 = f32x2(ks[x], ks[x]), b2 = f32x2(lv[x] - base, lv[x] - base);
+        for (int x = 0; x < 4; ++x) {
+          float(&w)[16] = x & 1 ? vb : va;
+          float(&next)[16] = x & 1 ? va : vb;
+          if (x < 3) tmem_get16(tS + (x + 1) * 16, next);
+          const uint64_t k2 = f32x2(ks[x], ks[x]), b2 = f32x2(lv[x] - base, lv[x] - base);
 #pragma unroll
-        for (int i = x * 16; i < x * 16 + 16; i += 2) {
-          const float2 e = f32x2_parts(fma_x2(f32x2(v[i], v[i + 1]), k2, b2));
-          v[i] = exp2_fast(e.x);
-          v[i + 1] = exp2_fast(e.y);
+          for (int i = 0; i < 16; i += 2) {
+            const float2 e = f32x2_parts(fma_x2(f32x2(w[i], w[i + 1]), k2, b2));
+            w[i] = exp2_fast(e.x);
+            w[i + 1] = exp2_fast(e.y);
+          }
+          if constexpr (decltype(masked)::value) {  // a masked token weighs 0 whatever its score and scales are
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (x * 16 + i < c0 || x * 16 + i >= c1) w[i] = 0.f;
+          }
+          uint64_t a0 = f32x2(w[0], w[1]), a1 = f32x2(w[2], w[3]);
+#pragma unroll
+          for (int i = 4; i < 16; i += 4) {
+            a0 = add_x2(a0, f32x2(w[i], w[i + 1]));
+            a1 = add_x2(a1, f32x2(w[i + 2], w[i + 3]));
+          }
+          const float2 a = f32x2_parts(add_x2(a0, a1));
+          const float sum = a.x + a.y;
+          l += sum == 0.f ? 0.f : sum * bar.scale[n & 3][x][2];
+          store_vec_from_f32<W>(reinterpret_cast<W*>(tile_piece(tileP, tid, 2 * x)), w);
+          store_vec_from_f32<W>(reinterpret_cast<W*>(tile_piece(tileP, tid, 2 * x + 1)), w + 8);
+          if (x < 3) tmem_got(next);
         }
-      }
-      if (mask) {  // a masked token weighs 0 whatever its score and scales are
-#pragma unroll
-        for (int i = 0; i < 64; ++i)
-          if (i < c0 || i >= c1) v[i] = 0.f;
-      }
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        uint64_t a0 = f32x2(v[x * 16], v[x * 16 + 1]), a1 = f32x2(v[x * 16 + 2], v[x * 16 + 3]);
-#pragma unroll
-        for (int i = x * 16 + 4; i < x * 16 + 16; i += 4) {
-          a0 = add_x2(a0, f32x2(v[i], v[i + 1]));
-          a1 = add_x2(a1, f32x2(v[i + 2], v[i + 3]));
-        }
-        const float2 a = f32x2_parts(add_x2(a0, a1));
-        const float sum = a.x + a.y;
-        l += sum == 0.f ? 0.f : sum * bar.scale[n & 3][x][2];
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (code)
-          store_vec_from_f32<__half>(reinterpret_cast<__half*>(tile_piece(tileP, tid, i)), v + i * 8);
-        else
-          store_vec_from_f32<T>(reinterpret_cast<T*>(tile_piece(tileP, tid, i)), v + i * 8);
-      }
+      };
+      if (!mask)
+        weights(std::false_type{}, __half{});
+      else if (code)
+        weights(std::true_type{}, __half{});
+      else
+        weights(std::true_type{}, T{});  // (the open page is never seen whole)
       fence_proxy_async_smem();
       tc_fence_before();
       __syncwarp();
