@@ -1008,85 +1008,96 @@ __device__ __forceinline__ void join_states(SoftState<DH, NT>& st, const float* 
     }
 }
 
-// An item whose parts are all in the workspace: part 0 is the second state of warp `first`, part w the first state of warp
-// first + w.
+// Large states (more than 8 vectors a lane). What the warps of a CTA hold of one item at its end is joined in the CTA's
+// shared memory first, so that an item shared by several CTAs has one state of each in the workspace, and one of the warp that
+// holds its last unit. `first` and `last` are the warps that share the item, `wpc` warps to a CTA.
 struct Join {
-  int row0, n, h, first, parts;
+  int row0, n, h, first, last, wpc;
+  __device__ __forceinline__ int parts() const { return (last - 1) / wpc - first / wpc + 2; }
 };
 
-// Joins 16 dims (tile x) of an item's states, in order, and writes them out: the form for large states, in which all warps
-// of a CTA share. No load is conditional (a branch around each kept them apart): a place without a part reads the last one and
-// counts it 0 times, columns of no row come to nothing.
-template <typename T, int DH, int NT>
-__device__ __noinline__ void join_tile(const AttnParams& p, const Join& j, const float* states, int x) {
-  using SH = SplitShape<DH, NT>;
-  constexpr int ROWS = 8 * NT, UN = 8;  // parts in flight
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int group = p.Hq / p.c.Hkv, R = j.n * group, parts = j.parts;
-  auto state_of = [&](int w) {
-    w = min(w, parts - 1);
-    return states + ((int64_t)(j.first + w) * 2 + (w == 0 ? 1 : 0)) * SH::STATE;
-  };
-  // maxima, sums and numerators together: a new maximum scales what there is
-  float m[NT][2], l[NT][2], acc[NT][4];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    m[nt][0] = m[nt][1] = -INFINITY;
-    l[nt][0] = l[nt][1] = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[nt][i] = 0.f;
-  }
+// Joins a tile (16 dims x of the 8 rows nt) of `parts` states, in order; get(part, i) is float4 i of a state. The code runs a
+// few times on an SM at the end of a call, and fetching it costs as much as its loads and sums: a tile at a time keeps it
+// small. No load is conditional (a branch around each kept them apart): a place without a part reads the last one and counts
+// it 0 times, columns of no row come to nothing. A part that saw nothing, or nothing but NaN, has no maximum: its sums count
+// as they are.
+template <int DH, int NT, typename Get>
+__device__ __forceinline__ void merge_tile(Get get, int parts, int x, int nt, float (&m)[2], float (&l)[2], float (&acc)[4]) {
+  constexpr int UN = 4;
+  const int lane = threadIdx.x & 31, t = lane & 3;
+  m[0] = m[1] = -INFINITY;
+  l[0] = l[1] = acc[0] = acc[1] = acc[2] = acc[3] = 0.f;
 #pragma unroll 1
   for (int w0 = 0; w0 < parts; w0 += UN) {
-    float4 ml[UN][NT], o[UN][NT];
+    float4 ml[UN], o[UN];
 #pragma unroll
     for (int y = 0; y < UN; ++y) {
-      const float4* s = reinterpret_cast<const float4*>(state_of(w0 + y));
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        ml[y][nt] = __ldcg(s + ROWS * DH / 4 + nt * 4 + t);
-        o[y][nt] = __ldcg(s + (x * NT + nt) * 32 + lane);
-      }
+      const int w = min(w0 + y, parts - 1);
+      ml[y] = get(w, 8 * NT * DH / 4 + nt * 4 + t);
+      o[y] = get(w, (x * NT + nt) * 32 + lane);
     }
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float mn = m[nt][i];
-#pragma unroll
-        for (int y = 0; y < UN; ++y) mn = fmaxf(mn, i ? ml[y][nt].y : ml[y][nt].x);
-        // (a part that saw nothing, or nothing but NaN, has no maximum: its sums count as they are)
-        const float f = m[nt][i] == -INFINITY ? 1.f : exp2_fast(m[nt][i] - mn);
-        m[nt][i] = mn;
-        l[nt][i] *= f;
-        acc[nt][i] *= f;
-        acc[nt][i + 2] *= f;
-#pragma unroll
-        for (int y = 0; y < UN; ++y) {
-          const float my = i ? ml[y][nt].y : ml[y][nt].x;
-          const float fy = w0 + y >= parts ? 0.f : (my == -INFINITY ? 1.f : exp2_fast(my - mn));
-          l[nt][i] += (i ? ml[y][nt].w : ml[y][nt].z) * fy;
-          acc[nt][i] += (i ? o[y][nt].y : o[y][nt].x) * fy;
-          acc[nt][i + 2] += (i ? o[y][nt].w : o[y][nt].z) * fy;
-        }
-      }
-  }
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int rr = nt * 8 + 2 * t + i;
-      if (rr >= R) continue;
-      const int64_t row = j.row0 + rr / group;
-      const int hq = j.h * group + rr % group;
-      T* out = reinterpret_cast<T*>(p.out) + row * p.o_sr + (int64_t)hq * p.o_sh + x * 16 + g;
-      const float inv = l[nt][i] == 0.f ? 0.f : 1.f / l[nt][i];
-      out[0] = from_f32<T>(acc[nt][i] * inv);
-      out[8] = from_f32<T>(acc[nt][i + 2] * inv);
-      if (p.lse && g == 0 && x == 0)
-        p.lse[row * p.Hq + hq] =
-            l[nt][i] == 0.f ? -INFINITY : (m[nt][i] - ATTN_SHIFT + log2f(l[nt][i])) * 0.69314718055994531f;
+      float mn = m[i];
+#pragma unroll
+      for (int y = 0; y < UN; ++y) mn = fmaxf(mn, i ? ml[y].y : ml[y].x);
+      const float f = m[i] == -INFINITY ? 1.f : exp2_fast(m[i] - mn);
+      m[i] = mn;
+      l[i] *= f;
+      acc[i] *= f;
+      acc[i + 2] *= f;
+#pragma unroll
+      for (int y = 0; y < UN; ++y) {
+        const float my = i ? ml[y].y : ml[y].x;
+        const float fy = w0 + y >= parts ? 0.f : (my == -INFINITY ? 1.f : exp2_fast(my - mn));
+        l[i] += (i ? ml[y].w : ml[y].z) * fy;
+        acc[i] += (i ? o[y].y : o[y].x) * fy;
+        acc[i + 2] += (i ? o[y].w : o[y].z) * fy;
+      }
     }
+  }
+}
+
+// A tile of the states of `parts` warps, one after the other in shared memory `pitch` bytes apart, into one state.
+template <int DH, int NT>
+__device__ __noinline__ void gather_tile(const unsigned char* from, int pitch, int parts, int x, int nt, float* to) {
+  const int lane = threadIdx.x & 31;
+  float m[2], l[2], acc[4];
+  merge_tile<DH, NT>([&](int w, int i) { return reinterpret_cast<const float4*>(from + w * pitch)[i]; }, parts, x, nt, m, l, acc);
+  __stcg(reinterpret_cast<float4*>(to) + (x * NT + nt) * 32 + lane, make_float4(acc[0], acc[1], acc[2], acc[3]));
+  if (x == 0 && lane < 4) __stcg(reinterpret_cast<float4*>(to + 8 * NT * DH) + nt * 4 + lane, make_float4(m[0], m[1], l[0], l[1]));
+}
+
+// A tile of an item whose states are all in the workspace, to the output. states: of the warps that hold last units; groups:
+// of CTAs, each in the place of its first warp of the item. out, lse: of the item's first row and head. (By value: a reference
+// to the kernel's parameters put them into local memory, a miss away: a join took 6 us against 4.)
+template <typename T, int DH, int NT>
+__device__ __noinline__ void join_tile(const Join* join, const float* states, const float* groups, int x, int nt, int group,
+                                       T* out, int64_t o_sr, int64_t o_sh, float* lse, int Hq) {
+  using SH = SplitShape<DH, NT>;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const Join j = *join;
+  const int R = j.n * group, parts = j.parts(), cta0 = j.first / j.wpc;
+  float m[2], l[2], acc[4];
+  merge_tile<DH, NT>(
+      [&](int w, int i) {
+        const float* s = w == parts - 1 ? states + (int64_t)j.last * SH::STATE
+                                        : groups + (int64_t)max(j.first, (cta0 + w) * j.wpc) * SH::STATE;
+        return __ldcg(reinterpret_cast<const float4*>(s) + i);
+      },
+      parts, x, nt, m, l, acc);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int rr = nt * 8 + 2 * t + i;
+    if (rr >= R) continue;
+    const int q = rr / group, gq = rr - q * group;
+    T* o = out + q * o_sr + gq * o_sh + x * 16 + g;
+    const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
+    o[0] = from_f32<T>(acc[i] * inv);
+    o[8] = from_f32<T>(acc[i + 2] * inv);
+    if (lse && g == 0 && x == 0)
+      lse[(int64_t)q * Hq + gq] = l[i] == 0.f ? -INFINITY : (m[i] - ATTN_SHIFT + log2f(l[i])) * 0.69314718055994531f;
+  }
 }
 
 template <typename T, int DH, int NT>
@@ -1098,7 +1109,9 @@ __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
   constexpr int TG = NT >= 3 ? 2 : UT / 16;  // 64 tokens' scores beside 24 or 32 rows' numerators do not fit the registers
   extern __shared__ __align__(128) unsigned char split_smem[];
   __shared__ int warp_sums[WARPS];
-  __shared__ Join joins[2 * WARPS];  // items that a warp of this CTA came last at: a warp has two parts at most
+  // large states: the item that each warp leaves unfinished (-1: none), and items whose last part is this CTA's
+  __shared__ int held[WARPS];
+  __shared__ Join held_join[WARPS], joins[2 * WARPS];
   __shared__ int n_joins;
   unsigned char* ring = split_smem;
   uint64_t* bars = reinterpret_cast<uint64_t*>(split_smem + SH::RING);
@@ -1116,6 +1129,7 @@ __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
     fence_mbar_init();
   }
   if (tid == 0) n_joins = 0;
+  if (tid < WARPS) held[tid] = -1;
   pdl_wait();
   pdl_launch_dependents();
   // where each sequence's units begin
@@ -1157,8 +1171,9 @@ __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
   const int total = s_first[p.B];
   if (total == 0) return;
   const int n_work = min((int)gridDim.x * WARPS, (total + SPLIT_MIN_UNITS - 1) / SPLIT_MIN_UNITS);
-  // a few warps: one on each SM first; all of them: neighbours share an SM, which spreads the joins
-  const int me = n_work < (int)gridDim.x * WARPS ? warp * gridDim.x + blockIdx.x : blockIdx.x * WARPS + warp;
+  // neighbours share an SM (which spreads the joins over the SMs), as few to each as leaves none without
+  const int wpc = (n_work + gridDim.x - 1) / gridDim.x;
+  const int me = warp < wpc ? blockIdx.x * wpc + warp : n_work;
   // even shares, the first `over` warps with one more (32-bit divisions only)
   const int share = total / n_work, over = total % n_work;
   auto first_of = [&](int w) { return w * share + min(w, over); };
@@ -1197,7 +1212,9 @@ __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
     return false;
   };
 
-  // ---- copies: `ahead` runs NS units before the one at work
+  // ---- copies: `ahead` runs NS units before the one at work. Records are read once: they leave the L2 first, so that they
+  // push out neither the states nor the code that runs once at the end (64 sequences 65 -> 61 us).
+  const uint64_t once = l2_policy_evict_first();
   Run ahead{};
   bool more = true;     // it has a unit to copy
   int batch = 0;        // page of the item that lane 0's table entry stands for
@@ -1232,10 +1249,11 @@ __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
       if (lane == 0) mbar_arrive_expect_tx(bar + slot, (uint32_t)(per * rec_e));
       __syncwarp();
       if (P <= UT) {
-        if (lane < per) bulk_g2s(dst + lane * rec_e, src, (uint32_t)rec_e, bar + slot);
+        if (lane < per) bulk_g2s_hint(dst + lane * rec_e, src, (uint32_t)rec_e, bar + slot, once);
       } else if (lane < 3) {  // keys, values and scales of a part of the page
         const int in = (ahead.k * UT) & (P - 1);
-        bulk_g2s(dst + lane * UT * DH, src + lane * P * DH + (lane < 2 ? in * DH : 0), lane < 2 ? UT * DH : 16, bar + slot);
+        bulk_g2s_hint(dst + lane * UT * DH, src + lane * P * DH + (lane < 2 ? in * DH : 0), lane < 2 ? UT * DH : 16, bar + slot,
+                      once);
       }
     } else if (lane == 0) {
       const int t0 = (ahead.k - ahead.it.nu8) * TT;  // token of the open page
@@ -1321,11 +1339,21 @@ __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
       }
     bool write = run.k == 0 && run.end == it.units;
     if (!write) {
-      // a warp's first state is of an item that others began, its second of one that it begins
-      float* mine = states + ((int64_t)me * 2 + (run.k > 0 ? 0 : 1)) * SH::STATE;
+      const int wa = owner_of(run.at), wb = owner_of(run.at + it.units - 1), item = run.b * Hkv + run.h;
+      const Join join{it.row0, it.n, run.h, wa, wb, wpc};
+      if (LATE && run.end < it.units) {
+        // (the warp's last run) stays in the registers until the CTA's warps are done
+        if (lane == 0) {
+          held[warp] = item;
+          held_join[warp] = join;
+        }
+        break;
+      }
+      // large states: one a warp; small ones: the first of an item that others began, the second of one that it begins
+      float* mine = states + (LATE ? (int64_t)me : (int64_t)me * 2 + (run.k > 0 ? 0 : 1)) * SH::STATE;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        if (nt * 8 + 2 * t >= R) continue;  // columns of no row are neither written nor read
+        if (nt * 8 + 2 * t >= R) continue;  // columns of no row are not written, and come to nothing where they are read
 #pragma unroll
         for (int x = 0; x < DH / 16; ++x)
           __stcg(reinterpret_cast<float4*>(mine) + (x * NT + nt) * 32 + lane,
@@ -1336,16 +1364,15 @@ __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
       }
       __threadfence();
       __syncwarp();
-      const int wa = owner_of(run.at), wb = owner_of(run.at + it.units - 1);
-      int32_t* cnt = counters + run.b * Hkv + run.h;
+      int32_t* cnt = counters + item;
       int before = 0;
       if (lane == 0) before = atomicAdd(cnt, 1);
       before = __shfl_sync(0xffffffffu, before, 0);
-      if (before == wb - wa) {
+      if (before == (LATE ? join.parts() - 1 : wb - wa)) {
         __threadfence();
         if (lane == 0) *cnt = 0;
         if constexpr (LATE) {
-          if (lane == 0) joins[atomicAdd(&n_joins, 1)] = Join{it.row0, it.n, run.h, wa, wb - wa + 1};
+          if (lane == 0) joins[atomicAdd(&n_joins, 1)] = join;
         } else {
           const float* later = states + (int64_t)wa * 2 * SH::STATE;
           join_states<DH, NT>(st, later + SH::STATE, later, 2 * SH::STATE, wb - wa + 1, R);
@@ -1377,11 +1404,55 @@ __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
   if (!ok)  // no copy of this warp may still be in flight when its CTA ends
     for (int i = step + 1; i < issued; ++i) mbar_wait_bounded(bar + i % NS, (i / NS) & 1, K_PAGED_ATTN, 2);
   if constexpr (LATE) {
-    // What this CTA's warps completed, joined by all of them once their units are done: one warp alone took 16 to 20 us for
-    // 12 parts of 20 rows at head dim 128, which kept it from its own next units (60 us in all against 54). Small states are
-    // joined on the spot, while the other warps stream (64 sequences, one row: 65 us against 73).
+    // What the CTA's warps leave unfinished, joined by all of them in the rings, which are done with: one state a CTA and
+    // item goes to the workspace, and the last to come joins an item's. (12 parts of 20 rows of head dim 128: one warp alone
+    // took 16 to 20 us, all warps of a CTA over 12 states in the workspace 9; this way 4 us here and 4 for each join.) Small states are joined on the spot by the
+    // last warp, while the others stream (64 sequences, one row: 65 us against 73).
     __syncthreads();
-    for (int i = warp; i < n_joins * (DH / 16); i += WARPS) join_tile<T, DH, NT>(p, joins[i / (DH / 16)], states, i % (DH / 16));
+    constexpr int PITCH = NS * SH::STAGE;
+    static_assert(SH::STATE * 4 <= PITCH, "a warp's state fits its ring");
+    if (held[warp] >= 0) {
+      float4* mine = reinterpret_cast<float4*>(ring + warp * PITCH);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int x = 0; x < DH / 16; ++x)
+          mine[(x * NT + nt) * 32 + lane] = make_float4(st.o[x][nt][0], st.o[x][nt][1], st.o[x][nt][2], st.o[x][nt][3]);
+        if (g == 0) mine[ROWS * DH / 4 + nt * 4 + t] = make_float4(st.m[nt][0], st.m[nt][1], st.l[nt][0], st.l[nt][1]);
+      }
+    }
+    __syncthreads();
+    float* groups = states + (int64_t)gridDim.x * WARPS * SH::STATE;
+    auto leads = [&](int w) { return held[w] >= 0 && (w == 0 || held[w - 1] != held[w]); };
+    int task = 0;
+    for (int w = 0; w < WARPS; ++w) {
+      if (!leads(w)) continue;
+      int count = 1;
+      while (w + count < WARPS && held[w + count] == held[w]) ++count;
+      for (int i = 0; i < NT * (DH / 16); ++i, ++task)
+        if (task % WARPS == warp)
+          gather_tile<DH, NT>(ring + w * PITCH, PITCH, count, i / NT, i % NT, groups + (int64_t)(blockIdx.x * wpc + w) * SH::STATE);
+    }
+    __threadfence();
+    __syncthreads();
+    if (lane == 0 && leads(warp)) {
+      int32_t* cnt = counters + held[warp];
+      if (atomicAdd(cnt, 1) == held_join[warp].parts() - 1) {
+        *cnt = 0;
+        joins[atomicAdd(&n_joins, 1)] = held_join[warp];
+      }
+      __threadfence();
+    }
+    __syncthreads();
+    constexpr int TILES = NT * (DH / 16);
+    for (int i = warp; i < n_joins * TILES; i += WARPS) {
+      const Join* j = joins + i / TILES;
+      const int64_t row = j->row0;
+      const int hq = j->h * group;
+      join_tile<T, DH, NT>(j, states, groups, i % TILES / NT, i % NT, group,
+                           reinterpret_cast<T*>(p.out) + row * p.o_sr + (int64_t)hq * p.o_sh, p.o_sr, p.o_sh,
+                           p.lse ? p.lse + row * p.Hq + hq : nullptr, p.Hq);
+    }
   }
 }
 
