@@ -386,6 +386,34 @@ def test_long_table_and_many_sequences():
     _no_device_error()
 
 
+@pytest.mark.parametrize('dh,Hq,Hkv,before,new,room', [
+    (64, 8, 1, [20000], [1], 0),              # every part of the one item: more than a hundred for each of a few heads
+    (128, 6, 2, [9000], [1], 0),
+    (64, 4, 2, [15000], [7], 0),              # two groups of rows
+    (32, 2, 1, [40000], [1], 0),
+    (64, 12, 12, [0], [1], 30000),            # a long table that holds little: no parts, one, a few
+    (64, 2, 1, [63, 0, 700], [1, 1, 1], 60000),
+    (128, 4, 2, [9000, 5, 127], [2, 0, 1], 9000),
+])
+def test_attention_of_many_parts(dh, Hq, Hkv, before, new, room):
+    """Few items over long tables: their states come from many warps of many CTAs."""
+    P = _mod()
+    r = Rig(len(new), Hkv, dh, 64, BF, max(max(a + b for a, b in zip(before, new)), room), seed=dh + Hq)
+    if any(before):
+        r.append(before)
+    r.append(new)
+    q = r.randn(sum(new), Hq, dh)
+    ws = P.paged_attn_workspace(len(new), Hq, Hkv, dh, max(new))
+    lse = torch.empty(sum(new), Hq, device=DEV)
+    got = P.paged_attn(r.cache, q, _starts(new), _i32(before), max(new), ws=ws, lse=lse)
+    want, tol, wl, ltol = _attend_ref(r, q, new, before, 1 / math.sqrt(dh), 0)
+    assert ((got.double() - want).abs() <= tol).all()
+    assert ((lse.double() - wl).abs() <= ltol).all()
+    for _ in range(3):
+        assert torch.equal(P.paged_attn(r.cache, q, _starts(new), _i32(before), max(new), ws=ws), got)
+    _no_device_error()
+
+
 def test_one_workspace_for_many_shapes():
     """A workspace large enough for every call serves calls of other shapes in turn: few rows, other batches and heads, tiles."""
     P = _mod()

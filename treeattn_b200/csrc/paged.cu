@@ -93,14 +93,28 @@ int64_t split_bytes_dh(int64_t rows) {
   return split_bytes<DH, 4>();
 }
 
-constexpr int kSplitRows = 32;  // rows of one (sequence, kv head) up to which the cache's bytes bound the call
+// Rows of one (sequence, kv head) up to which the call takes the split form. Split / tile form in us, 24 and 32 rows: 16 sequences
+// of 8000, 4 heads of 64: 37 / 59, 51 / 59; of 128: 64 / 92, 97 / 92; one of 30000, 8 heads of 128: 59 / 95, 83 / 95. (More than
+// 32 rows would not fit the split form's registers.)
+constexpr int kSplitRows = 32;
 
 bool split_takes(int64_t B, int64_t Hkv, int64_t rows, int64_t max_pages, int P) {
   return rows <= kSplitRows && B <= ta::SPLIT_MAX_BATCH && B * Hkv <= kItems && B * Hkv * (max_pages * P / 32 + 7) <= INT_MAX;
 }
 
-template <typename T, int DH, int NT>
-int run_split(const ta::AttnParams& p, void* ws, int64_t ws_bytes, cudaStream_t st) {
+// Whether an item's states are joined late: by the parts it has where the batch is even, and the cache as full as it can be
+// (the lengths are on the device).
+template <int DH, int NT>
+bool split_late(const ta::AttnParams& p) {
+  using SH = ta::SplitShape<DH, NT>;
+  const int64_t held = (int64_t)p.c.max_pages * p.c.P, seen = p.window > 0 ? std::min<int64_t>(held, p.window + p.max_new) : held;
+  const int64_t parts = std::min<int64_t>((int64_t)sm_count() * SH::WARPS / ((int64_t)p.B * p.c.Hkv),
+                                          seen / (SH::UT * ta::SPLIT_MIN_UNITS));
+  return parts * SH::STATE * 4 > ta::SPLIT_SPOT_BYTES;
+}
+
+template <typename T, int DH, int NT, bool LATE>
+int launch_split(const ta::AttnParams& p, void* ws, int64_t ws_bytes, cudaStream_t st) {
   using SH = ta::SplitShape<DH, NT>;
   const int64_t need = split_bytes<DH, NT>();
   if (!ws || !aligned16(ws) || ws_bytes < need)
@@ -108,12 +122,20 @@ int run_split(const ta::AttnParams& p, void* ws, int64_t ws_bytes, cudaStream_t 
                 (long long)ws_bytes);
   static SmemAttr attr;
   const int smem = SH::RING + SH::BAR_BYTES + 12 * (p.B + 1);
-  if (int r = allow_smem(attr, ta::paged_split_kernel<T, DH, NT>, smem, "ta_paged_attn")) return r;
+  if (int r = allow_smem(attr, ta::paged_split_kernel<T, DH, NT, LATE>, smem, "ta_paged_attn")) return r;
   float* states = reinterpret_cast<float*>(reinterpret_cast<char*>(ws) + kCounterBytes);
-  const cudaError_t e = launch_pdl(ta::paged_split_kernel<T, DH, NT>, dim3(sm_count()), dim3(SH::WARPS * 32), smem, st, p,
+  const cudaError_t e = launch_pdl(ta::paged_split_kernel<T, DH, NT, LATE>, dim3(sm_count()), dim3(SH::WARPS * 32), smem, st, p,
                                    reinterpret_cast<int32_t*>(ws), states);
   if (e != cudaSuccess) return fail(TA_ERR_CUDA, "ta_paged_attn: launch failed: %s", cudaGetErrorString(e));
   return TA_OK;
+}
+
+template <typename T, int DH, int NT>
+int run_split(const ta::AttnParams& p, void* ws, int64_t ws_bytes, cudaStream_t st) {
+  if constexpr (ta::split_spot<DH, NT>()) {
+    if (!split_late<DH, NT>(p)) return launch_split<T, DH, NT, false>(p, ws, ws_bytes, st);
+  }
+  return launch_split<T, DH, NT, true>(p, ws, ws_bytes, st);
 }
 
 // The tile form (head dims 64 and 128): CTAs that share a tile's blocks, as many as make the tiles fill the GPU.

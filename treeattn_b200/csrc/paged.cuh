@@ -897,13 +897,23 @@ struct SplitShape {
   static constexpr int RING = WARPS * NS * STAGE;
 };
 
-#ifndef TA_MIN_UNITS
-#define TA_MIN_UNITS 2
-#endif
-constexpr int SPLIT_MIN_UNITS = TA_MIN_UNITS;   // units per warp while warps are plenty: below, joining costs more than it spreads
+// Units per warp while warps are plenty: fewer spread more, but have more parts to join (one sequence of 4096, 12 heads:
+// 12.3 us with 1, 10.9 with 2, 11.7 with 3).
+constexpr int SPLIT_MIN_UNITS = 2;
 // An item's own cost, in units (its queries' loads, its output or state): without it a warp whose run is many short sequences
-// comes last (64 uneven sequences, one of them a single token: 67 us without it, 64.5 with)
+// comes last (64 uneven sequences, one of them a single token: 67 us without it, 64.5 with; windows
+// of five rows: 53.8 us with 1, 51.3 with 2 to 4)
 constexpr int SPLIT_ITEM_COST = 2;
+// Bytes of an item's states up to which the warp that comes last joins them by itself, on the spot, while the others stream;
+// the end of a kernel that joins late costs 2 to 7 us at any size. In us, by the last warp / late: 24 parts of 8 rows of head
+// dim 64 12.4 / 14.4, 98 parts of one row 18.1 / 17.0, 148 of 8 rows 30.5 / 18.6; of head dim 128, 18 parts 98.8 / 106, 37
+// parts 56.5 / 58.6, 46 parts 20.5 / 16.5, 148 parts 57.4 / 28.8; of 32 dims, 148 parts 26.7 / 26.6. States of more than 8
+// vectors a lane are always joined late: one warp does not hold two of them.
+constexpr int SPLIT_SPOT_BYTES = 176 << 10;
+template <int DH, int NT>
+constexpr bool split_spot() {
+  return DH / 16 * NT <= 8;
+}
 constexpr int SPLIT_MAX_BATCH = 2048;  // sequences whose geometry is kept in shared memory (12 bytes each)
 
 // The units of one item.
@@ -1008,7 +1018,7 @@ __device__ __forceinline__ void join_states(SoftState<DH, NT>& st, const float* 
     }
 }
 
-// Large states (more than 8 vectors a lane). What the warps of a CTA hold of one item at its end is joined in the CTA's
+// The late join. What the warps of a CTA hold of one item at its end is joined in the CTA's
 // shared memory first, so that an item shared by several CTAs has one state of each in the workspace, and one of the warp that
 // holds its last unit. `first` and `last` are the warps that share the item, `wpc` warps to a CTA.
 struct Join {
@@ -1100,16 +1110,15 @@ __device__ __noinline__ void join_tile(const Join* join, const float* states, co
   }
 }
 
-template <typename T, int DH, int NT>
+template <typename T, int DH, int NT, bool LATE>
 __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
     paged_split_kernel(AttnParams p, int32_t* counters, float* states) {
   using SH = SplitShape<DH, NT>;
   constexpr int WARPS = SH::WARPS, NS = SH::NS, ROWS = 8 * NT, UT = SH::UT, TT = SH::TT;
-  constexpr bool LATE = DH / 16 * NT > 8;  // joins by the whole CTA at its end
   constexpr int TG = NT >= 3 ? 2 : UT / 16;  // 64 tokens' scores beside 24 or 32 rows' numerators do not fit the registers
   extern __shared__ __align__(128) unsigned char split_smem[];
   __shared__ int warp_sums[WARPS];
-  // large states: the item that each warp leaves unfinished (-1: none), and items whose last part is this CTA's
+  // late joins: the item that each warp leaves unfinished (-1: none), and items whose last part is this CTA's
   __shared__ int held[WARPS];
   __shared__ Join held_join[WARPS], joins[2 * WARPS];
   __shared__ int n_joins;
@@ -1349,7 +1358,7 @@ __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
         }
         break;
       }
-      // large states: one a warp; small ones: the first of an item that others began, the second of one that it begins
+      // late joins: one a warp; others: the first of an item that others began, the second of one that it begins
       float* mine = states + (LATE ? (int64_t)me : (int64_t)me * 2 + (run.k > 0 ? 0 : 1)) * SH::STATE;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -1406,8 +1415,7 @@ __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
   if constexpr (LATE) {
     // What the CTA's warps leave unfinished, joined by all of them in the rings, which are done with: one state a CTA and
     // item goes to the workspace, and the last to come joins an item's. (12 parts of 20 rows of head dim 128: one warp alone
-    // took 16 to 20 us, all warps of a CTA over 12 states in the workspace 9; this way 4 us here and 4 for each join.) Small states are joined on the spot by the
-    // last warp, while the others stream (64 sequences, one row: 65 us against 73).
+    // took 16 to 20 us, all warps of a CTA over 12 states in the workspace 9; this way 4 us here and 4 for each join.)
     __syncthreads();
     constexpr int PITCH = NS * SH::STAGE;
     static_assert(SH::STATE * 4 <= PITCH, "a warp's state fits its ring");

@@ -11,8 +11,10 @@
 //   warps 0-3  softmax, one thread per row: maximum, weights (f16, into shared memory), denominator; O is rescaled in tensor
 //              memory only when a row's reference has to rise by more than 2^8.
 // The open page is the last block: 16-bit elements as they are, with a copy of the queries in that type.
-// The exponentials bound it at head dim 64 (128 x 64 of them a block at 16 a cycle), the products' issue and the softmax
-// warps' other instructions come next. Where the tiles do not fill the GPU, the blocks of a tile are shared by several
+// What bounds it is the chain of latencies of a block's softmax step (scores out of tensor memory, maximum, weights, their way
+// through shared memory to the next product): without the exponentials, the stores or the conversions it is 1 to 4 % faster.
+// Two sequences of up to 4000 tokens, chunks of 512, 12 heads of 64: 41 us; 16 sequences of 8000, 40 rows for each of 4 heads:
+// 59 us at head dim 64, 92 at 128 (one CTA an SM). Where the tiles do not fill the GPU, the blocks of a tile are shared by several
 // CTAs; their states meet in the workspace and the last to come (a counter per tile) joins them.
 #pragma once
 #include <cstddef>
