@@ -364,7 +364,8 @@ int ta_block_tail(const void* att, float* x, const void* w_proj, const float* ln
  *
  * ta_paged_append: rotates the first `rot` dims of k (and q, into q_out (n_rows, Hq, dh) contiguous; q_out NULL: none)
  *   by the position's angles, y1 = x1 cos - x2 sin, y2 = x2 cos + x1 sin on dims i and i + rot / 2 (cosv / sinv
- *   (n_pos, rot / 2) fp32; rot 0: none), in fp32 rounded once to the dtype, and puts k and v into the cache: into the
+ *   (n_pos, rot / 2) fp32; rot 0: none), in fp32 rounded once to the dtype, and puts k and v into the cache (rows of k and v are
+ *   16-byte aligned, base and strides; where rot is a multiple of 16, 0 included, so are q's, q_out and the tables): into the
  *   tail (pages from the last but one on) and, for each page whose last token arrives, into the pool: scale = top / 448,
  *   code = e4m3(x * (448 / top)), top the largest magnitude of the page's page x dh values of that head. Below 2^-100 a
  *   page has codes 0 and scale 1; with an infinity or NaN in it codes 0 and scale NaN. The codes depend on the tokens

@@ -113,3 +113,22 @@ def test_rotation_table():
     assert cos.shape == sin.shape == (50, 4) and cos.dtype == torch.float32
     assert torch.allclose(cos.double() ** 2 + sin.double() ** 2, torch.ones(50, 4).double(), atol=1e-6)
     assert cos[0].eq(1).all() and abs(float(sin[7, 0]) - 0.6569865987187891) < 1e-7
+
+
+def test_append_refuses_unaligned_queries_and_tables():
+    """Where queries and rotation tables are read in 16-byte pieces (rotations by multiples of 16 dims, none included), a row or
+    a table off that boundary is refused before any launch; k and v always."""
+    from treeattn_b200 import _lib
+    lib = _lib.load()
+    a = 1 << 20  # an aligned address that is never dereferenced
+
+    def append(rot=64, q=a, q_sr=512, q_sh=64, qo=a, cos=a, sin=a, k=a, k_sr=256):
+        return lib.ta_paged_append(a, a, a, 3, 9, 3, 16, 2, 2, 4, 64, k, a, k_sr, 64, 256, 64, 2, a, a, 1, cos, sin, 100, rot,
+                                   q, 8, q_sr, q_sh, qo, None)
+
+    for kw, what in ((dict(q=a + 2), 'q and q_out'), (dict(q_sr=513), 'q and q_out'), (dict(q_sh=68), 'q and q_out'),
+                     (dict(qo=a + 2), 'q and q_out'), (dict(cos=a + 4), 'tables'), (dict(sin=a + 8), 'tables'),
+                     (dict(rot=0, q=a + 2, cos=None, sin=None), 'q and q_out'), (dict(rot=32, qo=a + 8), 'q and q_out'),
+                     (dict(rot=24, k=a + 2), 'k and v'), (dict(k_sr=260), 'k and v')):
+        assert append(**kw) == _lib.TA_ERR_ARG, kw
+        assert 'ta_paged_append' in _lib.last_error() and what in _lib.last_error(), (kw, _lib.last_error())

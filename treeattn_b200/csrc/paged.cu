@@ -227,6 +227,12 @@ int ta_paged_append(void* pool, void* tail, const int32_t* table, int64_t table_
   if (!k || !v || (rot && (!cosv || !sinv || n_pos < 1)) || (q_out && !q)) return fail(TA_ERR_ARG, "%s: null pointer", who);
   if (!rows_aligned(k, 2, {k_sr, k_sh}) || !rows_aligned(v, 2, {v_sr, v_sh}))
     return fail(TA_ERR_ARG, "%s: k and v rows must be 16-byte aligned", who);
+  if (rot % 16 == 0) {  // pairs by eight: queries and tables are read in 16-byte pieces too (otherwise element by element)
+    if (q_out && (!rows_aligned(q, 2, {q_sr, q_sh}) || !aligned16(q_out)))
+      return fail(TA_ERR_ARG, "%s: q and q_out rows must be 16-byte aligned", who);
+    if (rot && (!aligned16(cosv) || !aligned16(sinv)))
+      return fail(TA_ERR_ARG, "%s: the rotation's tables must be 16-byte aligned", who);
+  }
   ta::AppendParams p{};
   p.c = {reinterpret_cast<unsigned char*>(pool), tail, table, table_sb, n_pages, max_pages, Hkv, page};
   p.k = k; p.v = v; p.q = q;

@@ -174,7 +174,8 @@ def _heads(name, cache, x, dtype):
 
 def paged_append(cache, k, v, start, pos, max_new, q=None, rotation=None, q_out=None):
     """Puts new rows into the cache: sequence b's rows [start[b], start[b + 1]) of k and v (n, n_kv_head, head_dim) (any row
-    and head strides) go to positions pos[b], pos[b] + 1, .... `max_new` bounds the rows of one sequence. rotation = (cos, sin)
+    and head strides that keep rows 16-byte aligned; q and the tables too where they rotate by multiples of 16 dims) go to
+    positions pos[b], pos[b] + 1, .... `max_new` bounds the rows of one sequence. rotation = (cos, sin)
     (rotation_table) turns the first dims of k, and of q (n, n_head, head_dim) into q_out (allocated here when not given).
     Without a rotation q is returned as it is. A page is quantised when its last token arrives; afterwards a sequence may be
     cut back to any length whose page is the last or last but one that was ever written."""
