@@ -132,3 +132,44 @@ def test_append_refuses_unaligned_queries_and_tables():
                      (dict(rot=24, k=a + 2), 'k and v'), (dict(k_sr=260), 'k and v')):
         assert append(**kw) == _lib.TA_ERR_ARG, kw
         assert 'ta_paged_append' in _lib.last_error() and what in _lib.last_error(), (kw, _lib.last_error())
+
+
+class _Gpu(torch.Tensor):
+    """A host tensor that says it is on a GPU: what the checks of a call let through, with no call made."""
+    is_cuda = property(lambda self: True)
+
+
+def _gpu(*shape, dtype=torch.bfloat16):
+    return torch.zeros(*shape, dtype=dtype).as_subclass(_Gpu)
+
+
+def _stub_cache(monkeypatch):
+    """A cache of 2 sequences (2 kv heads of 64, 16-token pages) whose calls end at the C entry point, which is recorded."""
+    from treeattn_b200 import paged
+    calls = []
+    monkeypatch.setattr(paged, '_call', lambda name, *args: calls.append(name))
+    monkeypatch.setattr(paged, '_stream', lambda t: 0)
+    cache = paged.PagedKV(_gpu(5, 2, 2 * 16 * 64 + 16, dtype=torch.uint8), _gpu(2, 2, 2, 2, 16 * 64),
+                          _gpu(2, 4, dtype=torch.int32), 16, 64)
+    return paged, cache, calls
+
+
+def test_host_buffers_are_refused_before_the_call(monkeypatch):
+    """Outputs and scratch in host memory, and a workspace with gaps, never reach a kernel."""
+    paged, cache, calls = _stub_cache(monkeypatch)
+    start, pos = _gpu(3, dtype=torch.int32), _gpu(2, dtype=torch.int32)
+    k, q = _gpu(2, 2, 64), _gpu(2, 4, 64)
+    rot = (_gpu(8, 32, dtype=torch.float32), _gpu(8, 32, dtype=torch.float32))
+    ws = _gpu(1 << 16, dtype=torch.uint8)
+    with pytest.raises(ValueError, match='paged_append.*CUDA'):
+        paged.paged_append(cache, k, k, start, pos, 1, q=q, rotation=rot, q_out=torch.zeros(2, 4, 64, dtype=torch.bfloat16))
+    with pytest.raises(ValueError, match='paged_attn.*CUDA'):
+        paged.paged_attn(cache, q, start, pos, 1, ws=ws, lse=torch.zeros(2, 4))
+    with pytest.raises(ValueError, match='paged_attn.*CUDA'):
+        paged.paged_attn(cache, q, start, pos, 1, ws=torch.zeros(1 << 16, dtype=torch.uint8))
+    with pytest.raises(ValueError, match='ws must be contiguous'):
+        paged.paged_attn(cache, q, start, pos, 1, ws=ws[::2])
+    assert calls == []
+    paged.paged_append(cache, k, k, start, pos, 1, q=q, rotation=rot, q_out=_gpu(2, 4, 64))
+    paged.paged_attn(cache, q, start, pos, 1, ws=ws, lse=_gpu(2, 4, dtype=torch.float32))
+    assert calls == ['ta_paged_append', 'ta_paged_attn']

@@ -210,6 +210,8 @@ def paged_append(cache, k, v, start, pos, max_new, q=None, rotation=None, q_out=
                 q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
             elif q_out.shape != qshape or q_out.dtype is not dt or not q_out.is_contiguous():
                 raise ValueError('paged_append: q_out must be contiguous, of q\'s shape and type')
+            elif not q_out.is_cuda:
+                _need_cuda('paged_append', q_out)
             qp, qo = q.data_ptr(), q_out.data_ptr()
         else:
             q_out = q
@@ -249,6 +251,10 @@ def paged_attn(cache, q, start, pos, max_new, scale=None, window=0, out=None, ls
         raise ValueError('paged_attn: lse must be (n, n_head) fp32, contiguous')
     if ws is None:
         ws = paged_attn_workspace(B, Hq, H, dh, max_new, q.device)
+    elif not ws.is_contiguous():
+        raise ValueError('paged_attn: ws must be contiguous')
+    if not (ws.is_cuda and (lse is None or lse.is_cuda)):
+        _need_cuda('paged_attn', ws, lse)
     _call('ta_paged_attn', pool.data_ptr(), tail.data_ptr(), table.data_ptr(), table.stride(0), n_pages, table.shape[1],
           cache.page, _DT[dt], B, Hq, H, dh, q.data_ptr(), qs[0], qs[1], n, start.data_ptr(), pos.data_ptr(), max_new,
           1.0 / math.sqrt(dh) if scale is None else scale, window, out.data_ptr(), os[0], os[1], _p(lse), ws.data_ptr(),
