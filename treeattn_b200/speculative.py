@@ -49,7 +49,9 @@ class PagedDecoder:
 
     @torch.no_grad()
     def forward(self, tok):
-        """Feeds tok (batch, n) at the sequences' next positions and returns the logits (batch, n, vocabulary) after each."""
+        """Feeds tok (batch, n) (whole numbers, on any device) at the sequences' next positions and returns the logits (batch, n,
+        vocabulary) after each."""
+        tok = tok.to(self.dev, torch.int64)
         B, n = tok.shape
         if B != self.batch:
             raise ValueError('PagedDecoder: %d sequences for a batch of %d' % (B, self.batch))
