@@ -188,3 +188,32 @@ def test_example_runs():
                         '100', '--tokens', '12'], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr[-2000:]
     assert 'tokens/s' in r.stdout
+
+
+@pytest.mark.parametrize('neighbors', [False, True])
+def test_a_context_is_used_to_its_last_position(neighbors):
+    """Rounds up to the last position of the caches, with the fused draft kernel and with a draft that borrows neighbours' leaves
+    (its stored leaves are indexed by position): every position is generated, nothing is fed beyond, then a round is refused. The
+    tokens are the dense model's (greedy)."""
+    from treeattn_b200.config import Config
+    from treeattn_b200.speculative import SpeculativeDecoder
+    cfg, W = _model(3, seq_len=128)
+    cfg = Config(**dict(cfg.to_dict(), neighbors=neighbors))
+    B, T = 2, 90
+    draft, target = _pair(cfg, W, B)
+    dec = SpeculativeDecoder(draft, target, 4, temperature=0)
+    prompt = torch.randint(cfg.vocab_size, (B, T), generator=torch.Generator().manual_seed(4))
+    out = [[int(t)] for t in dec.prefill(prompt)]
+    while max(target.pos) < 128:
+        for o, x in zip(out, dec.step()):
+            o.extend(x)
+    with pytest.raises(ValueError, match='all 128 positions'):
+        dec.step()
+    from treeattn_b200 import _ops
+    assert _ops.device_error()[0] == 0
+    assert target.pos == [T + len(o) - 1 for o in out]
+    for b in range(B):
+        idx = torch.cat([prompt[b], torch.tensor(out[b])])[None].to(DEV)
+        logits = _dense(W, cfg, idx[:, :-1], torch.bfloat16)[0, T - 1:]
+        chosen = logits.gather(1, idx[0, T:, None])[:, 0]
+        assert (logits.max(-1).values - chosen <= 0.5 * logits.std()).all()

@@ -47,3 +47,63 @@ def test_token_ids_reach_the_embedding_as_int64(host_model, dtype):
     got, pos = host_model.seen[-1]
     assert got.dtype is torch.int64 and got.is_contiguous() and got.tolist() == tok.reshape(-1).tolist()
     assert pos.tolist() == list(range(6)) * 2
+
+
+class Draft:
+    """A draft model that says which positions it was fed, and refuses those beyond its cache as the device would."""
+
+    def __init__(self, batch, cap, vocab, table=None):
+        self.batch, self.cap, self.vocab, self.cfg, self.fed = batch, cap, vocab, None, []
+        self.W = dict(wpe=torch.zeros(table or cap, 8))
+
+    def prefill(self, idx):
+        self.fed.append(list(range(idx.shape[1])))
+
+    def step(self, tok, at):
+        assert int(at.max()) < min(self.cap, self.W['wpe'].shape[0]), 'fed a position beyond its cache'
+        self.fed.append(at.tolist())
+        return torch.zeros(self.batch, self.vocab), None
+
+
+def _verified(p, q, drafts, u, n_draft=None):
+    """Every draft stands, token 1 follows."""
+    B, G = drafts.shape
+    assert p.shape[:2] == (B, G + 1) and q.shape[:2] == (B, G) and u.shape == (B, G + 1)
+    return torch.cat([drafts, torch.ones(B, 1, dtype=torch.int64)], 1), torch.full((B,), G, dtype=torch.int32)
+
+
+@pytest.mark.parametrize('max_len,cap,table', [(64, 64, 64), (64, 40, 64), (40, 64, 64), (64, 64, 40)])
+def test_rounds_end_at_the_last_position(host_model, monkeypatch, max_len, cap, table):
+    """No model is fed a position beyond the smaller cache; the last rounds draft fewer, the last position is used, and then a
+    round is refused before anything runs."""
+    from treeattn_b200 import speculative
+    monkeypatch.setattr(speculative, 'verify_drafts', _verified)
+    room = min(max_len, cap, table)
+    target, draft = host_model(max_len=max_len), Draft(2, cap, 64, table)
+    dec = speculative.SpeculativeDecoder(draft, target, 4)
+    dec.prefill(torch.zeros(2, 20, dtype=torch.int64))
+    assert [len(x) for x in dec.step()] == [5, 5]
+    while target.pos[0] < room:
+        assert 1 <= len(dec.step()[0]) <= 5
+    assert target.pos == [room, room] and draft.fed[-1] == [room - 1, room - 1]
+    fed, seen = len(draft.fed), len(host_model.seen)
+    with pytest.raises(ValueError, match='all %d positions' % room):
+        dec.step()
+    assert (len(draft.fed), len(host_model.seen), target.pos) == (fed, seen, [room, room])
+    with pytest.raises(ValueError, match='prompt of'):
+        dec.prefill(torch.zeros(2, room + 1, dtype=torch.int64))
+    assert len(draft.fed) == fed
+
+
+def test_the_longest_sequence_sets_the_round(host_model, monkeypatch):
+    """Uneven lengths: a round is as long as the longest sequence leaves room for."""
+    from treeattn_b200 import speculative
+    monkeypatch.setattr(speculative, 'verify_drafts', _verified)
+    target, draft = host_model(max_len=32), Draft(2, 32, 64)
+    dec = speculative.SpeculativeDecoder(draft, target, 4)
+    dec.prefill(torch.zeros(2, 30, dtype=torch.int64))
+    target.cut_back([30, 22])
+    assert [len(x) for x in dec.step()] == [2, 2]
+    assert target.pos == [32, 24]
+    with pytest.raises(ValueError, match='all 32'):
+        dec.step()

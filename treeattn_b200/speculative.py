@@ -89,7 +89,8 @@ class PagedDecoder:
 
 class SpeculativeDecoder:
     """draft: an engine.Decoder (mode 'seg') over the same vocabulary; target: a PagedDecoder, both of one batch size and both
-    prefilled by prefill(). Each step drafts `n_draft` tokens of every sequence and verifies them. temperature 0 is greedy.
+    prefilled by prefill(). Each step drafts `n_draft` tokens of every sequence (fewer where the longest one nears the end of
+    either cache, none for the last position) and verifies them. temperature 0 is greedy.
     generator: where the draws come from (a CUDA generator; default: torch's)."""
 
     def __init__(self, draft, target, n_draft=4, temperature=1.0, generator=None):
@@ -101,6 +102,7 @@ class SpeculativeDecoder:
         if cfg is not None and cfg.beam_mode == 'pred' and cfg.global_pool:
             raise ValueError('SpeculativeDecoder: a budget head over the running key mean cannot take drafts back')
         self.draft, self.target, self.G = draft, target, n_draft
+        self.room = min(target.max_len, draft.cap, draft.W['wpe'].shape[0])  # positions that both hold
         self.temperature, self.generator = float(temperature), generator
         self.last = None     # (batch,) the newest token of each sequence, not fed yet
         self.accepted = 0    # drafts that stood so far, of all sequences
@@ -114,6 +116,8 @@ class SpeculativeDecoder:
     @torch.no_grad()
     def prefill(self, idx):
         """Runs prompts idx (batch, T) through both models; returns the first new token of each sequence."""
+        if idx.shape[1] > self.room:
+            raise ValueError('SpeculativeDecoder: a prompt of %d positions for caches of %d' % (idx.shape[1], self.room))
         self.draft.prefill(idx)
         logits = self.target.forward(idx.to(self.target.dev))[:, -1]
         self.last = torch.multinomial(self._probs(logits), 1, generator=self.generator)[:, 0]
@@ -121,9 +125,14 @@ class SpeculativeDecoder:
 
     @torch.no_grad()
     def step(self):
-        """One round: the new tokens of each sequence (a list of lists, 1 to n_draft + 1 of them)."""
-        B, G, dev = self.draft.batch, self.G, self.target.dev
+        """One round: the new tokens of each sequence (a list of lists, 1 to n_draft + 1 of them). Raises ValueError, with nothing
+        run, when a sequence has no position left."""
+        B, dev = self.draft.batch, self.target.dev
         base = list(self.target.pos)
+        left = self.room - max(base)  # the newest token takes one position, each draft another
+        if left < 1:
+            raise ValueError('SpeculativeDecoder: a sequence holds all %d positions' % self.room)
+        G = min(self.G, left - 1)
         tok, drafts, probs = self.last, [], []
         at = torch.tensor(base, dtype=torch.int32).to(dev)
         for i in range(G + 1):  # the last round only puts the last draft into the draft's cache
@@ -133,10 +142,10 @@ class SpeculativeDecoder:
                 tok = torch.multinomial(q, 1, generator=self.generator)[:, 0]
                 drafts.append(tok)
                 probs.append(q)
-        drafts = torch.stack(drafts, 1)
+        drafts = torch.stack(drafts, 1) if G else self.last.new_empty(B, 0)
         p = self._probs(self.target.forward(torch.cat([self.last[:, None], drafts], 1)))
         u = torch.rand(B, G + 1, device=dev, generator=self.generator)
-        tokens, accepted = verify_drafts(p, torch.stack(probs, 1), drafts, u)
+        tokens, accepted = verify_drafts(p, torch.stack(probs, 1) if G else p[:, :0], drafts, u)
         self.last = tokens.gather(1, accepted[:, None].long())[:, 0]
         n = accepted.tolist()
         self.target.cut_back([b + 1 + a for b, a in zip(base, n)])
