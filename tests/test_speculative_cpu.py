@@ -107,3 +107,17 @@ def test_the_longest_sequence_sets_the_round(host_model, monkeypatch):
     assert target.pos == [32, 24]
     with pytest.raises(ValueError, match='all 32'):
         dec.step()
+
+
+def test_a_second_prompt_starts_anew(host_model, monkeypatch):
+    """prefill() begins both models at position 0 again, with every page of the last prompt free."""
+    from treeattn_b200 import speculative
+    monkeypatch.setattr(speculative, 'verify_drafts', _verified)
+    target, draft = host_model(max_len=96, n_pages=12), Draft(2, 96, 64)
+    dec = speculative.SpeculativeDecoder(draft, target, 4)
+    for T in (85, 20, 90):
+        dec.prefill(torch.zeros(2, T, dtype=torch.int64))
+        assert target.pos == [T, T] and host_model.seen[-1][1].tolist() == list(range(T)) * 2
+        dec.step()
+        assert draft.fed[-5:] == [[T + i] * 2 for i in range(5)] and target.pos == [T + 5, T + 5]
+        assert sorted(target.pool.free + sum(target.pool.owned, [])) == list(range(12))

@@ -47,6 +47,12 @@ class PagedDecoder:
             self._ws[n] = paged_attn_workspace(self.batch, self.H, self.H, self.dh, n, self.dev)
         return self._start[n], self._ws[n]
 
+    def reset(self):
+        """Empties every sequence and gives its pages back."""
+        for b in range(self.batch):
+            self.pool.release(b)
+        self.pos, self._floor = [0] * self.batch, [0] * self.batch
+
     @torch.no_grad()
     def forward(self, tok):
         """Feeds tok (batch, n) (whole numbers, on any device) at the sequences' next positions and returns the logits (batch, n,
@@ -115,9 +121,11 @@ class SpeculativeDecoder:
 
     @torch.no_grad()
     def prefill(self, idx):
-        """Runs prompts idx (batch, T) through both models; returns the first new token of each sequence."""
+        """Runs new prompts idx (batch, T) through both models, whatever they held before; returns the first new token of each
+        sequence."""
         if idx.shape[1] > self.room:
             raise ValueError('SpeculativeDecoder: a prompt of %d positions for caches of %d' % (idx.shape[1], self.room))
+        self.target.reset()
         self.draft.prefill(idx)
         logits = self.target.forward(idx.to(self.target.dev))[:, -1]
         self.last = torch.multinomial(self._probs(logits), 1, generator=self.generator)[:, 0]
