@@ -121,3 +121,16 @@ def test_a_second_prompt_starts_anew(host_model, monkeypatch):
         dec.step()
         assert draft.fed[-5:] == [[T + i] * 2 for i in range(5)] and target.pos == [T + 5, T + 5]
         assert sorted(target.pool.free + sum(target.pool.owned, [])) == list(range(12))
+
+
+def test_cut_back_wants_a_length_for_every_sequence(host_model):
+    """Fewer lengths than sequences would leave the embedding fewer positions than rows."""
+    dec = host_model(batch=3)
+    dec.forward(torch.zeros(3, 9, dtype=torch.int64))
+    for bad in ([8], [8, 8], [8] * 4):
+        with pytest.raises(ValueError, match='lengths for a batch of 3'):
+            dec.cut_back(bad)
+    assert dec.pos == [9, 9, 9]
+    dec.cut_back([8, 9, 0])
+    dec.forward(torch.zeros(3, 2, dtype=torch.int64))
+    assert host_model.seen[-1][1].tolist() == [8, 9, 9, 10, 0, 1]

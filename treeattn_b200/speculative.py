@@ -87,6 +87,8 @@ class PagedDecoder:
     def cut_back(self, pos):
         """Drops positions from pos[b] on (rejected drafts). A sequence can lose what is still in 16 bits: back to the start of
         the page before the furthest one written."""
+        if len(pos) != self.batch:
+            raise ValueError('PagedDecoder: %d lengths for a batch of %d' % (len(pos), self.batch))
         for b, (old, new) in enumerate(zip(self.pos, pos)):
             if not max(0, self._floor[b]) <= new <= old:
                 raise ValueError('PagedDecoder: sequence %d cannot go from %d back to %d positions' % (b, old, new))
