@@ -134,3 +134,28 @@ def test_cut_back_wants_a_length_for_every_sequence(host_model):
     dec.cut_back([8, 9, 0])
     dec.forward(torch.zeros(3, 2, dtype=torch.int64))
     assert host_model.seen[-1][1].tolist() == [8, 9, 9, 10, 0, 1]
+
+
+def test_prompts_of_many_lengths_keep_one_workspace(host_model, monkeypatch):
+    """What the decoder holds for its calls does not grow with the lengths it has seen: one workspace of the largest size, few row
+    offsets, each call's workspace large enough for it."""
+    from treeattn_b200 import speculative
+    from treeattn_b200.paged import paged_attn_workspace
+    given = []
+
+    def attn(c, q, start, pos, n, ws=None, **k):
+        assert start.tolist() == [0, n, 2 * n]
+        given.append((n, ws))
+        return q.contiguous()
+
+    monkeypatch.setattr(speculative, 'paged_attn', attn)
+    dec = host_model()
+    lengths = [1, 5] + list(range(7, 120, 4)) + [1, 5, 100]
+    for n in lengths:
+        dec.reset()
+        dec.forward(torch.zeros(2, n, dtype=torch.int64))
+    need = {n: paged_attn_workspace(2, 2, 2, 16, n, 'cpu').nbytes for n in lengths}
+    assert all(ws.nbytes >= need[n] for n, ws in given) and dec._ws.nbytes == max(need.values())
+    held = [x for v in vars(dec).values() for x in (v.values() if isinstance(v, dict) else [v]) if torch.is_tensor(x)
+            and x.dtype is torch.uint8]
+    assert sum(x.nbytes for x in held) == max(need.values()) and len(dec._start) <= 16

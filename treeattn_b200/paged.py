@@ -221,11 +221,14 @@ def paged_append(cache, k, v, start, pos, max_new, q=None, rotation=None, q_out=
     return q_out
 
 
+def _workspace_bytes(batch, n_head, n_kv_head, head_dim, max_new):
+    return max(_lib.load().ta_paged_attn_workspace(int(batch), int(n_head), int(n_kv_head), int(head_dim), int(max_new)), 16)
+
+
 def paged_attn_workspace(batch, n_head, n_kv_head, head_dim, max_new, device='cuda'):
     """A zeroed workspace for paged_attn at these sizes: one per stream of calls, kept by the caller. Calls of other sizes
     may share it when it is large enough for each."""
-    n = _lib.load().ta_paged_attn_workspace(int(batch), int(n_head), int(n_kv_head), int(head_dim), int(max_new))
-    return torch.zeros(max(int(n), 16), device=device, dtype=torch.uint8)
+    return torch.zeros(_workspace_bytes(batch, n_head, n_kv_head, head_dim, max_new), device=device, dtype=torch.uint8)
 
 
 def paged_attn(cache, q, start, pos, max_new, scale=None, window=0, out=None, lse=None, ws=None):

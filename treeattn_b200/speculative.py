@@ -7,7 +7,7 @@ model's own sampling."""
 import torch
 
 from . import _ops
-from .paged import PagedKV, PagePool, paged_append, paged_attn, paged_attn_workspace, verify_drafts
+from .paged import PagedKV, PagePool, _workspace_bytes, paged_append, paged_attn, paged_attn_workspace, verify_drafts
 
 
 class PagedDecoder:
@@ -16,7 +16,8 @@ class PagedDecoder:
 
     W: a decoder weight dict (engine.weights_from_ours / weights_from_nanogpt). max_len: positions of a sequence (at most the
     model's position table). n_pages: pages of the pool, shared by the layers' tables (default: enough for every sequence at
-    max_len). rotation: (cos, sin) of paged.rotation_table for models that rotate their keys and queries."""
+    max_len). rotation: (cos, sin) of paged.rotation_table for models that rotate their keys and queries.
+    max_new: new tokens of a sequence in a call that the workspace is made for (it grows where a call has more)."""
 
     def __init__(self, W, n_layer, n_head, n_embd, batch=1, max_len=None, page=64, n_pages=None, dtype=torch.bfloat16,
                  dev='cuda', rotation=None, max_new=8):
@@ -38,14 +39,24 @@ class PagedDecoder:
         self.pos = [0] * batch     # positions that each sequence holds
         self._floor = [0] * batch  # and how far back it can be cut: the start of the page before the furthest one written
         self._start = {}
-        self._ws = {}
+        self._ws = None
+        self._grow(max_new)
+
+    def _grow(self, n):
+        """One workspace for the calls of every length (they run one after the other), as large as the largest one asked for."""
+        sizes = self.batch, self.H, self.H, self.dh, n
+        if self._ws is None or _workspace_bytes(*sizes) > self._ws.nbytes:
+            self._ws = paged_attn_workspace(*sizes, self.dev)
 
     def _plan(self, n):
-        """Row offsets of n rows a sequence, and the attention's workspace for them: kept, one per n."""
+        """Row offsets of n rows a sequence (kept for the lengths that come up most, drafts and single tokens: a call less), and
+        the attention's workspace."""
         if n not in self._start:
+            if len(self._start) >= 16:
+                self._start.clear()
             self._start[n] = torch.arange(self.batch + 1, device=self.dev, dtype=torch.int32) * n
-            self._ws[n] = paged_attn_workspace(self.batch, self.H, self.H, self.dh, n, self.dev)
-        return self._start[n], self._ws[n]
+            self._grow(n)
+        return self._start[n], self._ws
 
     def reset(self):
         """Empties every sequence and gives its pages back."""
