@@ -159,3 +159,12 @@ def test_prompts_of_many_lengths_keep_one_workspace(host_model, monkeypatch):
     held = [x for v in vars(dec).values() for x in (v.values() if isinstance(v, dict) else [v]) if torch.is_tensor(x)
             and x.dtype is torch.uint8]
     assert sum(x.nbytes for x in held) == max(need.values()) and len(dec._start) <= 16
+
+
+def test_rotation_table_covers_the_context(host_model):
+    """Positions beyond the tables would be left out of the cache; a rotation of more dims than a head has is refused at once too."""
+    from treeattn_b200.paged import rotation_table
+    host_model(max_len=100, rotation=rotation_table(100, 16, device='cpu'))
+    for n, rot in ((99, 16), (128, 18)):
+        with pytest.raises(ValueError, match='rotation of %d positions and %d dims' % (n, rot)):
+            host_model(max_len=100, rotation=rotation_table(n, rot, device='cpu'))

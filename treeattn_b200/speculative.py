@@ -33,6 +33,9 @@ class PagedDecoder:
         self.max_len = int(max_len or W['wpe'].shape[0])
         if self.max_len > W['wpe'].shape[0]:
             raise ValueError('PagedDecoder: max_len %d above the position table\'s %d' % (self.max_len, W['wpe'].shape[0]))
+        if rotation is not None and (rotation[0].shape[0] < self.max_len or 2 * rotation[0].shape[1] > self.dh):
+            raise ValueError('PagedDecoder: a rotation of %d positions and %d dims for %d positions of %d' % (
+                rotation[0].shape[0], 2 * rotation[0].shape[1], self.max_len, self.dh))
         per_seq = -(-self.max_len // page)
         self.pool = PagePool(n_pages or batch * per_seq, batch, per_seq, page, self.dev)
         self.caches = [PagedKV.empty(self.pool.n_pages, n_head, self.dh, self.pool.table, page, dtype) for _ in range(n_layer)]
