@@ -677,3 +677,116 @@ def test_verify_distribution():
     assert first.sum() == B
     sd = (B * p.double() * (1 - p.double())).sqrt()
     assert ((first - B * p.double()).abs() <= 5 * sd + 1e-9).all(), first / B
+
+
+# ------------------------------------------------------------------------------------------------ sizes of the values
+def _value_units(r, b, L):
+    """What one code of each token's value stands for (an upper bound), in 64 bits: the page's scale; in the open page the power of
+    two that takes a 16-token group's largest value into [2^8, 2^9) (at least 1 for f16, which is not scaled down); 2^-64 where
+    all values are 0."""
+    V = r.cache.read(b, L)[1].double().abs()                       # (Hkv, L, dh)
+    u = torch.empty(r.Hkv, L, device=DEV, dtype=torch.float64)
+    full = L // r.page * r.page
+    for a in range(0, L, 16):
+        top = V[:, a:a + 16].amax((-1, -2))
+        if a < full:
+            page = a // r.page * r.page
+            unit = V[:, page:page + r.page].amax((-1, -2)) * 2 / 448  # (a page whose largest value is no multiple of a code)
+        else:
+            unit = top * 2.0 ** -8
+            if r.dt == HF:
+                unit = unit.clamp(min=2.0 ** -30)
+        u[:, a:a + 16] = torch.where(top > 0, unit, 2.0 ** -64)[:, None]
+    return u
+
+
+def _attend_tight(r, q, counts, pos, scale):
+    """As _attend_ref, but a tolerance that scales with the values: no absolute term but the output's last place (f16) and, for
+    every token, half of f16's smallest step (2^-25) of a weight where the largest weight of the row is at least 2^6."""
+    Hq, dh = q.shape[1:]
+    grp = Hq // r.Hkv
+    outs, tols = [], []
+    row = 0
+    for b, n in enumerate(counts):
+        L = pos[b] + n
+        K, V = [x.double() for x in r.cache.read(b, L)]
+        qb = q[row:row + n].double().view(n, r.Hkv, grp, dh).permute(1, 2, 0, 3)
+        s = torch.einsum('hgnd,htd->hgnt', qb, K) * scale
+        mag = torch.einsum('hgnd,htd->hgnt', qb.abs(), K.abs()).amax(-1) * abs(scale)
+        hide = torch.arange(L, device=DEV) > pos[b] + torch.arange(n, device=DEV)[:, None]
+        p = s.masked_fill(hide, -math.inf).softmax(-1)
+        unit = _value_units(r, b, L)
+        u = torch.full((L,), 2.0 ** -11, device=DEV, dtype=torch.float64)
+        u[L // r.page * r.page:] = U[r.dt]
+        d = 2 * dh * 2.0 ** -24 * mag
+        step = 2.0 ** -31 * (p * unit[:, None, None]).amax(-1, keepdim=True) / unit[:, None, None]  # of a token's p
+        part = p * u + p * (2 * d + 1e-5)[..., None] + step.masked_fill(hide, 0)
+        o = torch.einsum('hgnt,htd->nhgd', p, V).reshape(n, Hq, dh)
+        outs.append(o)
+        tols.append(U[r.dt] * o.abs() + torch.einsum('hgnt,htd->nhgd', part, V.abs()).reshape(n, Hq, dh)
+                    + (2.0 ** -25 if r.dt == HF else 2.0 ** -133))
+        row += n
+    return torch.cat(outs), torch.cat(tols)
+
+
+SIZES = [(64, 64, BF, 1, -20), (64, 64, BF, 1, -30), (64, 64, BF, 40, -20), (64, 64, BF, 40, -30), (128, 32, BF, 1, -30),
+         (128, 32, BF, 48, -30), (64, 16, HF, 1, -12), (64, 16, HF, 1, -20), (64, 64, HF, 40, -12), (128, 64, HF, 40, -20),
+         (32, 32, BF, 1, -30), (32, 32, BF, 40, -30), (16, 64, HF, 36, -12), (64, 64, BF, 1, 40), (64, 32, BF, 40, 40),
+         (64, 64, HF, 1, 10), (128, 64, HF, 40, 10), (64, 64, BF, 20, -30), (128, 64, HF, 20, -20)]
+
+
+def _many(n):
+    """Sequences: so many items of 160 kv heads that a warp, or a CTA, holds whole ones (the parts of an item that several share
+    meet in fp32)."""
+    return 8 if n <= 32 else 2
+
+
+@pytest.mark.parametrize('dh,page,dt,n,shift', SIZES)
+def test_attention_of_small_and_large_values(dh, page, dt, n, shift):
+    """Values scaled by a power of two, in full pages and in the open one: the output's error scales with them."""
+    P = _mod()
+    B, H = _many(n), 160
+    r = Rig(B, H, dh, page, dt, 400 + n, seed=dh + n - shift)
+    before = [256 + (i % 2) * (page // 2 + 3) for i in range(B)]
+    N = sum(before)
+    r.append(before, r.randn(N, H, dh), (r.randn(N, H, dh).float() * 2.0 ** shift).to(dt))
+    r.append([n] * B, r.randn(n * B, H, dh), (r.randn(n * B, H, dh).float() * 2.0 ** shift).to(dt))
+    q = r.randn(B * n, H, dh)
+    got = P.paged_attn(r.cache, q, _starts([n] * B), _i32(before), n)
+    want, tol = _attend_tight(r, q, [n] * B, before, 1 / math.sqrt(dh))
+    d = (got.double() - want).abs()
+    assert (d <= tol).all(), float((d / tol).max())
+    _no_device_error()
+
+
+@pytest.mark.parametrize('dh,page,dt,n,shift', SIZES)
+def test_attention_beside_zero_values(dh, page, dt, n, shift):
+    """Pages of zeros (which store scale 1) before and between pages of scaled values, 16 tokens of zeros inside another, and, in
+    every second sequence, an open page of zeros: they weigh what their scores say and the others keep their precision."""
+    P = _mod()
+    B, H = _many(n), 160
+    r = Rig(B, H, dh, page, dt, 400 + n, seed=dh + n + shift)
+    before = [256 + (i % 2) * (page // 2 + 3) for i in range(B)]
+    N = sum(before)
+    k, v = r.randn(N, H, dh, spread=2.0), (r.randn(N, H, dh).float() * 2.0 ** shift).to(dt)
+    new = (r.randn(n * B, H, dh).float() * 2.0 ** shift).to(dt)
+    row = 0
+    for b in range(B):
+        for a in (0, 128):
+            v[row + a:row + a + 64] = 0
+        v[row + 80:row + 96] = 0
+        if b % 2:
+            v[row + 256:row + before[b]] = 0
+            new[b * n:(b + 1) * n] = 0
+        row += before[b]
+    r.append(before, k, v)
+    r.append([n] * B, r.randn(n * B, H, dh), new)
+    q = r.randn(B * n, H, dh)
+    lse = torch.empty(B * n, H, device=DEV)
+    got = P.paged_attn(r.cache, q, _starts([n] * B), _i32(before), n, lse=lse)
+    want, tol = _attend_tight(r, q, [n] * B, before, 1 / math.sqrt(dh))
+    d = (got.double() - want).abs()
+    assert (d <= tol).all(), float((d / tol).max())
+    _, _, wl, ltol = _attend_ref(r, q, [n] * B, before, 1 / math.sqrt(dh), 0)
+    assert ((lse.double() - wl).abs() <= ltol).all()
+    _no_device_error()

@@ -400,8 +400,8 @@ __global__ void __launch_bounds__(APPEND_THREADS) paged_append_kernel(AppendPara
 //  * codes go to f16 exactly; q is scaled by a power of two per row (exact, undone in the score's factor) so that bf16
 //    rows fit f16 as well; the products are exact and the sums fp32.
 //  * the value scale joins the weight: w_t = exp2(s_t + log2 vs - ref), with the running reference taken over s + log2 vs, so
-//    that every w stays in f16's range (at most 2^12); the denominator adds w / vs in fp32. w is rounded to f16 (2^-12
-//    relative) for the product, the denominator takes it unrounded.
+//    that every w stays in f16's range (at most 2^12); the denominator adds w / vs in fp32. w is rounded to f16 (2^-11
+//    relative, 2^-25 of 1 below 2^-14) for the product, the denominator takes it unrounded.
 //  * the open page is read in 16 bits from the tail, in the same element order, with the 16-bit type's own mma.
 constexpr float ATTN_SHIFT = 12.f;
 
@@ -472,6 +472,26 @@ template <>
 __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
+}
+// A page whose values are all 0 (or below 2^-100) stores scale 1, whatever the pages beside it hold. Taken as it stands it would
+// lift the reference 2^20 and more above pages of small values, whose weights then fall among f16's subnormals (values of
+// 1e-6 behind such a page: 7 % off). Its codes are 0, so any scale will do: 2^-64 lets its tokens weigh what their scores say
+// while those of values between 2^-75 and 2^49 keep their bits. (The open page needs none: it is the last that a running
+// softmax takes, and what came before it is in fp32 by then.)
+constexpr float ZERO_LOG2 = -64.f;
+template <int DH>
+__device__ __forceinline__ void value_factors(float vs, const unsigned char* vp, float& lv, float& iv) {
+  lv = log2_fast(vs);
+  iv = rcp_fast(vs);
+  if (vs == 1.f) {  // one page of a warp at a time: no lane stays behind
+    uint32_t any = 0;
+#pragma unroll 1
+    for (int i = threadIdx.x & 31; i < DH * 4; i += 32) any |= reinterpret_cast<const uint32_t*>(vp)[i];
+    if (!__any_sync(0xffffffffu, any & 0x7f7f7f7fu)) {
+      lv = ZERO_LOG2;
+      iv = 18446744073709551616.f;  // 2^64
+    }
+  }
 }
 // The rows of one tile: query fragments and what the masks and scores need, per lane for its two columns of each n-tile.
 template <typename T, int DH, int NT>
@@ -818,8 +838,7 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32) paged_attn_kernel(AttnParams 
       vp[x] = kp[x] + P * DH;
       const float2 sc = *reinterpret_cast<const float2*>(rec + 2 * P * DH);
       ks[x] = sc.x;
-      lv[x] = log2_fast(sc.y);
-      iv[x] = rcp_fast(sc.y);
+      value_factors<DH>(sc.y, vp[x], lv[x], iv[x]);
     }
     const int tok0 = u * P;
     const bool mask = tok0 + 63 > min(qlo, limit - 1) || (p.window > 0 && tok0 <= qhi - p.window);
@@ -1319,8 +1338,7 @@ __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
             vp[x] = kp[x] + Pe * DH;
             const float2 sc = *reinterpret_cast<const float2*>(rp + 2 * Pe * DH);
             ks[x] = sc.x;
-            lv[x] = log2_fast(sc.y);
-            iv[x] = rcp_fast(sc.y);
+            value_factors<DH>(sc.y, vp[x], lv[x], iv[x]);
           }
           attend_codes<T, DH, NT, TG>(rt, st, kp, vp, ks, lv, iv, tok0 + y * 16, limit, p.window, mask);
         }

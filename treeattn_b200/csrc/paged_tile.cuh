@@ -289,8 +289,17 @@ __global__ void __launch_bounds__(TILE_THREADS, TileShape<T, DH>::CTAS) paged_ti
             *reinterpret_cast<uint4*>(tile_piece(tileK, row + 8 * r, 2 * t)) = make_uint4(f[0], f[1], f[2], f[3]);
             *reinterpret_cast<uint4*>(tile_piece(tileK, row + 8 * r, 2 * t + 1)) = make_uint4(f[4], f[5], f[6], f[7]);
           }
-        if (lane == 0)
-          *reinterpret_cast<float4*>(bar.scale[n & 3][cw]) = make_float4(sc.x, log2_fast(sc.y), rcp_fast(sc.y), 0.f);
+        float lv = log2_fast(sc.y), iv = rcp_fast(sc.y);
+        if (sc.y == 1.f) {  // (one page: the warp's lanes agree) values of 0 do not set the reference, see value_factors
+          uint32_t any = 0;
+#pragma unroll
+          for (int x = 0; x < VW; ++x) any |= vw[x];
+          if (!__any_sync(0xffffffffu, any & 0x7f7f7f7fu)) {
+            lv = ZERO_LOG2;
+            iv = 18446744073709551616.f;
+          }
+        }
+        if (lane == 0) *reinterpret_cast<float4*>(bar.scale[n & 3][cw]) = make_float4(sc.x, lv, iv, 0.f);
         filled(bar.k_full);
         if (!free_of(bar.o_full, 11)) return false;
 #pragma unroll
