@@ -352,8 +352,8 @@ int ta_block_tail(const void* att, float* x, const void* w_proj, const float* ln
 /* Serving over an 8-bit paged key / value cache (no counterpart in the reference, whose cache is one fp32 tensor per
  * sequence).
  * A page holds `page` tokens (16, 32 or 64) of one sequence. pool (n_pages, Hkv, 2 * page * dh + 16) bytes: per (page, kv
- * head) the e4m3 codes of its keys, those of its values, the fp32 scales of the two (value = code * scale) and 8 unused
- * bytes. tail (B, Hkv, 2, 2, page * dh) in `dtype` (bf16 or f16): the open page of each sequence and the page before it,
+ * head) the e4m3 codes of its keys, those of its values, the fp32 scales of the two (value = code * scale), a mark (fp32: 1
+ * where every value code is 0 for want of a value above 2^-100, else 0) and 4 unused bytes. tail (B, Hkv, 2, 2, page * dh) in `dtype` (bf16 or f16): the open page of each sequence and the page before it,
  * by page parity, keys then values. table (B, max_pages) int32, row stride table_sb: the pool page of each page of a
  * sequence, read for full pages only. Inside a page the elements of each 16-token group stand in fragment order:
  *   keys   [h][r][g][t][e]          token 8 r + g, dim h * 4E + t * E + e (E = min(16, dh / 4); r 2, g 8, t 4)

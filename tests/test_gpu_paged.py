@@ -790,3 +790,27 @@ def test_attention_beside_zero_values(dh, page, dt, n, shift):
     _, _, wl, ltol = _attend_ref(r, q, [n] * B, before, 1 / math.sqrt(dh), 0)
     assert ((lse.double() - wl).abs() <= ltol).all()
     _no_device_error()
+
+
+@pytest.mark.parametrize('page,dh,dt', [(16, 64, BF), (64, 128, HF), (32, 16, BF)])
+def test_pages_of_zero_values_are_marked(page, dh, dt):
+    """The record's third word is 1 for pages whose values are all 0 (or below 2^-100), whatever the keys hold, and 0 for every other
+    page, one that is quantised again with values among them."""
+    r = Rig(5, 1, dh, page, dt, 2 * page)
+    k, v = r.randn(5 * page, 1, dh), r.randn(5 * page, 1, dh)
+    v[:page] = 0
+    v[page:2 * page] = -0.0
+    k[2 * page:3 * page] = 0
+    v[3 * page + 1, 0, 2] = math.nan
+    v[4 * page:] = 448.0 if dt == BF else 1.0
+    if dt == BF:
+        v[page + 3] = 2.0 ** -104
+
+    def marks():
+        return [float(r.cache.pool[int(r.perm[b, 0])].view(torch.float32)[0, -2]) for b in range(5)]
+
+    r.append([page] * 5, k, v)
+    assert marks() == [1, 1, 0, 0, 0]
+    r.append([1] * 5, r.randn(5, 1, dh), r.randn(5, 1, dh), pos=[page - 1] * 5)  # the last token of each page replaced
+    assert marks() == [0, 0, 0, 0, 0]
+    _no_device_error()

@@ -1,7 +1,8 @@
 // The 8-bit paged key / value cache: its layout, appending to it with the position rotation, and attention over it.
 //
 // A page holds P tokens (16, 32 or 64) of one sequence. The pool keeps one record of 2 * P * DH + 16 bytes per (page,
-// kv head): the e4m3 codes of the keys, those of the values, then the fp32 scales of the two; value = code * scale. A page
+// kv head): the e4m3 codes of the keys, those of the values, then the fp32 scales of the two and a mark (1: all values are 0);
+// value = code * scale. A page
 // is quantised once, when its last token arrives, from 16-bit values: until then its tokens live in the 16-bit tail, a
 // ring of two pages per (sequence, kv head) addressed by the page's parity. So the codes depend on the tokens alone, not on
 // how they arrived, and a sequence can be cut back to any length whose last page is still in the ring.
@@ -104,6 +105,7 @@ __device__ __forceinline__ void store_words(void* p, const uint32_t (&w)[BYTES /
 // A page whose top is below 2^-100 has codes 0 and scale 1; one that holds an infinity or NaN has codes 0 and scale NaN, so
 // that it reads back as NaN.
 constexpr int APPEND_THREADS = 128;
+constexpr float ZERO_MARK = 1.f;  // beside a record's scales: its values are all 0
 
 struct AppendParams {
   PagedCache c;
@@ -345,7 +347,8 @@ __global__ void __launch_bounds__(APPEND_THREADS) paged_append_kernel(AppendPara
       scale[x] = odd ? __int_as_float(0x7fc00000) : (tiny ? 1.f : __fdiv_rn(top, 448.f));
     }
     unsigned char* rec = p.c.pool + ((int64_t)phys * p.c.Hkv + h) * (2 * P * DH + 16);
-    if (tid == 0) *reinterpret_cast<float2*>(rec + 2 * P * DH) = make_float2(scale[0], scale[1]);
+    if (tid == 0)  // (codes are 0 below 2^-100 alone: the marked pages have scale 1)
+      *reinterpret_cast<float4*>(rec + 2 * P * DH) = make_float4(scale[0], scale[1], mul[1] == 0.f && scale[1] == 1.f ? ZERO_MARK : 0.f, 0.f);
     // a page with a non-finite element has codes 0 (0 * NaN would not be)
     const bool zk = mul[0] == 0.f, zv = mul[1] == 0.f;
     for (int id = tid; id < P * DH / S::E; id += APPEND_THREADS) {
@@ -477,21 +480,11 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
 // lift the reference 2^20 and more above pages of small values, whose weights then fall among f16's subnormals (values of
 // 1e-6 behind such a page: 7 % off). Its codes are 0, so any scale will do: 2^-64 lets its tokens weigh what their scores say
 // while those of values between 2^-75 and 2^49 keep their bits. (The open page needs none: it is the last that a running
-// softmax takes, and what came before it is in fp32 by then.)
-constexpr float ZERO_LOG2 = -64.f;
-template <int DH>
-__device__ __forceinline__ void value_factors(float vs, const unsigned char* vp, float& lv, float& iv) {
+// softmax takes, and what came before it is in fp32 by then.) sc: the record's two scales and its mark.
+__device__ __forceinline__ void value_factors(const float4& sc, float& lv, float& iv) {
+  const float vs = sc.z == ZERO_MARK ? 5.421010862427522e-20f : sc.y;
   lv = log2_fast(vs);
   iv = rcp_fast(vs);
-  if (vs == 1.f) {  // one page of a warp at a time: no lane stays behind
-    uint32_t any = 0;
-#pragma unroll 1
-    for (int i = threadIdx.x & 31; i < DH * 4; i += 32) any |= reinterpret_cast<const uint32_t*>(vp)[i];
-    if (!__any_sync(0xffffffffu, any & 0x7f7f7f7fu)) {
-      lv = ZERO_LOG2;
-      iv = 18446744073709551616.f;  // 2^64
-    }
-  }
 }
 // The rows of one tile: query fragments and what the masks and scores need, per lane for its two columns of each n-tile.
 template <typename T, int DH, int NT>
@@ -836,9 +829,9 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32) paged_attn_kernel(AttnParams 
       const unsigned char* rec = p.c.pool + ((int64_t)phys * p.c.Hkv + h) * rec_bytes;
       kp[x] = rec + (x * 16 % P) * DH;
       vp[x] = kp[x] + P * DH;
-      const float2 sc = *reinterpret_cast<const float2*>(rec + 2 * P * DH);
+      const float4 sc = *reinterpret_cast<const float4*>(rec + 2 * P * DH);
       ks[x] = sc.x;
-      value_factors<DH>(sc.y, vp[x], lv[x], iv[x]);
+      value_factors(sc, lv[x], iv[x]);
     }
     const int tok0 = u * P;
     const bool mask = tok0 + 63 > min(qlo, limit - 1) || (p.window > 0 && tok0 <= qhi - p.window);
@@ -1336,9 +1329,9 @@ __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
             const unsigned char* rp = src + (((y + x) * 16) >> lpe) * rec_e;
             kp[x] = rp + (((y + x) * 16) & (Pe - 1)) * DH;
             vp[x] = kp[x] + Pe * DH;
-            const float2 sc = *reinterpret_cast<const float2*>(rp + 2 * Pe * DH);
+            const float4 sc = *reinterpret_cast<const float4*>(rp + 2 * Pe * DH);
             ks[x] = sc.x;
-            value_factors<DH>(sc.y, vp[x], lv[x], iv[x]);
+            value_factors(sc, lv[x], iv[x]);
           }
           attend_codes<T, DH, NT, TG>(rt, st, kp, vp, ks, lv, iv, tok0 + y * 16, limit, p.window, mask);
         }

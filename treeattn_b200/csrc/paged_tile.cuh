@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(TILE_THREADS, TileShape<T, DH>::CTAS) paged_ti
       const int page = min(p0 + ((j * TILE_KT + cw * 16) >> lp), p1 - 1);  // beyond the last page: the last again (masked)
       return table[page];
     };
-    auto fetch = [&](int j, int phys, uint32_t (&kw)[KW], uint32_t (&vw)[VW], float2& sc) {
+    auto fetch = [&](int j, int phys, uint32_t (&kw)[KW], uint32_t (&vw)[VW], float4& sc) {
       if (phys < 0 || phys >= p.c.n_pages) {
         record_error(DEV_INDEX_RANGE, K_PAGED_ATTN, b, phys);
         phys = 0;
@@ -250,12 +250,12 @@ __global__ void __launch_bounds__(TILE_THREADS, TileShape<T, DH>::CTAS) paged_ti
         const uint4 w = __ldg(reinterpret_cast<const uint4*>(v) + x * 32 + lane);
         vw[4 * x] = w.x; vw[4 * x + 1] = w.y; vw[4 * x + 2] = w.z; vw[4 * x + 3] = w.w;
       }
-      sc = __ldg(reinterpret_cast<const float2*>(r + 2 * P * DH));
+      sc = __ldg(reinterpret_cast<const float4*>(r + 2 * P * DH));
     };
     // block n: its codes are in the registers given, which then take those of block n + 2 (two sets in turn: moving one to
     // the other would wait for the loads); ent: the table entry of that block
     bool ok = true;
-    auto block = [&](int n, uint32_t (&kw)[KW], uint32_t (&vw)[VW], float2& sc, int& ent) -> bool {
+    auto block = [&](int n, uint32_t (&kw)[KW], uint32_t (&vw)[VW], float4& sc, int& ent) -> bool {
       const int st = n % NS;
       unsigned char* sK = sKV + st * 2 * C::K_BYTES;
       unsigned char* sV = sK + C::K_BYTES;
@@ -289,16 +289,8 @@ __global__ void __launch_bounds__(TILE_THREADS, TileShape<T, DH>::CTAS) paged_ti
             *reinterpret_cast<uint4*>(tile_piece(tileK, row + 8 * r, 2 * t)) = make_uint4(f[0], f[1], f[2], f[3]);
             *reinterpret_cast<uint4*>(tile_piece(tileK, row + 8 * r, 2 * t + 1)) = make_uint4(f[4], f[5], f[6], f[7]);
           }
-        float lv = log2_fast(sc.y), iv = rcp_fast(sc.y);
-        if (sc.y == 1.f) {  // (one page: the warp's lanes agree) values of 0 do not set the reference, see value_factors
-          uint32_t any = 0;
-#pragma unroll
-          for (int x = 0; x < VW; ++x) any |= vw[x];
-          if (!__any_sync(0xffffffffu, any & 0x7f7f7f7fu)) {
-            lv = ZERO_LOG2;
-            iv = 18446744073709551616.f;
-          }
-        }
+        float lv, iv;
+        value_factors(sc, lv, iv);
         if (lane == 0) *reinterpret_cast<float4*>(bar.scale[n & 3][cw]) = make_float4(sc.x, lv, iv, 0.f);
         filled(bar.k_full);
         if (!free_of(bar.o_full, 11)) return false;
@@ -350,7 +342,7 @@ __global__ void __launch_bounds__(TILE_THREADS, TileShape<T, DH>::CTAS) paged_ti
       return true;
     };
     uint32_t ka[KW], va[VW], kb[KW], vb[VW];
-    float2 sa, sb;
+    float4 sa, sb;
     int ea = 0, eb = 0;
     if (n_mine > 0) ea = entry(j0);
     if (n_mine > 1) eb = entry(j0 + 1);
