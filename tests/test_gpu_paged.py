@@ -814,3 +814,71 @@ def test_pages_of_zero_values_are_marked(page, dh, dt):
     r.append([1] * 5, r.randn(5, 1, dh), r.randn(5, 1, dh), pos=[page - 1] * 5)  # the last token of each page replaced
     assert marks() == [0, 0, 0, 0, 0]
     _no_device_error()
+
+
+@pytest.mark.parametrize('dh,page,dt,grp,n', [(64, 64, BF, 1, 30), (64, 64, HF, 1, 30), (64, 64, BF, 2, 30), (128, 64, HF, 2, 30),
+                                               (32, 32, BF, 1, 20), (32, 64, HF, 2, 30), (16, 16, BF, 4, 8), (128, 64, BF, 1, 9)])
+@pytest.mark.parametrize('window', [0, 4])
+def test_odd_values_in_the_open_page_stay_with_their_rows(dh, page, dt, grp, n, window):
+    """An infinity or NaN in a value of the open page reaches the rows that see its token, in its dim, and nothing else: neither
+    earlier queries of the call (some of them of the page before), nor those whose window has passed it."""
+    P = _mod()
+    r = Rig(2, 1, dh, page, dt, 4 * page, seed=dh + n)
+    before = [2 * page - 5, 7]                        # the first call's queries begin in the page before the open one
+    r.append(before)
+    k, v = r.randn(2 * n, 1, dh), r.randn(2 * n, 1, dh)
+    odd = v.clone()
+    at = [5 + (n - 5) // 3, 5 + (n - 5) // 2]         # rows of sequence 0 that stand in its open page
+    odd[at[0], 0, 3], odd[at[1], 0, 5], odd[at[1], 0, dh - 1] = math.nan, math.inf, -math.inf
+    odd[n, 0, 0] = -math.inf                          # sequence 1: its first new token
+    v = torch.where(torch.isfinite(odd), odd, 0)
+    q = r.randn(2 * n, grp, dh)
+    pos = list(r.len)
+    assert (pos[0] + n) // page == 2 and (pos[1] + n) < page or page < 64
+    r.append([n, n], k, v)
+    want, tol, wl, ltol = _attend_ref(r, q, [n, n], pos, 1 / math.sqrt(dh), window)
+    r.append([n, n], k, odd, pos=pos)
+    for b in range(2):  # only tokens that are still in 16 bits are asked about
+        assert torch.isfinite(r.cache.read(b, r.len[b] // page * page)[1]).all()
+    for i in range(2 * n):
+        b, j = divmod(i, n)
+        for row, dim in ((at[0], 3), (at[1], 5), (at[1], dh - 1), (n, 0)):
+            if row // n == b and row % n <= j and (not window or row % n > j - window):
+                want[i, :, dim] += float(odd[row, 0, dim])
+    lse = torch.empty(2 * n, grp, device=DEV)
+    got = P.paged_attn(r.cache, q, _starts([n, n]), _i32(pos), n, window=window, lse=lse).double()
+    fin = torch.isfinite(want)
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(got[torch.isinf(want)], want[torch.isinf(want)])
+    assert ((got - want).abs() <= tol)[fin].all()
+    assert ((lse.double() - wl).abs() <= ltol).all()
+    _no_device_error()
+
+
+@pytest.mark.parametrize('dh,Hq,Hkv,n,room', [(64, 2, 2, 2, 0), (64, 8, 1, 1, 30000), (128, 4, 1, 4, 20000), (128, 2, 2, 2, 0),
+                                               (64, 4, 1, 40, 0), (128, 4, 1, 50, 0), (32, 4, 2, 2, 40000)])
+def test_odd_values_of_items_in_parts(dh, Hq, Hkv, n, room):
+    """The same where an item's pages are shared by many warps or CTAs, joined on the spot or late: the open page's part tells the one
+    that writes the output."""
+    P = _mod()
+    r = Rig(2, Hkv, dh, 64, BF, max(6000 + n, room), seed=dh + n)
+    r.append([5000, 5504])                            # open pages of 8 and 0 tokens before the call
+    k, v = r.randn(2 * n, Hkv, dh), r.randn(2 * n, Hkv, dh)
+    q = r.randn(2 * n, Hq, dh)
+    pos = list(r.len)
+    odd = v.clone()
+    odd[n - 1, 0, 7], odd[n, Hkv - 1, dh - 2] = math.inf, math.nan  # sequence 0's last token, sequence 1's first
+    v = torch.where(torch.isfinite(odd), odd, 0)
+    r.append([n, n], k, v)
+    want, tol, wl, ltol = _attend_ref(r, q, [n, n], pos, 1 / math.sqrt(dh), 0)
+    r.append([n, n], k, odd, pos=pos)
+    want[n - 1, :Hq // Hkv, 7] += math.inf
+    want[n:, Hq - Hq // Hkv:, dh - 2] += math.nan
+    lse = torch.empty(2 * n, Hq, device=DEV)
+    ws = P.paged_attn_workspace(2, Hq, Hkv, dh, n)
+    for _ in range(2):
+        got = P.paged_attn(r.cache, q, _starts([n, n]), _i32(pos), n, lse=lse, ws=ws).double()
+        fin = torch.isfinite(want)
+        assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(got[torch.isinf(want)], want[torch.isinf(want)])
+        assert ((got - want).abs() <= tol)[fin].all()
+        assert ((lse.double() - wl).abs() <= ltol).all()
+    _no_device_error()

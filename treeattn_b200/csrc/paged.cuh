@@ -16,6 +16,7 @@
 #include <type_traits>
 #include <cuda_fp8.h>
 #include "common.cuh"
+#include "tc.cuh"
 
 namespace ta {
 
@@ -712,11 +713,63 @@ __device__ __forceinline__ uint32_t as_type(uint32_t f16x2) {
   return pack2<T>(f.x, f.y);
 }
 
+// Infinities and NaN among the open page's values. In the product a masked token's weight of 0 would make them NaN for every row
+// of the tile, so they stay out of it, and the rows that see their tokens get them at the end, when the output is written.
+// odd2: bit 15 (31) of two elements that are one: above the largest finite magnitude, one step of the exponent's last place
+// carries into it. finite2: the elements with those taken out (0).
+template <typename T>
+__device__ __forceinline__ uint32_t odd2(uint32_t w) {
+  return ((w & 0x7fff7fffu) + (std::is_same<T, __half>::value ? 0x04000400u : 0x00800080u)) & 0x80008000u;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t finite2(uint32_t w) {
+  return w & ~((odd2<T>(w) >> 15) * 0xffffu);
+}
+// Takes them out of n 16-byte pieces in shared memory (the warp's own); whether there were any.
+template <typename T>
+__device__ __forceinline__ bool clean_values(unsigned char* v, int n) {
+  const int lane = threadIdx.x & 31;
+  uint32_t odd = 0u;
+#pragma unroll 4
+  for (int i = lane; i < n; i += 32) {
+    const uint4 w = reinterpret_cast<const uint4*>(v)[i];
+    odd |= odd2<T>(w.x) | odd2<T>(w.y) | odd2<T>(w.z) | odd2<T>(w.w);
+  }
+  if (__builtin_expect(!__any_sync(0xffffffffu, odd != 0u), 1)) return false;
+#pragma unroll 1
+  for (int i = lane; i < n; i += 32) {
+    uint4 w = reinterpret_cast<uint4*>(v)[i];
+    w.x = finite2<T>(w.x); w.y = finite2<T>(w.y); w.z = finite2<T>(w.z); w.w = finite2<T>(w.w);
+    reinterpret_cast<uint4*>(v)[i] = w;
+  }
+  fence_proxy_async_smem();  // the place is filled by a bulk copy next
+  __syncwarp();
+  return true;
+}
+// Adds those of the open page (values tv; positions from `first` on) to a row that sees the positions [from, to), dims d0,
+// d0 + step, ... below d1.
+template <typename T, int DH>
+__device__ __noinline__ void add_odd(const T* tv, int first, int from, int to, int d0, int d1, int step, T* out) {
+  for (int at = max(from, first); at < to; ++at) {
+    const int i = at - first;
+    for (int d = d0; d < d1; d += step) {
+      const float v = to_f32(tv[(i >> 4) * 16 * DH + value_offset<DH>(i & 15, d)]);
+      if (!(fabsf(v) <= 3.402823466e38f)) out[d] = from_f32<T>(to_f32(out[d]) + v);
+    }
+  }
+}
+// The values of the open page of sequence b and kv head h: page n_full.
+template <typename T, int DH>
+__device__ __forceinline__ const T* open_values(const PagedCache& c, int b, int h, int n_full) {
+  return reinterpret_cast<const T*>(c.tail) + ((((int64_t)b * c.Hkv + h) * 2 + (n_full & 1)) * 2 + 1) * ((int64_t)c.P * DH);
+}
+
 // TG 16-token groups of the open page, 16-bit elements in the same order. len: tokens the sequence holds; later slots of
-// the page hold anything and are masked in the scores and zeroed in the values.
-template <typename T, int DH, int NT, int TG>
+// the page hold anything and are masked in the scores and zeroed in the values. CLEAN: the values hold no infinity or NaN;
+// otherwise those are left out here, and odd is set.
+template <typename T, int DH, int NT, int TG, bool CLEAN>
 __device__ __forceinline__ void attend_tail(const RowTile<T, DH, NT>& rt, SoftState<DH, NT>& st, const T* kp, const T* vp,
-                                            int tok0, int len, int window) {
+                                            int tok0, int len, int window, uint32_t& odd) {
   using S = PageShape<DH>;
   const int lane = threadIdx.x & 31, t = lane & 3;
   float s[TG][NT][4];
@@ -768,6 +821,13 @@ __device__ __forceinline__ void attend_tail(const RowTile<T, DH, NT>& rt, SoftSt
     for (int c = 0; c < S::C; ++c) {
       uint32_t w[4 * S::M];
       load_words<16 * S::M>(vp + x * 16 * DH + (c * 32 + lane) * 8 * S::M, w);
+      if constexpr (!CLEAN) {
+#pragma unroll
+        for (int i = 0; i < 4 * S::M; ++i) {
+          odd |= odd2<T>(w[i]);
+          w[i] = finite2<T>(w[i]);
+        }
+      }
 #pragma unroll
       for (int m = 0; m < S::M; ++m) {
         const uint32_t a[4] = {w[4 * m] & keep0, w[4 * m + 2] & keep0, w[4 * m + 1] & keep1, w[4 * m + 3] & keep1};
@@ -815,6 +875,7 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32) paged_attn_kernel(AttnParams 
   st.clear();
   const int32_t* tab = p.c.table + b * p.c.table_sb;
   const int64_t rec_bytes = 2 * P * DH + 16;
+  uint32_t odd = 0u;
   for (int u = p0 + warp * per; u < p1; u += ATTN_WARPS * per) {
     const unsigned char *kp[4], *vp[4];
     float ks[4], lv[4], iv[4];
@@ -841,8 +902,8 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32) paged_attn_kernel(AttnParams 
     const T* tk = reinterpret_cast<const T*>(p.c.tail) +
                   ((((int64_t)b * p.c.Hkv + h) * 2 + (n_full & 1)) * 2) * ((int64_t)P * DH);
     for (int x = warp; n_full * P + x * 16 <= qhi; x += ATTN_WARPS)
-      attend_tail<T, DH, NT, 1>(rt, st, tk + x * 16 * DH, tk + (int64_t)P * DH + x * 16 * DH, n_full * P + x * 16, len,
-                                p.window);
+      attend_tail<T, DH, NT, 1, false>(rt, st, tk + x * 16 * DH, tk + (int64_t)P * DH + x * 16 * DH, n_full * P + x * 16, len,
+                                       p.window, odd);
   }
   // join the warps
 #pragma unroll
@@ -864,7 +925,7 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32) paged_attn_kernel(AttnParams 
         so[(warp * ROWS + col) * PITCH + x * 16 + 8 + g] = st.o[x][nt][i + 2];
       }
     }
-  __syncthreads();
+  odd = __syncthreads_or(odd != 0u);
   for (int id = tid; id < ROWS * DH; id += ATTN_WARPS * 32) {
     const int col = id / DH, d = id % DH, rr = row0 + col;
     if (rr >= R) break;
@@ -881,7 +942,13 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32) paged_attn_kernel(AttnParams 
     }
     const int64_t row = nr.row0 + rr / group;
     const int hq = h * group + rr % group;
-    reinterpret_cast<T*>(p.out)[row * p.o_sr + hq * p.o_sh + d] = from_f32<T>(L == 0.f ? 0.f : o / L);
+    T* out = reinterpret_cast<T*>(p.out) + row * p.o_sr + hq * p.o_sh;
+    out[d] = from_f32<T>(L == 0.f ? 0.f : o / L);
+    if (odd) {
+      const int qp = nr.pos + rr / group;
+      add_odd<T, DH>(open_values<T, DH>(p.c, b, h, n_full), n_full * P, p.window > 0 ? qp - p.window + 1 : 0, min(len, qp + 1), d,
+                     d + 1, 1, out);
+    }
     if (p.lse && d == 0)
       p.lse[row * p.Hq + hq] = L == 0.f ? -INFINITY : (m - ATTN_SHIFT + log2f(L)) * 0.69314718055994531f;
   }
@@ -1035,6 +1102,7 @@ __device__ __forceinline__ void join_states(SoftState<DH, NT>& st, const float* 
 // holds its last unit. `first` and `last` are the warps that share the item, `wpc` warps to a CTA.
 struct Join {
   int row0, n, h, first, last, wpc;
+  int b, pos, odd;  // odd: the open page holds an infinity or NaN
   __device__ __forceinline__ int parts() const { return (last - 1) / wpc - first / wpc + 2; }
 };
 
@@ -1095,7 +1163,8 @@ __device__ __noinline__ void gather_tile(const unsigned char* from, int pitch, i
 // to the kernel's parameters put them into local memory, a miss away: a join took 6 us against 4.)
 template <typename T, int DH, int NT>
 __device__ __noinline__ void join_tile(const Join* join, const float* states, const float* groups, int x, int nt, int group,
-                                       T* out, int64_t o_sr, int64_t o_sh, float* lse, int Hq) {
+                                       T* out, int64_t o_sr, int64_t o_sh, float* lse, int Hq, void* tail, int Hkv, int P,
+                                       int window) {
   using SH = SplitShape<DH, NT>;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const Join j = *join;
@@ -1119,6 +1188,16 @@ __device__ __noinline__ void join_tile(const Join* join, const float* states, co
     o[8] = from_f32<T>(acc[i + 2] * inv);
     if (lse && g == 0 && x == 0)
       lse[(int64_t)q * Hq + gq] = l[i] == 0.f ? -INFINITY : (m[i] - ATTN_SHIFT + log2f(l[i])) * 0.69314718055994531f;
+  }
+  if (__builtin_expect(j.odd != 0, 0)) {
+    __syncwarp();
+    const int n_full = (j.pos + j.n) / P;
+    const PagedCache c{nullptr, tail, nullptr, 0, 0, 0, Hkv, P};
+    for (int rr = nt * 8; rr < min(R, nt * 8 + 8); ++rr) {
+      const int q = rr / group, qp = j.pos + q;
+      add_odd<T, DH>(open_values<T, DH>(c, j.b, j.h, n_full), n_full * P, window > 0 ? qp - window + 1 : 0, qp + 1, x * 16 + lane,
+                     x * 16 + 16, 32, out + q * o_sr + (rr - q * group) * o_sh);
+    }
   }
 }
 
@@ -1310,6 +1389,7 @@ __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
     const int R = it.n * group;
     st.clear();
     const int qhi = it.pos + it.n - 1;
+    uint32_t odd = 0u;  // the open page holds an infinity or NaN
     for (int k = run.k; k < run.end; ++k, ++step) {
       const int slot = step % NS;
       const unsigned char* src = ring + (warp * NS + slot) * SH::STAGE;
@@ -1337,8 +1417,10 @@ __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
         }
       } else {
         const int tok0 = (it.p1 << lp) + (k - it.nu8) * TT;
-        attend_tail<T, DH, NT, TT / 16>(rt, st, reinterpret_cast<const T*>(src), reinterpret_cast<const T*>(src + UT * DH),
-                                        tok0, it.len, p.window);
+        unsigned char* v = ring + (warp * NS + slot) * SH::STAGE + UT * DH;
+        if (clean_values<T>(v, (min(it.len - tok0, TT) + 15) / 16 * 2 * DH)) odd = 1u;
+        attend_tail<T, DH, NT, TT / 16, true>(rt, st, reinterpret_cast<const T*>(src), reinterpret_cast<const T*>(v), tok0,
+                                              it.len, p.window, odd);
       }
       __syncwarp();  // every lane has read the unit
       if (more) {
@@ -1360,7 +1442,7 @@ __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
     bool write = run.k == 0 && run.end == it.units;
     if (!write) {
       const int wa = owner_of(run.at), wb = owner_of(run.at + it.units - 1), item = run.b * Hkv + run.h;
-      const Join join{it.row0, it.n, run.h, wa, wb, wpc};
+      Join join{it.row0, it.n, run.h, wa, wb, wpc, run.b, it.pos, (int)odd};
       if (LATE && run.end < it.units) {
         // (the warp's last run) stays in the registers until the CTA's warps are done
         if (lane == 0) {
@@ -1386,11 +1468,13 @@ __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
       __syncwarp();
       int32_t* cnt = counters + item;
       int before = 0;
-      if (lane == 0) before = atomicAdd(cnt, 1);
+      if (lane == 0) before = atomicAdd(cnt, 1 + ((int)odd << 16));  // arrivals, and above them those of odd parts
       before = __shfl_sync(0xffffffffu, before, 0);
-      if (before == (LATE ? join.parts() - 1 : wb - wa)) {
+      if ((before & 0xffff) == (LATE ? join.parts() - 1 : wb - wa)) {
         __threadfence();
         if (lane == 0) *cnt = 0;
+        odd |= before >> 16;
+        join.odd = odd;
         if constexpr (LATE) {
           if (lane == 0) joins[atomicAdd(&n_joins, 1)] = join;
         } else {
@@ -1419,6 +1503,16 @@ __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
           if (p.lse && g == 0)
             p.lse[row * p.Hq + hq] = l == 0.f ? -INFINITY : (st.m[nt][i] - ATTN_SHIFT + log2f(l)) * 0.69314718055994531f;
         }
+      if (__builtin_expect(odd != 0u, 0)) {
+        __syncwarp();
+        const T* tv = open_values<T, DH>(p.c, run.b, run.h, it.p1);
+#pragma unroll 1
+        for (int rr = 0; rr < R; ++rr) {
+          const int q = rr / group, qp = it.pos + q;
+          add_odd<T, DH>(tv, it.p1 << lp, p.window > 0 ? qp - p.window + 1 : 0, qp + 1, lane, DH, 32,
+                         reinterpret_cast<T*>(p.out) + (it.row0 + q) * p.o_sr + (int64_t)(run.h * group + rr % group) * p.o_sh);
+        }
+      }
     }
   }
   if (!ok)  // no copy of this warp may still be in flight when its CTA ends
@@ -1456,9 +1550,13 @@ __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
     __syncthreads();
     if (lane == 0 && leads(warp)) {
       int32_t* cnt = counters + held[warp];
-      if (atomicAdd(cnt, 1) == held_join[warp].parts() - 1) {
+      Join join = held_join[warp];
+      for (int w = warp + 1; w < WARPS && held[w] == held[warp]; ++w) join.odd |= held_join[w].odd;
+      const int before = atomicAdd(cnt, 1 + (join.odd << 16));
+      if ((before & 0xffff) == join.parts() - 1) {
         *cnt = 0;
-        joins[atomicAdd(&n_joins, 1)] = held_join[warp];
+        join.odd |= before >> 16;
+        joins[atomicAdd(&n_joins, 1)] = join;
       }
       __threadfence();
     }
@@ -1470,7 +1568,7 @@ __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
       const int hq = j->h * group;
       join_tile<T, DH, NT>(j, states, groups, i % TILES / NT, i % NT, group,
                            reinterpret_cast<T*>(p.out) + row * p.o_sr + (int64_t)hq * p.o_sh, p.o_sr, p.o_sh,
-                           p.lse ? p.lse + row * p.Hq + hq : nullptr, p.Hq);
+                           p.lse ? p.lse + row * p.Hq + hq : nullptr, p.Hq, p.c.tail, Hkv, P, p.window);
     }
   }
 }

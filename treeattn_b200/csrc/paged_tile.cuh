@@ -10,7 +10,8 @@
 //              memory), so that the softmax of one block runs beside the products of its neighbours.
 //   warps 0-3  softmax, one thread per row: maximum, weights (f16, into shared memory), denominator; O is rescaled in tensor
 //              memory only when a row's reference has to rise by more than 2^8.
-// The open page is the last block: 16-bit elements as they are, with a copy of the queries in that type.
+// The open page is the last block: 16-bit elements as they are, with a copy of the queries in that type (its infinities and NaN
+// join at the end, row by row).
 // What bounds it is the chain of latencies of a block's softmax step (scores out of tensor memory, maximum, weights, their way
 // through shared memory to the next product): without the exponentials, the stores or the conversions it is 1 to 4 % faster.
 // Two sequences of up to 4000 tokens, chunks of 512, 12 heads of 64: 41 us; 16 sequences of 8000, 40 rows for each of 4 heads:
@@ -49,6 +50,7 @@ struct TileBars {
   alignas(16) float scale[4][4][4];
   uint32_t tmem_base;
   int abort_flag, last;
+  int odd;  // the open page holds an infinity or NaN among its values
 };
 
 static_assert(offsetof(TileBars, scale) % 16 == 0, "the scales are read as float4");
@@ -172,7 +174,7 @@ __global__ void __launch_bounds__(TILE_THREADS, TileShape<T, DH>::CTAS) paged_ti
       mbar_init(&bar.o_full[s], 1);
     }
     mbar_init(&bar.mma_done, 1);
-    bar.abort_flag = 0;
+    bar.abort_flag = bar.odd = 0;
     fence_mbar_init();
   }
   if (warp == 8) {
@@ -325,14 +327,19 @@ __global__ void __launch_bounds__(TILE_THREADS, TileShape<T, DH>::CTAS) paged_ti
         if (!free_of(bar.o_full, 11)) return false;
         const uint32_t keep0 = (2 * t < held ? 0xffffu : 0u) | (2 * t + 1 < held ? 0xffff0000u : 0u);
         const uint32_t keep1 = (2 * t + 8 < held ? 0xffffu : 0u) | (2 * t + 9 < held ? 0xffff0000u : 0u);
+        uint32_t odd = 0u;
 #pragma unroll
         for (int x = 0; x < VW; ++x) {
           const int d = (x / 2) * 16 + (x & 1) * 8 + g;
           uint32_t w[2] = {0u, 0u};
           if (held > 0) load_words<8>(tv + ((x / (2 * S::M)) * 32 + lane) * 8 * S::M + (x % (2 * S::M)) * 4, w);
-          *reinterpret_cast<uint32_t*>(tile_piece(sV, d, 2 * cw) + 4 * t) = w[0] & keep0;
-          *reinterpret_cast<uint32_t*>(tile_piece(sV, d, 2 * cw + 1) + 4 * t) = w[1] & keep1;
+          w[0] &= keep0;
+          w[1] &= keep1;
+          odd |= odd2<T>(w[0]) | odd2<T>(w[1]);
+          *reinterpret_cast<uint32_t*>(tile_piece(sV, d, 2 * cw) + 4 * t) = finite2<T>(w[0]);
+          *reinterpret_cast<uint32_t*>(tile_piece(sV, d, 2 * cw + 1) + 4 * t) = finite2<T>(w[1]);
         }
+        if (odd) bar.odd = 1;
       }
       if (n + 2 < n_mine) {
         fetch(j0 + n + 2, ent, kw, vw, sc);
@@ -537,7 +544,10 @@ __global__ void __launch_bounds__(TILE_THREADS, TileShape<T, DH>::CTAS) paged_ti
       hq = h * group + rr % group;
       out = reinterpret_cast<T*>(p.out) + out_row * p.o_sr + (int64_t)hq * p.o_sh;
     }
-    auto finish = [&]() {
+    auto finish = [&](int odd) {
+      if (__builtin_expect(odd != 0, 0) && live)
+        add_odd<T, DH>(open_values<T, DH>(p.c, b, h, n_full), n_full << lp, p.window > 0 ? qpos - p.window + 1 : 0, qpos + 1, 0, DH,
+                       1, out);
       if (p.lse && live) p.lse[out_row * p.Hq + hq] = l == 0.f ? -INFINITY : (ref - SHIFT + log2f(l)) * 0.69314718055994531f;
     };
     if (good && tp.splits == 1) {
@@ -553,7 +563,7 @@ __global__ void __launch_bounds__(TILE_THREADS, TileShape<T, DH>::CTAS) paged_ti
           for (int i = 0; i < 32; i += 8) store_vec_from_f32<T>(out + c + i, o + i);
         }
       }
-      finish();
+      finish(*reinterpret_cast<volatile int*>(&bar.odd));
     } else if (good) {
       // this CTA's share of the blocks; the last of the tile's CTAs joins them in order
       const int64_t item = ((int64_t)b * p.c.Hkv + h) * tp.tiles + tile;
@@ -572,7 +582,11 @@ __global__ void __launch_bounds__(TILE_THREADS, TileShape<T, DH>::CTAS) paged_ti
       __stcg(mine + TILE_ROWS * (DH + 1) + tid, l);
       __threadfence();
       named_bar_sync(1, 128);
-      if (tid == 0) bar.last = atomicAdd(tp.counters + item, 1) == tp.splits - 1;
+      if (tid == 0) {  // arrivals, and above them those of odd shares
+        const int before = atomicAdd(tp.counters + item, 1 + (bar.odd << 16));
+        bar.last = (before & 0xffff) == tp.splits - 1;
+        bar.odd |= before >> 16;
+      }
       named_bar_sync(1, 128);
       if (bar.last) {
         __threadfence();
@@ -608,7 +622,7 @@ __global__ void __launch_bounds__(TILE_THREADS, TileShape<T, DH>::CTAS) paged_ti
           for (int i = 0; i < 8; ++i) o[i] *= inv;
           if (live) store_vec_from_f32<T>(out + c, o);
         }
-        finish();
+        finish(*reinterpret_cast<volatile int*>(&bar.odd));
       }
     }
     tc_fence_before();
