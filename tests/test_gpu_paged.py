@@ -882,3 +882,20 @@ def test_odd_values_of_items_in_parts(dh, Hq, Hkv, n, room):
         assert ((got - want).abs() <= tol)[fin].all()
         assert ((lse.double() - wl).abs() <= ltol).all()
     _no_device_error()
+
+
+@pytest.mark.parametrize('dh,n', [(64, 1), (64, 40), (128, 3), (32, 40), (128, 50)])
+def test_large_keys_and_small_queries(dh, n):
+    """bf16 keys of 2^112 against queries of 2^-106: scores far below the type's end, from codes and from the open page alike."""
+    P = _mod()
+    r = Rig(2, 1, dh, 64, BF, 256, seed=dh + n)
+    before = [3, 150]
+    N = sum(before) + 2 * n
+    k = (r.randn(N, 1, dh).float() * 2.0 ** 112).to(BF)
+    r.append(before, k[2 * n:], r.randn(sum(before), 1, dh))
+    r.append([n, n], k[:2 * n], r.randn(2 * n, 1, dh))
+    q = (r.randn(2 * n, 2, dh).float() * 2.0 ** -106).to(BF)
+    got = P.paged_attn(r.cache, q, _starts([n, n]), _i32(before), n)
+    want, tol, _, _ = _attend_ref(r, q, [n, n], before, 1 / math.sqrt(dh), 0)
+    assert ((got.double() - want).abs() <= tol).all()
+    _no_device_error()

@@ -705,12 +705,17 @@ __device__ __forceinline__ void attend_codes(const RowTile<T, DH, NT>& rt, SoftS
     }
 }
 
-// A query fragment in the tail's type: the power of two keeps bf16 rows exact as well.
+// A query fragment in the tail's type: the power of two keeps bf16 rows exact as well. Those go back to magnitudes below 1: the
+// open page's keys are as they came, and 2^15 times one of 2^110 and its like would leave fp32 in the sum (tail_key_scale undoes it).
+template <typename T>
+__host__ __device__ constexpr float tail_key_scale() {
+  return std::is_same<T, __half>::value ? 1.f : 32768.f;
+}
 template <typename T>
 __device__ __forceinline__ uint32_t as_type(uint32_t f16x2) {
   if constexpr (std::is_same<T, __half>::value) return f16x2;
   const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&f16x2));
-  return pack2<T>(f.x, f.y);
+  return pack2<T>(f.x * (1.f / tail_key_scale<T>()), f.y * (1.f / tail_key_scale<T>()));
 }
 
 // Infinities and NaN among the open page's values. In the product a masked token's weight of 0 would make them NaN for every row
@@ -799,13 +804,14 @@ __device__ __forceinline__ void attend_tail(const RowTile<T, DH, NT>& rt, SoftSt
         for (int nt = 0; nt < NT; ++nt) mma_16<T>(s[x][nt], a, b0[nt], b1[nt]);
       }
     }
-  float one[TG], zero[TG];
+  float ks[TG], one[TG], zero[TG];
 #pragma unroll
   for (int x = 0; x < TG; ++x) {
+    ks[x] = tail_key_scale<T>();
     one[x] = 1.f;
     zero[x] = 0.f;
   }
-  soft_step<T, DH, NT, TG>(rt, st, s, one, zero, one, tok0, len, window, true);
+  soft_step<T, DH, NT, TG>(rt, st, s, ks, zero, one, tok0, len, window, true);
 #pragma unroll
   for (int x = 0; x < TG; ++x) {
     uint32_t pf[NT][2];
