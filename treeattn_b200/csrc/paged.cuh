@@ -531,8 +531,9 @@ struct RowTile {
         top = fmaxf(top, fmaxf(fabsf(bits_value<T>(raw.w[nt][i] & 0xffffu)), fabsf(bits_value<T>(raw.w[nt][i] >> 16))));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // 2^ex * top in [2^14, 2^15): exact, and what falls below f16's range is below 2^-39 of the row's largest element
-      const int ex = min(14 + 127 - (int)(__float_as_uint(top) >> 23), 120);
+      // 2^ex * top in [2^7, 2^8): exact down to 2^-21 of the row's largest element, and within 2^-32 of it below (fp32 sums lose
+      // 2^-24). Not higher: bf16 keys of the open page come as they are, and 2^15 times those of 2^110 left fp32's range.
+      const int ex = min(7 + 127 - (int)(__float_as_uint(top) >> 23), 120);
       // the sign of the scale joins the row; at scale 0 the row is 0
       const float up = p.scale == 0.f ? 0.f : copysignf(__int_as_float((ex + 127) << 23), p.scale);
 #pragma unroll
@@ -705,17 +706,12 @@ __device__ __forceinline__ void attend_codes(const RowTile<T, DH, NT>& rt, SoftS
     }
 }
 
-// A query fragment in the tail's type: the power of two keeps bf16 rows exact as well. Those go back to magnitudes below 1: the
-// open page's keys are as they came, and 2^15 times one of 2^110 and its like would leave fp32 in the sum (tail_key_scale undoes it).
-template <typename T>
-__host__ __device__ constexpr float tail_key_scale() {
-  return std::is_same<T, __half>::value ? 1.f : 32768.f;
-}
+// A query fragment in the tail's type: the power of two keeps bf16 rows exact as well.
 template <typename T>
 __device__ __forceinline__ uint32_t as_type(uint32_t f16x2) {
   if constexpr (std::is_same<T, __half>::value) return f16x2;
   const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&f16x2));
-  return pack2<T>(f.x * (1.f / tail_key_scale<T>()), f.y * (1.f / tail_key_scale<T>()));
+  return pack2<T>(f.x, f.y);
 }
 
 // Infinities and NaN among the open page's values. In the product a masked token's weight of 0 would make them NaN for every row
@@ -804,14 +800,13 @@ __device__ __forceinline__ void attend_tail(const RowTile<T, DH, NT>& rt, SoftSt
         for (int nt = 0; nt < NT; ++nt) mma_16<T>(s[x][nt], a, b0[nt], b1[nt]);
       }
     }
-  float ks[TG], one[TG], zero[TG];
+  float one[TG], zero[TG];
 #pragma unroll
   for (int x = 0; x < TG; ++x) {
-    ks[x] = tail_key_scale<T>();
     one[x] = 1.f;
     zero[x] = 0.f;
   }
-  soft_step<T, DH, NT, TG>(rt, st, s, ks, zero, one, tok0, len, window, true);
+  soft_step<T, DH, NT, TG>(rt, st, s, one, zero, one, tok0, len, window, true);
 #pragma unroll
   for (int x = 0; x < TG; ++x) {
     uint32_t pf[NT][2];

@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(TILE_THREADS, TileShape<T, DH>::CTAS) paged_ti
       for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
     }
     // as in RowTile: the row's power of two, the sign of the scale, a zero row at scale 0
-    const int ex = min(14 + 127 - (int)(__float_as_uint(top) >> 23), 120);
+    const int ex = min(7 + 127 - (int)(__float_as_uint(top) >> 23), 120);
     const float up = p.scale == 0.f ? 0.f : copysignf(__int_as_float((ex + 127) << 23), p.scale);
     cs = p.scale == 0.f ? 1.f : fabsf(p.scale) * 1.4426950408889634f * __int_as_float((127 - ex) << 23);
 #pragma unroll
@@ -215,11 +215,7 @@ __global__ void __launch_bounds__(TILE_THREADS, TileShape<T, DH>::CTAS) paged_ti
       for (int i = 0; i < 8; ++i) x[i] *= up;
       const int at = (c >> 3) * TILE_ROWS * 128;
       store_vec_from_f32<__half>(reinterpret_cast<__half*>(tile_piece(sQ + at, tid, c & 7)), x);
-      if constexpr (C::BF) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] *= 1.f / tail_key_scale<T>();
-        store_vec_from_f32<T>(reinterpret_cast<T*>(tile_piece(sQ2 + at, tid, c & 7)), x);
-      }
+      if constexpr (C::BF) store_vec_from_f32<T>(reinterpret_cast<T*>(tile_piece(sQ2 + at, tid, c & 7)), x);
     }
   }
   fence_proxy_async_smem();
@@ -326,7 +322,7 @@ __global__ void __launch_bounds__(TILE_THREADS, TileShape<T, DH>::CTAS) paged_ti
               *reinterpret_cast<uint4*>(tile_piece(tileK, row + 8 * r, 2 * t + 1)) = make_uint4(w[4], w[5], w[6], w[7]);
             }
         }
-        if (lane == 0) *reinterpret_cast<float4*>(bar.scale[n & 3][cw]) = make_float4(tail_key_scale<T>(), 0.f, 1.f, 0.f);
+        if (lane == 0) *reinterpret_cast<float4*>(bar.scale[n & 3][cw]) = make_float4(1.f, 0.f, 1.f, 0.f);
         filled(bar.k_full);
         if (!free_of(bar.o_full, 11)) return false;
         const uint32_t keep0 = (2 * t < held ? 0xffffu : 0u) | (2 * t + 1 < held ? 0xffff0000u : 0u);
