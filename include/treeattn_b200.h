@@ -360,7 +360,8 @@ int ta_block_tail(const void* att, float* x, const void* w_proj, const float* ln
  *   values [c][g][t][m][r][kh][lo]  token 8 kh + 2 t + lo, dim (c M + m) 16 + 8 r + g (M = min(2, dh / 16))
  * New rows: sequence b owns rows [start[b], start[b + 1]) (start: B + 1 int32, device) of the n_rows rows of the call, at
  * positions pos[b], pos[b] + 1, ...; max_new bounds the rows of one sequence (it sizes the grid). Rows that do not fit
- * these numbers, and pages outside the pool, are recorded in the device error record and left out.
+ * these numbers, and pages outside the pool, are recorded in the device error record and left out; rows of an attention that see
+ * such a page are NaN.
  *
  * ta_paged_append: rotates the first `rot` dims of k (and q, into q_out (n_rows, Hq, dh) contiguous; q_out NULL: none)
  *   by the position's angles, y1 = x1 cos - x2 sin, y2 = x2 cos + x1 sin on dims i and i + rot / 2 (cosv / sinv

@@ -899,3 +899,35 @@ def test_large_keys_and_small_queries(dh, n):
     want, tol, _, _ = _attend_ref(r, q, [n, n], before, 1 / math.sqrt(dh), 0)
     assert ((got.double() - want).abs() <= tol).all()
     _no_device_error()
+
+
+@pytest.mark.parametrize('dh,page,grp,n', [(64, 64, 1, 1), (64, 16, 2, 3), (128, 64, 1, 1), (128, 16, 4, 2), (64, 32, 2, 40),
+                                            (128, 64, 1, 70), (32, 16, 1, 40), (16, 32, 2, 1)])
+@pytest.mark.parametrize('entry', [-3, 10 ** 6])
+def test_pages_outside_the_pool_read_as_nan(dh, page, grp, n, entry):
+    """A table entry outside the pool is recorded, and rows that see its page are NaN, not what another page holds; rows that do
+    not see it (a window past it, another sequence) are as they would be."""
+    P = _mod()
+    r = Rig(2, 1, dh, page, BF, 4 * page + 2 * n + 16, seed=dh + n)
+    r.cache.pool[0] = 0                              # what a page outside must not be taken for
+    before = [4 * page + 5, 3 * page + 2]
+    r.append(before)
+    r.append([n, n])
+    q = r.randn(2 * n, grp, dh)
+    start, pos = _starts([n, n]), _i32(before)
+    for window in (0, 2 * page):
+        want, tol, _, _ = _attend_ref(r, q, [n, n], before, 1 / math.sqrt(dh), window)
+        r.cache.table[0, 1] = entry
+        got = P.paged_attn(r.cache, q, start, pos, n, window=window).double()
+        r.cache.table[0, 1] = r.perm[0, 1]
+        sees = torch.zeros(2 * n, dtype=torch.bool, device=DEV)
+        for i in range(n):
+            sees[i] = not window or before[0] + i - window + 1 < 2 * page
+        assert torch.isnan(got[sees]).all()
+        assert ((got - want).abs() <= tol)[~sees].all()
+        code = _device_error()
+        assert code[:3] == (3, 17, 0) if bool(sees.any()) else code[0] in (0, 3)
+    again = P.paged_attn(r.cache, q, start, pos, n)
+    want, tol, _, _ = _attend_ref(r, q, [n, n], before, 1 / math.sqrt(dh), 0)
+    assert ((again.double() - want).abs() <= tol).all()
+    _no_device_error()

@@ -74,6 +74,20 @@ __device__ __forceinline__ bool new_rows(const int32_t* start, const int32_t* po
   return true;
 }
 
+// What attention reads in place of a page outside the pool: codes 0 and a key scale of NaN, for the rows that see it. A record of
+// any page size ends where it ends.
+struct alignas(16) OutsideRecord {
+  float codes[2 * 64 * 128 / 4], scales[4];
+};
+static __device__ const OutsideRecord g_outside = {{}, {NAN, 1.f, 0.f, 0.f}};
+// The record of a page and kv head; one outside the pool is recorded.
+__device__ __forceinline__ const unsigned char* record_of(const PagedCache& c, int page, int h, int rec_bytes, int b) {
+  const bool outside = (uint32_t)page >= (uint32_t)c.n_pages;
+  if (__builtin_expect(outside, 0)) record_error(DEV_INDEX_RANGE, K_PAGED_ATTN, b, page);
+  const unsigned char* rec = c.pool + ((int64_t)page * c.Hkv + h) * rec_bytes;
+  return outside ? reinterpret_cast<const unsigned char*>(&g_outside + 1) - rec_bytes : rec;
+}
+
 template <int BYTES>
 __device__ __forceinline__ void load_words(const void* p, uint32_t (&w)[BYTES / 4]) {
   if constexpr (BYTES >= 16) {
@@ -875,7 +889,7 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32) paged_attn_kernel(AttnParams 
   SoftState<DH, NT> st;
   st.clear();
   const int32_t* tab = p.c.table + b * p.c.table_sb;
-  const int64_t rec_bytes = 2 * P * DH + 16;
+  const int rec_bytes = 2 * P * DH + 16;
   uint32_t odd = 0u;
   for (int u = p0 + warp * per; u < p1; u += ATTN_WARPS * per) {
     const unsigned char *kp[4], *vp[4];
@@ -883,12 +897,7 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32) paged_attn_kernel(AttnParams 
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
       const int pg = min(u + x * 16 / P, p1 - 1);
-      int phys = tab[pg];
-      if (phys < 0 || phys >= p.c.n_pages) {
-        if (lane == 0) record_error(DEV_INDEX_RANGE, K_PAGED_ATTN, b, phys);
-        phys = 0;
-      }
-      const unsigned char* rec = p.c.pool + ((int64_t)phys * p.c.Hkv + h) * rec_bytes;
+      const unsigned char* rec = record_of(p.c, tab[pg], h, rec_bytes, b);
       kp[x] = rec + (x * 16 % P) * DH;
       vp[x] = kp[x] + P * DH;
       const float4 sc = *reinterpret_cast<const float4*>(rec + 2 * P * DH);
@@ -1221,7 +1230,7 @@ __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
   int* s_pos = s_row + p.B + 1;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int P = p.c.P, lp = 31 - __clz(P), Hkv = p.c.Hkv, group = p.Hq / Hkv;
-  const int64_t rec = 2 * P * DH + 16;
+  const int rec = 2 * P * DH + 16;
   // a unit in shared memory: records of Pe tokens (whole ones, or a part of one with its scales)
   const int Pe = min(P, UT), lpe = 31 - __clz(Pe), per = UT >> lpe, rec_e = 2 * Pe * DH + 16;
   uint64_t* bar = bars + warp * NS;
@@ -1341,12 +1350,7 @@ __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
       }
       // a unit's pages beyond the last full one are copies of it (masked, but finite)
       const int at = min(page + (lane < per ? lane : 0), ahead.it.p1 - 1) - batch;
-      int phys = __shfl_sync(0xffffffffu, entry, at);
-      if (phys < 0 || phys >= p.c.n_pages) {
-        record_error(DEV_INDEX_RANGE, K_PAGED_ATTN, ahead.b, phys);
-        phys = 0;
-      }
-      const unsigned char* src = p.c.pool + ((int64_t)phys * Hkv + ahead.h) * rec;
+      const unsigned char* src = record_of(p.c, __shfl_sync(0xffffffffu, entry, at), ahead.h, rec, ahead.b);
       if (lane == 0) mbar_arrive_expect_tx(bar + slot, (uint32_t)(per * rec_e));
       __syncwarp();
       if (P <= UT) {

@@ -228,18 +228,14 @@ __global__ void __launch_bounds__(TILE_THREADS, TileShape<T, DH>::CTAS) paged_ti
     const int cw = warp - 4;
     constexpr int KW = S::HG * 2 * (S::E / 4), VW = S::C * 2 * S::M;  // words of a lane: keys, values
     const int32_t* table = p.c.table + b * p.c.table_sb;
-    const int64_t rec = 2 * P * DH + 16;
+    const int rec = 2 * P * DH + 16;
     const int n_mine = min(j1, n_code) - j0;  // blocks of codes
     auto entry = [&](int j) {
       const int page = min(p0 + ((j * TILE_KT + cw * 16) >> lp), p1 - 1);  // beyond the last page: the last again (masked)
       return table[page];
     };
     auto fetch = [&](int j, int phys, uint32_t (&kw)[KW], uint32_t (&vw)[VW], float4& sc) {
-      if (phys < 0 || phys >= p.c.n_pages) {
-        record_error(DEV_INDEX_RANGE, K_PAGED_ATTN, b, phys);
-        phys = 0;
-      }
-      const unsigned char* r = p.c.pool + ((int64_t)phys * p.c.Hkv + h) * rec;
+      const unsigned char* r = record_of(p.c, phys, h, rec, b);
       const unsigned char* k = r + ((j * TILE_KT + cw * 16) & (P - 1)) * DH;
       const unsigned char* v = k + P * DH;
 #pragma unroll
