@@ -40,7 +40,8 @@ const char* ta_last_error(void);
 
 /* Copy the device-side error record {code, kernel, a, b} of the current device into out4 and clear it.
  * Synchronizes the device. code 0 = no error, 1 = bounded wait gave up, 2 = position out of range,
- * 3 = index out of range. */
+ * 3 = index out of range. The serving kernels have a record of their own, which is read where the others' is clear: after an
+ * error, call again until the code is 0. */
 int ta_device_error(int* out4);
 
 /* No counterpart in the reference: a test of the kernels' bounded waits. One CTA waits on an mbarrier that no

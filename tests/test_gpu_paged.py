@@ -931,3 +931,16 @@ def test_pages_outside_the_pool_read_as_nan(dh, page, grp, n, entry):
     want, tol, _, _ = _attend_ref(r, q, [n, n], before, 1 / math.sqrt(dh), 0)
     assert ((again.double() - want).abs() <= tol).all()
     _no_device_error()
+
+
+def test_errors_of_both_kinds_are_reported():
+    """A wait that gave up in one kernel and a position out of range in a serving kernel: one after the other, none lost."""
+    from treeattn_b200 import _lib, _ops
+    P = _mod()
+    r = Rig(1, 1, 64, 16, BF, 64)
+    r.append([3])
+    _no_device_error()
+    _lib.call('ta_wait_probe', 1000 * 1000, _ops._stream(r.cache.pool))
+    P.paged_append(r.cache, r.randn(1, 1, 64), r.randn(1, 1, 64), _starts([1]), _i32([-4]), 1)
+    seen = [_device_error()[:2] for _ in range(3)]
+    assert sorted(seen) == [(0, 0), (1, 13), (2, 16)] and seen[2] == (0, 0)

@@ -111,7 +111,8 @@ def call(name, *args):
 
 
 def device_error():
-    """Read and clear the device-side error record: (code, kernel, a, b). Synchronizes the device."""
+    """Read and clear the device-side error record: (code, kernel, a, b); again until code 0, where there may be more than one.
+    Synchronizes the device."""
     out = (ctypes.c_int * 4)()
     call('ta_device_error', ctypes.cast(out, c_void_p))
     return tuple(out)

@@ -1,7 +1,7 @@
 // Shared device helpers for the treeattn_b200 kernels (sm_100a only).
 //
 // Each translation unit of the library has its own device error record (the symbol below is static); the host reads
-// and clears all of them (ta_device_error).
+// and clears them one after the other (ta_device_error).
 #pragma once
 
 #include <cuda_runtime.h>

@@ -11,11 +11,12 @@
 #include "verify.cuh"
 
 namespace ta_host {
-// This translation unit's device error record (see ta_device_error).
+// This translation unit's device error record (see ta_device_error), read and cleared.
 cudaError_t paged_device_error(int* out4) {
   cudaError_t e = cudaMemcpyFromSymbol(out4, ta::g_dev_err, 4 * sizeof(int));
+  if (e != cudaSuccess || out4[0] == 0) return e;
   const int zero[4] = {0, 0, 0, 0};
-  return e == cudaSuccess ? cudaMemcpyToSymbol(ta::g_dev_err, zero, 4 * sizeof(int)) : e;
+  return cudaMemcpyToSymbol(ta::g_dev_err, zero, 4 * sizeof(int));
 }
 }  // namespace ta_host
 

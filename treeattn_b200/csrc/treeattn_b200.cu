@@ -955,13 +955,13 @@ int ta_device_error(int* out4) {
   if (e != cudaSuccess) return fail(TA_ERR_CUDA, "ta_device_error: %s", cudaGetErrorString(e));
   e = cudaMemcpyFromSymbol(out4, ta::g_dev_err, 4 * sizeof(int));
   if (e != cudaSuccess) return fail(TA_ERR_CUDA, "ta_device_error: %s", cudaGetErrorString(e));
-  const int zero[4] = {0, 0, 0, 0};
-  e = cudaMemcpyToSymbol(ta::g_dev_err, zero, 4 * sizeof(int));
+  if (out4[0] == 0) {  // (an error of the serving kernels stays on record until the others' has been read)
+    e = ta_host::paged_device_error(out4);
+  } else {
+    const int zero[4] = {0, 0, 0, 0};
+    e = cudaMemcpyToSymbol(ta::g_dev_err, zero, 4 * sizeof(int));
+  }
   if (e != cudaSuccess) return fail(TA_ERR_CUDA, "ta_device_error: %s", cudaGetErrorString(e));
-  int other[4];
-  e = ta_host::paged_device_error(other);
-  if (e != cudaSuccess) return fail(TA_ERR_CUDA, "ta_device_error: %s", cudaGetErrorString(e));
-  if (out4[0] == 0) std::copy(other, other + 4, out4);
   return TA_OK;
 }
 
