@@ -944,3 +944,22 @@ def test_errors_of_both_kinds_are_reported():
     P.paged_append(r.cache, r.randn(1, 1, 64), r.randn(1, 1, 64), _starts([1]), _i32([-4]), 1)
     seen = [_device_error()[:2] for _ in range(3)]
     assert sorted(seen) == [(0, 0), (1, 13), (2, 16)] and seen[2] == (0, 0)
+
+
+@pytest.mark.parametrize('rot', [0, 32])
+def test_a_given_query_output_is_written(rot):
+    """q_out receives the queries, rotated or as they are, of the rows that belong to a sequence."""
+    P = _mod()
+    r = Rig(2, 2, 64, 16, BF, 64, seed=rot)
+    qkv = r.randn(5, 8 * 64)
+    q = qkv[:, :4 * 64].view(5, 4, 64)
+    k, v = r.randn(5, 2, 64), r.randn(5, 2, 64)
+    rotation = P.rotation_table(64, rot) if rot else None
+    out = torch.full((5, 4, 64), 9.0, device=DEV, dtype=BF)
+    got = P.paged_append(r.cache, k, v, _starts([3, 2]), _i32([4, 0]), 3, q=q, rotation=rotation, q_out=out)
+    assert got is out
+    want = q if not rot else P.paged_append(r.cache, k, v, _starts([3, 2]), _i32([4, 0]), 3, q=q, rotation=rotation)
+    assert torch.equal(out, want)
+    with pytest.raises(ValueError, match='q_out'):
+        P.paged_append(r.cache, k, v, _starts([3, 2]), _i32([4, 0]), 3, q=q, rotation=rotation, q_out=out[:4])
+    _no_device_error()

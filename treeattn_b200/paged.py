@@ -177,8 +177,8 @@ def paged_append(cache, k, v, start, pos, max_new, q=None, rotation=None, q_out=
     and head strides that keep rows 16-byte aligned; q and the tables too where they rotate by multiples of 16 dims) go to
     positions pos[b], pos[b] + 1, .... `max_new` bounds the rows of one sequence. rotation = (cos, sin)
     (rotation_table) turns the first dims of k, and of q (n, n_head, head_dim) into q_out (allocated here when not given).
-    Without a rotation q is returned as it is. A page is quantised when its last token arrives; afterwards a sequence may be
-    cut back to any length whose page is the last or last but one that was ever written."""
+    Without a rotation q is returned as it is (a given q_out gets a copy). A page is quantised when its last token arrives;
+    afterwards a sequence may be cut back to any length whose page is the last or last but one that was ever written."""
     pool, tail, table = cache.pool, cache.tail, cache.table
     dt = tail.dtype
     B = _rows('paged_append', cache, start, pos)
@@ -204,7 +204,7 @@ def paged_append(cache, k, v, start, pos, max_new, q=None, rotation=None, q_out=
         qshape, qs = _heads('paged_append', cache, q, dt)
         if qshape[0] != n:
             raise ValueError('paged_append: q has %d rows, k %d' % (qshape[0], n))
-        if rot:
+        if rot or q_out is not None:
             Hq, qr, qh = qshape[1], qs[0], qs[1]
             if q_out is None:
                 q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
