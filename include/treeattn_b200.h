@@ -354,9 +354,10 @@ int ta_block_tail(const void* att, float* x, const void* w_proj, const float* ln
  * sequence).
  * A page holds `page` tokens (16, 32 or 64) of one sequence. pool (n_pages, Hkv, 2 * page * dh + 16) bytes: per (page, kv
  * head) the e4m3 codes of its keys, those of its values, the fp32 scales of the two (value = code * scale), a mark (fp32: 1
- * where every value code is 0 for want of a value above 2^-100, else 0) and 4 unused bytes. tail (B, Hkv, 2, 2, page * dh) in `dtype` (bf16 or f16): the open page of each sequence and the page before it,
- * by page parity, keys then values. table (B, max_pages) int32, row stride table_sb: the pool page of each page of a
- * sequence, read for full pages only. Inside a page the elements of each 16-token group stand in fragment order:
+ * where every value code is 0 for want of a value above 2^-100, else 0) and 4 unused bytes. tail (B, Hkv, 2, 2, page * dh) in
+ * `dtype` (bf16 or f16): the open page of each sequence and the page before it, by page parity, keys then values. table (B,
+ * max_pages) int32, row stride table_sb: the pool page of each page of a sequence, read for full pages only. Inside a page the
+ * elements of each 16-token group stand in fragment order:
  *   keys   [h][r][g][t][e]          token 8 r + g, dim h * 4E + t * E + e (E = min(16, dh / 4); r 2, g 8, t 4)
  *   values [c][g][t][m][r][kh][lo]  token 8 kh + 2 t + lo, dim (c M + m) 16 + 8 r + g (M = min(2, dh / 16))
  * New rows: sequence b owns rows [start[b], start[b + 1]) (start: B + 1 int32, device) of the n_rows rows of the call, at
@@ -379,6 +380,10 @@ int ta_block_tail(const void* att, float* x, const void* w_proj, const float* ln
  *   the sum of exponentials (-inf, with zero rows in out, where nothing is attended). ws: scratch of at least
  *   ta_paged_attn_workspace bytes, zeroed before its first use; every call leaves it ready for the next. Calls of any shapes
  *   may share it; they must not overlap on the GPU.
+ *   A wait inside that gives up (2 s) is recorded; the rows of its sequences and heads are NaN, and the workspace is ready for
+ *   the next call all the same.
+ * ta_paged_attn_probe: a test of that. ta_paged_attn in which the copies of one of the call's workers (a warp where a kv head has
+ *   at most 8 rows, a CTA of its first sequence and head where it has more than 32; bf16, head dim 64) never come.
  * ta_verify_drafts: speculative sampling. p (B, G + 1, V) the target's and q (B, G, V) the draft's probabilities (dtype;
  *   unit inner stride, strides in elements), drafts (B, G), u (B, G + 1) uniform numbers in [0, 1), one for each
  *   draft and the last for the draw, n (B) drafts of each sequence or NULL (G). Draft i stands while u_i q_i(d_i) < p_i(d_i); accepted[b] = a, the drafts before the first that
@@ -396,6 +401,11 @@ int ta_paged_attn(const void* pool, const void* tail, const int32_t* table, int6
                   int page, int dtype, int B, int Hq, int Hkv, int dh, const void* q, int64_t q_sr, int64_t q_sh,
                   int n_rows, const int32_t* start, const int32_t* pos, int max_new, float scale, int window, void* out,
                   int64_t o_sr, int64_t o_sh, float* lse, void* ws, int64_t ws_bytes, void* stream);
+int ta_paged_attn_probe(int worker, const void* pool, const void* tail, const int32_t* table, int64_t table_sb, int n_pages,
+                        int max_pages, int page, int dtype, int B, int Hq, int Hkv, int dh, const void* q, int64_t q_sr,
+                        int64_t q_sh, int n_rows, const int32_t* start, const int32_t* pos, int max_new, float scale,
+                        int window, void* out, int64_t o_sr, int64_t o_sh, float* lse, void* ws, int64_t ws_bytes,
+                        void* stream);
 int ta_verify_drafts(const void* p, int64_t p_sb, int64_t p_sr, const void* q, int64_t q_sb, int64_t q_sr, int dtype, int B,
                      int G, int V, const int64_t* drafts, const float* u, const int32_t* n, int64_t* tokens,
                      int32_t* accepted, void* stream);

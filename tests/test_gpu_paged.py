@@ -963,3 +963,39 @@ def test_a_given_query_output_is_written(rot):
     with pytest.raises(ValueError, match='q_out'):
         P.paged_append(r.cache, k, v, _starts([3, 2]), _i32([4, 0]), 3, q=q, rotation=rotation, q_out=out[:4])
     _no_device_error()
+
+
+@pytest.mark.parametrize('Hkv,grp,n,before,room,worker', [(4, 1, 1, [3000, 700], 0, 1), (4, 1, 1, [3000, 700], 0, 9), (1, 8, 1, [9000, 300], 30000, 3),
+                                                           (2, 1, 4, [9000, 40], 30000, 1), (2, 1, 60, [3000, 40], 0, 0),
+                                                           (2, 1, 60, [3000, 40], 0, 2), (160, 1, 40, [100, 90], 0, 0)])
+def test_a_wait_that_gives_up_leaves_the_workspace_ready(Hkv, grp, n, before, room, worker):
+    """One worker's copies never come: its wait runs out after 2 s and is recorded, the rows of the items it took part in are NaN, all
+    others are as ever, and the next call on the same workspace gives what it gave before."""
+    from treeattn_b200 import _lib
+    P = _mod()
+    B, dh = len(before), 64
+    r = Rig(B, Hkv, dh, 64, BF, max(max(before) + n, room), seed=Hkv + n)
+    r.append(before)
+    r.append([n] * B)
+    q = r.randn(B * n, Hkv * grp, dh)
+    start, pos = _starts([n] * B), _i32(before)
+    ws = P.paged_attn_workspace(B, Hkv * grp, Hkv, dh, n)
+    want = P.paged_attn(r.cache, q, start, pos, n, ws=ws)
+    got, lse = torch.zeros_like(want), torch.zeros(B * n, Hkv * grp, device=DEV)
+    c = r.cache
+    _no_device_error()
+    _lib.call('ta_paged_attn_probe', worker, c.pool.data_ptr(), c.tail.data_ptr(), c.table.data_ptr(), c.table.stride(0),
+              c.pool.shape[0], c.table.shape[1], 64, 1, B, Hkv * grp, Hkv, dh, q.data_ptr(), q.stride(0), q.stride(1), B * n,
+              start.data_ptr(), pos.data_ptr(), n, 0.125, 0, got.data_ptr(), got.stride(0), got.stride(1), lse.data_ptr(),
+              ws.data_ptr(), ws.nbytes, P._stream(q))
+    code = _device_error()
+    assert code[0] == 1 and code[1] in (17, 19), code
+    bad = torch.isnan(lse)
+    assert bad.any() and not bad.all()
+    assert torch.isnan(got[bad]).all() and torch.equal(got[~bad], want[~bad])
+    heads = bad.view(B, n, Hkv, grp)
+    if n * grp <= 8:  # an item is NaN as a whole (a tile: 128 of its rows)
+        assert torch.equal(heads, heads[:, :1, :, :1].expand_as(heads))
+    for _ in range(2):
+        assert torch.equal(P.paged_attn(r.cache, q, start, pos, n, ws=ws), want)
+    _no_device_error()

@@ -67,6 +67,7 @@ SIGNATURES = {
     'ta_paged_append': [P, P, P, L, I, I, I, I, I, I, I, P, P, L, L, L, L, I, P, P, I, P, P, I, I, P, I, L, L, P, P],
     'ta_paged_attn_workspace': [I, I, I, I, I],
     'ta_paged_attn': [P, P, P, L, I, I, I, I, I, I, I, I, P, L, L, I, P, P, I, F, I, P, L, L, P, P, L, P],
+    'ta_paged_attn_probe': [I, P, P, P, L, I, I, I, I, I, I, I, I, P, L, L, I, P, P, I, F, I, P, L, L, P, P, L, P],
     'ta_verify_drafts': [P, L, L, P, L, L, I, I, I, I, P, P, P, P, P, P],
     'ta_block_tail': [P, P, P, P, P, P, P, P, F, I, I, I, P, P, P, L, P, P],
 }

@@ -114,7 +114,7 @@ bool split_late(const ta::AttnParams& p) {
   return parts * SH::STATE * 4 > ta::SPLIT_SPOT_BYTES;
 }
 
-template <typename T, int DH, int NT, bool LATE>
+template <typename T, int DH, int NT, bool LATE, bool PROBE = false>
 int launch_split(const ta::AttnParams& p, void* ws, int64_t ws_bytes, cudaStream_t st) {
   using SH = ta::SplitShape<DH, NT>;
   const int64_t need = split_bytes<DH, NT>();
@@ -123,20 +123,20 @@ int launch_split(const ta::AttnParams& p, void* ws, int64_t ws_bytes, cudaStream
                 (long long)ws_bytes);
   static SmemAttr attr;
   const int smem = SH::RING + SH::BAR_BYTES + 12 * (p.B + 1);
-  if (int r = allow_smem(attr, ta::paged_split_kernel<T, DH, NT, LATE>, smem, "ta_paged_attn")) return r;
+  if (int r = allow_smem(attr, ta::paged_split_kernel<T, DH, NT, LATE, PROBE>, smem, "ta_paged_attn")) return r;
   float* states = reinterpret_cast<float*>(reinterpret_cast<char*>(ws) + kCounterBytes);
-  const cudaError_t e = launch_pdl(ta::paged_split_kernel<T, DH, NT, LATE>, dim3(sm_count()), dim3(SH::WARPS * 32), smem, st, p,
-                                   reinterpret_cast<int32_t*>(ws), states);
+  const cudaError_t e = launch_pdl(ta::paged_split_kernel<T, DH, NT, LATE, PROBE>, dim3(sm_count()), dim3(SH::WARPS * 32), smem,
+                                   st, p, reinterpret_cast<int32_t*>(ws), states);
   if (e != cudaSuccess) return fail(TA_ERR_CUDA, "ta_paged_attn: launch failed: %s", cudaGetErrorString(e));
   return TA_OK;
 }
 
-template <typename T, int DH, int NT>
+template <typename T, int DH, int NT, bool PROBE = false>
 int run_split(const ta::AttnParams& p, void* ws, int64_t ws_bytes, cudaStream_t st) {
   if constexpr (ta::split_spot<DH, NT>()) {
-    if (!split_late<DH, NT>(p)) return launch_split<T, DH, NT, false>(p, ws, ws_bytes, st);
+    if (!split_late<DH, NT>(p)) return launch_split<T, DH, NT, false, PROBE>(p, ws, ws_bytes, st);
   }
-  return launch_split<T, DH, NT, true>(p, ws, ws_bytes, st);
+  return launch_split<T, DH, NT, true, PROBE>(p, ws, ws_bytes, st);
 }
 
 // The tile form (head dims 64 and 128): CTAs that share a tile's blocks, as many as make the tiles fill the GPU.
@@ -152,7 +152,7 @@ int64_t tile_bytes(int64_t B, int64_t Hkv, int64_t rows, int dh) {
   return kCounterBytes + items * splits * ta::TILE_ROWS * (dh + 2) * 4;
 }
 
-template <typename T, int DH>
+template <typename T, int DH, bool PROBE = false>
 int run_tile(const ta::AttnParams& p, int64_t rows, void* ws, int64_t ws_bytes, cudaStream_t st) {
   using C = ta::TileShape<T, DH>;
   const int64_t need = tile_bytes(p.B, p.c.Hkv, rows, DH), tiles = tiles_of(rows);
@@ -167,8 +167,8 @@ int run_tile(const ta::AttnParams& p, int64_t rows, void* ws, int64_t ws_bytes, 
   tp.states = reinterpret_cast<float*>(reinterpret_cast<char*>(ws) + kCounterBytes);
   static SmemAttr attr;
   constexpr int smem = 1024 + C::BYTES + (int)sizeof(ta::TileBars);
-  if (int r = allow_smem(attr, ta::paged_tile_kernel<T, DH>, smem, "ta_paged_attn")) return r;
-  const cudaError_t e = launch_pdl(ta::paged_tile_kernel<T, DH>, dim3((unsigned)(tiles * tp.splits), p.c.Hkv, p.B),
+  if (int r = allow_smem(attr, ta::paged_tile_kernel<T, DH, PROBE>, smem, "ta_paged_attn")) return r;
+  const cudaError_t e = launch_pdl(ta::paged_tile_kernel<T, DH, PROBE>, dim3((unsigned)(tiles * tp.splits), p.c.Hkv, p.B),
                                    dim3(ta::TILE_THREADS), smem, st, tp);
   if (e != cudaSuccess) return fail(TA_ERR_CUDA, "ta_paged_attn: launch failed: %s", cudaGetErrorString(e));
   return TA_OK;
@@ -206,6 +206,49 @@ cudaError_t launch_verify(void (*kern)(ta::VerifyParams), int cs, cudaStream_t s
   cfg.attrs = attr;
   cfg.numAttrs = 2;
   return cudaLaunchKernelEx(&cfg, kern, a);
+}
+
+int paged_attn(const char* who, int probe, const void* pool, const void* tail, const int32_t* table, int64_t table_sb,
+               int n_pages, int max_pages, int page, int dtype, int B, int Hq, int Hkv, int dh, const void* q, int64_t q_sr,
+               int64_t q_sh, int n_rows, const int32_t* start, const int32_t* pos, int max_new, float scale, int window,
+               void* out, int64_t o_sr, int64_t o_sh, float* lse, void* ws, int64_t ws_bytes, void* stream) {
+  g_err.clear();
+  if (int r = check_cache(who, pool, tail, table, table_sb, n_pages, max_pages, page, dtype, B, Hq, Hkv, dh, n_rows, start,
+                          pos, max_new))
+    return r;
+  if (window < 0) return fail(TA_ERR_ARG, "%s: window %d", who, window);
+  if (window >= (int64_t)(max_pages + 1) * page) window = 0;  // longer than any sequence
+  if (B == 0 || n_rows == 0 || max_new == 0) return TA_OK;
+  if (!q || !out) return fail(TA_ERR_ARG, "%s: null pointer", who);
+  if (!rows_aligned(q, 2, {q_sr, q_sh}) || !rows_aligned(out, 2, {o_sr, o_sh}))
+    return fail(TA_ERR_ARG, "%s: q and out rows must be 16-byte aligned", who);
+  if ((int64_t)max_new * (Hq / Hkv) > INT_MAX / 2) return fail(TA_ERR_ARG, "%s: too many rows", who);
+  ta::AttnParams p{};
+  p.c = {const_cast<unsigned char*>(reinterpret_cast<const unsigned char*>(pool)), const_cast<void*>(tail), table, table_sb,
+         n_pages, max_pages, Hkv, page};
+  p.q = q; p.q_sr = q_sr; p.q_sh = q_sh;
+  p.start = start; p.pos = pos;
+  p.B = B; p.n_rows = n_rows; p.max_new = max_new; p.Hq = Hq;
+  p.scale = scale; p.window = window;
+  p.out = out; p.o_sr = o_sr; p.o_sh = o_sh; p.lse = lse;
+  const cudaStream_t st = S(stream);
+  if (probe >= 0) {
+    const int64_t rows = (int64_t)max_new * (Hq / Hkv);
+    p.probe = probe;
+    if (dtype != TA_BF16 || dh != 64 || (rows > 8 && rows <= kSplitRows) || !split_takes(B, Hkv, 1, max_pages, page))
+      return fail(TA_ERR_ARG, "%s: bfloat16 rows of head dim 64, at most 8 or more than %d of a kv head", who, kSplitRows);
+    if (rows <= 8) return run_split<__nv_bfloat16, 64, 1, true>(p, ws, ws_bytes, st);
+    return run_tile<__nv_bfloat16, 64, true>(p, rows, ws, ws_bytes, st);
+  }
+#define TA_ATTN(T)                                                              \
+  switch (dh) {                                                                 \
+    case 16: return run_attn<T, 16>(p, ws, ws_bytes, st);                                   \
+    case 32: return run_attn<T, 32>(p, ws, ws_bytes, st);                                   \
+    case 64: return run_attn<T, 64>(p, ws, ws_bytes, st);                                   \
+    default: return run_attn<T, 128>(p, ws, ws_bytes, st);                                  \
+  }
+  if (dtype == TA_BF16) { TA_ATTN(__nv_bfloat16) } else { TA_ATTN(__half) }
+#undef TA_ATTN
 }
 
 }  // namespace
@@ -270,36 +313,19 @@ int ta_paged_attn(const void* pool, const void* tail, const int32_t* table, int6
                   int page, int dtype, int B, int Hq, int Hkv, int dh, const void* q, int64_t q_sr, int64_t q_sh,
                   int n_rows, const int32_t* start, const int32_t* pos, int max_new, float scale, int window, void* out,
                   int64_t o_sr, int64_t o_sh, float* lse, void* ws, int64_t ws_bytes, void* stream) {
+  return paged_attn("ta_paged_attn", -1, pool, tail, table, table_sb, n_pages, max_pages, page, dtype, B, Hq, Hkv, dh, q,
+                    q_sr, q_sh, n_rows, start, pos, max_new, scale, window, out, o_sr, o_sh, lse, ws, ws_bytes, stream);
+}
+
+int ta_paged_attn_probe(int worker, const void* pool, const void* tail, const int32_t* table, int64_t table_sb, int n_pages,
+                        int max_pages, int page, int dtype, int B, int Hq, int Hkv, int dh, const void* q, int64_t q_sr,
+                        int64_t q_sh, int n_rows, const int32_t* start, const int32_t* pos, int max_new, float scale,
+                        int window, void* out, int64_t o_sr, int64_t o_sh, float* lse, void* ws, int64_t ws_bytes,
+                        void* stream) {
   g_err.clear();
-  const char* who = "ta_paged_attn";
-  if (int r = check_cache(who, pool, tail, table, table_sb, n_pages, max_pages, page, dtype, B, Hq, Hkv, dh, n_rows, start,
-                          pos, max_new))
-    return r;
-  if (window < 0) return fail(TA_ERR_ARG, "%s: window %d", who, window);
-  if (window >= (int64_t)(max_pages + 1) * page) window = 0;  // longer than any sequence
-  if (B == 0 || n_rows == 0 || max_new == 0) return TA_OK;
-  if (!q || !out) return fail(TA_ERR_ARG, "%s: null pointer", who);
-  if (!rows_aligned(q, 2, {q_sr, q_sh}) || !rows_aligned(out, 2, {o_sr, o_sh}))
-    return fail(TA_ERR_ARG, "%s: q and out rows must be 16-byte aligned", who);
-  if ((int64_t)max_new * (Hq / Hkv) > INT_MAX / 2) return fail(TA_ERR_ARG, "%s: too many rows", who);
-  ta::AttnParams p{};
-  p.c = {const_cast<unsigned char*>(reinterpret_cast<const unsigned char*>(pool)), const_cast<void*>(tail), table, table_sb,
-         n_pages, max_pages, Hkv, page};
-  p.q = q; p.q_sr = q_sr; p.q_sh = q_sh;
-  p.start = start; p.pos = pos;
-  p.B = B; p.n_rows = n_rows; p.max_new = max_new; p.Hq = Hq;
-  p.scale = scale; p.window = window;
-  p.out = out; p.o_sr = o_sr; p.o_sh = o_sh; p.lse = lse;
-  const cudaStream_t st = S(stream);
-#define TA_ATTN(T)                                                              \
-  switch (dh) {                                                                 \
-    case 16: return run_attn<T, 16>(p, ws, ws_bytes, st);                                   \
-    case 32: return run_attn<T, 32>(p, ws, ws_bytes, st);                                   \
-    case 64: return run_attn<T, 64>(p, ws, ws_bytes, st);                                   \
-    default: return run_attn<T, 128>(p, ws, ws_bytes, st);                                  \
-  }
-  if (dtype == TA_BF16) { TA_ATTN(__nv_bfloat16) } else { TA_ATTN(__half) }
-#undef TA_ATTN
+  if (worker < 0) return fail(TA_ERR_ARG, "ta_paged_attn_probe: worker %d", worker);
+  return paged_attn("ta_paged_attn_probe", worker, pool, tail, table, table_sb, n_pages, max_pages, page, dtype, B, Hq, Hkv, dh, q,
+                    q_sr, q_sh, n_rows, start, pos, max_new, scale, window, out, o_sr, o_sh, lse, ws, ws_bytes, stream);
 }
 
 int ta_verify_drafts(const void* p, int64_t p_sb, int64_t p_sr, const void* q, int64_t q_sb, int64_t q_sr, int dtype, int B,

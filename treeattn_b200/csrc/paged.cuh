@@ -434,6 +434,7 @@ struct AttnParams {
   void* out;
   int64_t o_sr, o_sh;
   float* lse;  // (rows, Hq) or null
+  int probe;   // PROBE: the warp (split form) or CTA (tile form) whose first wait runs out
 };
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -570,11 +571,11 @@ struct RowTile {
 template <int DH, int NT>
 struct SoftState {
   float m[NT][2], l[NT][2], o[DH / 16][NT][4];
-  __device__ __forceinline__ void clear() {
+  __device__ __forceinline__ void clear(float sum = 0.f) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       m[nt][0] = m[nt][1] = -INFINITY;
-      l[nt][0] = l[nt][1] = 0.f;
+      l[nt][0] = l[nt][1] = sum;
 #pragma unroll
       for (int x = 0; x < DH / 16; ++x)
 #pragma unroll
@@ -1211,7 +1212,7 @@ __device__ __noinline__ void join_tile(const Join* join, const float* states, co
   }
 }
 
-template <typename T, int DH, int NT, bool LATE>
+template <typename T, int DH, int NT, bool LATE, bool PROBE = false>
 __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
     paged_split_kernel(AttnParams p, int32_t* counters, float* states) {
   using SH = SplitShape<DH, NT>;
@@ -1339,7 +1340,15 @@ __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
     entry = load_entry(batch + lane);
     entry_next = load_entry(batch + 32 + lane);
   };
+  bool skip = PROBE && me == p.probe;
   auto issue = [&](int slot) {
+    if constexpr (PROBE) {
+      if (skip) {  // a copy that never comes
+        skip = false;
+        if (++ahead.k == ahead.end) begin_ahead(ahead.next);
+        return;
+      }
+    }
     unsigned char* dst = ring + (warp * NS + slot) * SH::STAGE;
     if (ahead.k < ahead.it.nu8) {
       const int page = ahead.it.p0 + ((ahead.k * UT) >> lp);
@@ -1392,15 +1401,18 @@ __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
     rt.finish(p, run.it.pos, group, 0, run.it.n * group, raw);
     const Item& it = run.it;
     const int R = it.n * group;
-    st.clear();
+    st.clear(ok ? 0.f : NAN);
     const int qhi = it.pos + it.n - 1;
     uint32_t odd = 0u;  // the open page holds an infinity or NaN
-    for (int k = run.k; k < run.end; ++k, ++step) {
+    const int last = ok ? run.end : run.k;
+    for (int k = run.k; k < last; ++k, ++step) {
       const int slot = step % NS;
       const unsigned char* src = ring + (warp * NS + slot) * SH::STAGE;
       if (!mbar_wait_bounded(bar + slot, (step / NS) & 1, K_PAGED_ATTN, 1)) {
+        // This run and the warp's later ones are NaN; they arrive all the same, so that the others' counters come back to zero.
         ok = false;
-        break;
+        st.clear(NAN);
+        break;  // (step stays)
       }
       if (k < it.nu8) {
         const int tok0 = (it.p0 << lp) + k * UT, limit = it.p1 << lp;
@@ -1433,7 +1445,6 @@ __global__ void __launch_bounds__(SplitShape<DH, NT>::WARPS * 32, 1)
         ++issued;
       }
     }
-    if (!ok) break;
     // ---- the run's end: out, or into the workspace
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)

@@ -130,7 +130,7 @@ __device__ __forceinline__ unsigned char* tile_piece(unsigned char* tile, int ro
   return tile + row * 128 + ((c ^ (row & 7)) << 4);
 }
 
-template <typename T, int DH>
+template <typename T, int DH, bool PROBE = false>
 __global__ void __launch_bounds__(TILE_THREADS, TileShape<T, DH>::CTAS) paged_tile_kernel(TileParams tp) {
   using C = TileShape<T, DH>;
   using S = PageShape<DH>;
@@ -353,7 +353,8 @@ __global__ void __launch_bounds__(TILE_THREADS, TileShape<T, DH>::CTAS) paged_ti
     if (n_mine > 1) fetch(j0 + 1, eb, kb, vb, sb);
     if (n_mine > 2) ea = entry(j0 + 2);
     if (n_mine > 3) eb = entry(j0 + 3);
-    for (int n = 0; n < nblk; n += 2) {
+    const bool absent = PROBE && (int)blockIdx.x == p.probe && blockIdx.y + blockIdx.z == 0;  // its tiles never come
+    for (int n = 0; n < nblk && !absent; n += 2) {
       if (!block(n, ka, va, sa, ea)) break;
       if (n + 1 < nblk && !block(n + 1, kb, vb, sb, eb)) break;
     }
@@ -546,33 +547,38 @@ __global__ void __launch_bounds__(TILE_THREADS, TileShape<T, DH>::CTAS) paged_ti
                        1, out);
       if (p.lse && live) p.lse[out_row * p.Hq + hq] = l == 0.f ? -INFINITY : (ref - SHIFT + log2f(l)) * 0.69314718055994531f;
     };
-    if (good && tp.splits == 1) {
+    if (!good) {  // a wait that gave up: the rows are NaN, and the tile's counter comes back to zero all the same
+      l = NAN;
+      ref = -INFINITY;
+    }
+    if (tp.splits == 1) {
       const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll 1
       for (int c = 0; c < DH; c += 32) {
         float o[32];
-        tmem_ld32(lane_base + TM_O + c, o);
+        if (good) tmem_ld32(lane_base + TM_O + c, o);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) o[i] *= inv;
+        for (int i = 0; i < 32; ++i) o[i] = good ? o[i] * inv : NAN;
         if (live) {
 #pragma unroll
           for (int i = 0; i < 32; i += 8) store_vec_from_f32<T>(out + c + i, o + i);
         }
       }
       finish(*reinterpret_cast<volatile int*>(&bar.odd));
-    } else if (good) {
+    } else {
       // this CTA's share of the blocks; the last of the tile's CTAs joins them in order
       const int64_t item = ((int64_t)b * p.c.Hkv + h) * tp.tiles + tile;
       float* states = tp.states + item * tp.splits * C::STATE;
       float* mine = states + split * C::STATE;
+      const bool have = good && nblk > 0;
 #pragma unroll 1
       for (int c = 0; c < DH; c += 32) {
         float o[32];
-        if (nblk > 0) tmem_ld32(lane_base + TM_O + c, o);
+        if (have) tmem_ld32(lane_base + TM_O + c, o);
 #pragma unroll
         for (int i = 0; i < 32; i += 4)
           __stcg(reinterpret_cast<float4*>(mine) + (c + i) / 4 * TILE_ROWS + tid,
-                 nblk > 0 ? make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]) : make_float4(0.f, 0.f, 0.f, 0.f));
+                 have ? make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]) : make_float4(0.f, 0.f, 0.f, 0.f));
       }
       __stcg(mine + TILE_ROWS * DH + tid, ref);
       __stcg(mine + TILE_ROWS * (DH + 1) + tid, l);
