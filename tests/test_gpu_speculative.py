@@ -217,3 +217,35 @@ def test_a_context_is_used_to_its_last_position(neighbors):
         logits = _dense(W, cfg, idx[:, :-1], torch.bfloat16)[0, T - 1:]
         chosen = logits.gather(1, idx[0, T:, None])[:, 0]
         assert (logits.max(-1).values - chosen <= 0.5 * logits.std()).all()
+
+
+@pytest.mark.parametrize('neighbors', [False, True])
+def test_sampled_rounds_follow_the_target(neighbors):
+    """The first token of a round and the one before it: over many sequences and rounds of one prompt each pair's count within 5
+    standard deviations of what the target's probabilities give, whatever the draft proposes (its weights are another model's)."""
+    from treeattn_b200.config import Config
+    from treeattn_b200.engine import Decoder
+    from treeattn_b200.speculative import PagedDecoder, SpeculativeDecoder
+    V, B, T, rounds = 8, 1024, 24, 6
+    cfg, W = _model(7, n_layer=1, n_head=2, n_embd=128, vocab=V, seq_len=64)
+    cfg = Config(**dict(cfg.to_dict(), neighbors=neighbors))
+    _, other = _model(8, n_layer=1, n_head=2, n_embd=128, vocab=V, seq_len=64)
+    args = (cfg.n_layer, cfg.n_head, cfg.n_embd)
+    draft = Decoder(other, *args, cfg.seq_len, 'seg', cfg, DEV, batch=B, dtype=torch.bfloat16)
+    target = PagedDecoder(W, *args, batch=B, max_len=64, page=16)
+    dec = SpeculativeDecoder(draft, target, 3, generator=torch.Generator(DEV).manual_seed(1))
+    prompt = torch.randint(V, (1, T), generator=torch.Generator().manual_seed(9))
+    counts = torch.zeros(V, V, device=DEV, dtype=torch.float64)
+    for _ in range(rounds):
+        first = dec.prefill(prompt.expand(B, T)).clone()
+        second = torch.tensor([x[0] for x in dec.step()], device=DEV)
+        counts += torch.bincount(first * V + second, minlength=V * V).view(V, V)
+    one = PagedDecoder(W, *args, batch=V, max_len=64, page=16)
+    p0 = dec._probs(one.forward(prompt.expand(V, T))[:1, -1])[0].double()
+    p1 = dec._probs(one.forward(torch.arange(V)[:, None])[:, -1]).double()
+    p = p0[:, None] * p1
+    n = B * rounds
+    assert 0.02 < dec.accepted / dec.drafted < 0.98  # some drafts stand, some fall
+    # (the 16-bit logits of batches of other sizes differ by 2^-8 of them at most: a few per cent of a probability)
+    sd = (n * p * (1 - p)).sqrt()
+    assert ((counts - n * p).abs() <= 5 * sd + 0.02 * n * p + 1).all(), (counts / n, p)
