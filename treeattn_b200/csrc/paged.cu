@@ -94,21 +94,24 @@ int64_t split_bytes_dh(int64_t rows) {
   return split_bytes<DH, 4>();
 }
 
-// Rows of one (sequence, kv head) up to which the call takes the split form. Split / tile form in us, 24 and 32 rows: 16 sequences
-// of 8000, 4 heads of 64: 37 / 59, 51 / 59; of 128: 64 / 92, 97 / 92; one of 30000, 8 heads of 128: 59 / 95, 83 / 95. (More than
-// 32 rows would not fit the split form's registers.)
+// Rows of one (sequence, kv head) up to which the call takes the split form (more would not fit its registers). Split / tile form
+// in us: 24 rows, 16 sequences of 8000, 4 heads of 64: 37 / 59, of 128: 64 / 92. At 32 rows either may win: one sequence of 30000, 8
+// heads of 64: 46 / 72, of 128: 84 / 96; 8 of 30000: 127 / 165, 255 / 292; 16 of 8000, 4 heads: 53 / 60, 98 / 93; 64 of 2000: 62 / 54,
+// 108 / 94; 4 of 1000: 23 / 21, 33 / 27; 2 of 20000, 2 heads: 35 / 54, 86 / 68. The lengths, which decide it, are on the device.
 constexpr int kSplitRows = 32;
 
 bool split_takes(int64_t B, int64_t Hkv, int64_t rows, int64_t max_pages, int P) {
   return rows <= kSplitRows && B <= ta::SPLIT_MAX_BATCH && B * Hkv <= kItems && B * Hkv * (max_pages * P / 32 + 7) <= INT_MAX;
 }
 
-// Whether an item's states are joined late: by the parts it has where the batch is even, and the cache as full as it can be
-// (the lengths are on the device).
+// Whether an item's states are joined late: by the parts it has where the batch is even, and the cache as full as it can be (the
+// lengths are on the device). Where they are not, it is the wrong side: one sequence of 4096, 12 heads of 64, in a table for 32768
+// takes 11.6 us, in one of its own length 9.5; one of 30000 among 15 of 500, 8 heads, 8 rows, takes 27 us at 64 and 47 at 128, alone
+// 18.5 and 29.
 template <int DH, int NT>
 bool split_late(const ta::AttnParams& p) {
   using SH = ta::SplitShape<DH, NT>;
-  const int64_t held = (int64_t)p.c.max_pages * p.c.P, seen = p.window > 0 ? std::min<int64_t>(held, p.window + p.max_new) : held;
+  const int64_t held = (int64_t)p.c.max_pages * p.c.P, seen = p.window > 0 ? std::min<int64_t>(held, (int64_t)p.window + p.max_new) : held;
   const int64_t parts = std::min<int64_t>((int64_t)sm_count() * SH::WARPS / ((int64_t)p.B * p.c.Hkv),
                                           seen / (SH::UT * ta::SPLIT_MIN_UNITS));
   return parts * SH::STATE * 4 > ta::SPLIT_SPOT_BYTES;

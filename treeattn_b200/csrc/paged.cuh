@@ -415,7 +415,7 @@ __global__ void __launch_bounds__(APPEND_THREADS) paged_append_kernel(AppendPara
 // Rows of a (sequence, kv head): query i, head gq of the group -> row i * group + gq. A warp takes 8 NT rows as the N side of
 // mma.m16n8k16 and the keys (S^T = K Q^T) or the head dims (O^T = V^T P^T) as the M side, so that one key or value fragment
 // serves every row and a lone row costs one n-tile.
-//  * codes go to f16 exactly; q is scaled by a power of two per row (exact, undone in the score's factor) so that bf16
+//  * codes go to f16 exactly; q is scaled by a power of two per row (undone in the score's factor; see finish) so that bf16
 //    rows fit f16 as well; the products are exact and the sums fp32.
 //  * the value scale joins the weight: w_t = exp2(s_t + log2 vs - ref), with the running reference taken over s + log2 vs, so
 //    that every w stays in f16's range (at most 2^12); the denominator adds w / vs in fp32. w is rounded to f16 (2^-11

@@ -14,7 +14,8 @@ namespace ta {
 // that the token comes from; the shares meet through distributed shared memory, and the CTA whose share holds the mark
 // looks through the one warp-sized piece that does. Latency-bound: two dependent loads, one pass over the row, one cluster
 // barrier, one more look at a piece (in L2). Vocabulary 50304, four drafts, fp32: one sequence 7.6 us, 64 sequences 13 us (26 MB of
-// rows at most); 256 of 32000, eight drafts, bf16: 18 us.
+// rows at most); 256 of 32000, eight drafts, bf16: 18 us
+// (all CTAs resident at once; the second look is at a whole warp's 2048 words).
 constexpr int VERIFY_THREADS = 256;
 constexpr int VERIFY_WARPS = VERIFY_THREADS / 32;
 constexpr int VERIFY_MAX_CLUSTER = 8;
