@@ -111,7 +111,8 @@ bool split_takes(int64_t B, int64_t Hkv, int64_t rows, int64_t max_pages, int P)
 template <int DH, int NT>
 bool split_late(const ta::AttnParams& p) {
   using SH = ta::SplitShape<DH, NT>;
-  const int64_t held = (int64_t)p.c.max_pages * p.c.P, seen = p.window > 0 ? std::min<int64_t>(held, (int64_t)p.window + p.max_new) : held;
+  const int64_t held = (int64_t)p.c.max_pages * p.c.P;
+  const int64_t seen = p.window > 0 ? std::min<int64_t>(held, (int64_t)p.window + p.max_new) : held;
   const int64_t parts = std::min<int64_t>((int64_t)sm_count() * SH::WARPS / ((int64_t)p.B * p.c.Hkv),
                                           seen / (SH::UT * ta::SPLIT_MIN_UNITS));
   return parts * SH::STATE * 4 > ta::SPLIT_SPOT_BYTES;

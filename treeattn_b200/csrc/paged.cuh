@@ -2,10 +2,9 @@
 //
 // A page holds P tokens (16, 32 or 64) of one sequence. The pool keeps one record of 2 * P * DH + 16 bytes per (page,
 // kv head): the e4m3 codes of the keys, those of the values, then the fp32 scales of the two and a mark (1: all values are 0);
-// value = code * scale. A page
-// is quantised once, when its last token arrives, from 16-bit values: until then its tokens live in the 16-bit tail, a
-// ring of two pages per (sequence, kv head) addressed by the page's parity. So the codes depend on the tokens alone, not on
-// how they arrived, and a sequence can be cut back to any length whose last page is still in the ring.
+// value = code * scale. A page is quantised once, when its last token arrives, from 16-bit values: until then its tokens live in
+// the 16-bit tail, a ring of two pages per (sequence, kv head) addressed by the page's parity. So the codes depend on the tokens
+// alone, not on how they arrived, and a sequence can be cut back to any length whose last page is still in the ring.
 //
 // Inside a page (record and tail alike) the elements of each 16-token group stand in the order in which the m16n8k16
 // fragments take them, so that a warp reads a fragment with one vector load per lane from consecutive addresses:
@@ -363,7 +362,8 @@ __global__ void __launch_bounds__(APPEND_THREADS) paged_append_kernel(AppendPara
     }
     unsigned char* rec = p.c.pool + ((int64_t)phys * p.c.Hkv + h) * (2 * P * DH + 16);
     if (tid == 0)  // (codes are 0 below 2^-100 alone: the marked pages have scale 1)
-      *reinterpret_cast<float4*>(rec + 2 * P * DH) = make_float4(scale[0], scale[1], mul[1] == 0.f && scale[1] == 1.f ? ZERO_MARK : 0.f, 0.f);
+      *reinterpret_cast<float4*>(rec + 2 * P * DH) =
+          make_float4(scale[0], scale[1], mul[1] == 0.f && scale[1] == 1.f ? ZERO_MARK : 0.f, 0.f);
     // a page with a non-finite element has codes 0 (0 * NaN would not be)
     const bool zk = mul[0] == 0.f, zv = mul[1] == 0.f;
     for (int id = tid; id < P * DH / S::E; id += APPEND_THREADS) {

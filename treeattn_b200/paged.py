@@ -19,9 +19,9 @@ class PagedKV:
     """The cache of one layer: the tensors that the kernels read and write (include/treeattn_b200.h has the layout).
 
     pool (n_pages, n_kv_head, 2 * page * head_dim + 16) uint8: a record per (page, kv head): e4m3 codes of the keys, of the
-    values, their two fp32 scales, the mark of a page of zeros. tail (batch, n_kv_head, 2, 2, page * head_dim) bf16 or f16: the open page of each sequence
-    and the one before it. table (batch, max_pages) int32: the pool page of each page of a sequence (several layers may
-    share one). PagedKV.empty allocates pool and tail."""
+    values, their two fp32 scales, the mark of a page of zeros. tail (batch, n_kv_head, 2, 2, page * head_dim) bf16 or f16:
+    the open page of each sequence and the one before it. table (batch, max_pages) int32: the pool page of each page of a
+    sequence (several layers may share one). PagedKV.empty allocates pool and tail."""
     __slots__ = ('pool', 'tail', 'table', 'page', 'head_dim')
 
     def __init__(self, pool, tail, table, page, head_dim):
