@@ -406,6 +406,13 @@ int ta_paged_attn_probe(int worker, const void* pool, const void* tail, const in
                         int64_t q_sh, int n_rows, const int32_t* start, const int32_t* pos, int max_new, float scale,
                         int window, void* out, int64_t o_sr, int64_t o_sh, float* lse, void* ws, int64_t ws_bytes,
                         void* stream);
+/* ta_record_copy: in each of n_bufs buffers of n_records records (record_bytes, a multiple of 16), record dst[i] takes what record
+ *   src[i] held before the call, for all i at once: chains and cycles of moves are fine. bufs, src and dst are HOST arrays (their
+ *   content travels with the launch: they may be changed afterwards, and a captured call keeps its own). Refused: a record
+ *   outside the buffer, one that is written twice, buffers that overlap, a cycle of more than 2047 moves. Pages of a pool (layer by
+ *   layer) and the sequences of a tail are such records. */
+int ta_record_copy(void* const* bufs, int n_bufs, int64_t record_bytes, int n_records, const int32_t* src,
+                   const int32_t* dst, int n, void* stream);
 int ta_verify_drafts(const void* p, int64_t p_sb, int64_t p_sr, const void* q, int64_t q_sb, int64_t q_sr, int dtype, int B,
                      int G, int V, const int64_t* drafts, const float* u, const int32_t* n, int64_t* tokens,
                      int32_t* accepted, void* stream);

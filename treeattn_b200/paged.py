@@ -1,10 +1,12 @@
 """Serving over an 8-bit paged key / value cache: the cache, appending to it with the position rotation, attention over
-it for one or several new tokens of each sequence, and the verification of drafted tokens.
+it for one or several new tokens of each sequence, copies of its pages and sequences, and the verification of drafted tokens.
 
 The reference's engine keeps one fp32 tensor per sequence and decodes one token at a time (engine.py:74-81, 149-177); these
 operators are the dense model's side of speculative decoding: the segment-tree Decoder drafts, the dense model verifies
 (speculative.py runs the two together). Like every entry point of this package they take CUDA tensors, check them, and
 enqueue on the current stream without synchronising."""
+import array
+import ctypes
 import math
 
 import torch
@@ -89,35 +91,110 @@ class PagedKV:
 
 class PagePool:
     """Which pages of a pool are free, and the table of those that are not: host bookkeeping for a batch of sequences. The
-    device table is updated by one small copy when a sequence gets new pages."""
+    device table is updated by one small copy when a sequence's pages change.
+
+    Full pages may be shared: fork lets a sequence go on from another's positions. refs[p] counts the sequences that hold page p."""
 
     def __init__(self, n_pages, batch, max_pages, page, device='cuda'):
         self.page, self.n_pages, self.max_pages = int(page), int(n_pages), int(max_pages)
         self.free = list(range(n_pages - 1, -1, -1))
+        self.refs = [0] * self.n_pages
         self.owned = [[] for _ in range(batch)]
         self.host = torch.zeros(batch, max_pages, dtype=torch.int32)
         self.table = torch.zeros(batch, max_pages, device=device, dtype=torch.int32)
 
-    def reserve(self, lengths):
-        """Makes room for lengths[b] positions of each sequence b (a list; shorter ones keep what they have). Raises
+    def _take(self, b, at):
+        page = self.free.pop()
+        self.refs[page] = 1
+        self.host[b, at] = page
+        return page
+
+    def _drop(self, pages):
+        for p in reversed(pages):
+            self.refs[p] -= 1
+            if not self.refs[p]:
+                self.free.append(p)
+
+    def reserve(self, lengths, pos=None):
+        """Makes room for lengths[b] positions of each sequence b (a list; shorter ones keep what they have). pos: the position
+        that each sequence will write next. From its page on the sequence gets pages of its own where it shares them (what a page
+        that is not full holds is in the tail, so nothing is copied); needed where sequences are forked and cut back. Raises
         MemoryError, with nothing changed, when the pool has too few free pages."""
         need = [max(0, -(-int(n) // self.page) - len(o)) for n, o in zip(lengths, self.owned)]
         for n, k in zip(lengths, need):
             if -(-int(n) // self.page) > self.max_pages:
                 raise ValueError('PagePool: %d positions above the %d of a sequence' % (n, self.max_pages * self.page))
-        if sum(need) > len(self.free):
-            raise MemoryError('PagePool: %d pages wanted, %d free' % (sum(need), len(self.free)))
+        shared, left = [], {}
+        for b, at in enumerate(pos or ()):
+            own = self.owned[b]
+            for j in range(int(at) // self.page, len(own)):
+                n = left.get(own[j], self.refs[own[j]])
+                if n > 1:  # the last holder of a page keeps it
+                    left[own[j]] = n - 1
+                    shared.append((b, j))
+        if sum(need) + len(shared) > len(self.free):
+            raise MemoryError('PagePool: %d pages wanted, %d free' % (sum(need) + len(shared), len(self.free)))
+        for b, j in shared:
+            self.refs[self.owned[b][j]] -= 1
+            self.owned[b][j] = self._take(b, j)
         for b, k in enumerate(need):
             for _ in range(k):
-                self.host[b, len(self.owned[b])] = self.free[-1]
-                self.owned[b].append(self.free.pop())
-        if any(need):
+                self.owned[b].append(self._take(b, len(self.owned[b])))
+        if shared or any(need):
             self.table.copy_(self.host)
 
     def release(self, b):
-        """Gives sequence b's pages back."""
-        self.free.extend(reversed(self.owned[b]))
+        """Gives sequence b's pages back (those that no other sequence holds become free)."""
+        self._drop(self.owned[b])
         self.owned[b] = []
+
+    def fork(self, src, dst, lengths):
+        """Sequence dst[i] goes on from the first lengths[i] positions of sequence src[i], for all i at once (a sequence may be a
+        source and a destination): it shares the full pages among them, and what dst[i] held is given back. The open pages, which
+        live in the caches' tails, are paged_fork's to copy."""
+        B = len(self.owned)
+        if not len(src) == len(dst) == len(lengths):
+            raise ValueError('PagePool.fork: %d sources, %d destinations, %d lengths' % (len(src), len(dst), len(lengths)))
+        if any(not 0 <= int(b) < B for b in (*src, *dst)) or len(set(dst)) != len(dst):
+            raise ValueError('PagePool.fork: sequences in [0, %d), each a destination once' % B)
+        new = {}
+        for s, d, n in zip(src, dst, lengths):
+            full = int(n) // self.page
+            if n < 0 or full > len(self.owned[s]):
+                raise ValueError('PagePool.fork: sequence %d does not hold %d positions' % (s, n))
+            if s != d:
+                new[d] = self.owned[s][:full]
+        for pages in new.values():
+            for p in pages:
+                self.refs[p] += 1
+        for d, pages in new.items():
+            self._drop(self.owned[d])
+            self.owned[d] = pages
+            self.host[d, :len(pages)] = torch.tensor(pages, dtype=torch.int32)
+        if new:
+            self.table.copy_(self.host)
+
+    def compact(self, n_pages=None):
+        """Shrinks the pool to its first n_pages pages (default: as many as are held): returns (src, dst), the pages to move, for
+        paged_copy on every cache of the pool before anything else touches them. Raises MemoryError, with nothing changed, when
+        more pages than that are held."""
+        held = self.n_pages - len(self.free)
+        n_pages = max(held, 1) if n_pages is None else int(n_pages)
+        if not max(held, 1) <= n_pages <= self.n_pages:
+            raise MemoryError('PagePool: %d pages held, of %d, cannot become %d' % (held, self.n_pages, n_pages))
+        src = [p for p in range(n_pages, self.n_pages) if self.refs[p]]
+        free = sorted((p for p in self.free if p < n_pages), reverse=True)
+        dst = [free.pop() for _ in src]
+        to = dict(zip(src, dst))
+        for s, d in to.items():
+            self.refs[d] = self.refs[s]
+        for b, own in enumerate(self.owned):
+            own[:] = [to.get(p, p) for p in own]
+            self.host[b] = 0  # (a row's places beyond its pages may name pages that are gone)
+            self.host[b, :len(own)] = torch.tensor(own, dtype=torch.int32)
+        self.refs, self.free, self.n_pages = self.refs[:n_pages], free, n_pages
+        self.table.copy_(self.host)
+        return src, dst
 
 
 def rotation_table(n_pos, rot, base=10000.0, device='cuda'):
@@ -145,6 +222,24 @@ def _call(name, *args):
 
 def _stream(t):
     return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
+class _Here:
+    """Nothing to do: the tensors' device is the current one."""
+
+    def __enter__(self):
+        pass
+
+    def __exit__(self, *e):
+        pass
+
+
+_here = _Here()
+
+
+def _on(t):
+    """Makes t's device the current one for a call, where it is not."""
+    return _here if t.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
 
 
 def _rows(name, cache, start, pos):
@@ -219,6 +314,44 @@ def paged_append(cache, k, v, start, pos, max_new, q=None, rotation=None, q_out=
           cache.page, _DT[dt], B, H, dh, k.data_ptr(), v.data_ptr(), ks[0], ks[1], vs[0], vs[1], n, start.data_ptr(),
           pos.data_ptr(), max_new, cos, sin, n_pos, rot, qp, Hq, qr, qh, qo, _stream(k))
     return q_out
+
+
+def _records(name, caches, src, dst, of, per_record):
+    """One ta_record_copy over the caches' buffers; src and dst are whole numbers on the host."""
+    bufs = [of(c) for c in caches]
+    if not bufs:
+        raise ValueError('%s: no caches' % name)
+    first = bufs[0]
+    if any(b.shape != first.shape or b.dtype is not first.dtype or b.device != first.device for b in bufs):
+        raise ValueError('%s: the caches must be alike, and on one device' % name)
+    src, dst = [x.tolist() if torch.is_tensor(x) or hasattr(x, 'tolist') else x for x in (src, dst)]
+    if len(src) != len(dst):
+        raise ValueError('%s: %d sources, %d destinations' % (name, len(src), len(dst)))
+    if not len(src):
+        return
+    try:
+        moves = array.array('i', src), array.array('i', dst)
+    except (TypeError, OverflowError):
+        raise ValueError('%s: sources and destinations must be whole numbers of 32 bits' % name) from None
+    _need_cuda(name, first)
+    ptrs = (ctypes.c_void_p * len(bufs))(*[b.data_ptr() for b in bufs])
+    with _on(first):
+        _call('ta_record_copy', ptrs, len(bufs), per_record(first), first.shape[0], moves[0].buffer_info()[0],
+              moves[1].buffer_info()[0], len(src), _stream(first))
+
+
+def paged_copy(caches, src, dst):
+    """Copies page src[i] of the pool to page dst[i], for all i at once (every page is read before any is written: chains and cycles
+    of pages are fine; no page is written twice), in all caches (PagedKV of one shape, one per layer) by one launch. src and dst
+    are whole numbers on the host (lists, PagePool.compact's): a captured call repeats the same moves."""
+    _records('paged_copy', caches, src, dst, lambda c: c.pool, lambda t: t.shape[1] * t.shape[2])
+
+
+def paged_fork(caches, src, dst):
+    """Copies what sequence src[i] holds in 16 bits, its open page and the one before it, to sequence dst[i], for all i at once, in all
+    caches: what PagePool.fork leaves to do when a sequence goes on in another's slot (samples of one prompt, beams). src and
+    dst as paged_copy's."""
+    _records('paged_fork', caches, src, dst, lambda c: c.tail, lambda t: t.shape[1] * t.shape[2] * t.shape[3] * t.shape[4] * 2)
 
 
 def _workspace_bytes(batch, n_head, n_kv_head, head_dim, max_new):

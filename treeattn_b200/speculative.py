@@ -7,7 +7,8 @@ model's own sampling."""
 import torch
 
 from . import _ops
-from .paged import PagedKV, PagePool, _workspace_bytes, paged_append, paged_attn, paged_attn_workspace, verify_drafts
+from .paged import (PagedKV, PagePool, _workspace_bytes, paged_append, paged_attn, paged_attn_workspace, paged_copy, paged_fork,
+                    verify_drafts)
 
 
 class PagedDecoder:
@@ -77,7 +78,7 @@ class PagedDecoder:
             raise ValueError('PagedDecoder: %d sequences for a batch of %d' % (B, self.batch))
         if max(self.pos) + n > self.max_len:
             raise ValueError('PagedDecoder: position %d above max_len %d' % (max(self.pos) + n, self.max_len))
-        self.pool.reserve([p + n for p in self.pos])
+        self.pool.reserve([p + n for p in self.pos], self.pos)
         start, ws = self._plan(n)
         pos = torch.tensor(self.pos, dtype=torch.int32).to(self.dev, non_blocking=True)
         at = (pos[:, None] + torch.arange(n, device=self.dev, dtype=torch.int32)).reshape(-1)
@@ -107,6 +108,28 @@ class PagedDecoder:
             if not max(0, self._floor[b]) <= new <= old:
                 raise ValueError('PagedDecoder: sequence %d cannot go from %d back to %d positions' % (b, old, new))
         self.pos = list(pos)
+
+    def fork(self, src, dst):
+        """Sequence dst[i] goes on from where sequence src[i] is, for all i at once: a prompt into a group of samples, beams that take
+        over one another's slots. Full pages are shared; the open ones are copied. What dst[i] held is dropped."""
+        self.pool.fork(src, dst, [self.pos[s] if 0 <= s < self.batch else 0 for s in src])
+        paged_fork(self.caches, src, dst)
+        was = self.pos, self._floor
+        self.pos, self._floor = list(self.pos), list(self._floor)
+        for s, d in zip(src, dst):
+            self.pos[d], self._floor[d] = was[0][s], was[1][s]
+
+    def release(self, b):
+        """Empties sequence b and gives its pages back."""
+        self.pool.release(b)
+        self.pos[b] = self._floor[b] = 0
+
+    def compact(self, n_pages=None):
+        """Shrinks the pool to n_pages pages (default: as many as are held) and gives the rest of its memory back."""
+        paged_copy(self.caches, *self.pool.compact(n_pages))
+        for i, c in enumerate(self.caches):
+            pool = c.pool[:self.pool.n_pages].clone()
+            self.caches[i] = PagedKV(pool, c.tail, c.table, c.page, c.head_dim)
 
 
 class SpeculativeDecoder:
