@@ -413,6 +413,27 @@ int ta_paged_attn_probe(int worker, const void* pool, const void* tail, const in
  *   layer) and the sequences of a tail are such records. */
 int ta_record_copy(void* const* bufs, int n_bufs, int64_t record_bytes, int n_records, const int32_t* src,
                    const int32_t* dst, int n, void* stream);
+/* Losses over a vocabulary's logits (no counterpart in the reference, which trains on cross entropy). Row (b, t) of logits (B, T, V)
+ * in `dtype` starts at b * z_sb + t * z_st (unit inner stride, no alignment needed); tokens int64 by (b, t). With z = logits /
+ * temperature: logp = z_y - log sum exp z. A row whose token is outside [0, V) gives NaN and is recorded.
+ * ta_token_logp: logp (B, T) fp32, contiguous; stats (2, B, T) fp32: the rows' maxima (of the logits) and sums exp(z - max).
+ * ta_policy_loss: rho = exp(logp - old); term = -min(rho A, min(max(rho, lo), hi) A) + kl (exp(ref - logp) - (ref - logp) - 1);
+ *   *loss = sum of w term (in 64 bits, one order). by_row: HOST array of the four fp32 tensors old, A, ref (read where kl != 0), w
+ *   (NULL: weight0), by_row_strides their (b, t) strides, eight numbers. A row of w = 0 does not count, whatever it holds: logp 0.
+ *   stats (4, B, T): as above, then slope = dloss / dlogp / temperature (0 where not counted), then w term. grad: NULL, or the gradient
+ *   of the logits, slope ([j = y] - softmax_j), rows at b * g_sb + t * g_st; rows of slope 0 get zeros.
+ * ta_logits_grad: that gradient from saved stats, with slope (b, t) (any strides) times slope_by times *up (device; NULL: 1). unit_done:
+ *   grad already holds it for *up = 1, and is left as it is then. */
+int ta_token_logp(const void* logits, int dtype, int64_t z_sb, int64_t z_st, int B, int T, int V, const int64_t* tokens,
+                  int64_t t_sb, int64_t t_st, float temperature, float* logp, float* stats, void* stream);
+int ta_policy_loss(const void* logits, int dtype, int64_t z_sb, int64_t z_st, int B, int T, int V, const int64_t* tokens,
+                   int64_t t_sb, int64_t t_st, const float* const* by_row, const int64_t* by_row_strides, float weight0,
+                   float lo, float hi, float kl, float temperature, float* loss, float* logp, float* stats, void* grad,
+                   int64_t g_sb, int64_t g_st, void* stream);
+int ta_logits_grad(const void* logits, int dtype, int64_t z_sb, int64_t z_st, int B, int T, int V, const int64_t* tokens,
+                   int64_t t_sb, int64_t t_st, const float* stats, const float* slope, int64_t s_sb, int64_t s_st,
+                   float slope_by, float temperature, const float* up, int unit_done, void* grad, int64_t g_sb,
+                   int64_t g_st, void* stream);
 int ta_verify_drafts(const void* p, int64_t p_sb, int64_t p_sr, const void* q, int64_t q_sb, int64_t q_sr, int dtype, int B,
                      int G, int V, const int64_t* drafts, const float* u, const int32_t* n, int64_t* tokens,
                      int32_t* accepted, void* stream);

@@ -69,6 +69,9 @@ SIGNATURES = {
     'ta_paged_attn': [P, P, P, L, I, I, I, I, I, I, I, I, P, L, L, I, P, P, I, F, I, P, L, L, P, P, L, P],
     'ta_paged_attn_probe': [I, P, P, P, L, I, I, I, I, I, I, I, I, P, L, L, I, P, P, I, F, I, P, L, L, P, P, L, P],
     'ta_record_copy': [P, I, L, I, P, P, I, P],
+    'ta_token_logp': [P, I, L, L, I, I, I, P, L, L, F, P, P, P],
+    'ta_policy_loss': [P, I, L, L, I, I, I, P, L, L, P, P, F, F, F, F, F, P, P, P, P, L, L, P],
+    'ta_logits_grad': [P, I, L, L, I, I, I, P, L, L, P, P, L, L, F, F, P, I, P, L, L, P],
     'ta_verify_drafts': [P, L, L, P, L, L, I, I, I, I, P, P, P, P, P, P],
     'ta_block_tail': [P, P, P, P, P, P, P, P, F, I, I, I, P, P, P, L, P, P],
 }

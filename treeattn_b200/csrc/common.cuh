@@ -54,6 +54,8 @@ enum KernelId : int {
   K_PAGED_APPEND = 16,
   K_PAGED_ATTN = 17,
   K_VERIFY = 18,
+  K_LOSS = 19,
+  K_ADAPTER = 20,
 };
 
 // ------------------------------------------------------------------------------------------------ types

@@ -26,7 +26,8 @@
 #include "prefill.cuh"
 
 namespace ta_host {
-cudaError_t paged_device_error(int* out4);  // the error record of paged.cu, read and cleared
+cudaError_t paged_device_error(int* out4);   // the error records of paged.cu and losses.cu, read and cleared
+cudaError_t losses_device_error(int* out4);
 }
 
 namespace {
@@ -957,6 +958,7 @@ int ta_device_error(int* out4) {
   if (e != cudaSuccess) return fail(TA_ERR_CUDA, "ta_device_error: %s", cudaGetErrorString(e));
   if (out4[0] == 0) {  // (an error of the serving kernels stays on record until the others' has been read)
     e = ta_host::paged_device_error(out4);
+    if (e == cudaSuccess && out4[0] == 0) e = ta_host::losses_device_error(out4);
   } else {
     const int zero[4] = {0, 0, 0, 0};
     e = cudaMemcpyToSymbol(ta::g_dev_err, zero, 4 * sizeof(int));
