@@ -72,6 +72,8 @@ SIGNATURES = {
     'ta_token_logp': [P, I, L, L, I, I, I, P, L, L, F, P, P, P],
     'ta_policy_loss': [P, I, L, L, I, I, I, P, L, L, P, P, F, F, F, F, F, P, P, P, P, L, L, P],
     'ta_logits_grad': [P, I, L, L, I, I, I, P, L, L, P, P, L, L, F, F, P, I, P, L, L, P],
+    'ta_adapter_add': [P, L, P, L, P, P, P, I, I, I, I, I, I, P, P, I, I, P, L, P, P],
+    'ta_adapter_bwd': [P, L, P, L, P, P, P, I, I, I, I, I, P, P, I, I, P, P, P, L, P, P, P],
     'ta_verify_drafts': [P, L, L, P, L, L, I, I, I, I, P, P, P, P, P, P],
     'ta_block_tail': [P, P, P, P, P, P, P, P, F, I, I, I, P, P, P, L, P, P],
 }

@@ -26,8 +26,9 @@
 #include "prefill.cuh"
 
 namespace ta_host {
-cudaError_t paged_device_error(int* out4);   // the error records of paged.cu and losses.cu, read and cleared
+cudaError_t paged_device_error(int* out4);   // the error records of the other translation units, read and cleared
 cudaError_t losses_device_error(int* out4);
+cudaError_t adapters_device_error(int* out4);
 }
 
 namespace {
@@ -959,6 +960,7 @@ int ta_device_error(int* out4) {
   if (out4[0] == 0) {  // (an error of the serving kernels stays on record until the others' has been read)
     e = ta_host::paged_device_error(out4);
     if (e == cudaSuccess && out4[0] == 0) e = ta_host::losses_device_error(out4);
+    if (e == cudaSuccess && out4[0] == 0) e = ta_host::adapters_device_error(out4);
   } else {
     const int zero[4] = {0, 0, 0, 0};
     e = cudaMemcpyToSymbol(ta::g_dev_err, zero, 4 * sizeof(int));

@@ -17,11 +17,11 @@ class PagedDecoder:
 
     W: a decoder weight dict (engine.weights_from_ours / weights_from_nanogpt). max_len: positions of a sequence (at most the
     model's position table). n_pages: pages of the pool, shared by the layers' tables (default: enough for every sequence at
-    max_len). rotation: (cos, sin) of paged.rotation_table for models that rotate their keys and queries.
+    max_len). adapters: an adapters.AdapterSet; `which` then holds each sequence's adapter (-1: none; set_adapter changes it). rotation: (cos, sin) of paged.rotation_table for models that rotate their keys and queries.
     max_new: new tokens of a sequence in a call that the workspace is made for (it grows where a call has more)."""
 
     def __init__(self, W, n_layer, n_head, n_embd, batch=1, max_len=None, page=64, n_pages=None, dtype=torch.bfloat16,
-                 dev='cuda', rotation=None, max_new=8):
+                 dev='cuda', rotation=None, max_new=8, adapters=None):
         if dtype not in (torch.bfloat16, torch.float16):
             raise TypeError('PagedDecoder: bfloat16 or float16 (got %s)' % dtype)
         self.dev, self.dtype, self.rotation = torch.device(dev), dtype, rotation
@@ -40,6 +40,13 @@ class PagedDecoder:
         per_seq = -(-self.max_len // page)
         self.pool = PagePool(n_pages or batch * per_seq, batch, per_seq, page, self.dev)
         self.caches = [PagedKV.empty(self.pool.n_pages, n_head, self.dh, self.pool.table, page, dtype) for _ in range(n_layer)]
+        if adapters is not None and (adapters.n_layer < n_layer or adapters.n_embd != n_embd or adapters.scale.device != self.pool.table.device):
+            raise ValueError('PagedDecoder: adapters of %d blocks of width %d on %s for %d of %d on %s' % (
+                adapters.n_layer, adapters.n_embd, adapters.scale.device, n_layer, n_embd, self.pool.table.device))
+        if adapters is not None and adapters.a[0].dtype is not dtype:
+            raise TypeError('PagedDecoder: %s adapters for a %s model' % (adapters.a[0].dtype, dtype))
+        self.adapters = adapters
+        self.which = torch.full((batch,), -1, device=self.dev, dtype=torch.int32)
         self.pos = [0] * batch     # positions that each sequence holds
         self._floor = [0] * batch  # and how far back it can be cut: the start of the page before the furthest one written
         self._start = {}
@@ -61,6 +68,12 @@ class PagedDecoder:
             self._start[n] = torch.arange(self.batch + 1, device=self.dev, dtype=torch.int32) * n
             self._grow(n)
         return self._start[n], self._ws
+
+    def set_adapter(self, b, adapter):
+        """The adapter of sequence b from its next token on (-1: none); a fork takes its source's."""
+        if self.adapters is None or not 0 <= b < self.batch or not -1 <= adapter < self.adapters.n_adapters:
+            raise ValueError('PagedDecoder: sequence %d cannot take adapter %d' % (b, adapter))
+        self.which[b] = adapter
 
     def reset(self):
         """Empties every sequence and gives its pages back."""
@@ -86,14 +99,18 @@ class PagedDecoder:
         x = torch.empty(N, C, device=self.dev, dtype=torch.float32)
         h = torch.empty(N, C, device=self.dev, dtype=self.dtype)
         _ops.embed_ln(W['wte'], W['wpe'], tok.reshape(-1).contiguous(), at, W['layers'][0]['ln1'], x, h)
+        add = lambda y, x, i, name: y
+        if self.adapters is not None:
+            add = lambda y, x, i, name: self.adapters.apply_to(y, x, i, name, start, self.which, n)
         for i, L in enumerate(W['layers']):
-            qkv = h @ L['c_attn'].t()
+            qkv = add(h @ L['c_attn'].t(), h, i, 'c_attn')
             q, k, v = [qkv[:, j * C:(j + 1) * C].view(N, H, dh) for j in range(3)]
             q = paged_append(self.caches[i], k, v, start, pos, n, q=q, rotation=self.rotation)
             att = paged_attn(self.caches[i], q, start, pos, n, ws=ws)
-            _ops.add_ln(x, att.view(N, C) @ L['c_proj'].t(), L['ln2'], h)
-            f = _ops.gelu_(h @ L['c_fc'].t())
-            _ops.add_ln(x, f @ L['c_mlp'].t(), W['layers'][i + 1]['ln1'] if i + 1 < len(W['layers']) else W['ln_f'], h)
+            att = att.view(N, C)
+            _ops.add_ln(x, add(att @ L['c_proj'].t(), att, i, 'c_proj'), L['ln2'], h)
+            f = _ops.gelu_(add(h @ L['c_fc'].t(), h, i, 'c_fc'))
+            _ops.add_ln(x, add(f @ L['c_mlp'].t(), f, i, 'c_mlp'), W['layers'][i + 1]['ln1'] if i + 1 < len(W['layers']) else W['ln_f'], h)
         self.pos = [p + n for p in self.pos]
         page = self.pool.page
         self._floor = [max(f, ((p - 1) // page - 1) * page) for f, p in zip(self._floor, self.pos)]
@@ -114,6 +131,9 @@ class PagedDecoder:
         over one another's slots. Full pages are shared; the open ones are copied. What dst[i] held is dropped."""
         self.pool.fork(src, dst, [self.pos[s] if 0 <= s < self.batch else 0 for s in src])
         paged_fork(self.caches, src, dst)
+        if self.adapters is not None and len(src):
+            at = torch.tensor([list(src), list(dst)]).to(self.dev)
+            self.which[at[1]] = self.which[at[0]]
         was = self.pos, self._floor
         self.pos, self._floor = list(self.pos), list(self._floor)
         for s, d in zip(src, dst):
