@@ -80,7 +80,7 @@ def _check(logits, tokens, old, adv, ref, weight, clip, kl, tau, up=None):
 
 @pytest.mark.parametrize('dtype', ['f32', 'bf16', 'f16'])
 @pytest.mark.parametrize('B,T,V', [(1, 1, 1), (2, 3, 2), (1, 5, 7), (3, 2, 8), (2, 2, 9), (1, 37, 1000), (5, 7, 4099), (2, 9, 16384),
-                                   (3, 3, 50257), (1, 2, 131072), (2, 200, 2051), (1, 3, 300001)])
+                                   (3, 3, 50257), (1, 2, 131072), (2, 200, 2051), (1, 3, 262143)])
 def test_policy_loss(B, T, V, dtype):
     args = _inputs(B, T, V, dtype, seed=V)
     _check(*args, clip=(0.2, 0.28), kl=0.05, tau=1.0)
@@ -224,7 +224,7 @@ def test_gradient_against_differences():
 
 
 @pytest.mark.parametrize('dtype', ['f32', 'bf16', 'f16'])
-@pytest.mark.parametrize('B,T,V', [(1, 1, 1), (2, 3, 9), (1, 40, 1001), (3, 2, 50257), (1, 1, 299999)])
+@pytest.mark.parametrize('B,T,V', [(1, 1, 1), (2, 3, 9), (1, 40, 1001), (3, 2, 50257), (1, 1, 262144)])
 def test_token_logp(B, T, V, dtype):
     from treeattn_b200.losses import token_logp
     logits, tokens, *_ = _inputs(B, T, V, dtype, seed=V + 1)

@@ -23,24 +23,24 @@ namespace {
 
 using namespace ta_host;
 
-constexpr int MAX_V = 400000;             // a cluster of 8 holds a row of fp32
-constexpr int TWO_PER_SM = 104 * 1024;    // bytes of a row in a CTA's shared memory, with two CTAs on an SM
+constexpr int MAX_ROW = 1 << 20;          // bytes: a cluster of 8 holds a row
+constexpr int TWO_PER_SM = 108 * 1024;    // bytes of a row in a CTA's shared memory, with two CTAs on an SM
 
 int check_rows(const char* who, const void* z, int dtype, int B, int T, int V, const int64_t* tokens, float tau) {
   if (!valid_dtype(dtype)) return fail(TA_ERR_ARG, "%s: bad dtype %d", who, dtype);
-  if (B < 0 || T < 0 || V < 1 || V > MAX_V || (int64_t)B * T > (1 << 27))
-    return fail(TA_ERR_ARG, "%s: bad sizes B=%d T=%d V=%d (at most %d words, 2^27 rows)", who, B, T, V, MAX_V);
+  if (B < 0 || T < 0 || V < 1 || V > MAX_ROW / esize_of(dtype) || (int64_t)B * T > (1 << 27))
+    return fail(TA_ERR_ARG, "%s: bad sizes B=%d T=%d V=%d (rows of at most %d bytes, 2^27 of them)", who, B, T, V, MAX_ROW);
   if (!(tau > 0.f) || !std::isfinite(tau) || !std::isfinite(1.f / tau))
     return fail(TA_ERR_ARG, "%s: temperature %g (positive and finite)", who, tau);
   if ((int64_t)B * T > 0 && (!z || !tokens)) return fail(TA_ERR_ARG, "%s: null pointer", who);
   return TA_OK;
 }
 
-template <typename T, int THREADS, bool POLICY>
+template <typename T, int THREADS, int MODE, bool ALIGNED>
 int launch_loss(const ta::LossParams& a, int cs, cudaStream_t st, const char* who) {
   static SmemAttr attr;
   const size_t smem = (size_t)a.per * 16;
-  if (int r = allow_smem(attr, ta::loss_kernel<T, THREADS, POLICY>, smem, who)) return r;
+  if (int r = allow_smem(attr, ta::loss_kernel<T, THREADS, MODE, ALIGNED>, smem, who)) return r;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((int64_t)a.B * a.T * cs));
   cfg.blockDim = dim3(THREADS);
@@ -54,28 +54,37 @@ int launch_loss(const ta::LossParams& a, int cs, cudaStream_t st, const char* wh
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 2;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, ta::loss_kernel<T, THREADS, POLICY>, a);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, ta::loss_kernel<T, THREADS, MODE, ALIGNED>, a);
   if (e != cudaSuccess) return fail(TA_ERR_CUDA, "%s: launch failed: %s", who, cudaGetErrorString(e));
   return TA_OK;
 }
 
-template <typename T, bool POLICY>
+template <typename T, int MODE>
 int run_loss(ta::LossParams& a, cudaStream_t st, const char* who) {
-  const int64_t rows = (int64_t)a.B * a.T, bytes = (int64_t)a.V * sizeof(T) + 16;
+  constexpr int N = 16 / (int)sizeof(T);
+  const int64_t rows = (int64_t)a.B * a.T;
+  const int pieces = (a.V + 2 * N - 2) / N;  // at most, wherever the row begins
   // CTAs of a row: as few as leave room for two on an SM, more where the rows do not fill the GPU
   int cs = 1;
-  while (cs < 8 && (bytes / cs > TWO_PER_SM || (rows * cs < 2 * sm_count() && bytes / (2 * cs) >= 8192))) cs *= 2;
-  a.per = (int)((bytes + 15) / 16 + cs - 1) / cs;
-  if (a.per * 16 < 24 * 1024) return launch_loss<T, 128, POLICY>(a, cs, st, who);
-  return launch_loss<T, 512, POLICY>(a, cs, st, who);
+  while (cs < 8 && ((int64_t)pieces * 16 > (int64_t)cs * TWO_PER_SM || (rows * cs < 2 * sm_count() && pieces * 16 >= 2 * cs * 8192)))
+    cs *= 2;
+  a.per = (pieces + cs - 1) / cs;
+  const bool aligned = a.V % N == 0 && rows_aligned(a.z, sizeof(T), {a.z_sb, a.z_st}) &&
+                       (MODE < 2 || rows_aligned(a.grad, sizeof(T), {a.g_sb, a.g_st}));
+  if (a.per * 16 < 24 * 1024) {
+    if (aligned) return launch_loss<T, 128, MODE, true>(a, cs, st, who);
+    return launch_loss<T, 128, MODE, false>(a, cs, st, who);
+  }
+  if (aligned) return launch_loss<T, 512, MODE, true>(a, cs, st, who);
+  return launch_loss<T, 512, MODE, false>(a, cs, st, who);
 }
 
-template <bool POLICY>
+template <int MODE>
 int by_type(ta::LossParams& a, int dtype, cudaStream_t st, const char* who) {
   switch (dtype) {
-    case TA_F32: return run_loss<float, POLICY>(a, st, who);
-    case TA_BF16: return run_loss<__nv_bfloat16, POLICY>(a, st, who);
-    default: return run_loss<__half, POLICY>(a, st, who);
+    case TA_F32: return run_loss<float, MODE>(a, st, who);
+    case TA_BF16: return run_loss<__nv_bfloat16, MODE>(a, st, who);
+    default: return run_loss<__half, MODE>(a, st, who);
   }
 }
 
@@ -97,7 +106,7 @@ int ta_token_logp(const void* logits, int dtype, int64_t z_sb, int64_t z_st, int
   a.tokens = tokens; a.t_sb = t_sb; a.t_st = t_st;
   a.inv_tau = 1.f / temperature;
   a.logp = logp; a.top = stats; a.tot = stats + rows;
-  return by_type<false>(a, dtype, S(stream), who);
+  return by_type<0>(a, dtype, S(stream), who);
 }
 
 int ta_policy_loss(const void* logits, int dtype, int64_t z_sb, int64_t z_st, int B, int T, int V, const int64_t* tokens,
@@ -124,7 +133,7 @@ int ta_policy_loss(const void* logits, int dtype, int64_t z_sb, int64_t z_st, in
     a.w0 = weight0; a.lo = lo; a.hi = hi; a.kl = kl; a.inv_tau = 1.f / temperature;
     a.logp = logp; a.top = stats; a.tot = stats + rows; a.slope = stats + 2 * rows; a.term = stats + 3 * rows;
     a.grad = grad; a.g_sb = g_sb; a.g_st = g_st;
-    if (int r = by_type<true>(a, dtype, st, who)) return r;
+    if (int r = grad ? by_type<2>(a, dtype, st, who) : by_type<1>(a, dtype, st, who)) return r;
   }
   const cudaError_t e = launch_pdl(ta::loss_sum_kernel, dim3(1), dim3(1024), 0, st, (const float*)stats + 3 * rows, rows, loss);
   if (e != cudaSuccess) return fail(TA_ERR_CUDA, "%s: launch failed: %s", who, cudaGetErrorString(e));
@@ -153,6 +162,8 @@ int ta_logits_grad(const void* logits, int dtype, int64_t z_sb, int64_t z_st, in
   const int per = ta::GRAD_PIECES * 16 / esize_of(dtype);  // elements of a CTA's piece of a row
   a.chunks = (V + 16 / esize_of(dtype) + per - 1) / per;
   const int64_t items = rows * a.chunks;
+  if (items > UINT32_MAX / 2) return fail(TA_ERR_ARG, "%s: too many rows of %d words", who, V);
+  a.items = (uint32_t)items;
   const unsigned grid = (unsigned)std::min<int64_t>(items, (int64_t)sm_count() * 8);
   cudaError_t e;
   const cudaStream_t st = S(stream);

@@ -3,10 +3,12 @@
 //   term = -min(rho A, clip(rho, lo, hi) A) + kl (exp(ref - logp) - (ref - logp) - 1),  loss = sum over rows of w term
 //   slope = dloss / dlogp = w (-A rho [not clipped] + kl (1 - exp(ref - logp))),  dloss / dz_j = slope / tau ([j = y] - p_j)
 // Everything about a row but its softmax is a handful of scalars, so the gradient's factor is known as soon as the row's sum is: a
-// row is read once, stays in shared memory, and its gradient is written from there. The floor is one read and one write of the
+// row is read once, its exponentials stay in registers, and the gradient is written from there. The floor is one read and one write of the
 // logits; a gradient that waits for the backward pass (16-bit floats of 5 exponent bits, which need the loss's scale
 // before they are rounded) reads them twice.
 #pragma once
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace ta {
@@ -32,7 +34,7 @@ struct LossParams {
   int64_t g_sb, g_st;
 };
 
-constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 // The two elements of a word of a 16-byte piece, as fp32; a piece of fp32 has one a word.
 template <typename T> struct Piece;
@@ -94,30 +96,41 @@ __device__ __forceinline__ float exp2_fast(float x) {  // 2 ulp; 0 at -inf, NaN 
   return y;
 }
 
-// exp2((z - top) k) of a piece's elements, two at a time (packed arithmetic). The difference comes first: z k - top k, one operation, is off by
-// a step of top k in every element alike, and overflows where k tops the range.
-template <int N>
-__device__ __forceinline__ void exp_piece(float (&z)[N], float top, float k) {
-  uint64_t t2, k2;
-  asm("mov.b64 %0, {%1, %1};" : "=l"(t2) : "f"(-top));
-  asm("mov.b64 %0, {%1, %1};" : "=l"(k2) : "f"(k));
-#pragma unroll
-  for (int i = 0; i < N; i += 2) {
-    uint64_t x;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(z[i]), "f"(z[i + 1]));
-    asm("add.rn.f32x2 %0, %0, %1;" : "+l"(x) : "l"(t2));
-    asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(x) : "l"(k2));
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(z[i]), "=f"(z[i + 1]) : "l"(x));
-    z[i] = exp2_fast(z[i]);
-    z[i + 1] = exp2_fast(z[i + 1]);
+// A reference logit m that exponentials are taken about: exp2(z k - m k), one operation and the exponential. The product m k is rounded, which
+// puts one factor on all of a reference's exponentials: sums, logits and other references are compared with the same rounded product,
+// and it cancels. Where the products come near the range's end the difference is taken first.
+struct Ref {
+  float m, off;
+  bool far;
+  __device__ __forceinline__ Ref(float m_, float k) : m(m_), off(-m_ * k), far(!(fabsf(off) < 1e30f)) {}
+  __device__ __forceinline__ float of(float z, float k) const { return far ? (z - m) * k : fmaf(z, k, off); }
+  // what a sum about o is multiplied by to be one about this
+  __device__ __forceinline__ float from(const Ref& o, float k) const {
+    return exp2_fast(far || o.far ? (o.m - m) * k : off - o.off);
   }
-}
+};
 
 __device__ __forceinline__ uint4 load_once(const uint4* p) {
   uint4 v;
   asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
   return v;
+}
+
+// The element at a time forms of a piece that reaches beyond its row (elements [0, V) of it; the piece's first is `at`): -inf there.
+template <typename T>
+__device__ __noinline__ uint4 load_edge(const T* row, int at, int V) {
+  uint4 v = make_uint4(Piece<T>::lowest(), Piece<T>::lowest(), Piece<T>::lowest(), Piece<T>::lowest());
+  T* e = reinterpret_cast<T*>(&v);
+  for (int i = 0; i < Piece<T>::N; ++i)
+    if (at + i >= 0 && at + i < V) e[i] = row[at + i];
+  return v;
+}
+template <typename T>
+__device__ __noinline__ void store_edge(T* row, int at, int V, uint4 v) {
+  const T* e = reinterpret_cast<const T*>(&v);
+  for (int i = 0; i < Piece<T>::N; ++i)
+    if (at + i >= 0 && at + i < V) row[at + i] = e[i];
 }
 
 // A row in 16-byte pieces from the boundary before its first element on: piece j holds elements [j N - lead, (j + 1) N - lead).
@@ -127,117 +140,107 @@ struct RowPieces {
   static constexpr int N = Piece<T>::N;
   const T* row;
   int lead, V, pieces;
-  __device__ __forceinline__ RowPieces(const T* r, int v) : row(r), V(v) {
-    lead = (int)((reinterpret_cast<uintptr_t>(r) & 15u) / sizeof(T));
+  int first, last;  // the pieces that reach beyond the row, or -1
+  __device__ __forceinline__ RowPieces(const T* r, int v, bool aligned = false) : row(r), V(v) {
+    lead = aligned ? 0 : (int)((reinterpret_cast<uintptr_t>(r) & 15u) / sizeof(T));
     pieces = (V + lead + N - 1) / N;
+    first = lead ? 0 : -1;
+    last = (V + lead) % N ? pieces - 1 : -1;
   }
-  __device__ __forceinline__ bool whole(int j) const { return j * N >= lead && (j + 1) * N - lead <= V; }
-  __device__ __forceinline__ uint4 edge(int j) const {  // -inf beyond the row
-    uint4 v = make_uint4(Piece<T>::lowest(), Piece<T>::lowest(), Piece<T>::lowest(), Piece<T>::lowest());
-    T* e = reinterpret_cast<T*>(&v);
-    for (int i = 0; i < N; ++i) {
-      const int at = j * N - lead + i;
-      if (at >= 0 && at < V) e[i] = row[at];
-    }
-    return v;
-  }
-  __device__ __forceinline__ uint4 load(int j) const {
-    return whole(j) ? load_once(reinterpret_cast<const uint4*>(row - lead) + j) : edge(j);
-  }
+  __device__ __forceinline__ bool whole(int j) const { return j != first && j != last; }
+  __device__ __forceinline__ uint4 edge(int j) const { return load_edge(row, j * N - lead, V); }
+  __device__ __forceinline__ const uint4* at(int j) const { return reinterpret_cast<const uint4*>(row - lead) + j; }
+  __device__ __forceinline__ uint4 load(int j) const { return whole(j) ? load_once(at(j)) : edge(j); }
 };
 
-template <int THREADS, typename F>
-__device__ __forceinline__ float block_reduce(float x, float* shared, F op) {
-  constexpr int WARPS = THREADS / 32;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) x = op(x, __shfl_xor_sync(0xffffffffu, x, o));
-  if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = x;
-  __syncthreads();
-  x = shared[threadIdx.x & (WARPS - 1)];
-#pragma unroll
-  for (int o = WARPS / 2; o > 0; o >>= 1) x = op(x, __shfl_xor_sync(0xffffffffu, x, o));
-  return x;
-}
-
-// A row's gradient: f times exp2((z - top) k) taken off, `slope` added at element y. Where the output's row lies against 16-byte
-// boundaries as the input's does it is written in pieces, otherwise element by element.
-template <typename T>
+// A row's gradient. Where it lies against 16-byte boundaries as the row itself does it is written in pieces, otherwise element by
+// element.
+template <typename T, bool ALIGNED>
 struct GradRow {
   static constexpr int N = Piece<T>::N;
   const RowPieces<T>& r;
   T* out;
   bool same;
-  float k, top, f, slope;
-  int yj;
-  __device__ __forceinline__ GradRow(const RowPieces<T>& r_, T* o, float top_, float k_, float f_, float s, int y)
-      : r(r_), out(o), k(k_), top(top_), f(f_), slope(s), yj(y + r_.lead) {
+  __device__ __forceinline__ GradRow(const RowPieces<T>& r_, T* o) : r(r_), out(o) {
     same = (((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(r.row)) & 15u) == 0);
   }
-  __device__ __forceinline__ void put(int j, const uint4& piece) const {
-    float z[N];
-    Piece<T>::widen(piece, z);
-    exp_piece(z, top, k);
-#pragma unroll
-    for (int i = 0; i < N; ++i) z[i] *= -f;
-    if (yj >= j * N && yj < (j + 1) * N) {
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (yj - j * N == i) z[i] += slope;
-    }
-    store(j, Piece<T>::narrow(z));
-  }
   __device__ __forceinline__ void store(int j, const uint4& v) const {
-    if (same && r.whole(j)) {
+    if (ALIGNED || (same && r.whole(j)))
       reinterpret_cast<uint4*>(out - r.lead)[j] = v;
-    } else {
-      const T* e = reinterpret_cast<const T*>(&v);
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int at = j * N - r.lead + i;
-        if (at >= 0 && at < r.V) out[at] = e[i];
-      }
-    }
+    else
+      store_edge(out, j * N - r.lead, r.V, v);
   }
 };
 
-template <typename T, int THREADS>
-__device__ __forceinline__ void write_zeros(const RowPieces<T>& r, T* out, int j0, int j1) {
-  const GradRow<T> g(r, out, 0.f, 0.f, 0.f, 0.f, -1);
-  for (int j = j0 + threadIdx.x; j < j1; j += THREADS) g.store(j, make_uint4(0u, 0u, 0u, 0u));
+// A softmax's sum about a reference: s = sum of exp2(z k - m k). Empty (s = 0) it has no reference.
+struct Share {
+  float m, s;
+};
+
+// The warp's shares as one, in every lane and one order.
+__device__ __forceinline__ Share warp_share(const Share& x, float k) {
+  float m = x.s == 0.f ? -INFINITY : x.m;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (m == -INFINITY) m = 0.f;
+  float s = x.s == 0.f ? 0.f : x.s * Ref(m, k).from(Ref(x.m, k), k);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return {m, s};
 }
 
-// A cluster of CTAs takes a row, each a share of its pieces in shared memory: read and compared, summed about the share's own
-// maximum, the shares' (maximum, sum) met through distributed shared memory, the gradient written. exp is evaluated twice an element, to
-// keep 16 bits of it in shared memory instead of 32 and two CTAs on an SM: one reads its row while the other computes.
-template <typename T, int THREADS, bool POLICY>
+// A cluster of CTAs takes a row, each a share of its pieces. All of a share is asked for at once and lies in shared memory; a thread
+// copies the pieces that it will look at itself, so that no barrier is needed for them. It sums exponentials about the largest element
+// of its first piece; where that was a poor choice (the sum leaves [1/2, 2^100]) it looks for its largest element and sums again. The
+// warps' and CTAs' (reference, sum) meet in one step, one thread works out the row's scalars, and the gradient is written from the share:
+// exp2(z k - m k + log2(slope / sum)), so that it takes one operation, the exponential and the rounding an element. exp is evaluated twice, to keep
+// 16 bits of an element instead of 32 and two CTAs on an SM: one waits for its row while the other computes. (Kept in registers
+// instead, with the next row read ahead, an element costs less, but the CTAs that a row then needs wait for each other: 810 us against 290
+// for 8 x 1024 x 50304 bf16, a quarter of it not counted.)
+// ALIGNED: every row begins and ends on a 16-byte boundary, in the gradient too.
+template <typename T, int THREADS, int MODE, bool ALIGNED>  // MODE 0: log-probabilities, 1: the policy loss, 2: and its gradient
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) loss_kernel(const __grid_constant__ LossParams a) {
-  extern __shared__ uint4 s_row[];
-  __shared__ float s_red[2][THREADS / 32];
-  __shared__ float s_share[2];  // this CTA's maximum and sum
-  __shared__ float s_row_of[3];  // factor of the CTA's exponentials, slope / tau
-  const int cs = cluster_nctarank(), rank = cluster_ctarank();
-  const int64_t r = blockIdx.x / cs;
-  const int b = (int)(r / a.T), t = (int)(r - (int64_t)b * a.T);
-  const T* row = reinterpret_cast<const T*>(a.z) + b * a.z_sb + t * a.z_st;
-  T* out = reinterpret_cast<T*>(a.grad) + b * a.g_sb + t * a.g_st;
-  const RowPieces<T> p(row, a.V);
-  const int j0 = min(rank * a.per, p.pieces), j1 = min(j0 + a.per, p.pieces);
+  constexpr int N = Piece<T>::N, WARPS = THREADS / 32;
+  constexpr bool POLICY = MODE > 0;
+  extern __shared__ uint4 share[];
+  __shared__ Share s_warp[WARPS];
+  __shared__ float s_of[4];  // of the row: reference, factor of the exponentials, its logarithm (base 2) and slope / tau
+  __shared__ int s_token;
+  const int tid = threadIdx.x, cs = cluster_nctarank(), rank = cluster_ctarank();
+  const int r = blockIdx.x / cs;
+  const int b = r / a.T, t = r - b * a.T;
+  const T* const row = reinterpret_cast<const T*>(a.z) + b * a.z_sb + t * a.z_st;
   const float k = a.inv_tau * LOG2E;
+  const RowPieces<T> p(row, a.V, ALIGNED);
+  const int j0 = rank * a.per, n = min(a.per, p.pieces - j0);  // (n < 1: a share without pieces)
   pdl_wait();
   pdl_launch_dependents();
+  T* const out = MODE == 2 ? reinterpret_cast<T*>(a.grad) + b * a.g_sb + t * a.g_st : nullptr;
+  const GradRow<T, ALIGNED> g(p, out);
   float w = 1.f;
   if (POLICY) {
     w = a.weight.p ? a.weight.at(b, t) : a.w0;
     if (w == 0.f) {  // not counted, whatever is in it (the same in all threads of the cluster)
-      if (a.grad) write_zeros<T, THREADS>(p, out, j0, j1);
-      if (rank == 0 && threadIdx.x == 0) a.logp[r] = a.top[r] = a.tot[r] = a.slope[r] = a.term[r] = 0.f;
+      if (MODE == 2)
+        for (int j = tid; j < n; j += THREADS) g.store(j0 + j, make_uint4(0u, 0u, 0u, 0u));
+      if (rank == 0 && tid == 0) a.logp[r] = a.top[r] = a.tot[r] = a.slope[r] = a.term[r] = 0.f;
       return;
     }
   }
-  // the row's scalars, while it is read
+  {
+    const uint4* const from = p.at(j0);
+    for (int j = tid; j < n; j += THREADS) {
+      if (ALIGNED || p.whole(j0 + j))
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(share + j)), "l"(from + j) : "memory");
+      else
+        share[j] = p.edge(j0 + j);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  // the row's scalars, while it arrives
   int64_t y = -1;
   float zy = 0.f, old = 0.f, adv = 0.f, ref = 0.f;
-  if (threadIdx.x == 0) {
+  if (tid == 0) {
     y = a.tokens[b * a.t_sb + t * a.t_st];
     if (POLICY) {
       old = a.old.at(b, t);
@@ -245,106 +248,144 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) loss_kernel(const __g
       if (a.kl != 0.f) ref = a.ref.at(b, t);
     }
     if (y < 0 || y >= a.V) {
-      if (rank == 0) record_error(DEV_INDEX_RANGE, K_LOSS, (int)r, (int)y);
+      if (rank == 0) record_error(DEV_INDEX_RANGE, K_LOSS, r, (int)y);
       y = -1;
       zy = __int_as_float(0x7fc00000);
     } else {
       zy = to_f32(row[y]);
     }
   }
-  uint32_t top = Piece<T>::lowest();
-  {
-    constexpr int U = 4;
-    int j = j0 + threadIdx.x;
-    for (; j + (U - 1) * THREADS < j1; j += U * THREADS) {
-      uint4 v[U];
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  auto largest = [](const uint4& v) { return Piece<T>::top(Piece<T>::max2(Piece<T>::max2(v.x, v.y), Piece<T>::max2(v.z, v.w))); };
+  auto sum_about = [&](const Ref& m) {
+    float s = 0.f;
+    for (int j = tid; j < n; j += THREADS) {
+      float z[N];
+      Piece<T>::widen(share[j], z);
+      if (!m.far) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) v[u] = p.load(j + u * THREADS);
+        for (int i = 0; i < N; ++i) z[i] = exp2_fast(fmaf(z[i], k, m.off));
+      } else {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        s_row[j - j0 + u * THREADS] = v[u];
-        top = Piece<T>::max2(top, Piece<T>::max2(Piece<T>::max2(v[u].x, v[u].y), Piece<T>::max2(v[u].z, v[u].w)));
+        for (int i = 0; i < N; ++i) z[i] = exp2_fast((z[i] - m.m) * k);
       }
-    }
-    for (; j < j1; j += THREADS) {
-      const uint4 v = p.load(j);
-      s_row[j - j0] = v;
-      top = Piece<T>::max2(top, Piece<T>::max2(Piece<T>::max2(v.x, v.y), Piece<T>::max2(v.z, v.w)));
-    }
-  }
-  auto larger = [](float x, float z) { return fmaxf(x, z); };
-  auto plus = [](float x, float z) { return x + z; };
-  float m = block_reduce<THREADS>(Piece<T>::top(top), s_red[0], larger);
-  if (m == -INFINITY) m = 0.f;  // nothing to take off: every exponential is 0
-  float sum = 0.f;
-  for (int j = j0 + threadIdx.x; j < j1; j += THREADS) {
-    float z[Piece<T>::N];
-    Piece<T>::widen(s_row[j - j0], z);
-    exp_piece(z, m, k);
-    float part = 0.f;
 #pragma unroll
-    for (int i = 0; i < Piece<T>::N; ++i) part += z[i];
-    sum += part;
-  }
-  sum = block_reduce<THREADS>(sum, s_red[1], plus);
-  if (cs > 1) {
-    if (threadIdx.x == 0) {
-      s_share[0] = m;
-      s_share[1] = sum;
+      for (int o = N / 2; o > 0; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < o; ++i) z[i] += z[i + o];
+      s += z[0];
     }
-    cluster_sync_all();
-  }
-  if (threadIdx.x == 0) {
-    float gm = m, gs = sum;
-    if (cs > 1) {
-      gm = -INFINITY;
-      for (int c = 0; c < cs; ++c)
-        if (cluster_map(s_share, c)[1] != 0.f) gm = fmaxf(gm, cluster_map(s_share, c)[0]);  // (an empty share's 0 does not count)
-      if (gm == -INFINITY) gm = 0.f;
-      gs = 0.f;
-      for (int c = 0; c < cs; ++c) {
-        const float sc = cluster_map(s_share, c)[1];
-        if (sc != 0.f) gs += sc * exp2f((cluster_map(s_share, c)[0] - gm) * k);
-      }
-    }
-    const float logp = (zy - gm) * a.inv_tau - logf(gs);
-    float slope = 0.f;
-    if (POLICY) {
-      const float rho = expf(logp - old);
-      const float held = rho < a.lo ? a.lo : rho > a.hi ? a.hi : rho;  // (comparisons that keep a NaN)
-      const float free_ = rho * adv, kept = held * adv;
-      float term = -(kept < free_ ? kept : free_);
-      slope = (adv > 0.f ? rho > a.hi : rho < a.lo) ? 0.f : -adv * rho;
-      if (a.kl != 0.f) {
-        const float d = ref - logp, e = expm1f(d);
-        term += a.kl * (e - d);
-        slope -= a.kl * e;
-      }
-      slope *= w * a.inv_tau;
-      if (rank == 0) {
-        a.slope[r] = slope;
-        a.term[r] = w * term;
-      }
-    }
-    if (rank == 0) {
-      a.logp[r] = logp;
-      a.top[r] = gm;
-      a.tot[r] = gs;
-    }
-    s_row_of[0] = sum == 0.f && gs > 0.f ? 0.f : slope * exp2f((m - gm) * k) / gs;
-    s_row_of[1] = slope;
-    s_row_of[2] = __int_as_float((int)y);
+    return s;
+  };
+  float top = tid < n ? largest(share[tid]) : -INFINITY;
+  if (!(top > -INFINITY)) top = 0.f;  // nothing to take off
+  float s = sum_about(Ref(top, k));
+  if (!(s >= 0.5f && s < 1.2676506e30f) && tid < n) {
+    top = -INFINITY;
+    for (int j = tid; j < n; j += THREADS) top = fmaxf(top, largest(share[j]));
+    if (!(top > -INFINITY)) top = 0.f;
+    s = sum_about(Ref(top, k));
   }
   __syncwarp();
-  if (cs > 1) cluster_arrive();  // this CTA has read the others' shares
-  if (POLICY && a.grad) {
+  const Share mine = warp_share({top, s}, k);
+  if ((tid & 31) == 0) s_warp[tid >> 5] = mine;
+  if (cs > 1)
+    cluster_sync_all();
+  else
     __syncthreads();
-    const float f = s_row_of[0], slope = s_row_of[1];
+  if (tid < 32) {
+    Share sum = {0.f, 0.f};
+    for (int i = tid; i < cs * WARPS; i += 32) {
+      const Share x = (cs > 1 ? cluster_map(s_warp, i / WARPS) : s_warp)[i % WARPS];
+      if (x.s != 0.f) {
+        if (sum.s == 0.f) {
+          sum = x;
+        } else if (x.m > sum.m) {
+          sum.s = sum.s * Ref(x.m, k).from(Ref(sum.m, k), k) + x.s;
+          sum.m = x.m;
+        } else {
+          sum.s += x.s * Ref(sum.m, k).from(Ref(x.m, k), k);
+        }
+      }
+    }
+    sum = warp_share(sum, k);
+    if (tid == 0) {
+      const float logp = Ref(sum.m, k).of(zy, k) * LN2 - logf(sum.s);
+      float slope = 0.f;
+      if (POLICY) {
+        const float rho = expf(logp - old);
+        const float held = rho < a.lo ? a.lo : rho > a.hi ? a.hi : rho;  // (comparisons that keep a NaN)
+        const float free_ = rho * adv, kept = held * adv;
+        float term = -(kept < free_ ? kept : free_);
+        slope = (adv > 0.f ? rho > a.hi : rho < a.lo) ? 0.f : -adv * rho;
+        if (a.kl != 0.f) {
+          const float d = ref - logp, x = expm1f(d);
+          term += a.kl * (x - d);
+          slope -= a.kl * x;
+        }
+        slope *= w * a.inv_tau;
+        if (rank == 0) {
+          a.slope[r] = slope;
+          a.term[r] = w * term;
+        }
+        const float f = slope / sum.s;
+        s_of[0] = sum.m;
+        s_of[1] = -f;
+        s_of[2] = log2f(fabsf(f));
+        s_of[3] = slope;
+        s_token = (int)y;
+      }
+      if (rank == 0) {
+        a.logp[r] = logp;
+        a.top[r] = sum.m;
+        a.tot[r] = sum.s;
+      }
+    }
+    __syncwarp();
+  }
+  if (cs > 1) cluster_arrive();  // this CTA has read the others' shares
+  if (MODE == 2) {
+    __syncthreads();
+    const float slope = s_of[3];
+    const Ref m(s_of[0], k);
+    const int yt = s_token, yp = yt < 0 ? -1 : (yt + p.lead) / N - j0, yi = (yt + p.lead) % N;
+    auto add = [&](int j, float (&z)[N]) {
+      if (j == yp) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (yi == i) z[i] += slope;
+      }
+    };
     if (slope == 0.f) {
-      write_zeros<T, THREADS>(p, out, j0, j1);
+      for (int j = tid; j < n; j += THREADS) g.store(j0 + j, make_uint4(0u, 0u, 0u, 0u));
+    } else if (m.far || !(fabsf(s_of[2]) < 1e30f)) {
+      const float f = s_of[1];
+      for (int j = tid; j < n; j += THREADS) {
+        float z[N];
+        Piece<T>::widen(share[j], z);
+        for (int i = 0; i < N; ++i) z[i] = f * exp2_fast(m.of(z[i], k));
+        add(j, z);
+        g.store(j0 + j, Piece<T>::narrow(z));
+      }
     } else {
-      const GradRow<T> g(p, out, m, k, f, slope, __float_as_int(s_row_of[2]));
-      for (int j = j0 + threadIdx.x; j < j1; j += THREADS) g.put(j, s_row[j - j0]);
+      const float off = m.off + s_of[2];
+      auto all = [&](auto sign) {
+        for (int j = tid; j < n; j += THREADS) {
+          float z[N];
+          Piece<T>::widen(share[j], z);
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            const float e = exp2_fast(fmaf(z[i], k, off));
+            z[i] = decltype(sign)::value ? -e : e;
+          }
+          add(j, z);
+          g.store(j0 + j, Piece<T>::narrow(z));
+        }
+      };
+      if (slope > 0.f)
+        all(std::true_type());
+      else
+        all(std::false_type());
     }
   }
   if (cs > 1) cluster_wait();
@@ -371,7 +412,8 @@ struct LogitsGradParams {
   const void* z;
   int64_t z_sb, z_st;
   int B, T, V;
-  int chunks;  // CTAs of a row
+  int chunks;      // pieces of a row that CTAs take
+  uint32_t items;  // and of all rows
   const int64_t* tokens;
   int64_t t_sb, t_st;
   const float *top, *tot;
@@ -393,32 +435,52 @@ __global__ void __launch_bounds__(GRAD_THREADS) logits_grad_kernel(const __grid_
   pdl_launch_dependents();
   const float up = a.up ? *a.up : 1.f;
   if (a.unit_done && up == 1.f) return;
-  const int64_t items = (int64_t)a.B * a.T * a.chunks;
-  for (int64_t i = blockIdx.x; i < items; i += gridDim.x) {
-    const int64_t r = i / a.chunks;
-    const int b = (int)(r / a.T), t = (int)(r - (int64_t)b * a.T);
+  for (uint32_t i = blockIdx.x; i < a.items; i += gridDim.x) {
+    const uint32_t r = i / (uint32_t)a.chunks;
+    const int b = (int)(r / (uint32_t)a.T), t = (int)(r - (uint32_t)b * a.T);
     const RowPieces<T> p(reinterpret_cast<const T*>(a.z) + b * a.z_sb + t * a.z_st, a.V);
     T* out = reinterpret_cast<T*>(a.grad) + b * a.g_sb + t * a.g_st;
-    const int j0 = (int)(i - r * a.chunks) * GRAD_PIECES, j1 = min(j0 + GRAD_PIECES, p.pieces);
+    const int j0 = (int)(i - r * (uint32_t)a.chunks) * GRAD_PIECES, j1 = min(j0 + GRAD_PIECES, p.pieces);
     const float own = a.slope.at(b, t);
-    const float slope = own == 0.f ? 0.f : own * a.by * up;
-    if (own == 0.f) {
-      write_zeros<T, GRAD_THREADS>(p, out, j0, j1);
-      continue;
-    }
     const int64_t y = a.tokens[b * a.t_sb + t * a.t_st];
-    const float f = y >= 0 && y < a.V ? slope / a.tot[r] : __int_as_float(0x7fc00000);
-    const GradRow<T> g(p, out, a.top[r], a.inv_tau * LOG2E, f, slope, (int)y);
-    uint4 v[GRAD_PIECES / GRAD_THREADS];
+    const bool known = y >= 0 && y < a.V;
+    const float slope = own * a.by * up;
+    const GradRow<T, false> g(p, out);
+    const int yp = known ? ((int)y + p.lead) / Piece<T>::N : -1, yi = known ? ((int)y + p.lead) % Piece<T>::N : 0;
+    constexpr int U = GRAD_PIECES / GRAD_THREADS, N = Piece<T>::N;
+    uint4 v[U];
+    if (own != 0.f) {
 #pragma unroll
-    for (int u = 0; u < GRAD_PIECES / GRAD_THREADS; ++u) {
-      const int j = j0 + threadIdx.x + u * GRAD_THREADS;
-      if (j < j1) v[u] = p.load(j);
+      for (int u = 0; u < U; ++u) {
+        const int j = j0 + threadIdx.x + u * GRAD_THREADS;
+        if (j < j1) v[u] = p.load(j);
+      }
     }
+    const float f = known ? -slope / a.tot[r] : __int_as_float(0x7fc00000), k = a.inv_tau * LOG2E;
+    const Ref m(a.top[r], k);
 #pragma unroll
-    for (int u = 0; u < GRAD_PIECES / GRAD_THREADS; ++u) {
+    for (int u = 0; u < U; ++u) {
       const int j = j0 + threadIdx.x + u * GRAD_THREADS;
-      if (j < j1) g.put(j, v[u]);
+      if (j >= j1) break;
+      if (own == 0.f) {
+        g.store(j, make_uint4(0u, 0u, 0u, 0u));
+        continue;
+      }
+      float z[N];
+      Piece<T>::widen(v[u], z);
+      if (!m.far) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) z[i] = exp2_fast(fmaf(z[i], k, m.off)) * f;
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) z[i] = exp2_fast((z[i] - m.m) * k) * f;
+      }
+      if (j == yp) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (yi == i) z[i] += slope;
+      }
+      g.store(j, Piece<T>::narrow(z));
     }
   }
 }
