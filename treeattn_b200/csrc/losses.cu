@@ -39,7 +39,7 @@ int check_rows(const char* who, const void* z, int dtype, int B, int T, int V, c
 template <typename T, int THREADS, int MODE, bool ALIGNED>
 int launch_loss(const ta::LossParams& a, int cs, cudaStream_t st, const char* who) {
   static SmemAttr attr;
-  const size_t smem = (size_t)a.per * 16;
+  const size_t smem = MODE == 2 ? (size_t)a.per * 16 : 0;
   if (int r = allow_smem(attr, ta::loss_kernel<T, THREADS, MODE, ALIGNED>, smem, who)) return r;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((int64_t)a.B * a.T * cs));
@@ -64,9 +64,9 @@ int run_loss(ta::LossParams& a, cudaStream_t st, const char* who) {
   constexpr int N = 16 / (int)sizeof(T);
   const int64_t rows = (int64_t)a.B * a.T;
   const int pieces = (a.V + 2 * N - 2) / N;  // at most, wherever the row begins
-  // CTAs of a row: as few as leave room for two on an SM, more where the rows do not fill the GPU
+  // CTAs of a row: as few as leave room for two on an SM (one, where nothing is kept), more where the rows do not fill the GPU
   int cs = 1;
-  while (cs < 8 && ((int64_t)pieces * 16 > (int64_t)cs * TWO_PER_SM || (rows * cs < 2 * sm_count() && pieces * 16 >= 2 * cs * 8192)))
+  while (cs < 8 && ((MODE == 2 && (int64_t)pieces * 16 > (int64_t)cs * TWO_PER_SM) || (rows * cs < 2 * sm_count() && pieces * 16 >= 2 * cs * 8192)))
     cs *= 2;
   a.per = (pieces + cs - 1) / cs;
   const bool aligned = a.V % N == 0 && rows_aligned(a.z, sizeof(T), {a.z_sb, a.z_st}) &&
@@ -75,8 +75,9 @@ int run_loss(ta::LossParams& a, cudaStream_t st, const char* who) {
     if (aligned) return launch_loss<T, 128, MODE, true>(a, cs, st, who);
     return launch_loss<T, 128, MODE, false>(a, cs, st, who);
   }
-  if (aligned) return launch_loss<T, 512, MODE, true>(a, cs, st, who);
-  return launch_loss<T, 512, MODE, false>(a, cs, st, who);
+  constexpr int WIDE = MODE == 2 ? 512 : 256;
+  if (aligned) return launch_loss<T, WIDE, MODE, true>(a, cs, st, who);
+  return launch_loss<T, WIDE, MODE, false>(a, cs, st, who);
 }
 
 template <int MODE>
@@ -164,7 +165,8 @@ int ta_logits_grad(const void* logits, int dtype, int64_t z_sb, int64_t z_st, in
   const int64_t items = rows * a.chunks;
   if (items > UINT32_MAX / 2) return fail(TA_ERR_ARG, "%s: too many rows of %d words", who, V);
   a.items = (uint32_t)items;
-  const unsigned grid = (unsigned)std::min<int64_t>(items, (int64_t)sm_count() * 8);
+  // a CTA a piece; where the work is most likely done already, no more of them than the GPU holds
+  const unsigned grid = (unsigned)(unit_done ? std::min<int64_t>(items, (int64_t)sm_count() * 6) : items);
   cudaError_t e;
   const cudaStream_t st = S(stream);
   switch (dtype) {

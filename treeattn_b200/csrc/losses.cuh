@@ -164,11 +164,17 @@ struct GradRow {
   __device__ __forceinline__ GradRow(const RowPieces<T>& r_, T* o) : r(r_), out(o) {
     same = (((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(r.row)) & 15u) == 0);
   }
-  __device__ __forceinline__ void store(int j, const uint4& v) const {
-    if (ALIGNED || (same && r.whole(j)))
+  __device__ __forceinline__ void edge(int j, const uint4& v) const { store_edge(out, j * N - r.lead, r.V, v); }
+  __device__ __forceinline__ void whole(int j, const uint4& v) const {  // a piece that lies in the row
+    if (ALIGNED || same)
       reinterpret_cast<uint4*>(out - r.lead)[j] = v;
     else
-      store_edge(out, j * N - r.lead, r.V, v);
+      edge(j, v);
+  }
+  __device__ __forceinline__ void zeros(int j0, int j, int end, int step, int cut) const {
+    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+    for (; j < end; j += step) whole(j0 + j, zero);
+    if (cut >= 0) edge(j0 + cut, zero);
   }
 };
 
@@ -197,11 +203,12 @@ __device__ __forceinline__ Share warp_share(const Share& x, float k) {
 // 16 bits of an element instead of 32 and two CTAs on an SM: one waits for its row while the other computes. (Kept in registers
 // instead, with the next row read ahead, an element costs less, but the CTAs that a row then needs wait for each other: 810 us against 290
 // for 8 x 1024 x 50304 bf16, a quarter of it not counted.)
+// Without a gradient nothing is kept, and the row is summed as it arrives.
 // ALIGNED: every row begins and ends on a 16-byte boundary, in the gradient too.
 template <typename T, int THREADS, int MODE, bool ALIGNED>  // MODE 0: log-probabilities, 1: the policy loss, 2: and its gradient
-__global__ void __launch_bounds__(THREADS, 1024 / THREADS) loss_kernel(const __grid_constant__ LossParams a) {
+__global__ void __launch_bounds__(THREADS, (MODE == 2 ? 1024 : 1280) / THREADS) loss_kernel(const __grid_constant__ LossParams a) {
   constexpr int N = Piece<T>::N, WARPS = THREADS / 32;
-  constexpr bool POLICY = MODE > 0;
+  constexpr bool POLICY = MODE > 0, KEEP = MODE == 2;
   extern __shared__ uint4 share[];
   __shared__ Share s_warp[WARPS];
   __shared__ float s_of[4];  // of the row: reference, factor of the exponentials, its logarithm (base 2) and slope / tau
@@ -213,6 +220,9 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) loss_kernel(const __g
   const float k = a.inv_tau * LOG2E;
   const RowPieces<T> p(row, a.V, ALIGNED);
   const int j0 = rank * a.per, n = min(a.per, p.pieces - j0);  // (n < 1: a share without pieces)
+  // the share's whole pieces are [i0, i1); one that the row begins or ends in belongs to thread 0 or 1
+  const int i0 = !ALIGNED && n > 0 && p.first == j0, i1 = !ALIGNED && p.last == j0 + n - 1 && n > i0 ? n - 1 : n;
+  const int edge = ALIGNED ? -1 : tid == 0 && i0 ? 0 : tid == 1 && n > 0 && i1 < n ? n - 1 : -1;
   pdl_wait();
   pdl_launch_dependents();
   T* const out = MODE == 2 ? reinterpret_cast<T*>(a.grad) + b * a.g_sb + t * a.g_st : nullptr;
@@ -221,20 +231,16 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) loss_kernel(const __g
   if (POLICY) {
     w = a.weight.p ? a.weight.at(b, t) : a.w0;
     if (w == 0.f) {  // not counted, whatever is in it (the same in all threads of the cluster)
-      if (MODE == 2)
-        for (int j = tid; j < n; j += THREADS) g.store(j0 + j, make_uint4(0u, 0u, 0u, 0u));
+      if (MODE == 2) g.zeros(j0, i0 + tid, i1, THREADS, edge);
       if (rank == 0 && tid == 0) a.logp[r] = a.top[r] = a.tot[r] = a.slope[r] = a.term[r] = 0.f;
       return;
     }
   }
-  {
-    const uint4* const from = p.at(j0);
-    for (int j = tid; j < n; j += THREADS) {
-      if (ALIGNED || p.whole(j0 + j))
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(share + j)), "l"(from + j) : "memory");
-      else
-        share[j] = p.edge(j0 + j);
-    }
+  const uint4* const from = p.at(j0);
+  if (KEEP) {
+    for (int j = i0 + tid; j < i1; j += THREADS)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(share + j)), "l"(from + j) : "memory");
+    if (edge >= 0) share[edge] = p.edge(j0 + edge);
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
   // the row's scalars, while it arrives
@@ -255,36 +261,53 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) loss_kernel(const __g
       zy = to_f32(row[y]);
     }
   }
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  if (KEEP) asm volatile("cp.async.wait_group 0;" ::: "memory");
+  auto piece = [&](int j) { return KEEP ? share[j] : load_once(from + j); };  // a whole one
+  uint4 cut = make_uint4(0u, 0u, 0u, 0u);
+  if (edge >= 0) cut = KEEP ? share[edge] : p.edge(j0 + edge);
   auto largest = [](const uint4& v) { return Piece<T>::top(Piece<T>::max2(Piece<T>::max2(v.x, v.y), Piece<T>::max2(v.z, v.w))); };
-  auto sum_about = [&](const Ref& m) {
-    float s = 0.f;
-    for (int j = tid; j < n; j += THREADS) {
-      float z[N];
-      Piece<T>::widen(share[j], z);
-      if (!m.far) {
+  auto piece_sum = [&](const uint4& v, const Ref& m) {
+    float z[N];
+    Piece<T>::widen(v, z);
+    if (!m.far) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) z[i] = exp2_fast(fmaf(z[i], k, m.off));
-      } else {
+      for (int i = 0; i < N; ++i) z[i] = exp2_fast(fmaf(z[i], k, m.off));
+    } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) z[i] = exp2_fast((z[i] - m.m) * k);
-      }
-#pragma unroll
-      for (int o = N / 2; o > 0; o >>= 1)
-#pragma unroll
-        for (int i = 0; i < o; ++i) z[i] += z[i + o];
-      s += z[0];
+      for (int i = 0; i < N; ++i) z[i] = exp2_fast((z[i] - m.m) * k);
     }
-    return s;
+#pragma unroll
+    for (int o = N / 2; o > 0; o >>= 1)
+#pragma unroll
+      for (int i = 0; i < o; ++i) z[i] += z[i + o];
+    return z[0];
   };
-  float top = tid < n ? largest(share[tid]) : -INFINITY;
-  if (!(top > -INFINITY)) top = 0.f;  // nothing to take off
-  float s = sum_about(Ref(top, k));
-  if (!(s >= 0.5f && s < 1.2676506e30f) && tid < n) {
-    top = -INFINITY;
-    for (int j = tid; j < n; j += THREADS) top = fmaxf(top, largest(share[j]));
-    if (!(top > -INFINITY)) top = 0.f;
-    s = sum_about(Ref(top, k));
+  auto sum_about = [&](const Ref& m, int j, float s) {
+    if (!KEEP) {
+      constexpr int U = 4;
+      for (; j + (U - 1) * THREADS < i1; j += U * THREADS) {
+        uint4 v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = piece(j + u * THREADS);
+#pragma unroll
+        for (int u = 0; u < U; ++u) s += piece_sum(v[u], m);
+      }
+    }
+    for (; j < i1; j += THREADS) s += piece_sum(piece(j), m);
+    return edge >= 0 ? s + piece_sum(cut, m) : s;
+  };
+  float top = 0.f, s = 0.f;
+  const int first = i0 + tid;
+  if (first < i1 || edge >= 0) {
+    top = largest(first < i1 ? piece(first) : cut);
+    if (!(top > -INFINITY)) top = 0.f;  // nothing to take off
+    s = sum_about(Ref(top, k), first, 0.f);
+    if (!(s >= 0.5f && s < 1.2676506e30f)) {
+      top = edge >= 0 ? largest(cut) : -INFINITY;
+      for (int j = first; j < i1; j += THREADS) top = fmaxf(top, largest(piece(j)));
+      if (!(top > -INFINITY)) top = 0.f;
+      s = sum_about(Ref(top, k), first, 0.f);
+    }
   }
   __syncwarp();
   const Share mine = warp_share({top, s}, k);
@@ -357,20 +380,22 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) loss_kernel(const __g
       }
     };
     if (slope == 0.f) {
-      for (int j = tid; j < n; j += THREADS) g.store(j0 + j, make_uint4(0u, 0u, 0u, 0u));
+      g.zeros(j0, first, i1, THREADS, edge);
     } else if (m.far || !(fabsf(s_of[2]) < 1e30f)) {
       const float f = s_of[1];
-      for (int j = tid; j < n; j += THREADS) {
+      auto one = [&](int j) {
         float z[N];
         Piece<T>::widen(share[j], z);
         for (int i = 0; i < N; ++i) z[i] = f * exp2_fast(m.of(z[i], k));
         add(j, z);
-        g.store(j0 + j, Piece<T>::narrow(z));
-      }
+        return Piece<T>::narrow(z);
+      };
+      for (int j = first; j < i1; j += THREADS) g.whole(j0 + j, one(j));
+      if (edge >= 0) g.edge(j0 + edge, one(edge));
     } else {
       const float off = m.off + s_of[2];
       auto all = [&](auto sign) {
-        for (int j = tid; j < n; j += THREADS) {
+        auto one = [&](int j) {
           float z[N];
           Piece<T>::widen(share[j], z);
 #pragma unroll
@@ -379,8 +404,10 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) loss_kernel(const __g
             z[i] = decltype(sign)::value ? -e : e;
           }
           add(j, z);
-          g.store(j0 + j, Piece<T>::narrow(z));
-        }
+          return Piece<T>::narrow(z);
+        };
+        for (int j = first; j < i1; j += THREADS) g.whole(j0 + j, one(j));
+        if (edge >= 0) g.edge(j0 + edge, one(edge));
       };
       if (slope > 0.f)
         all(std::true_type());
@@ -463,7 +490,7 @@ __global__ void __launch_bounds__(GRAD_THREADS) logits_grad_kernel(const __grid_
       const int j = j0 + threadIdx.x + u * GRAD_THREADS;
       if (j >= j1) break;
       if (own == 0.f) {
-        g.store(j, make_uint4(0u, 0u, 0u, 0u));
+        p.whole(j) ? g.whole(j, make_uint4(0u, 0u, 0u, 0u)) : g.edge(j, make_uint4(0u, 0u, 0u, 0u));
         continue;
       }
       float z[N];
@@ -480,7 +507,10 @@ __global__ void __launch_bounds__(GRAD_THREADS) logits_grad_kernel(const __grid_
         for (int i = 0; i < N; ++i)
           if (yi == i) z[i] += slope;
       }
-      g.store(j, Piece<T>::narrow(z));
+      if (p.whole(j))
+        g.whole(j, Piece<T>::narrow(z));
+      else
+        g.edge(j, Piece<T>::narrow(z));
     }
   }
 }
