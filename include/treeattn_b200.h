@@ -441,14 +441,15 @@ int ta_logits_grad(const void* logits, int dtype, int64_t z_sb, int64_t z_st, in
  * multiples of 8; scale (n_adapters,) fp32 or NULL (1). Rows in `dtype`, 16-byte aligned, strides in elements. max_new: about the rows
  * of the longest sequence (it sizes the grid). An adapter outside [-1, n_adapters) gives NaN rows and is recorded.
  * ta_adapter_add: out = y + t B_a^T, t = scale_a x A_a^T (x (n_rows, K), y and out (n_rows, N); out may be y, with y's stride). Rows of no
- *   sequence and of no adapter are y's. t is fp32, and enters its product as two 16-bit numbers; one rounding of the sum. t_out
- *   (bf16 only): NULL, or (2, n_rows, r): those two numbers, high parts first, on the rows that have an adapter.
+ *   sequence and of no adapter are y's. t is fp32, and enters its product as two 16-bit numbers; one rounding of the sum. t: (2, n_rows, r)
+ *   of `dtype`, those two numbers, high parts first, on the rows that have an adapter (f16: each row brought near 1 by a power of two, and
+ *   behind them n_rows fp32 factors); written and read by the call, 16-byte aligned; may be NULL where max_new is at most 16.
  * ta_adapter_bwd (bf16): for dy (n_rows, N): u = scale_a dy B_a as (2, n_rows, r) scratch, dx = u A_a (0 on rows without an adapter), dA_a =
  *   u^T x, dB_a = dy^T t over all rows with adapter a, in one order (0 where there are none). dx, da, db: each NULL where not wanted; x is
  *   read for da, t for db, u is written for dx and da. */
 int ta_adapter_add(const void* y, int64_t y_sr, const void* x, int64_t x_sr, const void* a, const void* b, const float* scale,
                    int dtype, int n_adapters, int K, int N, int r, int n_rows, const int32_t* start, const int32_t* which, int B,
-                   int max_new, void* out, int64_t o_sr, void* t_out, void* stream);
+                   int max_new, void* out, int64_t o_sr, void* t, void* stream);
 int ta_adapter_bwd(const void* dy, int64_t d_sr, const void* x, int64_t x_sr, const void* a, const void* b, const float* scale,
                    int n_adapters, int K, int N, int r, int n_rows, const int32_t* start, const int32_t* which, int B, int max_new,
                    const void* t, void* u, void* dx, int64_t dx_sr, void* da, void* db, void* stream);

@@ -17,7 +17,7 @@ def test_rejected_arguments_without_gpu():
                      (dict(B=65535), 'bad sizes'), (dict(new=-1), 'bad sizes'), (dict(start=None), 'null'), (dict(which=None), 'null'),
                      (dict(x=None), 'null'), (dict(y=None), 'null'), (dict(a=None), 'null'), (dict(out=None), 'null'),
                      (dict(x=p + 8), 'aligned'), (dict(xsr=132), 'aligned'), (dict(ysr=68), 'aligned'), (dict(osr=1), 'aligned'),
-                     (dict(b=p + 2), 'aligned'), (dict(dtype=2, t=p), 'bfloat16 only'), (dict(out=p, osr=72), 'strides')):
+                     (dict(b=p + 2), 'aligned'), (dict(new=17), 't is needed'), (dict(new=17, t=p + 8), 't is needed'), (dict(out=p, osr=72), 'strides')):
         assert add(**kw) == _lib.TA_ERR_ARG
         assert 'ta_adapter_add' in _lib.last_error() and what in _lib.last_error(), (kw, _lib.last_error())
     assert add(n=0) == _lib.TA_OK

@@ -47,8 +47,11 @@ def _check(name, y, x, a, b, start, which, scale):
     _need_cuda(name, x)
 
 
-def _add(y, x, a, b, start, which, max_new, scale, out, t):
+def _add(y, x, a, b, start, which, max_new, scale, out, t=None):
     (na, r, K), N = a.shape, y.shape[1]
+    if t is None and max_new > 16:  # many rows: t goes by way of memory (f16's rows with a factor each)
+        n = x.shape[0]
+        t = torch.empty(2 * n * r + (2 * n if x.dtype is torch.float16 else 0), device=x.device, dtype=x.dtype)
     with _on(x):
         _call('ta_adapter_add', y.data_ptr(), y.stride(0), x.data_ptr(), x.stride(0), a.data_ptr(), b.data_ptr(), _p(scale),
               _DT[x.dtype], na, K, N, r, x.shape[0], start.data_ptr(), which.data_ptr(), which.shape[0], max_new, out.data_ptr(),
@@ -119,7 +122,7 @@ def adapter_add(y, x, a, b, start, which, max_new, scale=None, out=None):
         if out.shape != y.shape:
             raise ValueError('adapter_add: out must have y\'s shape')
         _need_cuda('adapter_add', out)
-    return _add(y, x, a, b, start, which, max_new, scale, out, None)
+    return _add(y, x, a, b, start, which, max_new, scale, out)
 
 
 class AdapterSet(nn.Module):

@@ -22,7 +22,7 @@ namespace {
 
 using namespace ta_host;
 
-constexpr int SMALL_ROWS = 16;  // rows of one sequence up to which a call takes tiles of 16
+constexpr int FUSED_ROWS = 16;  // rows of one sequence up to which a call takes one kernel, and t need not be kept
 
 int check(const char* who, int dtype, int n_adapters, int K, int N, int r, int n_rows, int B, int max_new, const void* start,
           const void* which) {
@@ -58,35 +58,66 @@ int launch(const char* who, void (*kern)(P), SmemAttr& attr, int smem, dim3 grid
   return TA_OK;
 }
 
-template <typename T, int TM, int RP, bool TRANS>
-int run_tiles(const char* who, ta::AdapterParams& p, int max_new, cudaStream_t st) {
-  using S = ta::AdapterShape<TM, RP, TRANS>;
-  static SmemAttr attr;
-  p.tiles = std::max(1, (int)(((int64_t)std::min(max_new, p.n_rows) + TM - 1) / TM));
-  // CTAs of a tile: more where the tiles do not fill the GPU and each keeps a stage of columns
-  const int64_t items = (int64_t)p.tiles * p.B, room = (int64_t)sm_count() * (TM == 16 ? 4 : 2);
-  const int chunks = std::max((p.K + S::KC - 1) / S::KC, (p.N + S::KC - 1) / S::KC);
+// CTAs of a tile: as many as fill the GPU with one wave of `on_sm` CTAs an SM, each with at least `keep` stages of columns.
+int cluster_size(int64_t items, int on_sm, int stages, int keep) {
   int cs = 1;
-  while (cs < (TM == 16 ? 8 : 4) && items * cs < room && cs < chunks) cs *= 2;
-  const int64_t x = (int64_t)p.tiles * cs;
-  if (x > INT_MAX) return fail(TA_ERR_ARG, "%s: too many rows", who);
-  const dim3 grid((unsigned)x, p.B + (p.out == p.y ? 0 : 1));
-  return launch(who, ta::adapter_kernel<T, TM, RP, TRANS>, attr, S::BYTES, grid, cs, st, p);
+  while (cs < 8 && items * (cs + 1) <= (int64_t)sm_count() * on_sm && (cs + 1) * keep <= stages) ++cs;
+  return cs;
 }
 
-template <typename T, bool TRANS>
-int run_adapter(const char* who, ta::AdapterParams& p, int max_new, cudaStream_t st) {
-#define TA_RANK(TM)                                                       \
-  if (p.r <= 16) return run_tiles<T, TM, 16, TRANS>(who, p, max_new, st); \
-  if (p.r <= 32) return run_tiles<T, TM, 32, TRANS>(who, p, max_new, st); \
-  if (p.r <= 64) return run_tiles<T, TM, 64, TRANS>(who, p, max_new, st); \
-  return run_tiles<T, TM, 128, TRANS>(who, p, max_new, st);
-  if (max_new <= SMALL_ROWS) {
-    TA_RANK(16)
-  }
-  TA_RANK(64)
-#undef TA_RANK
+template <typename T, int RP>
+int run_fused(const char* who, ta::AdapterParams& p, int max_new, cudaStream_t st) {
+  using S = ta::AdapterShape<16, RP, false, true>;
+  static SmemAttr attr;
+  p.tiles = std::max(1, (int)(((int64_t)std::min(max_new, p.n_rows) + 15) / 16));
+  const int cs = cluster_size((int64_t)p.tiles * p.B, RP <= 32 ? 4 : RP == 64 ? 2 : 1, (std::max(p.K, p.N) + S::KC - 1) / S::KC, 1);
+  const dim3 grid((unsigned)(p.tiles * cs), p.B + (p.out == p.y ? 0 : 1));
+  return launch(who, ta::adapter_kernel<T, 16, RP, false, true>, attr, S::BYTES, grid, cs, st, p);
 }
+
+template <typename T, int RP, bool TRANS>
+int run_shrink(const char* who, ta::AdapterParams& p, int max_new, cudaStream_t st) {
+  using S = ta::AdapterShape<64, RP, TRANS, false>;
+  static SmemAttr attr;
+  if (p.B == 0) return TA_OK;
+  p.tiles = std::max(1, (int)(((int64_t)std::min(max_new, p.n_rows) + 63) / 64));
+  const int64_t items = (int64_t)p.tiles * p.B;
+  const int cs = cluster_size(items, 8, (p.K + S::KC - 1) / S::KC, 2);
+  return launch(who, ta::adapter_kernel<T, 64, RP, TRANS, false>, attr, S::BYTES, dim3((unsigned)(p.tiles * cs), p.B), cs, st, p);
+}
+
+template <typename T, int RP, bool TRANS>
+int run_expand(const char* who, ta::AdapterParams& p, int max_new, cudaStream_t st) {
+  using S = ta::ExpandShape<RP, TRANS>;
+  static SmemAttr attr;
+  p.tiles = std::max(1, (int)(((int64_t)std::min(max_new, p.n_rows) + ta::EXPAND_ROWS - 1) / ta::EXPAND_ROWS));
+  const int64_t x = (int64_t)p.tiles * ((p.N + ta::EXPAND_COLS - 1) / ta::EXPAND_COLS);
+  if (x > INT_MAX) return fail(TA_ERR_ARG, "%s: too many rows", who);
+  const dim3 grid((unsigned)x, p.B + (p.out == p.y ? 0 : 1));
+  if (grid.y == 0) return TA_OK;
+  return launch(who, ta::adapter_expand_kernel<T, RP, TRANS>, attr, S::BYTES, grid, 1, st, p);
+}
+
+// By the rank, filled up to 16, 32, 64 or 128.
+#define TA_BY_RANK(F, ...)                  \
+  (p.r <= 16   ? F<T, 16 __VA_ARGS__>(who, p, max_new, st) \
+   : p.r <= 32 ? F<T, 32 __VA_ARGS__>(who, p, max_new, st) \
+   : p.r <= 64 ? F<T, 64 __VA_ARGS__>(who, p, max_new, st) \
+               : F<T, 128 __VA_ARGS__>(who, p, max_new, st))
+
+template <typename T>
+int run_add(const char* who, ta::AdapterParams& p, int max_new, cudaStream_t st) {
+  if (max_new <= FUSED_ROWS) return TA_BY_RANK(run_fused);
+  if (int e = TA_BY_RANK(run_shrink, , false)) return e;
+  return TA_BY_RANK(run_expand, , false);
+}
+
+int run_bwd(const char* who, ta::AdapterParams& p, int max_new, cudaStream_t st) {
+  using T = __nv_bfloat16;
+  if (int e = TA_BY_RANK(run_shrink, , true)) return e;
+  return p.out ? TA_BY_RANK(run_expand, , true) : TA_OK;
+}
+#undef TA_BY_RANK
 
 template <int RP>
 int run_grad(const char* who, const ta::AdapterGradParams& p, cudaStream_t st) {
@@ -112,7 +143,8 @@ int ta_adapter_add(const void* y, int64_t y_sr, const void* x, int64_t x_sr, con
   if (!x || !y || !a || !b || !out) return fail(TA_ERR_ARG, "%s: null pointer", who);
   if (!rows_aligned(x, 2, {x_sr}) || !rows_aligned(y, 2, {y_sr}) || !rows_aligned(out, 2, {o_sr}) || !aligned16(a) || !aligned16(b))
     return fail(TA_ERR_ARG, "%s: rows and factors must be 16-byte aligned", who);
-  if (t && dtype != TA_BF16) return fail(TA_ERR_ARG, "%s: t is kept for bfloat16 only", who);
+  if (max_new > FUSED_ROWS && (!t || !aligned16(t)))
+    return fail(TA_ERR_ARG, "%s: where a sequence may have more than %d rows t is needed (16-byte aligned)", who, FUSED_ROWS);
   if (out == y && o_sr != y_sr) return fail(TA_ERR_ARG, "%s: out in y's place with other strides", who);
   ta::AdapterParams p{};
   p.x = x; p.y = y; p.out = out;
@@ -120,10 +152,11 @@ int ta_adapter_add(const void* y, int64_t y_sr, const void* x, int64_t x_sr, con
   p.u = a; p.v = b; p.scale = scale;
   p.start = start; p.which = which;
   p.n_rows = n_rows; p.B = B; p.K = K; p.N = N; p.r = r; p.n_adapters = n_adapters;
-  p.t_out = t;
+  p.t = t;
+  p.t_by = reinterpret_cast<float*>(reinterpret_cast<char*>(t) + (int64_t)n_rows * r * 4);
   if (B == 0 && out == y) return TA_OK;
-  if (dtype == TA_BF16) return run_adapter<__nv_bfloat16, false>(who, p, max_new, S(stream));
-  return run_adapter<__half, false>(who, p, max_new, S(stream));
+  if (dtype == TA_BF16) return run_add<__nv_bfloat16>(who, p, max_new, S(stream));
+  return run_add<__half>(who, p, max_new, S(stream));
 }
 
 int ta_adapter_bwd(const void* dy, int64_t d_sr, const void* x, int64_t x_sr, const void* a, const void* b, const float* scale,
@@ -138,15 +171,15 @@ int ta_adapter_bwd(const void* dy, int64_t d_sr, const void* x, int64_t x_sr, co
       !aligned16(b) || !aligned16(t) || !aligned16(u))
     return fail(TA_ERR_ARG, "%s: rows and factors must be 16-byte aligned", who);
   const cudaStream_t st = S(stream);
-  if ((dx || da) && n_rows > 0) {  // u = s dy B, dx = u A: the forward's kernel with the factors' other sides
+  if ((dx || da) && n_rows > 0) {  // u = s dy B, dx = u A: the forward's kernels with the factors' other sides
     ta::AdapterParams p{};
     p.x = dy; p.x_sr = d_sr;
     p.out = dx; p.o_sr = dx_sr;
     p.u = b; p.v = a; p.scale = scale;
     p.start = start; p.which = which;
-    p.n_rows = n_rows; p.B = B; p.K = N; p.N = dx ? K : 0; p.r = r; p.n_adapters = n_adapters;
-    p.t_out = da ? u : nullptr;
-    if (int e = run_adapter<__nv_bfloat16, true>(who, p, max_new, st)) return e;
+    p.n_rows = n_rows; p.B = B; p.K = N; p.N = K; p.r = r; p.n_adapters = n_adapters;
+    p.t = u;
+    if (int e = run_bwd(who, p, max_new, st)) return e;
   }
   if (!da && !db) return TA_OK;
   ta::AdapterGradParams p{};
