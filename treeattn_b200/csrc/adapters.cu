@@ -67,23 +67,23 @@ int cluster_size(int64_t items, int on_sm, int stages, int keep) {
 
 template <typename T, int RP>
 int run_fused(const char* who, ta::AdapterParams& p, int max_new, cudaStream_t st) {
-  using S = ta::AdapterShape<16, RP, false, true>;
+  using S = ta::AdapterShape<RP>;
   static SmemAttr attr;
   p.tiles = std::max(1, (int)(((int64_t)std::min(max_new, p.n_rows) + 15) / 16));
   const int cs = cluster_size((int64_t)p.tiles * p.B, RP <= 32 ? 4 : RP == 64 ? 2 : 1, (std::max(p.K, p.N) + S::KC - 1) / S::KC, 1);
   const dim3 grid((unsigned)(p.tiles * cs), p.B + (p.out == p.y ? 0 : 1));
-  return launch(who, ta::adapter_kernel<T, 16, RP, false, true>, attr, S::BYTES, grid, cs, st, p);
+  return launch(who, ta::adapter_kernel<T, RP>, attr, S::BYTES, grid, cs, st, p);
 }
 
 template <typename T, int RP, bool TRANS>
 int run_shrink(const char* who, ta::AdapterParams& p, int max_new, cudaStream_t st) {
-  using S = ta::AdapterShape<64, RP, TRANS, false>;
+  using S = ta::ShrinkShape<RP>;
   static SmemAttr attr;
   if (p.B == 0) return TA_OK;
-  p.tiles = std::max(1, (int)(((int64_t)std::min(max_new, p.n_rows) + 63) / 64));
-  const int64_t items = (int64_t)p.tiles * p.B;
-  const int cs = cluster_size(items, 8, (p.K + S::KC - 1) / S::KC, 2);
-  return launch(who, ta::adapter_kernel<T, 64, RP, TRANS, false>, attr, S::BYTES, dim3((unsigned)(p.tiles * cs), p.B), cs, st, p);
+  p.tiles = std::max(1, (int)(((int64_t)std::min(max_new, p.n_rows) + S::ROWS - 1) / S::ROWS));
+  // (a CTA's eight warps take 256 columns at a time)
+  const int cs = cluster_size((int64_t)p.tiles * p.B, RP == 16 ? 3 : RP <= 64 ? 2 : 1, (p.K + 255) / 256, 1);
+  return launch(who, ta::adapter_shrink_kernel<T, RP, TRANS>, attr, S::BYTES, dim3((unsigned)(p.tiles * cs), p.B), cs, st, p);
 }
 
 template <typename T, int RP, bool TRANS>
@@ -123,10 +123,11 @@ template <int RP>
 int run_grad(const char* who, const ta::AdapterGradParams& p, cudaStream_t st) {
   using S = ta::AdapterGradShape<RP>;
   static SmemAttr attr;
-  const int tiles = (p.da ? (p.K + ta::GRAD_MC - 1) / ta::GRAD_MC : 0) + (p.db ? (p.N + ta::GRAD_MC - 1) / ta::GRAD_MC : 0);
-  int cs = 1;
-  while (cs < 8 && (int64_t)tiles * p.n_adapters * cs < 4 * sm_count() && (int64_t)cs * 2 * ta::GRAD_ROWS <= p.n_rows) cs *= 2;
-  return launch(who, ta::adapter_grad_kernel<__nv_bfloat16, RP>, attr, S::BYTES, dim3(tiles * cs, p.n_adapters), cs, st, p);
+  const int tiles = (p.da ? (p.K + S::MC - 1) / S::MC : 0) + (p.db ? (p.N + S::MC - 1) / S::MC : 0);
+  const dim3 grid(tiles, p.n_adapters, (p.r + S::RT - 1) / S::RT);
+  // (a CTA's eight warps take 128 rows at a time)
+  const int cs = cluster_size((int64_t)tiles * grid.y * grid.z, 2, (p.n_rows + 127) / 128, 1);
+  return launch(who, ta::adapter_grad_kernel<__nv_bfloat16, RP>, attr, S::BYTES, dim3(tiles * cs, grid.y, grid.z), cs, st, p);
 }
 
 }  // namespace

@@ -5,7 +5,7 @@
 // tensor cores, so the kernels are bound by the rows' bytes (by latency where there are few rows). That is why they use the
 // warp-level matrix instruction, whose fragments come from rows of any length.
 // Few rows of a sequence (decoding) take one kernel for both products; many take two, t going by way of memory (64 bytes a row at rank
-// 16): its columns and the output's are then shared out over the GPU apart, and no CTA waits for another but to sum t.
+// 16): its columns and the output's are then shared out over the GPU apart.
 // t is held in fp32 and enters its product as two 16-bit numbers, high and low: 16 bits of it (22 in f16), so that the output's one
 // rounding is what is seen.
 #pragma once
@@ -83,28 +83,398 @@ template <> __device__ __forceinline__ uint32_t narrow2<__half>(float a, float b
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// The B operand's 16 x 16 block (k k0.., n n0..), from n-major rows (k contiguous) or, TR, from k-major ones. pitch in bytes.
-template <bool TR>
+// The B operand's 16 x 16 block (n n0.., k k0..) from rows by n with k contiguous; pitch in bytes.
 __device__ __forceinline__ void load_b(uint32_t (&b)[4], uint32_t base, int pitch, int n0, int k0, int lane) {
-  if (TR)
-    ldsm4t(b, base + (k0 + (lane & 15)) * pitch + (n0 + (lane >> 4) * 8) * 2);
-  else
-    ldsm4(b, base + (n0 + (lane >> 4) * 8 + (lane & 7)) * pitch + (k0 + ((lane >> 3) & 1) * 8) * 2);
+  ldsm4(b, base + (n0 + (lane >> 4) * 8 + (lane & 7)) * pitch + (k0 + ((lane >> 3) & 1) * 8) * 2);
 }
 
-template <int TM, int RP, bool TRANS, bool FUSED>
+// A warp's row m of t: summed over the cluster's parts (rows of RP), scaled, split into high and low parts. They go to p.t's row `row`
+// (unless there is none), and to shared memory where that is given.
+template <typename T, int RP>
+__device__ __forceinline__ void split_row(const AdapterParams& p, const float* part, int cs, int m, int row, float scale, int lane,
+                                          unsigned char* hi = nullptr, unsigned char* lo = nullptr, float* by_out = nullptr) {
+  constexpr int VL = (RP + 31) / 32;
+  float s[VL], top = 0.f, by = 1.f;
+#pragma unroll
+  for (int v = 0; v < VL; ++v) {
+    const int c = lane + 32 * v;
+    s[v] = 0.f;
+    if (c < RP) {
+      if (cs > 1)
+        for (int q = 0; q < cs; ++q) s[v] += cluster_map(part, q)[m * RP + c];
+      else
+        s[v] = part[m * RP + c];
+    }
+    s[v] *= scale;
+    top = fmaxf(top, fabsf(s[v]));
+  }
+  if constexpr (std::is_same<T, __half>::value) {
+    // f16: the row is brought near 1 by a power of two, since t may lie beyond f16's range and its low part below it
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    by = __uint_as_float(__float_as_uint(top) & 0x7f800000u);
+    if (by == 0.f || by == INFINITY) by = 1.f;
+#pragma unroll
+    for (int v = 0; v < VL; ++v) s[v] *= 1.f / by;
+    if (p.t && row >= 0 && lane == 0) p.t_by[row] = by;
+  }
+  if (by_out) *by_out = by;
+#pragma unroll
+  for (int v = 0; v < VL; ++v) {
+    const int c = lane + 32 * v;
+    if (c >= RP) break;
+    const T h = from_f32<T>(s[v]);
+    const float rest = s[v] - to_f32(h);
+    const T l = from_f32<T>(fabsf(to_f32(h)) < INFINITY ? rest : 0.f);
+    if (hi) {
+      reinterpret_cast<T*>(hi)[c] = h;
+      reinterpret_cast<T*>(lo)[c] = l;
+    }
+    if (p.t && row >= 0 && c < p.r) {
+      T* const to = reinterpret_cast<T*>(p.t) + (int64_t)row * p.r + c;
+      to[0] = h;
+      to[(int64_t)p.n_rows * p.r] = l;
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ few rows
+template <int RP>
 struct AdapterShape {
-  static constexpr int WM = TM / 16, WK = 8 / WM;              // warps by rows, and by columns
-  static constexpr int KC = TM == 16 || RP <= 32 ? 128 : 64;   // columns of x, and of the output, in a stage: 256 bytes of a row where
-                                                               // they fit (of 128 the memory gives two thirds as much a second)
-  static constexpr int STAGES = KC == 128 ? 3 : 4;
-  static constexpr int XP = KC * 2 + 16, RPP = RP * 2 + 16;    // pitches of rows by columns and by rank
-  static constexpr int F = TRANS ? KC * RPP : RP * XP;         // a stage's part of u, ...
-  static constexpr int G = !FUSED ? 0 : TRANS ? RP * XP : KC * RPP;  // ... and of v
-  static constexpr int STAGE = TM * XP + (F > G ? F : G);
-  static constexpr int PART = WK * TM * RP * 4;
-  static constexpr int BYTES = STAGES * STAGE + PART + (FUSED ? 2 * TM * RPP + TM * 4 : 0);
+  static constexpr int KC = 128;                             // columns of x, and of the output, in a stage
+  static constexpr int STAGES = 3;
+  static constexpr int XP = KC * 2 + 16, RPP = RP * 2 + 16;  // pitches of rows by columns and by rank
+  static constexpr int U = RP * XP, V = KC * RPP;            // a stage's part of the factors
+  static constexpr int STAGE = 16 * XP + (U > V ? U : V);
+  static constexpr int PART = 8 * 16 * RP * 4;
+  static constexpr int BYTES = STAGES * STAGE + PART + 2 * 16 * RPP + 16 * 4;
 };
+
+// Both products of 16 rows of a sequence by one cluster of CTAs. Each contracts a share of x's columns (its warps by sixteens); the partial
+// t meet through distributed shared memory, summed in the ranks' order by each CTA for itself, and each adds its share of the
+// output's columns. The stages of both halves go through one ring of asynchronous copies, so that the second half's first stages arrive
+// while t is summed. Bound by latency: @@.
+template <typename T, int RP>
+__global__ void __launch_bounds__(ADAPTER_THREADS, RP <= 32 ? 4 : RP == 64 ? 2 : 1)
+    adapter_kernel(const __grid_constant__ AdapterParams p) {
+  using S = AdapterShape<RP>;
+  extern __shared__ __align__(16) unsigned char smem[];
+  float* const part = reinterpret_cast<float*>(smem + S::STAGES * S::STAGE);
+  unsigned char* const hi = smem + S::STAGES * S::STAGE + S::PART;
+  unsigned char* const lo = hi + 16 * S::RPP;
+  float* const row_by = reinterpret_cast<float*>(lo + 16 * S::RPP);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int cs = cluster_nctarank(), rank = cluster_ctarank();
+  const int tile0 = blockIdx.x / cs, b = blockIdx.y;
+  const T* const X = reinterpret_cast<const T*>(p.x);
+  const T* const Y = reinterpret_cast<const T*>(p.y);
+  T* const O = reinterpret_cast<T*>(p.out);
+  pdl_wait();
+  pdl_launch_dependents();
+
+  auto plain = [&](int r0, int r1, bool nan) {  // rows as they are, or NaN
+    if (p.out == p.y && !nan) return;
+    const int pieces = p.N / 8;
+    for (int64_t i = (int64_t)blockIdx.x * ADAPTER_THREADS + tid; i < (int64_t)(r1 - r0) * pieces;
+         i += (int64_t)gridDim.x * ADAPTER_THREADS) {
+      const int64_t row = r0 + i / pieces;
+      const int c = (int)(i % pieces) * 8;
+      uint4 v = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
+      if (!nan) v = *reinterpret_cast<const uint4*>(Y + row * p.y_sr + c);
+      *reinterpret_cast<uint4*>(O + row * p.o_sr + c) = v;
+    }
+  };
+  auto bound = [&](int r) { return min(max(r, 0), p.n_rows); };
+  if (b == p.B) {  // rows of no sequence
+    plain(0, bound(p.start[0]), false);
+    plain(bound(p.start[p.B]), p.n_rows, false);
+    return;
+  }
+  const int r0 = bound(p.start[b]), r1 = bound(p.start[b + 1]);
+  const int a = p.which[b];
+  if (a < 0 || a >= p.n_adapters) {
+    if (a != -1 && blockIdx.x == 0 && tid == 0) record_error(DEV_INDEX_RANGE, K_ADAPTER, b, a);
+    plain(r0, r1, a != -1);
+    return;
+  }
+  const T* const U = reinterpret_cast<const T*>(p.u) + (int64_t)a * p.r * p.K;
+  const T* const V = reinterpret_cast<const T*>(p.v) + (int64_t)a * p.r * p.N;
+  const float scale = p.scale ? p.scale[a] : 1.f;
+  const int kc = (p.K + S::KC - 1) / S::KC, nc = (p.N + S::KC - 1) / S::KC;
+  const int k_first = kc * rank / cs, nk = kc * (rank + 1) / cs - k_first;
+  const int n_first = nc * rank / cs, nn = nc * (rank + 1) / cs - n_first;
+  const uint32_t ring_at = smem_u32(smem), hi_at = smem_u32(hi);
+  // a thread's pieces of a stage: a row's columns (16 of its 16 rows' 256 bytes), a column's ranks
+  constexpr int CH = S::KC / 8, RH = RP / 8, CI = ADAPTER_THREADS / RH;
+  static_assert(ADAPTER_THREADS / CH == 16, "a row of threads for each row");
+  const int pm = tid / CH, pc = tid % CH * 8, qm = tid / RH, qc = tid % RH * 8;
+  const uint32_t row_to = ring_at + pm * S::XP + pc * 2, col_to = ring_at + 16 * S::XP + qm * S::RPP + qc * 2;
+  const bool whole_rank = p.r == RP;
+
+  for (int row0 = r0 + tile0 * 16; row0 < r1; row0 += p.tiles * 16) {
+    const int rows = min(16, r1 - row0);
+    const T* const x_at = X + (int64_t)(row0 + pm) * p.x_sr + pc;
+    const T* const y_at = Y + (int64_t)(row0 + pm) * p.y_sr + pc;
+    auto issue = [&](int i) {
+      if (i < nk + nn) {
+        const bool first = i < nk;
+        const uint32_t stage = (i % S::STAGES) * S::STAGE;
+        const int c0 = (first ? k_first + i : n_first + i - nk) * S::KC, C = first ? p.K : p.N;
+        const bool cut = c0 + S::KC > C;  // the columns end in this stage: x's and u's are filled up with zeros, y's do not matter
+        if (pm < rows) {                  // (the places of rows that are not there keep what they hold)
+          const bool real = c0 + pc < C;
+          cp16(row_to + stage, real ? (first ? x_at : y_at) + c0 : X, real);
+        }
+        if (first) {
+          const T* const w = U + (int64_t)pm * C + c0 + pc;
+#pragma unroll
+          for (int q = 0; q < RP / 16; ++q) {
+            const bool real = pm + 16 * q < p.r && c0 + pc < C;
+            cp16(row_to + 16 * S::XP + stage + q * 16 * S::XP, real ? w + (int64_t)q * 16 * C : U, real);
+          }
+        } else {
+          const T* const w = V + (int64_t)(c0 + qm) * p.r + qc;
+          if (!cut && whole_rank) {
+#pragma unroll
+            for (int q = 0; q < (S::KC + CI - 1) / CI; ++q)
+              if (S::KC % CI == 0 || qm + q * CI < S::KC) cp16(col_to + stage + q * CI * S::RPP, w + q * CI * RP);
+          } else {
+            for (int q = 0; q < (S::KC + CI - 1) / CI; ++q) {
+              const bool real = qc < p.r && c0 + qm + q * CI < C;
+              if (qm + q * CI < S::KC) cp16(col_to + stage + q * CI * S::RPP, real ? w + (int64_t)q * CI * p.r : V, real);
+            }
+          }
+        }
+      }
+      cp_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < S::STAGES - 1; ++i) issue(i);
+
+    float acc[RP / 8][4];
+#pragma unroll
+    for (int n = 0; n < RP / 8; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
+    for (int i = 0; i < nk; ++i) {
+      cp_wait<S::STAGES - 2>();
+      __syncthreads();
+      issue(i + S::STAGES - 1);
+      const uint32_t xs = ring_at + (i % S::STAGES) * S::STAGE, us = xs + 16 * S::XP;
+      uint32_t xa[4];
+      ldsm4(xa, xs + (lane & 15) * S::XP + (warp * 16 + (lane >> 4) * 8) * 2);
+#pragma unroll
+      for (int n = 0; n < RP / 16; ++n) {
+        uint32_t ub[4];
+        load_b(ub, us, S::XP, n * 16, warp * 16, lane);
+        mma16<T>(acc[2 * n], xa, ub[0], ub[1]);
+        mma16<T>(acc[2 * n + 1], xa, ub[2], ub[3]);
+      }
+    }
+    // the warps' parts, the CTA's, the cluster's
+    {
+      float* const to = part + (warp * 16 + lane / 4) * RP + (lane & 3) * 2;
+#pragma unroll
+      for (int n = 0; n < RP / 8; ++n) {
+        *reinterpret_cast<float2*>(to + n * 8) = make_float2(acc[n][0], acc[n][1]);
+        *reinterpret_cast<float2*>(to + 8 * RP + n * 8) = make_float2(acc[n][2], acc[n][3]);
+      }
+    }
+    __syncthreads();
+    for (int i = tid; i < 16 * RP; i += ADAPTER_THREADS) {
+      float s = part[i];
+#pragma unroll
+      for (int w = 1; w < 8; ++w) s += part[w * 16 * RP + i];
+      part[i] = s;
+    }
+    if (cs > 1)
+      cluster_sync_all();
+    else
+      __syncthreads();
+    for (int m = warp; m < 16; m += 8) {
+      float by;
+      split_row<T, RP>(p, part, cs, m, m < rows && m % cs == rank ? row0 + m : -1, scale, lane, hi + m * S::RPP, lo + m * S::RPP, &by);
+      if (lane == 0) row_by[m] = by;
+    }
+    __syncwarp();
+    if (cs > 1) cluster_arrive();  // the others' parts have been read
+    const uint32_t t_at = hi_at + (lane & 15) * S::RPP + (lane >> 4) * 16;
+    for (int i = nk; i < nk + nn; ++i) {
+      cp_wait<S::STAGES - 2>();
+      __syncthreads();
+      issue(i + S::STAGES - 1);
+      unsigned char* const ys = smem + (i % S::STAGES) * S::STAGE;
+      const uint32_t y_at16 = smem_u32(ys) + (lane & 15) * S::XP + (warp * 16 + (lane >> 4) * 8) * 2, vs = smem_u32(ys) + 16 * S::XP;
+      // a warp's 16 columns
+      float o[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+      for (int kk = 0; kk < RP / 16; ++kk) {
+        uint32_t th[4], tl[4], vb[4];
+        ldsm4(th, t_at + kk * 32);
+        ldsm4(tl, t_at + 16 * S::RPP + kk * 32);
+        load_b(vb, vs, S::RPP, warp * 16, kk * 16, lane);
+        mma16<T>(o[0], th, vb[0], vb[1]);
+        mma16<T>(o[1], th, vb[2], vb[3]);
+        mma16<T>(o[0], tl, vb[0], vb[1]);
+        mma16<T>(o[1], tl, vb[2], vb[3]);
+      }
+      // added to y where it lies, rounded once; whole 16-byte pieces then leave
+      uint32_t y4[4];
+      ldsm4(y4, y_at16);
+      const float by[2] = {row_by[lane / 4], row_by[lane / 4 + 8]};
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        const float2 f = widen2<T>(y4[h]);
+        y4[h] = narrow2<T>(fmaf(o[h / 2][h % 2 * 2], by[h % 2], f.x), fmaf(o[h / 2][h % 2 * 2 + 1], by[h % 2], f.y));
+      }
+      stsm4(y_at16, y4);
+      __syncwarp();
+      const int m = lane / 2, c = warp * 16 + lane % 2 * 8, c0 = (n_first + i - nk) * S::KC;
+      if (m < rows && c0 + c < p.N)
+        *reinterpret_cast<uint4*>(O + (int64_t)(row0 + m) * p.o_sr + c0 + c) = *reinterpret_cast<const uint4*>(ys + m * S::XP + c * 2);
+    }
+    cp_wait<0>();
+    __syncthreads();
+    if (cs > 1) cluster_wait();
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ many rows
+// The three kernels below take their operands from memory straight into the fragments of the matrix instruction: the order of a sum's
+// terms and of an output's columns is free, and it is chosen so that a thread's share of a fragment is 16 consecutive bytes
+// of a row. Nothing passes through shared memory but the warps' sums at the end, and no warp waits for another before that.
+//   k of a 32-wide block: step s (0, 1), the fragment's pair (lane % 4 = j, half h) <-> elements 8 j + 4 s + 2 h, + 1
+//   columns of a 32-wide block: tile q (0 to 3), the fragment's pair j <-> columns 8 j + 2 q, + 1
+// Where a factor's rows run the other way an 8 x 8 block is turned in registers.
+__device__ __forceinline__ uint32_t turned(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+__device__ __forceinline__ uint32_t word(const uint2& v, int i) { return i == 0 ? v.x : v.y; }
+__device__ __forceinline__ uint4 load16(const void* p, bool real) {
+  return real ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0u, 0u, 0u, 0u);
+}
+__device__ __forceinline__ uint2 load8(const void* p, bool real) {
+  return real ? __ldg(reinterpret_cast<const uint2*>(p)) : make_uint2(0u, 0u);
+}
+
+template <int RP>
+struct ShrinkShape {
+  static constexpr int MT = RP <= 32 ? 2 : 1, ROWS = 16 * MT;  // rows of a CTA
+  static constexpr int BYTES = 8 * ROWS * RP * 4;
+};
+
+// t = s x U^T by itself: a CTA takes 16 or 32 rows, its warps (and the CTAs of a cluster) every so many blocks of 32 columns; their sums meet
+// in one order.
+template <typename T, int RP, bool TRANS>
+__global__ void __launch_bounds__(ADAPTER_THREADS, RP == 16 ? 3 : RP <= 64 ? 2 : 1) adapter_shrink_kernel(const __grid_constant__ AdapterParams p) {
+  using S = ShrinkShape<RP>;
+  constexpr int MT = S::MT, NT = RP / 8;
+  extern __shared__ __align__(16) float part[];  // (8, ROWS, RP)
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, i = lane >> 2, j = lane & 3;
+  const int cs = cluster_nctarank(), rank = cluster_ctarank();
+  const int tile0 = blockIdx.x / cs, b = blockIdx.y;
+  pdl_wait();
+  pdl_launch_dependents();
+  auto bound = [&](int r) { return min(max(r, 0), p.n_rows); };
+  const int r0 = bound(p.start[b]), r1 = bound(p.start[b + 1]);
+  const int a = p.which[b];
+  if (a < 0 || a >= p.n_adapters) {
+    if (a != -1 && blockIdx.x == 0 && tid == 0) record_error(DEV_INDEX_RANGE, K_ADAPTER, b, a);
+    return;
+  }
+  const T* const U = reinterpret_cast<const T*>(p.u) + (int64_t)a * p.r * p.K;
+  const float scale = p.scale ? p.scale[a] : 1.f;
+  const int blocks = (p.K + 31) / 32;
+  for (int row0 = r0 + tile0 * S::ROWS; row0 < r1; row0 += p.tiles * S::ROWS) {
+    const int rows = min(S::ROWS, r1 - row0);
+    const T* const x = reinterpret_cast<const T*>(p.x) + (int64_t)(row0 + i) * p.x_sr + 8 * j;
+    float acc[MT][NT][4];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[m][n][e] = 0.f;
+#pragma unroll 2
+    for (int kb = rank * 8 + warp; kb < blocks; kb += 8 * cs) {
+      const int k0 = kb * 32;
+      const bool in = k0 + 8 * j < p.K;
+      uint4 xv[MT][2];
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          xv[m][h] = load16(x + (int64_t)(16 * m + 8 * h) * p.x_sr + k0, in && 16 * m + 8 * h + i < rows);
+      uint32_t ub[2][2][NT];  // step, half, tile
+      if (!TRANS) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const uint4 u = load16(U + (int64_t)(8 * n + i) * p.K + k0 + 8 * j, in && 8 * n + i < p.r);
+          ub[0][0][n] = u.x; ub[0][1][n] = u.y; ub[1][0][n] = u.z; ub[1][1][n] = u.w;
+        }
+      } else {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int k = k0 + 8 * (i >> 1) + 4 * s + 2 * h + (i & 1);
+            const T* const row = U + (int64_t)k * p.r;
+            if (RP == 16) {
+              const uint2 u = load8(row + 4 * j, k < p.K && 4 * j < p.r);
+              ub[s][h][0] = turned(u.x);
+              ub[s][h][1] = turned(u.y);
+            } else {
+#pragma unroll
+              for (int g = 0; g < RP / 32; ++g) {
+                const uint4 u = load16(row + 32 * g + 8 * j, k < p.K && 32 * g + 8 * j < p.r);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) ub[s][h][4 * g + q] = turned(word(u, q));
+              }
+            }
+          }
+      }
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          const uint32_t xa[4] = {word(xv[m][0], 2 * s), word(xv[m][1], 2 * s), word(xv[m][0], 2 * s + 1), word(xv[m][1], 2 * s + 1)};
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma16<T>(acc[m][n], xa, ub[s][0][n], ub[s][1][n]);
+        }
+    }
+    // the warps' sums, the CTA's, the cluster's
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const int c = !TRANS ? 8 * n + 2 * j : RP == 16 ? 4 * j + 2 * n : 32 * (n / 4) + 8 * j + 2 * (n % 4);
+        float* const to = part + (warp * S::ROWS + 16 * m + i) * RP + c;
+        *reinterpret_cast<float2*>(to) = make_float2(acc[m][n][0], acc[m][n][1]);
+        *reinterpret_cast<float2*>(to + 8 * RP) = make_float2(acc[m][n][2], acc[m][n][3]);
+      }
+    __syncthreads();
+    for (int e = tid; e < S::ROWS * RP; e += ADAPTER_THREADS) {
+      float s = part[e];
+#pragma unroll
+      for (int w = 1; w < 8; ++w) s += part[w * S::ROWS * RP + e];
+      part[e] = s;
+    }
+    if (cs > 1)
+      cluster_sync_all();
+    else
+      __syncthreads();
+    for (int m = warp * cs + rank; m < rows; m += 8 * cs)
+      split_row<T, RP>(p, part, cs, m, row0 + m, scale, lane);
+    __syncwarp();
+    if (cs > 1)
+      cluster_sync_all();  // the others' parts have been read
+    else
+      __syncthreads();
+  }
+}
 
 // The output's 16 x 8 NT block of a warp, from y's tile at `tile` (pitch XP): t's rows times v, added, rounded once and written back there;
 // whole 16-byte pieces then leave for rows below `rows` and columns below `cols` of `out` (the CTA's corner).
@@ -144,7 +514,10 @@ __device__ __forceinline__ void add_product(unsigned char* tile, int xp, uint32_
 #pragma unroll
     for (int n = 0; n < NT / 2; ++n) {
       uint32_t vb[4];
-      load_b<TRANS>(vb, vs, vp, n0 + n * 16, kk * 16, lane);
+      if (TRANS)
+        ldsm4t(vb, vs + (kk * 16 + (lane & 15)) * vp + (n0 + n * 16 + (lane >> 4) * 8) * 2);
+      else
+        load_b(vb, vs, vp, n0 + n * 16, kk * 16, lane);
       mma16<T>(o[2 * n], th, vb[0], vb[1]);
       mma16<T>(o[2 * n + 1], th, vb[2], vb[3]);
       mma16<T>(o[2 * n], tl, vb[0], vb[1]);
@@ -169,246 +542,6 @@ __device__ __forceinline__ void add_product(unsigned char* tile, int xp, uint32_
     for (int q = 0; q < NT / 2; ++q)
       if (m + q * STEP < rows)
         *reinterpret_cast<uint4*>(out + (m + q * STEP) * o_sr + c) = *reinterpret_cast<const uint4*>(tile + (m + q * STEP) * xp + c * 2);
-  }
-}
-
-// A cluster of CTAs takes a tile of a sequence's rows. Each contracts a share of x's columns; the partial t meet through distributed
-// shared memory, summed in the ranks' order.
-// FUSED (tiles of 16 rows): each CTA sums t for itself and adds its share of the output's columns. The stages of both halves go through one
-// ring of asynchronous copies, so that the second half's first stages arrive while t is summed.
-// Otherwise (tiles of 64) each CTA sums and writes a share of t's rows.
-template <typename T, int TM, int RP, bool TRANS, bool FUSED>
-__global__ void __launch_bounds__(ADAPTER_THREADS, RP <= 32 ? (FUSED ? 4 : 3) : RP == 64 ? 2 : 1)
-    adapter_kernel(const __grid_constant__ AdapterParams p) {
-  using S = AdapterShape<TM, RP, TRANS, FUSED>;
-  extern __shared__ __align__(16) unsigned char smem[];
-  unsigned char* const ring = smem;
-  float* const part = reinterpret_cast<float*>(smem + S::STAGES * S::STAGE);
-  unsigned char* const hi = smem + S::STAGES * S::STAGE + S::PART;
-  unsigned char* const lo = hi + TM * S::RPP;
-  float* const row_by = reinterpret_cast<float*>(lo + TM * S::RPP);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int cs = cluster_nctarank(), rank = cluster_ctarank();
-  const int tile0 = blockIdx.x / cs, b = blockIdx.y;
-  const T* const X = reinterpret_cast<const T*>(p.x);
-  const T* const Y = reinterpret_cast<const T*>(p.y);
-  T* const O = reinterpret_cast<T*>(p.out);
-  pdl_wait();
-  pdl_launch_dependents();
-
-  // rows [r0, r1) as they are (y, or 0), or NaN
-  auto plain = [&](int r0, int r1, bool nan) {
-    if (!FUSED || (p.out == p.y && !nan)) return;
-    const int pieces = p.N / 8;
-    for (int64_t i = (int64_t)blockIdx.x * ADAPTER_THREADS + tid; i < (int64_t)(r1 - r0) * pieces;
-         i += (int64_t)gridDim.x * ADAPTER_THREADS) {
-      const int64_t row = r0 + i / pieces;
-      const int c = (int)(i % pieces) * 8;
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (nan) v = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
-      else if (Y) v = *reinterpret_cast<const uint4*>(Y + row * p.y_sr + c);
-      *reinterpret_cast<uint4*>(O + row * p.o_sr + c) = v;
-    }
-  };
-  auto bound = [&](int r) { return min(max(r, 0), p.n_rows); };
-  if (b == p.B) {  // rows of no sequence
-    plain(0, bound(p.start[0]), false);
-    plain(bound(p.start[p.B]), p.n_rows, false);
-    return;
-  }
-  const int r0 = bound(p.start[b]), r1 = bound(p.start[b + 1]);
-  const int a = p.which[b];
-  if (a < 0 || a >= p.n_adapters) {
-    if (a != -1 && blockIdx.x == 0 && tid == 0) record_error(DEV_INDEX_RANGE, K_ADAPTER, b, a);
-    plain(r0, r1, a != -1);
-    return;
-  }
-  const T* const U = reinterpret_cast<const T*>(p.u) + (int64_t)a * p.r * p.K;
-  const T* const V = reinterpret_cast<const T*>(p.v) + (int64_t)a * p.r * p.N;
-  const float scale = p.scale ? p.scale[a] : 1.f;
-  const int wm = warp % S::WM, wk = warp / S::WM;
-  const int kc = (p.K + S::KC - 1) / S::KC, nc = (p.N + S::KC - 1) / S::KC;
-  const int k_first = kc * rank / cs, nk = kc * (rank + 1) / cs - k_first;
-  const int n_first = nc * rank / cs, nn = FUSED ? nc * (rank + 1) / cs - n_first : 0;
-  const uint32_t ring_at = smem_u32(ring), hi_at = smem_u32(hi), lo_at = smem_u32(lo);
-  // a thread's pieces of a stage: of the rows, by columns; of a factor by rank (columns contiguous: u forward, v TRANS) or by column
-  constexpr int CH = S::KC / 8, RH = RP / 8, RI = ADAPTER_THREADS / CH, CI = ADAPTER_THREADS / RH;
-  const int pm = tid / CH, pc = tid % CH * 8, qm = tid / RH, qc = tid % RH * 8;
-  const uint32_t row_to = ring_at + pm * S::XP + pc * 2, col_to = ring_at + TM * S::XP + qm * S::RPP + qc * 2;
-  const bool whole_rank = p.r == RP;
-
-  for (int row0 = r0 + tile0 * TM; row0 < r1; row0 += p.tiles * TM) {
-    const int rows = min(TM, r1 - row0);
-    const int mine = (rows - pm + RI - 1) / RI;  // this thread's rows: pm, pm + RI, ... (the others' places keep what they hold)
-    const T* const x_at = X + (int64_t)(row0 + pm) * p.x_sr + pc;
-    const T* const y_at = Y ? Y + (int64_t)(row0 + pm) * p.y_sr + pc : nullptr;
-    auto issue = [&](int i) {
-      if (i < nk + nn) {
-        const bool first = i < nk;
-        const uint32_t stage = (i % S::STAGES) * S::STAGE;
-        const int c0 = (first ? k_first + i : n_first + i - nk) * S::KC, C = first ? p.K : p.N;
-        const bool cut = c0 + S::KC > C;  // the columns end in this stage: u's and x's are filled up with zeros, y's do not matter
-        const T* const from = (first ? x_at : y_at) + c0;
-        const int64_t sr = first ? p.x_sr : p.y_sr;
-        if (first || Y) {
-          if (!cut) {
-#pragma unroll
-            for (int q = 0; q < TM / RI; ++q)
-              if (q < mine) cp16(row_to + stage + q * RI * S::XP, from + q * RI * sr);
-          } else {
-            const bool real = c0 + pc < C;
-#pragma unroll
-            for (int q = 0; q < TM / RI; ++q)
-              if (q < mine) cp16(row_to + stage + q * RI * S::XP, real ? from + q * RI * sr : X, real);
-          }
-        }
-        const T* const W = first ? U : V;
-        if (first != TRANS) {
-          const T* const w = W + (int64_t)pm * C + c0 + pc;
-          if (!cut && whole_rank) {
-#pragma unroll
-            for (int q = 0; q < (RP + RI - 1) / RI; ++q)
-              if (RP % RI == 0 || pm + q * RI < RP) cp16(row_to + TM * S::XP + stage + q * RI * S::XP, w + (int64_t)q * RI * C);
-          } else {
-            for (int q = 0; q < (RP + RI - 1) / RI; ++q) {
-              const int m = pm + q * RI;
-              const bool real = m < p.r && c0 + pc < C;
-              if (m < RP) cp16(row_to + TM * S::XP + stage + q * RI * S::XP, real ? w + (int64_t)q * RI * C : W, real);
-            }
-          }
-        } else {
-          const T* const w = W + (int64_t)(c0 + qm) * p.r + qc;
-          if (!cut && whole_rank) {
-#pragma unroll
-            for (int q = 0; q < (S::KC + CI - 1) / CI; ++q)
-              if (S::KC % CI == 0 || qm + q * CI < S::KC) cp16(col_to + stage + q * CI * S::RPP, w + q * CI * RP);
-          } else {
-            for (int q = 0; q < (S::KC + CI - 1) / CI; ++q) {
-              const bool real = qc < p.r && c0 + qm + q * CI < C;
-              if (qm + q * CI < S::KC) cp16(col_to + stage + q * CI * S::RPP, real ? w + (int64_t)q * CI * p.r : W, real);
-            }
-          }
-        }
-      }
-      cp_commit();
-    };
-#pragma unroll
-    for (int i = 0; i < S::STAGES - 1; ++i) issue(i);
-
-    float acc[RP / 8][4];
-#pragma unroll
-    for (int n = 0; n < RP / 8; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
-    for (int i = 0; i < nk; ++i) {
-      cp_wait<S::STAGES - 2>();
-      __syncthreads();
-      issue(i + S::STAGES - 1);
-      const uint32_t xs = ring_at + (i % S::STAGES) * S::STAGE, us = xs + TM * S::XP;
-#pragma unroll
-      for (int kk = 0; kk < S::KC / 16 / S::WK; ++kk) {
-        const int k0 = (kk * S::WK + wk) * 16;
-        uint32_t xa[4];
-        ldsm4(xa, xs + (wm * 16 + (lane & 15)) * S::XP + (k0 + (lane >> 4) * 8) * 2);
-#pragma unroll
-        for (int n = 0; n < RP / 16; ++n) {
-          uint32_t ub[4];
-          load_b<TRANS>(ub, us, TRANS ? S::RPP : S::XP, n * 16, k0, lane);
-          mma16<T>(acc[2 * n], xa, ub[0], ub[1]);
-          mma16<T>(acc[2 * n + 1], xa, ub[2], ub[3]);
-        }
-      }
-    }
-    // the warps' parts, the CTA's, the cluster's
-    {
-      float* const to = part + wk * TM * RP;
-      const int m = wm * 16 + lane / 4, c = (lane & 3) * 2;
-#pragma unroll
-      for (int n = 0; n < RP / 8; ++n) {
-        *reinterpret_cast<float2*>(to + m * RP + n * 8 + c) = make_float2(acc[n][0], acc[n][1]);
-        *reinterpret_cast<float2*>(to + (m + 8) * RP + n * 8 + c) = make_float2(acc[n][2], acc[n][3]);
-      }
-    }
-    __syncthreads();
-    if (S::WK > 1) {
-      for (int i = tid; i < TM * RP; i += ADAPTER_THREADS) {
-        float s = part[i];
-#pragma unroll
-        for (int w = 1; w < S::WK; ++w) s += part[w * TM * RP + i];
-        part[i] = s;
-      }
-    }
-    if (cs > 1)
-      cluster_sync_all();
-    else
-      __syncthreads();
-    // a warp a row: t summed over the cluster, scaled, split into high and low parts
-    for (int m = FUSED ? warp : warp * cs + rank; m < TM; m += ADAPTER_THREADS / 32 * (FUSED ? 1 : cs)) {
-      constexpr int VL = (RP + 31) / 32;
-      float s[VL];
-      float top = 0.f;
-#pragma unroll
-      for (int j = 0; j < VL; ++j) {
-        const int c = lane + 32 * j;
-        s[j] = 0.f;
-        if (c < RP) {
-          if (cs > 1)
-            for (int q = 0; q < cs; ++q) s[j] += cluster_map(part, q)[m * RP + c];
-          else
-            s[j] = part[m * RP + c];
-        }
-        s[j] *= scale;
-        top = fmaxf(top, fabsf(s[j]));
-      }
-      if constexpr (std::is_same<T, __half>::value) {
-        // f16: the row is brought near 1 by a power of two, since t may lie beyond f16's range and its low part below it
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        float by = __uint_as_float(__float_as_uint(top) & 0x7f800000u);
-        if (by == 0.f || by == INFINITY) by = 1.f;
-        if (lane == 0) {
-          if (FUSED)
-            row_by[m] = by;
-          else if (m < rows)
-            p.t_by[row0 + m] = by;
-        }
-#pragma unroll
-        for (int j = 0; j < VL; ++j) s[j] *= 1.f / by;
-      }
-#pragma unroll
-      for (int j = 0; j < VL; ++j) {
-        const int c = lane + 32 * j;
-        if (c < RP) {
-          const T h = from_f32<T>(s[j]);
-          const float rest = s[j] - to_f32(h);
-          const T l = from_f32<T>(fabsf(to_f32(h)) < INFINITY ? rest : 0.f);
-          if (FUSED) {
-            *reinterpret_cast<T*>(hi + m * S::RPP + c * 2) = h;
-            *reinterpret_cast<T*>(lo + m * S::RPP + c * 2) = l;
-          }
-          if (p.t && (!FUSED || m % cs == rank) && m < rows && c < p.r) {
-            T* const to = reinterpret_cast<T*>(p.t) + (int64_t)(row0 + m) * p.r + c;
-            to[0] = h;
-            to[(int64_t)p.n_rows * p.r] = l;
-          }
-        }
-      }
-    }
-    __syncwarp();
-    if (cs > 1) cluster_arrive();  // the others' parts have been read
-    for (int i = nk; i < nk + nn; ++i) {
-      cp_wait<S::STAGES - 2>();
-      __syncthreads();
-      issue(i + S::STAGES - 1);
-      unsigned char* const ys = ring + (i % S::STAGES) * S::STAGE;
-      const int c0 = (n_first + i - nk) * S::KC;
-      constexpr int NT = S::KC / S::WK / 8;
-      add_product<T, RP, NT, TRANS>(ys, S::XP, smem_u32(ys) + TM * S::XP, TRANS ? S::XP : S::RPP, hi_at, lo_at, S::RPP, row_by, Y != nullptr,
-                                    wm * 16, wk * NT * 8, lane, O + (int64_t)row0 * p.o_sr + c0, p.o_sr, rows, p.N - c0);
-    }
-    cp_wait<0>();
-    __syncthreads();
-    if (cs > 1) cluster_wait();
   }
 }
 
@@ -509,170 +642,131 @@ struct AdapterGradParams {
   int n_rows, B, K, N, r, n_adapters;
 };
 
-constexpr int GRAD_MC = 64;     // columns of a CTA
-constexpr int GRAD_ROWS = 64;   // rows of a stage
-constexpr int GRAD_BATCH = 128; // sequences looked at together
-
 template <int RP>
 struct AdapterGradShape {
-  static constexpr int PP = GRAD_MC * 2 + 16, RPP = RP * 2 + 16;
-  static constexpr int STAGE = GRAD_ROWS * (PP + 2 * RPP);
-  static constexpr int STAGES = RP == 128 ? 3 : 4;
-  static constexpr int PART = 2 * GRAD_MC * RP * 4;
-  static constexpr int BYTES = STAGES * STAGE + PART;
+  static constexpr int RT = RP == 16 ? 16 : 32;   // ranks of a CTA
+  static constexpr int MC = RP == 16 ? 128 : 64;  // columns of a CTA
+  static constexpr int BYTES = 8 * MC * RT * 4;
 };
 
-// dA and dB: a CTA takes 64 columns of x or of dy and sums their products with u or t over the rows of all sequences that use its
-// adapter; a cluster shares those rows out and meets through distributed shared memory, in the ranks' order. An adapter that nobody
-// uses gets zeros.
+// dA and dB: a CTA takes 64 or 128 columns of x or of dy and up to 32 ranks, and sums the products of those columns with u or t over the rows of
+// all sequences that use its adapter. Its warps, and the CTAs of a cluster, take every so many blocks of 16 rows; their sums meet
+// in one order. An adapter that nobody uses gets zeros. Both operands run along the rows, so both are turned in registers.
 template <typename T, int RP>
-__global__ void __launch_bounds__(ADAPTER_THREADS, RP <= 32 ? 3 : 1) adapter_grad_kernel(const __grid_constant__ AdapterGradParams p) {
+__global__ void __launch_bounds__(ADAPTER_THREADS, 2) adapter_grad_kernel(const __grid_constant__ AdapterGradParams p) {
   using S = AdapterGradShape<RP>;
-  extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ int s_which[GRAD_BATCH], s_start[GRAD_BATCH + 1];
-  float* const part = reinterpret_cast<float*>(smem + S::STAGES * S::STAGE);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  constexpr int MC = S::MC, RT = S::RT, MT = MC / 16, NT = RT / 8;
+  extern __shared__ __align__(16) float part[];  // (8, MC, RT)
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, i = lane >> 2, j = lane & 3;
   const int cs = cluster_nctarank(), rank = cluster_ctarank();
-  const int a = blockIdx.y;
-  const int k_tiles = p.da ? (p.K + GRAD_MC - 1) / GRAD_MC : 0;
+  const int a = blockIdx.y, rank0 = blockIdx.z * RT;
+  const int k_tiles = p.da ? (p.K + MC - 1) / MC : 0;
   int c0 = (int)(blockIdx.x / cs);
   const bool of_a = c0 < k_tiles;
-  c0 = (of_a ? c0 : c0 - k_tiles) * GRAD_MC;
+  c0 = (of_a ? c0 : c0 - k_tiles) * MC;
   const int C = of_a ? p.K : p.N;
   const T* const R = reinterpret_cast<const T*>(of_a ? p.x : p.dy);
   const int64_t sr = of_a ? p.x_sr : p.d_sr;
   const T* const W = reinterpret_cast<const T*>(of_a ? p.u : p.t);
-  const uint32_t ring_at = smem_u32(smem);
-  const int wm = warp & 3, wk = warp >> 2;  // warps by columns, and by rows of a stage
   pdl_wait();
   pdl_launch_dependents();
-
-  // this CTA's next rows: (first, count), count 0 at the end. All threads walk alike.
-  int b = 0, row = 0, row_end = 0, turn = 0;
-  auto next = [&](int& first) {
-    while (true) {
-      while (row >= row_end) {
-        if (b >= p.B) return 0;
-        const int j = b % GRAD_BATCH;
-        if (j == 0) {
-          __syncthreads();
-          if (tid < GRAD_BATCH && b + tid < p.B) s_which[tid] = p.which[b + tid];
-          for (int i = tid; i < GRAD_BATCH + 1 && b + i <= p.B; i += ADAPTER_THREADS)
-            s_start[i] = min(max(p.start[b + i], 0), p.n_rows);
-          __syncthreads();
-        }
-        if (s_which[j] == a) {
-          row = s_start[j];
-          row_end = s_start[j + 1];
-        }
-        ++b;
-      }
-      first = row;
-      const int n = min(GRAD_ROWS, row_end - row);
-      row += GRAD_ROWS;
-      if (turn++ % cs == rank) return n;
+  float acc[MT][NT][4];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[m][n][e] = 0.f;
+  auto block = [&](int row0, int n_rows) {  // 16 rows, n_rows of them there
+    uint4 pv[MC / 32][2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const T* const from = R + (int64_t)(row0 + 8 * h + i) * sr + c0 + 8 * j;
+#pragma unroll
+      for (int g = 0; g < MC / 32; ++g) pv[g][h] = load16(from + 32 * g, 8 * h + i < n_rows && c0 + 32 * g + 8 * j < C);
     }
-  };
-  int issued = 0, taken = 0;
-  bool more = true;
-  // a thread's pieces of a stage
-  constexpr int CH = GRAD_MC / 8, RI = ADAPTER_THREADS / CH, RH = RP / 8, TI = ADAPTER_THREADS / RH;
-  const int pm = tid / CH, pc = tid % CH * 8, qm = tid / RH, qc = tid % RH * 8;
-  const uint32_t row_to = ring_at + pm * S::PP + pc * 2, t_to = ring_at + GRAD_ROWS * S::PP + qm * S::RPP + qc * 2;
-  const bool column = c0 + pc < C, whole = c0 + GRAD_MC <= C && p.r == RP;
-  const int64_t lo_step = (int64_t)p.n_rows * p.r;
-  auto issue = [&]() {
-    int first = 0;
-    const int n = more ? next(first) : 0;
-    more = n > 0;
-    if (more) {
-      const uint32_t stage = (issued % S::STAGES) * S::STAGE;
-      const T* const from = R + (int64_t)(first + pm) * sr + c0 + pc;
-      const T* const w = W + (int64_t)(first + qm) * p.r + qc;
-      if (n == GRAD_ROWS && whole) {
+    uint32_t tb[2][NT][2];  // high or low, tile, half
 #pragma unroll
-        for (int q = 0; q < GRAD_ROWS / RI; ++q) cp16(row_to + stage + q * RI * S::PP, from + q * RI * sr);
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int q = 0; q < (GRAD_ROWS + TI - 1) / TI; ++q)
-          if (GRAD_ROWS % TI == 0 || qm + q * TI < GRAD_ROWS) {
-            cp16(t_to + stage + q * TI * S::RPP, w + q * TI * RP);
-            cp16(t_to + stage + (GRAD_ROWS + q * TI) * S::RPP, w + q * TI * RP + lo_step);
-          }
-      } else {
-        for (int q = 0; q < GRAD_ROWS / RI; ++q) {
-          const bool real = pm + q * RI < n && column;
-          cp16(row_to + stage + q * RI * S::PP, real ? from + q * RI * sr : R, real);
-        }
-        for (int q = 0; q < (GRAD_ROWS + TI - 1) / TI; ++q) {
-          const bool real = qm + q * TI < min(n, GRAD_ROWS) && qc < p.r;
-          const T* const at = real ? w + (int64_t)q * TI * p.r : W;
-          if (qm + q * TI < GRAD_ROWS) {
-            cp16(t_to + stage + q * TI * S::RPP, at, real);
-            cp16(t_to + stage + (GRAD_ROWS + q * TI) * S::RPP, real ? at + lo_step : W, real);
-          }
+      for (int l = 0; l < 2; ++l) {
+        const T* const from = W + ((int64_t)l * p.n_rows + row0 + 8 * h + i) * p.r + rank0;
+        if (RT == 16) {
+          const uint2 x = load8(from + 4 * j, 8 * h + i < n_rows && rank0 + 4 * j < p.r);
+          tb[l][0][h] = turned(x.x);
+          tb[l][1][h] = turned(x.y);
+        } else {
+          const uint4 x = load16(from + 8 * j, 8 * h + i < n_rows && rank0 + 8 * j < p.r);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) tb[l][q][h] = turned(word(x, q));
         }
       }
-      ++issued;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {  // tiles 2 g and 2 g + 1 of a 32-wide block: its column pairs q = 0, 1 and 2, 3
+      const uint4 &x0 = pv[m / 2][0], &x1 = pv[m / 2][1];
+      const int q = m % 2 * 2;
+      const uint32_t pa[4] = {turned(word(x0, q)), turned(word(x0, q + 1)), turned(word(x1, q)), turned(word(x1, q + 1))};
+#pragma unroll
+      for (int l = 0; l < 2; ++l)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma16<T>(acc[m][n], pa, tb[l][n][0], tb[l][n][1]);
     }
-    cp_commit();
   };
-  float acc[RP / 8][4];
-#pragma unroll
-  for (int n = 0; n < RP / 8; ++n)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
-#pragma unroll
-  for (int i = 0; i < S::STAGES - 1; ++i) issue();
-  while (taken < issued) {
-    cp_wait<S::STAGES - 2>();
-    __syncthreads();
-    issue();
-    const uint32_t ps = ring_at + (taken % S::STAGES) * S::STAGE, ts = ps + GRAD_ROWS * S::PP;
-    ++taken;
-#pragma unroll
-    for (int kk = 0; kk < GRAD_ROWS / 32; ++kk) {
-      const int k0 = (kk * 2 + wk) * 16;
-      // the columns as the product's rows: 16 x 16 of the stage's rows (k) by columns (m), transposed
-      uint32_t pa[4];
-      ldsm4t(pa, ps + (k0 + (lane >> 4) * 8 + (lane & 7)) * S::PP + (wm * 16 + ((lane >> 3) & 1) * 8) * 2);
-#pragma unroll
-      for (int n = 0; n < RP / 16; ++n) {
-        uint32_t h[4], l[4];
-        load_b<true>(h, ts, S::RPP, n * 16, k0, lane);
-        load_b<true>(l, ts + GRAD_ROWS * S::RPP, S::RPP, n * 16, k0, lane);
-        mma16<T>(acc[2 * n], pa, h[0], h[1]);
-        mma16<T>(acc[2 * n + 1], pa, h[2], h[3]);
-        mma16<T>(acc[2 * n], pa, l[0], l[1]);
-        mma16<T>(acc[2 * n + 1], pa, l[2], l[3]);
+  {
+    // this warp's blocks of 16 rows: every (8 cs)th of the adapter's, sequence after sequence
+    const int turns = 8 * cs;
+    int turn = rank * 8 + warp;  // blocks until the next one of this warp's
+    for (int b0 = 0; b0 < p.B; b0 += 32) {
+      const int b = b0 + lane;
+      int s0 = 0, s1 = 0;
+      if (b < p.B && p.which[b] == a) {
+        s0 = min(max(p.start[b], 0), p.n_rows);
+        s1 = min(max(p.start[b + 1], 0), p.n_rows);
+      }
+      uint32_t some = __ballot_sync(0xffffffffu, s1 > s0);
+      while (some) {
+        const int from = __ffs(some) - 1;
+        some &= some - 1;
+        const int q0 = __shfl_sync(0xffffffffu, s0, from), q1 = __shfl_sync(0xffffffffu, s1, from);
+        const int n = (q1 - q0 + 15) / 16;
+        for (; turn < n; turn += turns) block(q0 + turn * 16, q1 - q0 - turn * 16);
+        turn -= n;
       }
     }
   }
-  {
-    const int m = wk * GRAD_MC + wm * 16 + lane / 4, c = (lane & 3) * 2;
 #pragma unroll
-    for (int n = 0; n < RP / 8; ++n) {
-      *reinterpret_cast<float2*>(part + m * RP + n * 8 + c) = make_float2(acc[n][0], acc[n][1]);
-      *reinterpret_cast<float2*>(part + (m + 8) * RP + n * 8 + c) = make_float2(acc[n][2], acc[n][3]);
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      // the fragment's row i is column 32 (m / 2) + 8 (i / 2) + 4 (m % 2) + i % 2 of the CTA's, its row i + 8 two further
+      const int mm = 32 * (m / 2) + 8 * (i >> 1) + 4 * (m % 2) + (i & 1);
+      const int c = RT == 16 ? 4 * j + 2 * n : 8 * j + 2 * n;
+      float* const to = part + (warp * MC + mm) * RT + c;
+      *reinterpret_cast<float2*>(to) = make_float2(acc[m][n][0], acc[m][n][1]);
+      *reinterpret_cast<float2*>(to + 2 * RT) = make_float2(acc[m][n][2], acc[m][n][3]);
     }
+  __syncthreads();
+  for (int e = tid; e < MC * RT; e += ADAPTER_THREADS) {
+    float s = part[e];
+#pragma unroll
+    for (int w = 1; w < 8; ++w) s += part[w * MC * RT + e];
+    part[e] = s;
   }
   if (cs > 1)
     cluster_sync_all();
   else
     __syncthreads();
   // each CTA finishes a share of the columns: dA as [r][K], dB as [N][r]
-  const int m0 = GRAD_MC * rank / cs, m1 = GRAD_MC * (rank + 1) / cs, per = m1 - m0;
-  for (int i = tid; i < per * p.r; i += ADAPTER_THREADS) {
-    const int m = m0 + (of_a ? i % per : i / p.r), c = of_a ? i / per : i % p.r;
+  const int m0 = MC * rank / cs, m1 = MC * (rank + 1) / cs, per = m1 - m0, ranks = min(RT, p.r - rank0);
+  for (int e = tid; e < per * ranks; e += ADAPTER_THREADS) {
+    const int m = m0 + (of_a ? e % per : e / ranks), c = of_a ? e / per : e % ranks;
     float s = 0.f;
-    for (int q = 0; q < cs; ++q) {
-      const float* const from = (cs > 1 ? cluster_map(part, q) : part) + m * RP + c;
-      s += from[0] + from[GRAD_MC * RP];
-    }
+    for (int q = 0; q < cs; ++q) s += (cs > 1 ? cluster_map(part, q) : part)[m * RT + c];
     if (c0 + m < C) {
       if (of_a)
-        reinterpret_cast<T*>(p.da)[((int64_t)a * p.r + c) * p.K + c0 + m] = from_f32<T>(s);
+        reinterpret_cast<T*>(p.da)[((int64_t)a * p.r + rank0 + c) * p.K + c0 + m] = from_f32<T>(s);
       else
-        reinterpret_cast<T*>(p.db)[((int64_t)a * p.N + c0 + m) * p.r + c] = from_f32<T>(s);
+        reinterpret_cast<T*>(p.db)[((int64_t)a * p.N + c0 + m) * p.r + rank0 + c] = from_f32<T>(s);
     }
   }
   __syncwarp();
