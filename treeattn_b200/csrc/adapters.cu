@@ -81,8 +81,7 @@ int run_shrink(const char* who, ta::AdapterParams& p, int max_new, cudaStream_t 
   static SmemAttr attr;
   if (p.B == 0) return TA_OK;
   p.tiles = std::max(1, (int)(((int64_t)std::min(max_new, p.n_rows) + S::ROWS - 1) / S::ROWS));
-  // (a CTA's eight warps take 256 columns at a time)
-  const int cs = cluster_size((int64_t)p.tiles * p.B, RP == 16 ? 3 : RP <= 64 ? 2 : 1, (p.K + 255) / 256, 1);
+  const int cs = cluster_size((int64_t)p.tiles * p.B, RP == 16 ? 4 : RP == 32 ? 3 : 2, (p.K + 32 * S::KS - 1) / (32 * S::KS), 1);
   return launch(who, ta::adapter_shrink_kernel<T, RP, TRANS>, attr, S::BYTES, dim3((unsigned)(p.tiles * cs), p.B), cs, st, p);
 }
 

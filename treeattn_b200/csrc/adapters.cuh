@@ -362,18 +362,20 @@ __device__ __forceinline__ uint2 load8(const void* p, bool real) {
 
 template <int RP>
 struct ShrinkShape {
-  static constexpr int MT = RP <= 32 ? 2 : 1, ROWS = 16 * MT;  // rows of a CTA
-  static constexpr int BYTES = 8 * ROWS * RP * 4;
+  static constexpr int G = RP == 16 ? 1 : RP / 32, KS = 8 / G;      // warps by ranks (at most 32 each), and by columns
+  static constexpr int MT = RP <= 32 ? 2 : 4, ROWS = 16 * MT;       // rows of a CTA: more where a factor's row weighs more
+  static constexpr int BYTES = KS * ROWS * RP * 4;
 };
 
-// t = s x U^T by itself: a CTA takes 16 or 32 rows, its warps (and the CTAs of a cluster) every so many blocks of 32 columns; their sums meet
-// in one order.
+// t = s x U^T by itself: a CTA takes 32 or 64 rows, its warps (and the CTAs of a cluster) 32 ranks each and every so many blocks of 32
+// columns; their sums meet in one order.
 template <typename T, int RP, bool TRANS>
-__global__ void __launch_bounds__(ADAPTER_THREADS, RP == 16 ? 3 : RP <= 64 ? 2 : 1) adapter_shrink_kernel(const __grid_constant__ AdapterParams p) {
+__global__ void __launch_bounds__(ADAPTER_THREADS, RP == 16 ? 4 : RP == 32 ? 3 : 2) adapter_shrink_kernel(const __grid_constant__ AdapterParams p) {
   using S = ShrinkShape<RP>;
-  constexpr int MT = S::MT, NT = RP / 8;
-  extern __shared__ __align__(16) float part[];  // (8, ROWS, RP)
+  constexpr int MT = S::MT, NT = RP / 8 / S::G;
+  extern __shared__ __align__(16) float part[];  // (KS, ROWS, RP)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, i = lane >> 2, j = lane & 3;
+  const int rank0 = warp % S::G * 32, ks = warp / S::G;  // the warp's first rank
   const int cs = cluster_nctarank(), rank = cluster_ctarank();
   const int tile0 = blockIdx.x / cs, b = blockIdx.y;
   pdl_wait();
@@ -398,8 +400,8 @@ __global__ void __launch_bounds__(ADAPTER_THREADS, RP == 16 ? 3 : RP <= 64 ? 2 :
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[m][n][e] = 0.f;
-#pragma unroll 2
-    for (int kb = rank * 8 + warp; kb < blocks; kb += 8 * cs) {
+#pragma unroll 1
+    for (int kb = rank * S::KS + ks; kb < blocks; kb += S::KS * cs) {
       const int k0 = kb * 32;
       const bool in = k0 + 8 * j < p.K;
       uint4 xv[MT][2];
@@ -412,7 +414,8 @@ __global__ void __launch_bounds__(ADAPTER_THREADS, RP == 16 ? 3 : RP <= 64 ? 2 :
       if (!TRANS) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          const uint4 u = load16(U + (int64_t)(8 * n + i) * p.K + k0 + 8 * j, in && 8 * n + i < p.r);
+          const int c = rank0 + 8 * n + i;
+          const uint4 u = load16(U + (int64_t)c * p.K + k0 + 8 * j, in && c < p.r);
           ub[0][0][n] = u.x; ub[0][1][n] = u.y; ub[1][0][n] = u.z; ub[1][1][n] = u.w;
         }
       } else {
@@ -421,18 +424,15 @@ __global__ void __launch_bounds__(ADAPTER_THREADS, RP == 16 ? 3 : RP <= 64 ? 2 :
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int k = k0 + 8 * (i >> 1) + 4 * s + 2 * h + (i & 1);
-            const T* const row = U + (int64_t)k * p.r;
+            const T* const row = U + (int64_t)k * p.r + rank0;
             if (RP == 16) {
               const uint2 u = load8(row + 4 * j, k < p.K && 4 * j < p.r);
               ub[s][h][0] = turned(u.x);
               ub[s][h][1] = turned(u.y);
             } else {
+              const uint4 u = load16(row + 8 * j, k < p.K && rank0 + 8 * j < p.r);
 #pragma unroll
-              for (int g = 0; g < RP / 32; ++g) {
-                const uint4 u = load16(row + 32 * g + 8 * j, k < p.K && 32 * g + 8 * j < p.r);
-#pragma unroll
-                for (int q = 0; q < 4; ++q) ub[s][h][4 * g + q] = turned(word(u, q));
-              }
+              for (int q = 0; q < NT; ++q) ub[s][h][q] = turned(word(u, q));
             }
           }
       }
@@ -450,8 +450,8 @@ __global__ void __launch_bounds__(ADAPTER_THREADS, RP == 16 ? 3 : RP <= 64 ? 2 :
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const int c = !TRANS ? 8 * n + 2 * j : RP == 16 ? 4 * j + 2 * n : 32 * (n / 4) + 8 * j + 2 * (n % 4);
-        float* const to = part + (warp * S::ROWS + 16 * m + i) * RP + c;
+        const int c = rank0 + (!TRANS ? 8 * n + 2 * j : RP == 16 ? 4 * j + 2 * n : 8 * j + 2 * n);
+        float* const to = part + (ks * S::ROWS + 16 * m + i) * RP + c;
         *reinterpret_cast<float2*>(to) = make_float2(acc[m][n][0], acc[m][n][1]);
         *reinterpret_cast<float2*>(to + 8 * RP) = make_float2(acc[m][n][2], acc[m][n][3]);
       }
@@ -459,7 +459,7 @@ __global__ void __launch_bounds__(ADAPTER_THREADS, RP == 16 ? 3 : RP <= 64 ? 2 :
     for (int e = tid; e < S::ROWS * RP; e += ADAPTER_THREADS) {
       float s = part[e];
 #pragma unroll
-      for (int w = 1; w < 8; ++w) s += part[w * S::ROWS * RP + e];
+      for (int w = 1; w < S::KS; ++w) s += part[w * S::ROWS * RP + e];
       part[e] = s;
     }
     if (cs > 1)
@@ -645,7 +645,7 @@ struct AdapterGradParams {
 template <int RP>
 struct AdapterGradShape {
   static constexpr int RT = RP == 16 ? 16 : 32;   // ranks of a CTA
-  static constexpr int MC = RP == 16 ? 128 : 64;  // columns of a CTA
+  static constexpr int MC = 64;                   // columns of a CTA
   static constexpr int BYTES = 8 * MC * RT * 4;
 };
 
@@ -677,33 +677,38 @@ __global__ void __launch_bounds__(ADAPTER_THREADS, 2) adapter_grad_kernel(const 
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[m][n][e] = 0.f;
-  auto block = [&](int row0, int n_rows) {  // 16 rows, n_rows of them there
-    uint4 pv[MC / 32][2];
+  struct Rows {  // a thread's share of 16 rows: of the columns, of t's high and low parts
+    uint4 p[MC / 32][2], t[2][2];
+  };
+  auto load = [&](Rows& v, int row0, int n_rows) {  // n_rows of them there
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const T* const from = R + (int64_t)(row0 + 8 * h + i) * sr + c0 + 8 * j;
 #pragma unroll
-      for (int g = 0; g < MC / 32; ++g) pv[g][h] = load16(from + 32 * g, 8 * h + i < n_rows && c0 + 32 * g + 8 * j < C);
-    }
-    uint32_t tb[2][NT][2];  // high or low, tile, half
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
+      for (int g = 0; g < MC / 32; ++g) v.p[g][h] = load16(from + 32 * g, 8 * h + i < n_rows && c0 + 32 * g + 8 * j < C);
 #pragma unroll
       for (int l = 0; l < 2; ++l) {
-        const T* const from = W + ((int64_t)l * p.n_rows + row0 + 8 * h + i) * p.r + rank0;
+        const T* const of = W + ((int64_t)l * p.n_rows + row0 + 8 * h + i) * p.r + rank0;
         if (RT == 16) {
-          const uint2 x = load8(from + 4 * j, 8 * h + i < n_rows && rank0 + 4 * j < p.r);
-          tb[l][0][h] = turned(x.x);
-          tb[l][1][h] = turned(x.y);
+          const uint2 x = load8(of + 4 * j, 8 * h + i < n_rows && rank0 + 4 * j < p.r);
+          v.t[l][h] = make_uint4(x.x, x.y, 0u, 0u);
         } else {
-          const uint4 x = load16(from + 8 * j, 8 * h + i < n_rows && rank0 + 8 * j < p.r);
-#pragma unroll
-          for (int q = 0; q < 4; ++q) tb[l][q][h] = turned(word(x, q));
+          v.t[l][h] = load16(of + 8 * j, 8 * h + i < n_rows && rank0 + 8 * j < p.r);
         }
       }
+    }
+  };
+  auto multiply = [&](const Rows& v) {
+    uint32_t tb[2][NT][2];  // high or low, tile, half
+#pragma unroll
+    for (int l = 0; l < 2; ++l)
+#pragma unroll
+      for (int q = 0; q < NT; ++q)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) tb[l][q][h] = turned(word(v.t[l][h], q));
 #pragma unroll
     for (int m = 0; m < MT; ++m) {  // tiles 2 g and 2 g + 1 of a 32-wide block: its column pairs q = 0, 1 and 2, 3
-      const uint4 &x0 = pv[m / 2][0], &x1 = pv[m / 2][1];
+      const uint4 &x0 = v.p[m / 2][0], &x1 = v.p[m / 2][1];
       const int q = m % 2 * 2;
       const uint32_t pa[4] = {turned(word(x0, q)), turned(word(x0, q + 1)), turned(word(x1, q)), turned(word(x1, q + 1))};
 #pragma unroll
@@ -716,6 +721,8 @@ __global__ void __launch_bounds__(ADAPTER_THREADS, 2) adapter_grad_kernel(const 
     // this warp's blocks of 16 rows: every (8 cs)th of the adapter's, sequence after sequence
     const int turns = 8 * cs;
     int turn = rank * 8 + warp;  // blocks until the next one of this warp's
+    Rows v, w;                   // 16 ranks: the block before, multiplied while the next one arrives (with 32 both do not fit)
+    bool held = false;
     for (int b0 = 0; b0 < p.B; b0 += 32) {
       const int b = b0 + lane;
       int s0 = 0, s1 = 0;
@@ -729,10 +736,21 @@ __global__ void __launch_bounds__(ADAPTER_THREADS, 2) adapter_grad_kernel(const 
         some &= some - 1;
         const int q0 = __shfl_sync(0xffffffffu, s0, from), q1 = __shfl_sync(0xffffffffu, s1, from);
         const int n = (q1 - q0 + 15) / 16;
-        for (; turn < n; turn += turns) block(q0 + turn * 16, q1 - q0 - turn * 16);
+        for (; turn < n; turn += turns) {
+          if constexpr (RT == 16) {
+            load(w, q0 + turn * 16, q1 - q0 - turn * 16);
+            if (held) multiply(v);
+            v = w;
+            held = true;
+          } else {
+            load(v, q0 + turn * 16, q1 - q0 - turn * 16);
+            multiply(v);
+          }
+        }
         turn -= n;
       }
     }
+    if (RT == 16 && held) multiply(v);
   }
 #pragma unroll
   for (int m = 0; m < MT; ++m)
