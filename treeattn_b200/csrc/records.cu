@@ -126,7 +126,15 @@ int make_plan(Plan& p, const int32_t* src, const int32_t* dst, int n, int n_reco
     }
   for (int i = 0; i < n; ++i)
     if (src[i] != dst[i]) (next[i] < 0 && waits[i] == 0 ? alone : bound).push_back(i);
-  std::stable_sort(alone.begin(), alone.end(), [&](int x, int y) { return src[x] < src[y]; });
+  // those that read one record follow one another
+  bool again = false;
+  std::vector<char> seen(dense ? n_records : 0, 0);
+  if (dense)
+    for (int i : alone) {
+      again |= seen[src[i]] != 0;
+      seen[src[i]] = 1;
+    }
+  if (again || !dense) std::stable_sort(alone.begin(), alone.end(), [&](int x, int y) { return src[x] < src[y]; });
   for (size_t i = 0; i < alone.size(); ++i) {
     if (i % BATCH == 0) p.open();
     p.add(src[alone[i]], dst[alone[i]]);

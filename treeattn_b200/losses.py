@@ -17,38 +17,37 @@ _V4 = ctypes.c_void_p * 4
 _L8 = ctypes.c_int64 * 8
 
 
-def _logits(name, logits, tokens, temperature):
-    """Checks logits (..., V) and tokens (...): (logits' strides, tokens' strides, b, t, V), with one or two leading dims as two."""
-    if logits.dtype not in _DT:
+def _logits(name, logits, tokens):
+    """Checks logits (..., V) and tokens (...); returns what the entry points ask about them, one or two leading dims as two: (address,
+    type, strides (2), b, t, V, the tokens' address and strides (2))."""
+    code = _DT.get(logits.dtype)
+    if code is None:
         raise TypeError('%s: logits must be float32, bfloat16 or float16 (got %s)' % (name, logits.dtype))
-    if logits.dim() not in (2, 3):
+    shape, s, t = logits.shape, logits.stride(), tokens.stride()
+    if len(shape) not in (2, 3):
         raise ValueError('%s: logits must be (rows, vocabulary) or (batch, rows, vocabulary)' % name)
-    if logits.shape[-1] < 1 or logits.stride(-1) != 1:
+    if shape[-1] < 1 or s[-1] != 1:
         raise ValueError('%s: the innermost (vocabulary) dimension must be contiguous' % name)
-    if tokens.dtype is not torch.int64 or tokens.shape != logits.shape[:-1]:
-        raise ValueError('%s: tokens must be %s int64' % (name, tuple(logits.shape[:-1])))
-    _need_cuda(name, logits, tokens)
-    _same_device(name, logits, tokens)
-    s, t = logits.stride(), tokens.stride()
-    if logits.dim() == 3:
-        return (s[0], s[1]), (t[0], t[1]), logits.shape[0], logits.shape[1], logits.shape[2]
-    return (0, s[0]), (0, t[0]), 1, logits.shape[0], logits.shape[1]
-
-
-def _same_device(name, first, *rest):
-    for t in rest:
-        if t is not None and t.get_device() != first.get_device():
-            raise ValueError('%s: tensors on one device (got %s and %s)' % (name, first.device, t.device))
+    if tokens.dtype is not torch.int64 or tokens.shape != shape[:-1]:
+        raise ValueError('%s: tokens must be %s int64' % (name, tuple(shape[:-1])))
+    dev = logits.get_device()
+    if dev < 0 or tokens.get_device() != dev:
+        _need_cuda(name, logits, tokens)
+        raise ValueError('%s: tensors on one device (got %s and %s)' % (name, logits.device, tokens.device))
+    if len(shape) == 3:
+        return (logits.data_ptr(), code, s[0], s[1], shape[0], shape[1], shape[2], tokens.data_ptr(), t[0], t[1])
+    return (logits.data_ptr(), code, 0, s[0], 1, shape[0], shape[1], tokens.data_ptr(), 0, t[0])
 
 
 def _by_row(name, what, v, like):
     """Checks a float32 tensor by row and returns its strides."""
     if v.dtype is not torch.float32 or v.shape != like.shape:
         raise ValueError('%s: %s must be %s float32' % (name, what, tuple(like.shape)))
-    _need_cuda(name, v)
-    _same_device(name, like, v)
+    if v.get_device() != like.get_device():
+        _need_cuda(name, v)
+        raise ValueError('%s: tensors on one device (got %s and %s)' % (name, like.device, v.device))
     s = v.stride()
-    return (s[0], s[1]) if v.dim() == 2 else (0, s[0])
+    return s if len(s) == 2 else (0, s[0])
 
 
 def _grad_like(logits):
@@ -67,23 +66,20 @@ def _grad_strides(g):
     return (s[0], s[1]) if g.dim() == 3 else (0, s[0])
 
 
-def _logits_grad(logits, tokens, stats, slope, ss, by, temperature, up, unit_done, grad):
-    zs, ts, b, t, V = _logits('logits_grad', logits, tokens, temperature)
+def _logits_grad(logits, of, stats, slope, ss, by, temperature, up, unit_done, grad):
     gs = _grad_strides(grad)
     with _on(logits):
-        _call('ta_logits_grad', logits.data_ptr(), _DT[logits.dtype], zs[0], zs[1], b, t, V, tokens.data_ptr(), ts[0], ts[1],
-              stats.data_ptr(), slope if isinstance(slope, int) else slope.data_ptr(), ss[0], ss[1], by, temperature,
-              None if up is None else up.data_ptr(), int(unit_done), grad.data_ptr(), gs[0], gs[1], _stream(logits))
+        _call('ta_logits_grad', *of, stats.data_ptr(), slope, ss[0], ss[1], by, temperature, None if up is None else up.data_ptr(),
+              int(unit_done), grad.data_ptr(), gs[0], gs[1], _stream(logits))
 
 
 # ------------------------------------------------------------------------------------------------ log-probabilities
 def _token_logp(logits, tokens, temperature):
-    zs, ts, b, t, V = _logits('token_logp', logits, tokens, temperature)
+    of = _logits('token_logp', logits, tokens)
     logp = torch.empty(tokens.shape, device=logits.device, dtype=torch.float32)
-    stats = torch.empty(2, b * t, device=logits.device, dtype=torch.float32)  # the rows' maxima and sums
+    stats = torch.empty(2, of[4] * of[5], device=logits.device, dtype=torch.float32)  # the rows' references and sums
     with _on(logits):
-        _call('ta_token_logp', logits.data_ptr(), _DT[logits.dtype], zs[0], zs[1], b, t, V, tokens.data_ptr(), ts[0], ts[1],
-              temperature, logp.data_ptr(), stats.data_ptr(), _stream(logits))
+        _call('ta_token_logp', *of, temperature, logp.data_ptr(), stats.data_ptr(), _stream(logits))
     return logp, stats
 
 
@@ -101,8 +97,8 @@ class _TokenLogp(torch.autograd.Function):
         logits, tokens, stats = ctx.saved_tensors
         grad = _grad_like(logits)
         s = dlogp.stride()
-        _logits_grad(logits, tokens, stats, dlogp, (s[0], s[1]) if dlogp.dim() == 2 else (0, s[0]), 1.0 / ctx.temperature,
-                     ctx.temperature, None, False, grad)
+        _logits_grad(logits, _logits('token_logp', logits, tokens), stats, dlogp.data_ptr(), s if len(s) == 2 else (0, s[0]), 1.0 / ctx.temperature, ctx.temperature, None,
+                     False, grad)
         return grad, None, None
 
 
@@ -117,23 +113,29 @@ def token_logp(logits, tokens, temperature=1.0):
 
 
 # ------------------------------------------------------------------------------------------------ policy loss
-def _policy(logits, tokens, old_logp, advantages, ref_logp, weight, clip, kl, temperature, grad):
+def _policy(logits, tokens, old_logp, advantages, ref_logp, weight, clip, kl, temperature, with_grad):
     name = 'policy_loss'
-    zs, ts, b, t, V = _logits(name, logits, tokens, temperature)
-    ptrs, strides = [], []
-    for what, v in (('old_logp', old_logp), ('advantages', advantages), ('ref_logp', ref_logp), ('weight', weight)):
-        strides += (0, 0) if v is None else _by_row(name, what, v, tokens)
-        ptrs.append(None if v is None else v.data_ptr())
-    dev, n = logits.device, b * t
+    of = _logits(name, logits, tokens)
+    o, a = _by_row(name, 'old_logp', old_logp, tokens), _by_row(name, 'advantages', advantages, tokens)
+    r = w = (0, 0)
+    ref = wp = None
+    if ref_logp is not None:
+        r, ref = _by_row(name, 'ref_logp', ref_logp, tokens), ref_logp.data_ptr()
+    if weight is not None:
+        w, wp = _by_row(name, 'weight', weight, tokens), weight.data_ptr()
+    dev, n = logits.device, of[4] * of[5]
     loss = torch.empty((), device=dev, dtype=torch.float32)
     logp = torch.empty(tokens.shape, device=dev, dtype=torch.float32)
-    stats = torch.empty(4, n, device=dev, dtype=torch.float32)  # the rows' maxima, sums, slopes and terms
-    gs = (0, 0) if grad is None else _grad_strides(grad)
+    stats = torch.empty(4, n, device=dev, dtype=torch.float32)  # the rows' references, sums, slopes and terms
+    grad, gp, gs = None, None, (0, 0)
+    if with_grad:
+        grad = _grad_like(logits)
+        gp, gs = grad.data_ptr(), _grad_strides(grad)
     with _on(logits):
-        _call('ta_policy_loss', logits.data_ptr(), _DT[logits.dtype], zs[0], zs[1], b, t, V, tokens.data_ptr(), ts[0], ts[1],
-              _V4(*ptrs), _L8(*strides), 1.0 / max(n, 1), clip[0], clip[1], kl, temperature, loss.data_ptr(), logp.data_ptr(),
-              stats.data_ptr(), None if grad is None else grad.data_ptr(), gs[0], gs[1], _stream(logits))
-    return loss, logp, stats
+        _call('ta_policy_loss', *of, _V4(old_logp.data_ptr(), advantages.data_ptr(), ref, wp),
+              _L8(o[0], o[1], a[0], a[1], r[0], r[1], w[0], w[1]), 1.0 / max(n, 1), clip[0], clip[1], kl, temperature, loss.data_ptr(),
+              logp.data_ptr(), stats.data_ptr(), gp, gs[0], gs[1], _stream(logits))
+    return loss, logp, stats, grad
 
 
 class _PolicyLoss(torch.autograd.Function):
@@ -143,8 +145,8 @@ class _PolicyLoss(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, tokens, old_logp, advantages, ref_logp, weight, clip, kl, temperature):
-        ctx.grad = None if logits.dtype is torch.float16 else _grad_like(logits)
-        loss, logp, stats = _policy(logits, tokens, old_logp, advantages, ref_logp, weight, clip, kl, temperature, ctx.grad)
+        loss, logp, stats, ctx.grad = _policy(logits, tokens, old_logp, advantages, ref_logp, weight, clip, kl, temperature,
+                                                      logits.dtype is not torch.float16)
         ctx.save_for_backward(logits, tokens, stats)
         ctx.temperature = temperature
         ctx.mark_non_differentiable(logp)
@@ -161,9 +163,9 @@ class _PolicyLoss(torch.autograd.Function):
         formed = grad is not None
         if not formed:
             grad = _grad_like(logits)
-        n = tokens.numel()
-        t = tokens.shape[-1]
-        _logits_grad(logits, tokens, stats, stats.data_ptr() + 8 * n, (t, 1), 1.0, ctx.temperature, dloss.float(), formed, grad)
+        of = _logits('policy_loss', logits, tokens)
+        b, t = of[4], of[5]
+        _logits_grad(logits, of, stats, stats.data_ptr() + 8 * b * t, (t, 1), 1.0, ctx.temperature, dloss, formed, grad)
         return (grad,) + (None,) * 8
 
 
@@ -189,4 +191,4 @@ def policy_loss(logits, tokens, old_logp, advantages, ref_logp=None, weight=None
     args = (logits, tokens, old_logp, advantages, ref_logp if kl else None, weight, (1.0 - lo, 1.0 + hi), kl, temperature)
     if logits.requires_grad and torch.is_grad_enabled():
         return _PolicyLoss.apply(*args)
-    return _policy(*args, None)[:2]
+    return _policy(*args, False)[:2]

@@ -322,8 +322,10 @@ def _records(name, caches, src, dst, of, per_record):
     if not bufs:
         raise ValueError('%s: no caches' % name)
     first = bufs[0]
-    if any(b.shape != first.shape or b.dtype is not first.dtype or b.device != first.device for b in bufs):
-        raise ValueError('%s: the caches must be alike, and on one device' % name)
+    shape, dt, dev = first.shape, first.dtype, first.get_device()
+    for b in bufs:
+        if b.shape != shape or b.dtype is not dt or b.get_device() != dev:
+            raise ValueError('%s: the caches must be alike, and on one device' % name)
     src, dst = [x.tolist() if torch.is_tensor(x) or hasattr(x, 'tolist') else x for x in (src, dst)]
     if len(src) != len(dst):
         raise ValueError('%s: %d sources, %d destinations' % (name, len(src), len(dst)))
