@@ -70,6 +70,17 @@ def test_reserve_counts_replaced_pages():
     assert before[:3] == (pool.owned, pool.free, pool.refs) and torch.equal(before[3], pool.table)
 
 
+def test_positions_as_tensors():
+    """Sequences and lengths may be tensors or arrays of whole numbers."""
+    pool = _pool()
+    pool.reserve(torch.tensor([40, 20, 0, 16]), torch.tensor([0, 0, 0, 0]))
+    with pytest.raises(ValueError, match='once'):
+        pool.fork(torch.tensor([0, 0]), torch.tensor([2, 2]), torch.tensor([40, 40]))
+    pool.fork(torch.tensor([0]), torch.tensor([2]), torch.tensor([40]))
+    assert pool.owned[2] == pool.owned[0][:2]
+    _consistent(pool)
+
+
 def test_refused_forks():
     pool = _pool()
     pool.reserve([40, 0, 0, 0])

@@ -301,10 +301,50 @@ def test_refused():
         adapter_add(**s, out=torch.empty(5, 64, dtype=torch.bfloat16))
     with pytest.raises(ValueError, match='shape'):
         adapter_add(**s, out=torch.empty(6, 64, dtype=torch.bfloat16, device='cuda'))
+    with pytest.raises(ValueError, match='x.s place'):
+        adapter_add(**dict(s, y=s['x']), out=s['x'])
     y = torch.zeros(5, 68, device='cuda', dtype=torch.bfloat16)[:, 4:]
     from treeattn_b200._lib import TreeAttnError
     with pytest.raises(TreeAttnError, match='aligned'):
         adapter_add(**dict(s, y=y))
+
+
+def test_gradients_from_any_place():
+    """A gradient that comes in transposed, expanded, or off the 16-byte boundaries is taken as its values."""
+    from treeattn_b200.adapters import adapter_add
+    s = _inputs([40, 9], 64, 72, 8, torch.bfloat16, seed=3)
+    leaves = {k: s[k].clone().requires_grad_() for k in 'yxab'}
+    base = torch.randn(49, 72, device='cuda').to(torch.bfloat16)
+    off = torch.empty(49 * 72 + 1, device='cuda', dtype=torch.bfloat16)[1:].view(49, 72).copy_(base)
+    turned = base.t().contiguous().t()
+    wide = torch.zeros(49, 75, device='cuda', dtype=torch.bfloat16)[:, 1:73].copy_(base)
+    out = adapter_add(**dict(s, **leaves))
+    want = torch.autograd.grad(out, list(leaves.values()), base, retain_graph=True)
+    for dy in (off, turned, wide):
+        for g, w in zip(torch.autograd.grad(out, list(leaves.values()), dy, retain_graph=True), want):
+            assert torch.equal(g, w)
+    one = base[:1, :1].expand(49, 72)
+    got = torch.autograd.grad(out, list(leaves.values()), one, retain_graph=True)
+    for g, w in zip(got, torch.autograd.grad(out, list(leaves.values()), one.contiguous())):
+        assert torch.equal(g, w)
+
+
+def test_cast_sets():
+    """A set that is cast whole keeps working: its scale is taken in float32 all the same."""
+    model, cfg = _gpt(local=64)
+    model.requires_grad_(False)
+    s = _trained()
+    idx = torch.randint(0, 96, (2, 64), device='cuda')
+    handle = s.attach(model)
+    s.use([0, 1])
+    want = model(idx)[0]
+    s.to(torch.bfloat16)
+    assert s.scale.dtype is torch.bfloat16 and torch.equal(model(idx)[0], want)  # (alpha / rank is 2, which bf16 holds)
+    which = torch.tensor([0, 1], device='cuda', dtype=torch.int32)
+    s.use(which)
+    which[:] = 2  # the caller's tensor is the caller's
+    assert torch.equal(model(idx)[0], want)
+    handle.remove()
 
 
 def test_in_place_in_autograd():

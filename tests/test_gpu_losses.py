@@ -274,6 +274,23 @@ def test_backward_twice_and_after_changes():
                 torch.autograd.grad(out, x, retain_graph=True)
 
 
+def test_saved_elsewhere():
+    """Saved tensors that come back from host memory, at other addresses."""
+    from treeattn_b200.losses import policy_loss, token_logp
+    logits, tokens, old, adv, ref, weight = _inputs(2, 5, 3001, 'f16', seed=6)
+    up = torch.rand(2, 5, device='cuda')
+    grads = []
+    for elsewhere in (False, True):
+        x = logits.clone().requires_grad_()
+        with torch.autograd.graph.save_on_cpu() if elsewhere else torch.enable_grad():
+            y = x * 1
+            loss, lp = policy_loss(y, tokens, old, adv, weight=weight)[0], token_logp(y, tokens)
+        del y
+        torch.randn(1 << 20, device='cuda')
+        grads.append(torch.autograd.grad([loss, lp], x, [torch.tensor(1.0, device='cuda'), up])[0])
+    assert torch.equal(*grads)
+
+
 def test_no_gradient_asked():
     from treeattn_b200.losses import policy_loss
     logits, tokens, old, adv, ref, weight = _inputs(2, 5, 301, 'bf16')

@@ -17,7 +17,7 @@ def test_rejected_arguments_without_gpu():
     for kw, what in ((dict(z=None), 'null'), (dict(tokens=None), 'null'), (dict(dtype=5), 'dtype'), (dict(V=0), 'bad sizes'),
                      (dict(V=524289), 'bad sizes'), (dict(B=-1), 'bad sizes'), (dict(B=1 << 20, T=1 << 8), 'bad sizes'),
                      (dict(tau=0.0), 'temperature'), (dict(tau=-1.0), 'temperature'), (dict(tau=float('nan')), 'temperature'),
-                     (dict(tau=float('inf')), 'temperature'), (dict(tau=1e-42), 'temperature'), (dict(out=None), 'null'),
+                     (dict(tau=float('inf')), 'temperature'), (dict(tau=1e-42), 'temperature'), (dict(tau=4e-39), 'temperature'), (dict(out=None), 'null'),
                      (dict(stats=None), 'null')):
         assert logp(**kw) == _lib.TA_ERR_ARG
         assert 'ta_token_logp' in _lib.last_error() and what in _lib.last_error(), (kw, _lib.last_error())

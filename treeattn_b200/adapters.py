@@ -82,7 +82,7 @@ class _AdapterAdd(torch.autograd.Function):
         n, (na, r, K), N = x.shape[0], a.shape, b.shape[1]
         d = dy
         if d.stride(1) != 1 or d.stride(0) % 8 or d.data_ptr() % 16:
-            d = d.contiguous()
+            d = d.clone(memory_format=torch.contiguous_format)
         dx = torch.empty(n, K, device=x.device, dtype=x.dtype) if need[1] else None
         da, db = torch.empty_like(a) if need[2] else None, torch.empty_like(b) if need[3] else None
         u = torch.empty(2, n, r, device=x.device, dtype=x.dtype) if need[1] or need[2] else None
@@ -100,12 +100,14 @@ def adapter_add(y, x, a, b, start, which, max_new, scale=None, out=None):
     which[i] = -1: none. bfloat16 or float16; ranks a multiple of 8 up to 128 (adapters of smaller ranks are filled up with zeros);
     inputs and outputs multiples of 8, rows of any stride that keeps them 16-byte aligned. start (batch + 1,) and which (batch,) int32;
     max_new is about the rows of the longest sequence (it sizes the grid; more are done all the same). Rows of no sequence, and of
-    sequences without an adapter, are y's. Returns a new tensor, or `out` (y itself: in place). An adapter outside the set gives
-    NaN rows and is recorded (device_error).
+    sequences without an adapter, are y's. Returns a new tensor, or `out` (y itself: in place; it overlaps nothing else). An adapter outside the
+    set gives NaN rows and is recorded (device_error).
     Differentiable in y, x, a and b in bfloat16 (not with an `out` other than y); sequences that share an adapter add to one gradient, in
     one order. t = x A^T is summed in fp32 and multiplied with B as two 16-bit numbers; the sum with y is rounded once."""
     _check('adapter_add', y, x, a, b, start, which, scale)
     max_new = int(max_new)
+    if out is not None and out.data_ptr() == x.data_ptr() and x.numel():
+        raise ValueError('adapter_add: the output in x\'s place')
     if torch.is_grad_enabled() and (y.requires_grad or x.requires_grad or a.requires_grad or b.requires_grad or
                                     scale is not None and scale.requires_grad):
         if scale is not None and scale.requires_grad:
@@ -163,11 +165,12 @@ class AdapterSet(nn.Module):
 
     def _starts(self, B, n):
         """Row offsets of n rows a sequence (kept for the lengths that come up most)."""
-        if (B, n) not in self._start:
+        key = B, n, self.scale.device
+        if key not in self._start:
             if len(self._start) >= 16:
                 self._start.clear()
-            self._start[B, n] = torch.arange(B + 1, device=self.scale.device, dtype=torch.int32) * n
-        return self._start[B, n]
+            self._start[key] = torch.arange(B + 1, device=self.scale.device, dtype=torch.int32) * n
+        return self._start[key]
 
     def use(self, which):
         """The adapters of the next batches of the attached model: whole numbers, -1 for none (None: no adapters at all)."""
@@ -177,12 +180,15 @@ class AdapterSet(nn.Module):
         which = torch.as_tensor(which)
         if which.dim() != 1 or which.is_floating_point():
             raise ValueError('AdapterSet: which must be whole numbers, one a sequence')
-        self._which = which.to(self.scale.device, torch.int32)
+        self._which = which.to(self.scale.device, torch.int32, copy=True)
+
+    def _scale(self):
+        return self.scale if self.scale.dtype is torch.float32 else self.scale.float()  # (a cast of the whole set casts it too)
 
     def apply_to(self, y, x, layer, projection, start, which, max_new):
         """Adds a projection's adapters to its rows y, in place."""
         f = self.factors(layer, projection)
-        return y if f is None or which is None else adapter_add(y, x, *f, start, which, max_new, scale=self.scale, out=y)
+        return y if f is None or which is None else adapter_add(y, x, *f, start, which, max_new, scale=self._scale(), out=y)
 
     def attach(self, model):
         """Adds the adapters to the projections of a GPT (16-bit, on the set's device). Returns a handle whose remove() takes them
@@ -205,7 +211,7 @@ class AdapterSet(nn.Module):
             if self._which.shape[0] != B:
                 raise ValueError('AdapterSet: adapters for %d sequences, a batch of %d' % (self._which.shape[0], B))
             a, b = self.factors(layer, projection)
-            rows = adapter_add(y.reshape(B * n, -1), x.reshape(B * n, -1), a, b, self._starts(B, n), self._which, n, scale=self.scale)
+            rows = adapter_add(y.reshape(B * n, -1), x.reshape(B * n, -1), a, b, self._starts(B, n), self._which, n, scale=self._scale())
             return rows.view(y.shape)
         return add
 

@@ -30,7 +30,7 @@ int check(const char* who, int dtype, int n_adapters, int K, int N, int r, int n
   if (r < 8 || r > 128 || r % 8 != 0) return fail(TA_ERR_ARG, "%s: rank %d (a multiple of 8 up to 128)", who, r);
   if (K < 8 || N < 8 || K % 8 != 0 || N % 8 != 0 || K > (1 << 24) || N > (1 << 24))
     return fail(TA_ERR_ARG, "%s: rows of %d and %d columns (multiples of 8)", who, K, N);
-  if (n_adapters < 1 || n_adapters > 65535 || n_rows < 0 || B < 0 || B > 65534 || max_new < 0)
+  if (n_adapters < 1 || n_adapters > 65535 || n_rows < 0 || n_rows > (1 << 30) || B < 0 || B > 65534 || max_new < 0)
     return fail(TA_ERR_ARG, "%s: bad sizes adapters=%d rows=%d B=%d max_new=%d", who, n_adapters, n_rows, B, max_new);
   if (!start || (B && !which)) return fail(TA_ERR_ARG, "%s: null pointer", who);
   return TA_OK;

@@ -30,7 +30,7 @@ int check_rows(const char* who, const void* z, int dtype, int B, int T, int V, c
   if (!valid_dtype(dtype)) return fail(TA_ERR_ARG, "%s: bad dtype %d", who, dtype);
   if (B < 0 || T < 0 || V < 1 || V > MAX_ROW / esize_of(dtype) || (int64_t)B * T > (1 << 27))
     return fail(TA_ERR_ARG, "%s: bad sizes B=%d T=%d V=%d (rows of at most %d bytes, 2^27 of them)", who, B, T, V, MAX_ROW);
-  if (!(tau > 0.f) || !std::isfinite(tau) || !std::isfinite(1.f / tau))
+  if (!(tau > 0.f) || !std::isfinite(tau) || !std::isfinite(2.f / tau))
     return fail(TA_ERR_ARG, "%s: temperature %g (positive and finite)", who, tau);
   if ((int64_t)B * T > 0 && (!z || !tokens)) return fail(TA_ERR_ARG, "%s: null pointer", who);
   return TA_OK;

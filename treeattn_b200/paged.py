@@ -125,7 +125,7 @@ class PagePool:
             if -(-int(n) // self.page) > self.max_pages:
                 raise ValueError('PagePool: %d positions above the %d of a sequence' % (n, self.max_pages * self.page))
         shared, left = [], {}
-        for b, at in enumerate(pos or ()):
+        for b, at in enumerate(() if pos is None else pos):
             own = self.owned[b]
             for j in range(int(at) // self.page, len(own)):
                 n = left.get(own[j], self.refs[own[j]])
@@ -153,13 +153,14 @@ class PagePool:
         source and a destination): it shares the full pages among them, and what dst[i] held is given back. The open pages, which
         live in the caches' tails, are paged_fork's to copy."""
         B = len(self.owned)
+        src, dst, lengths = [[int(i) for i in x] for x in (src, dst, lengths)]
         if not len(src) == len(dst) == len(lengths):
             raise ValueError('PagePool.fork: %d sources, %d destinations, %d lengths' % (len(src), len(dst), len(lengths)))
-        if any(not 0 <= int(b) < B for b in (*src, *dst)) or len(set(dst)) != len(dst):
+        if any(not 0 <= b < B for b in (*src, *dst)) or len(set(dst)) != len(dst):
             raise ValueError('PagePool.fork: sequences in [0, %d), each a destination once' % B)
         new = {}
         for s, d, n in zip(src, dst, lengths):
-            full = int(n) // self.page
+            full = n // self.page
             if n < 0 or full > len(self.owned[s]):
                 raise ValueError('PagePool.fork: sequence %d does not hold %d positions' % (s, n))
             if s != d:

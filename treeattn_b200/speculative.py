@@ -129,10 +129,11 @@ class PagedDecoder:
     def fork(self, src, dst):
         """Sequence dst[i] goes on from where sequence src[i] is, for all i at once: a prompt into a group of samples, beams that take
         over one another's slots. Full pages are shared; the open ones are copied. What dst[i] held is dropped."""
+        src, dst = [int(b) for b in src], [int(b) for b in dst]
         self.pool.fork(src, dst, [self.pos[s] if 0 <= s < self.batch else 0 for s in src])
         paged_fork(self.caches, src, dst)
-        if self.adapters is not None and len(src):
-            at = torch.tensor([list(src), list(dst)]).to(self.dev)
+        if self.adapters is not None and src:
+            at = torch.tensor([src, dst]).to(self.dev)
             self.which[at[1]] = self.which[at[0]]
         was = self.pos, self._floor
         self.pos, self._floor = list(self.pos), list(self._floor)
