@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(ADAPTER_THREADS, RP <= 32 ? 4 : RP == 64 ? 2 :
 }
 
 // ------------------------------------------------------------------------------------------------ many rows
-// The three kernels below take their operands from memory straight into the fragments of the matrix instruction: the order of a sum's
+// t's kernel takes its operands from memory straight into the fragments of the matrix instruction: the order of a sum's
 // terms and of an output's columns is free, and it is chosen so that a thread's share of a fragment is 16 consecutive bytes
 // of a row. Nothing passes through shared memory but the warps' sums at the end, and no warp waits for another before that.
 //   k of a 32-wide block: step s (0, 1), the fragment's pair (lane % 4 = j, half h) <-> elements 8 j + 4 s + 2 h, + 1
@@ -644,20 +644,25 @@ struct AdapterGradParams {
 
 template <int RP>
 struct AdapterGradShape {
-  static constexpr int RT = RP == 16 ? 16 : 32;   // ranks of a CTA
-  static constexpr int MC = 64;                   // columns of a CTA
-  static constexpr int BYTES = 8 * MC * RT * 4;
+  static constexpr int RT = RP == 16 ? 16 : 32;               // ranks of a CTA
+  static constexpr int MC = 64;                               // columns of a CTA
+  static constexpr int PP = MC * 2 + 16, TP = RT * 2 + 16;    // pitches of rows by columns and by rank
+  static constexpr int STAGE = 16 * PP + 32 * TP;             // 16 rows: of the columns, of t's high and low parts
+  static constexpr int STAGES = RT == 16 ? 3 : 2;             // of a warp: what leaves room for two CTAs on an SM
+  static constexpr int RING = 8 * STAGES * STAGE, PART = 8 * MC * RT * 4;
+  static constexpr int BYTES = RING > PART ? RING : PART;     // (the warps' sums lie where the rows were)
 };
 
-// dA and dB: a CTA takes 64 or 128 columns of x or of dy and up to 32 ranks, and sums the products of those columns with u or t over the rows of
-// all sequences that use its adapter. Its warps, and the CTAs of a cluster, take every so many blocks of 16 rows; their sums meet
-// in one order. An adapter that nobody uses gets zeros. Both operands run along the rows, so both are turned in registers.
+// dA and dB: a CTA takes 64 columns of x or of dy and up to 32 ranks, and sums the products of those columns with u or t over the rows of
+// all sequences that use its adapter. Its warps, and the CTAs of a cluster, take every so many blocks of 16 rows, each through a ring of its
+// own, and wait for no other warp; their sums meet in one order. An adapter that nobody uses gets zeros.
 template <typename T, int RP>
 __global__ void __launch_bounds__(ADAPTER_THREADS, 2) adapter_grad_kernel(const __grid_constant__ AdapterGradParams p) {
   using S = AdapterGradShape<RP>;
   constexpr int MC = S::MC, RT = S::RT, MT = MC / 16, NT = RT / 8;
-  extern __shared__ __align__(16) float part[];  // (8, MC, RT)
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, i = lane >> 2, j = lane & 3;
+  extern __shared__ __align__(16) unsigned char smem[];
+  float* const part = reinterpret_cast<float*>(smem);  // (8, MC, RT), after the rows
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int cs = cluster_nctarank(), rank = cluster_ctarank();
   const int a = blockIdx.y, rank0 = blockIdx.z * RT;
   const int k_tiles = p.da ? (p.K + MC - 1) / MC : 0;
@@ -677,52 +682,64 @@ __global__ void __launch_bounds__(ADAPTER_THREADS, 2) adapter_grad_kernel(const 
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[m][n][e] = 0.f;
-  struct Rows {  // a thread's share of 16 rows: of the columns, of t's high and low parts
-    uint4 p[MC / 32][2], t[2][2];
-  };
-  auto load = [&](Rows& v, int row0, int n_rows) {  // n_rows of them there
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const T* const from = R + (int64_t)(row0 + 8 * h + i) * sr + c0 + 8 * j;
-#pragma unroll
-      for (int g = 0; g < MC / 32; ++g) v.p[g][h] = load16(from + 32 * g, 8 * h + i < n_rows && c0 + 32 * g + 8 * j < C);
-#pragma unroll
-      for (int l = 0; l < 2; ++l) {
-        const T* const of = W + ((int64_t)l * p.n_rows + row0 + 8 * h + i) * p.r + rank0;
-        if (RT == 16) {
-          const uint2 x = load8(of + 4 * j, 8 * h + i < n_rows && rank0 + 4 * j < p.r);
-          v.t[l][h] = make_uint4(x.x, x.y, 0u, 0u);
-        } else {
-          v.t[l][h] = load16(of + 8 * j, 8 * h + i < n_rows && rank0 + 8 * j < p.r);
-        }
-      }
-    }
-  };
-  auto multiply = [&](const Rows& v) {
-    uint32_t tb[2][NT][2];  // high or low, tile, half
+
+  const uint32_t ring = smem_u32(smem) + warp * S::STAGES * S::STAGE;
+  // a lane's pieces of a stage: rows pm, pm + 4, ... of the columns; rows tm (and tm + 8) of t's two parts
+  const int pm = lane / 8, pc = lane % 8 * 8, tm = lane / (RT / 8), tc = lane % (RT / 8) * 8;
+  constexpr int TI = 32 / (RT / 8);
+  const bool column = c0 + pc < C, ranks_here = rank0 + tc < p.r;
+  int put = 0, took = 0;
+  auto multiply = [&]() {
+    const uint32_t ps = ring + (took % S::STAGES) * S::STAGE, ts = ps + 16 * S::PP;
+    ++took;
+    uint32_t tb[2][NT / 2][4];
 #pragma unroll
     for (int l = 0; l < 2; ++l)
 #pragma unroll
-      for (int q = 0; q < NT; ++q)
+      for (int n = 0; n < NT / 2; ++n) ldsm4t(tb[l][n], ts + (16 * l + (lane & 15)) * S::TP + (n * 16 + (lane >> 4) * 8) * 2);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) tb[l][q][h] = turned(word(v.t[l][h], q));
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {  // tiles 2 g and 2 g + 1 of a 32-wide block: its column pairs q = 0, 1 and 2, 3
-      const uint4 &x0 = v.p[m / 2][0], &x1 = v.p[m / 2][1];
-      const int q = m % 2 * 2;
-      const uint32_t pa[4] = {turned(word(x0, q)), turned(word(x0, q + 1)), turned(word(x1, q)), turned(word(x1, q + 1))};
+    for (int m = 0; m < MT; ++m) {
+      uint32_t pa[4];  // the columns as the product's rows: 16 x 16 of the stage's rows (k) by columns (m), transposed
+      ldsm4t(pa, ps + ((lane >> 4) * 8 + (lane & 7)) * S::PP + (m * 16 + ((lane >> 3) & 1) * 8) * 2);
 #pragma unroll
       for (int l = 0; l < 2; ++l)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) mma16<T>(acc[m][n], pa, tb[l][n][0], tb[l][n][1]);
+        for (int n = 0; n < NT / 2; ++n) {
+          mma16<T>(acc[m][2 * n], pa, tb[l][n][0], tb[l][n][1]);
+          mma16<T>(acc[m][2 * n + 1], pa, tb[l][n][2], tb[l][n][3]);
+        }
+    }
+  };
+  // block `put` is asked for, block put - (STAGES - 1) has arrived
+  auto ask = [&](int row0, int n) {  // 16 rows, n of them there
+    __syncwarp();
+    const uint32_t at = ring + (put % S::STAGES) * S::STAGE;
+    ++put;
+    const T* const from = R + (int64_t)(row0 + pm) * sr + c0 + pc;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const bool real = pm + 4 * q < n && column;
+      cp16(at + (pm + 4 * q) * S::PP + pc * 2, real ? from + 4 * q * sr : R, real);
+    }
+#pragma unroll
+    for (int q = 0; q < 16 / TI; ++q) {
+      const bool real = tm + TI * q < n && ranks_here;
+      const T* const t = real ? W + (int64_t)(row0 + tm + TI * q) * p.r + rank0 + tc : W;
+#pragma unroll
+      for (int l = 0; l < 2; ++l)
+        cp16(at + 16 * S::PP + (16 * l + tm + TI * q) * S::TP + tc * 2, real ? t + (int64_t)l * p.n_rows * p.r : W, real);
+    }
+    cp_commit();
+    if (put - took >= S::STAGES) {
+      cp_wait<S::STAGES - 1>();
+      __syncwarp();
+      multiply();
     }
   };
   {
     // this warp's blocks of 16 rows: every (8 cs)th of the adapter's, sequence after sequence
     const int turns = 8 * cs;
     int turn = rank * 8 + warp;  // blocks until the next one of this warp's
-    Rows v, w;                   // 16 ranks: the block before, multiplied while the next one arrives (with 32 both do not fit)
-    bool held = false;
     for (int b0 = 0; b0 < p.B; b0 += 32) {
       const int b = b0 + lane;
       int s0 = 0, s1 = 0;
@@ -736,32 +753,22 @@ __global__ void __launch_bounds__(ADAPTER_THREADS, 2) adapter_grad_kernel(const 
         some &= some - 1;
         const int q0 = __shfl_sync(0xffffffffu, s0, from), q1 = __shfl_sync(0xffffffffu, s1, from);
         const int n = (q1 - q0 + 15) / 16;
-        for (; turn < n; turn += turns) {
-          if constexpr (RT == 16) {
-            load(w, q0 + turn * 16, q1 - q0 - turn * 16);
-            if (held) multiply(v);
-            v = w;
-            held = true;
-          } else {
-            load(v, q0 + turn * 16, q1 - q0 - turn * 16);
-            multiply(v);
-          }
-        }
+        for (; turn < n; turn += turns) ask(q0 + turn * 16, q1 - q0 - turn * 16);
         turn -= n;
       }
     }
-    if (RT == 16 && held) multiply(v);
+    cp_wait<0>();
+    __syncwarp();
+    while (took < put) multiply();
   }
+  __syncthreads();  // the warps' sums go where the rows were
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      // the fragment's row i is column 32 (m / 2) + 8 (i / 2) + 4 (m % 2) + i % 2 of the CTA's, its row i + 8 two further
-      const int mm = 32 * (m / 2) + 8 * (i >> 1) + 4 * (m % 2) + (i & 1);
-      const int c = RT == 16 ? 4 * j + 2 * n : 8 * j + 2 * n;
-      float* const to = part + (warp * MC + mm) * RT + c;
+      float* const to = part + (warp * MC + m * 16 + lane / 4) * RT + n * 8 + (lane & 3) * 2;
       *reinterpret_cast<float2*>(to) = make_float2(acc[m][n][0], acc[m][n][1]);
-      *reinterpret_cast<float2*>(to + 2 * RT) = make_float2(acc[m][n][2], acc[m][n][3]);
+      *reinterpret_cast<float2*>(to + 8 * RT) = make_float2(acc[m][n][2], acc[m][n][3]);
     }
   __syncthreads();
   for (int e = tid; e < MC * RT; e += ADAPTER_THREADS) {
