@@ -688,10 +688,15 @@ __global__ void __launch_bounds__(ADAPTER_THREADS, 2) adapter_grad_kernel(const 
   const int pm = lane / 8, pc = lane % 8 * 8, tm = lane / (RT / 8), tc = lane % (RT / 8) * 8;
   constexpr int TI = 32 / (RT / 8);
   const bool column = c0 + pc < C, ranks_here = rank0 + tc < p.r;
-  int put = 0, took = 0;
+  const bool whole = c0 + MC <= C && rank0 + RT <= p.r;
+  const int64_t step4 = 4 * sr, step8 = 8 * sr, step12 = 12 * sr, lo_step = (int64_t)p.n_rows * p.r;
+  int held = 0;                              // blocks asked for and not multiplied
+  uint32_t put = ring, took = ring;          // where the next one goes, and the oldest lies
+  const uint32_t row_to = pm * S::PP + pc * 2, t_to = 16 * S::PP + tm * S::TP + tc * 2;
   auto multiply = [&]() {
-    const uint32_t ps = ring + (took % S::STAGES) * S::STAGE, ts = ps + 16 * S::PP;
-    ++took;
+    const uint32_t ps = took, ts = ps + 16 * S::PP;
+    took = took + S::STAGE == ring + S::STAGES * S::STAGE ? ring : took + S::STAGE;
+    --held;
     uint32_t tb[2][NT / 2][4];
 #pragma unroll
     for (int l = 0; l < 2; ++l)
@@ -710,27 +715,36 @@ __global__ void __launch_bounds__(ADAPTER_THREADS, 2) adapter_grad_kernel(const 
         }
     }
   };
-  // block `put` is asked for, block put - (STAGES - 1) has arrived
+  // one block is asked for; the one STAGES - 1 before it has arrived, and is multiplied
   auto ask = [&](int row0, int n) {  // 16 rows, n of them there
     __syncwarp();
-    const uint32_t at = ring + (put % S::STAGES) * S::STAGE;
-    ++put;
+    const uint32_t at = put;
+    put = put + S::STAGE == ring + S::STAGES * S::STAGE ? ring : put + S::STAGE;
     const T* const from = R + (int64_t)(row0 + pm) * sr + c0 + pc;
+    const T* const t = W + (int64_t)(row0 + tm) * p.r + rank0 + tc;
+    if (whole && n >= 16) {
+      cp16(at + row_to, from);
+      cp16(at + row_to + 4 * S::PP, from + step4);
+      cp16(at + row_to + 8 * S::PP, from + step8);
+      cp16(at + row_to + 12 * S::PP, from + step12);
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const bool real = pm + 4 * q < n && column;
-      cp16(at + (pm + 4 * q) * S::PP + pc * 2, real ? from + 4 * q * sr : R, real);
-    }
-#pragma unroll
-    for (int q = 0; q < 16 / TI; ++q) {
-      const bool real = tm + TI * q < n && ranks_here;
-      const T* const t = real ? W + (int64_t)(row0 + tm + TI * q) * p.r + rank0 + tc : W;
-#pragma unroll
-      for (int l = 0; l < 2; ++l)
-        cp16(at + 16 * S::PP + (16 * l + tm + TI * q) * S::TP + tc * 2, real ? t + (int64_t)l * p.n_rows * p.r : W, real);
+      for (int q = 0; q < 16 / TI; ++q) {
+        cp16(at + t_to + TI * q * S::TP, t + TI * q * p.r);
+        cp16(at + t_to + (16 + TI * q) * S::TP, t + TI * q * p.r + lo_step);
+      }
+    } else {
+      for (int q = 0; q < 4; ++q) {
+        const bool real = pm + 4 * q < n && column;
+        cp16(at + row_to + 4 * q * S::PP, real ? from + q * step4 : R, real);
+      }
+      for (int q = 0; q < 16 / TI; ++q) {
+        const bool real = tm + TI * q < n && ranks_here;
+        cp16(at + t_to + TI * q * S::TP, real ? t + TI * q * p.r : W, real);
+        cp16(at + t_to + (16 + TI * q) * S::TP, real ? t + TI * q * p.r + lo_step : W, real);
+      }
     }
     cp_commit();
-    if (put - took >= S::STAGES) {
+    if (++held >= S::STAGES) {
       cp_wait<S::STAGES - 1>();
       __syncwarp();
       multiply();
@@ -759,7 +773,7 @@ __global__ void __launch_bounds__(ADAPTER_THREADS, 2) adapter_grad_kernel(const 
     }
     cp_wait<0>();
     __syncwarp();
-    while (took < put) multiply();
+    while (held > 0) multiply();
   }
   __syncthreads();  // the warps' sums go where the rows were
 #pragma unroll
