@@ -645,15 +645,15 @@ struct AdapterGradParams {
 template <int RP>
 struct AdapterGradShape {
   static constexpr int RT = RP == 16 ? 16 : 32;               // ranks of a CTA
-  static constexpr int MC = 64;                               // columns of a CTA
+  static constexpr int MC = RP == 16 ? 128 : 64;              // columns of a CTA
   static constexpr int PP = MC * 2 + 16, TP = RT * 2 + 16;    // pitches of rows by columns and by rank
   static constexpr int STAGE = 16 * PP + 32 * TP;             // 16 rows: of the columns, of t's high and low parts
-  static constexpr int STAGES = RT == 16 ? 3 : 2;             // of a warp: what leaves room for two CTAs on an SM
+  static constexpr int STAGES = 2;                            // of a warp: what leaves room for two CTAs on an SM
   static constexpr int RING = 8 * STAGES * STAGE, PART = 8 * MC * RT * 4;
   static constexpr int BYTES = RING > PART ? RING : PART;     // (the warps' sums lie where the rows were)
 };
 
-// dA and dB: a CTA takes 64 columns of x or of dy and up to 32 ranks, and sums the products of those columns with u or t over the rows of
+// dA and dB: a CTA takes 64 or 128 columns of x or of dy and up to 32 ranks, and sums the products of those columns with u or t over the rows of
 // all sequences that use its adapter. Its warps, and the CTAs of a cluster, take every so many blocks of 16 rows, each through a ring of its
 // own, and wait for no other warp; their sums meet in one order. An adapter that nobody uses gets zeros.
 template <typename T, int RP>
@@ -684,12 +684,13 @@ __global__ void __launch_bounds__(ADAPTER_THREADS, 2) adapter_grad_kernel(const 
       for (int e = 0; e < 4; ++e) acc[m][n][e] = 0.f;
 
   const uint32_t ring = smem_u32(smem) + warp * S::STAGES * S::STAGE;
-  // a lane's pieces of a stage: rows pm, pm + 4, ... of the columns; rows tm (and tm + 8) of t's two parts
-  const int pm = lane / 8, pc = lane % 8 * 8, tm = lane / (RT / 8), tc = lane % (RT / 8) * 8;
+  // a lane's pieces of a stage: rows pm, pm + PI, ... of the columns; rows tm (and tm + 8) of t's two parts
+  constexpr int PI = 32 / (MC / 8);
+  const int pm = lane / (MC / 8), pc = lane % (MC / 8) * 8, tm = lane / (RT / 8), tc = lane % (RT / 8) * 8;
   constexpr int TI = 32 / (RT / 8);
   const bool column = c0 + pc < C, ranks_here = rank0 + tc < p.r;
   const bool whole = c0 + MC <= C && rank0 + RT <= p.r;
-  const int64_t step4 = 4 * sr, step8 = 8 * sr, step12 = 12 * sr, lo_step = (int64_t)p.n_rows * p.r;
+  const int64_t step = PI * sr, lo_step = (int64_t)p.n_rows * p.r;
   int held = 0;                              // blocks asked for and not multiplied
   uint32_t put = ring, took = ring;          // where the next one goes, and the oldest lies
   const uint32_t row_to = pm * S::PP + pc * 2, t_to = 16 * S::PP + tm * S::TP + tc * 2;
@@ -723,19 +724,18 @@ __global__ void __launch_bounds__(ADAPTER_THREADS, 2) adapter_grad_kernel(const 
     const T* const from = R + (int64_t)(row0 + pm) * sr + c0 + pc;
     const T* const t = W + (int64_t)(row0 + tm) * p.r + rank0 + tc;
     if (whole && n >= 16) {
-      cp16(at + row_to, from);
-      cp16(at + row_to + 4 * S::PP, from + step4);
-      cp16(at + row_to + 8 * S::PP, from + step8);
-      cp16(at + row_to + 12 * S::PP, from + step12);
+      const T* f = from;
+#pragma unroll
+      for (int q = 0; q < 16 / PI; ++q, f += step) cp16(at + row_to + PI * q * S::PP, f);
 #pragma unroll
       for (int q = 0; q < 16 / TI; ++q) {
         cp16(at + t_to + TI * q * S::TP, t + TI * q * p.r);
         cp16(at + t_to + (16 + TI * q) * S::TP, t + TI * q * p.r + lo_step);
       }
     } else {
-      for (int q = 0; q < 4; ++q) {
-        const bool real = pm + 4 * q < n && column;
-        cp16(at + row_to + 4 * q * S::PP, real ? from + q * step4 : R, real);
+      for (int q = 0; q < 16 / PI; ++q) {
+        const bool real = pm + PI * q < n && column;
+        cp16(at + row_to + PI * q * S::PP, real ? from + q * step : R, real);
       }
       for (int q = 0; q < 16 / TI; ++q) {
         const bool real = tm + TI * q < n && ranks_here;
