@@ -21,55 +21,74 @@ def _rows(name, what, t, dtype=None):
 
 
 def _check(name, y, x, a, b, start, which, scale):
-    if x.dtype is not torch.bfloat16 and x.dtype is not torch.float16:
-        raise TypeError('%s: bfloat16 or float16 (got %s)' % (name, x.dtype))
-    _rows(name, 'x', x)
-    _rows(name, 'y', y, x.dtype)
-    if a.dim() != 3 or b.dim() != 3 or a.dtype is not x.dtype or b.dtype is not x.dtype:
+    """Checks a call's tensors; returns (adapters, rank, inputs, outputs, rows, batch)."""
+    dt, dev = x.dtype, x.get_device()
+    (n, K), (m, N), (na, r, ka), bs, (B,), (s,) = _dims(name, y, x, a, b, start, which)
+    if (dt is torch.bfloat16 or dt is torch.float16) and y.dtype is dt and a.dtype is dt and b.dtype is dt and m == n and ka == K and (
+            bs == (na, N, r)) and s == B + 1 and start.dtype is torch.int32 and which.dtype is torch.int32 and x.stride(1) == 1 and (
+            y.stride(1) == 1) and a.is_contiguous() and b.is_contiguous() and start.is_contiguous() and which.is_contiguous() and dev >= 0 and (
+            y.get_device() == dev and a.get_device() == dev and b.get_device() == dev and start.get_device() == dev and
+            which.get_device() == dev) and (scale is None or scale.dtype is torch.float32 and scale.shape == (na,) and
+                                            scale.is_contiguous() and scale.get_device() == dev):
+        return na, r, K, N, n, B
+    # something does not fit: what
+    if dt is not torch.bfloat16 and dt is not torch.float16:
+        raise TypeError('%s: bfloat16 or float16 (got %s)' % (name, dt))
+    for what, t in (('x', x), ('y', y)):
+        _rows(name, what, t, dt)
+    if a.dtype is not dt or b.dtype is not dt:
         raise ValueError('%s: a (adapters, rank, inputs) and b (adapters, outputs, rank) of x\'s type' % name)
-    na, r, K = a.shape
-    if x.shape[1] != K or b.shape != (na, y.shape[1], r) or y.shape[0] != x.shape[0]:
+    if ka != K or bs != (na, N, r) or m != n:
         raise ValueError('%s: x %s, y %s, a %s, b %s do not fit' % (name, tuple(x.shape), tuple(y.shape), tuple(a.shape),
                                                                    tuple(b.shape)))
     if not (a.is_contiguous() and b.is_contiguous()):
         raise ValueError('%s: a and b must be contiguous' % name)
     if start.dtype is not torch.int32 or which.dtype is not torch.int32 or not (start.is_contiguous() and which.is_contiguous()):
         raise TypeError('%s: start and which must be contiguous int32' % name)
-    if which.dim() != 1 or start.shape != (which.shape[0] + 1,):
+    if s != B + 1:
         raise ValueError('%s: which (batch,) and start (batch + 1,)' % name)
     if scale is not None and (scale.dtype is not torch.float32 or scale.shape != (na,) or not scale.is_contiguous()):
         raise ValueError('%s: scale must be (adapters,) float32, contiguous' % name)
-    dev = x.get_device()
-    for t in (x, y, a, b, start, which, scale):
+    _need_cuda(name, x, y, a, b, start, which, scale)
+    for t in (y, a, b, start, which, scale):
         if t is not None and t.get_device() != dev:
-            _need_cuda(name, t, x)
             raise ValueError('%s: tensors on one device (got %s and %s)' % (name, x.device, t.device))
-    _need_cuda(name, x)
+    return na, r, K, N, n, B  # (a single column's stride does not matter)
 
 
-def _add(y, x, a, b, start, which, max_new, scale, out, t=None):
-    (na, r, K), N = a.shape, y.shape[1]
+def _dims(name, y, x, a, b, start, which):
+    shapes = x.shape, y.shape, a.shape, b.shape, which.shape, start.shape
+    if tuple(len(s) for s in shapes) != (2, 2, 3, 3, 1, 1):
+        for what, t in (('x', x), ('y', y)):
+            _rows(name, what, t)
+        if a.dim() != 3 or b.dim() != 3:
+            raise ValueError('%s: a (adapters, rank, inputs) and b (adapters, outputs, rank)' % name)
+        raise ValueError('%s: which (batch,) and start (batch + 1,)' % name)
+    return shapes
+
+
+def _add(y, x, a, b, start, which, dims, max_new, scale, out, t=None):
+    na, r, K, N, n, B = dims
     if t is None and max_new > 16:  # many rows: t goes by way of memory (f16's rows with a factor each)
-        n = x.shape[0]
         t = torch.empty(2 * n * r + (2 * n if x.dtype is torch.float16 else 0), device=x.device, dtype=x.dtype)
     with _on(x):
-        _call('ta_adapter_add', y.data_ptr(), y.stride(0), x.data_ptr(), x.stride(0), a.data_ptr(), b.data_ptr(), _p(scale),
-              _DT[x.dtype], na, K, N, r, x.shape[0], start.data_ptr(), which.data_ptr(), which.shape[0], max_new, out.data_ptr(),
-              out.stride(0), _p(t), _stream(x))
+        _call('ta_adapter_add', y.data_ptr(), y.stride(0), x.data_ptr(), x.stride(0), a.data_ptr(), b.data_ptr(),
+              None if scale is None else scale.data_ptr(), _DT[x.dtype], na, K, N, r, n, start.data_ptr(), which.data_ptr(), B, max_new,
+              out.data_ptr(), out.stride(0), None if t is None else t.data_ptr(), _stream(x))
     return out
 
 
 class _AdapterAdd(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, y, x, a, b, start, which, max_new, scale, into):
+    def forward(ctx, y, x, a, b, start, which, dims, max_new, scale, into):
         need = ctx.needs_input_grad
         t = torch.empty(2, x.shape[0], a.shape[1], device=x.device, dtype=x.dtype) if need[3] else None  # what dB needs of x
         if into:
             out = y
             ctx.mark_dirty(y)
         else:
-            out = torch.empty(y.shape, device=y.device, dtype=y.dtype)
-        _add(y, x, a, b, start, which, max_new, scale, out, t)
+            out = torch.empty_like(y, memory_format=torch.contiguous_format)
+        _add(y, x, a, b, start, which, dims, max_new, scale, out, t)
         ctx.save_for_backward(x, a, b, start, which, scale, t)
         ctx.max_new = max_new
         return out
@@ -91,7 +110,7 @@ class _AdapterAdd(torch.autograd.Function):
                 _call('ta_adapter_bwd', d.data_ptr(), d.stride(0), x.data_ptr(), x.stride(0), a.data_ptr(), b.data_ptr(), _p(scale), na,
                       K, N, r, n, start.data_ptr(), which.data_ptr(), which.shape[0], ctx.max_new, _p(t), _p(u), _p(dx),
                       K if dx is None else dx.stride(0), _p(da), _p(db), _stream(x))
-        return dy if need[0] else None, dx, da, db, None, None, None, None, None
+        return (dy if need[0] else None, dx, da, db) + (None,) * 6
 
 
 def adapter_add(y, x, a, b, start, which, max_new, scale=None, out=None):
@@ -104,7 +123,7 @@ def adapter_add(y, x, a, b, start, which, max_new, scale=None, out=None):
     set gives NaN rows and is recorded (device_error).
     Differentiable in y, x, a and b in bfloat16 (not with an `out` other than y); sequences that share an adapter add to one gradient, in
     one order. t = x A^T is summed in fp32 and multiplied with B as two 16-bit numbers; the sum with y is rounded once."""
-    _check('adapter_add', y, x, a, b, start, which, scale)
+    dims = _check('adapter_add', y, x, a, b, start, which, scale)
     max_new = int(max_new)
     if out is not None and out.data_ptr() == x.data_ptr() and x.numel():
         raise ValueError('adapter_add: the output in x\'s place')
@@ -116,15 +135,15 @@ def adapter_add(y, x, a, b, start, which, max_new, scale=None, out=None):
             raise TypeError('adapter_add: gradients in bfloat16 only (got %s)' % x.dtype)
         if out is not None and out is not y:
             raise ValueError('adapter_add: no gradient through a given output (other than y itself)')
-        return _AdapterAdd.apply(y, x, a, b, start, which, max_new, scale, out is y)
+        return _AdapterAdd.apply(y, x, a, b, start, which, dims, max_new, scale, out is y)
     if out is None:
-        out = torch.empty(y.shape, device=y.device, dtype=y.dtype)
+        out = torch.empty_like(y, memory_format=torch.contiguous_format)
     elif out is not y:
         _rows('adapter_add', 'out', out, y.dtype)
         if out.shape != y.shape:
             raise ValueError('adapter_add: out must have y\'s shape')
         _need_cuda('adapter_add', out)
-    return _add(y, x, a, b, start, which, max_new, scale, out)
+    return _add(y, x, a, b, start, which, dims, max_new, scale, out)
 
 
 class AdapterSet(nn.Module):

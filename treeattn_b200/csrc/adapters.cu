@@ -70,7 +70,9 @@ int run_fused(const char* who, ta::AdapterParams& p, int max_new, cudaStream_t s
   using S = ta::AdapterShape<RP>;
   static SmemAttr attr;
   p.tiles = std::max(1, (int)(((int64_t)std::min(max_new, p.n_rows) + 15) / 16));
-  const int cs = cluster_size((int64_t)p.tiles * p.B, RP <= 32 ? 4 : RP == 64 ? 2 : 1, (std::max(p.K, p.N) + S::KC - 1) / S::KC, 1);
+  // (64 rows of 768 -> 2304, rank 16, on the device: 8.8 us with 8 CTAs a tile, four on an SM, 7.6 with 4; one row of 2048 -> 2048 5.1 with 8,
+  // 6.0 with 4)
+  const int cs = cluster_size((int64_t)p.tiles * p.B, RP <= 64 ? 2 : 1, (std::max(p.K, p.N) + S::KC - 1) / S::KC, 1);
   const dim3 grid((unsigned)(p.tiles * cs), p.B + (p.out == p.y ? 0 : 1));
   return launch(who, ta::adapter_kernel<T, RP>, attr, S::BYTES, grid, cs, st, p);
 }
