@@ -599,32 +599,53 @@ __global__ void __launch_bounds__(ADAPTER_THREADS, RP <= 32 ? 4 : 2) adapter_exp
   }
   const T* const V = reinterpret_cast<const T*>(p.v) + (int64_t)a * p.r * p.N;
   const uint32_t y_to = smem_u32(ys) + pm * S::XP + pc * 2, v_at = smem_u32(vs), t_to = smem_u32(ts) + qm * S::RPP + qc * 2;
-  const bool column = c0 + pc < p.N;
+  const bool column = c0 + pc < p.N, whole = c0 + EXPAND_COLS <= p.N && p.r == RP;
+  const int64_t y_step = RI * p.y_sr, lo_step = (int64_t)p.n_rows * p.r;
   for (int row0 = r0 + tile0 * EXPAND_ROWS; row0 < r1; row0 += p.tiles * EXPAND_ROWS) {
     const int rows = min(EXPAND_ROWS, r1 - row0);
-    if (Y && column) {  // (places beyond the rows and the columns do not matter)
-      const T* const from = Y + (int64_t)(row0 + pm) * p.y_sr + c0 + pc;
+    const T* const t = reinterpret_cast<const T*>(p.t) + (int64_t)(row0 + qm) * p.r + qc;
+    if (whole && rows == EXPAND_ROWS) {
+      if (Y) {
+        const T* from = Y + (int64_t)(row0 + pm) * p.y_sr + c0 + pc;
 #pragma unroll
-      for (int q = 0; q < EXPAND_ROWS / RI; ++q)
-        if (pm + q * RI < rows) cp16(y_to + q * RI * S::XP, from + q * RI * p.y_sr);
-    }
-    if (TRANS) {  // by rank, columns contiguous; what lies beyond the rank is 0
-      for (int m = pm; m < RP; m += RI) {
-        const bool real = m < p.r && column;
-        cp16(v_at + m * S::XP + pc * 2, real ? V + (int64_t)m * p.N + c0 + pc : V, real);
+        for (int q = 0; q < EXPAND_ROWS / RI; ++q, from += y_step) cp16(y_to + q * RI * S::XP, from);
       }
+#pragma unroll
+      for (int q = 0; q < (TRANS ? RP / RI : EXPAND_COLS / TI); ++q) {
+        if (TRANS)
+          cp16(v_at + (pm + q * RI) * S::XP + pc * 2, V + (int64_t)(pm + q * RI) * p.N + c0 + pc);
+        else
+          cp16(v_at + (qm + q * TI) * S::RPP + qc * 2, V + (int64_t)(c0 + qm) * RP + qc + q * TI * RP);
+      }
+#pragma unroll
+      for (int q = 0; q < (EXPAND_ROWS + TI - 1) / TI; ++q)
+        if (EXPAND_ROWS % TI == 0 || qm < EXPAND_ROWS) {
+          cp16(t_to + q * TI * S::RPP, t + q * TI * RP);
+          cp16(t_to + (EXPAND_ROWS + q * TI) * S::RPP, t + q * TI * RP + lo_step);
+        }
     } else {
-      for (int m = qm; m < EXPAND_COLS; m += TI) {
-        const bool real = qc < p.r && c0 + m < p.N;
-        cp16(v_at + m * S::RPP + qc * 2, real ? V + (int64_t)(c0 + m) * p.r + qc : V, real);
+      if (Y && column) {  // (places beyond the rows and the columns do not matter)
+        const T* const from = Y + (int64_t)(row0 + pm) * p.y_sr + c0 + pc;
+        for (int q = 0; q < EXPAND_ROWS / RI; ++q)
+          if (pm + q * RI < rows) cp16(y_to + q * RI * S::XP, from + q * y_step);
       }
-    }
-    const T* const t = reinterpret_cast<const T*>(p.t);
-    for (int m = qm; m < EXPAND_ROWS; m += TI) {
-      const bool real = qc < p.r && m < rows;
-      const T* const from = real ? t + (int64_t)(row0 + m) * p.r + qc : t;
-      cp16(t_to + (m - qm) * S::RPP, from, real);
-      cp16(t_to + (EXPAND_ROWS + m - qm) * S::RPP, real ? from + (int64_t)p.n_rows * p.r : t, real);
+      if (TRANS) {  // by rank, columns contiguous; what lies beyond the rank is 0
+        for (int m = pm; m < RP; m += RI) {
+          const bool real = m < p.r && column;
+          cp16(v_at + m * S::XP + pc * 2, real ? V + (int64_t)m * p.N + c0 + pc : V, real);
+        }
+      } else {
+        for (int m = qm; m < EXPAND_COLS; m += TI) {
+          const bool real = qc < p.r && c0 + m < p.N;
+          cp16(v_at + m * S::RPP + qc * 2, real ? V + (int64_t)(c0 + m) * p.r + qc : V, real);
+        }
+      }
+      for (int m = qm; m < EXPAND_ROWS; m += TI) {
+        const bool real = qc < p.r && m < rows;
+        const T* const from = real ? t + (int64_t)(m - qm) * p.r : V;
+        cp16(t_to + (m - qm) * S::RPP, from, real);
+        cp16(t_to + (EXPAND_ROWS + m - qm) * S::RPP, real ? from + lo_step : V, real);
+      }
     }
     if (std::is_same<T, __half>::value && tid < rows) row_by[tid] = p.t_by[row0 + tid];
     cp_commit();
