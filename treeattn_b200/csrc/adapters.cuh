@@ -485,58 +485,63 @@ template <typename T, int RP, int NT, bool TRANS>
 __device__ __forceinline__ void add_product(unsigned char* tile, int xp, uint32_t vs, int vp, uint32_t hi, uint32_t lo, int tp, const float* row_by,
                                             bool with_y, int m0, int n0, int lane, T* out, int64_t o_sr, int rows, int cols) {
   constexpr bool FROM_Y = !std::is_same<T, __half>::value;  // the sum begins with y (f16's rows have a factor of their own)
-  const uint32_t y_at = smem_u32(tile) + (m0 + (lane & 15)) * xp + (n0 + (lane >> 4) * 8) * 2;
+  uint32_t y_at = smem_u32(tile) + (m0 + (lane & 15)) * xp + (n0 + (lane >> 4) * 8) * 2;
   const uint32_t t_at = (m0 + (lane & 15)) * tp + (lane >> 4) * 16;
-  float o[NT][4];
-  auto begin = [&](auto set) {
+  constexpr int PN = RP <= 32 ? NT / 2 : NT;  // (small ranks in two parts: fewer registers, more warps' loads in flight)
+#pragma unroll 1
+  for (int part = 0; part < NT; part += PN, y_at += PN * 16, n0 += PN * 8) {
+    float o[PN][4];
+    auto begin = [&](auto set) {
 #pragma unroll
-    for (int n = 0; n < NT; n += 2) {
-      uint32_t y[4] = {0u, 0u, 0u, 0u};
-      if (with_y) ldsm4(y, y_at + n * 16);
+      for (int n = 0; n < PN; n += 2) {
+        uint32_t y[4] = {0u, 0u, 0u, 0u};
+        if (with_y) ldsm4(y, y_at + n * 16);
 #pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        const float2 f = widen2<T>(y[h]);
-        set(o[n + h / 2][h % 2 * 2], f.x, h % 2);
-        set(o[n + h / 2][h % 2 * 2 + 1], f.y, h % 2);
+        for (int h = 0; h < 4; ++h) {
+          const float2 f = widen2<T>(y[h]);
+          set(o[n + h / 2][h % 2 * 2], f.x, h % 2);
+          set(o[n + h / 2][h % 2 * 2 + 1], f.y, h % 2);
+        }
+      }
+    };
+    if (FROM_Y) {
+      begin([](float& a, float y, int) { a = y; });
+    } else {
+#pragma unroll
+      for (int n = 0; n < PN; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
+    }
+#pragma unroll
+    for (int kk = 0; kk < RP / 16; ++kk) {
+      uint32_t th[4], tl[4];
+      ldsm4(th, hi + t_at + kk * 32);
+      ldsm4(tl, lo + t_at + kk * 32);
+#pragma unroll
+      for (int n = 0; n < PN / 2; ++n) {
+        uint32_t vb[4];
+        if (TRANS)
+          ldsm4t(vb, vs + (kk * 16 + (lane & 15)) * vp + (n0 + n * 16 + (lane >> 4) * 8) * 2);
+        else
+          load_b(vb, vs, vp, n0 + n * 16, kk * 16, lane);
+        mma16<T>(o[2 * n], th, vb[0], vb[1]);
+        mma16<T>(o[2 * n + 1], th, vb[2], vb[3]);
+        mma16<T>(o[2 * n], tl, vb[0], vb[1]);
+        mma16<T>(o[2 * n + 1], tl, vb[2], vb[3]);
       }
     }
-  };
-  if (FROM_Y) {
-    begin([](float& a, float y, int) { a = y; });
-  } else {
+    if (!FROM_Y) {
+      const float by[2] = {row_by[m0 + lane / 4], row_by[m0 + lane / 4 + 8]};
+      begin([&](float& a, float y, int h) { a = fmaf(a, by[h], y); });
+    }
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
-  }
-#pragma unroll
-  for (int kk = 0; kk < RP / 16; ++kk) {
-    uint32_t th[4], tl[4];
-    ldsm4(th, hi + t_at + kk * 32);
-    ldsm4(tl, lo + t_at + kk * 32);
-#pragma unroll
-    for (int n = 0; n < NT / 2; ++n) {
-      uint32_t vb[4];
-      if (TRANS)
-        ldsm4t(vb, vs + (kk * 16 + (lane & 15)) * vp + (n0 + n * 16 + (lane >> 4) * 8) * 2);
-      else
-        load_b(vb, vs, vp, n0 + n * 16, kk * 16, lane);
-      mma16<T>(o[2 * n], th, vb[0], vb[1]);
-      mma16<T>(o[2 * n + 1], th, vb[2], vb[3]);
-      mma16<T>(o[2 * n], tl, vb[0], vb[1]);
-      mma16<T>(o[2 * n + 1], tl, vb[2], vb[3]);
+    for (int n = 0; n < PN; n += 2) {
+      const uint32_t r4[4] = {narrow2<T>(o[n][0], o[n][1]), narrow2<T>(o[n][2], o[n][3]), narrow2<T>(o[n + 1][0], o[n + 1][1]),
+                              narrow2<T>(o[n + 1][2], o[n + 1][3])};
+      stsm4(y_at + n * 16, r4);
     }
   }
-  if (!FROM_Y) {
-    const float by[2] = {row_by[m0 + lane / 4], row_by[m0 + lane / 4 + 8]};
-    begin([&](float& a, float y, int h) { a = fmaf(a, by[h], y); });
-  }
-#pragma unroll
-  for (int n = 0; n < NT; n += 2) {
-    const uint32_t r4[4] = {narrow2<T>(o[n][0], o[n][1]), narrow2<T>(o[n][2], o[n][3]), narrow2<T>(o[n + 1][0], o[n + 1][1]),
-                            narrow2<T>(o[n + 1][2], o[n + 1][3])};
-    stsm4(y_at + n * 16, r4);
-  }
+  n0 -= NT * 8;
   __syncwarp();
   constexpr int STEP = 32 / NT;
   const int m = m0 + lane / NT, c = n0 + lane % NT * 8;
@@ -559,10 +564,11 @@ struct ExpandShape {
 
 // The second product by itself: a CTA adds t's 64 rows times v's 128 columns to y. All that it reads is asked for at once; what it
 // waits for, the other CTAs of its SM work through. It also writes the rows that take nothing (none where out is y). 16384 rows of 2304
-// columns, rank 16: 35 us (150 MB read and written, 4.3 TB/s); rank 128: 87 us, the matrix instructions (two a product) at 0.4 of what
-// they can do. With fragments from memory instead of shared memory: 36 us, and 180 at rank 128, where v is read 4 times as often.
+// columns, rank 16: 31 us (150 MB read and written, 4.9 TB/s; 33 with four CTAs on an SM instead of six); rank 128: 73 us, the matrix
+// instructions (two a product) at half of what they can do. With fragments from memory instead of shared memory: 36 us, and 180 at rank
+// 128, where v is read 4 times as often.
 template <typename T, int RP, bool TRANS>
-__global__ void __launch_bounds__(ADAPTER_THREADS, RP <= 32 ? 4 : 2) adapter_expand_kernel(const __grid_constant__ AdapterParams p) {
+__global__ void __launch_bounds__(ADAPTER_THREADS, RP == 16 ? 6 : RP == 32 ? 5 : RP == 64 ? 3 : 2) adapter_expand_kernel(const __grid_constant__ AdapterParams p) {
   using S = ExpandShape<RP, TRANS>;
   extern __shared__ __align__(16) unsigned char smem[];
   unsigned char *const ys = smem, *const vs = smem + S::Y, *const ts = vs + S::V;
@@ -682,7 +688,7 @@ struct AdapterGradShape {
 // dA and dB: a CTA takes 64 or 128 columns of x or of dy and up to 32 ranks, and sums the products of those columns with u or t over the rows of
 // all sequences that use its adapter. Its warps, and the CTAs of a cluster, take every so many blocks of 16 rows, each through a ring of its
 // own, and wait for no other warp; their sums meet in one order. An adapter that nobody uses gets zeros. 16384 rows of 768 and 2304 columns, rank
-// 16: 37 us (103 MB, 2.8 TB/s; with 64 columns, 128 bytes of a row, 40 us); rank 128: 123 us.
+// 16: 36 us (103 MB, 2.9 TB/s; with 64 columns, 128 bytes of a row, 40 us); rank 128: 107 us.
 template <typename T, int RP>
 __global__ void __launch_bounds__(ADAPTER_THREADS, 2) adapter_grad_kernel(const __grid_constant__ AdapterGradParams p) {
   using S = AdapterGradShape<RP>;
