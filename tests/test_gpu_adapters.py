@@ -232,6 +232,21 @@ def test_values_at_the_ends():
     assert out[:3].isfinite().all() and out[4:].isfinite().all()
 
 
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('rank', [8, 24, 56, 72, 128])
+@pytest.mark.parametrize('rows', [7, 40])
+def test_infinite_rows(dtype, rank, rows):
+    """Where every term of a sum has one sign an infinity in x gives infinities, not NaN: at ranks that are filled up too."""
+    from treeattn_b200.adapters import adapter_add
+    s = _inputs([rows], 64, 72, rank, dtype, na=1, scale=False, seed=2)
+    s = dict(s, a=s['a'].abs() + 0.125, b=s['b'].abs() + 0.125)
+    s['which'][:] = 0
+    s['x'][3, 7] = math.inf
+    out = adapter_add(**s)
+    assert (out[3] == math.inf).all()
+    assert out[:3].isfinite().all() and out[4:].isfinite().all()
+
+
 def test_long_offsets():
     """Rows beyond 2^31 elements from the first."""
     from treeattn_b200.adapters import adapter_add

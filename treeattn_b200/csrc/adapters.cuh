@@ -99,7 +99,7 @@ __device__ __forceinline__ void split_row(const AdapterParams& p, const float* p
   for (int v = 0; v < VL; ++v) {
     const int c = lane + 32 * v;
     s[v] = 0.f;
-    if (c < RP) {
+    if (c < p.r) {  // (ranks that fill it up stay 0: an infinity in x times their zeros would be NaN)
       if (cs > 1)
         for (int q = 0; q < cs; ++q) s[v] += cluster_map(part, q)[m * RP + c];
       else
