@@ -408,6 +408,24 @@ def _hooked(model, s, hook):
             for i, block in enumerate(model.blocks) for name in s.projections]
 
 
+def test_outputs_that_overlap_are_refused():
+    from treeattn_b200.adapters import adapter_add
+    s = _inputs([5], 64, 64, 8, torch.bfloat16)
+    wide = torch.zeros(5 * 64, device='cuda', dtype=torch.bfloat16)
+    for strides in ((0, 1), (32, 1)):
+        out = wide.as_strided((5, 64), strides)
+        with pytest.raises(ValueError, match='overlap'):
+            adapter_add(**s, out=out)
+        with pytest.raises(ValueError, match='overlap'):
+            adapter_add(**dict(s, y=out), out=out)
+        with pytest.raises(ValueError, match='overlap'):
+            adapter_add(**dict(s, y=out, x=s['x'].clone().requires_grad_()), out=out)
+        _near(adapter_add(**dict(s, y=out)), _formula(**dict(s, y=out))['out'], 72, 'expanded y')  # as an input it may
+    one = _inputs([1], 64, 64, 8, torch.bfloat16)
+    out = wide.as_strided((1, 64), (0, 1))
+    _near(adapter_add(**one, out=out), _formula(**one)['out'], 72, 'one row')
+
+
 @pytest.mark.parametrize('attn', ['seg', 'dyn', 'block'])
 def test_set_on_every_model(attn):
     """The set's hooks are adapter_add on each projection's rows with that projection's factors; the frozen model's weights get no

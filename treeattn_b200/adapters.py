@@ -125,8 +125,11 @@ def adapter_add(y, x, a, b, start, which, max_new, scale=None, out=None):
     one order. t = x A^T is summed in fp32 and multiplied with B as two 16-bit numbers; the sum with y is rounded once."""
     dims = _check('adapter_add', y, x, a, b, start, which, scale)
     max_new = int(max_new)
-    if out is not None and out.data_ptr() == x.data_ptr() and x.numel():
-        raise ValueError('adapter_add: the output in x\'s place')
+    if out is not None:
+        if out.data_ptr() == x.data_ptr() and x.numel():
+            raise ValueError('adapter_add: the output in x\'s place')
+        if out.dim() == 2 and out.shape[0] > 1 and out.stride(0) < out.shape[1]:
+            raise ValueError('adapter_add: rows of the output overlap')
     if torch.is_grad_enabled() and (y.requires_grad or x.requires_grad or a.requires_grad or b.requires_grad or
                                     scale is not None and scale.requires_grad):
         if scale is not None and scale.requires_grad:
@@ -143,6 +146,8 @@ def adapter_add(y, x, a, b, start, which, max_new, scale=None, out=None):
         if out.shape != y.shape:
             raise ValueError('adapter_add: out must have y\'s shape')
         _need_cuda('adapter_add', out)
+        if out.get_device() != x.get_device():
+            raise ValueError('adapter_add: tensors on one device (got %s and %s)' % (x.device, out.device))
     return _add(y, x, a, b, start, which, dims, max_new, scale, out)
 
 
