@@ -408,6 +408,42 @@ def _hooked(model, s, hook):
             for i, block in enumerate(model.blocks) for name in s.projections]
 
 
+def test_captured_set():
+    """A captured pass keeps the adapters and row offsets that it was captured with, and what it works with stays in place, whatever
+    the set is used for afterwards; offsets first needed in a capture are none that a later call may find unwritten."""
+    model, cfg = _gpt()
+    model.requires_grad_(False)
+    s = _trained()
+    s.attach(model)
+    x = torch.randn(4, 64, 64, device='cuda').to(torch.bfloat16)
+
+    def blocks(x):
+        for block in model.blocks:
+            x = block(x)
+        return x
+
+    with torch.no_grad():
+        s.use([0, 1, -1, 2])
+        want = blocks(x).clone()
+        s.use([1, 1])
+        two = blocks(x[:2]).clone()
+        s._start.clear()
+        for warm in (False, True):  # the offsets of 2 rows of 64 are first needed in the capture, then kept from before
+            s.use([1, 1])
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                captured = blocks(x[:2])
+            assert torch.equal(blocks(x[:2]), two)  # before any replay
+            s.use([0, 1, -1, 2])
+            for n in range(1, 20):  # other shapes take the kept ones' places
+                s._starts(n, n)
+            held = [torch.full((m,), 7, device='cuda', dtype=torch.int32) for m in (1, 2, 3, 4, 5) for _ in range(64)]
+            assert torch.equal(blocks(x), want)
+            graph.replay()
+            assert torch.equal(captured, two)
+            assert all((h == 7).all() for h in held)
+
+
 def test_outputs_that_overlap_are_refused():
     from treeattn_b200.adapters import adapter_add
     s = _inputs([5], 64, 64, 8, torch.bfloat16)

@@ -178,7 +178,7 @@ class AdapterSet(nn.Module):
                 self.a.append(nn.Parameter((torch.randn(n_adapters, rank, i, device=device) * i ** -0.5).to(dtype)))
                 self.b.append(nn.Parameter(torch.zeros(n_adapters, o, rank, device=device, dtype=dtype)))
         self.register_buffer('scale', torch.full((n_adapters,), (rank if alpha is None else alpha) / rank, device=device))
-        self._which, self._start = None, {}
+        self._which, self._start, self._captured = None, {}, {}
 
     def factors(self, layer, projection):
         """(a, b) of a block's projection, or None where there are none."""
@@ -188,16 +188,30 @@ class AdapterSet(nn.Module):
         return self.a[i], self.b[i]
 
     def _starts(self, B, n):
-        """Row offsets of n rows a sequence (kept for the lengths that come up most)."""
-        key = B, n, self.scale.device
+        """Row offsets of n rows a sequence (kept for the lengths that come up most; copied from the host, so that they are there for
+        every stream). A graph that is being captured forms its own where there are none."""
+        dev = self.scale.device
+        key = B, n, dev
         if key not in self._start:
+            if dev.type == 'cuda' and torch.cuda.is_current_stream_capturing():
+                return torch.arange(B + 1, device=dev, dtype=torch.int32) * n
             if len(self._start) >= 16:
                 self._start.clear()
-            self._start[key] = torch.arange(B + 1, device=self.scale.device, dtype=torch.int32) * n
-        return self._start[key]
+            self._start[key] = (torch.arange(B + 1, dtype=torch.int32) * n).to(dev)
+        return self._held(self._start[key])
+
+    def _held(self, t):
+        """t, which this set may let go while the current stream, or a graph that is being captured, still reads it."""
+        if t.is_cuda:
+            if torch.cuda.is_current_stream_capturing():
+                self._captured[t.data_ptr()] = t
+            else:
+                t.record_stream(torch.cuda.current_stream(t.device))
+        return t
 
     def use(self, which):
-        """The adapters of the next batches of the attached model: whole numbers, -1 for none (None: no adapters at all)."""
+        """The adapters of the next batches of the attached model: whole numbers, -1 for none (None: no adapters at all). A captured pass
+        keeps those that it was captured with."""
         if which is None:
             self._which = None
             return
@@ -235,7 +249,8 @@ class AdapterSet(nn.Module):
             if self._which.shape[0] != B:
                 raise ValueError('AdapterSet: adapters for %d sequences, a batch of %d' % (self._which.shape[0], B))
             a, b = self.factors(layer, projection)
-            rows = adapter_add(y.reshape(B * n, -1), x.reshape(B * n, -1), a, b, self._starts(B, n), self._which, n, scale=self._scale())
+            rows = adapter_add(y.reshape(B * n, -1), x.reshape(B * n, -1), a, b, self._starts(B, n), self._held(self._which), n,
+                               scale=self._scale())
             return rows.view(y.shape)
         return add
 
