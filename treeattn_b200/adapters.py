@@ -197,15 +197,18 @@ class AdapterSet(nn.Module):
                 return torch.arange(B + 1, device=dev, dtype=torch.int32) * n
             if len(self._start) >= 16:
                 self._start.clear()
-            self._start[key] = (torch.arange(B + 1, dtype=torch.int32) * n).to(dev)
+            self._start[key] = self._held((torch.arange(B + 1, dtype=torch.int32) * n).to(dev), made=True)
         return self._held(self._start[key])
 
-    def _held(self, t):
-        """t, which this set may let go while the current stream, or a graph that is being captured, still reads it."""
+    def _held(self, t, made=False):
+        """t, which this set may let go while the current stream (another one than it was made on), or a graph that is being captured, still
+        reads it."""
         if t.is_cuda:
+            if made:
+                t.made_on = _stream(t)
             if torch.cuda.is_current_stream_capturing():
                 self._captured[t.data_ptr()] = t
-            else:
+            elif getattr(t, 'made_on', None) != _stream(t):
                 t.record_stream(torch.cuda.current_stream(t.device))
         return t
 
@@ -218,7 +221,7 @@ class AdapterSet(nn.Module):
         which = torch.as_tensor(which)
         if which.dim() != 1 or which.is_floating_point():
             raise ValueError('AdapterSet: which must be whole numbers, one a sequence')
-        self._which = which.to(self.scale.device, torch.int32, copy=True)
+        self._which = self._held(which.to(self.scale.device, torch.int32, copy=True), made=True)
 
     def _scale(self):
         return self.scale if self.scale.dtype is torch.float32 else self.scale.float()  # (a cast of the whole set casts it too)
