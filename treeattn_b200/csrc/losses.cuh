@@ -3,7 +3,7 @@
 //   term = -min(rho A, clip(rho, lo, hi) A) + kl (exp(ref - logp) - (ref - logp) - 1),  loss = sum over rows of w term
 //   slope = dloss / dlogp = w (-A rho [not clipped] + kl (1 - exp(ref - logp))),  dloss / dz_j = slope / tau ([j = y] - p_j)
 // Everything about a row but its softmax is a handful of scalars, so the gradient's factor is known as soon as the row's sum is: a
-// row is read once, its exponentials stay in registers, and the gradient is written from there. The floor is one read and one write of the
+// row is read once, stays in shared memory, and the gradient is written from there. The floor is one read and one write of the
 // logits; a gradient that waits for the backward pass (16-bit floats of 5 exponent bits, which need the loss's scale
 // before they are rounded) reads them twice.
 #pragma once
