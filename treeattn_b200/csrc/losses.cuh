@@ -208,7 +208,7 @@ __device__ __forceinline__ Share warp_share(const Share& x, float k) {
 // ALIGNED: every row begins and ends on a 16-byte boundary, in the gradient too.
 template <typename T, int THREADS, int MODE, bool ALIGNED>  // MODE 0: log-probabilities, 1: the policy loss, 2: and its gradient
 __global__ void __launch_bounds__(THREADS, (MODE == 2 ? 1024 : 1280) / THREADS) loss_kernel(const __grid_constant__ LossParams a) {
-  constexpr int N = Piece<T>::N, WARPS = THREADS / 32;
+  constexpr int N = Piece<T>::N, WARPS = THREADS / 32, U = 4;
   constexpr bool POLICY = MODE > 0, KEEP = MODE == 2;
   extern __shared__ uint4 share[];
   __shared__ Share s_warp[WARPS];
@@ -221,9 +221,10 @@ __global__ void __launch_bounds__(THREADS, (MODE == 2 ? 1024 : 1280) / THREADS) 
   const float k = a.inv_tau * LOG2E;
   const RowPieces<T> p(row, a.V, ALIGNED);
   const int j0 = rank * a.per, n = min(a.per, p.pieces - j0);  // (n < 1: a share without pieces)
-  // the share's whole pieces are [i0, i1); one that the row begins or ends in belongs to thread 0 or 1
+  // the share's whole pieces are [i0, i1); one that the row begins or ends in belongs to a thread of the second or third warp (the first has
+  // the row's scalars to read)
   const int i0 = !ALIGNED && n > 0 && p.first == j0, i1 = !ALIGNED && p.last == j0 + n - 1 && n > i0 ? n - 1 : n;
-  const int edge = ALIGNED ? -1 : tid == 0 && i0 ? 0 : tid == 1 && n > 0 && i1 < n ? n - 1 : -1;
+  const int edge = ALIGNED ? -1 : tid == 32 && i0 ? 0 : tid == 64 && n > 0 && i1 < n ? n - 1 : -1;
   pdl_wait();
   pdl_launch_dependents();
   T* const out = MODE == 2 ? reinterpret_cast<T*>(a.grad) + b * a.g_sb + t * a.g_st : nullptr;
@@ -246,9 +247,11 @@ __global__ void __launch_bounds__(THREADS, (MODE == 2 ? 1024 : 1280) / THREADS) 
   }
   // the row's scalars, while it arrives
   int64_t y = -1;
-  float zy = 0.f, old = 0.f, adv = 0.f, ref = 0.f;
-  if (tid == 0) {
-    y = a.tokens[b * a.t_sb + t * a.t_st];
+  T zy = from_f32<T>(0.f);
+  float old = 0.f, adv = 0.f, ref = 0.f;
+  if (tid == 0) y = a.tokens[b * a.t_sb + t * a.t_st];
+  auto scalars = [&]() {
+    if (tid != 0) return;
     if (POLICY) {
       old = a.old.at(b, t);
       adv = a.adv.at(b, t);
@@ -257,15 +260,15 @@ __global__ void __launch_bounds__(THREADS, (MODE == 2 ? 1024 : 1280) / THREADS) 
     if (y < 0 || y >= a.V) {
       if (rank == 0) record_error(DEV_INDEX_RANGE, K_LOSS, r, (int)y);
       y = -1;
-      zy = __int_as_float(0x7fc00000);
     } else {
-      zy = to_f32(row[y]);
+      zy = row[y];
     }
+  };
+  if (KEEP) {
+    scalars();
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
   }
-  if (KEEP) asm volatile("cp.async.wait_group 0;" ::: "memory");
   auto piece = [&](int j) { return KEEP ? share[j] : load_once(from + j); };  // a whole one
-  uint4 cut = make_uint4(0u, 0u, 0u, 0u);
-  if (edge >= 0) cut = KEEP ? share[edge] : p.edge(j0 + edge);
   auto largest = [](const uint4& v) { return Piece<T>::top(Piece<T>::max2(Piece<T>::max2(v.x, v.y), Piece<T>::max2(v.z, v.w))); };
   auto piece_sum = [&](const uint4& v, const Ref& m) {
     float z[N];
@@ -285,7 +288,6 @@ __global__ void __launch_bounds__(THREADS, (MODE == 2 ? 1024 : 1280) / THREADS) 
   };
   auto sum_about = [&](const Ref& m, int j, float s) {
     if (!KEEP) {
-      constexpr int U = 4;
       for (; j + (U - 1) * THREADS < i1; j += U * THREADS) {
         uint4 v[U];
 #pragma unroll
@@ -295,19 +297,36 @@ __global__ void __launch_bounds__(THREADS, (MODE == 2 ? 1024 : 1280) / THREADS) 
       }
     }
     for (; j < i1; j += THREADS) s += piece_sum(piece(j), m);
-    return edge >= 0 ? s + piece_sum(cut, m) : s;
+    return s;
   };
   float top = 0.f, s = 0.f;
   const int first = i0 + tid;
+  uint4 v[U], cut;
+  if (!KEEP) {  // the first pieces are asked for before anything is waited for, the scalars then
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (first + u * THREADS < i1) v[u] = piece(first + u * THREADS);
+    scalars();
+  }
+  if (edge >= 0) cut = KEEP ? share[edge] : p.edge(j0 + edge);
   if (first < i1 || edge >= 0) {
-    top = largest(first < i1 ? piece(first) : cut);
+    top = largest(first < i1 ? KEEP ? piece(first) : v[0] : cut);
     if (!(top > -INFINITY)) top = 0.f;  // nothing to take off
-    s = sum_about(Ref(top, k), first, 0.f);
+    const Ref m(top, k);
+    if (!KEEP) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (first + u * THREADS < i1) s += piece_sum(v[u], m);
+    }
+    s = sum_about(m, KEEP ? first : first + U * THREADS, s);
+    if (edge >= 0) s += piece_sum(cut, m);
     if (!(s >= 0.5f && s < 1.2676506e30f)) {
       top = edge >= 0 ? largest(cut) : -INFINITY;
       for (int j = first; j < i1; j += THREADS) top = fmaxf(top, largest(piece(j)));
       if (!(top > -INFINITY)) top = 0.f;
-      s = sum_about(Ref(top, k), first, 0.f);
+      const Ref again(top, k);
+      s = sum_about(again, first, 0.f);
+      if (edge >= 0) s += piece_sum(cut, again);
     }
   }
   __syncwarp();
@@ -334,7 +353,7 @@ __global__ void __launch_bounds__(THREADS, (MODE == 2 ? 1024 : 1280) / THREADS) 
     }
     sum = warp_share(sum, k);
     if (tid == 0) {
-      const float logp = Ref(sum.m, k).of(zy, k) * LN2 - logf(sum.s);
+      const float logp = Ref(sum.m, k).of(y < 0 ? __int_as_float(0x7fc00000) : to_f32(zy), k) * LN2 - logf(sum.s);
       float slope = 0.f;
       if (POLICY) {
         const float rho = expf(logp - old);
