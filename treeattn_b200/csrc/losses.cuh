@@ -203,11 +203,13 @@ __device__ __forceinline__ Share warp_share(const Share& x, float k) {
 // 16 bits of an element instead of 32 and two CTAs on an SM: one waits for its row while the other computes. (Kept in registers
 // instead, with the next row read ahead, an element costs less, but the CTAs that a row then needs wait for each other: 810 us against 290
 // for 8 x 1024 x 50304 bf16, a quarter of it not counted.)
-// Without a gradient nothing is kept, and the row is summed as it arrives: 8192 rows of 50304 bf16 in 130 us, 6.3 TB/s. With it 2048 rows
-// take 85 us, 4.9 TB/s read and written, the issue slots half full: it is the two CTAs' phases that do not always overlap.
+// Without a gradient nothing is kept, and the row is summed as it arrives: 8192 rows of 50304 bf16 in 128 us, 6.4 TB/s. With it 2048 rows
+// take 83 us, 5.0 TB/s read and written, the issue slots half full: it is the two CTAs' phases that do not always overlap.
 // ALIGNED: every row begins and ends on a 16-byte boundary, in the gradient too.
+// (Six CTAs of 256 threads on an SM where that costs nothing else, five otherwise: 8192 x 50304 bf16 133 against 135 us, 2048 x 50304 fp32 76
+// against 74.)
 template <typename T, int THREADS, int MODE, bool ALIGNED>  // MODE 0: log-probabilities, 1: the policy loss, 2: and its gradient
-__global__ void __launch_bounds__(THREADS, (MODE == 2 ? 1024 : 1280) / THREADS) loss_kernel(const __grid_constant__ LossParams a) {
+__global__ void __launch_bounds__(THREADS, (MODE == 2 ? 1024 : MODE == 0 && ALIGNED && sizeof(T) == 2 ? 1536 : 1280) / THREADS) loss_kernel(const __grid_constant__ LossParams a) {
   constexpr int N = Piece<T>::N, WARPS = THREADS / 32, U = 4;
   constexpr bool POLICY = MODE > 0, KEEP = MODE == 2;
   extern __shared__ uint4 share[];
