@@ -564,11 +564,12 @@ struct ExpandShape {
 
 // The second product by itself: a CTA adds t's 64 rows times v's 128 columns to y. All that it reads is asked for at once; what it
 // waits for, the other CTAs of its SM work through. It also writes the rows that take nothing (none where out is y). 16384 rows of 2304
-// columns, rank 16: 31 us (150 MB read and written, 4.9 TB/s; 33 with four CTAs on an SM instead of six); rank 128: 73 us, the matrix
+// columns, rank 16: 32 us (150 MB read and written, 4.7 TB/s; 34 with four CTAs on an SM instead of six); rank 128: 75 us, the matrix
 // instructions (two a product) at half of what they can do. With fragments from memory instead of shared memory: 36 us, and 180 at rank
 // 128, where v is read 4 times as often.
 template <typename T, int RP, bool TRANS>
-__global__ void __launch_bounds__(ADAPTER_THREADS, RP == 16 ? 6 : RP == 32 ? 5 : RP == 64 ? 3 : 2) adapter_expand_kernel(const __grid_constant__ AdapterParams p) {
+__global__ void __launch_bounds__(ADAPTER_THREADS, RP == 16 ? 6 : RP == 32 ? 5 : RP == 64 ? 3 : 2)
+    adapter_expand_kernel(const __grid_constant__ AdapterParams p) {
   using S = ExpandShape<RP, TRANS>;
   extern __shared__ __align__(16) unsigned char smem[];
   unsigned char *const ys = smem, *const vs = smem + S::Y, *const ts = vs + S::V;
@@ -688,7 +689,7 @@ struct AdapterGradShape {
 // dA and dB: a CTA takes 64 or 128 columns of x or of dy and up to 32 ranks, and sums the products of those columns with u or t over the rows of
 // all sequences that use its adapter. Its warps, and the CTAs of a cluster, take every so many blocks of 16 rows, each through a ring of its
 // own, and wait for no other warp; their sums meet in one order. An adapter that nobody uses gets zeros. 16384 rows of 768 and 2304 columns, rank
-// 16: 36 us (103 MB, 2.9 TB/s; with 64 columns, 128 bytes of a row, 40 us); rank 128: 107 us.
+// 16: 36 us (103 MB, 2.8 TB/s; with 64 columns, 128 bytes of a row, 40 us); rank 128: 110 us.
 template <typename T, int RP>
 __global__ void __launch_bounds__(ADAPTER_THREADS, 2) adapter_grad_kernel(const __grid_constant__ AdapterGradParams p) {
   using S = AdapterGradShape<RP>;

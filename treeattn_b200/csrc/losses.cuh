@@ -209,7 +209,8 @@ __device__ __forceinline__ Share warp_share(const Share& x, float k) {
 // (Six CTAs of 256 threads on an SM where that costs nothing else, five otherwise: 8192 x 50304 bf16 133 against 135 us, 2048 x 50304 fp32 76
 // against 74.)
 template <typename T, int THREADS, int MODE, bool ALIGNED>  // MODE 0: log-probabilities, 1: the policy loss, 2: and its gradient
-__global__ void __launch_bounds__(THREADS, (MODE == 2 ? 1024 : MODE == 0 && ALIGNED && sizeof(T) == 2 ? 1536 : 1280) / THREADS) loss_kernel(const __grid_constant__ LossParams a) {
+__global__ void __launch_bounds__(THREADS, (MODE == 2 ? 1024 : MODE == 0 && ALIGNED && sizeof(T) == 2 ? 1536 : 1280) / THREADS)
+    loss_kernel(const __grid_constant__ LossParams a) {
   constexpr int N = Piece<T>::N, WARPS = THREADS / 32, U = 4;
   constexpr bool POLICY = MODE > 0, KEEP = MODE == 2;
   extern __shared__ uint4 share[];

@@ -97,8 +97,8 @@ class _TokenLogp(torch.autograd.Function):
         logits, tokens, stats = ctx.saved_tensors
         grad = _grad_like(logits)
         s = dlogp.stride()
-        _logits_grad(logits, _logits('token_logp', logits, tokens), stats, dlogp.data_ptr(), s if len(s) == 2 else (0, s[0]), 1.0 / ctx.temperature, ctx.temperature, None,
-                     False, grad)
+        _logits_grad(logits, _logits('token_logp', logits, tokens), stats, dlogp.data_ptr(), s if len(s) == 2 else (0, s[0]),
+                     1.0 / ctx.temperature, ctx.temperature, None, False, grad)
         return grad, None, None
 
 
