@@ -26,7 +26,7 @@ def test_rejected_arguments_without_gpu():
         return lib.ta_adapter_bwd(dy, 64, x, xsr, a, p, None, 3, 128, 64, r, 9, p, p, 2, 4, t, u, dx, 128, da, db, None)
 
     for kw, what in ((dict(dy=None), 'null'), (dict(x=None), 'null'), (dict(t=None), 'null'), (dict(u=None), 'null'), (dict(a=None), 'null'),
-                     (dict(dx=p + 8), 'aligned'), (dict(xsr=4), 'aligned'), (dict(u=p + 8), 'aligned'), (dict(r=7), 'rank')):
+                     (dict(dx=p + 8), 'aligned'), (dict(da=p + 8), 'aligned'), (dict(db=p + 2), 'aligned'), (dict(xsr=4), 'aligned'), (dict(u=p + 8), 'aligned'), (dict(r=7), 'rank')):
         assert bwd(**kw) == _lib.TA_ERR_ARG
         assert 'ta_adapter_bwd' in _lib.last_error() and what in _lib.last_error(), (kw, _lib.last_error())
     assert bwd(dx=None, da=None, db=None) == _lib.TA_OK

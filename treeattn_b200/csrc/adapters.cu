@@ -170,7 +170,7 @@ int ta_adapter_bwd(const void* dy, int64_t d_sr, const void* x, int64_t x_sr, co
   if (n_rows && (!dy || (da && !x) || (db && !t) || ((dx || da) && (!a || !b || !u))))
     return fail(TA_ERR_ARG, "%s: null pointer", who);
   if (!rows_aligned(dy, 2, {d_sr}) || (da && !rows_aligned(x, 2, {x_sr})) || (dx && !rows_aligned(dx, 2, {dx_sr})) || !aligned16(a) ||
-      !aligned16(b) || !aligned16(t) || !aligned16(u))
+      !aligned16(b) || !aligned16(t) || !aligned16(u) || !aligned16(da) || !aligned16(db))
     return fail(TA_ERR_ARG, "%s: rows and factors must be 16-byte aligned", who);
   const cudaStream_t st = S(stream);
   if ((dx || da) && n_rows > 0) {  // u = s dy B, dx = u A: the forward's kernels with the factors' other sides

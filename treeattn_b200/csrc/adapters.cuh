@@ -688,8 +688,9 @@ struct AdapterGradShape {
 
 // dA and dB: a CTA takes 64 or 128 columns of x or of dy and up to 32 ranks, and sums the products of those columns with u or t over the rows of
 // all sequences that use its adapter. Its warps, and the CTAs of a cluster, take every so many blocks of 16 rows, each through a ring of its
-// own, and wait for no other warp; their sums meet in one order. An adapter that nobody uses gets zeros. 16384 rows of 768 and 2304 columns, rank
-// 16: 36 us (103 MB, 2.8 TB/s; with 64 columns, 128 bytes of a row, 40 us); rank 128: 110 us.
+// own, and wait for no other warp; their sums, those of warps that had a block, meet in one order. An adapter that nobody uses gets zeros. 16384 rows of 768 and 2304 columns, rank
+// 16: 36 us (103 MB, 2.8 TB/s; with 64 columns, 128 bytes of a row, 40 us); rank 128: 110 us. (16 sequences of up to 27 rows, 33 adapters
+// of rank 120, 6120 -> 200, all five kernels: 138 us, 355 with all eight warps' sums and two bytes a store.)
 template <typename T, int RP>
 __global__ void __launch_bounds__(ADAPTER_THREADS, 2) adapter_grad_kernel(const __grid_constant__ AdapterGradParams p) {
   using S = AdapterGradShape<RP>;
@@ -784,6 +785,7 @@ __global__ void __launch_bounds__(ADAPTER_THREADS, 2) adapter_grad_kernel(const 
       multiply();
     }
   };
+  int total = 0;  // the adapter's blocks
   {
     // this warp's blocks of 16 rows: every (8 cs)th of the adapter's, sequence after sequence
     const int turns = 8 * cs;
@@ -801,6 +803,7 @@ __global__ void __launch_bounds__(ADAPTER_THREADS, 2) adapter_grad_kernel(const 
         some &= some - 1;
         const int q0 = __shfl_sync(0xffffffffu, s0, from), q1 = __shfl_sync(0xffffffffu, s1, from);
         const int n = (q1 - q0 + 15) / 16;
+        total += n;
         for (; turn < n; turn += turns) ask(q0 + turn * 16, q1 - q0 - turn * 16);
         turn -= n;
       }
@@ -809,41 +812,57 @@ __global__ void __launch_bounds__(ADAPTER_THREADS, 2) adapter_grad_kernel(const 
     __syncwarp();
     while (held > 0) multiply();
   }
-  __syncthreads();  // the warps' sums go where the rows were
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      float* const to = part + (warp * MC + m * 16 + lane / 4) * RT + n * 8 + (lane & 3) * 2;
-      *reinterpret_cast<float2*>(to) = make_float2(acc[m][n][0], acc[m][n][1]);
-      *reinterpret_cast<float2*>(to + 8 * RT) = make_float2(acc[m][n][2], acc[m][n][3]);
-    }
+  // the warps that had a block (one at least) have sums; they go where the rows were
+  const int warps = max(1, min(8, total - rank * 8));
   __syncthreads();
+  if (warp < warps) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float* const to = part + (warp * MC + m * 16 + lane / 4) * RT + n * 8 + (lane & 3) * 2;
+        *reinterpret_cast<float2*>(to) = make_float2(acc[m][n][0], acc[m][n][1]);
+        *reinterpret_cast<float2*>(to + 8 * RT) = make_float2(acc[m][n][2], acc[m][n][3]);
+      }
+  }
+  __syncthreads();
+  const int ranks = min(RT, p.r - rank0);
+  T* const da = reinterpret_cast<T*>(p.da) + ((int64_t)a * p.r + rank0) * p.K + c0;
+  T* const db = reinterpret_cast<T*>(p.db) + ((int64_t)a * p.N + c0) * p.r + rank0;
+  if (cs == 1) {  // dA as [r][K], dB as [N][r], eight elements at a time
+    for (int e = tid; e < MC * RT / 8; e += ADAPTER_THREADS) {
+      const int c = of_a ? e % RT : e % (RT / 8) * 8, m = of_a ? e / RT * 8 : e / (RT / 8);
+      if (c >= ranks || c0 + m >= C) continue;
+      const int at = m * RT + c, by = of_a ? RT : 1;
+      float s[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[i] = part[at + i * by];
+      for (int w = 1; w < warps; ++w)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[i] += part[w * MC * RT + at + i * by];
+      const uint4 v = make_uint4(narrow2<T>(s[0], s[1]), narrow2<T>(s[2], s[3]), narrow2<T>(s[4], s[5]), narrow2<T>(s[6], s[7]));
+      *reinterpret_cast<uint4*>(of_a ? da + (int64_t)c * p.K + m : db + (int64_t)m * p.r + c) = v;
+    }
+    return;
+  }
   for (int e = tid; e < MC * RT; e += ADAPTER_THREADS) {
     float s = part[e];
 #pragma unroll
-    for (int w = 1; w < 8; ++w) s += part[w * MC * RT + e];
+    for (int w = 1; w < 8; ++w)
+      if (w < warps) s += part[w * MC * RT + e];
     part[e] = s;
   }
-  if (cs > 1)
-    cluster_sync_all();
-  else
-    __syncthreads();
-  // each CTA finishes a share of the columns: dA as [r][K], dB as [N][r]
-  const int m0 = MC * rank / cs, m1 = MC * (rank + 1) / cs, per = m1 - m0, ranks = min(RT, p.r - rank0);
+  cluster_sync_all();
+  // each CTA finishes a share of the columns
+  const int m0 = MC * rank / cs, m1 = MC * (rank + 1) / cs, per = m1 - m0;
   for (int e = tid; e < per * ranks; e += ADAPTER_THREADS) {
     const int m = m0 + (of_a ? e % per : e / ranks), c = of_a ? e / per : e % ranks;
     float s = 0.f;
-    for (int q = 0; q < cs; ++q) s += (cs > 1 ? cluster_map(part, q) : part)[m * RT + c];
-    if (c0 + m < C) {
-      if (of_a)
-        reinterpret_cast<T*>(p.da)[((int64_t)a * p.r + rank0 + c) * p.K + c0 + m] = from_f32<T>(s);
-      else
-        reinterpret_cast<T*>(p.db)[((int64_t)a * p.N + c0 + m) * p.r + rank0 + c] = from_f32<T>(s);
-    }
+    for (int q = 0; q < cs; ++q) s += cluster_map(part, q)[m * RT + c];
+    if (c0 + m < C) (of_a ? da[(int64_t)c * p.K + m] : db[(int64_t)m * p.r + c]) = from_f32<T>(s);
   }
   __syncwarp();
-  if (cs > 1) cluster_sync_all();  // the others have read this CTA's part
+  cluster_sync_all();  // the others have read this CTA's part
 }
 
 }  // namespace ta
