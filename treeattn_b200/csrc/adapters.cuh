@@ -686,11 +686,12 @@ struct AdapterGradShape {
   static constexpr int BYTES = RING > PART ? RING : PART;     // (the warps' sums lie where the rows were)
 };
 
-// dA and dB: a CTA takes 64 or 128 columns of x or of dy and up to 32 ranks, and sums the products of those columns with u or t over the rows of
-// all sequences that use its adapter. Its warps, and the CTAs of a cluster, take every so many blocks of 16 rows, each through a ring of its
-// own, and wait for no other warp; their sums, those of warps that had a block, meet in one order. An adapter that nobody uses gets zeros. 16384 rows of 768 and 2304 columns, rank
-// 16: 36 us (103 MB, 2.8 TB/s; with 64 columns, 128 bytes of a row, 40 us); rank 128: 110 us. (16 sequences of up to 27 rows, 33 adapters
-// of rank 120, 6120 -> 200, all five kernels: 138 us, 355 with all eight warps' sums and two bytes a store.)
+// dA and dB: a CTA takes 64 or 128 columns of x or of dy and up to 32 ranks, and sums the products of those columns with u or t over the
+// rows of all sequences that use its adapter. Its warps, and the CTAs of a cluster, take every so many blocks of 16 rows, each through a
+// ring of its own, and wait for no other warp; their sums, those of warps that had a block, meet in one order. An adapter that nobody uses
+// gets zeros. 16384 rows of 768 and 2304 columns, rank 16: 36 us (103 MB, 2.8 TB/s; with 64 columns, 128 bytes of a row, 40 us); rank
+// 128: 110 us. 16 sequences of up to 27 rows, 33 adapters of rank 120, 6120 -> 200, all five kernels: 129 us (355 with the sums of all warps
+// and two bytes a store).
 template <typename T, int RP>
 __global__ void __launch_bounds__(ADAPTER_THREADS, 2) adapter_grad_kernel(const __grid_constant__ AdapterGradParams p) {
   using S = AdapterGradShape<RP>;
@@ -812,6 +813,22 @@ __global__ void __launch_bounds__(ADAPTER_THREADS, 2) adapter_grad_kernel(const 
     __syncwarp();
     while (held > 0) multiply();
   }
+  const int ranks = min(RT, p.r - rank0);
+  T* const da = reinterpret_cast<T*>(p.da) + ((int64_t)a * p.r + rank0) * p.K + c0;
+  T* const db = reinterpret_cast<T*>(p.db) + ((int64_t)a * p.N + c0) * p.r + rank0;
+  // eight elements of the outputs, dA as [r][K] and dB as [N][r]: the first's rank and column
+  auto eight = [&](int e, int& c, int& m) {
+    c = of_a ? e % RT : e % (RT / 8) * 8;
+    m = of_a ? e / RT * 8 : e / (RT / 8);
+    return c < ranks && c0 + m < C;
+  };
+  auto put8 = [&](int c, int m, const uint4& v) { *reinterpret_cast<uint4*>(of_a ? da + (int64_t)c * p.K + m : db + (int64_t)m * p.r + c) = v; };
+  int c, m;
+  if (total == 0) {  // (in all CTAs of a cluster)
+    for (int e = rank * ADAPTER_THREADS + tid; e < MC * RT / 8; e += cs * ADAPTER_THREADS)
+      if (eight(e, c, m)) put8(c, m, make_uint4(0u, 0u, 0u, 0u));
+    return;
+  }
   // the warps that had a block (one at least) have sums; they go where the rows were
   const int warps = max(1, min(8, total - rank * 8));
   __syncthreads();
@@ -826,13 +843,9 @@ __global__ void __launch_bounds__(ADAPTER_THREADS, 2) adapter_grad_kernel(const 
       }
   }
   __syncthreads();
-  const int ranks = min(RT, p.r - rank0);
-  T* const da = reinterpret_cast<T*>(p.da) + ((int64_t)a * p.r + rank0) * p.K + c0;
-  T* const db = reinterpret_cast<T*>(p.db) + ((int64_t)a * p.N + c0) * p.r + rank0;
-  if (cs == 1) {  // dA as [r][K], dB as [N][r], eight elements at a time
+  if (cs == 1) {
     for (int e = tid; e < MC * RT / 8; e += ADAPTER_THREADS) {
-      const int c = of_a ? e % RT : e % (RT / 8) * 8, m = of_a ? e / RT * 8 : e / (RT / 8);
-      if (c >= ranks || c0 + m >= C) continue;
+      if (!eight(e, c, m)) continue;
       const int at = m * RT + c, by = of_a ? RT : 1;
       float s[8];
 #pragma unroll
@@ -840,8 +853,7 @@ __global__ void __launch_bounds__(ADAPTER_THREADS, 2) adapter_grad_kernel(const 
       for (int w = 1; w < warps; ++w)
 #pragma unroll
         for (int i = 0; i < 8; ++i) s[i] += part[w * MC * RT + at + i * by];
-      const uint4 v = make_uint4(narrow2<T>(s[0], s[1]), narrow2<T>(s[2], s[3]), narrow2<T>(s[4], s[5]), narrow2<T>(s[6], s[7]));
-      *reinterpret_cast<uint4*>(of_a ? da + (int64_t)c * p.K + m : db + (int64_t)m * p.r + c) = v;
+      put8(c, m, make_uint4(narrow2<T>(s[0], s[1]), narrow2<T>(s[2], s[3]), narrow2<T>(s[4], s[5]), narrow2<T>(s[6], s[7])));
     }
     return;
   }
@@ -856,7 +868,8 @@ __global__ void __launch_bounds__(ADAPTER_THREADS, 2) adapter_grad_kernel(const 
   // each CTA finishes a share of the columns
   const int m0 = MC * rank / cs, m1 = MC * (rank + 1) / cs, per = m1 - m0;
   for (int e = tid; e < per * ranks; e += ADAPTER_THREADS) {
-    const int m = m0 + (of_a ? e % per : e / ranks), c = of_a ? e / per : e % ranks;
+    m = m0 + (of_a ? e % per : e / ranks);
+    c = of_a ? e / per : e % ranks;
     float s = 0.f;
     for (int q = 0; q < cs; ++q) s += cluster_map(part, q)[m * RT + c];
     if (c0 + m < C) (of_a ? da[(int64_t)c * p.K + m] : db[(int64_t)m * p.r + c]) = from_f32<T>(s);
