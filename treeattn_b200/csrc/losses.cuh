@@ -233,22 +233,17 @@ __global__ void __launch_bounds__(THREADS, (MODE == 2 ? 1024 : MODE == 0 && ALIG
   T* const out = MODE == 2 ? reinterpret_cast<T*>(a.grad) + b * a.g_sb + t * a.g_st : nullptr;
   const GradRow<T, ALIGNED> g(p, out);
   float w = 1.f;
-  if (POLICY) w = a.weight.p ? a.weight.at(b, t) : a.w0;
-  const uint4* const from = p.at(j0);
-  const int first = i0 + tid, ahead = min(i1, first + 4 * THREADS);
-  if (KEEP)  // the first pieces are asked for before it is known whether the row counts
-    for (int j = first; j < ahead; j += THREADS)
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(share + j)), "l"(from + j) : "memory");
   if (POLICY) {
+    w = a.weight.p ? a.weight.at(b, t) : a.w0;
     if (w == 0.f) {  // not counted, whatever is in it (the same in all threads of the cluster)
       if (MODE == 2) g.zeros(j0, i0 + tid, i1, THREADS, edge);
       if (rank == 0 && tid == 0) a.logp[r] = a.top[r] = a.tot[r] = a.slope[r] = a.term[r] = 0.f;
-      if (KEEP) asm volatile("cp.async.wait_all;" ::: "memory");
       return;
     }
   }
+  const uint4* const from = p.at(j0);
   if (KEEP) {
-    for (int j = first + 4 * THREADS; j < i1; j += THREADS)
+    for (int j = i0 + tid; j < i1; j += THREADS)
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(share + j)), "l"(from + j) : "memory");
     if (edge >= 0) share[edge] = p.edge(j0 + edge);
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -308,6 +303,7 @@ __global__ void __launch_bounds__(THREADS, (MODE == 2 ? 1024 : MODE == 0 && ALIG
     return s;
   };
   float top = 0.f, s = 0.f;
+  const int first = i0 + tid;
   uint4 v[U], cut;
   if (!KEEP) {  // the first pieces are asked for before anything is waited for, the scalars then
 #pragma unroll
