@@ -364,3 +364,70 @@ def test_training_a_model_on_its_answers():
     assert abs(float(loss.detach()) - float(want.detach())) < 1e-5
     for n, p in model.named_parameters():
         assert (got[n] - p.grad).abs().max() <= 1e-4 * max(float(p.grad.abs().max()), 1e-3), n
+
+
+def _banned(B, T, V, dtype, value, seed):
+    """Rows whose words are banned by a finite value but for a few, in different places of the row; the tokens are among those."""
+    logits, tokens, old, adv, ref, weight = _inputs(B, T, V, dtype, seed=seed)
+    free = torch.zeros(B, T, V, device='cuda', dtype=torch.bool)
+    for i in range(B * T):
+        at = (i * 7919 * 13) % (V - 40)
+        free.view(B * T, V)[i, at:at + 40] = True
+        tokens.view(-1)[i] = at + i % 40
+    z = logits.double()
+    lp = z.masked_fill(~free, -math.inf).log_softmax(-1).gather(-1, tokens[..., None])[..., 0].float()
+    shift = lp - z.log_softmax(-1).gather(-1, tokens[..., None])[..., 0].float()
+    return logits.masked_fill(~free, value), free, tokens, old + shift, adv, ref + shift, weight.clamp(min=1e-3)
+
+
+@pytest.mark.parametrize('value', [-1e4, -1e9, -1e10, -1e12, -1e20, -1e29, -1e30, -3e38])
+@pytest.mark.parametrize('dtype', ['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('B,T,V', [(1, 2, 50304), (2, 200, 4099), (1, 1, 200003)])
+def test_words_banned_by_a_finite_value(B, T, V, dtype, value):
+    """Whole pieces, threads' and CTAs' shares of a row hold one large negative number: its words weigh nothing, the others what they
+    weigh among themselves. A banned word lies so far off that its probability is 0 in 64 bits too."""
+    from treeattn_b200.losses import policy_loss, token_logp
+    if dtype == 'f16' and value < -6e4:
+        value = -6e4
+    logits, free, tokens, old, adv, ref, weight = _banned(B, T, V, dtype, value, seed=V + 3)
+    # (the spread is the free words')
+    e = _logp_error(torch.where(free, logits, 0), 1.0)
+    rl, rp, rg = _reference(logits, tokens, old, adv, ref, weight, 0.2, 0.28, 0.05, 1.0)
+    rho = (rp - old.double()).exp()
+    size = weight.double() * (adv.double().abs() * rho + 0.05 * (1 + (ref.double() - rp).exp()))
+    edge = ((rho - 0.8).abs() < 4 * e) | ((rho - 1.28).abs() < 4 * e)
+    p = logits.double().softmax(-1)
+    hot = torch.nn.functional.one_hot(tokens, V).double()
+    least = {'f32': 2.0 ** -126, 'bf16': 2.0 ** -126, 'f16': 2.0 ** -24}[dtype]
+    tol = rg.abs() * torch.finfo(logits.dtype).eps / 2 * 1.01 + size[..., None] * 4 * (e + 8 * 2.0 ** -24) * (p + hot) + least
+    x = logits.clone().requires_grad_()
+    kw = dict(ref_logp=ref, weight=weight, clip=(0.2, 0.28), kl=0.05)
+    loss, logp = policy_loss(x, tokens, old, adv, **kw)
+    grad, = torch.autograd.grad(loss, x, retain_graph=True)
+    again, = torch.autograd.grad(loss, x)  # formed from the saved sums
+    bare, blogp = policy_loss(logits, tokens, old, adv, **kw)
+    for lp in (logp, blogp, token_logp(logits, tokens)):
+        assert (lp.double() - rp).abs().max() <= e
+    for l in (loss, bare):
+        assert (l.detach().double() - rl).abs() <= 2 * (e + 8 * 2.0 ** -24) * size.sum()
+    for g in (grad, again):
+        assert (((g.double() - rg).abs() <= tol) | edge[..., None]).all()
+    up = torch.rand(B, T, device='cuda') + 0.5
+    g, = torch.autograd.grad(token_logp(x, tokens), x, up)
+    want = up.double()[..., None] * (hot - p)
+    assert ((g.double() - want).abs() <= want.abs() * torch.finfo(logits.dtype).eps / 2 * 1.01 + up[..., None] * 4 * (e + 8 * 2.0 ** -24) * (p + hot) +
+            least).all()
+
+
+def test_references_beside_the_border():
+    """Rows whose products with log2(e) lie on both sides of 2^20, where an exponent's reference changes its form: sums about one and
+    about the other meet in one row."""
+    from treeattn_b200.losses import token_logp
+    g = torch.Generator(device='cuda').manual_seed(1)
+    for border in (2.0 ** 20 * math.log(2), -2.0 ** 20 * math.log(2)):
+        z = (torch.randint(-128, 129, (64, 9001), device='cuda', generator=g) / 16 + round(border)).float()
+        x = z.clone().requires_grad_()
+        tokens = torch.randint(0, 9001, (64,), device='cuda', generator=g)
+        logp = token_logp(x, tokens)
+        want = z.double().log_softmax(-1).gather(1, tokens[:, None])[:, 0]
+        assert (logp.double() - want).abs().max() <= _logp_error(z, 1.0)

@@ -96,17 +96,19 @@ __device__ __forceinline__ float exp2_fast(float x) {  // 2 ulp; 0 at -inf, NaN 
   return y;
 }
 
-// A reference logit m that exponentials are taken about: exp2(z k - m k), one operation and the exponential. The product m k is rounded, which
-// puts one factor on all of a reference's exponentials: sums, logits and other references are compared with the same rounded product,
-// and it cancels. Where the products come near the range's end the difference is taken first.
+// A reference logit m that exponentials are taken about: exp2(z k - R), R = m k rounded: one operation and the exponential. R is the
+// reference as it stands (the rounding of m k puts one factor on all of its exponentials), and whatever is compared with it takes R
+// itself, so that the factor cancels. From 2^20 on, where that factor may pass 2^(1/16) and further up leave the range (a word banned by a finite
+// -1e10: 2^439), the difference is taken first and the reference is m k.
 struct Ref {
-  float m, off;
+  float m, off;  // off = -R
   bool far;
-  __device__ __forceinline__ Ref(float m_, float k) : m(m_), off(-m_ * k), far(!(fabsf(off) < 1e30f)) {}
+  __device__ __forceinline__ Ref(float m_, float k) : m(m_), off(-m_ * k), far(!(fabsf(off) < 1048576.f)) {}
   __device__ __forceinline__ float of(float z, float k) const { return far ? (z - m) * k : fmaf(z, k, off); }
-  // what a sum about o is multiplied by to be one about this
+  // what a sum about o is multiplied by to be one about this: each as it stands, R or m k
   __device__ __forceinline__ float from(const Ref& o, float k) const {
-    return exp2_fast(far || o.far ? (o.m - m) * k : off - o.off);
+    if (!far) return exp2_fast(o.far ? fmaf(o.m, k, off) : off - o.off);
+    return exp2_fast(o.far ? (o.m - m) * k : -fmaf(m, k, o.off));
   }
 };
 
