@@ -431,3 +431,34 @@ def test_references_beside_the_border():
         logp = token_logp(x, tokens)
         want = z.double().log_softmax(-1).gather(1, tokens[:, None])[:, 0]
         assert (logp.double() - want).abs().max() <= _logp_error(z, 1.0)
+
+
+@pytest.mark.parametrize('c', [0.0, 100.0, 1e4, -1e4, 2.0 ** 19, 1e6, -1e6])
+@pytest.mark.parametrize('tau', [1.0, 0.125])
+def test_rows_far_from_zero(c, tau):
+    """A constant added to a row changes nothing (the sums are exact: words in steps of 1/16): logp, loss and the fp32 gradient keep the
+    accuracy that the row's spread allows, and the gradient is the same whether the forward pass formed it or the backward pass did."""
+    from treeattn_b200.losses import policy_loss
+    logits, tokens, old, adv, ref, weight = _inputs(2, 8, 3001, 'f32', seed=12)
+    logits = (logits * 16).round() / 16
+    lp = (logits.double() / tau).log_softmax(-1).gather(-1, tokens[..., None])[..., 0].float()
+    args = (logits + c, tokens, lp + (old - lp).clamp(-0.3, 0.3), adv, lp + 0.2, weight)
+    assert torch.equal(args[0].double() - c, logits.double())
+    _, _, grad = _check(*args, clip=(0.2, 0.28), kl=0.05, tau=tau)
+    _, _, twice = _check(*args, clip=(0.2, 0.28), kl=0.05, tau=tau, up=2.0)
+    # p by the same exponentials: products in another order, 4 steps of 2^-24, and what the token's sum cancels
+    p = (logits.double() / tau).softmax(-1)
+    hot = torch.nn.functional.one_hot(tokens, 3001)
+    slope = grad.double().abs().sum(-1, keepdim=True)
+    assert ((twice.double() / 2 - grad.double()).abs() <= 4 * 2.0 ** -24 * slope * (p + hot) + 2.0 ** -126).all()
+
+
+@pytest.mark.parametrize('c', [0.0, 100.0, 250.0, 512.0])
+def test_bf16_rows_far_from_zero(c):
+    """The same in bf16, on both sides of where the factor leaves the exponent."""
+    logits, tokens, old, adv, ref, weight = _inputs(2, 8, 3001, 'bf16', seed=12)
+    logits = logits.float().round()
+    lp = logits.double().log_softmax(-1).gather(-1, tokens[..., None])[..., 0].float()
+    logits = (logits + c).to(torch.bfloat16)
+    moved = logits.double().log_softmax(-1).gather(-1, tokens[..., None])[..., 0].float()
+    _check(logits, tokens, moved + (old - lp).clamp(-0.3, 0.3), adv, moved + 0.2, weight, clip=(0.2, 0.28), kl=0.05, tau=1.0)

@@ -201,7 +201,8 @@ __device__ __forceinline__ Share warp_share(const Share& x, float k) {
 // copies the pieces that it will look at itself, so that no barrier is needed for them. It sums exponentials about the largest element
 // of its first piece; where that was a poor choice (the sum leaves [1/2, 2^100]) it looks for its largest element and sums again. The
 // warps' and CTAs' (reference, sum) meet in one step, one thread works out the row's scalars, and the gradient is written from the share:
-// exp2(z k - m k + log2(slope / sum)), so that it takes one operation, the exponential and the rounding an element. exp is evaluated twice, to keep
+// exp2(z k - m k + log2(slope / sum)) in 16 bits, one operation, the exponential and the rounding an element, and slope / sum exp2(z k - m k) in
+// 32, where the sum's rounding would be seen. exp is evaluated twice, to keep
 // 16 bits of an element instead of 32 and two CTAs on an SM: one waits for its row while the other computes. (Kept in registers
 // instead, with the next row read ahead, an element costs less, but the CTAs that a row then needs wait for each other: 810 us against 290
 // for 8 x 1024 x 50304 bf16, a quarter of it not counted.)
@@ -406,18 +407,28 @@ __global__ void __launch_bounds__(THREADS, (MODE == 2 ? 1024 : MODE == 0 && ALIG
     };
     if (slope == 0.f) {
       g.zeros(j0, first, i1, THREADS, edge);
-    } else if (m.far || !(fabsf(s_of[2]) < 1e30f)) {
+    } else if (sizeof(T) == 4 || !(fabsf(m.off) + fabsf(s_of[2]) < 256.f)) {
+      // the factor after the exponential: exact to fp32's steps wherever the row lies
       const float f = s_of[1];
-      auto one = [&](int j) {
-        float z[N];
-        Piece<T>::widen(share[j], z);
-        for (int i = 0; i < N; ++i) z[i] = f * exp2_fast(m.of(z[i], k));
-        add(j, z);
-        return Piece<T>::narrow(z);
+      auto all = [&](auto far) {
+        auto one = [&](int j) {
+          float z[N];
+          Piece<T>::widen(share[j], z);
+#pragma unroll
+          for (int i = 0; i < N; ++i) z[i] = f * exp2_fast(decltype(far)::value ? (z[i] - m.m) * k : fmaf(z[i], k, m.off));
+          add(j, z);
+          return Piece<T>::narrow(z);
+        };
+        for (int j = first; j < i1; j += THREADS) g.whole(j0 + j, one(j));
+        if (edge >= 0) g.edge(j0 + edge, one(edge));
       };
-      for (int j = first; j < i1; j += THREADS) g.whole(j0 + j, one(j));
-      if (edge >= 0) g.edge(j0 + edge, one(edge));
+      if (m.far)
+        all(std::true_type());
+      else
+        all(std::false_type());
     } else {
+      // 16 bits: the factor joins the exponent. Their sum is rounded once more, by 2^-17 of its 256 at most: nothing beside the
+      // output's 2^-12 or 2^-9.
       const float off = m.off + s_of[2];
       auto all = [&](auto sign) {
         auto one = [&](int j) {
