@@ -462,3 +462,38 @@ def test_bf16_rows_far_from_zero(c):
     logits = (logits + c).to(torch.bfloat16)
     moved = logits.double().log_softmax(-1).gather(-1, tokens[..., None])[..., 0].float()
     _check(logits, tokens, moved + (old - lp).clamp(-0.3, 0.3), adv, moved + 0.2, weight, clip=(0.2, 0.28), kl=0.05, tau=1.0)
+
+
+@pytest.mark.parametrize('V', [8192, 8200])
+def test_logits_written_by_the_launch_before(V):
+    """Logits that a kernel of this library writes, which lets the next launch begin before it ends: the losses wait for them."""
+    from treeattn_b200.adapters import adapter_add
+    from treeattn_b200.losses import policy_loss, token_logp
+    g = torch.Generator(device='cuda').manual_seed(7)
+    rand = lambda *s: torch.randn(*s, device='cuda', generator=g).to(torch.bfloat16)
+    n, ys = 300, [rand(300, V) for _ in range(4)]
+    x, a, b = rand(n, 64), rand(1, 8, 64), rand(1, V, 8)
+    start, which = torch.tensor([0, n], device='cuda', dtype=torch.int32), torch.zeros(1, device='cuda', dtype=torch.int32)
+    tokens = torch.randint(0, V, (n,), device='cuda', generator=g)
+    old, adv = torch.full((n,), -9.0, device='cuda'), torch.randn(n, device='cuda', generator=g)
+    up = torch.ones(n, device='cuda')
+    outs = []
+
+    def losses(logits):
+        z = logits.detach().requires_grad_()
+        lp = token_logp(z, tokens)
+        loss, lp2 = policy_loss(logits, tokens, old, adv, clip=100.0)
+        return [token_logp(logits, tokens), lp.detach(), loss, lp2, torch.autograd.grad(lp, z, up)[0]]
+
+    want = []
+    for y in ys:
+        logits = adapter_add(y, x, a, b, start, which, n)
+        torch.cuda.synchronize()
+        want.append(losses(logits))
+    logits = torch.empty_like(ys[0])
+    for i in range(200):
+        adapter_add(ys[i % 4], x, a, b, start, which, n, out=logits)
+        outs.append(losses(logits) if i % 10 == 0 else [token_logp(logits, tokens)])
+    for i, got in enumerate(outs):
+        for o, w in zip(got, want[i % 4]):
+            assert torch.equal(o, w)

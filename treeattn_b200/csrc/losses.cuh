@@ -112,10 +112,12 @@ struct Ref {
   }
 };
 
+// A piece that is read once. Volatile, with memory as a clobber, and not through the read-only path: the launch before this one may write
+// the logits until pdl_wait returns, and nothing else keeps a load of an address that is known before from being moved above it.
 __device__ __forceinline__ uint4 load_once(const uint4* p) {
   uint4 v;
-  asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
   return v;
 }
 
