@@ -193,3 +193,58 @@ def test_refused_lists():
             paged.paged_copy(caches, src, dst)
     with pytest.raises(ValueError, match='paged_fork.*CUDA'):
         paged.paged_fork(one, [0], [1])
+
+
+def test_reserve_looks_at_pages_only_where_some_are_shared():
+    """A decode step of sequences that share nothing does not walk their pages; the count of further holders is right after every
+    fork, cut, replacement, release and compaction."""
+    class Pages(list):
+        walked = 0
+
+        def __getitem__(self, j):
+            Pages.walked += 1
+            return list.__getitem__(self, j)
+
+    pool = _pool(n_pages=60, batch=6, max_pages=10)
+    pool.reserve([100] * 6, [0] * 6)
+    pool.owned = [Pages(o) for o in pool.owned]
+    pool.reserve([101] * 6, [40] * 6)
+    assert Pages.walked == 0
+    pool.fork([0], [1], [100])
+    pool.reserve([101] * 6, [40] * 6)
+    assert Pages.walked > 0
+    extra = lambda: sum(max(r - 1, 0) for r in pool.refs)
+    assert pool.extra == extra()
+    rng = random.Random(11)
+    pos, some = [101] * 6, 0
+    for _ in range(300):
+        act = rng.random()
+        if act < 0.4:
+            new = [min(160, p + rng.randint(0, 20)) for p in pos]
+            try:
+                pool.reserve(new, pos)
+                pos = new
+            except MemoryError:
+                pass
+        elif act < 0.7:
+            k = rng.randint(1, 5)
+            dst, src = rng.sample(range(6), k), [rng.randrange(6) for _ in range(k)]
+            pool.fork(src, dst, [pos[s] for s in src])
+            was = list(pos)
+            for s, d in zip(src, dst):
+                pos[d] = was[s]
+        elif act < 0.85:
+            pos = [max(0, p - rng.randint(0, 40)) for p in pos]
+        elif act < 0.95 or pool.n_pages < 45:
+            b = rng.randrange(6)
+            pool.release(b)
+            pos[b] = 0
+        else:
+            pool.compact(max(pool.n_pages - len(pool.free), pool.n_pages - 1, 1))
+        assert pool.extra == extra()
+        some += pool.extra > 0
+        _consistent(pool)
+    assert some > 50
+    for b in range(6):
+        pool.release(b)
+    assert pool.extra == 0

@@ -99,6 +99,7 @@ class PagePool:
         self.page, self.n_pages, self.max_pages = int(page), int(n_pages), int(max_pages)
         self.free = list(range(n_pages - 1, -1, -1))
         self.refs = [0] * self.n_pages
+        self.extra = 0  # holders beyond each page's first: 0 where nothing is shared
         self.owned = [[] for _ in range(batch)]
         self.host = torch.zeros(batch, max_pages, dtype=torch.int32)
         self.table = torch.zeros(batch, max_pages, device=device, dtype=torch.int32)
@@ -112,7 +113,9 @@ class PagePool:
     def _drop(self, pages):
         for p in reversed(pages):
             self.refs[p] -= 1
-            if not self.refs[p]:
+            if self.refs[p]:
+                self.extra -= 1
+            else:
                 self.free.append(p)
 
     def reserve(self, lengths, pos=None):
@@ -125,7 +128,7 @@ class PagePool:
             if -(-int(n) // self.page) > self.max_pages:
                 raise ValueError('PagePool: %d positions above the %d of a sequence' % (n, self.max_pages * self.page))
         shared, left = [], {}
-        for b, at in enumerate(() if pos is None else pos):
+        for b, at in enumerate(() if pos is None or not self.extra else pos):
             own = self.owned[b]
             for j in range(int(at) // self.page, len(own)):
                 n = left.get(own[j], self.refs[own[j]])
@@ -134,6 +137,7 @@ class PagePool:
                     shared.append((b, j))
         if sum(need) + len(shared) > len(self.free):
             raise MemoryError('PagePool: %d pages wanted, %d free' % (sum(need) + len(shared), len(self.free)))
+        self.extra -= len(shared)
         for b, j in shared:
             self.refs[self.owned[b][j]] -= 1
             self.owned[b][j] = self._take(b, j)
@@ -166,6 +170,7 @@ class PagePool:
             if s != d:
                 new[d] = self.owned[s][:full]
         for pages in new.values():
+            self.extra += len(pages)
             for p in pages:
                 self.refs[p] += 1
         for d, pages in new.items():
