@@ -168,3 +168,18 @@ def test_rotation_table_covers_the_context(host_model):
     for n, rot in ((99, 16), (128, 18)):
         with pytest.raises(ValueError, match='rotation of %d positions and %d dims' % (n, rot)):
             host_model(max_len=100, rotation=rotation_table(n, rot, device='cpu'))
+
+
+def test_a_released_slot_has_no_adapter(host_model):
+    """The next request in a slot that was released does not run with the last one's adapter; reset keeps the adapters, as documented."""
+    from treeattn_b200.adapters import AdapterSet
+    dec = host_model(batch=3, adapters=AdapterSet(2, 1, 32, rank=8, device='cpu'))
+    for b, a in enumerate((1, 0, 1)):
+        dec.set_adapter(b, a)
+    dec.release(1)
+    assert dec.which.tolist() == [1, -1, 1] and dec.pos == [0, 0, 0]
+    dec.reset()
+    assert dec.which.tolist() == [1, -1, 1]
+    plain = host_model()
+    plain.release(0)
+    assert plain.which.tolist() == [-1, -1]

@@ -76,7 +76,8 @@ class PagedDecoder:
         self.which[b] = adapter
 
     def reset(self):
-        """Empties every sequence and gives its pages back."""
+        """Empties every sequence and gives its pages back. The slots keep their adapters (a new prompt of the same users: `which`,
+        set_adapter and release change them)."""
         for b in range(self.batch):
             self.pool.release(b)
         self.pos, self._floor = [0] * self.batch, [0] * self.batch
@@ -141,9 +142,11 @@ class PagedDecoder:
             self.pos[d], self._floor[d] = was[0][s], was[1][s]
 
     def release(self, b):
-        """Empties sequence b and gives its pages back."""
+        """Empties sequence b and gives its pages back; the slot's next sequence has no adapter (set_adapter gives it one)."""
         self.pool.release(b)
         self.pos[b] = self._floor[b] = 0
+        if self.adapters is not None:
+            self.which[b] = -1
 
     def compact(self, n_pages=None):
         """Shrinks the pool to n_pages pages (default: as many as are held) and gives the rest of its memory back."""
