@@ -183,3 +183,31 @@ def test_a_released_slot_has_no_adapter(host_model):
     plain = host_model()
     plain.release(0)
     assert plain.which.tolist() == [-1, -1]
+
+
+def test_a_refused_fork_changes_nothing(host_model, monkeypatch):
+    """Neither lists that the pool refuses nor moves that the copy refuses (a cycle above its limit) leave a sequence half forked."""
+    from treeattn_b200 import speculative
+    from treeattn_b200._lib import TreeAttnError
+    dec, copied = host_model(batch=3), []
+    monkeypatch.setattr(speculative, 'paged_fork', lambda caches, src, dst: copied.append((src, dst)))
+    dec.forward(torch.zeros(3, 40, dtype=torch.int64))
+    state = lambda: ([list(o) for o in dec.pool.owned], list(dec.pool.free), list(dec.pool.refs), dec.pool.extra, dec.pool.table.tolist(),
+                     list(dec.pos), list(dec._floor), dec.which.tolist())
+    before = state()
+    for src, dst in (([0], [3]), ([-1], [1]), ([0, 0], [1, 1]), ([0], [1, 2])):
+        with pytest.raises(ValueError):
+            dec.fork(src, dst)
+        assert state() == before and not copied
+
+    def refuse(caches, src, dst):
+        raise TreeAttnError('ta_record_copy: a cycle of 2048 moves (at most 2047)')
+
+    monkeypatch.setattr(speculative, 'paged_fork', refuse)
+    with pytest.raises(TreeAttnError):
+        dec.fork([0, 1], [1, 0])
+    assert state() == before
+    monkeypatch.setattr(speculative, 'paged_fork', lambda caches, src, dst: copied.append((src, dst)))
+    dec.fork([0, 1], [1, 2])
+    # 1 shares the two full pages of 0; what 1 held has gone to 2 alone
+    assert copied == [([0, 1], [1, 2])] and dec.pool.extra == 2

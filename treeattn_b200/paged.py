@@ -152,10 +152,8 @@ class PagePool:
         self._drop(self.owned[b])
         self.owned[b] = []
 
-    def fork(self, src, dst, lengths):
-        """Sequence dst[i] goes on from the first lengths[i] positions of sequence src[i], for all i at once (a sequence may be a
-        source and a destination): it shares the full pages among them, and what dst[i] held is given back. The open pages, which
-        live in the caches' tails, are paged_fork's to copy."""
+    def _forked(self, src, dst, lengths):
+        """Checks a fork's lists; the pages that each destination is to hold."""
         B = len(self.owned)
         src, dst, lengths = [[int(i) for i in x] for x in (src, dst, lengths)]
         if not len(src) == len(dst) == len(lengths):
@@ -169,6 +167,13 @@ class PagePool:
                 raise ValueError('PagePool.fork: sequence %d does not hold %d positions' % (s, n))
             if s != d:
                 new[d] = self.owned[s][:full]
+        return new
+
+    def fork(self, src, dst, lengths):
+        """Sequence dst[i] goes on from the first lengths[i] positions of sequence src[i], for all i at once (a sequence may be a
+        source and a destination): it shares the full pages among them, and what dst[i] held is given back. The open pages, which
+        live in the caches' tails, are paged_fork's to copy."""
+        new = self._forked(src, dst, lengths)
         for pages in new.values():
             self.extra += len(pages)
             for p in pages:
