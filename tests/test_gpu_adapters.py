@@ -572,3 +572,71 @@ def test_set_in_serving():
         PagedDecoder(W, 2, 2, 64, adapters=s, dtype=torch.float16)
     with pytest.raises(ValueError, match='adapters of'):
         PagedDecoder(W, 2, 4, 128, adapters=s)
+
+
+def _one_signed(lengths, dtype, exact, rank=16):
+    """Positive factors and rows; exact: t and u are numbers that the type holds, so that nothing is left for their low parts."""
+    s = _inputs(lengths, 64, 72, rank, dtype, na=1, scale=False, seed=2)
+    for k in 'xab':
+        s[k] = torch.full_like(s[k], 0.25) if exact else s[k].abs() + 0.125
+    s['which'][:] = 0
+    return s
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('rows', [7, 40])
+@pytest.mark.parametrize('exact', [False, True])
+@pytest.mark.parametrize('sign', [1, -1])
+def test_infinite_factors(dtype, rows, exact, sign):
+    """An infinity in A or B gives the formula's infinities, whatever t's low part is: 0, or of the other sign than its high part."""
+    from treeattn_b200.adapters import adapter_add
+    s = _one_signed([rows], dtype, exact)
+    b = s['b'].clone()
+    b[0, 5, 3] = sign * math.inf
+    out = adapter_add(**dict(s, b=b))
+    assert (out[:, 5] == sign * math.inf).all()
+    rest = [i for i in range(72) if i != 5]
+    assert out[:, rest].isfinite().all()
+    a = s['a'].clone()
+    a[0, 3, 7] = sign * math.inf
+    assert (adapter_add(**dict(s, a=a)) == sign * math.inf).all()
+    assert (adapter_add(**dict(s, a=a, b=s['b'] * -1)) == sign * -math.inf).all()
+
+
+@pytest.mark.parametrize('rows', [7, 40, 300])
+@pytest.mark.parametrize('exact', [False, True])
+def test_infinities_in_gradients(rows, exact):
+    """Infinities in A reach dx, those of x reach dA, those of dy reach dB: as infinities."""
+    from treeattn_b200.adapters import adapter_add
+    s = _one_signed([rows], torch.bfloat16, exact)
+    dy = torch.full_like(s['y'], 0.25) if exact else torch.rand_like(s['y']) + 0.125
+
+    def grads(dy, **kw):
+        leaves = {k: dict(s, **kw)[k].clone().requires_grad_() for k in 'yxab'}
+        return dict(zip('yxab', torch.autograd.grad(adapter_add(**dict(s, **leaves)), list(leaves.values()), dy)))
+
+    a = s['a'].clone()
+    a[0, 3, 7] = -math.inf
+    dx = grads(dy, a=a)['x']
+    assert (dx[:, 7] == -math.inf).all() and dx[:, [i for i in range(64) if i != 7]].isfinite().all()
+    x = s['x'].clone()
+    x[2, 9] = math.inf
+    da = grads(dy, x=x)['a']
+    assert (da[0, :, 9] == math.inf).all() and da[0, :, [i for i in range(64) if i != 9]].isfinite().all()
+    d = dy.clone()
+    d[4, 11] = -math.inf
+    db = grads(d)['b']
+    assert (db[0, 11] == -math.inf).all() and db[0, [i for i in range(72) if i != 11]].isfinite().all()
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16])
+def test_small_parts_of_t(dtype):
+    """Elements of t that are far below their row's largest, powers of two and subnormal numbers among them, weigh what they are."""
+    s = _inputs([20], 64, 64, 16, dtype, na=1, scale=False, seed=1)
+    s['which'][:] = 0
+    s['a'] = torch.zeros_like(s['a'])
+    s['a'][0, range(16), range(16)] = 1  # t is x's first columns
+    for by in (1.0, 3.0):
+        s['x'] = (torch.tensor([2.0 ** -i for i in range(16)] + [0.0] * 48, device='cuda') * by).to(dtype).expand(20, 64).contiguous()
+        s['y'] = torch.zeros_like(s['y'])
+        _forward(s)

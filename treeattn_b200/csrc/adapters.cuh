@@ -6,7 +6,7 @@
 // warp-level matrix instruction, whose fragments come from rows of any length.
 // Few rows of a sequence (decoding) take one kernel for both products; many take two, t going by way of memory (64 bytes a row at rank
 // 16): its columns and the output's are then shared out over the GPU apart.
-// t is held in fp32 and enters its product as two 16-bit numbers, high and low: 16 bits of it (22 in f16), so that the output's one
+// t is held in fp32 and enters its product as two 16-bit numbers, high and low: 16 bits of it (22 in f16; see split), so that the output's one
 // rounding is what is seen.
 #pragma once
 #include <type_traits>
@@ -88,6 +88,31 @@ __device__ __forceinline__ void load_b(uint32_t (&b)[4], uint32_t base, int pitc
   ldsm4(b, base + (n0 + (lane >> 4) * 8 + (lane & 7)) * pitch + (k0 + ((lane >> 3) & 1) * 8) * 2);
 }
 
+// s as two 16-bit numbers of one sign, h the next below s in magnitude (toward 0), l the rest, neither of them 0 where s is not: a factor
+// that is infinite then gives the infinity of s times it, and not the NaN of infinities of both signs or of 0 times one. l is rounded once, by
+// 2^-16 of s at most (bf16; f16 2^-22). An infinite s goes on as inf + 1. (bf16 numbers below 2^-132 keep h or l alone.)
+__device__ __forceinline__ void split(float s, __nv_bfloat16& h, __nv_bfloat16& l) {
+  const uint32_t u = __float_as_uint(s), mag = u & 0x7fffffffu;
+  const bool some = mag - 1u < 0x7f7fffffu;  // finite and not 0
+  const float f = some ? __uint_as_float((u - 1u) & 0xffff0000u) : s;
+  const float rest = some ? s - f : (mag == 0x7f800000u ? copysignf(1.f, s) : 0.f);
+  h = from_f32<__nv_bfloat16>(f);
+  l = from_f32<__nv_bfloat16>(rest);
+}
+// f16, |s| below 2 (or infinite): l is 2^-24 at least; h is 0 up to 2^-24.
+__device__ __forceinline__ void split(float s, __half& h, __half& l) {
+  h = __float2half_rz(s);
+  l = __float2half_rn(0.f);
+  if (fabsf(s) == INFINITY) {
+    l = __float2half_rn(copysignf(1.f, s));
+  } else if (fabsf(s) > 0.f) {
+    const uint16_t b = __half_as_ushort(h);
+    if ((b & 0x7fffu) && __half2float(h) == s) h = __ushort_as_half((uint16_t)(b - 1u));
+    const float rest = s - __half2float(h);
+    l = __float2half_rn(copysignf(fmaxf(fabsf(rest), 5.9604644775390625e-08f), s));
+  }
+}
+
 // A warp's row m of t: summed over the cluster's parts (rows of RP), scaled, split into high and low parts. They go to p.t's row `row`
 // (unless there is none), and to shared memory where that is given.
 template <typename T, int RP>
@@ -123,9 +148,8 @@ __device__ __forceinline__ void split_row(const AdapterParams& p, const float* p
   for (int v = 0; v < VL; ++v) {
     const int c = lane + 32 * v;
     if (c >= RP) break;
-    const T h = from_f32<T>(s[v]);
-    const float rest = s[v] - to_f32(h);
-    const T l = from_f32<T>(fabsf(to_f32(h)) < INFINITY ? rest : 0.f);
+    T h, l;
+    split(s[v], h, l);
     if (hi) {
       reinterpret_cast<T*>(hi)[c] = h;
       reinterpret_cast<T*>(lo)[c] = l;
