@@ -73,3 +73,15 @@ def test_adapter_set_shapes_and_refusals():
     assert sum(len(m._forward_hooks) for m in model.modules()) == 4
     attached.remove()
     assert sum(len(m._forward_hooks) for m in model.modules()) == 0
+
+
+def test_forward_mode_is_refused():
+    from torch.autograd import forward_ad
+    from treeattn_b200.adapters import adapter_add
+    x, y, a, b = [torch.randn(s).to(torch.bfloat16) for s in ((5, 16), (5, 24), (2, 8, 16), (2, 24, 8))]
+    start, which = torch.tensor([0, 5], dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    with forward_ad.dual_level():
+        for i in range(4):
+            args = [forward_ad.make_dual(t, torch.ones_like(t)) if j == i else t for j, t in enumerate((y, x, a, b))]
+            with pytest.raises(NotImplementedError, match='adapter_add.*forward-mode'):
+                adapter_add(*args, start, which, 5)

@@ -61,3 +61,18 @@ def test_refused_tensors():
         policy_loss(z, y, r, r, clip=(-0.1, 0.2))
     with pytest.raises(ValueError, match='clip'):
         policy_loss(z, y, r, r, clip=float('nan'))
+
+
+def test_forward_mode_is_refused():
+    """A tangent would be lost without a word: a dual tensor does not ask for gradients."""
+    from torch.autograd import forward_ad
+    from treeattn_b200.losses import policy_loss, token_logp
+    z, y, r = torch.randn(2, 3, 8), torch.zeros(2, 3, dtype=torch.int64), torch.zeros(2, 3)
+    with forward_ad.dual_level():
+        dz, dr = forward_ad.make_dual(z, torch.ones_like(z)), forward_ad.make_dual(r, torch.ones_like(r))
+        for call in (lambda: token_logp(dz, y), lambda: policy_loss(dz, y, r, r), lambda: policy_loss(z, y, dr, r),
+                     lambda: policy_loss(z, y, r, r, ref_logp=dr, kl=0.1), lambda: policy_loss(z, y, r, r, weight=dr)):
+            with pytest.raises(NotImplementedError, match='(token_logp|policy_loss).*forward-mode'):
+                call()
+        with pytest.raises(ValueError, match='CUDA'):  # tensors without a tangent are what they are elsewhere
+            token_logp(z, y)

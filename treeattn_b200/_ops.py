@@ -8,6 +8,7 @@ import ctypes
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -19,6 +20,12 @@ def _code(t):
         return _DT[t.dtype]
     except KeyError:
         raise TypeError('unsupported dtype %s (float32, bfloat16, float16)' % t.dtype) from None
+
+
+def _no_tangents(name, *tensors):
+    """Refuses tensors with a forward-mode tangent: the kernels take the values alone, and it would be lost without a word."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError('%s: no forward-mode derivatives' % name)
 
 
 def _need_cuda(name, *ts):

@@ -8,7 +8,7 @@ import torch
 import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
-from ._ops import _DT, _need_cuda, _p
+from ._ops import _DT, _need_cuda, _no_tangents, _p
 from .paged import _call, _on, _stream
 
 
@@ -123,6 +123,7 @@ def adapter_add(y, x, a, b, start, which, max_new, scale=None, out=None):
     set gives NaN rows and is recorded (device_error).
     Differentiable in y, x, a and b in bfloat16 (not with an `out` other than y); sequences that share an adapter add to one gradient, in
     one order. t = x A^T is summed in fp32 and multiplied with B as two 16-bit numbers; the sum with y is rounded once."""
+    _no_tangents('adapter_add', y, x, a, b, scale)
     dims = _check('adapter_add', y, x, a, b, start, which, scale)
     max_new = int(max_new)
     if out is not None:

@@ -10,7 +10,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._ops import _DT, _need_cuda
+from ._ops import _DT, _need_cuda, _no_tangents
 from .paged import _call, _on, _stream
 
 _V4 = ctypes.c_void_p * 4
@@ -107,6 +107,7 @@ def token_logp(logits, tokens, temperature=1.0):
     strides), tokens their leading shape, int64. Returns that shape in float32; differentiable in logits (rows whose gradient is 0 get
     zeros, whatever the logits hold). A token outside [0, V) gives NaN and is recorded (device_error)."""
     temperature = float(temperature)
+    _no_tangents('token_logp', logits)
     if logits.requires_grad and torch.is_grad_enabled():
         return _TokenLogp.apply(logits, tokens, temperature)
     return _token_logp(logits, tokens, temperature)[0]
@@ -184,6 +185,7 @@ def policy_loss(logits, tokens, old_logp, advantages, ref_logp=None, weight=None
         raise ValueError('policy_loss: clip %s (not negative)' % (clip,))
     if kl and ref_logp is None:
         raise ValueError('policy_loss: a KL term needs ref_logp')
+    _no_tangents('policy_loss', logits, old_logp, advantages, ref_logp, weight)
     if torch.is_grad_enabled():
         for what, v in (('old_logp', old_logp), ('advantages', advantages), ('ref_logp', ref_logp), ('weight', weight)):
             if v is not None and v.requires_grad:
