@@ -640,3 +640,23 @@ def test_small_parts_of_t(dtype):
         s['x'] = (torch.tensor([2.0 ** -i for i in range(16)] + [0.0] * 48, device='cuda') * by).to(dtype).expand(20, 64).contiguous()
         s['y'] = torch.zeros_like(s['y'])
         _forward(s)
+
+
+def test_outputs_that_autograd_has_saved():
+    """A given output that a backward pass still needs is found to have changed, as with torch's own in-place operations."""
+    from treeattn_b200.adapters import adapter_add
+    s = _inputs([5, 40], 64, 72, 8, torch.bfloat16, seed=3)
+    for new in (5, 40):
+        for into_y in (True, False):
+            out = s['y'].clone()
+            w = torch.ones_like(out, requires_grad=True)
+            loss = (w * out).sum()  # keeps `out` for w's gradient
+            before = out._version
+            with torch.no_grad():
+                adapter_add(**dict(s, y=out if into_y else s['y'], max_new=new), out=out)
+            assert out._version > before
+            with pytest.raises(RuntimeError, match='inplace'):
+                loss.backward()
+    with torch.inference_mode():
+        out = s['y'].clone()
+        assert torch.equal(adapter_add(**s, out=out), adapter_add(**s))

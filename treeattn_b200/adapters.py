@@ -141,15 +141,17 @@ def adapter_add(y, x, a, b, start, which, max_new, scale=None, out=None):
             raise ValueError('adapter_add: no gradient through a given output (other than y itself)')
         return _AdapterAdd.apply(y, x, a, b, start, which, dims, max_new, scale, out is y)
     if out is None:
-        out = torch.empty_like(y, memory_format=torch.contiguous_format)
-    elif out is not y:
+        return _add(y, x, a, b, start, which, dims, max_new, scale, torch.empty_like(y, memory_format=torch.contiguous_format))
+    if out is not y:
         _rows('adapter_add', 'out', out, y.dtype)
         if out.shape != y.shape:
             raise ValueError('adapter_add: out must have y\'s shape')
         _need_cuda('adapter_add', out)
         if out.get_device() != x.get_device():
             raise ValueError('adapter_add: tensors on one device (got %s and %s)' % (x.device, out.device))
-    return _add(y, x, a, b, start, which, dims, max_new, scale, out)
+    _add(y, x, a, b, start, which, dims, max_new, scale, out)
+    torch.autograd.graph.increment_version(out)  # (written through its address: what autograd saved of it before is gone)
+    return out
 
 
 class AdapterSet(nn.Module):
