@@ -660,3 +660,16 @@ def test_outputs_that_autograd_has_saved():
     with torch.inference_mode():
         out = s['y'].clone()
         assert torch.equal(adapter_add(**s, out=out), adapter_add(**s))
+
+
+def test_outputs_that_want_gradients_are_refused():
+    """Neither a leaf nor a result of autograd is written without a word to its graph."""
+    from treeattn_b200.adapters import adapter_add
+    for dtype in (torch.bfloat16, torch.float16):
+        s = _inputs([5], 64, 64, 8, dtype)
+        leaf = torch.zeros_like(s['y']).requires_grad_()
+        for out in (leaf, leaf * 1):
+            with pytest.raises((ValueError, TypeError), match='given output|bfloat16 only'):
+                adapter_add(**s, out=out)
+        with torch.no_grad():
+            assert torch.equal(adapter_add(**s, out=leaf), adapter_add(**s))

@@ -132,7 +132,7 @@ def adapter_add(y, x, a, b, start, which, max_new, scale=None, out=None):
         if out.dim() == 2 and out.shape[0] > 1 and out.stride(0) < out.shape[1]:
             raise ValueError('adapter_add: rows of the output overlap')
     if torch.is_grad_enabled() and (y.requires_grad or x.requires_grad or a.requires_grad or b.requires_grad or
-                                    scale is not None and scale.requires_grad):
+                                    scale is not None and scale.requires_grad or out is not None and out.requires_grad):
         if scale is not None and scale.requires_grad:
             raise ValueError('adapter_add: no gradient of scale')
         if x.dtype is not torch.bfloat16:
