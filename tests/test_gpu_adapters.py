@@ -673,3 +673,26 @@ def test_outputs_that_want_gradients_are_refused():
                 adapter_add(**s, out=out)
         with torch.no_grad():
             assert torch.equal(adapter_add(**s, out=leaf), adapter_add(**s))
+
+
+def test_captured_tensors_are_let_go():
+    """What captured passes read is kept until release_captured: captures of many shapes do not add up for the set's life."""
+    model, cfg = _gpt()
+    model.requires_grad_(False)
+    s = _trained()
+    s.attach(model)
+    x = torch.randn(2, 64, 64, device='cuda').to(torch.bfloat16)
+    with torch.no_grad():
+        s.use([0, 2])
+        want = model.blocks[0](x)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = model.blocks[0](x)
+        s.use([1, 1])
+        graph.replay()
+        assert torch.equal(out, want) and len(s._captured) > 0
+        del graph, out
+        s.release_captured()
+        assert len(s._captured) == 0
+        s.use([0, 2])
+        assert torch.equal(model.blocks[0](x), want)

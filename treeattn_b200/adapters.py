@@ -215,6 +215,11 @@ class AdapterSet(nn.Module):
                 t.record_stream(torch.cuda.current_stream(t.device))
         return t
 
+    def release_captured(self):
+        """Lets go of the adapters and row offsets that captured passes read: once their graphs are no longer replayed. (They are kept
+        for the set's life otherwise.)"""
+        self._captured.clear()
+
     def use(self, which):
         """The adapters of the next batches of the attached model: whole numbers, -1 for none (None: no adapters at all). A captured pass
         keeps those that it was captured with."""
