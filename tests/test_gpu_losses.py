@@ -497,3 +497,20 @@ def test_logits_written_by_the_launch_before(V):
     for i, got in enumerate(outs):
         for o, w in zip(got, want[i % 4]):
             assert torch.equal(o, w)
+
+
+@pytest.mark.parametrize('dtype', ['f32', 'bf16', 'f16'])
+def test_an_advantage_that_is_nan(dtype):
+    """A counted row whose advantage is NaN has a NaN gradient beside its NaN loss, whichever side of the clip its ratio lies on; the
+    other rows keep theirs."""
+    from treeattn_b200.losses import policy_loss
+    logits, tokens, old, adv, ref, weight = _inputs(1, 6, 1003, dtype, seed=21)
+    lp = logits.double().log_softmax(-1).gather(-1, tokens[..., None])[..., 0].float()
+    old = lp - torch.tensor([[-0.5, 0.0, 0.5, 0.0, -0.5, 0.5]], device='cuda')
+    weight[:] = 0.2
+    x = logits.requires_grad_()
+    want, = torch.autograd.grad(policy_loss(x, tokens, old, adv, weight=weight)[0], x)
+    adv[0, :3] = math.nan
+    loss, _ = policy_loss(x, tokens, old, adv, weight=weight)
+    got, = torch.autograd.grad(loss, x)
+    assert loss.isnan() and got[0, :3].isnan().all() and torch.equal(got[0, 3:], want[0, 3:])

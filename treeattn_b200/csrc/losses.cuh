@@ -368,7 +368,7 @@ __global__ void __launch_bounds__(THREADS, (MODE == 2 ? 1024 : MODE == 0 && ALIG
         const float held = rho < a.lo ? a.lo : rho > a.hi ? a.hi : rho;  // (comparisons that keep a NaN)
         const float free_ = rho * adv, kept = held * adv;
         float term = -(kept < free_ ? kept : free_);
-        slope = (adv > 0.f ? rho > a.hi : rho < a.lo) ? 0.f : -adv * rho;
+        slope = (adv > 0.f ? rho > a.hi : adv <= 0.f && rho < a.lo) ? 0.f : -adv * rho;  // (NaN where A is)
         if (a.kl != 0.f) {
           const float d = ref - logp, x = expm1f(d);
           term += a.kl * (x - d);
