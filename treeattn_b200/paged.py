@@ -173,7 +173,9 @@ class PagePool:
         """Sequence dst[i] goes on from the first lengths[i] positions of sequence src[i], for all i at once (a sequence may be a
         source and a destination): it shares the full pages among them, and what dst[i] held is given back. The open pages, which
         live in the caches' tails, are paged_fork's to copy."""
-        new = self._forked(src, dst, lengths)
+        self._share(self._forked(src, dst, lengths))
+
+    def _share(self, new):
         for pages in new.values():
             self.extra += len(pages)
             for p in pages:

@@ -131,10 +131,10 @@ class PagedDecoder:
         """Sequence dst[i] goes on from where sequence src[i] is, for all i at once: a prompt into a group of samples, beams that take
         over one another's slots. Full pages are shared; the open ones are copied. What dst[i] held is dropped."""
         src, dst = [int(b) for b in src], [int(b) for b in dst]
-        held = [self.pos[s] if 0 <= s < self.batch else 0 for s in src]
-        self.pool._forked(src, dst, held)  # (both refuse before anything has changed)
+        # (the check of the lists and the copy refuse before anything has changed)
+        pages = self.pool._forked(src, dst, [self.pos[s] if 0 <= s < self.batch else 0 for s in src])
         paged_fork(self.caches, src, dst)
-        self.pool.fork(src, dst, held)
+        self.pool._share(pages)
         if self.adapters is not None and src:
             at = torch.tensor([src, dst]).to(self.dev)
             self.which[at[1]] = self.which[at[0]]
