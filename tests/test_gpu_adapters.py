@@ -696,3 +696,22 @@ def test_captured_tensors_are_let_go():
         assert len(s._captured) == 0
         s.use([0, 2])
         assert torch.equal(model.blocks[0](x), want)
+
+
+@pytest.mark.parametrize('rows', [7, 40])
+def test_f16_rows_without_a_power_of_two(rows):
+    """Rows of t that cannot be brought near 1: all below 2^-126, which weigh nothing, and rows with an infinity beside numbers above
+    f16's range, which stay the infinity that they are."""
+    from treeattn_b200.adapters import adapter_add
+    s = _inputs([rows], 64, 64, 16, torch.float16, na=1, seed=1)
+    s['which'][:] = 0
+    s['scale'][:] = 2.0 ** -140
+    s['y'] = torch.zeros_like(s['y'])
+    assert not _forward(s).any()
+    # t is infinite in the first rank and 64 x 60000 in the others, whose part of the sum is finite
+    s['scale'][:] = 1
+    s['x'], s['a'] = torch.ones_like(s['x']), torch.full_like(s['a'], 60000.0)
+    s['a'][0, 0, 3] = math.inf
+    s['b'] = torch.full_like(s['b'], -2.0 ** -10)
+    s['b'][0, :, 0] = 1.0
+    assert (adapter_add(**s) == math.inf).all()

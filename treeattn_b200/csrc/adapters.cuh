@@ -99,7 +99,8 @@ __device__ __forceinline__ void split(float s, __nv_bfloat16& h, __nv_bfloat16& 
   h = from_f32<__nv_bfloat16>(f);
   l = from_f32<__nv_bfloat16>(rest);
 }
-// f16, |s| below 2 (or infinite): l is 2^-24 at least; h is 0 up to 2^-24.
+// f16, |s| below 2 but in rows that hold an infinity or are below 2^-126 whole: there l ends at 65504, and s up to 2^-24 is l alone, as
+// elsewhere. Beside an h that is not 0 l is 2^-24 at least.
 __device__ __forceinline__ void split(float s, __half& h, __half& l) {
   h = __float2half_rz(s);
   l = __float2half_rn(0.f);
@@ -108,8 +109,8 @@ __device__ __forceinline__ void split(float s, __half& h, __half& l) {
   } else if (fabsf(s) > 0.f) {
     const uint16_t b = __half_as_ushort(h);
     if ((b & 0x7fffu) && __half2float(h) == s) h = __ushort_as_half((uint16_t)(b - 1u));
-    const float rest = s - __half2float(h);
-    l = __float2half_rn(copysignf(fmaxf(fabsf(rest), 5.9604644775390625e-08f), s));
+    const float t = __half2float(h), rest = fminf(fabsf(s - t), 65504.f);
+    l = __float2half_rn(copysignf(t == 0.f ? rest : fmaxf(rest, 5.9604644775390625e-08f), s));
   }
 }
 
