@@ -416,8 +416,8 @@ int ta_record_copy(void* const* bufs, int n_bufs, int64_t record_bytes, int n_re
 /* Losses over a vocabulary's logits (no counterpart in the reference, which trains on cross entropy). Row (b, t) of logits (B, T, V)
  * in `dtype` starts at b * z_sb + t * z_st (unit inner stride, no alignment needed); tokens int64 by (b, t). With z = logits /
  * temperature: logp = z_y - log sum exp z. A row whose token is outside [0, V) gives NaN and is recorded.
- * ta_token_logp: logp (B, T) fp32, contiguous; stats (2, B, T) fp32: a logit m of about the row's maximum, and the
- *   sum exp(z - m / temperature).
+ * ta_token_logp: logp (B, T) fp32, contiguous; stats (2, B, T) fp32 for ta_logits_grad: a logit m of about the row's maximum, and the
+ *   sum of 2^(logit k - m k), k = log2(e) / temperature, with m k as one rounded number where that is below 2^20.
  * ta_policy_loss: rho = exp(logp - old); term = -min(rho A, min(max(rho, lo), hi) A) + kl (exp(ref - logp) - (ref - logp) - 1);
  *   *loss = sum of w term (in 64 bits, one order). by_row: HOST array of the four fp32 tensors old, A, ref (read where kl != 0), w
  *   (NULL: weight0), by_row_strides their (b, t) strides, eight numbers. A row of w = 0 does not count, whatever it holds: logp 0.

@@ -54,7 +54,7 @@ enum KernelId : int {
   K_PAGED_APPEND = 16,
   K_PAGED_ATTN = 17,
   K_VERIFY = 18,
-  K_LOSS = 19,
+  K_LOSS = 19,  // (the paged tile kernel's waits are recorded under 19 too, as DEV_WAIT_TIMEOUT; a loss records DEV_INDEX_RANGE alone)
   K_ADAPTER = 20,
 };
 

@@ -71,6 +71,9 @@ int run_loss(ta::LossParams& a, cudaStream_t st, const char* who) {
   a.per = (pieces + cs - 1) / cs;
   const bool aligned = a.V % N == 0 && rows_aligned(a.z, sizeof(T), {a.z_sb, a.z_st}) &&
                        (MODE < 2 || rows_aligned(a.grad, sizeof(T), {a.g_sb, a.g_st}));
+  // Small shares: 128 threads, so that more rows are under way on an SM. 8192 x 8192 bf16 with its gradient 61 us, 114 with 512 threads, without
+  // it 37, 39 with 256; 16384 x 1000 fp32 56 and 165, 39 and 53; 8192 x 11000 f16 without 49 and 51. Few rows lose: 300 x 8192 bf16 without
+  // 10.2 and 8.2.
   if (a.per * 16 < 24 * 1024) {
     if (aligned) return launch_loss<T, 128, MODE, true>(a, cs, st, who);
     return launch_loss<T, 128, MODE, false>(a, cs, st, who);

@@ -23,8 +23,8 @@ using namespace ta_host;
 //   move (s, d):  s >= 0 a record to read, SAME the value of the move before, SAVED the one that was saved;
 //                 d >= 0 a record to write, SAVE: kept for the end of a cycle, NONE: nothing
 // Bound by bytes; four moves' loads are in flight a thread, and a record that several moves read in a row is read once. 12 layers:
-// 683 pages of 98 KB moved in 243 us (6.64 TB/s of reads and writes), one sequence's 393 KB into 63 slots in 49 us (6.1 TB/s), six moves among
-// eight slots in 16 us, most of it the host's.
+// 683 pages of 98 KB moved in 248 us (6.5 TB/s of reads and writes), one sequence's 393 KB into 63 slots in 48 us (6.3 TB/s), six moves among
+// eight slots in 13 us, launch and one round of memory.
 // The moves travel as the launch's parameters: nothing is uploaded, and a captured call holds its own.
 constexpr int THREADS = 256;
 constexpr int BATCH = 4;
